@@ -226,6 +226,104 @@ int rt_sgd(rt_ctx* ctx, rt_tensor* theta, const rt_tensor* g, float lr);
  * dst (bf16) = round-to-nearest-even(src (f32)). */
 int rt_cast(rt_ctx* ctx, const rt_tensor* src, rt_tensor* dst);
 
+/* ------------------------------------------- microscaled 4-bit matrices */
+/* No counterpart in the reference.  A matrix [rows, k] in OCP microscaling
+ * MXFP4: E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) and one
+ * E8M0 scale (a power of two, 2^(byte - 127); byte 255 is NaN) for each block
+ * of 32 elements along k.  Device layout:
+ *   codes   rows of ceil(k/32) * 16 bytes, two elements to a byte, the lower
+ *           index in the low four bits; the elements past k are zero;
+ *   scales  tiles of 128 rows by 4 blocks, 512 bytes each, tile
+ *           [row / 128][block / 4], in it byte
+ *           [row % 32][row / 32 % 4][block % 4]: the order the tensor cores
+ *           read scales in.  The scales of blocks past the last one must not
+ *           be 255; those of rows past the last one may hold anything. */
+typedef struct rt_mx4 rt_mx4;
+/* rows x k zeros (rows, k >= 0). */
+int rt_mx4_zeros(rt_ctx* ctx, int64_t rows, int64_t k, rt_mx4** out);
+/* Non-owning view of caller memory in the layout above: codes of
+ * rt_mx4_code_bytes bytes, scales of rt_mx4_scale_bytes bytes, both 16-byte
+ * aligned. */
+int rt_mx4_wrap(rt_ctx* ctx, void* codes, void* scales, int64_t rows, int64_t k, rt_mx4** out);
+int rt_mx4_free(rt_mx4* q);
+int rt_mx4_dims(const rt_mx4* q, int64_t* rows, int64_t* k);
+void* rt_mx4_codes(const rt_mx4* q);
+void* rt_mx4_scales(const rt_mx4* q);
+/* Bytes of the codes and of the scales of a rows x k matrix (-1: bad extents). */
+int64_t rt_mx4_code_bytes(int64_t rows, int64_t k);
+int64_t rt_mx4_scale_bytes(int64_t rows, int64_t k);
+/* dst = src (f32 or bf16) in 4 bits.  axis 1: src [rows, k], blocks along a
+ * row.  axis 0: src [k, rows], blocks down a column, laid out transposed: the
+ * weights [inputs, outputs] of a Dense layer, or both operands of X^T dY.
+ * Scale exponent of a block: floor(log2 max|x|) - 2, at least -127 (the rule
+ * of the OCP microscaling specification 1.0); elements are rounded to nearest,
+ * ties to even, magnitudes above 6 scales to 6.  A block that holds a NaN or
+ * an infinity gets the NaN scale. */
+int rt_mx4_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_mx4* dst);
+/* dst [rows, k] (f32 or bf16) = the values q stands for. */
+int rt_mx4_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst);
+/* C[m,n] = A[m,k] B[n,k]^T + 1 bias, ReLU if relu != 0; bias [1,n] f32 or
+ * NULL, C f32 or bf16, f32 accumulation.  All three products of a Dense layer
+ * take this form once their operands' blocks run along the summed axis:
+ *   Y = X W      A = X axis 1,  B = W axis 0
+ *   dX = dY W^T  A = dY axis 1, B = W axis 1
+ *   dW = X^T dY  A = X axis 0,  B = dY axis 0 */
+int rt_mx4_matmul(rt_ctx* ctx, const rt_mx4* a, const rt_mx4* b, rt_tensor* c, const rt_tensor* bias, int relu);
+
+/* ------------------------------------------------ residual-block norms */
+/* No counterpart in the reference.  The row-wise work between two blocks of a
+ * residual stream r [m,n], in one pass:
+ *   u = N_post(y)         y the block's output
+ *   z = r + scale * (gate . u)
+ *   h = N_pre(z)          input of the next block
+ * N(x)_j = (x_j - mu) / sqrt(mean((x - mu)^2) + eps) * gamma_j + beta_j, with
+ * mu = mean(x) (RT_NORM_LAYER) or 0 (RT_NORM_RMS); RT_NORM_NONE is N(x) = x.
+ * gamma and beta are [1,n] f32; NULL is ones and zeros.  y, r, z and h have one
+ * type, f32 or bf16; the arithmetic is f32, h is computed from the unrounded z. */
+typedef enum { RT_NORM_NONE = 0, RT_NORM_RMS = 1, RT_NORM_LAYER = 2 } rt_norm_kind;
+typedef struct {
+    rt_norm_kind kind;
+    float eps;
+    const rt_tensor* gamma;
+    const rt_tensor* beta;
+} rt_norm;
+typedef struct {
+    const rt_tensor* r;
+    const rt_tensor* y;    /* NULL: no block before, z = r */
+    rt_norm post;
+    const rt_tensor* gate; /* NULL (ones), f32 [1,1], [1,n] or [m,1], or [m,n] of y's type */
+    float scale;
+    rt_tensor* z;          /* may be r itself; NULL: not stored */
+    rt_norm pre;
+    rt_tensor* h;          /* NULL: not stored */
+    rt_mx4* hq;            /* h, rounded to y's type, as rt_mx4_quantize(h, axis 1); NULL: not stored */
+} rt_block_args;
+int rt_block_forward(rt_ctx* ctx, const rt_block_args* args);
+/* The gradients of the above.  args is the forward call's, with z as it was
+ * stored (y = NULL: z may be NULL, r is read); its r, h and hq are not read
+ * otherwise.
+ *   dz, dh  gradients of z and h, of y's type; NULL is zeros
+ *   dr, dy  gradients of r and y, of y's type; dr may be dz itself
+ *   dgamma_*, dbeta_*  [1,n] f32; dgate the gate's shape and type
+ * A NULL output is not stored.  work: rt_block_backward_workspace(m, n) f32.
+ * Sums over rows are taken in a fixed order: results do not change from run
+ * to run on one kind of device. */
+typedef struct {
+    const rt_tensor* dz;
+    const rt_tensor* dh;
+    rt_tensor* dr;
+    rt_tensor* dy;
+    rt_tensor* dgamma_post;
+    rt_tensor* dbeta_post;
+    rt_tensor* dgamma_pre;
+    rt_tensor* dbeta_pre;
+    rt_tensor* dgate;
+    rt_tensor* work;
+} rt_block_grads;
+int rt_block_backward(rt_ctx* ctx, const rt_block_args* args, const rt_block_grads* grads);
+/* f32 elements of rt_block_grads.work on this context (-1: bad extents). */
+int64_t rt_block_backward_workspace(rt_ctx* ctx, int64_t m, int64_t n);
+
 /* ------------------------------------------------------------ MLP plan */
 typedef enum { RT_OPT_NONE = 0, RT_OPT_SGD = 1, RT_OPT_ADAM = 2 } rt_optimizer;
 /* How a bf16 plan stores its hidden activations (f32 plans ignore it):

@@ -9,6 +9,8 @@ from .gpu import (  # noqa: F401
     Gpu,
     GpuMlp,
     GpuTensor,
+    Mx4Tensor,
+    Norm,
     RtError,
     bf16_to_f32,
     f32_to_bf16,
@@ -16,7 +18,8 @@ from .gpu import (  # noqa: F401
     upload_labels,
 )
 
-__all__ = ["Comm", "Gpu", "GpuMlp", "GpuTensor", "RtError", "bf16_to_f32", "f32_to_bf16", "lib", "upload_labels"]
+__all__ = ["Comm", "Gpu", "GpuMlp", "GpuTensor", "Mx4Tensor", "Norm", "RtError", "bf16_to_f32", "f32_to_bf16", "lib",
+           "upload_labels"]
 
 
 def build(verbose: bool = False) -> str:

@@ -84,6 +84,18 @@ struct rt_tensor {
     bool owned = false;
 };
 
+// A matrix [rows, k] in microscaled 4-bit floating point (rtgpu.h has the layout).
+struct rt_mx4 {
+    rt_ctx* ctx = nullptr;
+    uint8_t* codes = nullptr;
+    uint8_t* scales = nullptr;
+    int64_t rows = 0, k = 0;
+    bool owned = false;
+    __host__ __device__ int64_t blocks() const { return (k + 31) / 32; }
+    __host__ __device__ int64_t row_bytes() const { return blocks() * 16; }
+    __host__ __device__ int64_t groups() const { return (blocks() + 3) / 4; }  // scale tiles along k
+};
+
 namespace rt {
 
 // ------------------------------------------------------------- kernels
@@ -252,6 +264,10 @@ int launch_sum_partials_own(rt_ctx* ctx, float* out, const float* own, const flo
 // turns the dW GEMM into a dW + db GEMM).
 int launch_fill_column(rt_ctx* ctx, void* p, rt_dtype dt, int64_t rows, int64_t ld, int64_t col, float value,
                        cudaStream_t stream);
+
+// C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU) of microscaled 4-bit matrices.
+int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
+                    cudaStream_t stream);
 
 // Multi-tensor optimiser.  Each entry updates a packed f32 buffer of n
 // elements (theta, g, m, v) and optionally writes a bf16 shadow copy.

@@ -25,10 +25,12 @@ RT_NN, RT_NT, RT_TN = 0, 1, 2
 RT_EPI_NONE, RT_EPI_BIAS, RT_EPI_BIAS_RELU, RT_EPI_RELU_MASK = 0, 1, 2, 3
 RT_OPT_NONE, RT_OPT_SGD, RT_OPT_ADAM = 0, 1, 2
 RT_ACT_SPLIT, RT_ACT_BF16 = 0, 1
+RT_NORM_NONE, RT_NORM_RMS, RT_NORM_LAYER = 0, 1, 2
 
 _DTYPES = {"f32": RT_F32, "float32": RT_F32, "bf16": RT_BF16, "bfloat16": RT_BF16, "u32": RT_U32}
 _OPTS = {"none": RT_OPT_NONE, "sgd": RT_OPT_SGD, "adam": RT_OPT_ADAM}
 _ACTS = {"split": RT_ACT_SPLIT, "bf16": RT_ACT_BF16}
+_NORMS = {"none": RT_NORM_NONE, "rms": RT_NORM_RMS, "layer": RT_NORM_LAYER}
 
 
 class RtError(RuntimeError):
@@ -58,6 +60,22 @@ class MlpConfig(C.Structure):
         ("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
         ("activations", C.c_int),
     ]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [("kind", C.c_int), ("eps", C.c_float), ("gamma", C.c_void_p), ("beta", C.c_void_p)]
+
+
+class BlockArgs(C.Structure):
+    _fields_ = [
+        ("r", C.c_void_p), ("y", C.c_void_p), ("post", NormArgs), ("gate", C.c_void_p), ("scale", C.c_float),
+        ("z", C.c_void_p), ("pre", NormArgs), ("h", C.c_void_p), ("hq", C.c_void_p),
+    ]
+
+
+class BlockGrads(C.Structure):
+    _fields_ = [(f, C.c_void_p) for f in ("dz", "dh", "dr", "dy", "dgamma_post", "dbeta_post", "dgamma_pre",
+                                          "dbeta_pre", "dgate", "work")]
 
 
 _lib = None
@@ -108,6 +126,20 @@ _SIGS = [
     ("rt_adam", C.c_int, [C.c_void_p] * 5 + [C.c_float] * 4 + [C.c_int]),
     ("rt_sgd", C.c_int, [C.c_void_p] * 3 + [C.c_float]),
     ("rt_cast", C.c_int, [C.c_void_p] * 3),
+    ("rt_mx4_zeros", C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.POINTER(C.c_void_p)]),
+    ("rt_mx4_wrap", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.POINTER(C.c_void_p)]),
+    ("rt_mx4_free", C.c_int, [C.c_void_p]),
+    ("rt_mx4_dims", C.c_int, [C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
+    ("rt_mx4_codes", C.c_void_p, [C.c_void_p]),
+    ("rt_mx4_scales", C.c_void_p, [C.c_void_p]),
+    ("rt_mx4_code_bytes", C.c_int64, [C.c_int64, C.c_int64]),
+    ("rt_mx4_scale_bytes", C.c_int64, [C.c_int64, C.c_int64]),
+    ("rt_mx4_quantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    ("rt_mx4_dequantize", C.c_int, [C.c_void_p] * 3),
+    ("rt_mx4_matmul", C.c_int, [C.c_void_p] * 5 + [C.c_int]),
+    ("rt_block_forward", C.c_int, [C.c_void_p, C.POINTER(BlockArgs)]),
+    ("rt_block_backward", C.c_int, [C.c_void_p, C.POINTER(BlockArgs), C.POINTER(BlockGrads)]),
+    ("rt_block_backward_workspace", C.c_int64, [C.c_void_p, C.c_int64, C.c_int64]),
     ("rt_mlp_create", C.c_int, [C.c_void_p, C.POINTER(MlpConfig), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p),
                                 C.POINTER(C.c_void_p)]),
     ("rt_mlp_destroy", C.c_int, [C.c_void_p]),
@@ -262,6 +294,69 @@ class GpuTensor:
             pass
 
 
+class Mx4Tensor:
+    """A device matrix [rows, k] in microscaled 4-bit floating point (rt_mx4):
+    E2M1 elements, one power-of-two scale per 32 along k."""
+
+    def __init__(self, gpu: "Gpu", handle: int):
+        self.gpu = gpu
+        self.handle = C.c_void_p(handle)
+        r, k = C.c_int64(), C.c_int64()
+        _check(lib().rt_mx4_dims(self.handle, C.byref(r), C.byref(k)))
+        self.rows, self.k = r.value, k.value
+
+    @property
+    def shape(self):
+        return (self.rows, self.k)
+
+    @property
+    def codes_ptr(self) -> int:
+        return lib().rt_mx4_codes(self.handle)
+
+    @property
+    def scales_ptr(self) -> int:
+        return lib().rt_mx4_scales(self.handle)
+
+    @staticmethod
+    def nbytes(rows: int, k: int):
+        """(bytes of the codes, bytes of the scales) of a rows x k matrix."""
+        return lib().rt_mx4_code_bytes(rows, k), lib().rt_mx4_scale_bytes(rows, k)
+
+    def free(self):
+        if self.handle and self.handle.value:
+            if self.gpu.alive():
+                lib().rt_mx4_free(self.handle)
+            self.handle = C.c_void_p(0)
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Norm:
+    """A row norm of Gpu.block_forward / block_backward: kind "rms", "layer" or
+    "none", gamma and beta [1, n] f32 tensors or None (ones, zeros)."""
+
+    def __init__(self, kind: str = "rms", eps: float = 1e-5, gamma: GpuTensor | None = None,
+                 beta: GpuTensor | None = None):
+        self.kind, self.eps, self.gamma, self.beta = kind, eps, gamma, beta
+        self.args = NormArgs(_NORMS[kind], eps, _handle(gamma), _handle(beta))
+
+
+_NO_NORM = NormArgs(RT_NORM_NONE, 0.0, None, None)
+
+
+def _handle(t):
+    """The handle of an optional argument; a freed tensor is not taken for none."""
+    if t is None:
+        return None
+    if not t.handle.value:
+        raise RtError(RT_ERR_INVALID, "a tensor was used after free()")
+    return t.handle
+
+
 class Gpu:
     """CUDA context on one B200 (Gpu, gpu/mod.rs:224-1287)."""
 
@@ -401,6 +496,64 @@ class Gpu:
 
     def cast(self, src, dst):
         _check(lib().rt_cast(self.handle, src.handle, dst.handle))
+
+    # --- microscaled 4-bit matrices (new; rtgpu.h has the format)
+    def mx4_zeros(self, rows: int, k: int) -> Mx4Tensor:
+        h = C.c_void_p()
+        _check(lib().rt_mx4_zeros(self.handle, rows, k, C.byref(h)))
+        return Mx4Tensor(self, h.value)
+
+    def mx4_wrap(self, codes_ptr: int, scales_ptr: int, rows: int, k: int) -> Mx4Tensor:
+        """View of caller memory; Mx4Tensor.nbytes gives the sizes."""
+        h = C.c_void_p()
+        _check(lib().rt_mx4_wrap(self.handle, codes_ptr, scales_ptr, rows, k, C.byref(h)))
+        return Mx4Tensor(self, h.value)
+
+    def mx4_quantize(self, src: GpuTensor, dst: Mx4Tensor | None = None, axis: int = 1) -> Mx4Tensor:
+        """src in 4 bits with blocks along a row (axis 1), or down a column and
+        laid out transposed (axis 0)."""
+        if dst is None:
+            dst = self.mx4_zeros(*(src.shape if axis == 1 else src.shape[::-1]))
+        _check(lib().rt_mx4_quantize(self.handle, src.handle, axis, dst.handle))
+        return dst
+
+    def mx4_dequantize(self, q: Mx4Tensor, dst: GpuTensor):
+        _check(lib().rt_mx4_dequantize(self.handle, q.handle, dst.handle))
+
+    def mx4_matmul(self, a: Mx4Tensor, b: Mx4Tensor, c: GpuTensor, bias: GpuTensor | None = None, relu: bool = False):
+        """C[m,n] = A[m,k] B[n,k]^T + bias, ReLU if asked."""
+        _check(lib().rt_mx4_matmul(self.handle, a.handle, b.handle, c.handle, _handle(bias), int(relu)))
+
+    # --- residual-block norms (new)
+    def block_forward(self, r: GpuTensor, *, y: GpuTensor | None = None, post: Norm | None = None,
+                      gate: GpuTensor | None = None, scale: float = 1.0, z: GpuTensor | None = None,
+                      pre: Norm | None = None, h: GpuTensor | None = None, hq: Mx4Tensor | None = None):
+        """z = r + scale * gate * post(y) and h = pre(z) in one pass; h also, or
+        only, in 4 bits (hq).  Without y, z = r."""
+        a = BlockArgs(r.handle, _handle(y), post.args if post else _NO_NORM, _handle(gate), scale, _handle(z),
+                      pre.args if pre else _NO_NORM, _handle(h), _handle(hq))
+        _check(lib().rt_block_forward(self.handle, C.byref(a)))
+
+    def block_backward(self, z: GpuTensor, *, y: GpuTensor | None = None, post: Norm | None = None,
+                       gate: GpuTensor | None = None, scale: float = 1.0, pre: Norm | None = None,
+                       dz: GpuTensor | None = None, dh: GpuTensor | None = None, dr: GpuTensor | None = None,
+                       dy: GpuTensor | None = None, dgamma_post: GpuTensor | None = None,
+                       dbeta_post: GpuTensor | None = None, dgamma_pre: GpuTensor | None = None,
+                       dbeta_pre: GpuTensor | None = None, dgate: GpuTensor | None = None,
+                       work: GpuTensor | None = None):
+        """Gradients of block_forward from those of z and h; z is the stored
+        residual stream, work block_backward_workspace(m, n) f32."""
+        a = BlockArgs(None, _handle(y), post.args if post else _NO_NORM, _handle(gate), scale, z.handle,
+                      pre.args if pre else _NO_NORM, None, None)
+        g = BlockGrads(_handle(dz), _handle(dh), _handle(dr), _handle(dy), _handle(dgamma_post), _handle(dbeta_post),
+                       _handle(dgamma_pre), _handle(dbeta_pre), _handle(dgate), _handle(work))
+        _check(lib().rt_block_backward(self.handle, C.byref(a), C.byref(g)))
+
+    def block_backward_workspace(self, m: int, n: int) -> int:
+        v = lib().rt_block_backward_workspace(self.handle, m, n)
+        if v < 0:
+            raise RtError(RT_ERR_INVALID, lib().rt_last_error().decode(errors="replace"))
+        return v
 
     def gemm(self, args: GemmArgs):
         _check(lib().rt_gemm(self.handle, C.byref(args)))
