@@ -1,70 +1,403 @@
-// Product of two microscaled 4-bit matrices, C[m,n] = A[m,k] B[n,k]^T.
+// Product of two microscaled 4-bit matrices on the tensor cores,
+// C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU): tcgen05.mma kind::mxf4 with one
+// E8M0 scale per 32 elements, f32 accumulators in TMEM.
+//
+// The tensor cores compute C^T: B's rows (C's columns) are the MMA's M rows, 128
+// to a CTA, and A's rows (C's rows, "tokens") its N columns.  An accumulator
+// lane is then one column of C, so 32 lanes store 32 neighbouring elements of a
+// row of C straight from registers, for any row stride and alignment of C, the
+// bias is one value per thread, and few tokens make a narrow MMA, not a wasted
+// one.
+//
+// A k stage is 256 elements: 128 bytes of codes per row (one 128-byte-swizzled
+// TMA box) and two 512-byte scale tiles per 128 rows, in memory already in the
+// order that tcgen05.cp spreads over TMEM (32 lanes x 4 columns, repeated in the
+// four lane quadrants).  Each shared-memory stage has TMEM columns for its scales
+// of its own, so the barrier that frees a stage frees its scales too.  A stage is
+// four MMAs of 64 elements, two scales a row each.  Boxes past the matrices read
+// zeros; MMAs wholly past k are not issued, and the last scale tile's bytes past
+// k's blocks are not NaN, so they meet zero codes harmlessly.
 #include "mx4.cuh"
+#include "tc_common.cuh"
 
 namespace rt {
 namespace {
 
-using namespace mx4;
+using namespace tc;
 
-// 64 x 64 outputs by 256 threads, 4 x 4 each; one block of 32 of k at a time,
-// decoded into shared memory.
-template <typename T>
-__global__ void __launch_bounds__(256) product_kernel(rt_mx4 a, rt_mx4 b, T* __restrict__ c, int64_t ldc,
-                                                      const float* __restrict__ bias, int relu) {
-    __shared__ float sa[32][65], sb[32][65];
-    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t blocks = a.blocks(), groups = a.groups();
-    float acc[4][4] = {};
-    for (int64_t kb = 0; kb < blocks; ++kb) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int r = i >> 4, p = i & 15;
-            uint32_t ca = 0, cb = 0;
-            float va = 0.0f, vb = 0.0f;
-            if (m0 + r < a.rows) {
-                ca = a.codes[((m0 + r) * blocks + kb) * 16 + p];
-                va = scale_value(a.scales[scale_offset(m0 + r, kb, groups)]);
-            }
-            if (n0 + r < b.rows) {
-                cb = b.codes[((n0 + r) * blocks + kb) * 16 + p];
-                vb = scale_value(b.scales[scale_offset(n0 + r, kb, groups)]);
-            }
-            sa[2 * p][r] = decode(ca & 15u) * va;
-            sa[2 * p + 1][r] = decode(ca >> 4) * va;
-            sb[2 * p][r] = decode(cb & 15u) * vb;
-            sb[2 * p + 1][r] = decode(cb >> 4) * vb;
+constexpr int kStageK = 256;          // elements of k in a stage
+constexpr int kStageBlocks = kStageK / 32;
+constexpr int kRowBytes = 128;        // codes of a row in a stage
+constexpr int kWBytes = 128 * kRowBytes;
+constexpr int kScaleTile = 512;       // scales of 128 rows x 4 blocks
+
+struct Mx4Params {
+    int64_t m, n;                     // C's extents
+    int tiles_m, tiles_n;             // token tiles, column tiles
+    int blocks;                       // blocks of 32 along k
+    int stages, stages_per_split;     // k stages in all, and of one split
+    void* c;
+    int64_t ldc;
+    int out_bf16;
+    const float* bias;
+    int relu;
+    int* err;
+};
+
+// kind::mxf4 instruction descriptor: E2M1 operands, both K-major, E8M0 scales;
+// `half` selects the scale bytes 0-1 or 2-3 of each TMEM word for A and B.
+__host__ __device__ constexpr uint32_t mx4_idesc(int m, int n, int half) {
+    return (1u << 7)                         // A: E2M1
+           | (1u << 10)                      // B: E2M1
+           | ((uint32_t)(n >> 3) << 17)      // N / 8
+           | (1u << 23)                      // scales: E8M0
+           | ((uint32_t)(m >> 7) << 27)      // M / 128
+           | ((uint32_t)(half * 2) << 29)    // A's scale bytes
+           | ((uint32_t)(half * 2) << 4);    // B's scale bytes
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
+                                        uint32_t sfb, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
+// One 512-byte scale tile from shared memory to four TMEM columns.
+template <int CG>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
+    // no swizzle, 8-row groups of 16-byte rows 128 bytes apart
+    const uint64_t desc = (uint64_t)((smem & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)8 << 32) | ((uint64_t)1 << 46);
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sync_cluster() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One element of C.  max(v, 0) keeps a NaN.
+__device__ __forceinline__ void store_c(const Mx4Params& p, int64_t row, int64_t col, float v, float bias) {
+    v += bias;
+    if (p.relu) v = v < 0.0f ? 0.0f : v;
+    if (p.out_bf16)
+        static_cast<__nv_bfloat16*>(p.c)[row * p.ldc + col] = __float2bfloat16_rn(v);
+    else
+        static_cast<float*>(p.c)[row * p.ldc + col] = v;
+}
+
+// ------------------------------------------------------------ one-CTA kernel
+// A CTA computes 128 columns of C for TN tokens over its share of k; the CTAs of
+// a cluster share one tile, split along k.  Their sums meet in shared memory and
+// are added in rank order, tokens dealt out over the CTAs.
+template <int TN>
+struct Geo1 {
+    static constexpr int T_BYTES = TN * kRowBytes;
+    static constexpr int STAGE_BYTES = kWBytes + T_BYTES + 4 * kScaleTile;  // codes, two scale tiles of either side
+    static constexpr int STAGES = TN <= 64 ? 4 : 3;
+    static constexpr int TMEM_COLS = TN <= 64 ? 128 : 256;  // TN, and 16 of scales a stage
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+    static_assert(TN + 16 * STAGES <= TMEM_COLS, "TMEM columns");
+    static_assert(2 * SMEM <= 226 * 1024, "two CTAs to an SM");
+    static_assert(TN * 512 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
+};
+
+constexpr int kThreads1 = 192;  // warps: 0 TMA, 1 MMA, 2-5 epilogue (one TMEM lane quadrant each)
+
+template <int TN>
+__global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                        const __grid_constant__ CUtensorMap map_t,
+                                                        const __grid_constant__ CUtensorMap map_sw,
+                                                        const __grid_constant__ CUtensorMap map_st, Mx4Params p) {
+    using G = Geo1<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* smem_w = smem;
+    uint8_t* smem_t = smem + G::STAGES * kWBytes;
+    uint8_t* smem_s = smem_t + G::STAGES * G::T_BYTES;  // [stage][W 2 tiles, T 2 tiles]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem_s + G::STAGES * 4 * kScaleTile);
+    uint64_t* empty = full + G::STAGES;
+    uint64_t* done = empty + G::STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cta_rank(), ranks = cluster_size();
+    const int tile = (int)(blockIdx.x / ranks);
+    const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+    const int s0 = (int)rank * p.stages_per_split, s1 = min(p.stages, s0 + p.stages_per_split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < G::STAGES; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
         }
-        __syncthreads();
-        for (int kk = 0; kk < 32; ++kk)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[kk][ty * 4 + i], sb[kk][tx * 4 + j], acc[i][j]);
-        __syncthreads();
+        mbar_init(smem_u32(done), 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&map_w);
+        prefetch_tmap(&map_t);
+        prefetch_tmap(&map_sw);
+        prefetch_tmap(&map_st);
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t row = m0 + ty * 4 + i, col = n0 + tx * 4 + j;
-            if (row >= a.rows || col >= b.rows) continue;
-            float v = acc[i][j] + (bias ? bias[col] : 0.0f);
-            if (relu) v = v < 0.0f ? 0.0f : v;
-            if constexpr (sizeof(T) == 2)
-                c[row * ldc + col] = __float2bfloat16_rn(v);
-            else
-                c[row * ldc + col] = v;
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(G::TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        int issued = 0;
+        bool ok = true;
+        for (int s = s0; s < s1; ++s, ++issued) {
+            const int slot = issued % G::STAGES;
+            if (!mbar_wait(smem_u32(&empty[slot]), ((issued / G::STAGES) & 1) ^ 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            const uint32_t bar = smem_u32(&full[slot]);
+            mbar_expect_tx(bar, G::STAGE_BYTES);
+            tma_load_2d(smem_u32(smem_w + slot * kWBytes), &map_w, s * kRowBytes, tn * 128, bar);
+            tma_load_2d(smem_u32(smem_t + slot * G::T_BYTES), &map_t, s * kRowBytes, tm * TN, bar);
+            const uint32_t ss = smem_u32(smem_s + slot * 4 * kScaleTile);
+            tma_load_3d(ss, &map_sw, 0, s * 2, tn, bar);
+            tma_load_3d(ss + 2 * kScaleTile, &map_st, 0, s * 2, tm * TN / 128, bar);
         }
+        if (!ok) {
+            record_error(p.err, DEV_TIMEOUT_PRODUCER, blockIdx.x);
+            *abort_flag = 1;
+            // the copies in flight write this CTA's shared memory: let them land before it exits
+            volatile int never = 0;
+            for (int i = max(0, issued - G::STAGES); i < issued; ++i)
+                mbar_wait(smem_u32(&full[i % G::STAGES]), (i / G::STAGES) & 1, &never);
+        }
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t token_col = (uint32_t)((tm * TN % 128) / 32);  // the tile's place in its 128-row scale tile
+        bool ok = true;
+        for (int s = s0, i = 0; s < s1; ++s, ++i) {
+            const int slot = i % G::STAGES;
+            if (!mbar_wait(smem_u32(&full[slot]), (i / G::STAGES) & 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t sw = smem_u32(smem_w + slot * kWBytes), st = smem_u32(smem_t + slot * G::T_BYTES);
+            const uint32_t ss = smem_u32(smem_s + slot * 4 * kScaleTile);
+            const uint32_t cols = tmem + TN + slot * 16;  // scales: W groups 0, 1, then T groups 0, 1
+#pragma unroll
+            for (int t = 0; t < 4; ++t) copy_scales<1>(cols + t * 4, ss + t * kScaleTile);
+            const int steps = min(4, (p.blocks - s * kStageBlocks + 1) / 2);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+                if (kk < steps)
+                    mma_mx4<1>(tmem, smem_desc(sw + kk * 32, 16, 1024), smem_desc(st + kk * 32, 16, 1024),
+                               mx4_idesc(128, TN, kk & 1), cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 4 + token_col,
+                               (i > 0 || kk > 0) ? 1u : 0u);
+            tc_commit(smem_u32(&empty[slot]));
+        }
+        if (!ok) {
+            record_error(p.err, DEV_TIMEOUT_MMA, blockIdx.x);
+            *abort_flag = 1;
+        }
+        tc_commit(smem_u32(done));
+    } else if (warp >= 2) {
+        const int quad = warp & 3;
+        const int64_t col = (int64_t)tn * 128 + quad * 32 + lane;
+        const int64_t row0 = (int64_t)tm * TN;
+        const int count = (int)min((int64_t)TN, p.m - row0);
+        const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
+        const bool got = mbar_wait(smem_u32(done), 0, abort_flag);
+        if (!got && lane == 0) {
+            record_error(p.err, DEV_TIMEOUT_EPILOGUE, blockIdx.x);
+            *abort_flag = 1;
+        }
+        __syncwarp();
+        tc_fence_after();
+        float* sums = reinterpret_cast<float*>(smem);  // [token][128 columns]; every stage has been read
+        for (int c = 0; c < count && __all_sync(0xffffffffu, got); c += 32) {
+            float v[32];
+            tmem_ld_32x32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
+            if (ranks == 1) {
+                if (col < p.n)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c + j < count) store_c(p, row0 + c + j, col, v[j], bias);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sums[(c + j) * 128 + quad * 32 + lane] = v[j];
+            }
+        }
+        tc_fence_before();
+    }
+    __syncwarp();
+    if (ranks > 1) {
+        sync_cluster();
+        if (warp >= 2) {
+            const int64_t col = (int64_t)tn * 128 + (warp & 3) * 32 + lane;
+            const int64_t row0 = (int64_t)tm * TN;
+            const int count = (int)min((int64_t)TN, p.m - row0);
+            const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
+            const uint32_t at = smem_u32(smem) + ((warp & 3) * 32 + lane) * 4;
+            for (int c = (int)rank; c < count; c += (int)ranks) {
+                float v = 0.0f;
+                for (uint32_t r = 0; r < ranks; ++r) v += ld_cluster(in_cta(at + c * 512, r));
+                if (col < p.n) store_c(p, row0 + c, col, v, bias);
+            }
+        }
+        sync_cluster();  // the sums are read before any CTA exits
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::TMEM_COLS) : "memory");
+    }
+}
+
+// C = bias (k = 0).
+__global__ void bias_kernel(Mx4Params p) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.m * p.n; i += (int64_t)gridDim.x * blockDim.x)
+        store_c(p, i / p.n, i % p.n, 0.0f, p.bias ? p.bias[i % p.n] : 0.0f);
+}
+
+// ---------------------------------------------------------------- host side
+int encode(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+           const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(RT_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const CUresult r = enc(map, type, rank, const_cast<void*>(base), dims, strides, box, ones,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RT_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return RT_OK;
+}
+
+// Codes: rows of row_bytes bytes, box of `rows` x 128 bytes.
+int map_codes(CUtensorMap* map, const rt_mx4& q, int rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)q.row_bytes(), (cuuint64_t)q.rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)q.row_bytes()};
+    const cuuint32_t box[2] = {kRowBytes, (cuuint32_t)rows};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q.codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Scales: tiles of 128 words, [row tile][k group]; box of 2 k groups of `tiles` row tiles.
+int map_scales(CUtensorMap* map, const rt_mx4& q, int tiles) {
+    const cuuint64_t dims[3] = {128, (cuuint64_t)q.groups(), (cuuint64_t)((q.rows + 127) / 128)};
+    const cuuint64_t strides[2] = {kScaleTile, (cuuint64_t)(q.groups() * kScaleTile)};
+    const cuuint32_t box[3] = {128, 2, (cuuint32_t)tiles};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, q.scales, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <int TN>
+int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaStream_t stream) {
+    using G = Geo1<TN>;
+    CUtensorMap w, t, sw, st;
+    RT_TRY(map_codes(&w, b, 128));
+    RT_TRY(map_codes(&t, a, TN));
+    RT_TRY(map_scales(&sw, b, 1));
+    RT_TRY(map_scales(&st, a, 1));
+    p.tiles_m = (int)((p.m + TN - 1) / TN);
+    p.tiles_n = (int)((p.n + 127) / 128);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    // split k while the CTAs fit two to an SM and each keeps two stages
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= 2 * (int64_t)ctx->sm_count && p.stages >= 4 * splits) splits *= 2;
+    p.stages_per_split = (p.stages + splits - 1) / splits;
+    splits = (p.stages + p.stages_per_split - 1) / p.stages_per_split;
+    RT_CHECK(tiles * splits <= INT32_MAX, "rt_mx4_matmul: C is too large");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * splits));
+    cfg.blockDim = dim3(kThreads1);
+    cfg.dynamicSmemBytes = G::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<TN>, w, t, sw, st, p));
+    count_launch(ctx);
+    return RT_OK;
+}
+
+template <int TN>
+int allow_smem() {
+    RT_CUDA(cudaFuncSetAttribute(mx4_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<TN>::SMEM));
+    return RT_OK;
 }
 
 }  // namespace
 
+int gemm_mx4_init() {
+    RT_TRY(allow_smem<32>());
+    RT_TRY(allow_smem<64>());
+    return allow_smem<128>();
+}
+
 int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
                     cudaStream_t stream) {
-    const dim3 grid((unsigned)((b.rows + 63) / 64), (unsigned)((a.rows + 63) / 64));
-    if (c.dtype == RT_BF16)
-        product_kernel<<<grid, 256, 0, stream>>>(a, b, static_cast<__nv_bfloat16*>(c.ptr), c.ld, bias, (int)relu);
-    else
-        product_kernel<<<grid, 256, 0, stream>>>(a, b, static_cast<float*>(c.ptr), c.ld, bias, (int)relu);
-    RT_CUDA(cudaGetLastError());
-    count_launch(ctx);
-    return RT_OK;
+    Mx4Params p{};
+    p.m = c.rows;
+    p.n = c.cols;
+    p.blocks = (int)a.blocks();
+    p.stages = (int)((a.blocks() + kStageBlocks - 1) / kStageBlocks);
+    p.c = c.ptr;
+    p.ldc = c.ld;
+    p.out_bf16 = c.dtype == RT_BF16;
+    p.bias = bias;
+    p.relu = relu;
+    p.err = ctx->dev_err;
+    RT_CUDA(cudaSetDevice(ctx->device));
+    if (p.blocks == 0) {
+        bias_kernel<<<ctx->sm_count * 4, 256, 0, stream>>>(p);
+        RT_CUDA(cudaGetLastError());
+        count_launch(ctx);
+        return RT_OK;
+    }
+    if (p.m <= 32) return launch_one<32>(ctx, a, b, p, stream);
+    if (p.m <= 64) return launch_one<64>(ctx, a, b, p, stream);
+    return launch_one<128>(ctx, a, b, p, stream);
 }
 
 }  // namespace rt

@@ -265,6 +265,7 @@ int launch_sum_partials_own(rt_ctx* ctx, float* out, const float* own, const flo
 int launch_fill_column(rt_ctx* ctx, void* p, rt_dtype dt, int64_t rows, int64_t ld, int64_t col, float value,
                        cudaStream_t stream);
 
+int gemm_mx4_init();
 // C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU) of microscaled 4-bit matrices.
 int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
                     cudaStream_t stream);
