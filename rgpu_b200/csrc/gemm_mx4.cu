@@ -17,6 +17,8 @@
 // four MMAs of 64 elements, two scales a row each.  Boxes past the matrices read
 // zeros; MMAs wholly past k are not issued, and the last scale tile's bytes past
 // k's blocks are not NaN, so they meet zero codes harmlessly.
+#include <algorithm>
+
 #include "mx4.cuh"
 #include "tc_common.cuh"
 
@@ -292,6 +294,257 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     }
 }
 
+// ----------------------------------------------------------- two-CTA kernel
+// A cluster of two CTAs on a pair of SMs computes 256 columns of C for 256
+// tokens: each CTA holds the codes of 128 of the columns and of 128 of the
+// tokens, the pair's MMAs read both, and each CTA's TMEM receives its 128
+// columns for all 256 tokens.  Half the bytes from L2 per MMA of the one-CTA
+// tile: a stage is 35 KB per CTA for 4 x 128 clocks of MMA.  The scales of all
+// 256 tokens are needed by both CTAs, so each loads them itself.
+//
+// The f32 accumulator takes 256 of the 512 TMEM columns and the scales 24 a
+// stage, which leaves no room for a second accumulator: instead the eight
+// epilogue warps draw the finished tile into 128 registers a thread and hand the
+// accumulator back at once, so the next tile's MMAs wait for that only, not for
+// the stores.  Persistent: tiles are dealt out round robin, the loads of the next
+// tile run on while this one's epilogue stores.
+constexpr int kPairStages = 6;
+constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of W and T, two tiles of W's scales, four of T's
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024 + 256;
+constexpr int kPairThreads = 320;  // warps: 0 TMA, 1 MMA (leader), 2-9 epilogue (two to a TMEM lane quadrant)
+static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
+static_assert(256 + 24 * kPairStages <= 512, "TMEM columns");
+
+__device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_pair_3d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// Token tiles in groups of eight, the columns inside: the tiles in flight share operands in L2.
+__device__ __forceinline__ void pair_tile(const Mx4Params& p, int t, int& tm, int& tn) {
+    const int per = 8 * p.tiles_n, first = t / per * 8, rows = min(8, p.tiles_m - first), in = t % per;
+    tm = first + in % rows;
+    tn = in / rows;
+}
+
+// 32 tokens of one column a lane, stored.  bf16 with even strides: neighbouring
+// lanes trade so that each stores two columns of one token, the even lane of one
+// token and the odd lane of the next.
+__device__ __forceinline__ void store_tokens(const Mx4Params& p, int64_t row0, int count, int64_t col, float bias,
+                                             bool pairs, float (&v)[32]) {
+    if (pairs) {
+        const bool odd = col & 1;
+        __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.c) + (row0 + (odd ? 1 : 0)) * p.ldc + (col & ~int64_t(1));
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            float a = v[j] + bias, b = v[j + 1] + bias;
+            if (p.relu) {
+                a = a < 0.0f ? 0.0f : a;
+                b = b < 0.0f ? 0.0f : b;
+            }
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+            const __nv_bfloat162 two = odd ? __floats2bfloat162_rn(other, b) : __floats2bfloat162_rn(a, other);
+            if (j + (odd ? 1 : 0) < count && col < p.n) *reinterpret_cast<__nv_bfloat162*>(c + j * p.ldc) = two;
+        }
+    } else if (col < p.n) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < count) store_c(p, row0 + j, col, v[j], bias);
+    }
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                   const __grid_constant__ CUtensorMap map_t,
+                                                                   const __grid_constant__ CUtensorMap map_sw,
+                                                                   const __grid_constant__ CUtensorMap map_st,
+                                                                   Mx4Params p) {
+    constexpr int S = kPairStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* smem_w = smem;
+    uint8_t* smem_t = smem + S * kWBytes;
+    uint8_t* smem_s = smem + 2 * S * kWBytes;  // [stage][W groups 0, 1; tokens 0-127 groups 0, 1; tokens 128-255]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem_s + S * 6 * kScaleTile);  // leader: both CTAs' bytes of a stage
+    uint64_t* empty = full + S;   // each CTA: stage read by the MMAs
+    uint64_t* tfull = empty + S;  // each CTA: accumulator complete
+    uint64_t* tempty = tfull + 1; // leader: accumulator drawn by both CTAs' epilogues
+    uint64_t* drain = tempty + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* issued_all = abort_flag + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cta_rank();
+    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+    const int tiles = p.tiles_m * p.tiles_n;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        mbar_init(smem_u32(tfull), 1);
+        mbar_init(smem_u32(tempty), 16);  // epilogue warps of both CTAs
+        mbar_init(smem_u32(drain), 1);
+        *abort_flag = 0;
+        *issued_all = 0;
+        fence_barrier_init();
+        prefetch_tmap(&map_w);
+        prefetch_tmap(&map_t);
+        prefetch_tmap(&map_sw);
+        prefetch_tmap(&map_st);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    sync_cluster();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto raise_abort = [&](int code) {
+        record_error(p.err, code, blockIdx.x);
+        *abort_flag = 1;
+        store_cluster(in_cta(smem_u32((const void*)abort_flag), rank ^ 1u), 1u);
+    };
+
+    if (warp == 0 && lane == 0) {
+        int issued = 0;
+        bool ok = true;
+        for (int t = cluster; t < tiles && ok; t += clusters) {
+            int tm, tn;
+            pair_tile(p, t, tm, tn);
+            for (int s = 0; s < p.stages; ++s) {
+                const int slot = issued % S;
+                if (!mbar_wait(smem_u32(&empty[slot]), ((issued / S) & 1) ^ 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                if (rank == 0) mbar_expect_tx(smem_u32(&full[slot]), 2 * kPairStageBytes);
+                const uint32_t bar = in_cta(smem_u32(&full[slot]), 0);
+                tma_pair_2d(smem_u32(smem_w + slot * kWBytes), &map_w, s * kRowBytes, tn * 256 + (int)rank * 128, bar);
+                tma_pair_2d(smem_u32(smem_t + slot * kWBytes), &map_t, s * kRowBytes, tm * 256 + (int)rank * 128, bar);
+                const uint32_t ss = smem_u32(smem_s + slot * 6 * kScaleTile);
+                tma_pair_3d(ss, &map_sw, 0, s * 2, tn * 2 + (int)rank, bar);
+                tma_pair_3d(ss + 2 * kScaleTile, &map_st, 0, s * 2, tm * 2, bar);
+                ++issued;
+            }
+        }
+        *issued_all = issued;
+        if (!ok) raise_abort(DEV_TIMEOUT_PRODUCER);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        int i = 0, done = 0;
+        bool ok = true;
+        for (int t = cluster; t < tiles && ok; t += clusters, ++done) {
+            if (!mbar_wait(smem_u32(tempty), (done & 1) ^ 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            for (int s = 0; s < p.stages; ++s, ++i) {
+                const int slot = i % S;
+                if (!mbar_wait(smem_u32(&full[slot]), (i / S) & 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t sw = smem_u32(smem_w + slot * kWBytes), st = smem_u32(smem_t + slot * kWBytes);
+                const uint32_t ss = smem_u32(smem_s + slot * 6 * kScaleTile);
+                const uint32_t cols = tmem + 256 + slot * 24;  // W group 0, W group 1, T group 0 (8 wide), T group 1
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    copy_scales<2>(cols + g * 4, ss + g * kScaleTile);
+                    copy_scales<2>(cols + 8 + g * 8, ss + (2 + g) * kScaleTile);
+                    copy_scales<2>(cols + 8 + g * 8 + 4, ss + (4 + g) * kScaleTile);
+                }
+                const int steps = min(4, (p.blocks - s * kStageBlocks + 1) / 2);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    if (kk < steps)
+                        mma_mx4<2>(tmem, smem_desc(sw + kk * 32, 16, 1024), smem_desc(st + kk * 32, 16, 1024),
+                                   mx4_idesc(256, 256, kk & 1), cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8,
+                                   (s > 0 || kk > 0) ? 1u : 0u);
+                commit_pair(smem_u32(&empty[slot]));
+                commit_pair(in_cta(smem_u32(&empty[slot]), 1));
+            }
+            if (!ok) break;
+            commit_pair(smem_u32(tfull));
+            commit_pair(in_cta(smem_u32(tfull), 1));
+        }
+        if (!ok) raise_abort(DEV_TIMEOUT_MMA);
+        commit_pair(smem_u32(drain));
+        mbar_wait(smem_u32(drain), 0, abort_flag);
+    } else if (warp >= 2) {
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        const bool pairs = p.out_bf16 && (p.ldc & 1) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 3) == 0 && (p.n & 1) == 0;
+        int done = 0;
+        bool ok = true;
+        for (int t = cluster; t < tiles; t += clusters, ++done) {
+            int tm, tn;
+            pair_tile(p, t, tm, tn);
+            const bool got = mbar_wait(smem_u32(tfull), done & 1, abort_flag);
+            if (!__all_sync(0xffffffffu, got)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            float v[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                tmem_ld_32x32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128 + c * 32), v[c]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), 0));
+            const int64_t col = (int64_t)tn * 256 + rank * 128 + quad * 32 + lane;
+            const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int64_t row0 = (int64_t)tm * 256 + half * 128 + c * 32;
+                const int count = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
+                store_tokens(p, row0, count, col, bias, pairs, v[c]);
+            }
+        }
+        if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
+    }
+    __syncwarp();
+    __syncthreads();
+    if (*abort_flag && rank == 0 && threadIdx.x == 0) {
+        // the pair's copies complete on the leader's barriers: wait for the last ones issued
+        volatile int never = 0;
+        for (int i = max(0, *issued_all - S); i < *issued_all; ++i) mbar_wait(smem_u32(&full[i % S]), (i / S) & 1, &never);
+    }
+    tc_fence_before();
+    __syncthreads();
+    sync_cluster();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
 // C = bias (k = 0).
 __global__ void bias_kernel(Mx4Params p) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.m * p.n; i += (int64_t)gridDim.x * blockDim.x)
@@ -361,6 +614,33 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaS
     return RT_OK;
 }
 
+int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaStream_t stream) {
+    CUtensorMap w, t, sw, st;
+    RT_TRY(map_codes(&w, b, 128));
+    RT_TRY(map_codes(&t, a, 128));
+    RT_TRY(map_scales(&sw, b, 1));
+    RT_TRY(map_scales(&st, a, 2));
+    p.tiles_m = (int)((p.m + 255) / 256);
+    p.tiles_n = (int)((p.n + 255) / 256);
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    RT_CHECK(tiles <= INT32_MAX, "rt_mx4_matmul: C is too large");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_pair_kernel, w, t, sw, st, p));
+    count_launch(ctx);
+    return RT_OK;
+}
+
 template <int TN>
 int allow_smem() {
     RT_CUDA(cudaFuncSetAttribute(mx4_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<TN>::SMEM));
@@ -372,6 +652,7 @@ int allow_smem() {
 int gemm_mx4_init() {
     RT_TRY(allow_smem<32>());
     RT_TRY(allow_smem<64>());
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
     return allow_smem<128>();
 }
 
@@ -397,6 +678,7 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
     }
     if (p.m <= 32) return launch_one<32>(ctx, a, b, p, stream);
     if (p.m <= 64) return launch_one<64>(ctx, a, b, p, stream);
+    if (((p.m + 255) / 256) * ((p.n + 255) / 256) * 4 >= ctx->sm_count) return launch_pair(ctx, a, b, p, stream);
     return launch_one<128>(ctx, a, b, p, stream);
 }
 

@@ -150,7 +150,8 @@ def _product_check(got, a, b, bias, relu, dtype):
 PRODUCTS = [(1, 1, 1), (1, 1, 32), (1, 17, 33), (2, 130, 64), (3, 128, 65), (16, 200, 100), (31, 129, 224), (32, 1000, 256),
             (33, 64, 288), (63, 500, 96), (64, 256, 512), (65, 257, 1000), (100, 1, 513), (127, 127, 127), (128, 128, 128),
             (129, 384, 320), (255, 130, 2048), (256, 256, 256), (257, 513, 640), (300, 1000, 1024), (513, 777, 1056),
-            (1024, 512, 96), (1, 4096, 4096), (7, 1000, 8192), (48, 3000, 1500), (640, 1280, 2560)]
+            (1024, 512, 96), (1, 4096, 4096), (7, 1000, 8192), (48, 3000, 1500), (640, 1280, 2560),
+            (2000, 2001, 1100), (1601, 2304, 800), (2305, 1537, 64), (4100, 3001, 33)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
