@@ -77,16 +77,32 @@ __device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t ad, uint64_t bd, ui
             : "memory");
 }
 
+// Descriptor of a scale tile in shared memory: no swizzle, 8-row groups of
+// 16-byte rows 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem) {
+    return (uint64_t)((smem & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)8 << 32) | ((uint64_t)1 << 46);
+}
+
 // One 512-byte scale tile from shared memory to four TMEM columns.
 template <int CG>
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
-    // no swizzle, 8-row groups of 16-byte rows 128 bytes apart
-    const uint64_t desc = (uint64_t)((smem & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)8 << 32) | ((uint64_t)1 << 46);
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
     if constexpr (CG == 1)
         asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
     else
         asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
+
+// One lane of a converged warp.  The MMA warps run their loops with all lanes
+// and issue from the elected one: descriptors and TMEM addresses then stay in
+// uniform registers, where a lone diverged lane moves each into one for every
+// instruction (measured at 8192^3: 120 clocks for each MMA issued, 335 more a
+// stage, against 128 that the MMA takes).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 __device__ __forceinline__ uint32_t cta_rank() {
     uint32_t r;
@@ -157,7 +173,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t rank = cta_rank(), ranks = cluster_size();
     const int tile = (int)(blockIdx.x / ranks);
     const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
@@ -185,7 +201,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
 
     if (warp == 0 && lane == 0) {
         int issued = 0;
@@ -212,35 +228,47 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
             for (int i = max(0, issued - G::STAGES); i < issued; ++i)
                 mbar_wait(smem_u32(&full[i % G::STAGES]), (i / G::STAGES) & 1, &never);
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         const uint32_t token_col = (uint32_t)((tm * TN % 128) / 32);  // the tile's place in its 128-row scale tile
+        const uint64_t w0 = smem_desc(smem_u32(smem_w), 16, 1024), t0 = smem_desc(smem_u32(smem_t), 16, 1024);
+        const uint64_t sc0 = scale_desc(smem_u32(smem_s));
+        const uint32_t cols0 = tmem + TN;
         bool ok = true;
-        for (int s = s0, i = 0; s < s1; ++s, ++i) {
-            const int slot = i % G::STAGES;
-            if (!mbar_wait(smem_u32(&full[slot]), (i / G::STAGES) & 1, abort_flag)) {
+        int slot = 0, phase = 0;
+        for (int s = s0; s < s1; ++s) {
+            ok = mbar_wait(smem_u32(&full[slot]), phase, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t sw = smem_u32(smem_w + slot * kWBytes), st = smem_u32(smem_t + slot * G::T_BYTES);
-            const uint32_t ss = smem_u32(smem_s + slot * 4 * kScaleTile);
-            const uint32_t cols = tmem + TN + slot * 16;  // scales: W groups 0, 1, then T groups 0, 1
-#pragma unroll
-            for (int t = 0; t < 4; ++t) copy_scales<1>(cols + t * 4, ss + t * kScaleTile);
+            const uint64_t w = w0 + slot * (kWBytes >> 4), t = t0 + slot * (G::T_BYTES >> 4);
+            const uint64_t sc = sc0 + slot * (4 * kScaleTile >> 4);
+            const uint32_t cols = cols0 + slot * 16;  // scales: W groups 0, 1, then T groups 0, 1
             const int steps = min(4, (p.blocks - s * kStageBlocks + 1) / 2);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-                if (kk < steps)
-                    mma_mx4<1>(tmem, smem_desc(sw + kk * 32, 16, 1024), smem_desc(st + kk * 32, 16, 1024),
-                               mx4_idesc(128, TN, kk & 1), cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 4 + token_col,
-                               (i > 0 || kk > 0) ? 1u : 0u);
-            tc_commit(smem_u32(&empty[slot]));
+                for (int i = 0; i < 4; ++i) copy_scales<1>(cols + i * 4, sc + i * (kScaleTile >> 4));
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    if (kk < steps)
+                        mma_mx4<1>(tmem, w + kk * 2, t + kk * 2, mx4_idesc(128, TN, kk & 1), cols + (kk >> 1) * 4,
+                                   cols + 8 + (kk >> 1) * 4 + token_col, (s > s0 || kk > 0) ? 1u : 0u);
+                tc_commit(smem_u32(&empty[slot]));
+            }
+            __syncwarp();
+            if (++slot == G::STAGES) {
+                slot = 0;
+                phase ^= 1;
+            }
         }
-        if (!ok) {
-            record_error(p.err, DEV_TIMEOUT_MMA, blockIdx.x);
-            *abort_flag = 1;
+        if (elect_one()) {
+            if (!ok) {
+                record_error(p.err, DEV_TIMEOUT_MMA, blockIdx.x);
+                *abort_flag = 1;
+            }
+            tc_commit(smem_u32(done));
         }
-        tc_commit(smem_u32(done));
     } else if (warp >= 2) {
         const int quad = warp & 3;
         const int64_t col = (int64_t)tn * 128 + quad * 32 + lane;
@@ -393,7 +421,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* issued_all = abort_flag + 1;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t rank = cta_rank();
     const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
     const int tiles = p.tiles_m * p.tiles_n;
@@ -424,7 +452,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     __syncthreads();
     sync_cluster();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     auto raise_abort = [&](int code) {
         record_error(p.err, code, blockIdx.x);
         *abort_flag = 1;
@@ -455,48 +483,58 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         }
         *issued_all = issued;
         if (!ok) raise_abort(DEV_TIMEOUT_PRODUCER);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        int i = 0, done = 0;
+    } else if (warp == 1 && rank == 0) {
+        const uint64_t w0 = smem_desc(smem_u32(smem_w), 16, 1024), t0 = smem_desc(smem_u32(smem_t), 16, 1024);
+        const uint64_t sc0 = scale_desc(smem_u32(smem_s));
+        const uint32_t empty0 = smem_u32(empty), empty1 = in_cta(empty0, 1);
+        const uint32_t tfull0 = smem_u32(tfull), tfull1 = in_cta(tfull0, 1);
+        int slot = 0, phase = 0, done = 0;
         bool ok = true;
         for (int t = cluster; t < tiles && ok; t += clusters, ++done) {
-            if (!mbar_wait(smem_u32(tempty), (done & 1) ^ 1, abort_flag)) {
-                ok = false;
-                break;
-            }
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(tempty), (done & 1) ^ 1, abort_flag));
+            if (!ok) break;
             tc_fence_after();
-            for (int s = 0; s < p.stages; ++s, ++i) {
-                const int slot = i % S;
-                if (!mbar_wait(smem_u32(&full[slot]), (i / S) & 1, abort_flag)) {
-                    ok = false;
-                    break;
-                }
+            for (int s = 0; s < p.stages; ++s) {
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), phase, abort_flag));
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t sw = smem_u32(smem_w + slot * kWBytes), st = smem_u32(smem_t + slot * kWBytes);
-                const uint32_t ss = smem_u32(smem_s + slot * 6 * kScaleTile);
+                const uint64_t wd = w0 + slot * (kWBytes >> 4), td = t0 + slot * (kWBytes >> 4);
+                const uint64_t sc = sc0 + slot * (6 * kScaleTile >> 4);
                 const uint32_t cols = tmem + 256 + slot * 24;  // W group 0, W group 1, T group 0 (8 wide), T group 1
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    copy_scales<2>(cols + g * 4, ss + g * kScaleTile);
-                    copy_scales<2>(cols + 8 + g * 8, ss + (2 + g) * kScaleTile);
-                    copy_scales<2>(cols + 8 + g * 8 + 4, ss + (4 + g) * kScaleTile);
-                }
                 const int steps = min(4, (p.blocks - s * kStageBlocks + 1) / 2);
+                if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    if (kk < steps)
-                        mma_mx4<2>(tmem, smem_desc(sw + kk * 32, 16, 1024), smem_desc(st + kk * 32, 16, 1024),
-                                   mx4_idesc(256, 256, kk & 1), cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8,
-                                   (s > 0 || kk > 0) ? 1u : 0u);
-                commit_pair(smem_u32(&empty[slot]));
-                commit_pair(in_cta(smem_u32(&empty[slot]), 1));
+                    for (int g = 0; g < 2; ++g) {
+                        copy_scales<2>(cols + g * 4, sc + g * (kScaleTile >> 4));
+                        copy_scales<2>(cols + 8 + g * 8, sc + (2 + g) * (kScaleTile >> 4));
+                        copy_scales<2>(cols + 8 + g * 8 + 4, sc + (4 + g) * (kScaleTile >> 4));
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        if (kk < steps)
+                            mma_mx4<2>(tmem, wd + kk * 2, td + kk * 2, mx4_idesc(256, 256, kk & 1),
+                                       cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8, (s > 0 || kk > 0) ? 1u : 0u);
+                    commit_pair(empty0 + slot * 8);
+                    commit_pair(empty1 + slot * 8);
+                }
+                __syncwarp();
+                if (++slot == S) {
+                    slot = 0;
+                    phase ^= 1;
+                }
             }
             if (!ok) break;
-            commit_pair(smem_u32(tfull));
-            commit_pair(in_cta(smem_u32(tfull), 1));
+            if (elect_one()) {
+                commit_pair(tfull0);
+                commit_pair(tfull1);
+            }
+            __syncwarp();
         }
-        if (!ok) raise_abort(DEV_TIMEOUT_MMA);
-        commit_pair(smem_u32(drain));
-        mbar_wait(smem_u32(drain), 0, abort_flag);
+        if (elect_one()) {
+            if (!ok) raise_abort(DEV_TIMEOUT_MMA);
+            commit_pair(smem_u32(drain));
+            mbar_wait(smem_u32(drain), 0, abort_flag);
+        }
     } else if (warp >= 2) {
         const int quad = warp & 3, half = (warp - 2) >> 2;
         const bool pairs = p.out_bf16 && (p.ldc & 1) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 3) == 0 && (p.n & 1) == 0;
