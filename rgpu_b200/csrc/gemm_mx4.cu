@@ -43,6 +43,7 @@ struct Mx4Params {
     int out_bf16;
     const float* bias;
     int relu;
+    int staged;                       // two-CTA kernel: C is stored through TMA boxes
     int* err;
 };
 
@@ -119,13 +120,37 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 __device__ __forceinline__ void sync_cluster() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_nowait(uint32_t taddr, float (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+// Waits for the loads above; naming the registers keeps their uses behind it.
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[4][32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) asm volatile("" : "+f"(v[c][j]));
 }
 
 // One element of C.  max(v, 0) keeps a NaN.
@@ -136,6 +161,31 @@ __device__ __forceinline__ void store_c(const Mx4Params& p, int64_t row, int64_t
         static_cast<__nv_bfloat16*>(p.c)[row * p.ldc + col] = __float2bfloat16_rn(v);
     else
         static_cast<float*>(p.c)[row * p.ldc + col] = v;
+}
+
+// Four neighbouring elements of a row of C, as one store where they lie so.
+__device__ __forceinline__ void store_c4(const Mx4Params& p, int64_t row, int64_t col, float4 v, const float (&bias)[4]) {
+    float x[4] = {v.x, v.y, v.z, v.w};
+    const int64_t at = row * p.ldc + col;
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(p.c) + at * (p.out_bf16 ? 2 : 4);
+    if (col + 3 < p.n && (addr & (p.out_bf16 ? 7 : 15)) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] += bias[i];
+            if (p.relu) x[i] = x[i] < 0.0f ? 0.0f : x[i];
+        }
+        if (p.out_bf16) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+            *reinterpret_cast<uint2*>(addr) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+            *reinterpret_cast<float4*>(addr) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (col + i < p.n) store_c(p, row, col + i, x[i], bias[i]);
+    }
 }
 
 // ------------------------------------------------------------ one-CTA kernel
@@ -302,15 +352,28 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     if (ranks > 1) {
         sync_cluster();
         if (warp >= 2) {
-            const int64_t col = (int64_t)tn * 128 + (warp & 3) * 32 + lane;
-            const int64_t row0 = (int64_t)tm * TN;
+            // a lane adds four columns of a token over the ranks; the warps take the tokens of this rank in turn
+            const int64_t row0 = (int64_t)tm * TN, col = (int64_t)tn * 128 + lane * 4;
             const int count = (int)min((int64_t)TN, p.m - row0);
-            const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
-            const uint32_t at = smem_u32(smem) + ((warp & 3) * 32 + lane) * 4;
-            for (int c = (int)rank; c < count; c += (int)ranks) {
-                float v = 0.0f;
-                for (uint32_t r = 0; r < ranks; ++r) v += ld_cluster(in_cta(at + c * 512, r));
-                if (col < p.n) store_c(p, row0 + c, col, v, bias);
+            const uint32_t at = smem_u32(smem) + lane * 16;
+            float bias[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? p.bias[col + i] : 0.0f;
+            for (int c = (int)rank + (warp - 2) * (int)ranks; c < count; c += 4 * (int)ranks) {
+                float4 part[8];
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r)
+                    if (r < ranks) part[r] = ld_cluster4(in_cta(at + c * 512, r));
+                float4 v = part[0];
+#pragma unroll
+                for (uint32_t r = 1; r < 8; ++r)
+                    if (r < ranks) {
+                        v.x += part[r].x;
+                        v.y += part[r].y;
+                        v.z += part[r].z;
+                        v.w += part[r].w;
+                    }
+                store_c4(p, row0 + c, col, v, bias);
             }
         }
         sync_cluster();  // the sums are read before any CTA exits
@@ -336,9 +399,14 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 // accumulator back at once, so the next tile's MMAs wait for that only, not for
 // the stores.  Persistent: tiles are dealt out round robin, the loads of the next
 // tile run on while this one's epilogue stores.
+//
+// Where C's rows can be TMA boxes (16-byte aligned base and stride) the epilogue
+// stages 32 tokens x 128 columns at a time in shared memory and stores them as
+// one box, whole 128-byte lines; otherwise it stores from registers.
 constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of W and T, two tiles of W's scales, four of T's
-constexpr int kPairSmem = kPairStages * kPairStageBytes + 1024 + 256;
+constexpr int kChunkBytes = 32 * 128 * 2;  // staged output of either half of the tokens: 128 columns of 32 (f32: 16) tokens
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 2 * kChunkBytes + 256;
 constexpr int kPairThreads = 320;  // warps: 0 TMA, 1 MMA (leader), 2-9 epilogue (two to a TMEM lane quadrant)
 static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
 static_assert(256 + 24 * kPairStages <= 512, "TMEM columns");
@@ -375,7 +443,7 @@ __device__ __forceinline__ void pair_tile(const Mx4Params& p, int t, int& tm, in
     tn = in / rows;
 }
 
-// 32 tokens of one column a lane, stored.  bf16 with even strides: neighbouring
+// 32 tokens of one column a lane, stored from registers.  bf16 with even strides: neighbouring
 // lanes trade so that each stores two columns of one token, the even lane of one
 // token and the odd lane of the next.
 __device__ __forceinline__ void store_tokens(const Mx4Params& p, int64_t row0, int count, int64_t col, float bias,
@@ -401,18 +469,49 @@ __device__ __forceinline__ void store_tokens(const Mx4Params& p, int64_t row0, i
     }
 }
 
+// Barrier of the four epilogue warps of one half of the tokens.
+__device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+
+// The tokens FIRST.. of a lane's 32 (as many as a chunk holds) through the
+// half's chunk [token][128 columns], stored as one box at (col0, row0).
+template <typename T, int FIRST>
+__device__ __forceinline__ void stage_chunk(const Mx4Params& p, const CUtensorMap* map, uint8_t* chunk, int half,
+                                            int quad, int lane, int col0, int64_t row0, const float (&v)[32],
+                                            float bias) {
+    const bool storer = quad == 0 && lane == 0;
+    if (storer) bulk_wait_read_all();  // the chunk's last store has read it
+    half_sync(half);
+    T* at = reinterpret_cast<T*>(chunk) + quad * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < kChunkBytes / (128 * (int)sizeof(T)); ++j) {
+        float x = v[FIRST + j] + bias;
+        if (p.relu) x = x < 0.0f ? 0.0f : x;
+        if constexpr (sizeof(T) == 2)
+            at[j * 128] = __float2bfloat16_rn(x);
+        else
+            at[j * 128] = x;
+    }
+    fence_async_shared();
+    half_sync(half);
+    if (storer) {
+        if (row0 < p.m && col0 < p.n) tma_store_2d(map, smem_u32(chunk), col0, (int)row0);
+        bulk_commit();
+    }
+}
+
 __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ CUtensorMap map_t,
                                                                    const __grid_constant__ CUtensorMap map_sw,
                                                                    const __grid_constant__ CUtensorMap map_st,
+                                                                   const __grid_constant__ CUtensorMap map_c,
                                                                    Mx4Params p) {
     constexpr int S = kPairStages;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* smem_w = smem;
     uint8_t* smem_t = smem + S * kWBytes;
     uint8_t* smem_s = smem + 2 * S * kWBytes;  // [stage][W groups 0, 1; tokens 0-127 groups 0, 1; tokens 128-255]
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem_s + S * 6 * kScaleTile);  // leader: both CTAs' bytes of a stage
+    uint8_t* smem_c = smem_s + S * 6 * kScaleTile;  // [token half]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem_c + 2 * kChunkBytes);  // leader: both CTAs' bytes of a stage
     uint64_t* empty = full + S;   // each CTA: stage read by the MMAs
     uint64_t* tfull = empty + S;  // each CTA: accumulator complete
     uint64_t* tempty = tfull + 1; // leader: accumulator drawn by both CTAs' epilogues
@@ -441,6 +540,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         prefetch_tmap(&map_t);
         prefetch_tmap(&map_sw);
         prefetch_tmap(&map_st);
+        if (p.staged) prefetch_tmap(&map_c);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -538,6 +638,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     } else if (warp >= 2) {
         const int quad = warp & 3, half = (warp - 2) >> 2;
         const bool pairs = p.out_bf16 && (p.ldc & 1) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 3) == 0 && (p.n & 1) == 0;
+        uint8_t* chunk = smem_c + half * kChunkBytes;
         int done = 0;
         bool ok = true;
         for (int t = cluster; t < tiles; t += clusters, ++done) {
@@ -552,7 +653,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             float v[4][32];
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                tmem_ld_32x32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128 + c * 32), v[c]);
+                tmem_ld_nowait(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * 128 + c * 32), v[c]);
+            tmem_ld_wait(v);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), 0));
@@ -561,11 +663,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int64_t row0 = (int64_t)tm * 256 + half * 128 + c * 32;
-                const int count = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
-                store_tokens(p, row0, count, col, bias, pairs, v[c]);
+                if (p.staged) {
+                    const int col0 = tn * 256 + (int)rank * 128;
+                    if (p.out_bf16) {
+                        stage_chunk<__nv_bfloat16, 0>(p, &map_c, chunk, half, quad, lane, col0, row0, v[c], bias);
+                    } else {
+                        stage_chunk<float, 0>(p, &map_c, chunk, half, quad, lane, col0, row0, v[c], bias);
+                        stage_chunk<float, 16>(p, &map_c, chunk, half, quad, lane, col0, row0 + 16, v[c], bias);
+                    }
+                } else {
+                    const int count = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
+                    store_tokens(p, row0, count, col, bias, pairs, v[c]);
+                }
             }
         }
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
+        if (lane == 0) bulk_wait_all();
     }
     __syncwarp();
     __syncthreads();
@@ -653,11 +766,20 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaS
 }
 
 int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaStream_t stream) {
-    CUtensorMap w, t, sw, st;
+    CUtensorMap w, t, sw, st, c;
     RT_TRY(map_codes(&w, b, 128));
     RT_TRY(map_codes(&t, a, 128));
     RT_TRY(map_scales(&sw, b, 1));
     RT_TRY(map_scales(&st, a, 2));
+    const int64_t row = p.ldc * (p.out_bf16 ? 2 : 4);
+    p.staged = row % 16 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
+    c = w;
+    if (p.staged) {
+        const cuuint64_t dims[2] = {(cuuint64_t)p.n, (cuuint64_t)p.m}, strides[1] = {(cuuint64_t)row};
+        const cuuint32_t box[2] = {128, p.out_bf16 ? 32u : 16u};
+        RT_TRY(encode(&c, p.out_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, p.c, dims,
+                      strides, box, CU_TENSOR_MAP_SWIZZLE_NONE));
+    }
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
@@ -674,7 +796,7 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cuda
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_pair_kernel, w, t, sw, st, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_pair_kernel, w, t, sw, st, c, p));
     count_launch(ctx);
     return RT_OK;
 }
