@@ -247,6 +247,217 @@ __global__ void __launch_bounds__(256) backward_kernel(BlockP p, GradP g) {
     }
 }
 
+
+// ------------------------------------------------------- rows in registers
+// Eight elements as they are stored: 16 bytes of bf16, 32 of f32.
+template <typename T>
+struct Raw8 {
+    uint4 u[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> zero8() {
+    Raw8<T> r;
+#pragma unroll
+    for (auto& x : r.u) x = make_uint4(0, 0, 0, 0);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const void* base, int64_t at) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(base) + at);
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = p[i];
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+        const uint32_t w[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(void* base, int64_t at, const float (&v)[8]) {
+    uint4* p = reinterpret_cast<uint4*>(static_cast<T*>(base) + at);
+    uint32_t w[8];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+        p[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+// v = p[at..], or `other` where there is no vector.
+__device__ __forceinline__ void vector8(const float* p, int64_t at, float other, float (&v)[8]) {
+    if (p) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p + at)), b = __ldg(reinterpret_cast<const float4*>(p + at) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = other;
+    }
+}
+
+// Sum over the TPR threads of a row, to each of them, in a fixed order.  `red`
+// holds 2 x 32 floats of the row; `turn` alternates between the halves, so one
+// barrier a sum is enough.  Rows of more than a warp in a CTA of several rows
+// share the CTA's barrier: all rows make the same sums.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red, int& turn) {
+    v = warp_sum(v);
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        float* half = red + turn * 32;
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) half[(threadIdx.x % TPR) >> 5] = v;
+        __syncthreads();
+        v = (threadIdx.x & 31) < W ? half[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+        for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        v = __shfl_sync(0xffffffffu, v, 0);
+    }
+    return v;
+}
+
+// Mean and reciprocal deviation of a row held 8 C elements a thread.
+template <int TPR, int C>
+__device__ __forceinline__ Stat stat_of(const NormP& p, const float (&x)[C][8], const bool (&has)[C], float inv_n,
+                                        float* red, int& turn) {
+    Stat s{0.0f, 1.0f};
+    if (p.kind == RT_NORM_NONE) return s;
+    if (p.kind == RT_NORM_LAYER) {
+        float t = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t += x[c][i];  // zeros where the row has ended
+        s.mu = row_sum<TPR>(t, red, turn) * inv_n;
+    }
+    float t = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+        if (has[c])
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = x[c][i] - s.mu;
+                t += d * d;
+            }
+    s.rho = 1.0f / sqrtf(row_sum<TPR>(t, red, turn) * inv_n + p.eps);
+    return s;
+}
+
+// One pass: a row lies in the registers of TPR threads, 8 neighbouring elements
+// in each of C turns, so y and r are read once, z and h written once and the
+// sums of a norm are taken twice over the same registers (mean, then the centred
+// squares).  HBM-bound: 4 elements moved for each of the row.  Needs 16-byte
+// aligned rows and whole eights (n % 8 = 0); a CTA holds ROWS = max(1, 128 / TPR)
+// rows.
+constexpr int cta_threads(int tpr) { return tpr < 128 ? 128 : tpr; }
+
+template <typename T, int TPR, int C>
+__global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p) {
+    constexpr int ROWS = cta_threads(TPR) / TPR;
+    __shared__ float red_all[ROWS][64];
+    float* red = red_all[threadIdx.x / TPR];
+    int turn = 0;
+    const int t = threadIdx.x % TPR;
+    const int n = (int)p.n;
+    const float inv_n = 1.0f / (float)n;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    const bool live = row < p.m;
+    bool has[C];
+    float z[C][8];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        has[c] = live && (c * TPR + t) * 8 < n;
+        const Raw8<T> raw = has[c] ? load_raw8<T>(p.r, row * p.ldr + (c * TPR + t) * 8) : zero8<T>();
+        unpack8<T>(raw, z[c]);
+    }
+    if (p.y) {
+        float y[C][8];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const Raw8<T> raw = has[c] ? load_raw8<T>(p.y, row * p.ldy + (c * TPR + t) * 8) : zero8<T>();
+            unpack8<T>(raw, y[c]);
+        }
+        const Stat s = stat_of<TPR, C>(p.post, y, has, inv_n, red, turn);
+        const float one = p.gate_mode == GATE_ONE              ? __ldg(static_cast<const float*>(p.gate))
+                          : p.gate_mode == GATE_COLUMN && live ? __ldg(static_cast<const float*>(p.gate) + row * p.ldg)
+                                                               : 1.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (has[c]) {
+                const int j = (c * TPR + t) * 8;
+                float gamma[8], beta[8], gate[8];
+                vector8(p.post.gamma, j, 1.0f, gamma);
+                vector8(p.post.beta, j, 0.0f, beta);
+                if (p.gate_mode == GATE_FULL)
+                    unpack8<T>(load_raw8<T>(p.gate, row * p.ldg + j), gate);
+                else
+                    vector8(p.gate_mode == GATE_ROW ? static_cast<const float*>(p.gate) : nullptr, j, one, gate);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float u = (y[c][i] - s.mu) * s.rho * gamma[i] + beta[i];
+                    z[c][i] += p.scale * gate[i] * u;
+                }
+            }
+    }
+    const Stat s = stat_of<TPR, C>(p.pre, z, has, inv_n, red, turn);
+    const int blocks = (n + 31) / 32, groups = (blocks + 3) / 4;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int j = (c * TPR + t) * 8;
+        if (has[c]) {
+            if (p.z) store8<T>(p.z, row * p.ldz + j, z[c]);
+            float gamma[8], beta[8];
+            vector8(p.pre.gamma, j, 1.0f, gamma);
+            vector8(p.pre.beta, j, 0.0f, beta);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[c][i] = (z[c][i] - s.mu) * s.rho * gamma[i] + beta[i];
+            if (p.h) store8<T>(p.h, row * p.ldh + j, z[c]);
+        }
+        if (p.codes) {
+            // four neighbouring lanes hold a block of 32
+            uint32_t amax = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                z[c][i] = has[c] ? as_stored<T>(z[c][i]) : 0.0f;
+                amax = max(amax, __float_as_uint(z[c][i]) & 0x7fffffffu);
+            }
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const uint32_t byte = mx4::scale_byte(amax);
+            const float inv = mx4::inv_scale(byte);
+            uint32_t code = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) code |= mx4::encode2(z[c][i] * inv, z[c][i + 1] * inv) << (4 * i);
+            if (byte == mx4::kNanScale) code = 0;
+            if (live && j < blocks * 32) *reinterpret_cast<uint32_t*>(p.codes + row * blocks * 16 + (j >> 1)) = code;
+            // the scales of a group's four blocks as one word
+            uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, 4) << 8;
+            word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
+            if (live && (threadIdx.x & 15) == 0 && j < groups * 128)
+                *reinterpret_cast<uint32_t*>(p.scales + mx4::scale_offset(row, j >> 5, groups)) = word;
+        }
+    }
+}
+
 struct ReduceP {
     const float* partials;
     int parts, sums;
@@ -358,6 +569,40 @@ int block_params(const rt_block_args* a, const rt_tensor* r, BlockP* p) {
     return RT_OK;
 }
 
+bool aligned16(const void* p, int64_t ld, size_t es) {
+    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * (int64_t)es)) & 15) == 0;
+}
+
+// Whether the kernels that hold rows in registers apply: whole eights of 16-byte
+// aligned rows, and 16-byte aligned vectors.
+bool rows_aligned(const BlockP& p, size_t es) {
+    return p.n % 8 == 0 && aligned16(p.r, p.ldr, es) && aligned16(p.y, p.ldy, es) && aligned16(p.z, p.ldz, es) &&
+           aligned16(p.h, p.ldh, es) && aligned16(p.post.gamma, 0, 4) && aligned16(p.post.beta, 0, 4) &&
+           aligned16(p.pre.gamma, 0, 4) && aligned16(p.pre.beta, 0, 4) &&
+           (p.gate_mode == GATE_FULL ? aligned16(p.gate, p.ldg, es) : p.gate_mode != GATE_ROW || aligned16(p.gate, 0, 4));
+}
+
+template <typename T, int TPR, int C = 1>
+void launch_forward_rows(const BlockP& p, cudaStream_t st) {
+    constexpr int threads = cta_threads(TPR), rows = threads / TPR;
+    forward_rows_kernel<T, TPR, C><<<(unsigned)((p.m + rows - 1) / rows), threads, 0, st>>>(p);
+}
+
+// Up to 16384 wide: the fewest threads that hold a row eight elements each (the
+// widest rows, sixteen).
+template <typename T>
+bool forward_rows(const BlockP& p, cudaStream_t st) {
+    if (!rows_aligned(p, sizeof(T)) || p.n > 16384 || p.m > INT32_MAX) return false;
+    if (p.n <= 256) launch_forward_rows<T, 32>(p, st);
+    else if (p.n <= 512) launch_forward_rows<T, 64>(p, st);
+    else if (p.n <= 1024) launch_forward_rows<T, 128>(p, st);
+    else if (p.n <= 2048) launch_forward_rows<T, 256>(p, st);
+    else if (p.n <= 4096) launch_forward_rows<T, 512>(p, st);
+    else if (p.n <= 8192) launch_forward_rows<T, 1024>(p, st);
+    else launch_forward_rows<T, 1024, 2>(p, st);
+    return true;
+}
+
 int parts_for(const rt_ctx* ctx, int64_t m) { return (int)std::max<int64_t>(1, std::min<int64_t>(m, ctx->sm_count)); }
 
 }  // namespace
@@ -393,10 +638,11 @@ int rt_block_forward(rt_ctx* ctx, const rt_block_args* a) {
     if (p.m == 0 || p.n == 0) return RT_OK;
     RT_CUDA(cudaSetDevice(ctx->device));
     const int grid = (int)std::min<int64_t>(p.m, (int64_t)ctx->sm_count * 8);
-    if (a->r->dtype == RT_BF16)
-        forward_kernel<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(p);
-    else
-        forward_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
+    if (a->r->dtype == RT_BF16) {
+        if (!forward_rows<__nv_bfloat16>(p, ctx->stream)) forward_kernel<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(p);
+    } else {
+        if (!forward_rows<float>(p, ctx->stream)) forward_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
+    }
     RT_CUDA(cudaGetLastError());
     count_launch(ctx);
     return RT_OK;

@@ -45,15 +45,6 @@ __device__ __forceinline__ uint32_t encode2(float lo, float hi) {
     return r;
 }
 
-// The value of a 4-bit code: sign, two exponent bits, one mantissa bit
-// (exponent 0: 0 or 0.5).
-__device__ __forceinline__ float decode(uint32_t code) {
-    const uint32_t mag = code & 7u;
-    // exponent e > 0: (1 + m/2) 2^(e-1), field 126 + e; e = 0: m/2, field 126 if m
-    const uint32_t bits = mag >= 2 ? ((126u + (mag >> 1)) << 23) | ((mag & 1u) << 22) : (mag ? 126u << 23 : 0u);
-    return __uint_as_float(bits | ((code & 8u) << 28));
-}
-
 // Byte offset of the scale of (row, block) in a matrix of `groups` scale
 // tiles along k.
 __device__ __forceinline__ int64_t scale_offset(int64_t row, int64_t block, int64_t groups) {
