@@ -8,13 +8,14 @@
 //   N^T(d) = rho (a - [layer] mean(a) - x^ mean(a x^)),   a = d gamma
 //   dr = dz + N_pre^T(dh),  du = s g dr,  dy = N_post^T(du)
 //   dgamma_pre = sum_rows dh z^,  dbeta_pre = sum_rows dh
-// and, with w = s dr (times g where the gate differs from row to row), the sums
-// over rows A = sum w y^ and B = sum w give every other vector:
-//   dgamma_post = g A,  dbeta_post = g B,  dgate = gamma_post A + beta_post B
+// and, with w = dr (times g where the gate differs from row to row), the sums over
+// rows A = sum w y^ and B = sum w give every other vector:
+//   dgamma_post = s g A,  dbeta_post = s g B,  dgate = s (gamma_post A + beta_post B)
 // (g = 1 where w holds it; the [1,1] gate's gradient sums dgate over columns).
 #include <algorithm>
 
 #include "mx4.cuh"
+#include "tc_common.cuh"
 
 namespace rt {
 namespace {
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(256) backward_kernel(BlockP p, GradP g) {
                 if (g.dy) st<T>(g.dy, row * g.lddy + j, (b - b0 - hat * b1) * sy.rho);
                 if (g.dgate && p.gate_mode == GATE_FULL)
                     st<T>(g.dgate, row * g.lddg + j, dt * (hat * gamma_at(p.post, j) + beta_at(p.post, j)));
-                const float w = p.gate_mode >= GATE_COLUMN ? dt * gt : dt;
+                const float w = p.gate_mode >= GATE_COLUMN ? dr * gt : dr;
                 if (g.sums & 1) acc[j] += w * hat;
                 if (g.sums & 2) acc[n + j] += w;
             }
@@ -362,6 +363,36 @@ __device__ __forceinline__ Stat stat_of(const NormP& p, const float (&x)[C][8], 
     return s;
 }
 
+// Eight elements of h, stored and in 4 bits; called by whole warps, `has` where
+// the eight lie in the row (which `live` says exists).
+template <typename T>
+__device__ __forceinline__ void store_h(const BlockP& p, int64_t row, int j, bool live, bool has, float (&h)[8]) {
+    if (p.h && has) store8<T>(p.h, row * p.ldh + j, h);
+    if (!p.codes) return;
+    const int blocks = (int)((p.n + 31) / 32), groups = (blocks + 3) / 4;
+    // four neighbouring lanes hold a block of 32
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        h[i] = has ? as_stored<T>(h[i]) : 0.0f;
+        amax = max(amax, __float_as_uint(h[i]) & 0x7fffffffu);
+    }
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t byte = mx4::scale_byte(amax);
+    const float inv = mx4::inv_scale(byte);
+    uint32_t code = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) code |= mx4::encode2(h[i] * inv, h[i + 1] * inv) << (4 * i);
+    if (byte == mx4::kNanScale) code = 0;
+    if (live && j < blocks * 32) *reinterpret_cast<uint32_t*>(p.codes + row * blocks * 16 + (j >> 1)) = code;
+    // the scales of a group's four blocks as one word
+    uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, 4) << 8;
+    word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
+    if (live && (threadIdx.x & 15) == 0 && j < groups * 128)
+        *reinterpret_cast<uint32_t*>(p.scales + mx4::scale_offset(row, j >> 5, groups)) = word;
+}
+
 // One pass: a row lies in the registers of TPR threads, 8 neighbouring elements
 // in each of C turns, so y and r are read once, z and h written once and the
 // sums of a norm are taken twice over the same registers (mean, then the centred
@@ -419,7 +450,6 @@ __global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p
             }
     }
     const Stat s = stat_of<TPR, C>(p.pre, z, has, inv_n, red, turn);
-    const int blocks = (n + 31) / 32, groups = (blocks + 3) / 4;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int j = (c * TPR + t) * 8;
@@ -430,31 +460,647 @@ __global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p
             vector8(p.pre.beta, j, 0.0f, beta);
 #pragma unroll
             for (int i = 0; i < 8; ++i) z[c][i] = (z[c][i] - s.mu) * s.rho * gamma[i] + beta[i];
-            if (p.h) store8<T>(p.h, row * p.ldh + j, z[c]);
         }
-        if (p.codes) {
-            // four neighbouring lanes hold a block of 32
-            uint32_t amax = 0;
+        store_h<T>(p, row, j, live, has[c], z[c]);
+    }
+}
+
+// ------------------------------------------------------ rows through a ring
+// For many rows: one CTA of 1024 threads to an SM, its groups of TPR threads each
+// take a row at a time.  The rows arrive by bulk copies into a ring of slots, so
+// the next rows are on their way while this one is summed, however few registers
+// that leaves; the vectors (gamma, beta and a gate of one row, folded together
+// where they meet) lie in shared memory once, in f32.
+constexpr int kRingThreads = 1024;
+constexpr int kRingSmem = 226 * 1024;
+constexpr int kRingScratch = 26 * 1024;  // sums (24 KB for 32 groups) and barriers
+
+struct RingP {
+    int depth;         // slots of a group
+    int slot_bytes;    // the row of each tensor
+    int vectors;       // f32 vectors in shared memory
+    int* err;
+};
+
+template <int TPR>
+struct Group {
+    static constexpr int COUNT = kRingThreads / TPR;
+    int index, t;    // of the group in its CTA, of the thread in its group
+    float* red;      // [2][3][32]
+    int turn = 0;
+
+    __device__ __forceinline__ void sync() const {
+        if constexpr (TPR == 32)
+            __syncwarp();
+        else if constexpr (TPR == kRingThreads)
+            __syncthreads();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "n"(TPR) : "memory");
+    }
+    // Sums over the group, to every thread, in a fixed order; one barrier.
+    template <int K>
+    __device__ __forceinline__ void sum(float (&v)[K]) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                z[c][i] = has[c] ? as_stored<T>(z[c][i]) : 0.0f;
-                amax = max(amax, __float_as_uint(z[c][i]) & 0x7fffffffu);
+        for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+        if constexpr (TPR == 32) {
+            __syncwarp();
+        } else {
+            constexpr int W = TPR / 32;
+            const int lane = threadIdx.x & 31;
+            float* half = red + turn * 96;
+            turn ^= 1;
+            if (lane == 0)
+#pragma unroll
+                for (int k = 0; k < K; ++k) half[k * 32 + (t >> 5)] = v[k];
+            sync();
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float s = lane < W ? half[k * 32 + lane] : 0.0f;
+#pragma unroll
+                for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                v[k] = __shfl_sync(0xffffffffu, s, 0);
             }
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const uint32_t byte = mx4::scale_byte(amax);
-            const float inv = mx4::inv_scale(byte);
-            uint32_t code = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) code |= mx4::encode2(z[c][i] * inv, z[c][i + 1] * inv) << (4 * i);
-            if (byte == mx4::kNanScale) code = 0;
-            if (live && j < blocks * 32) *reinterpret_cast<uint32_t*>(p.codes + row * blocks * 16 + (j >> 1)) = code;
-            // the scales of a group's four blocks as one word
-            uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, 4) << 8;
-            word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
-            if (live && (threadIdx.x & 15) == 0 && j < groups * 128)
-                *reinterpret_cast<uint32_t*>(p.scales + mx4::scale_offset(row, j >> 5, groups)) = word;
         }
+    }
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// Shared memory of a ring kernel: vectors, slots, sums, barriers.
+struct RingSmem {
+    float* vec;
+    uint8_t* slots;
+    float* red;
+    uint64_t* full;
+    volatile int* abort_flag;
+};
+__device__ __forceinline__ RingSmem ring_smem(uint8_t* smem, const RingP& r, int n, int groups) {
+    RingSmem s;
+    s.vec = reinterpret_cast<float*>(smem);
+    s.slots = smem + (size_t)r.vectors * n * 4;
+    s.red = reinterpret_cast<float*>(s.slots + (size_t)groups * r.depth * r.slot_bytes);
+    s.full = reinterpret_cast<uint64_t*>(s.red + groups * 192);  // a group's sums: [2][3][32]
+    s.abort_flag = reinterpret_cast<volatile int*>(s.full + groups * r.depth);
+    return s;
+}
+
+// Pairs of f32 in one 64-bit register and Blackwell's packed arithmetic on them:
+// the ring kernels would otherwise be bound by instructions, not by HBM.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ f2 splat2(float a) { return pack2(a, a); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float both(f2 a) {
+    const float2 x = unpack2(a);
+    return x.x + x.y;
+}
+
+// Eight elements of a slot's row, of a vector in shared memory.
+template <typename T>
+__device__ __forceinline__ void slot8(const uint8_t* row, int j, f2 (&v)[4]) {
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(row) + j);
+    if constexpr (sizeof(T) == 2) {
+        const uint4 u = p[0];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    } else {
+        const ulonglong2 a = reinterpret_cast<const ulonglong2*>(p)[0], b = reinterpret_cast<const ulonglong2*>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
+}
+__device__ __forceinline__ void vec8(const float* p, int j, f2 (&v)[4]) {
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(p + j), b = *reinterpret_cast<const ulonglong2*>(p + j + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+__device__ __forceinline__ void floats8(const f2 (&v)[4], float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = unpack2(v[i]);
+        x[2 * i] = a.x;
+        x[2 * i + 1] = a.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(void* base, int64_t at, const f2 (&v)[4]) {
+    float x[8];
+    floats8(v, x);
+    store8<T>(base, at, x);
+}
+
+// The gate where it is the same for every row (1 where it is not).
+__device__ __forceinline__ float shared_gate(const BlockP& p, int j) {
+    return p.gate_mode == GATE_ONE   ? __ldg(static_cast<const float*>(p.gate))
+           : p.gate_mode == GATE_ROW ? __ldg(static_cast<const float*>(p.gate) + j)
+                                     : 1.0f;
+}
+
+// Forward.  Slots hold r and y; vectors P = s g gamma_post, Q = s g beta_post (g
+// where all rows share it), gamma_pre, beta_pre, those that there are (mask 1 2 4
+// 8).  8192 x 8192 bf16: see the table of measurements in the design notes.
+// FULL: with layer norms, betas and gates that rows do not share; else RMS norms
+// and shared gates alone.
+template <typename T, int TPR, int C, bool FULL>
+__global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p, RingP r, int mask) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    using G = Group<TPR>;
+    const int n = (int)p.n;
+    const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
+    G g;
+    g.index = threadIdx.x / TPR;
+    g.t = threadIdx.x % TPR;
+    g.red = sm.red + g.index * 192;
+    uint8_t* slots = sm.slots + (size_t)g.index * r.depth * r.slot_bytes;
+    const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
+    const uint32_t row_bytes = (uint32_t)n * sizeof(T);
+    const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < G::COUNT * r.depth; ++i) tc::mbar_init(tc::smem_u32(sm.full + i), 1);
+        *sm.abort_flag = 0;
+        tc::fence_barrier_init();
+    }
+    float *vp = sm.vec, *vq = vp + (mask & 1 ? n : 0), *v2 = vq + (mask & 2 ? n : 0), *vb = v2 + (mask & 4 ? n : 0);
+    for (int j = threadIdx.x; j < n; j += kRingThreads) {
+        const float sg = p.scale * shared_gate(p, j);
+        if (mask & 1) vp[j] = sg * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
+        if (mask & 2) vq[j] = sg * __ldg(p.post.beta + j);
+        if (mask & 4) v2[j] = __ldg(p.pre.gamma + j);
+        if (mask & 8) vb[j] = __ldg(p.pre.beta + j);
+    }
+    __syncthreads();
+    auto issue = [&](int64_t row, int slot) {
+        const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * r.slot_bytes);
+        tc::mbar_expect_tx(bar, (uint32_t)r.slot_bytes);
+        bulk_load(dst, static_cast<const T*>(p.r) + row * p.ldr, row_bytes, bar);
+        if (p.y) bulk_load(dst + row_bytes, static_cast<const T*>(p.y) + row * p.ldy, row_bytes, bar);
+    };
+    if (g.t == 0)
+        for (int d = 0; d < r.depth && first + d * step < p.m; ++d) issue(first + d * step, d);
+    const float inv_n = 1.0f / (float)n;
+    int slot = 0;
+    uint32_t phase = 0;
+    bool has[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) has[c] = (c * TPR + g.t) * 8 < n;
+    for (int64_t row = first; row < p.m; row += step) {
+        if (!tc::mbar_wait(full + slot * 8, phase, sm.abort_flag)) {
+            *sm.abort_flag = 1;
+            tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+        }
+        const uint8_t* at = slots + (size_t)slot * r.slot_bytes;
+        f2 z[C][4];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[c][i] = 0;
+            if (has[c]) slot8<T>(at, (c * TPR + g.t) * 8, z[c]);
+        }
+        if (p.y) {
+            const uint8_t* ay = at + row_bytes;
+            Stat s{0.0f, 1.0f};
+            if (FULL && p.post.kind == RT_NORM_LAYER) {
+                f2 v2x = 0;
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    if (has[c]) {
+                        f2 y[4];
+                        slot8<T>(ay, (c * TPR + g.t) * 8, y);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v2x = add2(v2x, y[i]);
+                    }
+                float v[1] = {both(v2x)};
+                g.sum(v);
+                s.mu = v[0] * inv_n;
+            }
+            const f2 less_mu = splat2(-s.mu);
+            if (p.post.kind != RT_NORM_NONE) {
+                f2 v2x = 0;
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    if (has[c]) {
+                        f2 y[4];
+                        slot8<T>(ay, (c * TPR + g.t) * 8, y);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (FULL) y[i] = add2(y[i], less_mu);
+                            v2x = fma2(y[i], y[i], v2x);
+                        }
+                    }
+                float v[1] = {both(v2x)};
+                g.sum(v);
+                s.rho = 1.0f / sqrtf(v[0] * inv_n + p.post.eps);
+            }
+            const f2 rho = splat2(mask & 1 ? s.rho : s.rho * p.scale);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (has[c]) {
+                    const int j = (c * TPR + g.t) * 8;
+                    f2 y[4], w[4];
+                    slot8<T>(ay, j, y);
+                    if (FULL)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = add2(y[i], less_mu);
+                    if (mask & 1) {
+                        vec8(vp, j, w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], w[i]);
+                    }
+                    if (!FULL) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[c][i] = fma2(y[i], rho, z[c][i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], rho);
+                        if (mask & 2) {
+                            vec8(vq, j, w);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[i] = add2(y[i], w[i]);
+                        }
+                        if (p.gate_mode == GATE_COLUMN) {
+                            const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], one);
+                        } else if (p.gate_mode == GATE_FULL) {
+                            slot8<T>(reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.gate) + row * p.ldg), j, w);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], w[i]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) z[c][i] = add2(z[c][i], y[i]);
+                    }
+                }
+        }
+        // z is complete: its slot is free once the whole group is past the next barrier
+        Stat s{0.0f, 1.0f};
+        bool freed = false;
+        auto refill = [&] {
+            freed = true;
+            if (g.t == 0 && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
+        };
+        if (FULL && p.pre.kind == RT_NORM_LAYER) {
+            f2 v2x = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v2x = add2(v2x, z[c][i]);
+            float v[1] = {both(v2x)};
+            g.sum(v);
+            refill();
+            s.mu = v[0] * inv_n;
+        }
+        const f2 less_mu = splat2(-s.mu);
+        if (p.pre.kind != RT_NORM_NONE) {
+            f2 v2x = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (has[c])
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f2 d = FULL ? add2(z[c][i], less_mu) : z[c][i];
+                        v2x = fma2(d, d, v2x);
+                    }
+            float v[1] = {both(v2x)};
+            g.sum(v);
+            if (!freed) refill();
+            s.rho = 1.0f / sqrtf(v[0] * inv_n + p.pre.eps);
+        }
+        if (!freed) {
+            g.sync();
+            refill();
+        }
+        const f2 rho = splat2(s.rho);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (c * TPR + g.t) * 8;
+            if (has[c]) {
+                if (p.z) store8<T>(p.z, row * p.ldz + j, z[c]);
+                f2 w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[c][i] = mul2(FULL ? add2(z[c][i], less_mu) : z[c][i], rho);
+                if (mask & 4) {
+                    vec8(v2, j, w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[c][i] = mul2(z[c][i], w[i]);
+                }
+                if (FULL && (mask & 8)) {
+                    vec8(vb, j, w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[c][i] = add2(z[c][i], w[i]);
+                }
+            }
+            float h[8];
+            floats8(z[c], h);
+            store_h<T>(p, row, j, true, has[c], h);
+        }
+        if (++slot == r.depth) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+}
+
+// Backward.  Slots hold z and those of y, dz and dh that there are; vectors
+// gamma_pre, P = s gamma_post (times g where all rows share it) and, for the
+// gradient of a gate that rows do not share, s beta_post (mask 1 2 4).  A thread
+// keeps the sums over rows of its eight columns in registers (FULL: those of the
+// betas too); the groups' sums are joined in shared memory in order, one partial
+// a CTA, and column_kernel adds the partials in order.
+template <typename T, int TPR, bool FULL>
+__global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(BlockP p, GradP q, RingP r, int mask) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    using G = Group<TPR>;
+    const int n = (int)p.n;
+    const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
+    G g;
+    g.index = threadIdx.x / TPR;
+    g.t = threadIdx.x % TPR;
+    g.red = sm.red + g.index * 192;
+    uint8_t* slots = sm.slots + (size_t)g.index * r.depth * r.slot_bytes;
+    const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
+    const uint32_t row_bytes = (uint32_t)n * sizeof(T);
+    const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
+    const bool own_gate = FULL && (p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < G::COUNT * r.depth; ++i) tc::mbar_init(tc::smem_u32(sm.full + i), 1);
+        *sm.abort_flag = 0;
+        tc::fence_barrier_init();
+    }
+    float *v2 = sm.vec, *vp = v2 + (mask & 1 ? n : 0), *vb = vp + (mask & 2 ? n : 0);
+    for (int j = threadIdx.x; j < n; j += kRingThreads) {
+        if (mask & 1) v2[j] = __ldg(p.pre.gamma + j);
+        if (mask & 2) vp[j] = p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
+        if (mask & 4) vb[j] = p.scale * __ldg(p.post.beta + j);
+    }
+    __syncthreads();
+    // the slot's rows: z, then y, dz, dh
+    const uint32_t at_y = row_bytes, at_dz = at_y + (p.y ? row_bytes : 0), at_dh = at_dz + (q.dz ? row_bytes : 0);
+    auto issue = [&](int64_t row, int slot) {
+        const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * r.slot_bytes);
+        tc::mbar_expect_tx(bar, (uint32_t)r.slot_bytes);
+        bulk_load(dst, static_cast<const T*>(p.z) + row * p.ldz, row_bytes, bar);
+        if (p.y) bulk_load(dst + at_y, static_cast<const T*>(p.y) + row * p.ldy, row_bytes, bar);
+        if (q.dz) bulk_load(dst + at_dz, static_cast<const T*>(q.dz) + row * q.lddz, row_bytes, bar);
+        if (q.dh) bulk_load(dst + at_dh, static_cast<const T*>(q.dh) + row * q.lddh, row_bytes, bar);
+    };
+    if (g.t == 0)
+        for (int d = 0; d < r.depth && first + d * step < p.m; ++d) issue(first + d * step, d);
+    const float inv_n = 1.0f / (float)n;
+    const int j = g.t * 8;
+    const bool has = j < n;
+    f2 sum_a[4], sum_b[FULL ? 4 : 1], sum_c[4], sum_d[FULL ? 4 : 1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sum_a[i] = sum_c[i] = 0;
+        if constexpr (FULL) sum_b[i] = sum_d[i] = 0;
+    }
+    int slot = 0;
+    uint32_t phase = 0;
+    const bool back = q.dh && p.pre.kind != RT_NORM_NONE;
+    for (int64_t row = first; row < p.m; row += step) {
+        if (!tc::mbar_wait(full + slot * 8, phase, sm.abort_flag)) {
+            *sm.abort_flag = 1;
+            tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+        }
+        const uint8_t* at = slots + (size_t)slot * r.slot_bytes;
+        // sums of both norms: means first where there is a layer norm, then the
+        // centred squares and a (z - mu)
+        Stat sz{0.0f, 1.0f}, sy{0.0f, 1.0f};
+        float a0 = 0.0f, a1 = 0.0f;
+        if (FULL && (p.pre.kind == RT_NORM_LAYER || p.post.kind == RT_NORM_LAYER)) {
+            f2 sums[3] = {0, 0, 0};
+            if (has) {
+                f2 x[4], w[4];
+                if (p.pre.kind == RT_NORM_LAYER) {
+                    slot8<T>(at, j, x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sums[0] = add2(sums[0], x[i]);
+                    if (back) {
+                        slot8<T>(at + at_dh, j, x);
+                        if (mask & 1) {
+                            vec8(v2, j, w);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], w[i]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sums[1] = add2(sums[1], x[i]);
+                    }
+                }
+                if (p.post.kind == RT_NORM_LAYER) {
+                    slot8<T>(at + at_y, j, x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sums[2] = add2(sums[2], x[i]);
+                }
+            }
+            float v[3] = {both(sums[0]), both(sums[1]), both(sums[2])};
+            g.sum(v);
+            sz.mu = v[0] * inv_n;
+            a0 = v[1] * inv_n;
+            sy.mu = v[2] * inv_n;
+        }
+        const f2 less_z = splat2(-sz.mu), less_y = splat2(-sy.mu);
+        if (p.pre.kind != RT_NORM_NONE || p.post.kind != RT_NORM_NONE) {
+            f2 sums[3] = {0, 0, 0};
+            if (has) {
+                f2 x[4];
+                if (p.pre.kind != RT_NORM_NONE) {
+                    slot8<T>(at, j, x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (FULL) x[i] = add2(x[i], less_z);
+                        sums[0] = fma2(x[i], x[i], sums[0]);
+                    }
+                    if (back) {
+                        f2 d[4], w[4];
+                        slot8<T>(at + at_dh, j, d);
+                        if (mask & 1) {
+                            vec8(v2, j, w);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) d[i] = mul2(d[i], w[i]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sums[1] = fma2(d[i], x[i], sums[1]);
+                    }
+                }
+                if (p.post.kind != RT_NORM_NONE) {
+                    slot8<T>(at + at_y, j, x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (FULL) x[i] = add2(x[i], less_y);
+                        sums[2] = fma2(x[i], x[i], sums[2]);
+                    }
+                }
+            }
+            float v[3] = {both(sums[0]), both(sums[1]), both(sums[2])};
+            g.sum(v);
+            if (p.pre.kind != RT_NORM_NONE) sz.rho = 1.0f / sqrtf(v[0] * inv_n + p.pre.eps);
+            if (p.post.kind != RT_NORM_NONE) sy.rho = 1.0f / sqrtf(v[2] * inv_n + p.post.eps);
+            a1 = v[1] * inv_n * sz.rho;  // mean of a z^
+        }
+        // dr, and the sums over rows of dh
+        f2 dr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dr[i] = 0;
+        if (has) {
+            if (q.dz) slot8<T>(at + at_dz, j, dr);
+            if (q.dh) {
+                f2 d[4], hat[4], w[4];
+                const f2 rho = splat2(sz.rho), less_a0 = splat2(-a0), less_a1 = splat2(-a1);
+                slot8<T>(at + at_dh, j, d);
+                slot8<T>(at, j, hat);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    hat[i] = mul2(FULL ? add2(hat[i], less_z) : hat[i], rho);
+                    sum_c[i] = fma2(d[i], hat[i], sum_c[i]);
+                    if constexpr (FULL) sum_d[i] = add2(sum_d[i], d[i]);
+                }
+                if (mask & 1) {
+                    vec8(v2, j, w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) d[i] = mul2(d[i], w[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (FULL) d[i] = add2(d[i], less_a0);
+                    dr[i] = fma2(fma2(hat[i], less_a1, d[i]), rho, dr[i]);
+                }
+            }
+            if (q.dr) store8<T>(q.dr, row * q.lddr + j, dr);
+        }
+        if (p.y) {
+            f2 sums[3] = {0, 0, 0};
+            f2 b[4], hat[4];
+            if (has) {
+                f2 w[4];
+                const f2 rho = splat2(sy.rho);
+                slot8<T>(at + at_y, j, hat);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) hat[i] = mul2(FULL ? add2(hat[i], less_y) : hat[i], rho);
+                if (mask & 2) {
+                    vec8(vp, j, w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = splat2(p.scale);
+                }
+                if (own_gate) {
+                    // s u dr is the gate's gradient, and g dr takes the place of dr
+                    f2 u[4], gate[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) u[i] = mul2(hat[i], w[i]);
+                    if (mask & 4) {
+                        vec8(vb, j, gate);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) u[i] = add2(u[i], gate[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u[i] = mul2(u[i], dr[i]);
+                        sums[2] = add2(sums[2], u[i]);
+                    }
+                    if (p.gate_mode == GATE_FULL) {
+                        slot8<T>(reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.gate) + row * p.ldg), j, gate);
+                        if (q.dgate) store8<T>(q.dgate, row * q.lddg + j, u);
+                    } else {
+                        const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) gate[i] = one;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dr[i] = mul2(dr[i], gate[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum_a[i] = fma2(dr[i], hat[i], sum_a[i]);
+                    if constexpr (FULL) sum_b[i] = add2(sum_b[i], dr[i]);
+                    b[i] = mul2(dr[i], w[i]);
+                    if (FULL) sums[0] = add2(sums[0], b[i]);
+                    sums[1] = fma2(b[i], hat[i], sums[1]);
+                }
+            }
+            float v[3] = {0.0f, both(sums[1]), 0.0f};
+            if constexpr (FULL) {
+                v[0] = both(sums[0]);
+                v[2] = both(sums[2]);
+                g.sum(v);
+                if (g.t == 0 && q.dgate && p.gate_mode == GATE_COLUMN) static_cast<float*>(q.dgate)[row * q.lddg] = v[2];
+            } else {
+                float one[1] = {v[1]};
+                g.sum(one);
+                v[1] = one[0];
+            }
+            if (has && q.dy) {
+                const f2 rho = splat2(sy.rho), b0 = splat2(p.post.kind == RT_NORM_LAYER ? -v[0] * inv_n : 0.0f);
+                const f2 b1 = splat2(p.post.kind != RT_NORM_NONE ? -v[1] * inv_n : 0.0f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (FULL) b[i] = add2(b[i], b0);
+                    b[i] = mul2(fma2(hat[i], b1, b[i]), rho);
+                }
+                store8<T>(q.dy, row * q.lddy + j, b);
+            }
+        } else {
+            g.sync();
+        }
+        // every thread of the group has read the slot: all of it before the last barrier
+        if (g.t == 0 && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
+        if (++slot == r.depth) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+    if (!q.partials) return;
+    // the groups' sums, added in order; the slots are all read
+    __syncthreads();
+    float* acc = reinterpret_cast<float*>(sm.slots);  // [n]
+    auto join = [&](int which, const f2* sums) {
+        if (!((q.sums >> which) & 1)) return;
+        for (int k = 0; k < G::COUNT; ++k) {
+            if (g.index == k && has) {
+                f2* a = reinterpret_cast<f2*>(acc + j);
+                f2 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[i]) : sums[i];
+                if (k == G::COUNT - 1)
+                    a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * n + j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = x[i];
+            }
+            if (G::COUNT > 1) __syncthreads();
+        }
+    };
+    join(0, sum_a);
+    join(2, sum_c);
+    if constexpr (FULL) {
+        join(1, sum_b);
+        join(3, sum_d);
     }
 }
 
@@ -464,6 +1110,7 @@ struct ReduceP {
     int64_t n;
     int gate_mode;
     const float* gate;
+    float scale;
     const float *gamma, *beta;  // of the norm after the block
     float *dgamma_post, *dbeta_post, *dgamma_pre, *dbeta_pre, *dgate;
     float* gate_row;  // [n]: a [1,1] gate's gradient by column
@@ -478,6 +1125,8 @@ __global__ void __launch_bounds__(256) column_kernel(ReduceP p) {
 #pragma unroll
         for (int v = 0; v < 4; ++v)
             if ((p.sums >> v) & 1) s[v] += p.partials[((int64_t)i * 4 + v) * p.n + j];
+    s[0] *= p.scale;
+    s[1] *= p.scale;
     const float g = p.gate_mode == GATE_ONE ? p.gate[0] : p.gate_mode == GATE_ROW ? p.gate[j] : 1.0f;
     if (p.dgamma_post) p.dgamma_post[j] = s[0] * g;
     if (p.dbeta_post) p.dbeta_post[j] = s[1] * g;
@@ -588,6 +1237,84 @@ void launch_forward_rows(const BlockP& p, cudaStream_t st) {
     forward_rows_kernel<T, TPR, C><<<(unsigned)((p.m + rows - 1) / rows), threads, 0, st>>>(p);
 }
 
+// Fills in the ring's shape; false where not even one slot a group fits.
+bool plan_ring(RingP* r, int64_t n, int groups, int tensors, size_t es, int vectors) {
+    r->slot_bytes = (int)(tensors * n * (int64_t)es);
+    r->vectors = vectors;
+    const int64_t room = kRingSmem - kRingScratch - (int64_t)vectors * n * 4;
+    r->depth = (int)std::min<int64_t>(4, room / ((int64_t)groups * r->slot_bytes));
+    return r->depth >= 1;
+}
+
+template <typename T, int TPR, int C>
+int launch_forward_ring(rt_ctx* ctx, const BlockP& p, RingP r, int mask, cudaStream_t st) {
+    const int64_t ctas = std::min<int64_t>(ctx->sm_count, (p.m + Group<TPR>::COUNT - 1) / Group<TPR>::COUNT);
+    const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (mask & 10) ||
+                      p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
+    auto* kernel = full ? forward_ring_kernel<T, TPR, C, true> : forward_ring_kernel<T, TPR, C, false>;
+    RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+    kernel<<<(unsigned)ctas, kRingThreads, kRingSmem, st>>>(p, r, mask);
+    return RT_OK;
+}
+
+// The ring's kernel where there are rows enough for it: true if it was launched.
+template <typename T>
+int forward_ring(rt_ctx* ctx, const BlockP& p, cudaStream_t st, bool* done) {
+    *done = false;
+    if (!rows_aligned(p, sizeof(T)) || p.n > 8192) return RT_OK;
+    const bool shared = p.gate_mode == GATE_ONE || p.gate_mode == GATE_ROW;
+    const int mask = (p.y && (p.post.gamma || shared) ? 1 : 0) | (p.post.beta ? 2 : 0) | (p.pre.gamma ? 4 : 0) |
+                     (p.pre.beta ? 8 : 0);
+    const int tpr = p.n <= 512 ? 32 : p.n <= 2048 ? 128 : p.n <= 4096 ? 256 : 512;
+    if (p.m < (int64_t)2 * ctx->sm_count * (kRingThreads / tpr)) return RT_OK;
+    RingP r{};
+    r.err = ctx->dev_err;
+    if (!plan_ring(&r, p.n, kRingThreads / tpr, p.y ? 2 : 1, sizeof(T), __builtin_popcount(mask))) return RT_OK;
+    *done = true;
+    if (tpr == 32) return launch_forward_ring<T, 32, 2>(ctx, p, r, mask, st);
+    if (tpr == 128) return launch_forward_ring<T, 128, 2>(ctx, p, r, mask, st);
+    if (tpr == 256) return launch_forward_ring<T, 256, 2>(ctx, p, r, mask, st);
+    return launch_forward_ring<T, 512, 2>(ctx, p, r, mask, st);
+}
+
+template <typename T, int TPR>
+int launch_backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, const RingP& r, int mask, int ctas, cudaStream_t st) {
+    const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
+                      p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
+    auto* kernel = full ? backward_ring_kernel<T, TPR, true> : backward_ring_kernel<T, TPR, false>;
+    RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+    kernel<<<(unsigned)ctas, kRingThreads, kRingSmem, st>>>(p, q, r, mask);
+    return RT_OK;
+}
+
+// The backward pass through the ring where the rows are aligned and fit; *parts
+// is then the number of partials.
+template <typename T>
+int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st, int* parts, bool* done) {
+    *done = false;
+    const size_t es = sizeof(T);
+    if (!rows_aligned(p, es) || p.n > 8192 || p.m == 0 || !aligned16(q.dz, q.lddz, es) || !aligned16(q.dh, q.lddh, es) ||
+        !aligned16(q.dr, q.lddr, es) || !aligned16(q.dy, q.lddy, es) || !aligned16(q.partials, 0, 4) ||
+        (p.gate_mode == GATE_FULL && !aligned16(q.dgate, q.lddg, es)))
+        return RT_OK;
+    const bool shared = p.gate_mode == GATE_ONE || p.gate_mode == GATE_ROW;
+    const int mask = (p.pre.gamma ? 1 : 0) | (p.post.gamma || (p.y && shared) ? 2 : 0) |
+                     (p.post.beta && q.dgate && !shared ? 4 : 0);
+    const int tpr = p.n <= 256 ? 32 : p.n <= 1024 ? 128 : p.n <= 2048 ? 256 : p.n <= 4096 ? 512 : 1024;
+    const int groups = kRingThreads / tpr;
+    RingP r{};
+    r.err = ctx->dev_err;
+    if (!plan_ring(&r, p.n, groups, 1 + (p.y ? 1 : 0) + (q.dz ? 1 : 0) + (q.dh ? 1 : 0), es, __builtin_popcount(mask)))
+        return RT_OK;
+    *done = true;
+    *parts = (int)std::min<int64_t>(ctx->sm_count, (p.m + groups - 1) / groups);
+    if (tpr == 32) return launch_backward_ring<T, 32>(ctx, p, q, r, mask, *parts, st);
+    if (tpr == 128) return launch_backward_ring<T, 128>(ctx, p, q, r, mask, *parts, st);
+    if (tpr == 256) return launch_backward_ring<T, 256>(ctx, p, q, r, mask, *parts, st);
+    if (tpr == 512) return launch_backward_ring<T, 512>(ctx, p, q, r, mask, *parts, st);
+    return launch_backward_ring<T, 1024>(ctx, p, q, r, mask, *parts, st);
+}
+
 // Up to 16384 wide: the fewest threads that hold a row eight elements each (the
 // widest rows, sixteen).
 template <typename T>
@@ -638,7 +1365,11 @@ int rt_block_forward(rt_ctx* ctx, const rt_block_args* a) {
     if (p.m == 0 || p.n == 0) return RT_OK;
     RT_CUDA(cudaSetDevice(ctx->device));
     const int grid = (int)std::min<int64_t>(p.m, (int64_t)ctx->sm_count * 8);
-    if (a->r->dtype == RT_BF16) {
+    bool done = false;
+    RT_TRY(a->r->dtype == RT_BF16 ? forward_ring<__nv_bfloat16>(ctx, p, ctx->stream, &done)
+                                  : forward_ring<float>(ctx, p, ctx->stream, &done));
+    if (done) {
+    } else if (a->r->dtype == RT_BF16) {
         if (!forward_rows<__nv_bfloat16>(p, ctx->stream)) forward_kernel<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(p);
     } else {
         if (!forward_rows<float>(p, ctx->stream)) forward_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
@@ -717,7 +1448,7 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     q.sums = (g->dgamma_post || gate_sums ? 1 : 0) | (g->dbeta_post || (gate_sums && p.post.beta) ? 2 : 0) |
              (g->dgamma_pre ? 4 : 0) | (g->dbeta_pre ? 8 : 0);
     if (p.n == 0) return RT_OK;
-    const int parts = parts_for(ctx, p.m);
+    int parts = parts_for(ctx, p.m);
     if (q.sums) {
         RT_CHECK(g->work && g->work->dtype == RT_F32 && g->work->rows == 1 &&
                      g->work->cols >= rt_block_backward_workspace(ctx, p.m, p.n),
@@ -726,8 +1457,12 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
         q.partials = static_cast<float*>(g->work->ptr);
     }
     RT_CUDA(cudaSetDevice(ctx->device));
+    bool done = false;
+    RT_TRY(z->dtype == RT_BF16 ? backward_ring<__nv_bfloat16>(ctx, p, q, ctx->stream, &parts, &done)
+                               : backward_ring<float>(ctx, p, q, ctx->stream, &parts, &done));
     // without rows the sums over rows are zero: the partials of one CTA
-    if (z->dtype == RT_BF16)
+    if (done) {
+    } else if (z->dtype == RT_BF16)
         backward_kernel<__nv_bfloat16><<<parts, 256, 0, ctx->stream>>>(p, q);
     else
         backward_kernel<float><<<parts, 256, 0, ctx->stream>>>(p, q);
@@ -740,9 +1475,10 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     c.n = p.n;
     c.gate_mode = p.gate_mode;
     c.gate = static_cast<const float*>(p.gate);
+    c.scale = p.scale;
     c.gamma = p.post.gamma;
     c.beta = p.post.beta;
-    if (gate_sums && p.gate_mode == GATE_ONE) c.gate_row = q.partials + (int64_t)parts * 4 * p.n;
+    if (gate_sums && p.gate_mode == GATE_ONE) c.gate_row = q.partials + (int64_t)parts_for(ctx, p.m) * 4 * p.n;
     column_kernel<<<(unsigned)((p.n + 255) / 256), 256, 0, ctx->stream>>>(c);
     RT_CUDA(cudaGetLastError());
     count_launch(ctx);

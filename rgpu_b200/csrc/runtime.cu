@@ -33,6 +33,9 @@ static int check_device_error(rt_ctx* ctx) {
         RT_CUDA(cudaMemcpy(ctx->dev_err, zero, sizeof zero, cudaMemcpyHostToDevice));
         if (h[0] == DEV_TIMEOUT_SELFTEST)
             return fail(RT_ERR_DEVICE_TIMEOUT, "the self-test wait expired on the device, as it is meant to");
+        if (h[0] == DEV_TIMEOUT_ROWS)
+            return fail(RT_ERR_DEVICE_TIMEOUT,
+                        "a block norm's wait for its rows expired on the device (CTA %d); its output is invalid", h[1]);
         const char* role = h[0] == DEV_TIMEOUT_PRODUCER ? "TMA producer"
                            : h[0] == DEV_TIMEOUT_MMA    ? "MMA issuer"
                                                         : "epilogue";

@@ -122,6 +122,30 @@ def test_forward(gpu, m, n, post, pre, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("m,n", [(9600, 96), (9500, 504), (2400, 1000), (2500, 2048), (1300, 2056), (600, 4104), (601, 8192)])
+def test_many_rows(gpu, m, n, kind, dtype):
+    for gate in ("row", "column") if n < 4000 else ("full" if kind == "layer" else "one",):
+        c = Case(gpu, m, n, dtype, kind, kind, gate, seed=m + n, pad=8)
+        z, zv = c.out()
+        h, hv = c.out()
+        q = gpu.mx4_zeros(m, n)
+        gpu.block_forward(c.dev["r"], y=c.dev["y"], post=c.norms["post"], gate=c.dev.get("gate"), scale=c.scale, z=z,
+                          pre=c.norms["pre"], h=h, hq=q)
+        wz, wh = R.block_forward(c.host["r"], c.host["y"], c.ref["post"], c.gate_ref, c.scale, c.ref["pre"])
+        gpu.sync()
+        tz, th = _forward_tolerance(c, wz, wh)
+        _near(zv, wz, _store(wz, tz, dtype), "z")
+        _near(hv, wh, _store(wh, th, dtype), "h")
+        a, b = gpu.zeros((m, n)), gpu.zeros((m, n))
+        gpu.mx4_dequantize(q, a)
+        gpu.mx4_dequantize(gpu.mx4_quantize(h), b)
+        assert np.array_equal(gpu.download(a), gpu.download(b))
+        if gate != "full":
+            _backward_check(c, c.host["r"], _backward(gpu, c, c.dev["r"]), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("gate", ["none", "one", "row", "column", "full"])
 def test_every_gate_and_in_place(gpu, gate, dtype):
     c = Case(gpu, 19, 320, dtype, "layer", "rms", gate, seed=4)
