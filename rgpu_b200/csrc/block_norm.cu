@@ -466,14 +466,15 @@ __global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p
 }
 
 // ------------------------------------------------------ rows through a ring
-// For many rows: one CTA of 1024 threads to an SM, its groups of TPR threads each
-// take a row at a time.  The rows arrive by bulk copies into a ring of slots, so
+// For many rows: one CTA of 1024 threads (backward: 512, for the registers that its
+// sums over rows take) to an SM, its groups of TPR threads each take a row at a
+// time.  The rows arrive by bulk copies into a ring of slots, so
 // the next rows are on their way while this one is summed, however few registers
 // that leaves; the vectors (gamma, beta and a gate of one row, folded together
 // where they meet) lie in shared memory once, in f32.
 constexpr int kRingThreads = 1024;
 constexpr int kRingSmem = 226 * 1024;
-constexpr int kRingScratch = 26 * 1024;  // sums (24 KB for 32 groups) and barriers
+constexpr int kRingScratch = 34 * 1024;  // sums (32 KB for 32 groups) and barriers
 
 struct RingP {
     int depth;         // slots of a group
@@ -482,45 +483,70 @@ struct RingP {
     int* err;
 };
 
-template <int TPR>
+// Warp sums of four values by halves: each exchange hands over the values that
+// the other half of the lanes goes on with, 6 shuffles in all and not 20.  Lane l
+// returns the sum of value l >> 3.
+__device__ __forceinline__ float warp_sum4(float v0, float v1, float v2, float v3) {
+    const int lane = threadIdx.x & 31;
+    const bool hi = lane & 16;
+    float a = (hi ? v2 : v0) + __shfl_xor_sync(0xffffffffu, hi ? v0 : v2, 16);
+    float b = (hi ? v3 : v1) + __shfl_xor_sync(0xffffffffu, hi ? v1 : v3, 16);
+    const bool odd = lane & 8;
+    a = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    return a;
+}
+
+template <int THREADS, int TPR>
 struct Group {
-    static constexpr int COUNT = kRingThreads / TPR;
+    static constexpr int COUNT = THREADS / TPR;
     int index, t;    // of the group in its CTA, of the thread in its group
-    float* red;      // [2][3][32]
+    float* red;      // [2][32 warps][4]
     int turn = 0;
 
     __device__ __forceinline__ void sync() const {
         if constexpr (TPR == 32)
             __syncwarp();
-        else if constexpr (TPR == kRingThreads)
+        else if constexpr (TPR == THREADS)
             __syncthreads();
         else
             asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "n"(TPR) : "memory");
     }
     // Sums over the group, to every thread, in a fixed order; one barrier.
-    template <int K>
-    __device__ __forceinline__ void sum(float (&v)[K]) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+    __device__ __forceinline__ void sum(float& v) {
+        v = warp_sum(v);
         if constexpr (TPR == 32) {
             __syncwarp();
         } else {
             constexpr int W = TPR / 32;
             const int lane = threadIdx.x & 31;
-            float* half = red + turn * 96;
+            float* half = red + turn * 128;
             turn ^= 1;
-            if (lane == 0)
-#pragma unroll
-                for (int k = 0; k < K; ++k) half[k * 32 + (t >> 5)] = v[k];
+            if (lane == 0) half[t >> 5] = v;
             sync();
+            v = half[lane % W];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float s = lane < W ? half[k * 32 + lane] : 0.0f;
-#pragma unroll
-                for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                v[k] = __shfl_sync(0xffffffffu, s, 0);
-            }
+            for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         }
+    }
+    __device__ __forceinline__ void sum(float (&v)[3]) {
+        float a = warp_sum4(v[0], v[1], v[2], 0.0f);
+        const int lane = threadIdx.x & 31;
+        if constexpr (TPR == 32) {
+            __syncwarp();
+        } else {
+            constexpr int W = TPR / 32;
+            float* half = red + turn * 128;
+            turn ^= 1;
+            if ((lane & 7) == 0) half[(t >> 5) * 4 + (lane >> 3)] = a;
+            sync();
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (lane < W) x = *reinterpret_cast<const float4*>(half + lane * 4);
+            a = warp_sum4(x.x, x.y, x.z, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) v[k] = __shfl_sync(0xffffffffu, a, k * 8);
     }
 };
 
@@ -543,7 +569,7 @@ __device__ __forceinline__ RingSmem ring_smem(uint8_t* smem, const RingP& r, int
     s.vec = reinterpret_cast<float*>(smem);
     s.slots = smem + (size_t)r.vectors * n * 4;
     s.red = reinterpret_cast<float*>(s.slots + (size_t)groups * r.depth * r.slot_bytes);
-    s.full = reinterpret_cast<uint64_t*>(s.red + groups * 192);  // a group's sums: [2][3][32]
+    s.full = reinterpret_cast<uint64_t*>(s.red + groups * 256);  // a group's sums: [2][32][4]
     s.abort_flag = reinterpret_cast<volatile int*>(s.full + groups * r.depth);
     return s;
 }
@@ -630,13 +656,13 @@ __device__ __forceinline__ float shared_gate(const BlockP& p, int j) {
 template <typename T, int TPR, int C, bool FULL>
 __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p, RingP r, int mask) {
     extern __shared__ __align__(128) uint8_t smem[];
-    using G = Group<TPR>;
+    using G = Group<kRingThreads, TPR>;
     const int n = (int)p.n;
     const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
     G g;
     g.index = threadIdx.x / TPR;
     g.t = threadIdx.x % TPR;
-    g.red = sm.red + g.index * 192;
+    g.red = sm.red + g.index * 256;
     uint8_t* slots = sm.slots + (size_t)g.index * r.depth * r.slot_bytes;
     const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
     const uint32_t row_bytes = (uint32_t)n * sizeof(T);
@@ -696,9 +722,9 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v2x = add2(v2x, y[i]);
                     }
-                float v[1] = {both(v2x)};
+                float v = both(v2x);
                 g.sum(v);
-                s.mu = v[0] * inv_n;
+                s.mu = v * inv_n;
             }
             const f2 less_mu = splat2(-s.mu);
             if (p.post.kind != RT_NORM_NONE) {
@@ -714,9 +740,9 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
                             v2x = fma2(y[i], y[i], v2x);
                         }
                     }
-                float v[1] = {both(v2x)};
+                float v = both(v2x);
                 g.sum(v);
-                s.rho = 1.0f / sqrtf(v[0] * inv_n + p.post.eps);
+                s.rho = 1.0f / sqrtf(v * inv_n + p.post.eps);
             }
             const f2 rho = splat2(mask & 1 ? s.rho : s.rho * p.scale);
 #pragma unroll
@@ -771,10 +797,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v2x = add2(v2x, z[c][i]);
-            float v[1] = {both(v2x)};
+            float v = both(v2x);
             g.sum(v);
             refill();
-            s.mu = v[0] * inv_n;
+            s.mu = v * inv_n;
         }
         const f2 less_mu = splat2(-s.mu);
         if (p.pre.kind != RT_NORM_NONE) {
@@ -787,10 +813,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
                         const f2 d = FULL ? add2(z[c][i], less_mu) : z[c][i];
                         v2x = fma2(d, d, v2x);
                     }
-            float v[1] = {both(v2x)};
+            float v = both(v2x);
             g.sum(v);
             if (!freed) refill();
-            s.rho = 1.0f / sqrtf(v[0] * inv_n + p.pre.eps);
+            s.rho = 1.0f / sqrtf(v * inv_n + p.pre.eps);
         }
         if (!freed) {
             g.sync();
@@ -833,16 +859,19 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
 // keeps the sums over rows of its eight columns in registers (FULL: those of the
 // betas too); the groups' sums are joined in shared memory in order, one partial
 // a CTA, and column_kernel adds the partials in order.
+constexpr int kBackThreads = 512;
+
 template <typename T, int TPR, bool FULL>
-__global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(BlockP p, GradP q, RingP r, int mask) {
+__global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p, GradP q, RingP r, int mask) {
     extern __shared__ __align__(128) uint8_t smem[];
-    using G = Group<TPR>;
+    using G = Group<kBackThreads, TPR>;
+    constexpr int C = 2;
     const int n = (int)p.n;
     const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
     G g;
     g.index = threadIdx.x / TPR;
     g.t = threadIdx.x % TPR;
-    g.red = sm.red + g.index * 192;
+    g.red = sm.red + g.index * 256;
     uint8_t* slots = sm.slots + (size_t)g.index * r.depth * r.slot_bytes;
     const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
     const uint32_t row_bytes = (uint32_t)n * sizeof(T);
@@ -855,7 +884,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(BlockP p
         tc::fence_barrier_init();
     }
     float *v2 = sm.vec, *vp = v2 + (mask & 1 ? n : 0), *vb = vp + (mask & 2 ? n : 0);
-    for (int j = threadIdx.x; j < n; j += kRingThreads) {
+    for (int j = threadIdx.x; j < n; j += kBackThreads) {
         if (mask & 1) v2[j] = __ldg(p.pre.gamma + j);
         if (mask & 2) vp[j] = p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
         if (mask & 4) vb[j] = p.scale * __ldg(p.post.beta + j);
@@ -874,13 +903,18 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(BlockP p
     if (g.t == 0)
         for (int d = 0; d < r.depth && first + d * step < p.m; ++d) issue(first + d * step, d);
     const float inv_n = 1.0f / (float)n;
-    const int j = g.t * 8;
-    const bool has = j < n;
-    f2 sum_a[4], sum_b[FULL ? 4 : 1], sum_c[4], sum_d[FULL ? 4 : 1];
+    int j[C];
+    bool has[C];
+    f2 sum_a[C][4], sum_b[FULL ? C : 1][4], sum_c[C][4], sum_d[FULL ? C : 1][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        sum_a[i] = sum_c[i] = 0;
-        if constexpr (FULL) sum_b[i] = sum_d[i] = 0;
+    for (int c = 0; c < C; ++c) {
+        j[c] = (c * TPR + g.t) * 8;
+        has[c] = j[c] < n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum_a[c][i] = sum_c[c][i] = 0;
+            if constexpr (FULL) sum_b[c][i] = sum_d[c][i] = 0;
+        }
     }
     int slot = 0;
     uint32_t phase = 0;
@@ -897,29 +931,31 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(BlockP p
         float a0 = 0.0f, a1 = 0.0f;
         if (FULL && (p.pre.kind == RT_NORM_LAYER || p.post.kind == RT_NORM_LAYER)) {
             f2 sums[3] = {0, 0, 0};
-            if (has) {
-                f2 x[4], w[4];
-                if (p.pre.kind == RT_NORM_LAYER) {
-                    slot8<T>(at, j, x);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sums[0] = add2(sums[0], x[i]);
-                    if (back) {
-                        slot8<T>(at + at_dh, j, x);
-                        if (mask & 1) {
-                            vec8(v2, j, w);
+            for (int c = 0; c < C; ++c)
+                if (has[c]) {
+                    f2 x[4], w[4];
+                    if (p.pre.kind == RT_NORM_LAYER) {
+                        slot8<T>(at, j[c], x);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], w[i]);
+                        for (int i = 0; i < 4; ++i) sums[0] = add2(sums[0], x[i]);
+                        if (back) {
+                            slot8<T>(at + at_dh, j[c], x);
+                            if (mask & 1) {
+                                vec8(v2, j[c], w);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], w[i]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) sums[1] = add2(sums[1], x[i]);
                         }
+                    }
+                    if (p.post.kind == RT_NORM_LAYER) {
+                        slot8<T>(at + at_y, j[c], x);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sums[1] = add2(sums[1], x[i]);
+                        for (int i = 0; i < 4; ++i) sums[2] = add2(sums[2], x[i]);
                     }
                 }
-                if (p.post.kind == RT_NORM_LAYER) {
-                    slot8<T>(at + at_y, j, x);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sums[2] = add2(sums[2], x[i]);
-                }
-            }
             float v[3] = {both(sums[0]), both(sums[1]), both(sums[2])};
             g.sum(v);
             sz.mu = v[0] * inv_n;
@@ -929,148 +965,150 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(BlockP p
         const f2 less_z = splat2(-sz.mu), less_y = splat2(-sy.mu);
         if (p.pre.kind != RT_NORM_NONE || p.post.kind != RT_NORM_NONE) {
             f2 sums[3] = {0, 0, 0};
-            if (has) {
-                f2 x[4];
-                if (p.pre.kind != RT_NORM_NONE) {
-                    slot8<T>(at, j, x);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (FULL) x[i] = add2(x[i], less_z);
-                        sums[0] = fma2(x[i], x[i], sums[0]);
-                    }
-                    if (back) {
-                        f2 d[4], w[4];
-                        slot8<T>(at + at_dh, j, d);
-                        if (mask & 1) {
-                            vec8(v2, j, w);
+            for (int c = 0; c < C; ++c)
+                if (has[c]) {
+                    f2 x[4];
+                    if (p.pre.kind != RT_NORM_NONE) {
+                        slot8<T>(at, j[c], x);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) d[i] = mul2(d[i], w[i]);
+                        for (int i = 0; i < 4; ++i) {
+                            if (FULL) x[i] = add2(x[i], less_z);
+                            sums[0] = fma2(x[i], x[i], sums[0]);
                         }
+                        if (back) {
+                            f2 d[4], w[4];
+                            slot8<T>(at + at_dh, j[c], d);
+                            if (mask & 1) {
+                                vec8(v2, j[c], w);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sums[1] = fma2(d[i], x[i], sums[1]);
+                                for (int i = 0; i < 4; ++i) d[i] = mul2(d[i], w[i]);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) sums[1] = fma2(d[i], x[i], sums[1]);
+                        }
+                    }
+                    if (p.post.kind != RT_NORM_NONE) {
+                        slot8<T>(at + at_y, j[c], x);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (FULL) x[i] = add2(x[i], less_y);
+                            sums[2] = fma2(x[i], x[i], sums[2]);
+                        }
                     }
                 }
-                if (p.post.kind != RT_NORM_NONE) {
-                    slot8<T>(at + at_y, j, x);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (FULL) x[i] = add2(x[i], less_y);
-                        sums[2] = fma2(x[i], x[i], sums[2]);
-                    }
-                }
-            }
             float v[3] = {both(sums[0]), both(sums[1]), both(sums[2])};
             g.sum(v);
             if (p.pre.kind != RT_NORM_NONE) sz.rho = 1.0f / sqrtf(v[0] * inv_n + p.pre.eps);
             if (p.post.kind != RT_NORM_NONE) sy.rho = 1.0f / sqrtf(v[2] * inv_n + p.post.eps);
             a1 = v[1] * inv_n * sz.rho;  // mean of a z^
         }
-        // dr, and the sums over rows of dh
-        f2 dr[4];
+        // dr and the sums over rows of dh; then b = s g gamma_post dr and its sums
+        f2 b[C][4], hat[C][4];
+        f2 sums[3] = {0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dr[i] = 0;
-        if (has) {
-            if (q.dz) slot8<T>(at + at_dz, j, dr);
+        for (int c = 0; c < C; ++c) {
+            if (!has[c]) continue;
+            f2 dr[4], w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dr[i] = 0;
+            if (q.dz) slot8<T>(at + at_dz, j[c], dr);
             if (q.dh) {
-                f2 d[4], hat[4], w[4];
+                f2 d[4], h[4];
                 const f2 rho = splat2(sz.rho), less_a0 = splat2(-a0), less_a1 = splat2(-a1);
-                slot8<T>(at + at_dh, j, d);
-                slot8<T>(at, j, hat);
+                slot8<T>(at + at_dh, j[c], d);
+                slot8<T>(at, j[c], h);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    hat[i] = mul2(FULL ? add2(hat[i], less_z) : hat[i], rho);
-                    sum_c[i] = fma2(d[i], hat[i], sum_c[i]);
-                    if constexpr (FULL) sum_d[i] = add2(sum_d[i], d[i]);
+                    h[i] = mul2(FULL ? add2(h[i], less_z) : h[i], rho);
+                    sum_c[c][i] = fma2(d[i], h[i], sum_c[c][i]);
+                    if constexpr (FULL) sum_d[c][i] = add2(sum_d[c][i], d[i]);
                 }
                 if (mask & 1) {
-                    vec8(v2, j, w);
+                    vec8(v2, j[c], w);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) d[i] = mul2(d[i], w[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (FULL) d[i] = add2(d[i], less_a0);
-                    dr[i] = fma2(fma2(hat[i], less_a1, d[i]), rho, dr[i]);
+                    dr[i] = fma2(fma2(h[i], less_a1, d[i]), rho, dr[i]);
                 }
             }
-            if (q.dr) store8<T>(q.dr, row * q.lddr + j, dr);
-        }
-        if (p.y) {
-            f2 sums[3] = {0, 0, 0};
-            f2 b[4], hat[4];
-            if (has) {
-                f2 w[4];
-                const f2 rho = splat2(sy.rho);
-                slot8<T>(at + at_y, j, hat);
+            if (q.dr) store8<T>(q.dr, row * q.lddr + j[c], dr);
+            if (!p.y) continue;
+            const f2 rho = splat2(sy.rho);
+            slot8<T>(at + at_y, j[c], hat[c]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) hat[i] = mul2(FULL ? add2(hat[i], less_y) : hat[i], rho);
-                if (mask & 2) {
-                    vec8(vp, j, w);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = splat2(p.scale);
-                }
-                if (own_gate) {
-                    // s u dr is the gate's gradient, and g dr takes the place of dr
-                    f2 u[4], gate[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) u[i] = mul2(hat[i], w[i]);
-                    if (mask & 4) {
-                        vec8(vb, j, gate);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) u[i] = add2(u[i], gate[i]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        u[i] = mul2(u[i], dr[i]);
-                        sums[2] = add2(sums[2], u[i]);
-                    }
-                    if (p.gate_mode == GATE_FULL) {
-                        slot8<T>(reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.gate) + row * p.ldg), j, gate);
-                        if (q.dgate) store8<T>(q.dgate, row * q.lddg + j, u);
-                    } else {
-                        const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) gate[i] = one;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) dr[i] = mul2(dr[i], gate[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sum_a[i] = fma2(dr[i], hat[i], sum_a[i]);
-                    if constexpr (FULL) sum_b[i] = add2(sum_b[i], dr[i]);
-                    b[i] = mul2(dr[i], w[i]);
-                    if (FULL) sums[0] = add2(sums[0], b[i]);
-                    sums[1] = fma2(b[i], hat[i], sums[1]);
-                }
-            }
-            float v[3] = {0.0f, both(sums[1]), 0.0f};
-            if constexpr (FULL) {
-                v[0] = both(sums[0]);
-                v[2] = both(sums[2]);
-                g.sum(v);
-                if (g.t == 0 && q.dgate && p.gate_mode == GATE_COLUMN) static_cast<float*>(q.dgate)[row * q.lddg] = v[2];
+            for (int i = 0; i < 4; ++i) hat[c][i] = mul2(FULL ? add2(hat[c][i], less_y) : hat[c][i], rho);
+            if (mask & 2) {
+                vec8(vp, j[c], w);
             } else {
-                float one[1] = {v[1]};
-                g.sum(one);
-                v[1] = one[0];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = splat2(p.scale);
             }
-            if (has && q.dy) {
-                const f2 rho = splat2(sy.rho), b0 = splat2(p.post.kind == RT_NORM_LAYER ? -v[0] * inv_n : 0.0f);
-                const f2 b1 = splat2(p.post.kind != RT_NORM_NONE ? -v[1] * inv_n : 0.0f);
+            if (own_gate) {
+                // s u dr is the gate's gradient, and g dr takes the place of dr
+                f2 u[4], gate[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u[i] = mul2(hat[c][i], w[i]);
+                if (mask & 4) {
+                    vec8(vb, j[c], gate);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) u[i] = add2(u[i], gate[i]);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (FULL) b[i] = add2(b[i], b0);
-                    b[i] = mul2(fma2(hat[i], b1, b[i]), rho);
+                    u[i] = mul2(u[i], dr[i]);
+                    sums[2] = add2(sums[2], u[i]);
                 }
-                store8<T>(q.dy, row * q.lddy + j, b);
+                if (p.gate_mode == GATE_FULL) {
+                    slot8<T>(reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.gate) + row * p.ldg), j[c], gate);
+                    if (q.dgate) store8<T>(q.dgate, row * q.lddg + j[c], u);
+                } else {
+                    const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) gate[i] = one;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dr[i] = mul2(dr[i], gate[i]);
             }
-        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sum_a[c][i] = fma2(dr[i], hat[c][i], sum_a[c][i]);
+                if constexpr (FULL) sum_b[c][i] = add2(sum_b[c][i], dr[i]);
+                b[c][i] = mul2(dr[i], w[i]);
+                if (FULL) sums[0] = add2(sums[0], b[c][i]);
+                sums[1] = fma2(b[c][i], hat[c][i], sums[1]);
+            }
+        }
+        float b0 = 0.0f, b1 = both(sums[1]);
+        if (!p.y) {
             g.sync();
+        } else if constexpr (FULL) {
+            float v[3] = {both(sums[0]), b1, both(sums[2])};
+            g.sum(v);
+            b0 = p.post.kind == RT_NORM_LAYER ? -v[0] * inv_n : 0.0f;
+            b1 = v[1];
+            if (g.t == 0 && q.dgate && p.gate_mode == GATE_COLUMN) static_cast<float*>(q.dgate)[row * q.lddg] = v[2];
+        } else {
+            g.sum(b1);
         }
         // every thread of the group has read the slot: all of it before the last barrier
         if (g.t == 0 && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
+        if (q.dy) {
+            const f2 rho = splat2(sy.rho), add = splat2(b0), less_b1 = splat2(p.post.kind != RT_NORM_NONE ? -b1 * inv_n : 0.0f);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (has[c]) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (FULL) b[c][i] = add2(b[c][i], add);
+                        b[c][i] = mul2(fma2(hat[c][i], less_b1, b[c][i]), rho);
+                    }
+                    store8<T>(q.dy, row * q.lddy + j[c], b[c]);
+                }
+        }
         if (++slot == r.depth) {
             slot = 0;
             phase ^= 1;
@@ -1080,19 +1118,22 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(BlockP p
     // the groups' sums, added in order; the slots are all read
     __syncthreads();
     float* acc = reinterpret_cast<float*>(sm.slots);  // [n]
-    auto join = [&](int which, const f2* sums) {
+    auto join = [&](int which, const f2 (&sums)[C][4]) {
         if (!((q.sums >> which) & 1)) return;
         for (int k = 0; k < G::COUNT; ++k) {
-            if (g.index == k && has) {
-                f2* a = reinterpret_cast<f2*>(acc + j);
-                f2 x[4];
+            if (g.index == k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[i]) : sums[i];
-                if (k == G::COUNT - 1)
-                    a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * n + j);
+                for (int c = 0; c < C; ++c)
+                    if (has[c]) {
+                        f2* a = reinterpret_cast<f2*>(acc + j[c]);
+                        f2 x[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = x[i];
-            }
+                        for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[c][i]) : sums[c][i];
+                        if (k == G::COUNT - 1)
+                            a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * n + j[c]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) a[i] = x[i];
+                    }
             if (G::COUNT > 1) __syncthreads();
         }
     };
@@ -1116,15 +1157,28 @@ struct ReduceP {
     float* gate_row;  // [n]: a [1,1] gate's gradient by column
 };
 
-// Column sums of the partials, parts in order, and the vectors they give.
-__global__ void __launch_bounds__(256) column_kernel(ReduceP p) {
-    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (j >= p.n) return;
+// Column sums of the partials and the vectors they give.  A CTA takes 32 columns;
+// each of its 16 warps adds every 16th part in order, the warps' sums are added
+// in order: 148 parts one after another took 82 us at 8192 columns, all latency.
+__global__ void __launch_bounds__(512) column_kernel(ReduceP p) {
+    __shared__ float sums[16][4][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t j = (int64_t)blockIdx.x * 32 + lane;
     float s[4] = {};
-    for (int i = 0; i < p.parts; ++i)
+    if (j < p.n)
+#pragma unroll 5
+        for (int i = warp; i < p.parts; i += 16)
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
-            if ((p.sums >> v) & 1) s[v] += p.partials[((int64_t)i * 4 + v) * p.n + j];
+            for (int v = 0; v < 4; ++v)
+                if ((p.sums >> v) & 1) s[v] += p.partials[((int64_t)i * 4 + v) * p.n + j];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) sums[warp][v][lane] = s[v];
+    __syncthreads();
+    if (warp > 0 || j >= p.n) return;
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s[v] += sums[w][v][lane];
     s[0] *= p.scale;
     s[1] *= p.scale;
     const float g = p.gate_mode == GATE_ONE ? p.gate[0] : p.gate_mode == GATE_ROW ? p.gate[j] : 1.0f;
@@ -1248,7 +1302,8 @@ bool plan_ring(RingP* r, int64_t n, int groups, int tensors, size_t es, int vect
 
 template <typename T, int TPR, int C>
 int launch_forward_ring(rt_ctx* ctx, const BlockP& p, RingP r, int mask, cudaStream_t st) {
-    const int64_t ctas = std::min<int64_t>(ctx->sm_count, (p.m + Group<TPR>::COUNT - 1) / Group<TPR>::COUNT);
+    constexpr int groups = kRingThreads / TPR;
+    const int64_t ctas = std::min<int64_t>(ctx->sm_count, (p.m + groups - 1) / groups);
     const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (mask & 10) ||
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
     auto* kernel = full ? forward_ring_kernel<T, TPR, C, true> : forward_ring_kernel<T, TPR, C, false>;
@@ -1283,7 +1338,7 @@ int launch_backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, const Rin
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
     auto* kernel = full ? backward_ring_kernel<T, TPR, true> : backward_ring_kernel<T, TPR, false>;
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    kernel<<<(unsigned)ctas, kRingThreads, kRingSmem, st>>>(p, q, r, mask);
+    kernel<<<(unsigned)ctas, kBackThreads, kRingSmem, st>>>(p, q, r, mask);
     return RT_OK;
 }
 
@@ -1300,8 +1355,8 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
     const bool shared = p.gate_mode == GATE_ONE || p.gate_mode == GATE_ROW;
     const int mask = (p.pre.gamma ? 1 : 0) | (p.post.gamma || (p.y && shared) ? 2 : 0) |
                      (p.post.beta && q.dgate && !shared ? 4 : 0);
-    const int tpr = p.n <= 256 ? 32 : p.n <= 1024 ? 128 : p.n <= 2048 ? 256 : p.n <= 4096 ? 512 : 1024;
-    const int groups = kRingThreads / tpr;
+    const int tpr = p.n <= 512 ? 32 : p.n <= 1024 ? 64 : p.n <= 2048 ? 128 : p.n <= 4096 ? 256 : 512;
+    const int groups = kBackThreads / tpr;
     RingP r{};
     r.err = ctx->dev_err;
     if (!plan_ring(&r, p.n, groups, 1 + (p.y ? 1 : 0) + (q.dz ? 1 : 0) + (q.dh ? 1 : 0), es, __builtin_popcount(mask)))
@@ -1309,10 +1364,10 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
     *done = true;
     *parts = (int)std::min<int64_t>(ctx->sm_count, (p.m + groups - 1) / groups);
     if (tpr == 32) return launch_backward_ring<T, 32>(ctx, p, q, r, mask, *parts, st);
+    if (tpr == 64) return launch_backward_ring<T, 64>(ctx, p, q, r, mask, *parts, st);
     if (tpr == 128) return launch_backward_ring<T, 128>(ctx, p, q, r, mask, *parts, st);
     if (tpr == 256) return launch_backward_ring<T, 256>(ctx, p, q, r, mask, *parts, st);
-    if (tpr == 512) return launch_backward_ring<T, 512>(ctx, p, q, r, mask, *parts, st);
-    return launch_backward_ring<T, 1024>(ctx, p, q, r, mask, *parts, st);
+    return launch_backward_ring<T, 512>(ctx, p, q, r, mask, *parts, st);
 }
 
 // Up to 16384 wide: the fewest threads that hold a row eight elements each (the
@@ -1479,7 +1534,7 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     c.gamma = p.post.gamma;
     c.beta = p.post.beta;
     if (gate_sums && p.gate_mode == GATE_ONE) c.gate_row = q.partials + (int64_t)parts_for(ctx, p.m) * 4 * p.n;
-    column_kernel<<<(unsigned)((p.n + 255) / 256), 256, 0, ctx->stream>>>(c);
+    column_kernel<<<(unsigned)((p.n + 31) / 32), 512, 0, ctx->stream>>>(c);
     RT_CUDA(cudaGetLastError());
     count_launch(ctx);
     if (c.gate_row) {
