@@ -20,6 +20,9 @@
 namespace rt {
 namespace {
 
+// Every kernel here launches as a programmatic dependent of the one before it on
+// the stream (launch_k), and waits for it before touching global memory.
+
 enum GateMode : int { GATE_NONE = 0, GATE_ONE = 1, GATE_ROW = 2, GATE_COLUMN = 3, GATE_FULL = 4 };
 
 struct NormP {
@@ -113,7 +116,7 @@ __device__ __forceinline__ Stat row_stat(const NormP& p, int64_t n, float* red, 
         const float d = x(j) - s.mu;
         t += d * d;
     }
-    s.rho = 1.0f / sqrtf(block_sum(t, red) / (float)n + p.eps);
+    s.rho = rsqrtf(block_sum(t, red) / (float)n + p.eps);
     return s;
 }
 
@@ -135,6 +138,8 @@ __device__ __forceinline__ float gate_at(const BlockP& p, int64_t row, int64_t j
 template <typename T>
 __global__ void __launch_bounds__(256) forward_kernel(BlockP p) {
     __shared__ float red[8];
+    pdl_wait();
+    pdl_launch_dependents();
     const int64_t n = p.n, blocks = (n + 31) / 32, groups = (blocks + 3) / 4;
     for (int64_t row = blockIdx.x; row < p.m; row += gridDim.x) {
         Stat sy{0.0f, 1.0f};
@@ -178,6 +183,8 @@ __global__ void __launch_bounds__(256) forward_kernel(BlockP p) {
 template <typename T>
 __global__ void __launch_bounds__(256) backward_kernel(BlockP p, GradP g) {
     __shared__ float red[8];
+    pdl_wait();
+    pdl_launch_dependents();
     const int64_t n = p.n;
     float* acc = g.partials ? g.partials + (int64_t)blockIdx.x * 4 * n : nullptr;
     if (acc)
@@ -359,7 +366,7 @@ __device__ __forceinline__ Stat stat_of(const NormP& p, const float (&x)[C][8], 
                 const float d = x[c][i] - s.mu;
                 t += d * d;
             }
-    s.rho = 1.0f / sqrtf(row_sum<TPR>(t, red, turn) * inv_n + p.eps);
+    s.rho = rsqrtf(row_sum<TPR>(t, red, turn) * inv_n + p.eps);
     return s;
 }
 
@@ -404,6 +411,8 @@ constexpr int cta_threads(int tpr) { return tpr < 128 ? 128 : tpr; }
 template <typename T, int TPR, int C>
 __global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p) {
     constexpr int ROWS = cta_threads(TPR) / TPR;
+    pdl_wait();
+    pdl_launch_dependents();
     __shared__ float red_all[ROWS][64];
     float* red = red_all[threadIdx.x / TPR];
     int turn = 0;
@@ -473,8 +482,9 @@ __global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p
 // that leaves; the vectors (gamma, beta and a gate of one row, folded together
 // where they meet) lie in shared memory once, in f32.
 constexpr int kRingThreads = 1024;
-constexpr int kRingSmem = 226 * 1024;
-constexpr int kRingScratch = 34 * 1024;  // sums (32 KB for 32 groups) and barriers
+constexpr int kRingSmem = 227 * 1024;
+// a group's sums, its barriers (up to eight) and the abort flag
+constexpr int ring_scratch(int groups) { return groups * (1024 + 64) + 16; }
 
 struct RingP {
     int depth;         // slots of a group
@@ -530,8 +540,10 @@ struct Group {
             for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         }
     }
-    __device__ __forceinline__ void sum(float (&v)[3]) {
-        float a = warp_sum4(v[0], v[1], v[2], 0.0f);
+    template <int K>
+    __device__ __forceinline__ void sum(float (&v)[K]) {
+        static_assert(K == 3 || K == 4, "three or four sums at a time");
+        float a = warp_sum4(v[0], v[1], v[2], K == 4 ? v[K - 1] : 0.0f);
         const int lane = threadIdx.x & 31;
         if constexpr (TPR == 32) {
             __syncwarp();
@@ -543,10 +555,10 @@ struct Group {
             sync();
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (lane < W) x = *reinterpret_cast<const float4*>(half + lane * 4);
-            a = warp_sum4(x.x, x.y, x.z, 0.0f);
+            a = warp_sum4(x.x, x.y, x.z, K == 4 ? x.w : 0.0f);
         }
 #pragma unroll
-        for (int k = 0; k < 3; ++k) v[k] = __shfl_sync(0xffffffffu, a, k * 8);
+        for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, a, k * 8);
     }
 };
 
@@ -562,7 +574,6 @@ struct RingSmem {
     uint8_t* slots;
     float* red;
     uint64_t* full;
-    volatile int* abort_flag;
 };
 __device__ __forceinline__ RingSmem ring_smem(uint8_t* smem, const RingP& r, int n, int groups) {
     RingSmem s;
@@ -570,7 +581,6 @@ __device__ __forceinline__ RingSmem ring_smem(uint8_t* smem, const RingP& r, int
     s.slots = smem + (size_t)r.vectors * n * 4;
     s.red = reinterpret_cast<float*>(s.slots + (size_t)groups * r.depth * r.slot_bytes);
     s.full = reinterpret_cast<uint64_t*>(s.red + groups * 256);  // a group's sums: [2][32][4]
-    s.abort_flag = reinterpret_cast<volatile int*>(s.full + groups * r.depth);
     return s;
 }
 
@@ -608,15 +618,18 @@ __device__ __forceinline__ float both(f2 a) {
     return x.x + x.y;
 }
 
-// Eight elements of a slot's row, of a vector in shared memory.
+// Eight elements as pairs: of a register's worth of bf16, of a slot's row, of a
+// vector in shared memory.
+__device__ __forceinline__ void pairs8(const Raw8<__nv_bfloat16>& r, f2 (&v)[4]) {
+    const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
 template <typename T>
 __device__ __forceinline__ void slot8(const uint8_t* row, int j, f2 (&v)[4]) {
     const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(row) + j);
     if constexpr (sizeof(T) == 2) {
-        const uint4 u = p[0];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        pairs8(Raw8<T>{{p[0]}}, v);
     } else {
         const ulonglong2 a = reinterpret_cast<const ulonglong2*>(p)[0], b = reinterpret_cast<const ulonglong2*>(p)[1];
         v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
@@ -667,12 +680,15 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
     const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
     const uint32_t row_bytes = (uint32_t)n * sizeof(T);
     const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * r.depth);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < G::COUNT * r.depth; ++i) tc::mbar_init(tc::smem_u32(sm.full + i), 1);
-        *sm.abort_flag = 0;
+        *abort_flag = 0;
         tc::fence_barrier_init();
     }
+    pdl_wait();
+    pdl_launch_dependents();
     float *vp = sm.vec, *vq = vp + (mask & 1 ? n : 0), *v2 = vq + (mask & 2 ? n : 0), *vb = v2 + (mask & 4 ? n : 0);
     for (int j = threadIdx.x; j < n; j += kRingThreads) {
         const float sg = p.scale * shared_gate(p, j);
@@ -697,8 +713,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
 #pragma unroll
     for (int c = 0; c < C; ++c) has[c] = (c * TPR + g.t) * 8 < n;
     for (int64_t row = first; row < p.m; row += step) {
-        if (!tc::mbar_wait(full + slot * 8, phase, sm.abort_flag)) {
-            *sm.abort_flag = 1;
+        if (!tc::mbar_wait(full + slot * 8, phase, abort_flag)) {
+            *abort_flag = 1;
             tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
         }
         const uint8_t* at = slots + (size_t)slot * r.slot_bytes;
@@ -742,7 +758,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
                     }
                 float v = both(v2x);
                 g.sum(v);
-                s.rho = 1.0f / sqrtf(v * inv_n + p.post.eps);
+                s.rho = rsqrtf(v * inv_n + p.post.eps);
             }
             const f2 rho = splat2(mask & 1 ? s.rho : s.rho * p.scale);
 #pragma unroll
@@ -816,7 +832,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
             float v = both(v2x);
             g.sum(v);
             if (!freed) refill();
-            s.rho = 1.0f / sqrtf(v * inv_n + p.pre.eps);
+            s.rho = rsqrtf(v * inv_n + p.pre.eps);
         }
         if (!freed) {
             g.sync();
@@ -861,6 +877,29 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
 // a CTA, and column_kernel adds the partials in order.
 constexpr int kBackThreads = 512;
 
+// The groups' sums of one kind, added in order through acc [n], to the CTA's partial.
+template <typename G, int C>
+__device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc, int n, int which,
+                                          const f2 (&sums)[C][4], const int (&j)[C], const bool (&has)[C]) {
+    if (!((q.sums >> which) & 1)) return;
+    for (int k = 0; k < G::COUNT; ++k) {
+        if (g.index == k)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (has[c]) {
+                    f2* a = reinterpret_cast<f2*>(acc + j[c]);
+                    f2 x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[c][i]) : sums[c][i];
+                    if (k == G::COUNT - 1)
+                        a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * n + j[c]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) a[i] = x[i];
+                }
+        if (G::COUNT > 1) __syncthreads();
+    }
+}
+
 template <typename T, int TPR, bool FULL>
 __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p, GradP q, RingP r, int mask) {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -877,12 +916,15 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     const uint32_t row_bytes = (uint32_t)n * sizeof(T);
     const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
     const bool own_gate = FULL && (p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * r.depth);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < G::COUNT * r.depth; ++i) tc::mbar_init(tc::smem_u32(sm.full + i), 1);
-        *sm.abort_flag = 0;
+        *abort_flag = 0;
         tc::fence_barrier_init();
     }
+    pdl_wait();
+    pdl_launch_dependents();
     float *v2 = sm.vec, *vp = v2 + (mask & 1 ? n : 0), *vb = vp + (mask & 2 ? n : 0);
     for (int j = threadIdx.x; j < n; j += kBackThreads) {
         if (mask & 1) v2[j] = __ldg(p.pre.gamma + j);
@@ -920,8 +962,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     uint32_t phase = 0;
     const bool back = q.dh && p.pre.kind != RT_NORM_NONE;
     for (int64_t row = first; row < p.m; row += step) {
-        if (!tc::mbar_wait(full + slot * 8, phase, sm.abort_flag)) {
-            *sm.abort_flag = 1;
+        if (!tc::mbar_wait(full + slot * 8, phase, abort_flag)) {
+            *abort_flag = 1;
             tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
         }
         const uint8_t* at = slots + (size_t)slot * r.slot_bytes;
@@ -999,8 +1041,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                 }
             float v[3] = {both(sums[0]), both(sums[1]), both(sums[2])};
             g.sum(v);
-            if (p.pre.kind != RT_NORM_NONE) sz.rho = 1.0f / sqrtf(v[0] * inv_n + p.pre.eps);
-            if (p.post.kind != RT_NORM_NONE) sy.rho = 1.0f / sqrtf(v[2] * inv_n + p.post.eps);
+            if (p.pre.kind != RT_NORM_NONE) sz.rho = rsqrtf(v[0] * inv_n + p.pre.eps);
+            if (p.post.kind != RT_NORM_NONE) sy.rho = rsqrtf(v[2] * inv_n + p.post.eps);
             a1 = v[1] * inv_n * sz.rho;  // mean of a z^
         }
         // dr and the sums over rows of dh; then b = s g gamma_post dr and its sums
@@ -1115,34 +1157,196 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
         }
     }
     if (!q.partials) return;
-    // the groups' sums, added in order; the slots are all read
+    __syncthreads();  // the slots are all read
+    float* acc = reinterpret_cast<float*>(sm.slots);
+    join_sums<G>(g, q, acc, n, 0, sum_a, j, has);
+    join_sums<G>(g, q, acc, n, 2, sum_c, j, has);
+    if constexpr (FULL) {
+        join_sums<G>(g, q, acc, n, 1, sum_b, j, has);
+        join_sums<G>(g, q, acc, n, 3, sum_d, j, has);
+    }
+}
+
+// Backward for the common training step, bf16 rows between two RMS norms with
+// dz, dh and y all there: rows overlap, so each costs one barrier.  While row i's
+// dr is computed and summed against y^ its successor's three sums are taken, and
+// all four are joined at once.  z, y and dh of a row are read into registers when
+// its sums are taken and their slots are then free; dz has slots of its own.
+template <int TPR>
+__global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p, GradP q, RingP r) {
+    using T = __nv_bfloat16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    using G = Group<kBackThreads, TPR>;
+    constexpr int C = 2;
+    const int n = (int)p.n, depth = r.depth;
+    const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
+    G g;
+    g.index = threadIdx.x / TPR;
+    g.t = threadIdx.x % TPR;
+    g.red = sm.red + g.index * 256;
+    // slots: [depth] of z, y, dh, then [depth] of dz; barriers likewise
+    uint8_t* slots = sm.slots + (size_t)g.index * depth * r.slot_bytes;
+    const uint32_t row_bytes = (uint32_t)n * sizeof(T);
+    uint8_t* slots_dz = slots + (size_t)depth * 3 * row_bytes;
+    const uint32_t full = tc::smem_u32(sm.full + g.index * 2 * depth), full_dz = full + depth * 8;
+    const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * 2 * depth);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < G::COUNT * 2 * depth; ++i) tc::mbar_init(tc::smem_u32(sm.full + i), 1);
+        *abort_flag = 0;
+        tc::fence_barrier_init();
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    float *v2 = sm.vec, *vp = v2 + n;
+    for (int j = threadIdx.x; j < n; j += kBackThreads) {
+        v2[j] = p.pre.gamma ? __ldg(p.pre.gamma + j) : 1.0f;
+        vp[j] = p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
+    }
     __syncthreads();
-    float* acc = reinterpret_cast<float*>(sm.slots);  // [n]
-    auto join = [&](int which, const f2 (&sums)[C][4]) {
-        if (!((q.sums >> which) & 1)) return;
-        for (int k = 0; k < G::COUNT; ++k) {
-            if (g.index == k)
-#pragma unroll
-                for (int c = 0; c < C; ++c)
-                    if (has[c]) {
-                        f2* a = reinterpret_cast<f2*>(acc + j[c]);
-                        f2 x[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[c][i]) : sums[c][i];
-                        if (k == G::COUNT - 1)
-                            a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * n + j[c]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) a[i] = x[i];
-                    }
-            if (G::COUNT > 1) __syncthreads();
+    auto issue = [&](int64_t row, int slot) {
+        const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * 3 * row_bytes);
+        tc::mbar_expect_tx(bar, 3 * row_bytes);
+        bulk_load(dst, static_cast<const T*>(p.z) + row * p.ldz, row_bytes, bar);
+        bulk_load(dst + row_bytes, static_cast<const T*>(p.y) + row * p.ldy, row_bytes, bar);
+        bulk_load(dst + 2 * row_bytes, static_cast<const T*>(q.dh) + row * q.lddh, row_bytes, bar);
+    };
+    auto issue_dz = [&](int64_t row, int slot) {
+        const uint32_t bar = full_dz + slot * 8;
+        tc::mbar_expect_tx(bar, row_bytes);
+        bulk_load(tc::smem_u32(slots_dz + (size_t)slot * row_bytes), static_cast<const T*>(q.dz) + row * q.lddz, row_bytes, bar);
+    };
+    if (g.t == 0)
+        for (int d = 0; d < depth && first + d * step < p.m; ++d) {
+            issue(first + d * step, d);
+            issue_dz(first + d * step, d);
+        }
+    auto wait = [&](uint32_t bar, uint32_t phase) {
+        if (!tc::mbar_wait(bar, phase, abort_flag)) {
+            *abort_flag = 1;
+            tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
         }
     };
-    join(0, sum_a);
-    join(2, sum_c);
-    if constexpr (FULL) {
-        join(1, sum_b);
-        join(3, sum_d);
+    const float inv_n = 1.0f / (float)n;
+    int j[C];
+    bool has[C];
+    f2 sum_a[C][4], sum_c[C][4];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        j[c] = (c * TPR + g.t) * 8;
+        has[c] = j[c] < n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum_a[c][i] = sum_c[c][i] = 0;
     }
+    Raw8<T> rz[C], ry[C], rd[C];
+    // z, y and dh of the row in `slot`, and what they add to z^2, gamma_pre dh z, y^2
+    auto take = [&](int slot, float (&v)[3]) {
+        const uint8_t* at = slots + (size_t)slot * 3 * row_bytes;
+        f2 sums[3] = {0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (!has[c]) continue;
+            rz[c] = load_raw8<T>(at, j[c]);
+            ry[c] = load_raw8<T>(at + row_bytes, j[c]);
+            rd[c] = load_raw8<T>(at + 2 * row_bytes, j[c]);
+            f2 x[4], d[4], w[4];
+            pairs8(rz[c], x);
+            pairs8(rd[c], d);
+            vec8(v2, j[c], w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sums[0] = fma2(x[i], x[i], sums[0]);
+                sums[1] = fma2(mul2(d[i], w[i]), x[i], sums[1]);
+            }
+            pairs8(ry[c], x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[2] = fma2(x[i], x[i], sums[2]);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) v[k] = both(sums[k]);
+    };
+    float rho_z = 0.0f, rho_y = 0.0f, a1 = 0.0f;
+    auto stats = [&](float z2, float az, float y2) {
+        rho_z = rsqrtf(z2 * inv_n + p.pre.eps);
+        rho_y = rsqrtf(y2 * inv_n + p.post.eps);
+        a1 = az * inv_n * rho_z;
+    };
+    int slot = 0;
+    uint32_t phase = 0;
+    if (first < p.m) {
+        wait(full, 0);
+        float v[3];
+        take(0, v);
+        g.sum(v);
+        stats(v[0], v[1], v[2]);
+        if (g.t == 0 && first + depth * step < p.m) issue(first + depth * step, 0);
+    }
+    for (int64_t row = first; row < p.m; row += step) {
+        wait(full_dz + slot * 8, phase);
+        const uint8_t* at = slots_dz + (size_t)slot * row_bytes;
+        f2 b[C][4], hat[C][4];
+        f2 sum_b = 0;
+        const f2 rz2 = splat2(rho_z), ry2 = splat2(rho_y), less_a1 = splat2(-a1);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (!has[c]) continue;
+            f2 dr[4], d[4], h[4], w[4];
+            slot8<T>(at, j[c], dr);
+            pairs8(rd[c], d);
+            pairs8(rz[c], h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[i] = mul2(h[i], rz2);
+                sum_c[c][i] = fma2(d[i], h[i], sum_c[c][i]);
+            }
+            vec8(v2, j[c], w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dr[i] = fma2(fma2(h[i], less_a1, mul2(d[i], w[i])), rz2, dr[i]);
+            if (q.dr) store8<T>(q.dr, row * q.lddr + j[c], dr);
+            pairs8(ry[c], hat[c]);
+            vec8(vp, j[c], w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hat[c][i] = mul2(hat[c][i], ry2);
+                sum_a[c][i] = fma2(dr[i], hat[c][i], sum_a[c][i]);
+                b[c][i] = mul2(dr[i], w[i]);
+                sum_b = fma2(b[c][i], hat[c][i], sum_b);
+            }
+        }
+        const int next = slot + 1 == depth ? 0 : slot + 1;
+        const uint32_t next_phase = next ? phase : phase ^ 1;
+        const bool more = row + step < p.m;
+        float t[3] = {0.0f, 0.0f, 0.0f};
+        if (more) {
+            wait(full + next * 8, next_phase);
+            take(next, t);
+        }
+        float v[4] = {t[0], t[1], t[2], both(sum_b)};
+        g.sum(v);
+        if (g.t == 0) {
+            if (row + depth * step < p.m) issue_dz(row + depth * step, slot);
+            if (row + (depth + 1) * step < p.m) issue(row + (depth + 1) * step, next);
+        }
+        if (q.dy) {
+            const f2 less_b1 = splat2(-v[3] * inv_n);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (has[c]) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) b[c][i] = mul2(fma2(hat[c][i], less_b1, b[c][i]), ry2);
+                    store8<T>(q.dy, row * q.lddy + j[c], b[c]);
+                }
+        }
+        stats(v[0], v[1], v[2]);
+        slot = next;
+        phase = next_phase;
+    }
+    if (!q.partials) return;
+    __syncthreads();  // the slots are all read
+    float* acc = reinterpret_cast<float*>(sm.slots);
+    join_sums<G>(g, q, acc, n, 0, sum_a, j, has);
+    join_sums<G>(g, q, acc, n, 2, sum_c, j, has);
 }
 
 struct ReduceP {
@@ -1162,6 +1366,8 @@ struct ReduceP {
 // in order: 148 parts one after another took 82 us at 8192 columns, all latency.
 __global__ void __launch_bounds__(512) column_kernel(ReduceP p) {
     __shared__ float sums[16][4][32];
+    pdl_wait();
+    pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t j = (int64_t)blockIdx.x * 32 + lane;
     float s[4] = {};
@@ -1193,6 +1399,8 @@ __global__ void __launch_bounds__(512) column_kernel(ReduceP p) {
 
 __global__ void __launch_bounds__(256) gate_one_kernel(const float* row, int64_t n, float* out) {
     __shared__ float red[8];
+    pdl_wait();
+    pdl_launch_dependents();
     float s = 0.0f;
     for (int64_t j = threadIdx.x; j < n; j += 256) s += row[j];
     s = block_sum(s, red);
@@ -1286,16 +1494,16 @@ bool rows_aligned(const BlockP& p, size_t es) {
 }
 
 template <typename T, int TPR, int C = 1>
-void launch_forward_rows(const BlockP& p, cudaStream_t st) {
+cudaError_t launch_forward_rows(bool pdl, const BlockP& p, cudaStream_t st) {
     constexpr int threads = cta_threads(TPR), rows = threads / TPR;
-    forward_rows_kernel<T, TPR, C><<<(unsigned)((p.m + rows - 1) / rows), threads, 0, st>>>(p);
+    return launch_k(pdl, forward_rows_kernel<T, TPR, C>, (unsigned)((p.m + rows - 1) / rows), threads, 0, st, p);
 }
 
 // Fills in the ring's shape; false where not even one slot a group fits.
 bool plan_ring(RingP* r, int64_t n, int groups, int tensors, size_t es, int vectors) {
     r->slot_bytes = (int)(tensors * n * (int64_t)es);
     r->vectors = vectors;
-    const int64_t room = kRingSmem - kRingScratch - (int64_t)vectors * n * 4;
+    const int64_t room = kRingSmem - ring_scratch(groups) - (int64_t)vectors * n * 4;
     r->depth = (int)std::min<int64_t>(4, room / ((int64_t)groups * r->slot_bytes));
     return r->depth >= 1;
 }
@@ -1308,7 +1516,7 @@ int launch_forward_ring(rt_ctx* ctx, const BlockP& p, RingP r, int mask, cudaStr
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
     auto* kernel = full ? forward_ring_kernel<T, TPR, C, true> : forward_ring_kernel<T, TPR, C, false>;
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    kernel<<<(unsigned)ctas, kRingThreads, kRingSmem, st>>>(p, r, mask);
+    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kRingThreads, kRingSmem, st, p, r, mask));
     return RT_OK;
 }
 
@@ -1338,7 +1546,14 @@ int launch_backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, const Rin
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
     auto* kernel = full ? backward_ring_kernel<T, TPR, true> : backward_ring_kernel<T, TPR, false>;
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    kernel<<<(unsigned)ctas, kBackThreads, kRingSmem, st>>>(p, q, r, mask);
+    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kBackThreads, kRingSmem, st, p, q, r, mask));
+    return RT_OK;
+}
+
+template <int TPR>
+int launch_backward_pipe(bool pdl, const BlockP& p, const GradP& q, const RingP& r, int ctas, cudaStream_t st) {
+    RT_CUDA(cudaFuncSetAttribute(backward_pipe_kernel<TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+    RT_CUDA(launch_k(pdl, backward_pipe_kernel<TPR>, (unsigned)ctas, kBackThreads, kRingSmem, st, p, q, r));
     return RT_OK;
 }
 
@@ -1363,6 +1578,18 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
         return RT_OK;
     *done = true;
     *parts = (int)std::min<int64_t>(ctx->sm_count, (p.m + groups - 1) / groups);
+    if constexpr (sizeof(T) == 2) {
+        RingP two{};
+        two.err = ctx->dev_err;
+        if (p.post.kind == RT_NORM_RMS && p.pre.kind == RT_NORM_RMS && q.dz && q.dh && !(q.sums & 10) &&
+            p.gate_mode != GATE_COLUMN && p.gate_mode != GATE_FULL && plan_ring(&two, p.n, groups, 4, es, 2) && two.depth >= 2) {
+            if (tpr == 32) return launch_backward_pipe<32>(ctx->pdl, p, q, two, *parts, st);
+            if (tpr == 64) return launch_backward_pipe<64>(ctx->pdl, p, q, two, *parts, st);
+            if (tpr == 128) return launch_backward_pipe<128>(ctx->pdl, p, q, two, *parts, st);
+            if (tpr == 256) return launch_backward_pipe<256>(ctx->pdl, p, q, two, *parts, st);
+            return launch_backward_pipe<512>(ctx->pdl, p, q, two, *parts, st);
+        }
+    }
     if (tpr == 32) return launch_backward_ring<T, 32>(ctx, p, q, r, mask, *parts, st);
     if (tpr == 64) return launch_backward_ring<T, 64>(ctx, p, q, r, mask, *parts, st);
     if (tpr == 128) return launch_backward_ring<T, 128>(ctx, p, q, r, mask, *parts, st);
@@ -1373,16 +1600,32 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
 // Up to 16384 wide: the fewest threads that hold a row eight elements each (the
 // widest rows, sixteen).
 template <typename T>
-bool forward_rows(const BlockP& p, cudaStream_t st) {
-    if (!rows_aligned(p, sizeof(T)) || p.n > 16384 || p.m > INT32_MAX) return false;
-    if (p.n <= 256) launch_forward_rows<T, 32>(p, st);
-    else if (p.n <= 512) launch_forward_rows<T, 64>(p, st);
-    else if (p.n <= 1024) launch_forward_rows<T, 128>(p, st);
-    else if (p.n <= 2048) launch_forward_rows<T, 256>(p, st);
-    else if (p.n <= 4096) launch_forward_rows<T, 512>(p, st);
-    else if (p.n <= 8192) launch_forward_rows<T, 1024>(p, st);
-    else launch_forward_rows<T, 1024, 2>(p, st);
-    return true;
+int forward_rows(rt_ctx* ctx, const BlockP& p, cudaStream_t st, bool* done) {
+    *done = false;
+    if (!rows_aligned(p, sizeof(T)) || p.n > 16384 || p.m > INT32_MAX) return RT_OK;
+    *done = true;
+    const bool pdl = ctx->pdl;
+    RT_CUDA(p.n <= 256    ? (launch_forward_rows<T, 32>(pdl, p, st))
+            : p.n <= 512  ? (launch_forward_rows<T, 64>(pdl, p, st))
+            : p.n <= 1024 ? (launch_forward_rows<T, 128>(pdl, p, st))
+            : p.n <= 2048 ? (launch_forward_rows<T, 256>(pdl, p, st))
+            : p.n <= 4096 ? (launch_forward_rows<T, 512>(pdl, p, st))
+            : p.n <= 8192 ? (launch_forward_rows<T, 1024>(pdl, p, st))
+                          : (launch_forward_rows<T, 1024, 2>(pdl, p, st)));
+    return RT_OK;
+}
+
+// The forward pass on the kernel that fits it.
+template <typename T>
+int forward_any(rt_ctx* ctx, const BlockP& p, cudaStream_t st) {
+    bool done = false;
+    RT_TRY(forward_ring<T>(ctx, p, st, &done));
+    if (!done) RT_TRY(forward_rows<T>(ctx, p, st, &done));
+    if (!done)
+        RT_CUDA(launch_k(ctx->pdl, forward_kernel<T>, (unsigned)std::min<int64_t>(p.m, (int64_t)ctx->sm_count * 8), 256, 0,
+                         st, p));
+    count_launch(ctx);
+    return RT_OK;
 }
 
 int parts_for(const rt_ctx* ctx, int64_t m) { return (int)std::max<int64_t>(1, std::min<int64_t>(m, ctx->sm_count)); }
@@ -1419,19 +1662,7 @@ int rt_block_forward(rt_ctx* ctx, const rt_block_args* a) {
     }
     if (p.m == 0 || p.n == 0) return RT_OK;
     RT_CUDA(cudaSetDevice(ctx->device));
-    const int grid = (int)std::min<int64_t>(p.m, (int64_t)ctx->sm_count * 8);
-    bool done = false;
-    RT_TRY(a->r->dtype == RT_BF16 ? forward_ring<__nv_bfloat16>(ctx, p, ctx->stream, &done)
-                                  : forward_ring<float>(ctx, p, ctx->stream, &done));
-    if (done) {
-    } else if (a->r->dtype == RT_BF16) {
-        if (!forward_rows<__nv_bfloat16>(p, ctx->stream)) forward_kernel<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(p);
-    } else {
-        if (!forward_rows<float>(p, ctx->stream)) forward_kernel<float><<<grid, 256, 0, ctx->stream>>>(p);
-    }
-    RT_CUDA(cudaGetLastError());
-    count_launch(ctx);
-    return RT_OK;
+    return a->r->dtype == RT_BF16 ? forward_any<__nv_bfloat16>(ctx, p, ctx->stream) : forward_any<float>(ctx, p, ctx->stream);
 }
 
 int64_t rt_block_backward_workspace(rt_ctx* ctx, int64_t m, int64_t n) {
@@ -1516,12 +1747,9 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     RT_TRY(z->dtype == RT_BF16 ? backward_ring<__nv_bfloat16>(ctx, p, q, ctx->stream, &parts, &done)
                                : backward_ring<float>(ctx, p, q, ctx->stream, &parts, &done));
     // without rows the sums over rows are zero: the partials of one CTA
-    if (done) {
-    } else if (z->dtype == RT_BF16)
-        backward_kernel<__nv_bfloat16><<<parts, 256, 0, ctx->stream>>>(p, q);
-    else
-        backward_kernel<float><<<parts, 256, 0, ctx->stream>>>(p, q);
-    RT_CUDA(cudaGetLastError());
+    if (!done)
+        RT_CUDA(launch_k(ctx->pdl, z->dtype == RT_BF16 ? backward_kernel<__nv_bfloat16> : backward_kernel<float>, parts, 256, 0,
+                         ctx->stream, p, q));
     count_launch(ctx);
     if (!q.sums) return RT_OK;
     c.partials = q.partials;
@@ -1534,12 +1762,10 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     c.gamma = p.post.gamma;
     c.beta = p.post.beta;
     if (gate_sums && p.gate_mode == GATE_ONE) c.gate_row = q.partials + (int64_t)parts_for(ctx, p.m) * 4 * p.n;
-    column_kernel<<<(unsigned)((p.n + 31) / 32), 512, 0, ctx->stream>>>(c);
-    RT_CUDA(cudaGetLastError());
+    RT_CUDA(launch_k(ctx->pdl, column_kernel, (unsigned)((p.n + 31) / 32), 512, 0, ctx->stream, c));
     count_launch(ctx);
     if (c.gate_row) {
-        gate_one_kernel<<<1, 256, 0, ctx->stream>>>(c.gate_row, p.n, c.dgate);
-        RT_CUDA(cudaGetLastError());
+        RT_CUDA(launch_k(ctx->pdl, gate_one_kernel, 1, 256, 0, ctx->stream, c.gate_row, p.n, c.dgate));
         count_launch(ctx);
     }
     return RT_OK;

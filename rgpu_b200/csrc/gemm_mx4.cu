@@ -252,6 +252,9 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_slot);
+    // a programmatic dependent launch: the set-up above touched no global memory
+    pdl_wait();
+    pdl_launch_dependents();
 
     if (warp == 0 && lane == 0) {
         int issued = 0;
@@ -553,6 +556,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     sync_cluster();
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_slot);
+    pdl_wait();
+    pdl_launch_dependents();
     auto raise_abort = [&](int code) {
         record_error(p.err, code, blockIdx.x);
         *abort_flag = 1;
@@ -698,6 +703,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
 
 // C = bias (k = 0).
 __global__ void bias_kernel(Mx4Params p) {
+    pdl_wait();
+    pdl_launch_dependents();
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.m * p.n; i += (int64_t)gridDim.x * blockDim.x)
         store_c(p, i / p.n, i % p.n, 0.0f, p.bias ? p.bias[i % p.n] : 0.0f);
 }
@@ -753,13 +760,15 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaS
     cfg.blockDim = dim3(kThreads1);
     cfg.dynamicSmemBytes = G::SMEM;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = splits;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = ctx->pdl ? 2 : 1;
     RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<TN>, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
@@ -789,13 +798,15 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cuda
     cfg.blockDim = dim3(kPairThreads);
     cfg.dynamicSmemBytes = kPairSmem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = ctx->pdl ? 2 : 1;
     RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_pair_kernel, w, t, sw, st, c, p));
     count_launch(ctx);
     return RT_OK;
@@ -831,8 +842,7 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
     p.err = ctx->dev_err;
     RT_CUDA(cudaSetDevice(ctx->device));
     if (p.blocks == 0) {
-        bias_kernel<<<ctx->sm_count * 4, 256, 0, stream>>>(p);
-        RT_CUDA(cudaGetLastError());
+        RT_CUDA(launch_k(ctx->pdl, bias_kernel, ctx->sm_count * 4, 256, 0, stream, p));
         count_launch(ctx);
         return RT_OK;
     }

@@ -12,6 +12,9 @@ namespace {
 
 using namespace mx4;
 
+// Every kernel here launches as a programmatic dependent of the one before it on
+// the stream (launch_k), and waits for it before touching memory.
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>
@@ -92,6 +95,8 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
                                                             int64_t k, Tasks w, int64_t blocks, int64_t groups,
                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < w.total; i += (int64_t)gridDim.x * 8) {
         int64_t chunk, row;
@@ -142,6 +147,8 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restri
                                                                int64_t k, int64_t blocks, int64_t groups,
                                                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     __shared__ uint32_t tile[128];
+    pdl_wait();
+    pdl_launch_dependents();
     constexpr int W = PAIR ? 2 : 1;  // columns of a thread
     const int64_t group = blockIdx.x % groups, col0 = blockIdx.x / groups * 128;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -215,6 +222,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
                                                          const uint8_t* __restrict__ scales, int64_t rows, int64_t k,
                                                          Tasks w, int64_t blocks, int64_t groups, T* __restrict__ dst,
                                                          int64_t ld) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < w.total; i += (int64_t)gridDim.x * 8) {
         int64_t chunk, row;
@@ -264,17 +273,17 @@ int launch_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_mx4* q) {
         const Tasks w = tasks_for(q->rows, q->k);
         const int grid = grid_for(ctx, w.total, 8);
         auto* kernel = aligned16(src) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-        kernel<<<grid, 256, 0, ctx->stream>>>(p, src->ld, q->rows, q->k, w, q->blocks(), q->groups(), q->codes, q->scales);
+        RT_CUDA(launch_k(ctx->pdl, kernel, grid, 256, 0, ctx->stream, p, src->ld, q->rows, q->k, w, q->blocks(),
+                         q->groups(), q->codes, q->scales));
     } else {
         const int64_t grid = q->groups() * ((q->rows + 127) / 128);
         RT_CHECK(grid <= INT_MAX, "rt_mx4_quantize: src is too large");
         auto* kernel = quantize_columns_kernel<T, false>;
         if constexpr (sizeof(T) == 2)
             if ((reinterpret_cast<uintptr_t>(p) & 3) == 0 && src->ld % 2 == 0) kernel = quantize_columns_kernel<T, true>;
-        kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(p, src->ld, q->rows, q->k, q->blocks(), q->groups(), q->codes,
-                                                        q->scales);
+        RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)grid, 256, 0, ctx->stream, p, src->ld, q->rows, q->k, q->blocks(),
+                         q->groups(), q->codes, q->scales));
     }
-    RT_CUDA(cudaGetLastError());
     count_launch(ctx);
     return RT_OK;
 }
@@ -284,9 +293,8 @@ int launch_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst) {
     const Tasks w = tasks_for(q->rows, q->k);
     const int grid = grid_for(ctx, w.total, 8);
     auto* kernel = aligned16(dst) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
-    kernel<<<grid, 256, 0, ctx->stream>>>(q->codes, q->scales, q->rows, q->k, w, q->blocks(), q->groups(),
-                                          static_cast<T*>(dst->ptr), dst->ld);
-    RT_CUDA(cudaGetLastError());
+    RT_CUDA(launch_k(ctx->pdl, kernel, grid, 256, 0, ctx->stream, q->codes, q->scales, q->rows, q->k, w, q->blocks(),
+                     q->groups(), static_cast<T*>(dst->ptr), dst->ld));
     count_launch(ctx);
     return RT_OK;
 }

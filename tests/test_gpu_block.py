@@ -40,7 +40,8 @@ class Case:
             g = b = None
             if vectors and kind != "none":
                 g = self._put("gamma_" + name, rng.standard_normal((1, n)) * 0.2 + 1.0, "f32")
-                b = self._put("beta_" + name, rng.standard_normal((1, n)) * 0.1, "f32")
+                if vectors != "gamma":
+                    b = self._put("beta_" + name, rng.standard_normal((1, n)) * 0.1, "f32")
             self.norms[name] = rgpu_b200.Norm(kind, EPS, g, b)
             self.ref[name] = (kind, EPS, self.host.get("gamma_" + name, np.ones((1, n))),
                               self.host.get("beta_" + name, np.zeros((1, n))))
@@ -143,6 +144,20 @@ def test_many_rows(gpu, m, n, kind, dtype):
         assert np.array_equal(gpu.download(a), gpu.download(b))
         if gate != "full":
             _backward_check(c, c.host["r"], _backward(gpu, c, c.dev["r"]), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n", [(1, 8), (3, 96), (2400, 104), (700, 504), (1000, 1000), (1300, 2048), (700, 4096), (450, 4104),
+                                 (299, 8192)])
+def test_rms_training_step(gpu, m, n, dtype):
+    # two RMS norms without betas and a gate that rows share: rows overlap in the backward pass
+    for gate in ("none", "one", "row"):
+        c = Case(gpu, m, n, dtype, "rms", "rms", gate, seed=m + n, vectors="gamma" if gate != "none" else False)
+        which = ("dr", "dy", "dgamma_post", "dgamma_pre", "dgate")
+        got = _backward(gpu, c, c.dev["r"], which=which)
+        _backward_check(c, c.host["r"], got, dtype)
+        some = _backward(gpu, c, c.dev["r"], which=("dr",))
+        assert torch.equal(some["dr"], got["dr"])
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
