@@ -620,6 +620,13 @@ __device__ __forceinline__ float both(f2 a) {
 
 // Eight elements as pairs: of a register's worth of bf16, of a slot's row, of a
 // vector in shared memory.
+__device__ __forceinline__ void pairs8(const Raw8<float>& r, f2 (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        v[2 * i] = pack2(__uint_as_float(r.u[i].x), __uint_as_float(r.u[i].y));
+        v[2 * i + 1] = pack2(__uint_as_float(r.u[i].z), __uint_as_float(r.u[i].w));
+    }
+}
 __device__ __forceinline__ void pairs8(const Raw8<__nv_bfloat16>& r, f2 (&v)[4]) {
     const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
 #pragma unroll
@@ -628,12 +635,10 @@ __device__ __forceinline__ void pairs8(const Raw8<__nv_bfloat16>& r, f2 (&v)[4])
 template <typename T>
 __device__ __forceinline__ void slot8(const uint8_t* row, int j, f2 (&v)[4]) {
     const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(row) + j);
-    if constexpr (sizeof(T) == 2) {
-        pairs8(Raw8<T>{{p[0]}}, v);
-    } else {
-        const ulonglong2 a = reinterpret_cast<const ulonglong2*>(p)[0], b = reinterpret_cast<const ulonglong2*>(p)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-    }
+    Raw8<T> raw;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw.u[i] = p[i];
+    pairs8(raw, v);
 }
 __device__ __forceinline__ void vec8(const float* p, int j, f2 (&v)[4]) {
     const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(p + j), b = *reinterpret_cast<const ulonglong2*>(p + j + 4);
@@ -900,11 +905,13 @@ __device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc
     }
 }
 
-template <typename T, int TPR, bool FULL>
+// C: eights of a thread.  With the betas' sums a thread of sixteen columns spills
+// (and with all of shared memory taken, spills go to L2), so FULL takes eight up
+// to 4096 wide: 2047 x 1000 f32 layer norms, full gate: 45 us with C = 2.
+template <typename T, int TPR, int C, bool FULL>
 __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p, GradP q, RingP r, int mask) {
     extern __shared__ __align__(128) uint8_t smem[];
     using G = Group<kBackThreads, TPR>;
-    constexpr int C = 2;
     const int n = (int)p.n;
     const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
     G g;
@@ -967,6 +974,11 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
             tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
         }
         const uint8_t* at = slots + (size_t)slot * r.slot_bytes;
+        Raw8<T> own[FULL ? C : 1];  // a full gate's row: under way while the sums are taken
+        if constexpr (FULL)
+            if (p.gate_mode == GATE_FULL)
+#pragma unroll
+                for (int c = 0; c < C; ++c) own[c] = has[c] ? load_raw8<T>(p.gate, row * p.ldg + j[c]) : zero8<T>();
         // sums of both norms: means first where there is a layer norm, then the
         // centred squares and a (z - mu)
         Stat sz{0.0f, 1.0f}, sy{0.0f, 1.0f};
@@ -1089,7 +1101,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = splat2(p.scale);
             }
-            if (own_gate) {
+            if constexpr (FULL) if (own_gate) {
                 // s u dr is the gate's gradient, and g dr takes the place of dr
                 f2 u[4], gate[4];
 #pragma unroll
@@ -1105,7 +1117,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                     sums[2] = add2(sums[2], u[i]);
                 }
                 if (p.gate_mode == GATE_FULL) {
-                    slot8<T>(reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.gate) + row * p.ldg), j[c], gate);
+                    pairs8(own[c], gate);
                     if (q.dgate) store8<T>(q.dgate, row * q.lddg + j[c], u);
                 } else {
                     const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
@@ -1540,11 +1552,9 @@ int forward_ring(rt_ctx* ctx, const BlockP& p, cudaStream_t st, bool* done) {
     return launch_forward_ring<T, 512, 2>(ctx, p, r, mask, st);
 }
 
-template <typename T, int TPR>
+template <typename T, int TPR, int C, bool FULL>
 int launch_backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, const RingP& r, int mask, int ctas, cudaStream_t st) {
-    const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
-                      p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
-    auto* kernel = full ? backward_ring_kernel<T, TPR, true> : backward_ring_kernel<T, TPR, false>;
+    auto* kernel = backward_ring_kernel<T, TPR, C, FULL>;
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
     RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kBackThreads, kRingSmem, st, p, q, r, mask));
     return RT_OK;
@@ -1570,7 +1580,11 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
     const bool shared = p.gate_mode == GATE_ONE || p.gate_mode == GATE_ROW;
     const int mask = (p.pre.gamma ? 1 : 0) | (p.post.gamma || (p.y && shared) ? 2 : 0) |
                      (p.post.beta && q.dgate && !shared ? 4 : 0);
-    const int tpr = p.n <= 512 ? 32 : p.n <= 1024 ? 64 : p.n <= 2048 ? 128 : p.n <= 4096 ? 256 : 512;
+    const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
+                      p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
+    const int eights = full && p.n <= 4096 ? 1 : 2;
+    int tpr = 32;
+    while (tpr * eights * 8 < p.n) tpr *= 2;
     const int groups = kBackThreads / tpr;
     RingP r{};
     r.err = ctx->dev_err;
@@ -1581,20 +1595,32 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
     if constexpr (sizeof(T) == 2) {
         RingP two{};
         two.err = ctx->dev_err;
-        if (p.post.kind == RT_NORM_RMS && p.pre.kind == RT_NORM_RMS && q.dz && q.dh && !(q.sums & 10) &&
-            p.gate_mode != GATE_COLUMN && p.gate_mode != GATE_FULL && plan_ring(&two, p.n, groups, 4, es, 2) && two.depth >= 2) {
-            if (tpr == 32) return launch_backward_pipe<32>(ctx->pdl, p, q, two, *parts, st);
-            if (tpr == 64) return launch_backward_pipe<64>(ctx->pdl, p, q, two, *parts, st);
-            if (tpr == 128) return launch_backward_pipe<128>(ctx->pdl, p, q, two, *parts, st);
-            if (tpr == 256) return launch_backward_pipe<256>(ctx->pdl, p, q, two, *parts, st);
-            return launch_backward_pipe<512>(ctx->pdl, p, q, two, *parts, st);
+        if (!full && p.post.kind == RT_NORM_RMS && p.pre.kind == RT_NORM_RMS && q.dz && q.dh &&
+            plan_ring(&two, p.n, groups, 4, es, 2) && two.depth >= 2) {
+            switch (tpr) {
+                case 32: return launch_backward_pipe<32>(ctx->pdl, p, q, two, *parts, st);
+                case 64: return launch_backward_pipe<64>(ctx->pdl, p, q, two, *parts, st);
+                case 128: return launch_backward_pipe<128>(ctx->pdl, p, q, two, *parts, st);
+                case 256: return launch_backward_pipe<256>(ctx->pdl, p, q, two, *parts, st);
+                default: return launch_backward_pipe<512>(ctx->pdl, p, q, two, *parts, st);
+            }
         }
     }
-    if (tpr == 32) return launch_backward_ring<T, 32>(ctx, p, q, r, mask, *parts, st);
-    if (tpr == 64) return launch_backward_ring<T, 64>(ctx, p, q, r, mask, *parts, st);
-    if (tpr == 128) return launch_backward_ring<T, 128>(ctx, p, q, r, mask, *parts, st);
-    if (tpr == 256) return launch_backward_ring<T, 256>(ctx, p, q, r, mask, *parts, st);
-    return launch_backward_ring<T, 512>(ctx, p, q, r, mask, *parts, st);
+    if (!full) switch (tpr) {
+            case 32: return launch_backward_ring<T, 32, 2, false>(ctx, p, q, r, mask, *parts, st);
+            case 64: return launch_backward_ring<T, 64, 2, false>(ctx, p, q, r, mask, *parts, st);
+            case 128: return launch_backward_ring<T, 128, 2, false>(ctx, p, q, r, mask, *parts, st);
+            case 256: return launch_backward_ring<T, 256, 2, false>(ctx, p, q, r, mask, *parts, st);
+            default: return launch_backward_ring<T, 512, 2, false>(ctx, p, q, r, mask, *parts, st);
+        }
+    if (eights == 2) return launch_backward_ring<T, 512, 2, true>(ctx, p, q, r, mask, *parts, st);
+    switch (tpr) {
+        case 32: return launch_backward_ring<T, 32, 1, true>(ctx, p, q, r, mask, *parts, st);
+        case 64: return launch_backward_ring<T, 64, 1, true>(ctx, p, q, r, mask, *parts, st);
+        case 128: return launch_backward_ring<T, 128, 1, true>(ctx, p, q, r, mask, *parts, st);
+        case 256: return launch_backward_ring<T, 256, 1, true>(ctx, p, q, r, mask, *parts, st);
+        default: return launch_backward_ring<T, 512, 1, true>(ctx, p, q, r, mask, *parts, st);
+    }
 }
 
 // Up to 16384 wide: the fewest threads that hold a row eight elements each (the
