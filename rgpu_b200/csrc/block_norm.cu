@@ -388,9 +388,7 @@ __device__ __forceinline__ void store_h(const BlockP& p, int64_t row, int j, boo
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const uint32_t byte = mx4::scale_byte(amax);
     const float inv = mx4::inv_scale(byte);
-    uint32_t code = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) code |= mx4::encode2(h[i] * inv, h[i + 1] * inv) << (4 * i);
+    uint32_t code = mx4::encode8(h, inv);
     if (byte == mx4::kNanScale) code = 0;
     if (live && j < blocks * 32) *reinterpret_cast<uint32_t*>(p.codes + row * blocks * 16 + (j >> 1)) = code;
     // the scales of a group's four blocks as one word

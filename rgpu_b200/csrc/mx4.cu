@@ -3,8 +3,6 @@
 #include <climits>
 #include <new>
 
-#include <cuda_fp16.h>
-
 #include "mx4.cuh"
 
 namespace rt {
@@ -22,119 +20,164 @@ __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Eight elements of a row from p (those at `left` and after read as 0), as f32.
-// VEC: p is 16-byte aligned.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
-    if (VEC && left >= 8) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        } else {
-            const float4 x = __ldg(reinterpret_cast<const float4*>(p)), y = __ldg(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-            v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32<T>(p[i]) : 0.0f;
-    }
-}
+// A lane's piece of a row: 32 bytes, 16 bf16 or 8 f32.  V: bytes of an access, 32
+// (one 256-bit access, Blackwell's widest) or 16 where the rows are so aligned,
+// else 0: element by element, as at a row's end.
+template <typename T>
+struct Piece {
+    static constexpr int E = 32 / sizeof(T);         // elements
+    static constexpr int PER_BLOCK = 32 / E;         // lanes that share a block
+    static constexpr int PER_GROUP = 128 / E;        // and a scale group
+    static constexpr int WARP = 32 * E;              // elements of a warp
+    uint32_t w[8];
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int64_t left, const float (&v)[8]) {
-    if (VEC && left >= 8) {
-        if constexpr (sizeof(T) == 2) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    template <int V>
+    __device__ __forceinline__ void load(const T* p, int64_t left) {
+        if (V == 32 && left >= E) {
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(p));
+        } else if (V == 16 && left >= E) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
         } else {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            *(reinterpret_cast<float4*>(p) + 1) = make_float4(v[4], v[5], v[6], v[7]);
-        }
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) {
-                if constexpr (sizeof(T) == 2)
-                    p[i] = __float2bfloat16_rn(v[i]);
-                else
-                    p[i] = v[i];
-            }
+            for (int i = 0; i < 8; ++i) w[i] = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < left) {
+                    if constexpr (sizeof(T) == 2)
+                        w[e / 2] |= (uint32_t)__bfloat16_as_ushort(p[e]) << (16 * (e & 1));
+                    else
+                        w[e] = __float_as_uint(p[e]);
+                }
+        }
     }
-}
-
-// Blocks along a row.  A warp takes 256 elements (two scale groups) of the four
-// rows r, r + 32, r + 64, r + 96 of a 128-row tile: the scales of these rows lie
-// side by side, 16 bytes for a group, and every lane has four independent reads
-// of 16 (f32: 32) bytes under way.  A lane encodes 8 elements of each row to 4
-// bytes; the four lanes of a block find its largest magnitude by shuffles.
-// HBM-bound: 2 (f32: 4) bytes in and 17/32 out per element.
-struct Tasks {
-    int64_t total;   // warps' worth of work
-    int64_t chunks;  // of 256 elements along k
-    int rcount;      // rows r of a tile: 32, or fewer where the matrix has fewer
+    template <int V>
+    __device__ __forceinline__ void store(T* p, int64_t left) const {
+        if (V == 32 && left >= E) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                         "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        } else if (V == 16 && left >= E) {
+            reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < left) {
+                    if constexpr (sizeof(T) == 2)
+                        p[e] = __ushort_as_bfloat16((unsigned short)(w[e / 2] >> (16 * (e & 1))));
+                    else
+                        p[e] = __uint_as_float(w[e]);
+                }
+        }
+    }
+    // Bit pattern (as f32) of the largest magnitude in the lane.
+    __device__ __forceinline__ uint32_t amax() const {
+        uint32_t m = 0;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+            return max(m << 16, m & 0xffff0000u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+            return m;
+        }
+    }
+    // Codes of the elements 8 i .. 8 i + 7.
+    __device__ __forceinline__ uint32_t encode(int i, float inv) const {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (sizeof(T) == 2) {
+                const uint32_t x = w[i * 4 + e / 2];
+                v[e] = __uint_as_float(e & 1 ? x & 0xffff0000u : x << 16);
+            } else {
+                v[e] = __uint_as_float(w[e]);
+            }
+        }
+        return encode8(v, inv);
+    }
 };
 
-__device__ __forceinline__ void task_at(const Tasks& w, int64_t i, int64_t& chunk, int64_t& row) {
-    chunk = i % w.chunks;
-    const int64_t q = i / w.chunks;
-    row = q / w.rcount * 128 + q % w.rcount;
+// Blocks along a row.  A warp takes 512 (f32: 256) elements of the four rows r,
+// r + 32, r + 64, r + 96 of a 128-row tile: the scales of these rows lie side by
+// side, 16 bytes for a group, and every lane has four 32-byte reads under way.  Few
+// lanes to a block keep the instructions per element low enough for HBM to be the
+// bound: 2 (f32: 4) bytes in and 17/32 out per element.
+struct Rows {
+    int64_t sets;  // sets of four rows
+    int rcount;    // rows r of a tile: 32, or fewer where the matrix has fewer
+    int chunks;    // warps' worth of elements along k
+    int split;     // log2 of the warps of a CTA that lie along k; the others take other sets
+};
+
+// The warp's first chunk along k and first set, and the grid's strides.
+struct Place {
+    int chunk, chunk_step;
+    int64_t set, set_step;
+    __device__ __forceinline__ explicit Place(const Rows& w) {
+        const int warp = threadIdx.x >> 5;
+        chunk = ((int)blockIdx.x << w.split) + (warp & ((1 << w.split) - 1));
+        chunk_step = (int)gridDim.x << w.split;
+        set = ((int64_t)blockIdx.y << (3 - w.split)) + (warp >> w.split);
+        set_step = (int64_t)gridDim.y << (3 - w.split);
+    }
+};
+// First row of a set.
+__device__ __forceinline__ int64_t set_row(const Rows& w, int64_t set) {
+    return w.rcount == 32 ? (set >> 5) * 128 + (set & 31) : set;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
-                                                            int64_t k, Tasks w, int64_t blocks, int64_t groups,
-                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+template <typename T, int V>
+__global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
+                                                               int64_t k, Rows w, int64_t blocks, int64_t groups,
+                                                               uint8_t* __restrict__ codes,
+                                                               uint8_t* __restrict__ scales) {
+    using P = Piece<T>;
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < w.total; i += (int64_t)gridDim.x * 8) {
-        int64_t chunk, row;
-        task_at(w, i, chunk, row);
-        const int64_t j = chunk * 256 + lane * 8;
-        float v[4][8];
+    const int64_t row_bytes = blocks * 16;
+    const Place at(w);
+    for (int64_t set = at.set; set < w.sets; set += at.set_step)
+        for (int chunk = at.chunk; chunk < w.chunks; chunk += at.chunk_step) {
+            const int64_t row = set_row(w, set), j = (int64_t)chunk * P::WARP + lane * P::E;
+            const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);  // rows of the set that there are
+            const T* p = src + row * ld + j;
+            P x[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (row + 32 * q < rows)
-                load8<T, VEC>(src + (row + 32 * q) * ld + j, k - j, v[q]);
-            else
+            for (int q = 0; q < 4; ++q) x[q].template load<V>(p + q * (32 * ld), q < live ? k - j : 0);
+            uint32_t word[4];
+            uint8_t* out = codes + row * row_bytes + (j >> 1);
+            const bool inside = j < blocks * 32;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[q][e] = 0.0f;
-        uint32_t word[4];
+            for (int q = 0; q < 4; ++q) {
+                uint32_t amax = x[q].amax();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint32_t amax = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(v[q][e]) & 0x7fffffffu);
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const uint32_t byte = scale_byte(amax);
-            const float inv = inv_scale(byte);
-            uint32_t c = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) c |= encode2(v[q][e] * inv, v[q][e + 1] * inv) << (4 * e);
-            if (byte == kNanScale) c = 0;
-            if (row + 32 * q < rows && j < blocks * 32)
-                *reinterpret_cast<uint32_t*>(codes + (row + 32 * q) * blocks * 16 + (j >> 1)) = c;
-            // the bytes of a group's four blocks into its first lane
-            word[q] = byte | __shfl_down_sync(0xffffffffu, byte, 4) << 8;
-            word[q] |= __shfl_down_sync(0xffffffffu, word[q], 8) << 16;
+                for (int o = 1; o < P::PER_BLOCK; o *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                const uint32_t byte = scale_byte(amax);
+                const float inv = inv_scale(byte);
+                const bool nan = byte == kNanScale;
+                if (q < live && inside) {
+                    if constexpr (sizeof(T) == 2)
+                        *reinterpret_cast<uint2*>(out + q * (32 * row_bytes)) =
+                            make_uint2(nan ? 0u : x[q].encode(0, inv), nan ? 0u : x[q].encode(1, inv));
+                    else
+                        *reinterpret_cast<uint32_t*>(out + q * (32 * row_bytes)) = nan ? 0u : x[q].encode(0, inv);
+                }
+                // the bytes of a group's four blocks into its first lane
+                word[q] = byte | __shfl_down_sync(0xffffffffu, byte, P::PER_BLOCK) << 8;
+                word[q] |= __shfl_down_sync(0xffffffffu, word[q], 2 * P::PER_BLOCK) << 16;
+            }
+            const int64_t group = j >> 7;
+            if (lane % P::PER_GROUP == 0 && group < groups)
+                *reinterpret_cast<uint4*>(scales + ((row >> 7) * groups + group) * 512 + (row & 31) * 16) =
+                    make_uint4(word[0], word[1], word[2], word[3]);
         }
-        const int64_t group = chunk * 2 + (lane >> 4);
-        if ((lane & 15) == 0 && group < groups)
-            *reinterpret_cast<uint4*>(scales + ((row >> 7) * groups + group) * 512 + (row & 31) * 16) =
-                make_uint4(word[0], word[1], word[2], word[3]);
-    }
 }
 
 // Blocks down a column, laid out transposed.  A CTA takes one scale tile: 128
@@ -186,9 +229,14 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restri
             for (int i = 0; i < 32; ++i) amax = max(amax, __float_as_uint(v[x][i]) & 0x7fffffffu);
             const uint32_t byte = scale_byte(amax);
             const float inv = inv_scale(byte);
-            uint32_t out[4] = {0, 0, 0, 0};
+            uint32_t out[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) out[i / 8] |= encode2(v[x][i] * inv, v[x][i + 1] * inv) << (4 * (i % 8));
+            for (int i = 0; i < 4; ++i) {
+                float e[8];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) e[y] = v[x][i * 8 + y];
+                out[i] = encode8(e, inv);
+            }
             if (byte == kNanScale) out[0] = out[1] = out[2] = out[3] = 0;
             if (block < blocks && col + x < rows)
                 *reinterpret_cast<uint4*>(codes + (col + x) * blocks * 16 + block * 16) =
@@ -202,77 +250,109 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restri
         reinterpret_cast<uint32_t*>(scales + (col0 / 128 * groups + group) * 512)[threadIdx.x] = tile[threadIdx.x];
 }
 
-// 8 codes (element i in bits 4i) to f32.
-__device__ __forceinline__ void decode8(uint32_t c, float scale, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t h;  // two halves
-        asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(h) : "r"((c >> (8 * i)) & 255u));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        v[2 * i] = f.x * scale;
-        v[2 * i + 1] = f.y * scale;
+// Codes to values.  The bits s e e m of a code, put where bf16 has its sign, its
+// lowest exponent bits and its first mantissa bit, are the value times 2^-126
+// (bf16's subnormals hold 0.5 too); two exact products with powers of two make up
+// for that and the scale.
+struct Unit {
+    uint32_t a, b;  // f32 patterns, a b = 2^126 scale: 2^(byte - 1) up to 2^127, and the rest
+    __device__ __forceinline__ explicit Unit(uint32_t byte) {
+        a = byte == kNanScale ? 0x7fc00000u : min(byte + 126u, 254u) << 23;
+        b = (byte > 128u ? byte - 1u : 127u) << 23;
     }
+};
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// The same tasks as quantize_rows_kernel, the other way.  bf16 holds every value
-// exactly: two significant bits, exponents 2^-128 to 2^130 (an overflow is the
-// same infinity in f32).  HBM-bound: 17/32 bytes in, 2 (f32: 4) out per element.
-template <typename T, bool VEC>
+// The rows of quantize_rows_kernel, the other way.  bf16 holds every value exactly:
+// two significant bits, exponents 2^-128 to 2^129 (past 2^128 the same infinity as
+// in f32).  HBM-bound: 17/32 bytes in, 2 (f32: 4) out per element.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, int64_t rows, int64_t k,
-                                                         Tasks w, int64_t blocks, int64_t groups, T* __restrict__ dst,
+                                                         Rows w, int64_t blocks, int64_t groups, T* __restrict__ dst,
                                                          int64_t ld) {
+    using P = Piece<T>;
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < w.total; i += (int64_t)gridDim.x * 8) {
-        int64_t chunk, row;
-        task_at(w, i, chunk, row);
-        const int64_t j = chunk * 256 + lane * 8;
-        if (j >= k) continue;
-        const uint4 s = __ldg(reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j >> 7)) * 512 + (row & 31) * 16));
-        const uint32_t word[4] = {s.x, s.y, s.z, s.w};
-        uint32_t c[4];
+    const int64_t row_bytes = blocks * 16;
+    const Place at(w);
+    for (int64_t set = at.set; set < w.sets; set += at.set_step)
+        for (int chunk = at.chunk; chunk < w.chunks; chunk += at.chunk_step) {
+            const int64_t row = set_row(w, set), j = (int64_t)chunk * P::WARP + lane * P::E;
+            if (j >= k) continue;
+            const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);
+            const uint4 s = __ldg(reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j >> 7)) * 512 + (row & 31) * 16));
+            const uint32_t word[4] = {s.x, s.y, s.z, s.w};
+            const uint8_t* in = codes + row * row_bytes + (j >> 1);
+            uint32_t c[4][P::E / 8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (row + 32 * q < rows)
-                c[q] = __ldg(reinterpret_cast<const uint32_t*>(codes + (row + 32 * q) * blocks * 16 + (j >> 1)));
+            for (int q = 0; q < 4; ++q)
+                if (q < live) {
+                    if constexpr (sizeof(T) == 2) {
+                        const uint2 two = __ldg(reinterpret_cast<const uint2*>(in + q * (32 * row_bytes)));
+                        c[q][0] = two.x;
+                        c[q][P::E / 8 - 1] = two.y;
+                    } else {
+                        c[q][0] = __ldg(reinterpret_cast<const uint32_t*>(in + q * (32 * row_bytes)));
+                    }
+                }
+            const int shift = (int)(j >> 5 & 3) * 8;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (row + 32 * q < rows) {
-                float v[8];
-                decode8(c[q], scale_value((word[q] >> (8 * ((j >> 5) & 3))) & 255u), v);
-                store8<T, VEC>(dst + (row + 32 * q) * ld + j, k - j, v);
+            for (int q = 0; q < 4; ++q) {
+                if (q >= live) break;
+                const Unit u((word[q] >> shift) & 255u);
+                P x;
+#pragma unroll
+                for (int i = 0; i < P::E / 2; ++i) {
+                    // two codes to two bf16 patterns
+                    const uint32_t two = c[q][i / 4] >> (8 * (i & 3)) & 255u, y = two | two << 12;
+                    const uint32_t h = (y & 0x00070007u) << 6 | (y & 0x00080008u) << 12;
+                    if constexpr (sizeof(T) == 2) {
+                        x.w[i] = mul_bf16x2(mul_bf16x2(h, u.a | u.a >> 16), u.b | u.b >> 16);
+                    } else {
+                        x.w[2 * i] = __float_as_uint(__uint_as_float(h << 16) * __uint_as_float(u.a) * __uint_as_float(u.b));
+                        x.w[2 * i + 1] = __float_as_uint(__uint_as_float(h & 0xffff0000u) * __uint_as_float(u.a) * __uint_as_float(u.b));
+                    }
+                }
+                x.template store<V>(dst + (row + 32 * q) * ld + j, k - j);
             }
-    }
+        }
 }
 
-// CTAs for `items` of `per_cta` each: all of them, or as many as the kernels' loops
-// share out evenly enough.
-int grid_for(const rt_ctx* ctx, int64_t items, int per_cta) {
-    const int64_t want = (items + per_cta - 1) / per_cta;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)ctx->sm_count * 64));
-}
-
-Tasks tasks_for(int64_t rows, int64_t k) {
-    Tasks w;
-    w.chunks = (k + 255) / 256;
+// Sets and chunks, and a grid that covers chunks before sets.
+Rows rows_for(const rt_ctx* ctx, int64_t rows, int64_t k, int chunk, dim3* grid) {
+    Rows w;
     w.rcount = (int)std::min<int64_t>(rows, 32);
-    w.total = w.chunks * w.rcount * ((rows + 127) / 128);
+    w.sets = w.rcount * ((rows + 127) / 128);
+    w.chunks = (int)((k + chunk - 1) / chunk);
+    w.split = w.chunks > 4 ? 3 : w.chunks > 2 ? 2 : w.chunks > 1 ? 1 : 0;
+    const int64_t along = (w.chunks + (1 << w.split) - 1) >> w.split;
+    const int64_t across = (w.sets + (8 >> w.split) - 1) >> (3 - w.split), limit = (int64_t)ctx->sm_count * 64;
+    grid->x = (unsigned)std::min(along, limit);
+    grid->y = (unsigned)std::min<int64_t>(std::min(across, std::max<int64_t>(1, limit / grid->x)), 65535);
+    grid->z = 1;
     return w;
 }
 
-bool aligned16(const rt_tensor* t) {
-    return ((reinterpret_cast<uintptr_t>(t->ptr) | (uintptr_t)(t->ld * dtype_size(t->dtype))) & 15) == 0;
+// Widest access that every row of t allows: 32, 16 or 0.
+int access_of(const rt_tensor* t) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t->ptr) | (uintptr_t)(t->ld * (int64_t)dtype_size(t->dtype));
+    return (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 0;
 }
 
 template <typename T>
 int launch_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_mx4* q) {
     const T* p = static_cast<const T*>(src->ptr);
     if (axis == 1) {
-        const Tasks w = tasks_for(q->rows, q->k);
-        const int grid = grid_for(ctx, w.total, 8);
-        auto* kernel = aligned16(src) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
+        dim3 grid;
+        const Rows w = rows_for(ctx, q->rows, q->k, Piece<T>::WARP, &grid);
+        const int v = access_of(src);
+        auto* kernel = v == 32 ? quantize_rows_kernel<T, 32> : v == 16 ? quantize_rows_kernel<T, 16> : quantize_rows_kernel<T, 0>;
         RT_CUDA(launch_k(ctx->pdl, kernel, grid, 256, 0, ctx->stream, p, src->ld, q->rows, q->k, w, q->blocks(),
                          q->groups(), q->codes, q->scales));
     } else {
@@ -290,9 +370,10 @@ int launch_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_mx4* q) {
 
 template <typename T>
 int launch_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst) {
-    const Tasks w = tasks_for(q->rows, q->k);
-    const int grid = grid_for(ctx, w.total, 8);
-    auto* kernel = aligned16(dst) ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
+    dim3 grid;
+    const Rows w = rows_for(ctx, q->rows, q->k, Piece<T>::WARP, &grid);
+    const int v = access_of(dst);
+    auto* kernel = v == 32 ? dequantize_kernel<T, 32> : v == 16 ? dequantize_kernel<T, 16> : dequantize_kernel<T, 0>;
     RT_CUDA(launch_k(ctx->pdl, kernel, grid, 256, 0, ctx->stream, q->codes, q->scales, q->rows, q->k, w, q->blocks(),
                      q->groups(), static_cast<T*>(dst->ptr), dst->ld));
     count_launch(ctx);

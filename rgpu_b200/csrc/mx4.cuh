@@ -45,6 +45,22 @@ __device__ __forceinline__ uint32_t encode2(float lo, float hi) {
     return r;
 }
 
+// Eight elements to eight codes (element i in bits
+// 4i), each times `inv`.
+__device__ __forceinline__ uint32_t encode8(const float (&v)[8], float inv) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
+          "f"(v[6] * inv), "f"(v[7] * inv));
+    return r;
+}
+
 // Byte offset of the scale of (row, block) in a matrix of `groups` scale
 // tiles along k.
 __device__ __forceinline__ int64_t scale_offset(int64_t row, int64_t block, int64_t groups) {
