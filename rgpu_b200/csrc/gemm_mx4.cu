@@ -188,30 +188,72 @@ __device__ __forceinline__ void store_c4(const Mx4Params& p, int64_t row, int64_
     }
 }
 
+// Adds the splits' sums of a tile in order and stores C.  Each of `splits` CTAs of
+// the cluster (ranks `stride` apart from `offset` on) holds [token][128 columns] f32
+// at `sums` of its shared memory; the tokens are dealt out over the splits (this one
+// is number `split`) and their warps.  A lane takes four columns; four tokens are
+// under way at a time, since a read from another SM takes most of a microsecond.
+__device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t stride,
+                                           uint32_t offset, uint32_t split, int warp, int warps, int64_t row0, int count,
+                                           int64_t col, int lane) {
+    constexpr int U = 4;
+    float bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? p.bias[col + i] : 0.0f;
+    const int step = warps * (int)splits;
+    for (int c = (int)split + warp * (int)splits; c < count; c += U * step) {
+        float4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+        for (uint32_t r = 0; r < splits; ++r) {
+            const uint32_t at = in_cta(sums + lane * 16, offset + r * stride);
+            float4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c + u * step < count) x[u] = ld_cluster4(at + (c + u * step) * 512);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c + u * step < count) {
+                    v[u].x += x[u].x;
+                    v[u].y += x[u].y;
+                    v[u].z += x[u].z;
+                    v[u].w += x[u].w;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c + u * step < count) store_c4(p, row0 + c + u * step, col, v[u], bias);
+    }
+}
+
 // ------------------------------------------------------------ one-CTA kernel
 // A CTA computes 128 columns of C for TN tokens over its share of k; the CTAs of
 // a cluster share one tile, split along k.  Their sums meet in shared memory and
 // are added in rank order, tokens dealt out over the CTAs.
-template <int TN>
+// STAGES: a short ring for two CTAs to an SM, or one that fills the SM's shared
+// memory for one: a stage takes over a microsecond to arrive, so the ring's depth
+// sets the pace of a CTA.
+template <int TN, bool DEEP>
 struct Geo1 {
     static constexpr int T_BYTES = TN * kRowBytes;
     static constexpr int STAGE_BYTES = kWBytes + T_BYTES + 4 * kScaleTile;  // codes, two scale tiles of either side
-    static constexpr int STAGES = TN <= 64 ? 4 : 3;
-    static constexpr int TMEM_COLS = TN <= 64 ? 128 : 256;  // TN, and 16 of scales a stage
+    static constexpr int STAGES = !DEEP ? 4 : TN == 32 ? 10 : 8;
+    static constexpr int TMEM_COLS = DEEP ? 256 : 128;  // TN, and 16 of scales a stage
     static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
     static_assert(TN + 16 * STAGES <= TMEM_COLS, "TMEM columns");
-    static_assert(2 * SMEM <= 226 * 1024, "two CTAs to an SM");
+    static_assert((DEEP ? 1 : 2) * SMEM <= 226 * 1024, "CTAs to an SM");
     static_assert(TN * 512 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
 };
 
 constexpr int kThreads1 = 192;  // warps: 0 TMA, 1 MMA, 2-5 epilogue (one TMEM lane quadrant each)
 
-template <int TN>
+template <int TN, bool DEEP>
 __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ CUtensorMap map_w,
                                                         const __grid_constant__ CUtensorMap map_t,
                                                         const __grid_constant__ CUtensorMap map_sw,
                                                         const __grid_constant__ CUtensorMap map_st, Mx4Params p) {
-    using G = Geo1<TN>;
+    using G = Geo1<TN, DEEP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* smem_w = smem;
@@ -355,29 +397,9 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     if (ranks > 1) {
         sync_cluster();
         if (warp >= 2) {
-            // a lane adds four columns of a token over the ranks; the warps take the tokens of this rank in turn
-            const int64_t row0 = (int64_t)tm * TN, col = (int64_t)tn * 128 + lane * 4;
-            const int count = (int)min((int64_t)TN, p.m - row0);
-            const uint32_t at = smem_u32(smem) + lane * 16;
-            float bias[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? p.bias[col + i] : 0.0f;
-            for (int c = (int)rank + (warp - 2) * (int)ranks; c < count; c += 4 * (int)ranks) {
-                float4 part[8];
-#pragma unroll
-                for (uint32_t r = 0; r < 8; ++r)
-                    if (r < ranks) part[r] = ld_cluster4(in_cta(at + c * 512, r));
-                float4 v = part[0];
-#pragma unroll
-                for (uint32_t r = 1; r < 8; ++r)
-                    if (r < ranks) {
-                        v.x += part[r].x;
-                        v.y += part[r].y;
-                        v.z += part[r].z;
-                        v.w += part[r].w;
-                    }
-                store_c4(p, row0 + c, col, v, bias);
-            }
+            const int64_t row0 = (int64_t)tm * TN;
+            add_splits(p, smem_u32(smem), ranks, 1, 0, rank, warp - 2, 4, row0, (int)min((int64_t)TN, p.m - row0),
+                       (int64_t)tn * 128 + lane * 4, lane);
         }
         sync_cluster();  // the sums are read before any CTA exits
     }
@@ -410,6 +432,7 @@ constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of W and T, two tiles of W's scales, four of T's
 constexpr int kChunkBytes = 32 * 128 * 2;  // staged output of either half of the tokens: 128 columns of 32 (f32: 16) tokens
 constexpr int kPairSmem = kPairStages * kPairStageBytes + 2 * kChunkBytes + 256;
+static_assert(256 * 512 <= kPairStages * kPairStageBytes, "the split sums reuse the stages");
 constexpr int kPairThreads = 320;  // warps: 0 TMA, 1 MMA (leader), 2-9 epilogue (two to a TMEM lane quadrant)
 static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
 static_assert(256 + 24 * kPairStages <= 512, "TMEM columns");
@@ -524,9 +547,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     volatile int* issued_all = abort_flag + 1;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const uint32_t rank = cta_rank();
-    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+    // a cluster is one pair, or the pairs of a tile's splits along k
+    const uint32_t cluster_rank = cta_rank(), ctas = cluster_size();
+    const uint32_t rank = cluster_rank & 1, leader = cluster_rank & ~1u, split = cluster_rank >> 1, splits = ctas >> 1;
+    const int cluster = (int)(blockIdx.x / ctas), clusters = (int)(gridDim.x / ctas);
     const int tiles = p.tiles_m * p.tiles_n;
+    const int s0 = (int)split * p.stages_per_split, s1 = min(p.stages, s0 + p.stages_per_split);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -561,7 +587,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     auto raise_abort = [&](int code) {
         record_error(p.err, code, blockIdx.x);
         *abort_flag = 1;
-        store_cluster(in_cta(smem_u32((const void*)abort_flag), rank ^ 1u), 1u);
+        store_cluster(in_cta(smem_u32((const void*)abort_flag), cluster_rank ^ 1u), 1u);
     };
 
     if (warp == 0 && lane == 0) {
@@ -570,14 +596,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         for (int t = cluster; t < tiles && ok; t += clusters) {
             int tm, tn;
             pair_tile(p, t, tm, tn);
-            for (int s = 0; s < p.stages; ++s) {
+            for (int s = s0; s < s1; ++s) {
                 const int slot = issued % S;
                 if (!mbar_wait(smem_u32(&empty[slot]), ((issued / S) & 1) ^ 1, abort_flag)) {
                     ok = false;
                     break;
                 }
                 if (rank == 0) mbar_expect_tx(smem_u32(&full[slot]), 2 * kPairStageBytes);
-                const uint32_t bar = in_cta(smem_u32(&full[slot]), 0);
+                const uint32_t bar = in_cta(smem_u32(&full[slot]), leader);
                 tma_pair_2d(smem_u32(smem_w + slot * kWBytes), &map_w, s * kRowBytes, tn * 256 + (int)rank * 128, bar);
                 tma_pair_2d(smem_u32(smem_t + slot * kWBytes), &map_t, s * kRowBytes, tm * 256 + (int)rank * 128, bar);
                 const uint32_t ss = smem_u32(smem_s + slot * 6 * kScaleTile);
@@ -591,15 +617,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     } else if (warp == 1 && rank == 0) {
         const uint64_t w0 = smem_desc(smem_u32(smem_w), 16, 1024), t0 = smem_desc(smem_u32(smem_t), 16, 1024);
         const uint64_t sc0 = scale_desc(smem_u32(smem_s));
-        const uint32_t empty0 = smem_u32(empty), empty1 = in_cta(empty0, 1);
-        const uint32_t tfull0 = smem_u32(tfull), tfull1 = in_cta(tfull0, 1);
+        const uint32_t empty0 = smem_u32(empty), empty1 = in_cta(empty0, leader + 1);
+        const uint32_t tfull0 = smem_u32(tfull), tfull1 = in_cta(tfull0, leader + 1);
         int slot = 0, phase = 0, done = 0;
         bool ok = true;
         for (int t = cluster; t < tiles && ok; t += clusters, ++done) {
             ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(tempty), (done & 1) ^ 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            for (int s = 0; s < p.stages; ++s) {
+            for (int s = s0; s < s1; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), phase, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
@@ -618,7 +644,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                     for (int kk = 0; kk < 4; ++kk)
                         if (kk < steps)
                             mma_mx4<2>(tmem, wd + kk * 2, td + kk * 2, mx4_idesc(256, 256, kk & 1),
-                                       cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8, (s > 0 || kk > 0) ? 1u : 0u);
+                                       cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8, (s > s0 || kk > 0) ? 1u : 0u);
                     commit_pair(empty0 + slot * 8);
                     commit_pair(empty1 + slot * 8);
                 }
@@ -662,7 +688,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             tmem_ld_wait(v);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), 0));
+            if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), leader));
+            if (splits > 1) {
+                // the tile's sums over the stages, which have all been read
+                float* sums = reinterpret_cast<float*>(smem) + (size_t)half * 128 * 128 + quad * 32 + lane;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sums[(c * 32 + j) * 128] = v[c][j];
+                continue;
+            }
             const int64_t col = (int64_t)tn * 256 + rank * 128 + quad * 32 + lane;
             const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
 #pragma unroll
@@ -686,6 +721,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         if (lane == 0) bulk_wait_all();
     }
     __syncwarp();
+    if (splits > 1) {
+        // one tile to a cluster (the launch sees to it)
+        sync_cluster();
+        if (warp >= 2) {
+            int tm, tn;
+            pair_tile(p, cluster, tm, tn);
+            const int64_t row0 = (int64_t)tm * 256;
+            add_splits(p, smem_u32(smem), splits, 2, rank, split, warp - 2, 8, row0, (int)min((int64_t)256, p.m - row0),
+                       (int64_t)tn * 256 + rank * 128 + lane * 4, lane);
+        }
+        sync_cluster();
+    }
     __syncthreads();
     if (*abort_flag && rank == 0 && threadIdx.x == 0) {
         // the pair's copies complete on the leader's barriers: wait for the last ones issued
@@ -738,20 +785,24 @@ int map_scales(CUtensorMap* map, const rt_mx4& q, int tiles) {
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, q.scales, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int TN>
-int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaStream_t stream) {
-    using G = Geo1<TN>;
-    CUtensorMap w, t, sw, st;
-    RT_TRY(map_codes(&w, b, 128));
-    RT_TRY(map_codes(&t, a, TN));
-    RT_TRY(map_scales(&sw, b, 1));
-    RT_TRY(map_scales(&st, a, 1));
+}  // namespace
+
+int mx4_encode_maps(rt_mx4* q) {
+    if (q->rows == 0 || q->k == 0) return RT_OK;
+    for (int i = 0; i < 3; ++i) RT_TRY(map_codes(&q->maps.codes[i], *q, 32 << i));
+    for (int i = 0; i < 2; ++i) RT_TRY(map_scales(&q->maps.scales[i], *q, 1 + i));
+    return RT_OK;
+}
+
+namespace {
+
+template <int TN, bool DEEP>
+int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int splits, cudaStream_t stream) {
+    using G = Geo1<TN, DEEP>;
+    const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[TN / 64], &sw = b.maps.scales[0], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + TN - 1) / TN);
     p.tiles_n = (int)((p.n + 127) / 128);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    // split k while the CTAs fit two to an SM and each keeps two stages
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 2 * (int64_t)ctx->sm_count && p.stages >= 4 * splits) splits *= 2;
     p.stages_per_split = (p.stages + splits - 1) / splits;
     splits = (p.stages + p.stages_per_split - 1) / p.stages_per_split;
     RT_CHECK(tiles * splits <= INT32_MAX, "rt_mx4_matmul: C is too large");
@@ -769,17 +820,14 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaS
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 2 : 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<TN>, w, t, sw, st, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<TN, DEEP>, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
 }
 
-int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaStream_t stream) {
-    CUtensorMap w, t, sw, st, c;
-    RT_TRY(map_codes(&w, b, 128));
-    RT_TRY(map_codes(&t, a, 128));
-    RT_TRY(map_scales(&sw, b, 1));
-    RT_TRY(map_scales(&st, a, 2));
+int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int splits, cudaStream_t stream) {
+    const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[0], &st = a.maps.scales[1];
+    CUtensorMap c;
     const int64_t row = p.ldc * (p.out_bf16 ? 2 : 4);
     p.staged = row % 16 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
     c = w;
@@ -792,9 +840,11 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cuda
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    RT_CHECK(tiles <= INT32_MAX, "rt_mx4_matmul: C is too large");
+    RT_CHECK(tiles <= INT32_MAX / 16, "rt_mx4_matmul: C is too large");
+    p.stages_per_split = (p.stages + splits - 1) / splits;
+    splits = (p.stages + p.stages_per_split - 1) / p.stages_per_split;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
+    cfg.gridDim = dim3((unsigned)(2 * (splits > 1 ? tiles * splits : std::min<int64_t>(tiles, ctx->sm_count / 2))));
     cfg.blockDim = dim3(kPairThreads);
     cfg.dynamicSmemBytes = kPairSmem;
     cfg.stream = stream;
@@ -802,7 +852,7 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cuda
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = 2 * splits;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -812,19 +862,20 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cuda
     return RT_OK;
 }
 
-template <int TN>
+template <int TN, bool DEEP>
 int allow_smem() {
-    RT_CUDA(cudaFuncSetAttribute(mx4_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<TN>::SMEM));
+    RT_CUDA(cudaFuncSetAttribute(mx4_kernel<TN, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<TN, DEEP>::SMEM));
     return RT_OK;
 }
 
 }  // namespace
 
 int gemm_mx4_init() {
-    RT_TRY(allow_smem<32>());
-    RT_TRY(allow_smem<64>());
+    RT_TRY((allow_smem<32, false>()));
+    RT_TRY((allow_smem<64, false>()));
+    RT_TRY((allow_smem<32, true>()));
     RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    return allow_smem<128>();
+    return allow_smem<64, true>();
 }
 
 int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
@@ -846,10 +897,15 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
         count_launch(ctx);
         return RT_OK;
     }
-    if (p.m <= 32) return launch_one<32>(ctx, a, b, p, stream);
-    if (p.m <= 64) return launch_one<64>(ctx, a, b, p, stream);
-    if (((p.m + 255) / 256) * ((p.n + 255) / 256) * 4 >= ctx->sm_count) return launch_pair(ctx, a, b, p, stream);
-    return launch_one<128>(ctx, a, b, p, stream);
+    const int64_t pairs = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    if (pairs * 4 >= ctx->sm_count) return launch_pair(ctx, a, b, p, 1, stream);
+    const int tn = p.m <= 32 ? 32 : 64;
+    const int64_t tiles = ((p.m + tn - 1) / tn) * ((p.n + 127) / 128);
+    // split k while the CTAs fit two to an SM and each keeps two stages
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= 2 * (int64_t)ctx->sm_count && p.stages >= 4 * splits) splits *= 2;
+    if (tn == 32) return launch_one<32, false>(ctx, a, b, p, splits, stream);
+    return launch_one<64, false>(ctx, a, b, p, splits, stream);
 }
 
 }  // namespace rt

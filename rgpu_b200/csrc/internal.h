@@ -1,6 +1,7 @@
 // Internal declarations shared by the translation units of librtgpu.so.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cstdint>
@@ -91,6 +92,11 @@ struct rt_mx4 {
     uint8_t* scales = nullptr;
     int64_t rows = 0, k = 0;
     bool owned = false;
+    // TMA descriptors of the product's boxes, made with the handle: codes of 32,
+    // 64 and 128 rows, scales of one and two row tiles
+    struct {
+        CUtensorMap codes[3], scales[2];
+    } maps;
     __host__ __device__ int64_t blocks() const { return (k + 31) / 32; }
     __host__ __device__ int64_t row_bytes() const { return blocks() * 16; }
     __host__ __device__ int64_t groups() const { return (blocks() + 3) / 4; }  // scale tiles along k
@@ -266,6 +272,7 @@ int launch_fill_column(rt_ctx* ctx, void* p, rt_dtype dt, int64_t rows, int64_t 
                        cudaStream_t stream);
 
 int gemm_mx4_init();
+int mx4_encode_maps(rt_mx4* q);
 // C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU) of microscaled 4-bit matrices.
 int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
                     cudaStream_t stream);

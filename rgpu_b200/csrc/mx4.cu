@@ -432,6 +432,12 @@ int rt_mx4_zeros(rt_ctx* ctx, int64_t rows, int64_t k, rt_mx4** out) {
     q->rows = rows;
     q->k = k;
     q->owned = true;
+    const int s = mx4_encode_maps(q);
+    if (s != RT_OK) {
+        cudaFree(p);
+        delete q;
+        return s;
+    }
     *out = q;
     return RT_OK;
 }
@@ -450,6 +456,11 @@ int rt_mx4_wrap(rt_ctx* ctx, void* codes, void* scales, int64_t rows, int64_t k,
     q->scales = static_cast<uint8_t*>(scales);
     q->rows = rows;
     q->k = k;
+    const int s = mx4_encode_maps(q);
+    if (s != RT_OK) {
+        delete q;
+        return s;
+    }
     *out = q;
     return RT_OK;
 }
