@@ -366,10 +366,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
         }
     } else if (warp >= 2) {
         const int quad = warp & 3;
-        const int64_t col = (int64_t)tn * 128 + quad * 32 + lane;
-        const int64_t row0 = (int64_t)tm * TN;
-        const int count = (int)min((int64_t)TN, p.m - row0);
-        const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
+        const int count = (int)min((int64_t)TN, p.m - (int64_t)tm * TN);
         const bool got = mbar_wait(smem_u32(done), 0, abort_flag);
         if (!got && lane == 0) {
             record_error(p.err, DEV_TIMEOUT_EPILOGUE, blockIdx.x);
@@ -377,32 +374,27 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
         }
         __syncwarp();
         tc_fence_after();
-        float* sums = reinterpret_cast<float*>(smem);  // [token][128 columns]; every stage has been read
+        float* sums = reinterpret_cast<float*>(smem) + quad * 32 + lane;  // [token][128 columns]; every stage has been read
         for (int c = 0; c < count && __all_sync(0xffffffffu, got); c += 32) {
             float v[32];
             tmem_ld_32x32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
-            if (ranks == 1) {
-                if (col < p.n)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (c + j < count) store_c(p, row0 + c + j, col, v[j], bias);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) sums[(c + j) * 128 + quad * 32 + lane] = v[j];
-            }
+            for (int j = 0; j < 32; ++j) sums[(c + j) * 128] = v[j];
         }
         tc_fence_before();
     }
     __syncwarp();
-    if (ranks > 1) {
+    // the splits' sums (or this CTA's own) to C: rows of it, four columns a lane
+    if (ranks > 1)
         sync_cluster();
-        if (warp >= 2) {
-            const int64_t row0 = (int64_t)tm * TN;
-            add_splits(p, smem_u32(smem), ranks, 1, 0, rank, warp - 2, 4, row0, (int)min((int64_t)TN, p.m - row0),
-                       (int64_t)tn * 128 + lane * 4, lane);
-        }
-        sync_cluster();  // the sums are read before any CTA exits
+    else
+        __syncthreads();
+    {
+        const int64_t row0 = (int64_t)tm * TN;
+        add_splits(p, smem_u32(smem), ranks, 1, 0, rank, warp, kThreads1 / 32, row0, (int)min((int64_t)TN, p.m - row0),
+                   (int64_t)tn * 128 + lane * 4, lane);
     }
+    if (ranks > 1) sync_cluster();  // the sums are read before any CTA exits
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
@@ -521,6 +513,34 @@ __device__ __forceinline__ void stage_chunk(const Mx4Params& p, const CUtensorMa
     half_sync(half);
     if (storer) {
         if (row0 < p.m && col0 < p.n) tma_store_2d(map, smem_u32(chunk), col0, (int)row0);
+        bulk_commit();
+    }
+}
+
+// A lane's 128 tokens of a CTA's last tile through the ring, which is free by then:
+// all staged at once, one barrier, and every warp of the half stores a chunk.
+template <typename T>
+__device__ __forceinline__ void stage_last(const Mx4Params& p, const CUtensorMap* map, uint8_t* ring, int half, int quad,
+                                           int lane, int col0, int64_t row0, const float (&v)[4][32], float bias) {
+    constexpr int kTokens = kChunkBytes / (128 * (int)sizeof(T));  // of a box
+    T* at = reinterpret_cast<T*>(ring) + (size_t)half * 128 * 128 + quad * 32 + lane;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            float x = v[c][j] + bias;
+            if (p.relu) x = x < 0.0f ? 0.0f : x;
+            if constexpr (sizeof(T) == 2)
+                at[(c * 32 + j) * 128] = __float2bfloat16_rn(x);
+            else
+                at[(c * 32 + j) * 128] = x;
+        }
+    fence_async_shared();
+    half_sync(half);
+    if (lane == 0 && col0 < p.n) {
+        for (int j = quad * 32; j < quad * 32 + 32; j += kTokens)
+            if (row0 + j < p.m)
+                tma_store_2d(map, smem_u32(reinterpret_cast<T*>(ring) + ((size_t)half * 128 + j) * 128), col0, (int)(row0 + j));
         bulk_commit();
     }
 }
@@ -700,6 +720,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             }
             const int64_t col = (int64_t)tn * 256 + rank * 128 + quad * 32 + lane;
             const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
+            if (p.staged && t + clusters >= tiles) {
+                const int col0 = tn * 256 + (int)rank * 128;
+                const int64_t row0 = (int64_t)tm * 256 + half * 128;
+                if (p.out_bf16)
+                    stage_last<__nv_bfloat16>(p, &map_c, smem, half, quad, lane, col0, row0, v, bias);
+                else
+                    stage_last<float>(p, &map_c, smem, half, quad, lane, col0, row0, v, bias);
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int64_t row0 = (int64_t)tm * 256 + half * 128 + c * 32;
@@ -718,7 +747,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             }
         }
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
-        if (lane == 0) bulk_wait_all();
+        if (lane == 0) bulk_wait_read_all();  // the stores have read shared memory; the kernel's end completes them
     }
     __syncwarp();
     if (splits > 1) {
