@@ -2,12 +2,7 @@
 // C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU): tcgen05.mma kind::mxf4 with one
 // E8M0 scale per 32 elements, f32 accumulators in TMEM.
 //
-// The tensor cores compute C^T: B's rows (C's columns) are the MMA's M rows, 128
-// to a CTA, and A's rows (C's rows, "tokens") its N columns.  An accumulator
-// lane is then one column of C, so 32 lanes store 32 neighbouring elements of a
-// row of C straight from registers, for any row stride and alignment of C, the
-// bias is one value per thread, and few tokens make a narrow MMA, not a wasted
-// one.
+// A's rows are called tokens here, T; B's rows are C's columns, W.
 //
 // A k stage is 256 elements: 128 bytes of codes per row (one 128-byte-swizzled
 // TMA box) and two 512-byte scale tiles per 128 rows, in memory already in the
@@ -43,7 +38,7 @@ struct Mx4Params {
     int out_bf16;
     const float* bias;
     int relu;
-    int staged;                       // two-CTA kernel: C is stored through TMA boxes
+    int access;                       // two-CTA kernel: bytes that pieces of 32 of C's rows are aligned to (32, 16, 0)
     int* err;
 };
 
@@ -188,14 +183,20 @@ __device__ __forceinline__ void store_c4(const Mx4Params& p, int64_t row, int64_
     }
 }
 
+// Where the 16-byte piece of a row of 256 sums lies, pieces exchanged within eight
+// by the row.
+__device__ __forceinline__ int sum_piece(int piece, int row) { return piece ^ (row & 7); }
+
 // Adds the splits' sums of a tile in order and stores C.  Each of `splits` CTAs of
 // the cluster (ranks `stride` apart from `offset` on) holds [token][128 columns] f32
-// at `sums` of its shared memory; the tokens are dealt out over the splits (this one
-// is number `split`) and their warps.  A lane takes four columns; four tokens are
+// (WIDE: [token][256] by sum_piece, of which the 128 from `piece` on) at `sums` of
+// its shared memory; the tokens are dealt out over the splits (this one is number
+// `split`) and their warps.  A lane takes four columns; four tokens are
 // under way at a time, since a read from another SM takes most of a microsecond.
+template <bool WIDE = false>
 __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t stride,
                                            uint32_t offset, uint32_t split, int warp, int warps, int64_t row0, int count,
-                                           int64_t col, int lane) {
+                                           int64_t col, int lane, int piece = 0) {
     constexpr int U = 4;
     float bias[4];
 #pragma unroll
@@ -207,11 +208,14 @@ __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, ui
         for (int u = 0; u < U; ++u) v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 2
         for (uint32_t r = 0; r < splits; ++r) {
-            const uint32_t at = in_cta(sums + lane * 16, offset + r * stride);
+            const uint32_t at = in_cta(sums, offset + r * stride);
             float4 x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (c + u * step < count) x[u] = ld_cluster4(at + (c + u * step) * 512);
+            for (int u = 0; u < U; ++u) {
+                const int row = c + u * step;
+                if (row < count)
+                    x[u] = ld_cluster4(at + (WIDE ? row * 1024 + sum_piece(piece + lane, row) * 16 : row * 512 + lane * 16));
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (c + u * step < count) {
@@ -228,8 +232,10 @@ __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, ui
 }
 
 // ------------------------------------------------------------ one-CTA kernel
-// A CTA computes 128 columns of C for TN tokens over its share of k; the CTAs of
-// a cluster share one tile, split along k.  Their sums meet in shared memory and
+// For few tokens or little work.  The tensor cores compute C^T: 128 of W's rows are
+// the MMA's M rows and TN tokens its N columns, so a CTA computes 128 columns of C
+// for TN tokens over its share of k.  The CTAs of a cluster share one tile, split
+// along k.  Their sums meet in shared memory and
 // are added in rank order, tokens dealt out over the CTAs.
 // STAGES: a short ring for two CTAs to an SM, or one that fills the SM's shared
 // memory for one: a stage takes over a microsecond to arrive, so the ring's depth
@@ -403,27 +409,31 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 }
 
 // ----------------------------------------------------------- two-CTA kernel
-// A cluster of two CTAs on a pair of SMs computes 256 columns of C for 256
-// tokens: each CTA holds the codes of 128 of the columns and of 128 of the
-// tokens, the pair's MMAs read both, and each CTA's TMEM receives its 128
-// columns for all 256 tokens.  Half the bytes from L2 per MMA of the one-CTA
-// tile: a stage is 35 KB per CTA for 4 x 128 clocks of MMA.  The scales of all
-// 256 tokens are needed by both CTAs, so each loads them itself.
+// A cluster of two CTAs on a pair of SMs computes 256 tokens by 256 columns of C:
+// each CTA holds the codes of 128 of the tokens and of 128 of the columns, the
+// pair's MMAs (M = N = 256) read both, and each CTA's TMEM receives its 128 tokens
+// for all 256 columns.  Half the bytes from L2 per MMA of a one-CTA tile: a stage is
+// 35 KB per CTA for 4 x 128 clocks of MMA.  The scales of all 256 columns are
+// needed by both CTAs, so each loads them itself.
 //
-// The f32 accumulator takes 256 of the 512 TMEM columns and the scales 24 a
-// stage, which leaves no room for a second accumulator: instead the eight
-// epilogue warps draw the finished tile into 128 registers a thread and hand the
-// accumulator back at once, so the next tile's MMAs wait for that only, not for
-// the stores.  Persistent: tiles are dealt out round robin, the loads of the next
-// tile run on while this one's epilogue stores.
+// Here the tokens are the MMA's M rows, an accumulator lane is a row of C, and a
+// thread holds 128 neighbouring elements of it: it stores them as 32-byte sectors,
+// 256 bits an instruction, with nothing to wait for afterwards.  (Columns as lanes,
+// staged through shared memory for TMA boxes, took 3.3 us a tile against the 2.3 us
+// of MMAs that 2048 of k give it to hide in.)
 //
-// Where C's rows can be TMA boxes (16-byte aligned base and stride) the epilogue
-// stages 32 tokens x 128 columns at a time in shared memory and stores them as
-// one box, whole 128-byte lines; otherwise it stores from registers.
+// The f32 accumulator takes 256 of the 512 TMEM columns and the scales 24 a stage,
+// which leaves no room for a second accumulator: instead the eight epilogue warps
+// draw the finished tile into 128 registers a thread and hand the accumulator back
+// at once (0.13 us), so the next tile's MMAs wait for that only, not for the stores.
+// Persistent: tiles are dealt out round robin, the loads of the next tile run on
+// while this one's epilogue stores.
+//
+// The pairs of a cluster of more share one tile, split along k; their sums meet as
+// those of the one-CTA kernel do.
 constexpr int kPairStages = 6;
-constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of W and T, two tiles of W's scales, four of T's
-constexpr int kChunkBytes = 32 * 128 * 2;  // staged output of either half of the tokens: 128 columns of 32 (f32: 16) tokens
-constexpr int kPairSmem = kPairStages * kPairStageBytes + 2 * kChunkBytes + 256;
+constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of T and W, two tiles of T's scales, four of W's
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 8 * 512 /* bias of each epilogue warp's columns */ + 256;
 static_assert(256 * 512 <= kPairStages * kPairStageBytes, "the split sums reuse the stages");
 constexpr int kPairThreads = 320;  // warps: 0 TMA, 1 MMA (leader), 2-9 epilogue (two to a TMEM lane quadrant)
 static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
@@ -461,87 +471,51 @@ __device__ __forceinline__ void pair_tile(const Mx4Params& p, int t, int& tm, in
     tn = in / rows;
 }
 
-// 32 tokens of one column a lane, stored from registers.  bf16 with even strides: neighbouring
-// lanes trade so that each stores two columns of one token, the even lane of one
-// token and the odd lane of the next.
-__device__ __forceinline__ void store_tokens(const Mx4Params& p, int64_t row0, int count, int64_t col, float bias,
-                                             bool pairs, float (&v)[32]) {
-    if (pairs) {
-        const bool odd = col & 1;
-        __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.c) + (row0 + (odd ? 1 : 0)) * p.ldc + (col & ~int64_t(1));
+// 32 neighbouring elements of a row of C from `bias` on; ACCESS: bytes that every
+// such piece's address is a multiple of (32, 16, or 0: element by element).
+template <typename T, int ACCESS>
+__device__ __forceinline__ void store_row32(T* c, int64_t left, const float* bias, bool relu, const float (&v)[32]) {
+    if (left <= 0) return;
+    float x[32];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-            float a = v[j] + bias, b = v[j + 1] + bias;
-            if (p.relu) {
-                a = a < 0.0f ? 0.0f : a;
-                b = b < 0.0f ? 0.0f : b;
+    for (int i = 0; i < 32; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + i);
+        x[i] = v[i] + b.x, x[i + 1] = v[i + 1] + b.y, x[i + 2] = v[i + 2] + b.z, x[i + 3] = v[i + 3] + b.w;
+    }
+    if (relu)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = x[i] < 0.0f ? 0.0f : x[i];  // keeps a NaN
+    if (ACCESS > 0 && left >= 32) {
+        constexpr int WORDS = 8 * (int)sizeof(T);
+        uint32_t w[WORDS];
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                w[i] = __float_as_uint(x[i]);
             }
-            const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
-            const __nv_bfloat162 two = odd ? __floats2bfloat162_rn(other, b) : __floats2bfloat162_rn(a, other);
-            if (j + (odd ? 1 : 0) < count && col < p.n) *reinterpret_cast<__nv_bfloat162*>(c + j * p.ldc) = two;
         }
-    } else if (col < p.n) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < count) store_c(p, row0 + j, col, v[j], bias);
-    }
-}
-
-// Barrier of the four epilogue warps of one half of the tokens.
-__device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
-
-// The tokens FIRST.. of a lane's 32 (as many as a chunk holds) through the
-// half's chunk [token][128 columns], stored as one box at (col0, row0).
-template <typename T, int FIRST>
-__device__ __forceinline__ void stage_chunk(const Mx4Params& p, const CUtensorMap* map, uint8_t* chunk, int half,
-                                            int quad, int lane, int col0, int64_t row0, const float (&v)[32],
-                                            float bias) {
-    const bool storer = quad == 0 && lane == 0;
-    if (storer) bulk_wait_read_all();  // the chunk's last store has read it
-    half_sync(half);
-    T* at = reinterpret_cast<T*>(chunk) + quad * 32 + lane;
-#pragma unroll
-    for (int j = 0; j < kChunkBytes / (128 * (int)sizeof(T)); ++j) {
-        float x = v[FIRST + j] + bias;
-        if (p.relu) x = x < 0.0f ? 0.0f : x;
-        if constexpr (sizeof(T) == 2)
-            at[j * 128] = __float2bfloat16_rn(x);
-        else
-            at[j * 128] = x;
-    }
-    fence_async_shared();
-    half_sync(half);
-    if (storer) {
-        if (row0 < p.m && col0 < p.n) tma_store_2d(map, smem_u32(chunk), col0, (int)row0);
-        bulk_commit();
-    }
-}
-
-// A lane's 128 tokens of a CTA's last tile through the ring, which is free by then:
-// all staged at once, one barrier, and every warp of the half stores a chunk.
-template <typename T>
-__device__ __forceinline__ void stage_last(const Mx4Params& p, const CUtensorMap* map, uint8_t* ring, int half, int quad,
-                                           int lane, int col0, int64_t row0, const float (&v)[4][32], float bias) {
-    constexpr int kTokens = kChunkBytes / (128 * (int)sizeof(T));  // of a box
-    T* at = reinterpret_cast<T*>(ring) + (size_t)half * 128 * 128 + quad * 32 + lane;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            float x = v[c][j] + bias;
-            if (p.relu) x = x < 0.0f ? 0.0f : x;
-            if constexpr (sizeof(T) == 2)
-                at[(c * 32 + j) * 128] = __float2bfloat16_rn(x);
+        for (int i = 0; i < WORDS; i += ACCESS == 32 ? 8 : 4) {
+            uint32_t* p = reinterpret_cast<uint32_t*>(c) + i;
+            if constexpr (ACCESS == 32)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[i]), "r"(w[i + 1]),
+                             "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                             : "memory");
             else
-                at[(c * 32 + j) * 128] = x;
+                *reinterpret_cast<uint4*>(p) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
         }
-    fence_async_shared();
-    half_sync(half);
-    if (lane == 0 && col0 < p.n) {
-        for (int j = quad * 32; j < quad * 32 + 32; j += kTokens)
-            if (row0 + j < p.m)
-                tma_store_2d(map, smem_u32(reinterpret_cast<T*>(ring) + ((size_t)half * 128 + j) * 128), col0, (int)(row0 + j));
-        bulk_commit();
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < left) {
+                if constexpr (sizeof(T) == 2)
+                    c[i] = __float2bfloat16_rn(x[i]);
+                else
+                    c[i] = x[i];
+            }
     }
 }
 
@@ -549,15 +523,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                                                                    const __grid_constant__ CUtensorMap map_t,
                                                                    const __grid_constant__ CUtensorMap map_sw,
                                                                    const __grid_constant__ CUtensorMap map_st,
-                                                                   const __grid_constant__ CUtensorMap map_c,
                                                                    Mx4Params p) {
     constexpr int S = kPairStages;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* smem_w = smem;
     uint8_t* smem_t = smem + S * kWBytes;
-    uint8_t* smem_s = smem + 2 * S * kWBytes;  // [stage][W groups 0, 1; tokens 0-127 groups 0, 1; tokens 128-255]
-    uint8_t* smem_c = smem_s + S * 6 * kScaleTile;  // [token half]
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem_c + 2 * kChunkBytes);  // leader: both CTAs' bytes of a stage
+    uint8_t* smem_s = smem + 2 * S * kWBytes;  // [stage][T groups 0, 1; columns 0-127 groups 0, 1; columns 128-255]
+    float* smem_bias = reinterpret_cast<float*>(smem_s + S * 6 * kScaleTile);  // [epilogue warp][128]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem_bias + 8 * 128);  // leader: both CTAs' bytes of a stage
     uint64_t* empty = full + S;   // each CTA: stage read by the MMAs
     uint64_t* tfull = empty + S;  // each CTA: accumulator complete
     uint64_t* tempty = tfull + 1; // leader: accumulator drawn by both CTAs' epilogues
@@ -589,7 +562,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         prefetch_tmap(&map_t);
         prefetch_tmap(&map_sw);
         prefetch_tmap(&map_st);
-        if (p.staged) prefetch_tmap(&map_c);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -627,8 +599,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                 tma_pair_2d(smem_u32(smem_w + slot * kWBytes), &map_w, s * kRowBytes, tn * 256 + (int)rank * 128, bar);
                 tma_pair_2d(smem_u32(smem_t + slot * kWBytes), &map_t, s * kRowBytes, tm * 256 + (int)rank * 128, bar);
                 const uint32_t ss = smem_u32(smem_s + slot * 6 * kScaleTile);
-                tma_pair_3d(ss, &map_sw, 0, s * 2, tn * 2 + (int)rank, bar);
-                tma_pair_3d(ss + 2 * kScaleTile, &map_st, 0, s * 2, tm * 2, bar);
+                tma_pair_3d(ss, &map_st, 0, s * 2, tm * 2 + (int)rank, bar);
+                tma_pair_3d(ss + 2 * kScaleTile, &map_sw, 0, s * 2, tn * 2, bar);
                 ++issued;
             }
         }
@@ -651,7 +623,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                 tc_fence_after();
                 const uint64_t wd = w0 + slot * (kWBytes >> 4), td = t0 + slot * (kWBytes >> 4);
                 const uint64_t sc = sc0 + slot * (6 * kScaleTile >> 4);
-                const uint32_t cols = tmem + 256 + slot * 24;  // W group 0, W group 1, T group 0 (8 wide), T group 1
+                const uint32_t cols = tmem + 256 + slot * 24;  // T group 0, T group 1, W group 0 (8 wide), W group 1
                 const int steps = min(4, (p.blocks - s * kStageBlocks + 1) / 2);
                 if (elect_one()) {
 #pragma unroll
@@ -663,7 +635,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
                         if (kk < steps)
-                            mma_mx4<2>(tmem, wd + kk * 2, td + kk * 2, mx4_idesc(256, 256, kk & 1),
+                            mma_mx4<2>(tmem, td + kk * 2, wd + kk * 2, mx4_idesc(256, 256, kk & 1),
                                        cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8, (s > s0 || kk > 0) ? 1u : 0u);
                     commit_pair(empty0 + slot * 8);
                     commit_pair(empty1 + slot * 8);
@@ -687,14 +659,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             mbar_wait(smem_u32(drain), 0, abort_flag);
         }
     } else if (warp >= 2) {
-        const int quad = warp & 3, half = (warp - 2) >> 2;
-        const bool pairs = p.out_bf16 && (p.ldc & 1) == 0 && (reinterpret_cast<uintptr_t>(p.c) & 3) == 0 && (p.n & 1) == 0;
-        uint8_t* chunk = smem_c + half * kChunkBytes;
+        const int quad = warp & 3, half = (warp - 2) >> 2;  // lanes, columns
+        float* bias = smem_bias + (warp - 2) * 128;
         int done = 0;
         bool ok = true;
         for (int t = cluster; t < tiles; t += clusters, ++done) {
             int tm, tn;
             pair_tile(p, t, tm, tn);
+            const int64_t row = (int64_t)tm * 256 + rank * 128 + quad * 32 + lane, col0 = (int64_t)tn * 256 + half * 128;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t col = col0 + i * 32 + lane;
+                bias[i * 32 + lane] = p.bias && col < p.n ? p.bias[col] : 0.0f;
+            }
+            __syncwarp();
             const bool got = mbar_wait(smem_u32(tfull), done & 1, abort_flag);
             if (!__all_sync(0xffffffffu, got)) {
                 ok = false;
@@ -710,56 +689,49 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             __syncwarp();
             if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), leader));
             if (splits > 1) {
-                // the tile's sums over the stages, which have all been read
-                float* sums = reinterpret_cast<float*>(smem) + (size_t)half * 128 * 128 + quad * 32 + lane;
+                // the tile's sums over the stages, which have all been read: [token][256 columns],
+                // the 16-byte pieces of a row exchanged so that 8 lanes' rows take all banks
+                float* sums = reinterpret_cast<float*>(smem) + (quad * 32 + lane) * 256;
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sums[(c * 32 + j) * 128] = v[c][j];
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4*>(sums + sum_piece(half * 32 + c * 8 + j / 4, lane) * 4) =
+                            make_float4(v[c][j], v[c][j + 1], v[c][j + 2], v[c][j + 3]);
                 continue;
             }
-            const int64_t col = (int64_t)tn * 256 + rank * 128 + quad * 32 + lane;
-            const float bias = p.bias && col < p.n ? p.bias[col] : 0.0f;
-            if (p.staged && t + clusters >= tiles) {
-                const int col0 = tn * 256 + (int)rank * 128;
-                const int64_t row0 = (int64_t)tm * 256 + half * 128;
-                if (p.out_bf16)
-                    stage_last<__nv_bfloat16>(p, &map_c, smem, half, quad, lane, col0, row0, v, bias);
-                else
-                    stage_last<float>(p, &map_c, smem, half, quad, lane, col0, row0, v, bias);
-                continue;
-            }
+            if (row >= p.m) continue;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int64_t row0 = (int64_t)tm * 256 + half * 128 + c * 32;
-                if (p.staged) {
-                    const int col0 = tn * 256 + (int)rank * 128;
-                    if (p.out_bf16) {
-                        stage_chunk<__nv_bfloat16, 0>(p, &map_c, chunk, half, quad, lane, col0, row0, v[c], bias);
-                    } else {
-                        stage_chunk<float, 0>(p, &map_c, chunk, half, quad, lane, col0, row0, v[c], bias);
-                        stage_chunk<float, 16>(p, &map_c, chunk, half, quad, lane, col0, row0 + 16, v[c], bias);
-                    }
+                const int64_t at = row * p.ldc + col0 + c * 32, left = p.n - col0 - c * 32;
+                const bool relu = p.relu;
+                if (p.out_bf16) {
+                    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.c) + at;
+                    if (p.access == 32) store_row32<__nv_bfloat16, 32>(to, left, bias + c * 32, relu, v[c]);
+                    else if (p.access == 16) store_row32<__nv_bfloat16, 16>(to, left, bias + c * 32, relu, v[c]);
+                    else store_row32<__nv_bfloat16, 0>(to, left, bias + c * 32, relu, v[c]);
                 } else {
-                    const int count = (int)max((int64_t)0, min((int64_t)32, p.m - row0));
-                    store_tokens(p, row0, count, col, bias, pairs, v[c]);
+                    float* to = static_cast<float*>(p.c) + at;
+                    if (p.access == 32) store_row32<float, 32>(to, left, bias + c * 32, relu, v[c]);
+                    else if (p.access == 16) store_row32<float, 16>(to, left, bias + c * 32, relu, v[c]);
+                    else store_row32<float, 0>(to, left, bias + c * 32, relu, v[c]);
                 }
             }
         }
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
-        if (lane == 0) bulk_wait_read_all();  // the stores have read shared memory; the kernel's end completes them
     }
     __syncwarp();
     if (splits > 1) {
         // one tile to a cluster (the launch sees to it)
         sync_cluster();
-        if (warp >= 2) {
-            int tm, tn;
-            pair_tile(p, cluster, tm, tn);
-            const int64_t row0 = (int64_t)tm * 256;
-            add_splits(p, smem_u32(smem), splits, 2, rank, split, warp - 2, 8, row0, (int)min((int64_t)256, p.m - row0),
-                       (int64_t)tn * 256 + rank * 128 + lane * 4, lane);
-        }
+        int tm, tn;
+        pair_tile(p, cluster, tm, tn);
+        const int64_t row0 = (int64_t)tm * 256 + rank * 128;
+        const int count = (int)max((int64_t)0, min((int64_t)128, p.m - row0));
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h)
+            add_splits<true>(p, smem_u32(smem), splits, 2, rank, split, warp, kPairThreads / 32, row0, count,
+                             (int64_t)tn * 256 + h * 128 + lane * 4, lane, h * 32);
         sync_cluster();
     }
     __syncthreads();
@@ -855,17 +827,9 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int s
 }
 
 int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int splits, cudaStream_t stream) {
-    const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[0], &st = a.maps.scales[1];
-    CUtensorMap c;
-    const int64_t row = p.ldc * (p.out_bf16 ? 2 : 4);
-    p.staged = row % 16 == 0 && (reinterpret_cast<uintptr_t>(p.c) & 15) == 0;
-    c = w;
-    if (p.staged) {
-        const cuuint64_t dims[2] = {(cuuint64_t)p.n, (cuuint64_t)p.m}, strides[1] = {(cuuint64_t)row};
-        const cuuint32_t box[2] = {128, p.out_bf16 ? 32u : 16u};
-        RT_TRY(encode(&c, p.out_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, p.c, dims,
-                      strides, box, CU_TENSOR_MAP_SWIZZLE_NONE));
-    }
+    const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[1], &st = a.maps.scales[0];
+    const uintptr_t rows = reinterpret_cast<uintptr_t>(p.c) | (uintptr_t)(p.ldc * (p.out_bf16 ? 2 : 4));
+    p.access = (rows & 31) == 0 ? 32 : (rows & 15) == 0 ? 16 : 0;
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
@@ -886,7 +850,7 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 2 : 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_pair_kernel, w, t, sw, st, c, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_pair_kernel, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
 }

@@ -161,7 +161,7 @@ def test_product(gpu, m, n, k, dtype):
     b, bv = _operand(gpu, n, k, n * 13 + k + 1)
     bias = np.random.default_rng(n).standard_normal((1, n)).astype(np.float32) * 10
     tb = gpu.upload(bias)
-    for pad, offset, epi in ((0, 0, "none"), (0, 0, "bias"), (3, 1, "bias_relu")):
+    for pad, offset, epi in ((0, 0, "none"), (-n % 32, 0, "bias"), (-n % 16 + 8, 8, "bias"), (3, 1, "bias_relu")):
         c, buf, view = _upload(gpu, np.zeros((m, n)), dtype, n + pad, offset)
         before = buf.clone()
         gpu.mx4_matmul(a.q, b.q, c, bias=None if epi == "none" else tb, relu=epi == "bias_relu")
