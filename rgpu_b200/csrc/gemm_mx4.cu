@@ -38,7 +38,7 @@ struct Mx4Params {
     int out_bf16;
     const float* bias;
     int relu;
-    int access;                       // two-CTA kernel: bytes that pieces of 32 of C's rows are aligned to (32, 16, 0)
+    int access;                       // bytes that C's rows are aligned to (32, 16, 8, or 0 for less)
     int* err;
 };
 
@@ -148,39 +148,25 @@ __device__ __forceinline__ void tmem_ld_wait(float (&v)[4][32]) {
         for (int j = 0; j < 32; ++j) asm volatile("" : "+f"(v[c][j]));
 }
 
-// One element of C.  max(v, 0) keeps a NaN.
-__device__ __forceinline__ void store_c(const Mx4Params& p, int64_t row, int64_t col, float v, float bias) {
-    v += bias;
-    if (p.relu) v = v < 0.0f ? 0.0f : v;
-    if (p.out_bf16)
-        static_cast<__nv_bfloat16*>(p.c)[row * p.ldc + col] = __float2bfloat16_rn(v);
-    else
-        static_cast<float*>(p.c)[row * p.ldc + col] = v;
+// The larger of the two, a NaN if either is one: ReLU with floor 0, nothing with
+// floor -infinity.
+__device__ __forceinline__ float at_least(float v, float floor) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(floor));
+    return r;
 }
 
-// Four neighbouring elements of a row of C, as one store where they lie so.
-__device__ __forceinline__ void store_c4(const Mx4Params& p, int64_t row, int64_t col, float4 v, const float (&bias)[4]) {
-    float x[4] = {v.x, v.y, v.z, v.w};
-    const int64_t at = row * p.ldc + col;
-    const uintptr_t addr = reinterpret_cast<uintptr_t>(p.c) + at * (p.out_bf16 ? 2 : 4);
-    if (col + 3 < p.n && (addr & (p.out_bf16 ? 7 : 15)) == 0) {
+__device__ __forceinline__ void load_bias4(const Mx4Params& p, int64_t col, float (&bias)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] += bias[i];
-            if (p.relu) x[i] = x[i] < 0.0f ? 0.0f : x[i];
-        }
-        if (p.out_bf16) {
-            const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-            *reinterpret_cast<uint2*>(addr) =
-                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-        } else {
-            *reinterpret_cast<float4*>(addr) = make_float4(x[0], x[1], x[2], x[3]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (col + i < p.n) store_c(p, row, col + i, x[i], bias[i]);
-    }
+    for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? __ldg(p.bias + col + i) : 0.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_one(T* c, float v) {
+    if constexpr (sizeof(T) == 2)
+        *c = __float2bfloat16_rn(v);
+    else
+        *c = v;
 }
 
 // Where the 16-byte piece of a row of 256 sums lies, pieces exchanged within eight
@@ -193,16 +179,20 @@ __device__ __forceinline__ int sum_piece(int piece, int row) { return piece ^ (r
 // its shared memory; the tokens are dealt out over the splits (this one is number
 // `split`) and their warps.  A lane takes four columns; four tokens are
 // under way at a time, since a read from another SM takes most of a microsecond.
-template <bool WIDE = false>
-__device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t stride,
-                                           uint32_t offset, uint32_t split, int warp, int warps, int64_t row0, int count,
-                                           int64_t col, int lane, int piece = 0) {
+template <typename T, bool WIDE>
+__device__ __forceinline__ void add_splits_as(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t stride,
+                                              uint32_t offset, uint32_t split, int warp, int warps, int64_t row0, int count,
+                                              int64_t col, const float (&bias)[4], int lane, int piece) {
     constexpr int U = 4;
-    float bias[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? p.bias[col + i] : 0.0f;
+    const float floor = p.relu ? 0.0f : -INFINITY;
     const int step = warps * (int)splits;
-    for (int c = (int)split + warp * (int)splits; c < count; c += U * step) {
+    int c = (int)split + warp * (int)splits;
+    T* to = static_cast<T*>(p.c) + (row0 + c) * p.ldc + col;
+    const int64_t ld = p.ldc * step;
+    // four neighbouring elements of a row as one store, where they lie so in every row
+    const bool whole = col + 3 < p.n && p.access >= 4 * (int)sizeof(T);
+    const int left = (int)max((int64_t)0, min((int64_t)4, p.n - col));
+    for (; c < count; c += U * step, to += U * ld) {
         float4 v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -226,9 +216,36 @@ __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, ui
                 }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c + u * step < count) store_c4(p, row0 + c + u * step, col, v[u], bias);
+        for (int u = 0; u < U; ++u) {
+            if (c + u * step >= count) continue;
+            T* at = to + u * ld;
+            const float x[4] = {at_least(v[u].x + bias[0], floor), at_least(v[u].y + bias[1], floor),
+                                at_least(v[u].z + bias[2], floor), at_least(v[u].w + bias[3], floor)};
+            if (whole) {
+                if constexpr (sizeof(T) == 2) {
+                    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+                    *reinterpret_cast<uint2*>(at) =
+                        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                } else {
+                    *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < left) store_one(at + i, x[i]);
+            }
+        }
     }
+}
+
+template <bool WIDE = false>
+__device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t stride,
+                                           uint32_t offset, uint32_t split, int warp, int warps, int64_t row0, int count,
+                                           int64_t col, const float (&bias)[4], int lane, int piece = 0) {
+    if (p.out_bf16)
+        add_splits_as<__nv_bfloat16, WIDE>(p, sums, splits, stride, offset, split, warp, warps, row0, count, col, bias, lane, piece);
+    else
+        add_splits_as<float, WIDE>(p, sums, splits, stride, offset, split, warp, warps, row0, count, col, bias, lane, piece);
 }
 
 // ------------------------------------------------------------ one-CTA kernel
@@ -303,6 +320,8 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     // a programmatic dependent launch: the set-up above touched no global memory
     pdl_wait();
     pdl_launch_dependents();
+    float bias[4];  // of the lane's columns of the epilogue
+    load_bias4(p, (int64_t)tn * 128 + lane * 4, bias);
 
     if (warp == 0 && lane == 0) {
         int issued = 0;
@@ -398,7 +417,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     {
         const int64_t row0 = (int64_t)tm * TN;
         add_splits(p, smem_u32(smem), ranks, 1, 0, rank, warp, kThreads1 / 32, row0, (int)min((int64_t)TN, p.m - row0),
-                   (int64_t)tn * 128 + lane * 4, lane);
+                   (int64_t)tn * 128 + lane * 4, bias, lane);
     }
     if (ranks > 1) sync_cluster();  // the sums are read before any CTA exits
     __syncthreads();
@@ -471,51 +490,43 @@ __device__ __forceinline__ void pair_tile(const Mx4Params& p, int t, int& tm, in
     tn = in / rows;
 }
 
-// 32 neighbouring elements of a row of C from `bias` on; ACCESS: bytes that every
-// such piece's address is a multiple of (32, 16, or 0: element by element).
+// 128 neighbouring elements of a row of C.  ACCESS: bytes that every 32 of them are
+// aligned to (32, 16, or 0: element by element).
 template <typename T, int ACCESS>
-__device__ __forceinline__ void store_row32(T* c, int64_t left, const float* bias, bool relu, const float (&v)[32]) {
-    if (left <= 0) return;
-    float x[32];
+__device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias, float floor, float (&v)[4][32]) {
+    constexpr int E = (ACCESS == 16 ? 16 : 32) / (int)sizeof(T);  // elements of a store
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(bias + i);
-        x[i] = v[i] + b.x, x[i + 1] = v[i + 1] + b.y, x[i + 2] = v[i + 2] + b.z, x[i + 3] = v[i + 3] + b.w;
-    }
-    if (relu)
+    for (int k = 0; k < 128; k += E) {
+        float x[E];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = x[i] < 0.0f ? 0.0f : x[i];  // keeps a NaN
-    if (ACCESS > 0 && left >= 32) {
-        constexpr int WORDS = 8 * (int)sizeof(T);
-        uint32_t w[WORDS];
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            if constexpr (sizeof(T) == 2) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                w[i] = __float_as_uint(x[i]);
-            }
+        for (int i = 0; i < E; i += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + k + i);
+            const float* y = &v[k / 32][k % 32 + i];
+            x[i] = at_least(y[0] + b.x, floor), x[i + 1] = at_least(y[1] + b.y, floor);
+            x[i + 2] = at_least(y[2] + b.z, floor), x[i + 3] = at_least(y[3] + b.w, floor);
         }
+        if (ACCESS > 0 && left >= k + E) {
+            uint32_t w[E * sizeof(T) / 4];
 #pragma unroll
-        for (int i = 0; i < WORDS; i += ACCESS == 32 ? 8 : 4) {
-            uint32_t* p = reinterpret_cast<uint32_t*>(c) + i;
+            for (int i = 0; i < (int)(E * sizeof(T) / 4); ++i) {
+                if constexpr (sizeof(T) == 2) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    w[i] = __float_as_uint(x[i]);
+                }
+            }
             if constexpr (ACCESS == 32)
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[i]), "r"(w[i + 1]),
-                             "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(c + k), "r"(w[0]), "r"(w[1]),
+                             "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                              : "memory");
             else
-                *reinterpret_cast<uint4*>(p) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-        }
-    } else {
+                *reinterpret_cast<uint4*>(c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < left) {
-                if constexpr (sizeof(T) == 2)
-                    c[i] = __float2bfloat16_rn(x[i]);
-                else
-                    c[i] = x[i];
-            }
+            for (int i = 0; i < E; ++i)
+                if (k + i < left) store_one(c + k + i, x[i]);
+        }
     }
 }
 
@@ -701,21 +712,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                 continue;
             }
             if (row >= p.m) continue;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int64_t at = row * p.ldc + col0 + c * 32, left = p.n - col0 - c * 32;
-                const bool relu = p.relu;
-                if (p.out_bf16) {
-                    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.c) + at;
-                    if (p.access == 32) store_row32<__nv_bfloat16, 32>(to, left, bias + c * 32, relu, v[c]);
-                    else if (p.access == 16) store_row32<__nv_bfloat16, 16>(to, left, bias + c * 32, relu, v[c]);
-                    else store_row32<__nv_bfloat16, 0>(to, left, bias + c * 32, relu, v[c]);
-                } else {
-                    float* to = static_cast<float*>(p.c) + at;
-                    if (p.access == 32) store_row32<float, 32>(to, left, bias + c * 32, relu, v[c]);
-                    else if (p.access == 16) store_row32<float, 16>(to, left, bias + c * 32, relu, v[c]);
-                    else store_row32<float, 0>(to, left, bias + c * 32, relu, v[c]);
-                }
+            const int64_t at = row * p.ldc + col0, left = p.n - col0;
+            const float floor = p.relu ? 0.0f : -INFINITY;
+            if (p.out_bf16) {
+                __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.c) + at;
+                if (p.access == 32) store_row<__nv_bfloat16, 32>(to, left, bias, floor, v);
+                else if (p.access == 16) store_row<__nv_bfloat16, 16>(to, left, bias, floor, v);
+                else store_row<__nv_bfloat16, 0>(to, left, bias, floor, v);
+            } else {
+                float* to = static_cast<float*>(p.c) + at;
+                if (p.access == 32) store_row<float, 32>(to, left, bias, floor, v);
+                else if (p.access == 16) store_row<float, 16>(to, left, bias, floor, v);
+                else store_row<float, 0>(to, left, bias, floor, v);
             }
         }
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
@@ -729,9 +737,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         const int64_t row0 = (int64_t)tm * 256 + rank * 128;
         const int count = (int)max((int64_t)0, min((int64_t)128, p.m - row0));
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h)
-            add_splits<true>(p, smem_u32(smem), splits, 2, rank, split, warp, kPairThreads / 32, row0, count,
-                             (int64_t)tn * 256 + h * 128 + lane * 4, lane, h * 32);
+        for (int h = 0; h < 2; ++h) {
+            const int64_t col = (int64_t)tn * 256 + h * 128 + lane * 4;
+            float bias[4];
+            load_bias4(p, col, bias);
+            add_splits<true>(p, smem_u32(smem), splits, 2, rank, split, warp, kPairThreads / 32, row0, count, col, bias, lane,
+                             h * 32);
+        }
         sync_cluster();
     }
     __syncthreads();
@@ -754,7 +766,14 @@ __global__ void bias_kernel(Mx4Params p) {
     pdl_wait();
     pdl_launch_dependents();
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.m * p.n; i += (int64_t)gridDim.x * blockDim.x)
-        store_c(p, i / p.n, i % p.n, 0.0f, p.bias ? p.bias[i % p.n] : 0.0f);
+    {
+        const int64_t at = i / p.n * p.ldc + i % p.n;
+        const float v = at_least(p.bias ? p.bias[i % p.n] : 0.0f, p.relu ? 0.0f : -INFINITY);
+        if (p.out_bf16)
+            store_one(static_cast<__nv_bfloat16*>(p.c) + at, v);
+        else
+            store_one(static_cast<float*>(p.c) + at, v);
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -828,8 +847,6 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int s
 
 int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int splits, cudaStream_t stream) {
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[1], &st = a.maps.scales[0];
-    const uintptr_t rows = reinterpret_cast<uintptr_t>(p.c) | (uintptr_t)(p.ldc * (p.out_bf16 ? 2 : 4));
-    p.access = (rows & 31) == 0 ? 32 : (rows & 15) == 0 ? 16 : 0;
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
@@ -884,6 +901,8 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
     p.bias = bias;
     p.relu = relu;
     p.err = ctx->dev_err;
+    const uintptr_t rows = reinterpret_cast<uintptr_t>(p.c) | (uintptr_t)(p.ldc * (p.out_bf16 ? 2 : 4));
+    p.access = (rows & 31) == 0 ? 32 : (rows & 15) == 0 ? 16 : (rows & 7) == 0 ? 8 : 0;
     RT_CUDA(cudaSetDevice(ctx->device));
     if (p.blocks == 0) {
         RT_CUDA(launch_k(ctx->pdl, bias_kernel, ctx->sm_count * 4, 256, 0, stream, p));
