@@ -169,20 +169,14 @@ __device__ __forceinline__ void store_one(T* c, float v) {
         *c = v;
 }
 
-// Where the 16-byte piece of a row of 256 sums lies, pieces exchanged within eight
-// by the row.
-__device__ __forceinline__ int sum_piece(int piece, int row) { return piece ^ (row & 7); }
-
-// Adds the splits' sums of a tile in order and stores C.  Each of `splits` CTAs of
-// the cluster (ranks `stride` apart from `offset` on) holds [token][128 columns] f32
-// (WIDE: [token][256] by sum_piece, of which the 128 from `piece` on) at `sums` of
-// its shared memory; the tokens are dealt out over the splits (this one is number
-// `split`) and their warps.  A lane takes four columns; four tokens are
-// under way at a time, since a read from another SM takes most of a microsecond.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void add_splits_as(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t stride,
-                                              uint32_t offset, uint32_t split, int warp, int warps, int64_t row0, int count,
-                                              int64_t col, const float (&bias)[4], int lane, int piece) {
+// Adds the splits' sums of a tile in order and stores C.  Each of the cluster's
+// `splits` CTAs holds [token][128 columns] f32 at `sums` of its shared memory; the
+// tokens are dealt out over the splits (this one is number `split`) and their warps.
+// A lane takes four columns from `col` on; four tokens are under way at a time.
+template <typename T>
+__device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t split, int warp,
+                                           int warps, int64_t row0, int count, int64_t col, const float (&bias)[4],
+                                           int lane) {
     constexpr int U = 4;
     const float floor = p.relu ? 0.0f : -INFINITY;
     const int step = warps * (int)splits;
@@ -198,13 +192,11 @@ __device__ __forceinline__ void add_splits_as(const Mx4Params& p, uint32_t sums,
         for (int u = 0; u < U; ++u) v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 2
         for (uint32_t r = 0; r < splits; ++r) {
-            const uint32_t at = in_cta(sums, offset + r * stride);
+            const uint32_t at = in_cta(sums + lane * 16, r);
             float4 x[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int row = c + u * step;
-                if (row < count)
-                    x[u] = ld_cluster4(at + (WIDE ? row * 1024 + sum_piece(piece + lane, row) * 16 : row * 512 + lane * 16));
+                if (c + u * step < count) x[u] = ld_cluster4(at + (c + u * step) * 512);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -238,45 +230,32 @@ __device__ __forceinline__ void add_splits_as(const Mx4Params& p, uint32_t sums,
     }
 }
 
-template <bool WIDE = false>
-__device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, uint32_t splits, uint32_t stride,
-                                           uint32_t offset, uint32_t split, int warp, int warps, int64_t row0, int count,
-                                           int64_t col, const float (&bias)[4], int lane, int piece = 0) {
-    if (p.out_bf16)
-        add_splits_as<__nv_bfloat16, WIDE>(p, sums, splits, stride, offset, split, warp, warps, row0, count, col, bias, lane, piece);
-    else
-        add_splits_as<float, WIDE>(p, sums, splits, stride, offset, split, warp, warps, row0, count, col, bias, lane, piece);
-}
-
 // ------------------------------------------------------------ one-CTA kernel
 // For few tokens or little work.  The tensor cores compute C^T: 128 of W's rows are
 // the MMA's M rows and TN tokens its N columns, so a CTA computes 128 columns of C
 // for TN tokens over its share of k.  The CTAs of a cluster share one tile, split
 // along k.  Their sums meet in shared memory and
 // are added in rank order, tokens dealt out over the CTAs.
-// STAGES: a short ring for two CTAs to an SM, or one that fills the SM's shared
-// memory for one: a stage takes over a microsecond to arrive, so the ring's depth
-// sets the pace of a CTA.
-template <int TN, bool DEEP>
+template <int TN>
 struct Geo1 {
     static constexpr int T_BYTES = TN * kRowBytes;
     static constexpr int STAGE_BYTES = kWBytes + T_BYTES + 4 * kScaleTile;  // codes, two scale tiles of either side
-    static constexpr int STAGES = !DEEP ? 4 : TN == 32 ? 10 : 8;
-    static constexpr int TMEM_COLS = DEEP ? 256 : 128;  // TN, and 16 of scales a stage
+    static constexpr int STAGES = 4;
+    static constexpr int TMEM_COLS = 256;  // two accumulators of TN, and 16 of scales a stage
     static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
-    static_assert(TN + 16 * STAGES <= TMEM_COLS, "TMEM columns");
-    static_assert((DEEP ? 1 : 2) * SMEM <= 226 * 1024, "CTAs to an SM");
+    static_assert(2 * TN + 16 * STAGES <= TMEM_COLS, "TMEM columns");
+    static_assert(2 * SMEM <= 226 * 1024, "two CTAs to an SM");
     static_assert(TN * 512 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
 };
 
 constexpr int kThreads1 = 192;  // warps: 0 TMA, 1 MMA, 2-5 epilogue (one TMEM lane quadrant each)
 
-template <int TN, bool DEEP>
+template <int TN>
 __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ CUtensorMap map_w,
                                                         const __grid_constant__ CUtensorMap map_t,
                                                         const __grid_constant__ CUtensorMap map_sw,
                                                         const __grid_constant__ CUtensorMap map_st, Mx4Params p) {
-    using G = Geo1<TN, DEEP>;
+    using G = Geo1<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* smem_w = smem;
@@ -323,24 +302,29 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     float bias[4];  // of the lane's columns of the epilogue
     load_bias4(p, (int64_t)tn * 128 + lane * 4, bias);
 
-    if (warp == 0 && lane == 0) {
-        int issued = 0;
+    if (warp == 0) {
+        const uint32_t w0 = smem_u32(smem_w), t0 = smem_u32(smem_t), sc0 = smem_u32(smem_s);
+        const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
+        int slot = 0, phase = 1, issued = 0;
         bool ok = true;
         for (int s = s0; s < s1; ++s, ++issued) {
-            const int slot = issued % G::STAGES;
-            if (!mbar_wait(smem_u32(&empty[slot]), ((issued / G::STAGES) & 1) ^ 1, abort_flag)) {
-                ok = false;
-                break;
+            ok = __all_sync(0xffffffffu, mbar_wait(empty0 + slot * 8, phase, abort_flag));
+            if (!ok) break;
+            if (elect_one()) {
+                const uint32_t bar = full0 + slot * 8, ss = sc0 + slot * 4 * kScaleTile;
+                mbar_expect_tx(bar, G::STAGE_BYTES);
+                tma_load_2d(w0 + slot * kWBytes, &map_w, s * kRowBytes, tn * 128, bar);
+                tma_load_2d(t0 + slot * G::T_BYTES, &map_t, s * kRowBytes, tm * TN, bar);
+                tma_load_3d(ss, &map_sw, 0, s * 2, tn, bar);
+                tma_load_3d(ss + 2 * kScaleTile, &map_st, 0, s * 2, tm * TN / 128, bar);
             }
-            const uint32_t bar = smem_u32(&full[slot]);
-            mbar_expect_tx(bar, G::STAGE_BYTES);
-            tma_load_2d(smem_u32(smem_w + slot * kWBytes), &map_w, s * kRowBytes, tn * 128, bar);
-            tma_load_2d(smem_u32(smem_t + slot * G::T_BYTES), &map_t, s * kRowBytes, tm * TN, bar);
-            const uint32_t ss = smem_u32(smem_s + slot * 4 * kScaleTile);
-            tma_load_3d(ss, &map_sw, 0, s * 2, tn, bar);
-            tma_load_3d(ss + 2 * kScaleTile, &map_st, 0, s * 2, tm * TN / 128, bar);
+            __syncwarp();
+            if (++slot == G::STAGES) {
+                slot = 0;
+                phase ^= 1;
+            }
         }
-        if (!ok) {
+        if (!ok && elect_one()) {
             record_error(p.err, DEV_TIMEOUT_PRODUCER, blockIdx.x);
             *abort_flag = 1;
             // the copies in flight write this CTA's shared memory: let them land before it exits
@@ -352,7 +336,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
         const uint32_t token_col = (uint32_t)((tm * TN % 128) / 32);  // the tile's place in its 128-row scale tile
         const uint64_t w0 = smem_desc(smem_u32(smem_w), 16, 1024), t0 = smem_desc(smem_u32(smem_t), 16, 1024);
         const uint64_t sc0 = scale_desc(smem_u32(smem_s));
-        const uint32_t cols0 = tmem + TN;
+        const uint32_t cols0 = tmem + 2 * TN;
         bool ok = true;
         int slot = 0, phase = 0;
         for (int s = s0; s < s1; ++s) {
@@ -372,8 +356,9 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
                     if (kk < steps)
-                        mma_mx4<1>(tmem, w + kk * 2, t + kk * 2, mx4_idesc(128, TN, kk & 1), cols + (kk >> 1) * 4,
-                                   cols + 8 + (kk >> 1) * 4 + token_col, (s > s0 || kk > 0) ? 1u : 0u);
+                        mma_mx4<1>(tmem + (kk & 1) * TN, w + kk * 2, t + kk * 2, mx4_idesc(128, TN, kk & 1),
+                                   cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 4 + token_col,
+                                   (s > s0 || kk > 1) ? 1u : 0u);
                 tc_commit(smem_u32(&empty[slot]));
             }
             __syncwarp();
@@ -400,9 +385,16 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
         __syncwarp();
         tc_fence_after();
         float* sums = reinterpret_cast<float*>(smem) + quad * 32 + lane;  // [token][128 columns]; every stage has been read
+        const bool two = s1 - s0 > 1 || p.blocks - s0 * kStageBlocks > 2;  // the second accumulator was written
         for (int c = 0; c < count && __all_sync(0xffffffffu, got); c += 32) {
             float v[32];
             tmem_ld_32x32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
+            if (two) {
+                float u[32];
+                tmem_ld_32x32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(TN + c), u);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += u[j];
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j) sums[(c + j) * 128] = v[j];
         }
@@ -415,9 +407,12 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     else
         __syncthreads();
     {
-        const int64_t row0 = (int64_t)tm * TN;
-        add_splits(p, smem_u32(smem), ranks, 1, 0, rank, warp, kThreads1 / 32, row0, (int)min((int64_t)TN, p.m - row0),
-                   (int64_t)tn * 128 + lane * 4, bias, lane);
+        const int64_t row0 = (int64_t)tm * TN, col = (int64_t)tn * 128 + lane * 4;
+        const int count = (int)min((int64_t)TN, p.m - row0);
+        if (p.out_bf16)
+            add_splits<__nv_bfloat16>(p, smem_u32(smem), ranks, rank, warp, kThreads1 / 32, row0, count, col, bias, lane);
+        else
+            add_splits<float>(p, smem_u32(smem), ranks, rank, warp, kThreads1 / 32, row0, count, col, bias, lane);
     }
     if (ranks > 1) sync_cluster();  // the sums are read before any CTA exits
     __syncthreads();
@@ -447,13 +442,9 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 // at once (0.13 us), so the next tile's MMAs wait for that only, not for the stores.
 // Persistent: tiles are dealt out round robin, the loads of the next tile run on
 // while this one's epilogue stores.
-//
-// The pairs of a cluster of more share one tile, split along k; their sums meet as
-// those of the one-CTA kernel do.
 constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of T and W, two tiles of T's scales, four of W's
 constexpr int kPairSmem = kPairStages * kPairStageBytes + 8 * 512 /* bias of each epilogue warp's columns */ + 256;
-static_assert(256 * 512 <= kPairStages * kPairStageBytes, "the split sums reuse the stages");
 constexpr int kPairThreads = 320;  // warps: 0 TMA, 1 MMA (leader), 2-9 epilogue (two to a TMEM lane quadrant)
 static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
 static_assert(256 + 24 * kPairStages <= 512, "TMEM columns");
@@ -551,12 +542,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     volatile int* issued_all = abort_flag + 1;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    // a cluster is one pair, or the pairs of a tile's splits along k
-    const uint32_t cluster_rank = cta_rank(), ctas = cluster_size();
-    const uint32_t rank = cluster_rank & 1, leader = cluster_rank & ~1u, split = cluster_rank >> 1, splits = ctas >> 1;
-    const int cluster = (int)(blockIdx.x / ctas), clusters = (int)(gridDim.x / ctas);
+    const uint32_t rank = cta_rank();
+    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
     const int tiles = p.tiles_m * p.tiles_n;
-    const int s0 = (int)split * p.stages_per_split, s1 = min(p.stages, s0 + p.stages_per_split);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -590,45 +578,53 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     auto raise_abort = [&](int code) {
         record_error(p.err, code, blockIdx.x);
         *abort_flag = 1;
-        store_cluster(in_cta(smem_u32((const void*)abort_flag), cluster_rank ^ 1u), 1u);
+        store_cluster(in_cta(smem_u32((const void*)abort_flag), rank ^ 1u), 1u);
     };
 
-    if (warp == 0 && lane == 0) {
-        int issued = 0;
+    if (warp == 0) {
+        const uint32_t w0 = smem_u32(smem_w), t0 = smem_u32(smem_t), sc0 = smem_u32(smem_s);
+        const uint32_t full0 = smem_u32(full), leader_full0 = in_cta(full0, 0), empty0 = smem_u32(empty);
+        int slot = 0, phase = 1, issued = 0;
         bool ok = true;
         for (int t = cluster; t < tiles && ok; t += clusters) {
             int tm, tn;
             pair_tile(p, t, tm, tn);
-            for (int s = s0; s < s1; ++s) {
-                const int slot = issued % S;
-                if (!mbar_wait(smem_u32(&empty[slot]), ((issued / S) & 1) ^ 1, abort_flag)) {
-                    ok = false;
-                    break;
+            const int w_row = tn * 256 + (int)rank * 128, t_row = tm * 256 + (int)rank * 128;
+            for (int s = 0; s < p.stages; ++s) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + slot * 8, phase, abort_flag));
+                if (!ok) break;
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(full0 + slot * 8, 2 * kPairStageBytes);
+                    const uint32_t bar = leader_full0 + slot * 8, ss = sc0 + slot * 6 * kScaleTile;
+                    tma_pair_2d(w0 + slot * kWBytes, &map_w, s * kRowBytes, w_row, bar);
+                    tma_pair_2d(t0 + slot * kWBytes, &map_t, s * kRowBytes, t_row, bar);
+                    tma_pair_3d(ss, &map_st, 0, s * 2, tm * 2 + (int)rank, bar);
+                    tma_pair_3d(ss + 2 * kScaleTile, &map_sw, 0, s * 2, tn * 2, bar);
                 }
-                if (rank == 0) mbar_expect_tx(smem_u32(&full[slot]), 2 * kPairStageBytes);
-                const uint32_t bar = in_cta(smem_u32(&full[slot]), leader);
-                tma_pair_2d(smem_u32(smem_w + slot * kWBytes), &map_w, s * kRowBytes, tn * 256 + (int)rank * 128, bar);
-                tma_pair_2d(smem_u32(smem_t + slot * kWBytes), &map_t, s * kRowBytes, tm * 256 + (int)rank * 128, bar);
-                const uint32_t ss = smem_u32(smem_s + slot * 6 * kScaleTile);
-                tma_pair_3d(ss, &map_st, 0, s * 2, tm * 2 + (int)rank, bar);
-                tma_pair_3d(ss + 2 * kScaleTile, &map_sw, 0, s * 2, tn * 2, bar);
+                __syncwarp();
                 ++issued;
+                if (++slot == S) {
+                    slot = 0;
+                    phase ^= 1;
+                }
             }
         }
-        *issued_all = issued;
-        if (!ok) raise_abort(DEV_TIMEOUT_PRODUCER);
+        if (elect_one()) {
+            *issued_all = issued;
+            if (!ok) raise_abort(DEV_TIMEOUT_PRODUCER);
+        }
     } else if (warp == 1 && rank == 0) {
         const uint64_t w0 = smem_desc(smem_u32(smem_w), 16, 1024), t0 = smem_desc(smem_u32(smem_t), 16, 1024);
         const uint64_t sc0 = scale_desc(smem_u32(smem_s));
-        const uint32_t empty0 = smem_u32(empty), empty1 = in_cta(empty0, leader + 1);
-        const uint32_t tfull0 = smem_u32(tfull), tfull1 = in_cta(tfull0, leader + 1);
+        const uint32_t empty0 = smem_u32(empty), empty1 = in_cta(empty0, 1);
+        const uint32_t tfull0 = smem_u32(tfull), tfull1 = in_cta(tfull0, 1);
         int slot = 0, phase = 0, done = 0;
         bool ok = true;
         for (int t = cluster; t < tiles && ok; t += clusters, ++done) {
             ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(tempty), (done & 1) ^ 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            for (int s = s0; s < s1; ++s) {
+            for (int s = 0; s < p.stages; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), phase, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
@@ -647,7 +643,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                     for (int kk = 0; kk < 4; ++kk)
                         if (kk < steps)
                             mma_mx4<2>(tmem, td + kk * 2, wd + kk * 2, mx4_idesc(256, 256, kk & 1),
-                                       cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8, (s > s0 || kk > 0) ? 1u : 0u);
+                                       cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8, (s > 0 || kk > 0) ? 1u : 0u);
                     commit_pair(empty0 + slot * 8);
                     commit_pair(empty1 + slot * 8);
                 }
@@ -698,19 +694,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             tmem_ld_wait(v);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), leader));
-            if (splits > 1) {
-                // the tile's sums over the stages, which have all been read: [token][256 columns],
-                // the 16-byte pieces of a row exchanged so that 8 lanes' rows take all banks
-                float* sums = reinterpret_cast<float*>(smem) + (quad * 32 + lane) * 256;
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4*>(sums + sum_piece(half * 32 + c * 8 + j / 4, lane) * 4) =
-                            make_float4(v[c][j], v[c][j + 1], v[c][j + 2], v[c][j + 3]);
-                continue;
-            }
+            if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), 0));
             if (row >= p.m) continue;
             const int64_t at = row * p.ldc + col0, left = p.n - col0;
             const float floor = p.relu ? 0.0f : -INFINITY;
@@ -729,23 +713,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
     }
     __syncwarp();
-    if (splits > 1) {
-        // one tile to a cluster (the launch sees to it)
-        sync_cluster();
-        int tm, tn;
-        pair_tile(p, cluster, tm, tn);
-        const int64_t row0 = (int64_t)tm * 256 + rank * 128;
-        const int count = (int)max((int64_t)0, min((int64_t)128, p.m - row0));
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-            const int64_t col = (int64_t)tn * 256 + h * 128 + lane * 4;
-            float bias[4];
-            load_bias4(p, col, bias);
-            add_splits<true>(p, smem_u32(smem), splits, 2, rank, split, warp, kPairThreads / 32, row0, count, col, bias, lane,
-                             h * 32);
-        }
-        sync_cluster();
-    }
     __syncthreads();
     if (*abort_flag && rank == 0 && threadIdx.x == 0) {
         // the pair's copies complete on the leader's barriers: wait for the last ones issued
@@ -816,9 +783,9 @@ int mx4_encode_maps(rt_mx4* q) {
 
 namespace {
 
-template <int TN, bool DEEP>
+template <int TN>
 int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int splits, cudaStream_t stream) {
-    using G = Geo1<TN, DEEP>;
+    using G = Geo1<TN>;
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[TN / 64], &sw = b.maps.scales[0], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + TN - 1) / TN);
     p.tiles_n = (int)((p.n + 127) / 128);
@@ -840,21 +807,19 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int s
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 2 : 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<TN, DEEP>, w, t, sw, st, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<TN>, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
 }
 
-int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int splits, cudaStream_t stream) {
+int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaStream_t stream) {
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[1], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    RT_CHECK(tiles <= INT32_MAX / 16, "rt_mx4_matmul: C is too large");
-    p.stages_per_split = (p.stages + splits - 1) / splits;
-    splits = (p.stages + p.stages_per_split - 1) / p.stages_per_split;
+    RT_CHECK(tiles <= INT32_MAX, "rt_mx4_matmul: C is too large");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * (splits > 1 ? tiles * splits : std::min<int64_t>(tiles, ctx->sm_count / 2))));
+    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
     cfg.blockDim = dim3(kPairThreads);
     cfg.dynamicSmemBytes = kPairSmem;
     cfg.stream = stream;
@@ -862,7 +827,7 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int 
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2 * splits;
+    attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -872,20 +837,18 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int 
     return RT_OK;
 }
 
-template <int TN, bool DEEP>
+template <int TN>
 int allow_smem() {
-    RT_CUDA(cudaFuncSetAttribute(mx4_kernel<TN, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<TN, DEEP>::SMEM));
+    RT_CUDA(cudaFuncSetAttribute(mx4_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<TN>::SMEM));
     return RT_OK;
 }
 
 }  // namespace
 
 int gemm_mx4_init() {
-    RT_TRY((allow_smem<32, false>()));
-    RT_TRY((allow_smem<64, false>()));
-    RT_TRY((allow_smem<32, true>()));
+    RT_TRY(allow_smem<32>());
     RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    return allow_smem<64, true>();
+    return allow_smem<64>();
 }
 
 int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
@@ -909,15 +872,20 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
         count_launch(ctx);
         return RT_OK;
     }
-    const int64_t pairs = ((p.m + 255) / 256) * ((p.n + 255) / 256);
-    if (pairs * 4 >= ctx->sm_count) return launch_pair(ctx, a, b, p, 1, stream);
+    // One-CTA tiles while they fit the device at once, two to an SM (2047 x 1000 x
+    // 8192: 14.4 us against 16.5 with pairs; 256 x 8192 x 2048: 7.5 / 9.2), else pairs,
+    // which load half as much per MMA (1024 x 4096 x 1024: 8.6 / 11.5; 2048^3: 9.8 /
+    // 13.9).
     const int tn = p.m <= 32 ? 32 : 64;
-    const int64_t tiles = ((p.m + tn - 1) / tn) * ((p.n + 127) / 128);
-    // split k while the CTAs fit two to an SM and each keeps two stages
+    const int64_t tiles = ((p.m + tn - 1) / tn) * ((p.n + 127) / 128), slots = 2 * (int64_t)ctx->sm_count;
+    if (tiles > slots) return launch_pair(ctx, a, b, p, stream);
+    // Split k until a CTA has at most 8 stages, within those slots: joining the
+    // splits costs about 2 us, a stage 0.25 (1024 x 1024 x 8192, 32 stages: 11.2 us in
+    // two, 13.1 in one; 1024^3, 4 stages: 7.1 / 5.6).
     int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 2 * (int64_t)ctx->sm_count && p.stages >= 4 * splits) splits *= 2;
-    if (tn == 32) return launch_one<32, false>(ctx, a, b, p, splits, stream);
-    return launch_one<64, false>(ctx, a, b, p, splits, stream);
+    while (splits < 8 && p.stages > 8 * splits && tiles * splits * 2 <= slots) splits *= 2;
+    if (tn == 32) return launch_one<32>(ctx, a, b, p, splits, stream);
+    return launch_one<64>(ctx, a, b, p, splits, stream);
 }
 
 }  // namespace rt
