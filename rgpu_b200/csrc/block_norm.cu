@@ -13,6 +13,7 @@
 //   dgamma_post = s g A,  dbeta_post = s g B,  dgate = s (gamma_post A + beta_post B)
 // (g = 1 where w holds it; the [1,1] gate's gradient sums dgate over columns).
 #include <algorithm>
+#include <initializer_list>
 
 #include "mx4.cuh"
 #include "tc_common.cuh"
@@ -1418,6 +1419,11 @@ __global__ void __launch_bounds__(256) gate_one_kernel(const float* row, int64_t
 }
 
 // --------------------------------------------------------------- host side
+int check_ctx(const rt_ctx* ctx, std::initializer_list<const rt_tensor*> ts) {
+    for (const rt_tensor* t : ts) RT_CHECK(!t || t->ctx == ctx, "tensor belongs to another context");
+    return RT_OK;
+}
+
 int check_like(const char* what, const rt_tensor* t, const rt_tensor* r) {
     RT_CHECK(t->dtype == r->dtype, "%s must have r's type", what);
     RT_CHECK(t->rows == r->rows && t->cols == r->cols, "%s is %lldx%lld, not %lldx%lld", what, (long long)t->rows,
@@ -1663,6 +1669,8 @@ extern "C" {
 
 int rt_block_forward(rt_ctx* ctx, const rt_block_args* a) {
     RT_CHECK(ctx && a && a->r, "rt_block_forward: bad arguments");
+    RT_TRY(check_ctx(ctx, {a->r, a->y, a->gate, a->z, a->h, a->post.gamma, a->post.beta, a->pre.gamma, a->pre.beta}));
+    RT_CHECK(!a->hq || a->hq->ctx == ctx, "tensor belongs to another context");
     BlockP p{};
     RT_TRY(block_params(a, a->r, &p));
     p.r = a->r->ptr;
@@ -1699,6 +1707,8 @@ int64_t rt_block_backward_workspace(rt_ctx* ctx, int64_t m, int64_t n) {
 
 int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads* g) {
     RT_CHECK(ctx && a && g, "rt_block_backward: bad arguments");
+    RT_TRY(check_ctx(ctx, {a->r, a->y, a->gate, a->z, a->post.gamma, a->post.beta, a->pre.gamma, a->pre.beta, g->dz, g->dh,
+                           g->dr, g->dy, g->dgamma_post, g->dbeta_post, g->dgamma_pre, g->dbeta_pre, g->dgate, g->work}));
     const rt_tensor* z = a->z ? a->z : a->r;
     RT_CHECK(z && (a->z || !a->y), "rt_block_backward: z is needed where there is a y");
     BlockP p{};

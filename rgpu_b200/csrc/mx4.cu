@@ -488,6 +488,7 @@ void* rt_mx4_scales(const rt_mx4* q) { return q ? q->scales : nullptr; }
 
 int rt_mx4_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_mx4* dst) {
     RT_CHECK(ctx && src && dst, "rt_mx4_quantize: bad arguments");
+    RT_CHECK(src->ctx == ctx && dst->ctx == ctx, "tensor belongs to another context");
     RT_CHECK(axis == 0 || axis == 1, "rt_mx4_quantize: axis must be 0 or 1 (got %d)", axis);
     RT_CHECK(src->dtype == RT_F32 || src->dtype == RT_BF16, "rt_mx4_quantize: src must be f32 or bf16");
     const int64_t rows = axis == 1 ? src->rows : src->cols, k = axis == 1 ? src->cols : src->rows;
@@ -501,6 +502,7 @@ int rt_mx4_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_mx4* dst) {
 
 int rt_mx4_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst) {
     RT_CHECK(ctx && q && dst, "rt_mx4_dequantize: bad arguments");
+    RT_CHECK(q->ctx == ctx && dst->ctx == ctx, "tensor belongs to another context");
     RT_CHECK(dst->dtype == RT_F32 || dst->dtype == RT_BF16, "rt_mx4_dequantize: dst must be f32 or bf16");
     RT_CHECK(q->rows == dst->rows && q->k == dst->cols, "rt_mx4_dequantize: q is %lldx%lld, dst %lldx%lld",
              (long long)q->rows, (long long)q->k, (long long)dst->rows, (long long)dst->cols);
@@ -511,6 +513,8 @@ int rt_mx4_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst) {
 
 int rt_mx4_matmul(rt_ctx* ctx, const rt_mx4* a, const rt_mx4* b, rt_tensor* c, const rt_tensor* bias, int relu) {
     RT_CHECK(ctx && a && b && c, "rt_mx4_matmul: bad arguments");
+    RT_CHECK(a->ctx == ctx && b->ctx == ctx && c->ctx == ctx && (!bias || bias->ctx == ctx),
+             "tensor belongs to another context");
     RT_CHECK(c->dtype == RT_F32 || c->dtype == RT_BF16, "rt_mx4_matmul: C must be f32 or bf16");
     RT_CHECK(a->k == b->k, "rt_mx4_matmul: A is %lldx%lld, B %lldx%lld: the second extents differ", (long long)a->rows,
              (long long)a->k, (long long)b->rows, (long long)b->k);

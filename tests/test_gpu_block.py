@@ -400,5 +400,10 @@ def test_refusals(gpu):
     refused("without dh", bw, f, y=f, pre=rms, dz=f, dgamma_pre=v, work=work)
     refused("work must be", bw, f, y=f, post=rms, dz=f, dgamma_post=v)
     refused("work must be", bw, f, y=f, post=rms, dz=f, dgamma_post=v, work=gpu.zeros((8,)))
-    f.free()
-    refused("after free", fw, f, y=f, z=f)
+    other = rgpu_b200.Gpu(0)
+    refused("another context", fw, f, pre=rms, h=other.zeros((4, 64)))
+    refused("another context", fw, f, pre=rms, hq=other.mx4_zeros(4, 64))
+    refused("another context", bw, f, dz=f, dr=other.zeros((4, 64)))
+    y = gpu.zeros((4, 64))
+    y.free()
+    refused("after free", fw, f, y=y, z=f)

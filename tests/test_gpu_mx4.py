@@ -284,5 +284,9 @@ def test_refusals(gpu):
     refused(lambda: gpu.mx4_zeros(1 << 31, 4), "2^31")
     refused(lambda: gpu.mx4_wrap(q.codes_ptr + 8, q.scales_ptr, 4, 64), "16-byte aligned")
     refused(lambda: gpu.mx4_wrap(0, q.scales_ptr, 4, 64), "NULL")
+    other = rgpu_b200.Gpu(0)
+    refused(lambda: gpu.mx4_quantize(f, other.mx4_zeros(4, 64)), "another context")
+    refused(lambda: gpu.mx4_dequantize(q, other.zeros((4, 64))), "another context")
+    refused(lambda: gpu.mx4_matmul(q, q, gpu.zeros((4, 4)), bias=other.zeros((1, 4))), "another context")
     f.free()
     refused(lambda: gpu.block_forward(f, h=gpu.zeros((4, 64))), "")
