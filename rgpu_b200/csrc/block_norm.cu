@@ -26,6 +26,9 @@ namespace {
 
 enum GateMode : int { GATE_NONE = 0, GATE_ONE = 1, GATE_ROW = 2, GATE_COLUMN = 3, GATE_FULL = 4 };
 
+// Stride of a vector of partial sums: whole eights.
+__host__ __device__ constexpr int64_t columns(int64_t n) { return (n + 7) & ~int64_t(7); }
+
 struct NormP {
     int kind;
     float eps;
@@ -54,7 +57,7 @@ struct GradP {
     int64_t lddr, lddy;
     void* dgate;       // column and full gates (y's type under GATE_FULL)
     int64_t lddg;
-    float* partials;   // [parts][4][n]: A, B, sum dh z^, sum dh of each CTA's rows
+    float* partials;   // [parts][4][columns(n)]: A, B, sum dh z^, sum dh of each CTA's rows
     int sums;          // bit i: sum i is wanted
 };
 
@@ -135,7 +138,23 @@ __device__ __forceinline__ float gate_at(const BlockP& p, int64_t row, int64_t j
     }
 }
 
-// One CTA per row at a time, any width: the row is read once per pass.
+// One block of 32 in 4 bits by a whole warp, a lane's element h at j.
+__device__ __forceinline__ void store_block(const BlockP& p, int64_t row, int j, int blocks, int groups, float h) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
+    const uint32_t byte = mx4::scale_byte(amax);
+    const float q = byte == mx4::kNanScale ? 0.0f : h * mx4::inv_scale(byte);
+    const float next = __shfl_down_sync(0xffffffffu, q, 1);
+    if ((lane & 1) == 0) p.codes[row * blocks * 16 + (j >> 1)] = (uint8_t)mx4::encode2(q, next);
+    if (lane == 0) {
+        p.scales[mx4::scale_offset(row, j >> 5, groups)] = (uint8_t)byte;
+        if ((j >> 5) == blocks - 1)
+            for (int b = blocks; b < groups * 4; ++b) p.scales[mx4::scale_offset(row, b, groups)] = 0;
+    }
+}
+
+// Rows wider than the other kernels hold: one CTA per row at a time, the row read
+// once per pass.
 template <typename T>
 __global__ void __launch_bounds__(256) forward_kernel(BlockP p) {
     __shared__ float red[8];
@@ -163,19 +182,7 @@ __global__ void __launch_bounds__(256) forward_kernel(BlockP p) {
                 if (p.h) st<T>(p.h, row * p.ldh + j, h);
             }
             if (p.codes) {
-                // a warp holds one block of 32
-                h = as_stored<T>(h);
-                const int lane = threadIdx.x & 31;
-                const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
-                const uint32_t byte = mx4::scale_byte(amax);
-                const float q = byte == mx4::kNanScale ? 0.0f : h * mx4::inv_scale(byte);
-                const float next = __shfl_down_sync(0xffffffffu, q, 1);
-                if ((lane & 1) == 0) p.codes[row * blocks * 16 + (j >> 1)] = (uint8_t)mx4::encode2(q, next);
-                if (lane == 0) {
-                    p.scales[mx4::scale_offset(row, j >> 5, groups)] = (uint8_t)byte;
-                    if ((j >> 5) == blocks - 1)
-                        for (int64_t b = blocks; b < groups * 4; ++b) p.scales[mx4::scale_offset(row, b, groups)] = 0;
-                }
+                store_block(p, row, (int)j, (int)blocks, (int)groups, as_stored<T>(h));
             }
         }
     }
@@ -187,10 +194,11 @@ __global__ void __launch_bounds__(256) backward_kernel(BlockP p, GradP g) {
     pdl_wait();
     pdl_launch_dependents();
     const int64_t n = p.n;
-    float* acc = g.partials ? g.partials + (int64_t)blockIdx.x * 4 * n : nullptr;
+    const int64_t cols = columns(n);
+    float* acc = g.partials ? g.partials + (int64_t)blockIdx.x * 4 * cols : nullptr;
     if (acc)
-        for (int64_t i = threadIdx.x; i < 4 * n; i += 256)
-            if ((g.sums >> (i / n)) & 1) acc[i] = 0.0f;
+        for (int64_t i = threadIdx.x; i < 4 * cols; i += 256)
+            if ((g.sums >> (i / cols)) & 1) acc[i] = 0.0f;
     __syncthreads();
     const float inv_n = 1.0f / (float)n;
     for (int64_t row = blockIdx.x; row < p.m; row += gridDim.x) {
@@ -244,12 +252,12 @@ __global__ void __launch_bounds__(256) backward_kernel(BlockP p, GradP g) {
                     st<T>(g.dgate, row * g.lddg + j, dt * (hat * gamma_at(p.post, j) + beta_at(p.post, j)));
                 const float w = p.gate_mode >= GATE_COLUMN ? dr * gt : dr;
                 if (g.sums & 1) acc[j] += w * hat;
-                if (g.sums & 2) acc[n + j] += w;
+                if (g.sums & 2) acc[cols + j] += w;
             }
             if (g.dh) {
                 const float dh = ld<T>(g.dh, row * g.lddh + j);
-                if (g.sums & 4) acc[2 * n + j] += dh * (z_at(j) - sz.mu) * sz.rho;
-                if (g.sums & 8) acc[3 * n + j] += dh;
+                if (g.sums & 4) acc[2 * cols + j] += dh * (z_at(j) - sz.mu) * sz.rho;
+                if (g.sums & 8) acc[3 * cols + j] += dh;
             }
             if (g.dr) st<T>(g.dr, row * g.lddr + j, dr);
         }
@@ -473,6 +481,111 @@ __global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p
     }
 }
 
+// ---------------------------------------------------- rows of any alignment
+// The same for rows that are not 16-byte aligned or whole eights (an odd width): a
+// thread holds every S-th element, so a warp's 2- or 4-byte accesses are always
+// neighbours.  E elements a thread; WARP: a warp to a row (four to a CTA), else a
+// CTA, of as many warps as the row needs.
+__device__ __forceinline__ float cta_sum(float v, float* red, int& turn) {
+    v = warp_sum(v);
+    const int lane = threadIdx.x & 31;
+    float* half = red + turn * 32;
+    turn ^= 1;
+    if (lane == 0) half[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_sum(lane < (int)(blockDim.x >> 5) ? half[lane] : 0.0f);
+}
+
+template <typename T, bool WARP, int E>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) forward_strided_kernel(BlockP p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    __shared__ float red[64];
+    int turn = 0;
+    const int S = WARP ? 32 : (int)blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const int n = (int)p.n;
+    const float inv_n = 1.0f / (float)n;
+    const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= p.m) return;  // a whole warp, and rows of a warp share no barrier
+    auto sum = [&](float v) { return WARP ? warp_sum(v) : cta_sum(v, red, turn); };
+    auto load = [&](auto x, float other, float (&v)[E]) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = i * S + t < n ? x(i * S + t) : other;
+    };
+    auto stat = [&](const NormP& norm, const float (&x)[E]) {
+        Stat s{0.0f, 1.0f};
+        if (norm.kind == RT_NORM_NONE) return s;
+        float v = 0.0f;
+        if (norm.kind == RT_NORM_LAYER) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) v += x[i];
+            s.mu = sum(v) * inv_n;
+            v = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float d = i * S + t < n ? x[i] - s.mu : 0.0f;
+            v += d * d;
+        }
+        s.rho = rsqrtf(sum(v) * inv_n + norm.eps);
+        return s;
+    };
+    // x = x^ gamma + beta
+    auto scale = [&](const Stat& s, const float (&gamma)[E], const float* beta, float (&x)[E]) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = (x[i] - s.mu) * s.rho * gamma[i];
+        if (beta) {
+            float w[E];
+            load([&](int j) { return __ldg(beta + j); }, 0.0f, w);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] += w[i];
+        }
+    };
+    // the vectors are on their way while the sums are taken; one choice for all of a
+    // thread's elements, so that their reads are under way together
+    auto vector = [&](const float* x, int stride, float (&v)[E]) {
+        if (x)
+            load([&](int j) { return __ldg(x + (int64_t)j * stride); }, 0.0f, v);
+        else
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = 1.0f;
+    };
+    float z[E], gamma[E];
+    load([&](int j) { return ld<T>(p.r, row * p.ldr + j); }, 0.0f, z);
+    if (p.y) {
+        float y[E], gate[E];
+        load([&](int j) { return ld<T>(p.y, row * p.ldy + j); }, 0.0f, y);
+        vector(p.post.gamma, 1, gamma);
+        if (p.gate_mode == GATE_FULL)
+            load([&](int j) { return ld<T>(p.gate, row * p.ldg + j); }, 0.0f, gate);
+        else
+            vector(p.gate_mode == GATE_NONE ? nullptr
+                                            : static_cast<const float*>(p.gate) + (p.gate_mode == GATE_COLUMN ? row * p.ldg : 0),
+                   p.gate_mode == GATE_ROW ? 1 : 0, gate);
+        scale(stat(p.post, y), gamma, p.post.beta, y);
+#pragma unroll
+        for (int i = 0; i < E; ++i) z[i] += i * S + t < n ? p.scale * gate[i] * y[i] : 0.0f;
+    }
+    vector(p.pre.gamma, 1, gamma);
+    const Stat s = stat(p.pre, z);
+    if (p.z)
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (i * S + t < n) st<T>(p.z, row * p.ldz + i * S + t, z[i]);
+    scale(s, gamma, p.pre.beta, z);
+    if (p.h)
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (i * S + t < n) st<T>(p.h, row * p.ldh + i * S + t, z[i]);
+    if (!p.codes) return;
+    const int blocks = (n + 31) / 32, groups = (blocks + 3) / 4;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int j = i * S + t;  // a warp holds one block of 32
+        if (i * S + (t & ~31) < n) store_block(p, row, j, blocks, groups, j < n ? as_stored<T>(z[i]) : 0.0f);
+    }
+}
+
 // ------------------------------------------------------ rows through a ring
 // For many rows: one CTA of 1024 threads (backward: 512, for the registers that its
 // sums over rows take) to an SM, its groups of TPR threads each take a row at a
@@ -489,6 +602,7 @@ struct RingP {
     int depth;         // slots of a group
     int slot_bytes;    // the row of each tensor
     int vectors;       // f32 vectors in shared memory
+    int smem;          // bytes in all: what they leave is L1
     int* err;
 };
 
@@ -650,6 +764,10 @@ __device__ __forceinline__ void floats8(const f2 (&v)[4], float (&x)[8]) {
         x[2 * i] = a.x;
         x[2 * i + 1] = a.y;
     }
+}
+// The pair with what lies past a row's end as zeros: `left` elements are in it.
+__device__ __forceinline__ f2 keep2(f2 v, int left) {
+    return left >= 2 ? v : left == 1 ? v & 0xffffffffull : 0ull;
 }
 template <typename T>
 __device__ __forceinline__ void store8(void* base, int64_t at, const f2 (&v)[4]) {
@@ -896,7 +1014,7 @@ __device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[c][i]) : sums[c][i];
                     if (k == G::COUNT - 1)
-                        a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * n + j[c]);
+                        a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * columns(n) + j[c]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) a[i] = x[i];
                 }
@@ -907,19 +1025,25 @@ __device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc
 // C: eights of a thread.  With the betas' sums a thread of sixteen columns spills
 // (and with all of shared memory taken, spills go to L2), so FULL takes eight up
 // to 4096 wide: 2047 x 1000 f32 layer norms, full gate: 45 us with C = 2.
-template <typename T, int TPR, int C, bool FULL>
+//
+// BULK: rows arrive by bulk copies, which want 16-byte aligned rows of whole eights.
+// Else the group copies a row's tensors into its one slot itself, neighbouring
+// elements by neighbouring threads, a row ending in zeros up to whole eights, and
+// its results out of it likewise; groups of a CTA hide each other's waits.
+template <typename T, int TPR, int C, bool FULL, bool BULK>
 __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p, GradP q, RingP r, int mask) {
     extern __shared__ __align__(128) uint8_t smem[];
     using G = Group<kBackThreads, TPR>;
     const int n = (int)p.n;
-    const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
+    const int cols = (int)columns(n);
+    const RingSmem sm = ring_smem(smem, r, cols, G::COUNT);
     G g;
     g.index = threadIdx.x / TPR;
     g.t = threadIdx.x % TPR;
     g.red = sm.red + g.index * 256;
     uint8_t* slots = sm.slots + (size_t)g.index * r.depth * r.slot_bytes;
     const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
-    const uint32_t row_bytes = (uint32_t)n * sizeof(T);
+    const uint32_t row_bytes = (uint32_t)cols * sizeof(T);
     const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
     const bool own_gate = FULL && (p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * r.depth);
@@ -931,15 +1055,17 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     }
     pdl_wait();
     pdl_launch_dependents();
-    float *v2 = sm.vec, *vp = v2 + (mask & 1 ? n : 0), *vb = vp + (mask & 2 ? n : 0);
-    for (int j = threadIdx.x; j < n; j += kBackThreads) {
-        if (mask & 1) v2[j] = __ldg(p.pre.gamma + j);
-        if (mask & 2) vp[j] = p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
-        if (mask & 4) vb[j] = p.scale * __ldg(p.post.beta + j);
+    float *v2 = sm.vec, *vp = v2 + (mask & 1 ? cols : 0), *vb = vp + (mask & 2 ? cols : 0);
+    for (int j = threadIdx.x; j < cols; j += kBackThreads) {
+        const bool in = BULK || j < n;
+        if (mask & 1) v2[j] = in ? __ldg(p.pre.gamma + j) : 0.0f;
+        if (mask & 2) vp[j] = in ? p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f) : 0.0f;
+        if (mask & 4) vb[j] = in ? p.scale * __ldg(p.post.beta + j) : 0.0f;
     }
     __syncthreads();
-    // the slot's rows: z, then y, dz, dh
-    const uint32_t at_y = row_bytes, at_dz = at_y + (p.y ? row_bytes : 0), at_dh = at_dz + (q.dz ? row_bytes : 0);
+    // the slot's rows: z, then y, dz, dh; not BULK: all of them, and a gate's
+    const uint32_t at_y = row_bytes, at_dz = at_y + (p.y || !BULK ? row_bytes : 0),
+                   at_dh = at_dz + (q.dz || !BULK ? row_bytes : 0), at_gate = at_dh + row_bytes;
     auto issue = [&](int64_t row, int slot) {
         const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * r.slot_bytes);
         tc::mbar_expect_tx(bar, (uint32_t)r.slot_bytes);
@@ -948,7 +1074,30 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
         if (q.dz) bulk_load(dst + at_dz, static_cast<const T*>(q.dz) + row * q.lddz, row_bytes, bar);
         if (q.dh) bulk_load(dst + at_dh, static_cast<const T*>(q.dh) + row * q.lddh, row_bytes, bar);
     };
-    if (g.t == 0)
+    // a row into the slot, or out of it, by the group (not BULK)
+    // (every read of a row before its first write: the compiler cannot tell them apart)
+    auto take_row = [&](const void* from, int64_t stride, int64_t row, T (&v)[8 * C]) {
+        const T* x = static_cast<const T*>(from) + row * stride + g.t;
+#pragma unroll
+        for (int i = 0; i < 8 * C; ++i) v[i] = i * TPR + g.t < n ? x[i * TPR] : T(0.0f);
+    };
+    auto put_slot = [&](uint32_t to, const T (&v)[8 * C]) {
+        T* d = reinterpret_cast<T*>(slots + to) + g.t;
+#pragma unroll
+        for (int i = 0; i < 8 * C; ++i)
+            if (i * TPR + g.t < cols) d[i * TPR] = v[i];
+    };
+    auto copy_out = [&](void* to, int64_t stride, int64_t row, uint32_t from) {
+        const T* x = reinterpret_cast<const T*>(slots + from) + g.t;
+        T* d = static_cast<T*>(to) + row * stride + g.t;
+        T v[8 * C];
+#pragma unroll
+        for (int i = 0; i < 8 * C; ++i) v[i] = i * TPR + g.t < n ? x[i * TPR] : T(0.0f);
+#pragma unroll
+        for (int i = 0; i < 8 * C; ++i)
+            if (i * TPR + g.t < n) d[i * TPR] = v[i];
+    };
+    if (BULK && g.t == 0)
         for (int d = 0; d < r.depth && first + d * step < p.m; ++d) issue(first + d * step, d);
     const float inv_n = 1.0f / (float)n;
     int j[C];
@@ -968,16 +1117,34 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     uint32_t phase = 0;
     const bool back = q.dh && p.pre.kind != RT_NORM_NONE;
     for (int64_t row = first; row < p.m; row += step) {
-        if (!tc::mbar_wait(full + slot * 8, phase, abort_flag)) {
-            *abort_flag = 1;
-            tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+        if constexpr (BULK) {
+            if (!tc::mbar_wait(full + slot * 8, phase, abort_flag)) {
+                *abort_flag = 1;
+                tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+            }
+        } else {
+            T a[8 * C], b[8 * C];
+            take_row(p.z, p.ldz, row, a);
+            if (p.y) take_row(p.y, p.ldy, row, b);
+            put_slot(0, a);
+            if (p.y) put_slot(at_y, b);
+            if (q.dz) take_row(q.dz, q.lddz, row, a);
+            if (q.dh) take_row(q.dh, q.lddh, row, b);
+            if (q.dz) put_slot(at_dz, a);
+            if (q.dh) put_slot(at_dh, b);
+            if (p.gate_mode == GATE_FULL) {
+                take_row(p.gate, p.ldg, row, a);
+                put_slot(at_gate, a);
+            }
+            g.sync();
         }
         const uint8_t* at = slots + (size_t)slot * r.slot_bytes;
         Raw8<T> own[FULL ? C : 1];  // a full gate's row: under way while the sums are taken
         if constexpr (FULL)
             if (p.gate_mode == GATE_FULL)
 #pragma unroll
-                for (int c = 0; c < C; ++c) own[c] = has[c] ? load_raw8<T>(p.gate, row * p.ldg + j[c]) : zero8<T>();
+                for (int c = 0; c < C; ++c)
+                    own[c] = !has[c] ? zero8<T>() : BULK ? load_raw8<T>(p.gate, row * p.ldg + j[c]) : load_raw8<T>(at + at_gate, j[c]);
         // sums of both norms: means first where there is a layer norm, then the
         // centred squares and a (z - mu)
         Stat sz{0.0f, 1.0f}, sy{0.0f, 1.0f};
@@ -1027,6 +1194,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             if (FULL) x[i] = add2(x[i], less_z);
+                            if (!BULK) x[i] = keep2(x[i], n - j[c] - 2 * i);
                             sums[0] = fma2(x[i], x[i], sums[0]);
                         }
                         if (back) {
@@ -1046,6 +1214,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             if (FULL) x[i] = add2(x[i], less_y);
+                            if (!BULK) x[i] = keep2(x[i], n - j[c] - 2 * i);
                             sums[2] = fma2(x[i], x[i], sums[2]);
                         }
                     }
@@ -1086,9 +1255,11 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                 for (int i = 0; i < 4; ++i) {
                     if (FULL) d[i] = add2(d[i], less_a0);
                     dr[i] = fma2(fma2(h[i], less_a1, d[i]), rho, dr[i]);
+                    if (!BULK) dr[i] = keep2(dr[i], n - j[c] - 2 * i);
                 }
             }
-            if (q.dr) store8<T>(q.dr, row * q.lddr + j[c], dr);
+            if (!BULK) store8<T>(slots, at_dz / sizeof(T) + j[c], dr);
+            else if (q.dr) store8<T>(q.dr, row * q.lddr + j[c], dr);
             if (!p.y) continue;
             const f2 rho = splat2(sy.rho);
             slot8<T>(at + at_y, j[c], hat[c]);
@@ -1117,7 +1288,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                 }
                 if (p.gate_mode == GATE_FULL) {
                     pairs8(own[c], gate);
-                    if (q.dgate) store8<T>(q.dgate, row * q.lddg + j[c], u);
+                    if (!BULK) store8<T>(slots, at_gate / sizeof(T) + j[c], u);
+                    else if (q.dgate) store8<T>(q.dgate, row * q.lddg + j[c], u);
                 } else {
                     const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
 #pragma unroll
@@ -1148,7 +1320,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
             g.sum(b1);
         }
         // every thread of the group has read the slot: all of it before the last barrier
-        if (g.t == 0 && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
+        if (BULK && g.t == 0 && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
         if (q.dy) {
             const f2 rho = splat2(sy.rho), add = splat2(b0), less_b1 = splat2(p.post.kind != RT_NORM_NONE ? -b1 * inv_n : 0.0f);
 #pragma unroll
@@ -1159,8 +1331,17 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                         if (FULL) b[c][i] = add2(b[c][i], add);
                         b[c][i] = mul2(fma2(hat[c][i], less_b1, b[c][i]), rho);
                     }
-                    store8<T>(q.dy, row * q.lddy + j[c], b[c]);
+                    if (BULK) store8<T>(q.dy, row * q.lddy + j[c], b[c]);
+                    else store8<T>(slots, at_y / sizeof(T) + j[c], b[c]);
                 }
+        }
+        if constexpr (!BULK) {
+            g.sync();
+            if (q.dr) copy_out(q.dr, q.lddr, row, at_dz);
+            if (q.dy) copy_out(q.dy, q.lddy, row, at_y);
+            if (q.dgate && p.gate_mode == GATE_FULL) copy_out(q.dgate, q.lddg, row, at_gate);
+            g.sync();
+            continue;
         }
         if (++slot == r.depth) {
             slot = 0;
@@ -1387,7 +1568,7 @@ __global__ void __launch_bounds__(512) column_kernel(ReduceP p) {
         for (int i = warp; i < p.parts; i += 16)
 #pragma unroll
             for (int v = 0; v < 4; ++v)
-                if ((p.sums >> v) & 1) s[v] += p.partials[((int64_t)i * 4 + v) * p.n + j];
+                if ((p.sums >> v) & 1) s[v] += p.partials[((int64_t)i * 4 + v) * columns(p.n) + j];
 #pragma unroll
     for (int v = 0; v < 4; ++v) sums[warp][v][lane] = s[v];
     __syncthreads();
@@ -1515,12 +1696,14 @@ cudaError_t launch_forward_rows(bool pdl, const BlockP& p, cudaStream_t st) {
     return launch_k(pdl, forward_rows_kernel<T, TPR, C>, (unsigned)((p.m + rows - 1) / rows), threads, 0, st, p);
 }
 
-// Fills in the ring's shape; false where not even one slot a group fits.
-bool plan_ring(RingP* r, int64_t n, int groups, int tensors, size_t es, int vectors) {
+// Fills in the ring's shape, of at most `most` slots a group; false where not even
+// one fits.
+bool plan_ring(RingP* r, int64_t n, int groups, int tensors, size_t es, int vectors, int most = 4) {
     r->slot_bytes = (int)(tensors * n * (int64_t)es);
     r->vectors = vectors;
     const int64_t room = kRingSmem - ring_scratch(groups) - (int64_t)vectors * n * 4;
-    r->depth = (int)std::min<int64_t>(4, room / ((int64_t)groups * r->slot_bytes));
+    r->depth = (int)std::min<int64_t>(most, room / ((int64_t)groups * r->slot_bytes));
+    r->smem = (int)(kRingSmem - room) + groups * r->depth * r->slot_bytes;
     return r->depth >= 1;
 }
 
@@ -1532,7 +1715,7 @@ int launch_forward_ring(rt_ctx* ctx, const BlockP& p, RingP r, int mask, cudaStr
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
     auto* kernel = full ? forward_ring_kernel<T, TPR, C, true> : forward_ring_kernel<T, TPR, C, false>;
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kRingThreads, kRingSmem, st, p, r, mask));
+    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kRingThreads, r.smem, st, p, r, mask));
     return RT_OK;
 }
 
@@ -1556,50 +1739,50 @@ int forward_ring(rt_ctx* ctx, const BlockP& p, cudaStream_t st, bool* done) {
     return launch_forward_ring<T, 512, 2>(ctx, p, r, mask, st);
 }
 
-template <typename T, int TPR, int C, bool FULL>
+template <typename T, int TPR, int C, bool FULL, bool BULK = true>
 int launch_backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, const RingP& r, int mask, int ctas, cudaStream_t st) {
-    auto* kernel = backward_ring_kernel<T, TPR, C, FULL>;
+    auto* kernel = backward_ring_kernel<T, TPR, C, FULL, BULK>;
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kBackThreads, kRingSmem, st, p, q, r, mask));
+    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kBackThreads, r.smem, st, p, q, r, mask));
     return RT_OK;
 }
 
 template <int TPR>
 int launch_backward_pipe(bool pdl, const BlockP& p, const GradP& q, const RingP& r, int ctas, cudaStream_t st) {
     RT_CUDA(cudaFuncSetAttribute(backward_pipe_kernel<TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    RT_CUDA(launch_k(pdl, backward_pipe_kernel<TPR>, (unsigned)ctas, kBackThreads, kRingSmem, st, p, q, r));
+    RT_CUDA(launch_k(pdl, backward_pipe_kernel<TPR>, (unsigned)ctas, kBackThreads, r.smem, st, p, q, r));
     return RT_OK;
 }
 
-// The backward pass through the ring where the rows are aligned and fit; *parts
-// is then the number of partials.
+// The backward pass through the ring, where a row of every tensor fits in it for
+// each group: up to 8192 wide.  *parts is then the number of partials.
 template <typename T>
 int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st, int* parts, bool* done) {
     *done = false;
     const size_t es = sizeof(T);
-    if (!rows_aligned(p, es) || p.n > 8192 || p.m == 0 || !aligned16(q.dz, q.lddz, es) || !aligned16(q.dh, q.lddh, es) ||
-        !aligned16(q.dr, q.lddr, es) || !aligned16(q.dy, q.lddy, es) || !aligned16(q.partials, 0, 4) ||
-        (p.gate_mode == GATE_FULL && !aligned16(q.dgate, q.lddg, es)))
-        return RT_OK;
+    if (p.n > 8192 || p.m == 0 || !aligned16(q.partials, 0, 4)) return RT_OK;
+    const bool bulk = rows_aligned(p, es) && aligned16(q.dz, q.lddz, es) && aligned16(q.dh, q.lddh, es) &&
+                      aligned16(q.dr, q.lddr, es) && aligned16(q.dy, q.lddy, es) &&
+                      (p.gate_mode != GATE_FULL || aligned16(q.dgate, q.lddg, es));
     const bool shared = p.gate_mode == GATE_ONE || p.gate_mode == GATE_ROW;
     const int mask = (p.pre.gamma ? 1 : 0) | (p.post.gamma || (p.y && shared) ? 2 : 0) |
                      (p.post.beta && q.dgate && !shared ? 4 : 0);
     const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
-    const int eights = full && p.n <= 4096 ? 1 : 2;
+    const int eights = (full || !bulk) && p.n <= 4096 ? 1 : 2;
     int tpr = 32;
     while (tpr * eights * 8 < p.n) tpr *= 2;
     const int groups = kBackThreads / tpr;
     RingP r{};
     r.err = ctx->dev_err;
-    if (!plan_ring(&r, p.n, groups, 1 + (p.y ? 1 : 0) + (q.dz ? 1 : 0) + (q.dh ? 1 : 0), es, __builtin_popcount(mask)))
-        return RT_OK;
+    const int tensors = bulk ? 1 + (p.y ? 1 : 0) + (q.dz ? 1 : 0) + (q.dh ? 1 : 0) : p.gate_mode == GATE_FULL ? 5 : 4;
+    if (!plan_ring(&r, columns(p.n), groups, tensors, es, __builtin_popcount(mask), bulk ? 4 : 1)) return RT_OK;
     *done = true;
     *parts = (int)std::min<int64_t>(ctx->sm_count, (p.m + groups - 1) / groups);
     if constexpr (sizeof(T) == 2) {
         RingP two{};
         two.err = ctx->dev_err;
-        if (!full && p.post.kind == RT_NORM_RMS && p.pre.kind == RT_NORM_RMS && q.dz && q.dh &&
+        if (bulk && !full && p.post.kind == RT_NORM_RMS && p.pre.kind == RT_NORM_RMS && q.dz && q.dh &&
             plan_ring(&two, p.n, groups, 4, es, 2) && two.depth >= 2) {
             switch (tpr) {
                 case 32: return launch_backward_pipe<32>(ctx->pdl, p, q, two, *parts, st);
@@ -1608,6 +1791,18 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
                 case 256: return launch_backward_pipe<256>(ctx->pdl, p, q, two, *parts, st);
                 default: return launch_backward_pipe<512>(ctx->pdl, p, q, two, *parts, st);
             }
+        }
+    }
+    if (!bulk) {
+        if (eights == 2)
+            return full ? launch_backward_ring<T, 512, 2, true, false>(ctx, p, q, r, mask, *parts, st)
+                        : launch_backward_ring<T, 512, 2, false, false>(ctx, p, q, r, mask, *parts, st);
+        switch (tpr) {
+            case 32: return launch_backward_ring<T, 32, 1, true, false>(ctx, p, q, r, mask, *parts, st);
+            case 64: return launch_backward_ring<T, 64, 1, true, false>(ctx, p, q, r, mask, *parts, st);
+            case 128: return launch_backward_ring<T, 128, 1, true, false>(ctx, p, q, r, mask, *parts, st);
+            case 256: return launch_backward_ring<T, 256, 1, true, false>(ctx, p, q, r, mask, *parts, st);
+            default: return launch_backward_ring<T, 512, 1, true, false>(ctx, p, q, r, mask, *parts, st);
         }
     }
     if (!full) switch (tpr) {
@@ -1645,12 +1840,28 @@ int forward_rows(rt_ctx* ctx, const BlockP& p, cudaStream_t st, bool* done) {
     return RT_OK;
 }
 
+template <typename T>
+int forward_strided(rt_ctx* ctx, const BlockP& p, cudaStream_t st, bool* done) {
+    *done = false;
+    if (p.n > 16384 || p.m > INT32_MAX) return RT_OK;
+    *done = true;
+    if (p.n <= 256) {
+        RT_CUDA(launch_k(ctx->pdl, forward_strided_kernel<T, true, 8>, (unsigned)((p.m + 3) / 4), 128, 0, st, p));
+    } else if (p.n <= 8192) {
+        RT_CUDA(launch_k(ctx->pdl, forward_strided_kernel<T, false, 8>, (unsigned)p.m, (unsigned)((p.n + 255) / 256 * 32), 0, st, p));
+    } else {
+        RT_CUDA(launch_k(ctx->pdl, forward_strided_kernel<T, false, 16>, (unsigned)p.m, (unsigned)((p.n + 511) / 512 * 32), 0, st, p));
+    }
+    return RT_OK;
+}
+
 // The forward pass on the kernel that fits it.
 template <typename T>
 int forward_any(rt_ctx* ctx, const BlockP& p, cudaStream_t st) {
     bool done = false;
     RT_TRY(forward_ring<T>(ctx, p, st, &done));
     if (!done) RT_TRY(forward_rows<T>(ctx, p, st, &done));
+    if (!done) RT_TRY(forward_strided<T>(ctx, p, st, &done));
     if (!done)
         RT_CUDA(launch_k(ctx->pdl, forward_kernel<T>, (unsigned)std::min<int64_t>(p.m, (int64_t)ctx->sm_count * 8), 256, 0,
                          st, p));
@@ -1702,7 +1913,7 @@ int64_t rt_block_backward_workspace(rt_ctx* ctx, int64_t m, int64_t n) {
         set_error("rt_block_backward_workspace: bad arguments");
         return -1;
     }
-    return (int64_t)parts_for(ctx, m) * 4 * n + n;
+    return ((int64_t)parts_for(ctx, m) * 4 + 1) * columns(n);
 }
 
 int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads* g) {
@@ -1780,7 +1991,7 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     bool done = false;
     RT_TRY(z->dtype == RT_BF16 ? backward_ring<__nv_bfloat16>(ctx, p, q, ctx->stream, &parts, &done)
                                : backward_ring<float>(ctx, p, q, ctx->stream, &parts, &done));
-    // without rows the sums over rows are zero: the partials of one CTA
+    // wider rows; and without rows the sums over rows are zero: the partials of one CTA
     if (!done)
         RT_CUDA(launch_k(ctx->pdl, z->dtype == RT_BF16 ? backward_kernel<__nv_bfloat16> : backward_kernel<float>, parts, 256, 0,
                          ctx->stream, p, q));
@@ -1795,7 +2006,7 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     c.scale = p.scale;
     c.gamma = p.post.gamma;
     c.beta = p.post.beta;
-    if (gate_sums && p.gate_mode == GATE_ONE) c.gate_row = q.partials + (int64_t)parts_for(ctx, p.m) * 4 * p.n;
+    if (gate_sums && p.gate_mode == GATE_ONE) c.gate_row = q.partials + (int64_t)parts_for(ctx, p.m) * 4 * columns(p.n);
     RT_CUDA(launch_k(ctx->pdl, column_kernel, (unsigned)((p.n + 31) / 32), 512, 0, ctx->stream, c));
     count_launch(ctx);
     if (c.gate_row) {

@@ -481,11 +481,45 @@ __device__ __forceinline__ void pair_tile(const Mx4Params& p, int t, int& tm, in
     tn = in / rows;
 }
 
+// A 32 x 32 exchange over the warp: lane l's v[i] for lane i's v[l].
+__device__ __forceinline__ void transpose32(float (&v)[32], int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (!(i & o)) {
+                const bool hi = lane & o;
+                const float other = __shfl_xor_sync(0xffffffffu, hi ? v[i] : v[i | o], o);
+                if (hi)
+                    v[i] = other;
+                else
+                    v[i | o] = other;
+            }
+}
+
+// 32 rows of 128 columns of C whose rows are not 16-byte aligned: lanes and
+// columns change places, so that a warp's 2- or 4-byte stores are neighbours.  c: the
+// first row's; rows, left: how many rows and columns there are from it on.
+template <typename T>
+__device__ __forceinline__ void store_columns(T* c, int64_t ldc, int64_t rows, int64_t left, const float* bias,
+                                              float floor, int lane, float (&v)[4][32]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        transpose32(v[k], lane);
+        const float b = bias[k * 32 + lane];
+        T* to = c + k * 32 + lane;
+        if (k * 32 + lane < left)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i < rows) store_one(to + i * ldc, at_least(v[k][i] + b, floor));
+    }
+}
+
 // 128 neighbouring elements of a row of C.  ACCESS: bytes that every 32 of them are
-// aligned to (32, 16, or 0: element by element).
+// aligned to (32 or 16; past the row's end element by element).
 template <typename T, int ACCESS>
 __device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias, float floor, float (&v)[4][32]) {
-    constexpr int E = (ACCESS == 16 ? 16 : 32) / (int)sizeof(T);  // elements of a store
+    constexpr int E = ACCESS / (int)sizeof(T);  // elements of a store
 #pragma unroll
     for (int k = 0; k < 128; k += E) {
         float x[E];
@@ -496,7 +530,7 @@ __device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias,
             x[i] = at_least(y[0] + b.x, floor), x[i + 1] = at_least(y[1] + b.y, floor);
             x[i + 2] = at_least(y[2] + b.z, floor), x[i + 3] = at_least(y[3] + b.w, floor);
         }
-        if (ACCESS > 0 && left >= k + E) {
+        if (left >= k + E) {
             uint32_t w[E * sizeof(T) / 4];
 #pragma unroll
             for (int i = 0; i < (int)(E * sizeof(T) / 4); ++i) {
@@ -521,6 +555,8 @@ __device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias,
     }
 }
 
+// ALIGNED: C's rows are 16-byte aligned.
+template <bool ALIGNED>
 __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ CUtensorMap map_t,
                                                                    const __grid_constant__ CUtensorMap map_sw,
@@ -695,19 +731,24 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), 0));
-            if (row >= p.m) continue;
-            const int64_t at = row * p.ldc + col0, left = p.n - col0;
+            const int64_t at = row * p.ldc + col0, left = p.n - col0, rows = p.m - row;
             const float floor = p.relu ? 0.0f : -INFINITY;
-            if (p.out_bf16) {
-                __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.c) + at;
-                if (p.access == 32) store_row<__nv_bfloat16, 32>(to, left, bias, floor, v);
-                else if (p.access == 16) store_row<__nv_bfloat16, 16>(to, left, bias, floor, v);
-                else store_row<__nv_bfloat16, 0>(to, left, bias, floor, v);
-            } else {
-                float* to = static_cast<float*>(p.c) + at;
-                if (p.access == 32) store_row<float, 32>(to, left, bias, floor, v);
-                else if (p.access == 16) store_row<float, 16>(to, left, bias, floor, v);
-                else store_row<float, 0>(to, left, bias, floor, v);
+            if constexpr (!ALIGNED) {
+                const int64_t first = at - lane * p.ldc;
+                if (p.out_bf16)
+                    store_columns(static_cast<__nv_bfloat16*>(p.c) + first, p.ldc, rows + lane, left, bias, floor, lane, v);
+                else
+                    store_columns(static_cast<float*>(p.c) + first, p.ldc, rows + lane, left, bias, floor, lane, v);
+            } else if (rows > 0) {
+                if (p.out_bf16) {
+                    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.c) + at;
+                    if (p.access == 32) store_row<__nv_bfloat16, 32>(to, left, bias, floor, v);
+                    else store_row<__nv_bfloat16, 16>(to, left, bias, floor, v);
+                } else {
+                    float* to = static_cast<float*>(p.c) + at;
+                    if (p.access == 32) store_row<float, 32>(to, left, bias, floor, v);
+                    else store_row<float, 16>(to, left, bias, floor, v);
+                }
             }
         }
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
@@ -832,7 +873,7 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cuda
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 2 : 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_pair_kernel, w, t, sw, st, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, p.access >= 16 ? mx4_pair_kernel<true> : mx4_pair_kernel<false>, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
 }
@@ -847,7 +888,8 @@ int allow_smem() {
 
 int gemm_mx4_init() {
     RT_TRY(allow_smem<32>());
-    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
     return allow_smem<64>();
 }
 

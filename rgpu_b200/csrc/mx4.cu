@@ -21,8 +21,9 @@ template <>
 __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // A lane's piece of a row: 32 bytes, 16 bf16 or 8 f32.  V: bytes of an access, 32
-// (one 256-bit access, Blackwell's widest) or 16 where the rows are so aligned,
-// else 0: element by element, as at a row's end.
+// (one 256-bit access, Blackwell's widest) or 16 where the rows are so aligned.
+// Else (0) a warp's accesses take neighbouring elements, which change hands through
+// its kilobyte of shared memory; an aligned row's last piece goes element by element.
 template <typename T>
 struct Piece {
     static constexpr int E = 32 / sizeof(T);         // elements
@@ -73,6 +74,29 @@ struct Piece {
                         p[e] = __uint_as_float(w[e]);
                 }
         }
+    }
+    // The warp's piece of an unaligned row of which `left` elements lie from p on; box:
+    // the warp's 1 KB.  p and left are the warp's, not the lane's.
+    __device__ __forceinline__ void load_any(const T* p, int64_t left, T* box, int lane) {
+        T v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = e * 32 + lane < left ? p[e * 32 + lane] : T(0.0f);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < E; ++e) box[e * 32 + lane] = v[e];
+        __syncwarp();
+        const uint4 a = reinterpret_cast<const uint4*>(box)[lane * 2], b = reinterpret_cast<const uint4*>(box)[lane * 2 + 1];
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    }
+    __device__ __forceinline__ void store_any(T* p, int64_t left, T* box, int lane) const {
+        __syncwarp();
+        reinterpret_cast<uint4*>(box)[lane * 2] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(box)[lane * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e * 32 + lane < left) p[e * 32 + lane] = box[e * 32 + lane];
     }
     // Bit pattern (as f32) of the largest magnitude in the lane.
     __device__ __forceinline__ uint32_t amax() const {
@@ -138,6 +162,7 @@ __global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const T* __restri
                                                                uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales) {
     using P = Piece<T>;
+    __shared__ __align__(16) T boxes[V ? 1 : 8][P::WARP];
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -145,12 +170,17 @@ __global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const T* __restri
     const Place at(w);
     for (int64_t set = at.set; set < w.sets; set += at.set_step)
         for (int chunk = at.chunk; chunk < w.chunks; chunk += at.chunk_step) {
-            const int64_t row = set_row(w, set), j = (int64_t)chunk * P::WARP + lane * P::E;
+            const int64_t row = set_row(w, set), j0 = (int64_t)chunk * P::WARP, j = j0 + lane * P::E;
             const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);  // rows of the set that there are
-            const T* p = src + row * ld + j;
+            const T* p = src + row * ld + j0;
             P x[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) x[q].template load<V>(p + q * (32 * ld), q < live ? k - j : 0);
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (V == 0)
+                    x[q].load_any(p + q * (32 * ld), q < live ? k - j0 : 0, boxes[threadIdx.x >> 5], lane);
+                else
+                    x[q].template load<V>(p + q * (32 * ld) + lane * P::E, q < live ? k - j : 0);
+            }
             uint32_t word[4];
             uint8_t* out = codes + row * row_bytes + (j >> 1);
             const bool inside = j < blocks * 32;
@@ -276,6 +306,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
                                                          Rows w, int64_t blocks, int64_t groups, T* __restrict__ dst,
                                                          int64_t ld) {
     using P = Piece<T>;
+    __shared__ __align__(16) T boxes[V ? 1 : 8][P::WARP];
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -283,16 +314,18 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
     const Place at(w);
     for (int64_t set = at.set; set < w.sets; set += at.set_step)
         for (int chunk = at.chunk; chunk < w.chunks; chunk += at.chunk_step) {
-            const int64_t row = set_row(w, set), j = (int64_t)chunk * P::WARP + lane * P::E;
-            if (j >= k) continue;
+            const int64_t row = set_row(w, set), j0 = (int64_t)chunk * P::WARP, j = j0 + lane * P::E;
+            if (V ? j >= k : j0 >= k) continue;
+            const bool inside = j < blocks * 32;
             const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);
-            const uint4 s = __ldg(reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j >> 7)) * 512 + (row & 31) * 16));
+            const uint4 s = !inside ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j >> 7)) * 512 + (row & 31) * 16));
             const uint32_t word[4] = {s.x, s.y, s.z, s.w};
             const uint8_t* in = codes + row * row_bytes + (j >> 1);
             uint32_t c[4][P::E / 8];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (q < live) {
+            for (int q = 0; q < 4; ++q) {
+                c[q][0] = c[q][P::E / 8 - 1] = 0;
+                if (q < live && inside) {
                     if constexpr (sizeof(T) == 2) {
                         const uint2 two = __ldg(reinterpret_cast<const uint2*>(in + q * (32 * row_bytes)));
                         c[q][0] = two.x;
@@ -301,6 +334,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
                         c[q][0] = __ldg(reinterpret_cast<const uint32_t*>(in + q * (32 * row_bytes)));
                     }
                 }
+            }
             const int shift = (int)(j >> 5 & 3) * 8;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -319,7 +353,10 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
                         x.w[2 * i + 1] = __float_as_uint(__uint_as_float(h & 0xffff0000u) * __uint_as_float(u.a) * __uint_as_float(u.b));
                     }
                 }
-                x.template store<V>(dst + (row + 32 * q) * ld + j, k - j);
+                if constexpr (V == 0)
+                    x.store_any(dst + (row + 32 * q) * ld + j0, k - j0, boxes[threadIdx.x >> 5], lane);
+                else
+                    x.template store<V>(dst + (row + 32 * q) * ld + j, k - j);
             }
         }
 }
