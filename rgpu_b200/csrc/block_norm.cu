@@ -89,57 +89,85 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Sum over the 256 threads of a block, to every thread, in a fixed order.
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += red[i];
-    return s;
-}
-
 struct Stat {
     float mu, rho;
 };
 
-// Mean (layer) and reciprocal deviation of a row, x(j) its elements.
+__device__ __forceinline__ float gamma_at(const NormP& p, int64_t j) { return p.gamma ? p.gamma[j] : 1.0f; }
+
+// ------------------------------------------------------------- rows of any width
+// For rows that the kernels below do not hold: a CTA of 1024 threads per row, which
+// it reads once per pass, four elements a thread at a time, all of their reads under
+// way together.
+constexpr int kWide = 1024;
+
+// Sum over the CTA, to every thread, in a fixed order; `red` holds 32 floats.
+__device__ __forceinline__ float wide_sum(float v, float* red) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_sum(red[threadIdx.x & 31]);
+}
+
+// The thread's four elements of a pass's turn at `base`: of a row, of a vector (or
+// what stands for it), of the gate.
+template <typename T>
+__device__ __forceinline__ void row4(const void* x, int64_t at, int64_t base, int64_t n, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t j = base + i * kWide + threadIdx.x;
+        v[i] = j < n ? ld<T>(x, at + j) : 0.0f;
+    }
+}
+__device__ __forceinline__ void vector4(const float* x, float other, int64_t base, int64_t n, float (&v)[4], int stride = 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t j = base + i * kWide + threadIdx.x;
+        v[i] = x && j < n ? __ldg(x + j * stride) : other;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void gate4(const BlockP& p, int64_t row, int64_t base, int64_t n, float (&v)[4]) {
+    if (p.gate_mode == GATE_FULL)
+        row4<T>(p.gate, row * p.ldg, base, n, v);
+    else
+        vector4(p.gate_mode == GATE_NONE ? nullptr
+                                         : static_cast<const float*>(p.gate) + (p.gate_mode == GATE_COLUMN ? row * p.ldg : 0),
+                1.0f, base, n, v, p.gate_mode == GATE_ROW ? 1 : 0);
+}
+
+// Mean (layer) and reciprocal deviation of a row; x(base, v) gives four elements,
+// zeros past the end.
 template <typename F>
 __device__ __forceinline__ Stat row_stat(const NormP& p, int64_t n, float* red, F x) {
     Stat s{0.0f, 1.0f};
     if (p.kind == RT_NORM_NONE) return s;
     if (p.kind == RT_NORM_LAYER) {
         float t = 0.0f;
-        for (int64_t j = threadIdx.x; j < n; j += 256) t += x(j);
-        s.mu = block_sum(t, red) / (float)n;
+        for (int64_t base = 0; base < n; base += 4 * kWide) {
+            float v[4];
+            x(base, v);
+            t += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        s.mu = wide_sum(t, red) / (float)n;
     }
     float t = 0.0f;
-    for (int64_t j = threadIdx.x; j < n; j += 256) {
-        const float d = x(j) - s.mu;
-        t += d * d;
+    for (int64_t base = 0; base < n; base += 4 * kWide) {
+        float v[4];
+        x(base, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float d = base + i * kWide + threadIdx.x < n ? v[i] - s.mu : 0.0f;
+            t += d * d;
+        }
     }
-    s.rho = rsqrtf(block_sum(t, red) / (float)n + p.eps);
+    s.rho = rsqrtf(wide_sum(t, red) / (float)n + p.eps);
     return s;
 }
 
-__device__ __forceinline__ float gamma_at(const NormP& p, int64_t j) { return p.gamma ? p.gamma[j] : 1.0f; }
-__device__ __forceinline__ float beta_at(const NormP& p, int64_t j) { return p.beta ? p.beta[j] : 0.0f; }
-
-template <typename T>
-__device__ __forceinline__ float gate_at(const BlockP& p, int64_t row, int64_t j) {
-    switch (p.gate_mode) {
-        case GATE_ONE: return static_cast<const float*>(p.gate)[0];
-        case GATE_ROW: return static_cast<const float*>(p.gate)[j];
-        case GATE_COLUMN: return static_cast<const float*>(p.gate)[row * p.ldg];
-        case GATE_FULL: return ld<T>(p.gate, row * p.ldg + j);
-        default: return 1.0f;
-    }
-}
-
 // One block of 32 in 4 bits by a whole warp, a lane's element h at j.
-__device__ __forceinline__ void store_block(const BlockP& p, int64_t row, int j, int blocks, int groups, float h) {
+__device__ __forceinline__ void store_block(const BlockP& p, int64_t row, int64_t j, int64_t blocks, int64_t groups, float h) {
     const int lane = threadIdx.x & 31;
     const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
     const uint32_t byte = mx4::scale_byte(amax);
@@ -149,121 +177,168 @@ __device__ __forceinline__ void store_block(const BlockP& p, int64_t row, int j,
     if (lane == 0) {
         p.scales[mx4::scale_offset(row, j >> 5, groups)] = (uint8_t)byte;
         if ((j >> 5) == blocks - 1)
-            for (int b = blocks; b < groups * 4; ++b) p.scales[mx4::scale_offset(row, b, groups)] = 0;
+            for (int64_t b = blocks; b < groups * 4; ++b) p.scales[mx4::scale_offset(row, b, groups)] = 0;
     }
 }
 
-// Rows wider than the other kernels hold: one CTA per row at a time, the row read
-// once per pass.
 template <typename T>
-__global__ void __launch_bounds__(256) forward_kernel(BlockP p) {
-    __shared__ float red[8];
+__global__ void __launch_bounds__(kWide) forward_kernel(BlockP p) {
+    __shared__ float red[32];
     pdl_wait();
     pdl_launch_dependents();
     const int64_t n = p.n, blocks = (n + 31) / 32, groups = (blocks + 3) / 4;
     for (int64_t row = blockIdx.x; row < p.m; row += gridDim.x) {
         Stat sy{0.0f, 1.0f};
-        if (p.y) sy = row_stat(p.post, n, red, [&](int64_t j) { return ld<T>(p.y, row * p.ldy + j); });
-        auto z_at = [&](int64_t j) {
-            float z = ld<T>(p.r, row * p.ldr + j);
-            if (p.y) {
-                const float u = (ld<T>(p.y, row * p.ldy + j) - sy.mu) * sy.rho * gamma_at(p.post, j) + beta_at(p.post, j);
-                z += p.scale * gate_at<T>(p, row, j) * u;
-            }
-            return z;
+        if (p.y) sy = row_stat(p.post, n, red, [&](int64_t base, float (&v)[4]) { row4<T>(p.y, row * p.ldy, base, n, v); });
+        auto z4 = [&](int64_t base, float (&z)[4]) {
+            row4<T>(p.r, row * p.ldr, base, n, z);
+            if (!p.y) return;
+            float y[4], gamma[4], beta[4], gate[4];
+            row4<T>(p.y, row * p.ldy, base, n, y);
+            vector4(p.post.gamma, 1.0f, base, n, gamma);
+            vector4(p.post.beta, 0.0f, base, n, beta);
+            gate4<T>(p, row, base, n, gate);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (base + i * kWide + threadIdx.x < n)
+                    z[i] += p.scale * gate[i] * ((y[i] - sy.mu) * sy.rho * gamma[i] + beta[i]);
         };
-        const Stat sz = row_stat(p.pre, n, red, z_at);
-        for (int64_t j = threadIdx.x; j < blocks * 32; j += 256) {
-            float h = 0.0f;
-            if (j < n) {
-                const float z = z_at(j);
-                h = (z - sz.mu) * sz.rho * gamma_at(p.pre, j) + beta_at(p.pre, j);
-                if (p.z) st<T>(p.z, row * p.ldz + j, z);
-                if (p.h) st<T>(p.h, row * p.ldh + j, h);
-            }
-            if (p.codes) {
-                store_block(p, row, (int)j, (int)blocks, (int)groups, as_stored<T>(h));
+        const Stat sz = row_stat(p.pre, n, red, z4);
+        for (int64_t base = 0; base < n; base += 4 * kWide) {
+            float z[4], gamma[4], beta[4];
+            z4(base, z);
+            vector4(p.pre.gamma, 1.0f, base, n, gamma);
+            vector4(p.pre.beta, 0.0f, base, n, beta);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t j = base + i * kWide + threadIdx.x;
+                const float h = j < n ? (z[i] - sz.mu) * sz.rho * gamma[i] + beta[i] : 0.0f;
+                if (j < n && p.z) st<T>(p.z, row * p.ldz + j, z[i]);
+                if (j < n && p.h) st<T>(p.h, row * p.ldh + j, h);
+                if (p.codes && (j & ~int64_t(31)) < n) store_block(p, row, j, blocks, groups, as_stored<T>(h));
             }
         }
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) backward_kernel(BlockP p, GradP g) {
-    __shared__ float red[8];
+__global__ void __launch_bounds__(kWide) backward_kernel(BlockP p, GradP g) {
+    __shared__ float red[32];
     pdl_wait();
     pdl_launch_dependents();
     const int64_t n = p.n;
     const int64_t cols = columns(n);
     float* acc = g.partials ? g.partials + (int64_t)blockIdx.x * 4 * cols : nullptr;
     if (acc)
-        for (int64_t i = threadIdx.x; i < 4 * cols; i += 256)
+        for (int64_t i = threadIdx.x; i < 4 * cols; i += kWide)
             if ((g.sums >> (i / cols)) & 1) acc[i] = 0.0f;
     __syncthreads();
     const float inv_n = 1.0f / (float)n;
+    const bool own_gate = p.gate_mode >= GATE_COLUMN;
     for (int64_t row = blockIdx.x; row < p.m; row += gridDim.x) {
-        auto z_at = [&](int64_t j) { return ld<T>(p.z, row * p.ldz + j); };
-        auto y_at = [&](int64_t j) { return ld<T>(p.y, row * p.ldy + j); };
-        const Stat sz = row_stat(p.pre, n, red, z_at);
+        auto z4 = [&](int64_t base, float (&v)[4]) { row4<T>(p.z, row * p.ldz, base, n, v); };
+        auto y4 = [&](int64_t base, float (&v)[4]) { row4<T>(p.y, row * p.ldy, base, n, v); };
+        const Stat sz = row_stat(p.pre, n, red, z4);
         Stat sy{0.0f, 1.0f};
-        if (p.y) sy = row_stat(p.post, n, red, y_at);
+        if (p.y) sy = row_stat(p.post, n, red, y4);
         // means of a and a z^ of the norm before the next block
         float a0 = 0.0f, a1 = 0.0f;
         if (g.dh && p.pre.kind != RT_NORM_NONE) {
-            for (int64_t j = threadIdx.x; j < n; j += 256) {
-                const float a = ld<T>(g.dh, row * g.lddh + j) * gamma_at(p.pre, j);
-                a0 += a;
-                a1 += a * (z_at(j) - sz.mu) * sz.rho;
+            for (int64_t base = 0; base < n; base += 4 * kWide) {
+                float z[4], d[4], gamma[4];
+                z4(base, z);
+                row4<T>(g.dh, row * g.lddh, base, n, d);
+                vector4(p.pre.gamma, 1.0f, base, n, gamma);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // d is zero past the row's end
+                    a0 += d[i] * gamma[i];
+                    a1 += d[i] * gamma[i] * ((z[i] - sz.mu) * sz.rho);
+                }
             }
-            a0 = p.pre.kind == RT_NORM_LAYER ? block_sum(a0, red) * inv_n : 0.0f;
-            a1 = block_sum(a1, red) * inv_n;
+            a0 = p.pre.kind == RT_NORM_LAYER ? wide_sum(a0, red) * inv_n : 0.0f;
+            a1 = wide_sum(a1, red) * inv_n;
         }
-        auto dr_at = [&](int64_t j) {
-            float d = g.dz ? ld<T>(g.dz, row * g.lddz + j) : 0.0f;
-            if (g.dh) {
-                const float a = ld<T>(g.dh, row * g.lddh + j) * gamma_at(p.pre, j);
-                d += (a - a0 - (z_at(j) - sz.mu) * sz.rho * a1) * sz.rho;
+        // four elements of dr; dh and z^ beside it
+        auto dr4 = [&](int64_t base, float (&dr)[4], float (&d)[4], float (&hat)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dr[i] = d[i] = hat[i] = 0.0f;
+            float gamma[4];
+            if (g.dz) row4<T>(g.dz, row * g.lddz, base, n, dr);
+            if (!g.dh) return;
+            row4<T>(g.dh, row * g.lddh, base, n, d);
+            z4(base, hat);
+            vector4(p.pre.gamma, 1.0f, base, n, gamma);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hat[i] = (hat[i] - sz.mu) * sz.rho;
+                if (base + i * kWide + threadIdx.x < n) dr[i] += (d[i] * gamma[i] - a0 - hat[i] * a1) * sz.rho;
             }
-            return d;
         };
-        float b0 = 0.0f, b1 = 0.0f, gsum = 0.0f;
+        float b0 = 0.0f, b1 = 0.0f;
         if (p.y) {
-            for (int64_t j = threadIdx.x; j < n; j += 256) {
-                const float dt = p.scale * dr_at(j), hat = (y_at(j) - sy.mu) * sy.rho;
-                const float b = dt * gate_at<T>(p, row, j) * gamma_at(p.post, j);
-                b0 += b;
-                b1 += b * hat;
-                gsum += dt * (hat * gamma_at(p.post, j) + beta_at(p.post, j));
+            float gsum = 0.0f;
+            for (int64_t base = 0; base < n; base += 4 * kWide) {
+                float dr[4], d[4], hat[4], y[4], gate[4], gamma[4], beta[4];
+                dr4(base, dr, d, hat);
+                y4(base, y);
+                gate4<T>(p, row, base, n, gate);
+                vector4(p.post.gamma, 1.0f, base, n, gamma);
+                vector4(p.post.beta, 0.0f, base, n, beta);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // dr is zero past the row's end
+                    const float dt = p.scale * dr[i], yh = (y[i] - sy.mu) * sy.rho, b = dt * gate[i] * gamma[i];
+                    b0 += b;
+                    b1 += b * yh;
+                    gsum += dt * (yh * gamma[i] + beta[i]);
+                }
             }
-            b0 = p.post.kind == RT_NORM_LAYER ? block_sum(b0, red) * inv_n : 0.0f;
-            b1 = p.post.kind != RT_NORM_NONE ? block_sum(b1, red) * inv_n : 0.0f;
+            b0 = p.post.kind == RT_NORM_LAYER ? wide_sum(b0, red) * inv_n : 0.0f;
+            b1 = p.post.kind != RT_NORM_NONE ? wide_sum(b1, red) * inv_n : 0.0f;
             if (g.dgate && p.gate_mode == GATE_COLUMN) {
-                gsum = block_sum(gsum, red);
+                gsum = wide_sum(gsum, red);
                 if (threadIdx.x == 0) static_cast<float*>(g.dgate)[row * g.lddg] = gsum;
             }
         }
-        for (int64_t j = threadIdx.x; j < n; j += 256) {
-            const float dr = dr_at(j);
+        for (int64_t base = 0; base < n; base += 4 * kWide) {
+            float dr[4], d[4], hat[4], y[4], gate[4], gamma[4], beta[4], sum[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if ((g.sums >> k) & 1) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t j = base + i * kWide + threadIdx.x;
+                        sum[k][i] = j < n ? acc[k * cols + j] : 0.0f;
+                    }
+                }
+            dr4(base, dr, d, hat);
             if (p.y) {
-                const float dt = p.scale * dr, hat = (y_at(j) - sy.mu) * sy.rho, gt = gate_at<T>(p, row, j);
-                const float b = dt * gt * gamma_at(p.post, j);
-                if (g.dy) st<T>(g.dy, row * g.lddy + j, (b - b0 - hat * b1) * sy.rho);
-                if (g.dgate && p.gate_mode == GATE_FULL)
-                    st<T>(g.dgate, row * g.lddg + j, dt * (hat * gamma_at(p.post, j) + beta_at(p.post, j)));
-                const float w = p.gate_mode >= GATE_COLUMN ? dr * gt : dr;
-                if (g.sums & 1) acc[j] += w * hat;
-                if (g.sums & 2) acc[cols + j] += w;
+                y4(base, y);
+                gate4<T>(p, row, base, n, gate);
+                vector4(p.post.gamma, 1.0f, base, n, gamma);
+                vector4(p.post.beta, 0.0f, base, n, beta);
             }
-            if (g.dh) {
-                const float dh = ld<T>(g.dh, row * g.lddh + j);
-                if (g.sums & 4) acc[2 * cols + j] += dh * (z_at(j) - sz.mu) * sz.rho;
-                if (g.sums & 8) acc[3 * cols + j] += dh;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t j = base + i * kWide + threadIdx.x;
+                if (j >= n) continue;
+                if (p.y) {
+                    const float dt = p.scale * dr[i], yh = (y[i] - sy.mu) * sy.rho, b = dt * gate[i] * gamma[i];
+                    if (g.dy) st<T>(g.dy, row * g.lddy + j, (b - b0 - yh * b1) * sy.rho);
+                    if (g.dgate && p.gate_mode == GATE_FULL)
+                        st<T>(g.dgate, row * g.lddg + j, dt * (yh * gamma[i] + beta[i]));
+                    const float w = own_gate ? dr[i] * gate[i] : dr[i];
+                    if (g.sums & 1) acc[j] = sum[0][i] + w * yh;
+                    if (g.sums & 2) acc[cols + j] = sum[1][i] + w;
+                }
+                if (g.dh) {
+                    if (g.sums & 4) acc[2 * cols + j] = sum[2][i] + d[i] * hat[i];
+                    if (g.sums & 8) acc[3 * cols + j] = sum[3][i] + d[i];
+                }
+                if (g.dr) st<T>(g.dr, row * g.lddr + j, dr[i]);
             }
-            if (g.dr) st<T>(g.dr, row * g.lddr + j, dr);
         }
     }
 }
-
 
 // ------------------------------------------------------- rows in registers
 // Eight elements as they are stored: 16 bytes of bf16, 32 of f32.
@@ -1589,13 +1664,13 @@ __global__ void __launch_bounds__(512) column_kernel(ReduceP p) {
     else if (p.dgate) p.dgate[j] = dg;
 }
 
-__global__ void __launch_bounds__(256) gate_one_kernel(const float* row, int64_t n, float* out) {
-    __shared__ float red[8];
+__global__ void __launch_bounds__(kWide) gate_one_kernel(const float* row, int64_t n, float* out) {
+    __shared__ float red[32];
     pdl_wait();
     pdl_launch_dependents();
     float s = 0.0f;
-    for (int64_t j = threadIdx.x; j < n; j += 256) s += row[j];
-    s = block_sum(s, red);
+    for (int64_t j = threadIdx.x; j < n; j += kWide) s += row[j];
+    s = wide_sum(s, red);
     if (threadIdx.x == 0) out[0] = s;
 }
 
@@ -1769,6 +1844,9 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
                      (p.post.beta && q.dgate && !shared ? 4 : 0);
     const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
+    // sixteen columns with all sums spill; with the copies' registers beside them the
+    // kernel for rows of any width is faster (4096 x 4099 bf16 layer: 400 us, 540 here)
+    if (full && !bulk && p.n > 4096) return RT_OK;
     const int eights = (full || !bulk) && p.n <= 4096 ? 1 : 2;
     int tpr = 32;
     while (tpr * eights * 8 < p.n) tpr *= 2;
@@ -1794,9 +1872,7 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
         }
     }
     if (!bulk) {
-        if (eights == 2)
-            return full ? launch_backward_ring<T, 512, 2, true, false>(ctx, p, q, r, mask, *parts, st)
-                        : launch_backward_ring<T, 512, 2, false, false>(ctx, p, q, r, mask, *parts, st);
+        if (eights == 2) return launch_backward_ring<T, 512, 2, false, false>(ctx, p, q, r, mask, *parts, st);
         switch (tpr) {
             case 32: return launch_backward_ring<T, 32, 1, true, false>(ctx, p, q, r, mask, *parts, st);
             case 64: return launch_backward_ring<T, 64, 1, true, false>(ctx, p, q, r, mask, *parts, st);
@@ -1863,7 +1939,7 @@ int forward_any(rt_ctx* ctx, const BlockP& p, cudaStream_t st) {
     if (!done) RT_TRY(forward_rows<T>(ctx, p, st, &done));
     if (!done) RT_TRY(forward_strided<T>(ctx, p, st, &done));
     if (!done)
-        RT_CUDA(launch_k(ctx->pdl, forward_kernel<T>, (unsigned)std::min<int64_t>(p.m, (int64_t)ctx->sm_count * 8), 256, 0,
+        RT_CUDA(launch_k(ctx->pdl, forward_kernel<T>, (unsigned)std::min<int64_t>(p.m, (int64_t)ctx->sm_count * 8), kWide, 0,
                          st, p));
     count_launch(ctx);
     return RT_OK;
@@ -1993,7 +2069,7 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
                                : backward_ring<float>(ctx, p, q, ctx->stream, &parts, &done));
     // wider rows; and without rows the sums over rows are zero: the partials of one CTA
     if (!done)
-        RT_CUDA(launch_k(ctx->pdl, z->dtype == RT_BF16 ? backward_kernel<__nv_bfloat16> : backward_kernel<float>, parts, 256, 0,
+        RT_CUDA(launch_k(ctx->pdl, z->dtype == RT_BF16 ? backward_kernel<__nv_bfloat16> : backward_kernel<float>, parts, kWide, 0,
                          ctx->stream, p, q));
     count_launch(ctx);
     if (!q.sums) return RT_OK;
@@ -2010,7 +2086,7 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     RT_CUDA(launch_k(ctx->pdl, column_kernel, (unsigned)((p.n + 31) / 32), 512, 0, ctx->stream, c));
     count_launch(ctx);
     if (c.gate_row) {
-        RT_CUDA(launch_k(ctx->pdl, gate_one_kernel, 1, 256, 0, ctx->stream, c.gate_row, p.n, c.dgate));
+        RT_CUDA(launch_k(ctx->pdl, gate_one_kernel, 1, kWide, 0, ctx->stream, c.gate_row, p.n, c.dgate));
         count_launch(ctx);
     }
     return RT_OK;

@@ -161,6 +161,16 @@ def test_rms_training_step(gpu, m, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind,vectors", [("layer", True), ("rms", "gamma")])
+@pytest.mark.parametrize("m,n,pad", [(150, 5001, 0), (3, 8190, 0), (9, 8191, 1), (300, 1003, 0), (5, 12001, 0), (2, 16384, 0)])
+def test_wide_and_odd_rows(gpu, m, n, pad, kind, vectors, dtype):
+    for gate in ("row", "full") if vectors is True else ("row",):
+        c = Case(gpu, m, n, dtype, kind, kind, gate, seed=m + n, vectors=vectors, pad=pad)
+        which = None if vectors is True else ("dr", "dy", "dgamma_post", "dgamma_pre", "dgate")
+        _backward_check(c, c.host["r"], _backward(gpu, c, c.dev["r"], which=which), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("gate", ["none", "one", "row", "column", "full"])
 def test_every_gate_and_in_place(gpu, gate, dtype):
     c = Case(gpu, 19, 320, dtype, "layer", "rms", gate, seed=4)
