@@ -1844,9 +1844,6 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
                      (p.post.beta && q.dgate && !shared ? 4 : 0);
     const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
-    // sixteen columns with all sums spill; with the copies' registers beside them the
-    // kernel for rows of any width is faster (4096 x 4099 bf16 layer: 400 us, 540 here)
-    if (full && !bulk && p.n > 4096) return RT_OK;
     const int eights = (full || !bulk) && p.n <= 4096 ? 1 : 2;
     int tpr = 32;
     while (tpr * eights * 8 < p.n) tpr *= 2;
@@ -1872,7 +1869,9 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
         }
     }
     if (!bulk) {
-        if (eights == 2) return launch_backward_ring<T, 512, 2, false, false>(ctx, p, q, r, mask, *parts, st);
+        if (eights == 2)
+            return full ? launch_backward_ring<T, 512, 2, true, false>(ctx, p, q, r, mask, *parts, st)
+                        : launch_backward_ring<T, 512, 2, false, false>(ctx, p, q, r, mask, *parts, st);
         switch (tpr) {
             case 32: return launch_backward_ring<T, 32, 1, true, false>(ctx, p, q, r, mask, *parts, st);
             case 64: return launch_backward_ring<T, 64, 1, true, false>(ctx, p, q, r, mask, *parts, st);
