@@ -427,7 +427,9 @@ __device__ __forceinline__ float row_sum(float v, float* red, int& turn) {
     return v;
 }
 
-// Mean and reciprocal deviation of a row held 8 C elements a thread.
+// Mean and reciprocal deviation of a row held 8 C elements a thread.  (rsqrtf, here
+// and below, is within 2 units in the last place: sums of hundreds of rounded terms
+// precede it.)
 template <int TPR, int C>
 __device__ __forceinline__ Stat stat_of(const NormP& p, const float (&x)[C][8], const bool (&has)[C], float inv_n,
                                         float* red, int& turn) {
@@ -670,8 +672,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_strided_kernel(Bloc
 // where they meet) lie in shared memory once, in f32.
 constexpr int kRingThreads = 1024;
 constexpr int kRingSmem = 227 * 1024;
-// a group's sums, its barriers (up to eight) and the abort flag
-constexpr int ring_scratch(int groups) { return groups * (1024 + 64) + 16; }
+// a group's sums, its barriers (up to eight), the abort flag and where each group gave up
+constexpr int ring_scratch(int groups) { return groups * (1024 + 64 + 4) + 16; }
 
 struct RingP {
     int depth;         // slots of a group
@@ -754,6 +756,28 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                  "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
+}
+
+// A wait that gave up leaves its slot and phase for the end of the kernel, where
+// the thread that issues (it issues no more) waits, again with a limit, for the
+// copies on their way.  That wait inside the loop took backward_pipe_kernel from
+// 144 to 158 us at 8192x8192, although no call reached it.
+__device__ __forceinline__ void gave_up(const RingP& r, volatile int* abort_flag, int group, int slot, uint32_t phase) {
+    *abort_flag = 1;
+    tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+    if (group >= 0) abort_flag[1 + group] = slot * 2 + (int)phase;
+}
+__device__ __noinline__ void land_copies(uint32_t full, int depth, int at) {
+    int slot = at >> 1;
+    uint32_t phase = at & 1;
+    volatile int never = 0;
+    for (int d = 0; d < depth; ++d) {
+        tc::mbar_wait(full + slot * 8, phase, &never);
+        if (++slot == depth) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
 }
 
 // Shared memory of a ring kernel: vectors, slots, sums, barriers.
@@ -895,6 +919,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
         if (mask & 8) vb[j] = __ldg(p.pre.beta + j);
     }
     __syncthreads();
+    bool ok = true;  // this thread's waits so far
     auto issue = [&](int64_t row, int slot) {
         const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * r.slot_bytes);
         tc::mbar_expect_tx(bar, (uint32_t)r.slot_bytes);
@@ -911,8 +936,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
     for (int c = 0; c < C; ++c) has[c] = (c * TPR + g.t) * 8 < n;
     for (int64_t row = first; row < p.m; row += step) {
         if (!tc::mbar_wait(full + slot * 8, phase, abort_flag)) {
-            *abort_flag = 1;
-            tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+            if (ok) gave_up(r, abort_flag, g.t == 0 ? g.index : -1, slot, phase);
+            ok = false;
         }
         const uint8_t* at = slots + (size_t)slot * r.slot_bytes;
         f2 z[C][4];
@@ -1002,7 +1027,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
         bool freed = false;
         auto refill = [&] {
             freed = true;
-            if (g.t == 0 && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
+            if (g.t == 0 && ok && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
         };
         if (FULL && p.pre.kind == RT_NORM_LAYER) {
             f2 v2x = 0;
@@ -1064,6 +1089,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
             phase ^= 1;
         }
     }
+    if (!ok && g.t == 0) land_copies(full, r.depth, abort_flag[1 + g.index]);
 }
 
 // Backward.  Slots hold z and those of y, dz and dh that there are; vectors
@@ -1141,6 +1167,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     // the slot's rows: z, then y, dz, dh; not BULK: all of them, and a gate's
     const uint32_t at_y = row_bytes, at_dz = at_y + (p.y || !BULK ? row_bytes : 0),
                    at_dh = at_dz + (q.dz || !BULK ? row_bytes : 0), at_gate = at_dh + row_bytes;
+    bool ok = true;  // this thread's waits so far
     auto issue = [&](int64_t row, int slot) {
         const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * r.slot_bytes);
         tc::mbar_expect_tx(bar, (uint32_t)r.slot_bytes);
@@ -1194,8 +1221,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     for (int64_t row = first; row < p.m; row += step) {
         if constexpr (BULK) {
             if (!tc::mbar_wait(full + slot * 8, phase, abort_flag)) {
-                *abort_flag = 1;
-                tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+                if (ok) gave_up(r, abort_flag, g.t == 0 ? g.index : -1, slot, phase);
+                ok = false;
             }
         } else {
             T a[8 * C], b[8 * C];
@@ -1395,7 +1422,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
             g.sum(b1);
         }
         // every thread of the group has read the slot: all of it before the last barrier
-        if (BULK && g.t == 0 && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
+        if (BULK && g.t == 0 && ok && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
         if (q.dy) {
             const f2 rho = splat2(sy.rho), add = splat2(b0), less_b1 = splat2(p.post.kind != RT_NORM_NONE ? -b1 * inv_n : 0.0f);
 #pragma unroll
@@ -1423,6 +1450,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
             phase ^= 1;
         }
     }
+    if (BULK && !ok && g.t == 0) land_copies(full, r.depth, abort_flag[1 + g.index]);
     if (!q.partials) return;
     __syncthreads();  // the slots are all read
     float* acc = reinterpret_cast<float*>(sm.slots);
@@ -1472,6 +1500,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
         vp[j] = p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
     }
     __syncthreads();
+    bool ok = true;  // this thread's waits so far
     auto issue = [&](int64_t row, int slot) {
         const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * 3 * row_bytes);
         tc::mbar_expect_tx(bar, 3 * row_bytes);
@@ -1489,10 +1518,11 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
             issue(first + d * step, d);
             issue_dz(first + d * step, d);
         }
-    auto wait = [&](uint32_t bar, uint32_t phase) {
-        if (!tc::mbar_wait(bar, phase, abort_flag)) {
-            *abort_flag = 1;
-            tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
+    // the wait for `slot` of either ring; dz's ring is at most one slot behind
+    auto wait = [&](uint32_t ring, int slot, uint32_t phase) {
+        if (!tc::mbar_wait(ring + slot * 8, phase, abort_flag)) {
+            if (ok) gave_up(r, abort_flag, g.t == 0 ? g.index : -1, slot, phase);
+            ok = false;
         }
     };
     const float inv_n = 1.0f / (float)n;
@@ -1542,15 +1572,15 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
     int slot = 0;
     uint32_t phase = 0;
     if (first < p.m) {
-        wait(full, 0);
+        wait(full, 0, 0);
         float v[3];
         take(0, v);
         g.sum(v);
         stats(v[0], v[1], v[2]);
-        if (g.t == 0 && first + depth * step < p.m) issue(first + depth * step, 0);
+        if (g.t == 0 && ok && first + depth * step < p.m) issue(first + depth * step, 0);
     }
     for (int64_t row = first; row < p.m; row += step) {
-        wait(full_dz + slot * 8, phase);
+        wait(full_dz, slot, phase);
         const uint8_t* at = slots_dz + (size_t)slot * row_bytes;
         f2 b[C][4], hat[C][4];
         f2 sum_b = 0;
@@ -1586,12 +1616,12 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
         const bool more = row + step < p.m;
         float t[3] = {0.0f, 0.0f, 0.0f};
         if (more) {
-            wait(full + next * 8, next_phase);
+            wait(full, next, next_phase);
             take(next, t);
         }
         float v[4] = {t[0], t[1], t[2], both(sum_b)};
         g.sum(v);
-        if (g.t == 0) {
+        if (g.t == 0 && ok) {
             if (row + depth * step < p.m) issue_dz(row + depth * step, slot);
             if (row + (depth + 1) * step < p.m) issue(row + (depth + 1) * step, next);
         }
@@ -1608,6 +1638,10 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
         stats(v[0], v[1], v[2]);
         slot = next;
         phase = next_phase;
+    }
+    if (!ok && g.t == 0) {
+        land_copies(full, depth, abort_flag[1 + g.index]);
+        land_copies(full_dz, depth, abort_flag[1 + g.index]);
     }
     if (!q.partials) return;
     __syncthreads();  // the slots are all read

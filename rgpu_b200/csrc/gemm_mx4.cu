@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
     uint64_t* done = empty + G::STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* issued_all = abort_flag + 1;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t rank = cta_rank(), ranks = cluster_size();
@@ -280,6 +281,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
         }
         mbar_init(smem_u32(done), 1);
         *abort_flag = 0;
+        *issued_all = 0;
         fence_barrier_init();
         prefetch_tmap(&map_w);
         prefetch_tmap(&map_t);
@@ -324,13 +326,12 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
                 phase ^= 1;
             }
         }
-        if (!ok && elect_one()) {
-            record_error(p.err, DEV_TIMEOUT_PRODUCER, blockIdx.x);
-            *abort_flag = 1;
-            // the copies in flight write this CTA's shared memory: let them land before it exits
-            volatile int never = 0;
-            for (int i = max(0, issued - G::STAGES); i < issued; ++i)
-                mbar_wait(smem_u32(&full[i % G::STAGES]), (i / G::STAGES) & 1, &never);
+        if (elect_one()) {
+            *issued_all = issued;
+            if (!ok) {
+                record_error(p.err, DEV_TIMEOUT_PRODUCER, blockIdx.x);
+                *abort_flag = 1;
+            }
         }
     } else if (warp == 1) {
         const uint32_t token_col = (uint32_t)((tm * TN % 128) / 32);  // the tile's place in its 128-row scale tile
@@ -415,6 +416,14 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
             add_splits<float>(p, smem_u32(smem), ranks, rank, warp, kThreads1 / 32, row0, count, col, bias, lane);
     }
     if (ranks > 1) sync_cluster();  // the sums are read before any CTA exits
+    __syncthreads();
+    if (*abort_flag && threadIdx.x == 0) {
+        // copies and MMAs on their way use this CTA's memory: wait, again with a limit, for the last of them
+        volatile int never = 0;
+        for (int i = max(0, *issued_all - G::STAGES); i < *issued_all; ++i)
+            mbar_wait(smem_u32(&full[i % G::STAGES]), (i / G::STAGES) & 1, &never);
+        mbar_wait(smem_u32(done), 0, &never);
+    }
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
