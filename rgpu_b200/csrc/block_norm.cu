@@ -96,7 +96,7 @@ struct Stat {
 __device__ __forceinline__ float gamma_at(const NormP& p, int64_t j) { return p.gamma ? p.gamma[j] : 1.0f; }
 
 // ------------------------------------------------------------- rows of any width
-// For rows that the kernels below do not hold: a CTA of 1024 threads per row, which
+// For rows that the kernels below do not hold (over 16384 wide): a CTA of 1024 threads per row, which
 // it reads once per pass, four elements a thread at a time, all of their reads under
 // way together.
 constexpr int kWide = 1024;
@@ -487,7 +487,8 @@ __device__ __forceinline__ void store_h(const BlockP& p, int64_t row, int j, boo
 // One pass: a row lies in the registers of TPR threads, 8 neighbouring elements
 // in each of C turns, so y and r are read once, z and h written once and the
 // sums of a norm are taken twice over the same registers (mean, then the centred
-// squares).  HBM-bound: 4 elements moved for each of the row.  Needs 16-byte
+// squares).  HBM-bound: 4 elements moved for each of the row; few rows are bound by
+// the launch (one of 8192 bf16: 4.3 us in a stream of launches).  Needs 16-byte
 // aligned rows and whole eights (n % 8 = 0); a CTA holds ROWS = max(1, 128 / TPR)
 // rows.
 constexpr int cta_threads(int tpr) { return tpr < 128 ? 128 : tpr; }
@@ -672,8 +673,10 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_strided_kernel(Bloc
 // where they meet) lie in shared memory once, in f32.
 constexpr int kRingThreads = 1024;
 constexpr int kRingSmem = 227 * 1024;
-// a group's sums, its barriers (up to eight), the abort flag and where each group gave up
-constexpr int ring_scratch(int groups) { return groups * (1024 + 64 + 4) + 16; }
+// a group's sums [2][warps of its cluster, 32 at least][4], its barriers (up to eight),
+// the abort flag and where each group gave up
+constexpr int sum_floats(int cluster) { return cluster > 2 ? 128 * cluster : 256; }
+constexpr int ring_scratch(int groups, int cluster) { return groups * (sum_floats(cluster) * 4 + 64 + 4) + 16; }
 
 struct RingP {
     int depth;         // slots of a group
@@ -698,13 +701,40 @@ __device__ __forceinline__ float warp_sum4(float v0, float v1, float v2, float v
     return a;
 }
 
-template <int THREADS, int TPR>
+// The threads of a row: TPR of a CTA, or (CL > 1) the CTAs of a cluster, each with its
+// share of the columns.
+template <int THREADS, int TPR, int CL = 1>
 struct Group {
-    static constexpr int COUNT = THREADS / TPR;
+    static_assert(CL == 1 || TPR == THREADS, "a cluster's row takes whole CTAs");
+    static constexpr int COUNT = THREADS / TPR, W = TPR / 32, HALF = sum_floats(CL) / 2;
     int index, t;    // of the group in its CTA, of the thread in its group
-    float* red;      // [2][32 warps][4]
+    float* red;      // [2][warps][4]
     int turn = 0;
+    int rank = 0;        // of the CTA in its cluster
+    uint32_t there = 0;  // CL > 1: red of the CTA that this lane hands its warp's sums to
 
+    __device__ __forceinline__ void join_cluster() {
+        if constexpr (CL > 1) {
+            uint32_t at = tc::smem_u32(red);
+            asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(threadIdx.x & (CL - 1)));
+            sync_row();  // every CTA runs before it is written to
+        }
+    }
+    // Waits for all that take the row; what they handed over is then here.
+    __device__ __forceinline__ void sync_row() const {
+        if constexpr (CL > 1)
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else
+            sync();
+    }
+    // A value of the warp to every CTA of the row: called by CL neighbouring lanes.
+    __device__ __forceinline__ void hand(int at, float v) const {
+        if constexpr (CL > 1)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + (uint32_t)(turn * HALF + at) * 4), "f"(v) : "memory");
+        else
+            red[turn * HALF + at] = v;
+    }
     __device__ __forceinline__ void sync() const {
         if constexpr (TPR == 32)
             __syncwarp();
@@ -719,15 +749,15 @@ struct Group {
         if constexpr (TPR == 32) {
             __syncwarp();
         } else {
-            constexpr int W = TPR / 32;
             const int lane = threadIdx.x & 31;
-            float* half = red + turn * 128;
+            const float* half = red + turn * HALF;
+            if (lane < CL) hand(rank * W + (t >> 5), v);
             turn ^= 1;
-            if (lane == 0) half[t >> 5] = v;
-            sync();
-            v = half[lane % W];
+            sync_row();
+            v = half[lane % (W * CL)];
+            if constexpr (W * CL > 32) v += half[lane + 32];
 #pragma unroll
-            for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            for (int o = (W * CL > 32 ? 32 : W * CL) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         }
     }
     template <int K>
@@ -738,13 +768,16 @@ struct Group {
         if constexpr (TPR == 32) {
             __syncwarp();
         } else {
-            constexpr int W = TPR / 32;
-            float* half = red + turn * 128;
+            const float* half = red + turn * HALF;
+            if ((lane & 7) < CL) hand((rank * W + (t >> 5)) * 4 + (lane >> 3), a);
             turn ^= 1;
-            if ((lane & 7) == 0) half[(t >> 5) * 4 + (lane >> 3)] = a;
-            sync();
+            sync_row();
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (lane < W) x = *reinterpret_cast<const float4*>(half + lane * 4);
+            if (lane < W * CL) x = *reinterpret_cast<const float4*>(half + lane * 4);
+            if constexpr (W * CL > 32) {
+                const float4 y = *reinterpret_cast<const float4*>(half + (lane + 32) * 4);
+                x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+            }
             a = warp_sum4(x.x, x.y, x.z, K == 4 ? x.w : 0.0f);
         }
 #pragma unroll
@@ -787,12 +820,12 @@ struct RingSmem {
     float* red;
     uint64_t* full;
 };
-__device__ __forceinline__ RingSmem ring_smem(uint8_t* smem, const RingP& r, int n, int groups) {
+__device__ __forceinline__ RingSmem ring_smem(uint8_t* smem, const RingP& r, int n, int groups, int cluster = 1) {
     RingSmem s;
     s.vec = reinterpret_cast<float*>(smem);
     s.slots = smem + (size_t)r.vectors * n * 4;
     s.red = reinterpret_cast<float*>(s.slots + (size_t)groups * r.depth * r.slot_bytes);
-    s.full = reinterpret_cast<uint64_t*>(s.red + groups * 256);  // a group's sums: [2][32][4]
+    s.full = reinterpret_cast<uint64_t*>(s.red + groups * sum_floats(cluster));
     return s;
 }
 
@@ -884,7 +917,9 @@ __device__ __forceinline__ float shared_gate(const BlockP& p, int j) {
 
 // Forward.  Slots hold r and y; vectors P = s g gamma_post, Q = s g beta_post (g
 // where all rows share it), gamma_pre, beta_pre, those that there are (mask 1 2 4
-// 8).  8192 x 8192 bf16: see the table of measurements in the design notes.
+// 8).  8192 x 8192 bf16, RMS norms and a gate: 95 us and 5.7 TB/s, HBM-bound (a
+// device copy reaches 6.55); forward_rows_kernel, whose reads wait behind each row's
+// sums, took 241.
 // FULL: with layer norms, betas and gates that rows do not share; else RMS norms
 // and shared gates alone.
 template <typename T, int TPR, int C, bool FULL>
@@ -1100,9 +1135,16 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
 // a CTA, and column_kernel adds the partials in order.
 constexpr int kBackThreads = 512;
 
-// The groups' sums of one kind, added in order through acc [n], to the CTA's partial.
+// Columns of each CTA of a cluster of CL (the last may have fewer): whole eights.
+template <int CL>
+__device__ __host__ __forceinline__ int share_of(int64_t n) {
+    return CL == 1 ? (int)n : (int)columns((n + CL - 1) / CL);
+}
+
+// The groups' sums of one kind, added in order through acc [n], to the partial
+// `part` of rows of n columns, from column col0 on.
 template <typename G, int C>
-__device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc, int n, int which,
+__device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc, int64_t n, int part, int col0, int which,
                                           const f2 (&sums)[C][4], const int (&j)[C], const bool (&has)[C]) {
     if (!((q.sums >> which) & 1)) return;
     for (int k = 0; k < G::COUNT; ++k) {
@@ -1115,7 +1157,7 @@ __device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[c][i]) : sums[c][i];
                     if (k == G::COUNT - 1)
-                        a = reinterpret_cast<f2*>(q.partials + ((int64_t)blockIdx.x * 4 + which) * columns(n) + j[c]);
+                        a = reinterpret_cast<f2*>(q.partials + ((int64_t)part * 4 + which) * columns(n) + col0 + j[c]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) a[i] = x[i];
                 }
@@ -1124,28 +1166,33 @@ __device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc
 }
 
 // C: eights of a thread.  With the betas' sums a thread of sixteen columns spills
-// (and with all of shared memory taken, spills go to L2), so FULL takes eight up
-// to 4096 wide: 2047 x 1000 f32 layer norms, full gate: 45 us with C = 2.
+// (and with all of shared memory taken, spills go to L2), so FULL takes eight: 2047 x 1000 f32 layer norms, full gate: 45 us with C = 2, 30 so,
+// bound by the latency of a row's barriers among 16 warps (3.5 rows a group).
 //
 // BULK: rows arrive by bulk copies, which want 16-byte aligned rows of whole eights.
 // Else the group copies a row's tensors into its one slot itself, neighbouring
 // elements by neighbouring threads, a row ending in zeros up to whole eights, and
 // its results out of it likewise; groups of a CTA hide each other's waits.
-template <typename T, int TPR, int C, bool FULL, bool BULK>
+//
+// CL: CTAs of the cluster that shares a row, an equal share of its columns each.
+template <typename T, int TPR, int C, bool FULL, bool BULK, int CL>
 __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p, GradP q, RingP r, int mask) {
     extern __shared__ __align__(128) uint8_t smem[];
-    using G = Group<kBackThreads, TPR>;
-    const int n = (int)p.n;
-    const int cols = (int)columns(n);
-    const RingSmem sm = ring_smem(smem, r, cols, G::COUNT);
+    using G = Group<kBackThreads, TPR, CL>;
+    const int width = share_of<CL>(p.n), cols = (int)columns(width);
+    const RingSmem sm = ring_smem(smem, r, cols, G::COUNT, CL);
     G g;
     g.index = threadIdx.x / TPR;
     g.t = threadIdx.x % TPR;
     g.red = sm.red + g.index * 256;
+    g.join_cluster();
+    // the CTA's columns: n from col0 on
+    const int col0 = CL > 1 ? g.rank * width : 0, n = CL > 1 ? min(width, (int)p.n - col0) : (int)p.n;
+    const int part = blockIdx.x / CL;
     uint8_t* slots = sm.slots + (size_t)g.index * r.depth * r.slot_bytes;
     const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
-    const uint32_t row_bytes = (uint32_t)cols * sizeof(T);
-    const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
+    const uint32_t row_bytes = (uint32_t)(CL > 1 && BULK ? n : cols) * sizeof(T);
+    const int64_t step = (int64_t)(gridDim.x / CL) * G::COUNT, first = (int64_t)part * G::COUNT + g.index;
     const bool own_gate = FULL && (p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * r.depth);
 
@@ -1158,28 +1205,30 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     pdl_launch_dependents();
     float *v2 = sm.vec, *vp = v2 + (mask & 1 ? cols : 0), *vb = vp + (mask & 2 ? cols : 0);
     for (int j = threadIdx.x; j < cols; j += kBackThreads) {
-        const bool in = BULK || j < n;
-        if (mask & 1) v2[j] = in ? __ldg(p.pre.gamma + j) : 0.0f;
-        if (mask & 2) vp[j] = in ? p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f) : 0.0f;
-        if (mask & 4) vb[j] = in ? p.scale * __ldg(p.post.beta + j) : 0.0f;
+        const bool in = (BULK && CL == 1) || j < n;
+        const int at = col0 + j;
+        if (mask & 1) v2[j] = in ? __ldg(p.pre.gamma + at) : 0.0f;
+        if (mask & 2) vp[j] = in ? p.scale * shared_gate(p, at) * (p.post.gamma ? __ldg(p.post.gamma + at) : 1.0f) : 0.0f;
+        if (mask & 4) vb[j] = in ? p.scale * __ldg(p.post.beta + at) : 0.0f;
     }
     __syncthreads();
     // the slot's rows: z, then y, dz, dh; not BULK: all of them, and a gate's
     const uint32_t at_y = row_bytes, at_dz = at_y + (p.y || !BULK ? row_bytes : 0),
                    at_dh = at_dz + (q.dz || !BULK ? row_bytes : 0), at_gate = at_dh + row_bytes;
+    const uint32_t tensors = 1 + (p.y ? 1 : 0) + (q.dz ? 1 : 0) + (q.dh ? 1 : 0);
     bool ok = true;  // this thread's waits so far
     auto issue = [&](int64_t row, int slot) {
         const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * r.slot_bytes);
-        tc::mbar_expect_tx(bar, (uint32_t)r.slot_bytes);
-        bulk_load(dst, static_cast<const T*>(p.z) + row * p.ldz, row_bytes, bar);
-        if (p.y) bulk_load(dst + at_y, static_cast<const T*>(p.y) + row * p.ldy, row_bytes, bar);
-        if (q.dz) bulk_load(dst + at_dz, static_cast<const T*>(q.dz) + row * q.lddz, row_bytes, bar);
-        if (q.dh) bulk_load(dst + at_dh, static_cast<const T*>(q.dh) + row * q.lddh, row_bytes, bar);
+        tc::mbar_expect_tx(bar, CL > 1 ? tensors * row_bytes : (uint32_t)r.slot_bytes);
+        bulk_load(dst, static_cast<const T*>(p.z) + row * p.ldz + col0, row_bytes, bar);
+        if (p.y) bulk_load(dst + at_y, static_cast<const T*>(p.y) + row * p.ldy + col0, row_bytes, bar);
+        if (q.dz) bulk_load(dst + at_dz, static_cast<const T*>(q.dz) + row * q.lddz + col0, row_bytes, bar);
+        if (q.dh) bulk_load(dst + at_dh, static_cast<const T*>(q.dh) + row * q.lddh + col0, row_bytes, bar);
     };
     // a row into the slot, or out of it, by the group (not BULK)
     // (every read of a row before its first write: the compiler cannot tell them apart)
     auto take_row = [&](const void* from, int64_t stride, int64_t row, T (&v)[8 * C]) {
-        const T* x = static_cast<const T*>(from) + row * stride + g.t;
+        const T* x = static_cast<const T*>(from) + row * stride + col0 + g.t;
 #pragma unroll
         for (int i = 0; i < 8 * C; ++i) v[i] = i * TPR + g.t < n ? x[i * TPR] : T(0.0f);
     };
@@ -1191,7 +1240,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     };
     auto copy_out = [&](void* to, int64_t stride, int64_t row, uint32_t from) {
         const T* x = reinterpret_cast<const T*>(slots + from) + g.t;
-        T* d = static_cast<T*>(to) + row * stride + g.t;
+        T* d = static_cast<T*>(to) + row * stride + col0 + g.t;
         T v[8 * C];
 #pragma unroll
         for (int i = 0; i < 8 * C; ++i) v[i] = i * TPR + g.t < n ? x[i * TPR] : T(0.0f);
@@ -1201,7 +1250,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     };
     if (BULK && g.t == 0)
         for (int d = 0; d < r.depth && first + d * step < p.m; ++d) issue(first + d * step, d);
-    const float inv_n = 1.0f / (float)n;
+    const float inv_n = 1.0f / (float)p.n;
     int j[C];
     bool has[C];
     f2 sum_a[C][4], sum_b[FULL ? C : 1][4], sum_c[C][4], sum_d[FULL ? C : 1][4];
@@ -1246,7 +1295,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
             if (p.gate_mode == GATE_FULL)
 #pragma unroll
                 for (int c = 0; c < C; ++c)
-                    own[c] = !has[c] ? zero8<T>() : BULK ? load_raw8<T>(p.gate, row * p.ldg + j[c]) : load_raw8<T>(at + at_gate, j[c]);
+                    own[c] = !has[c] ? zero8<T>() : BULK ? load_raw8<T>(p.gate, row * p.ldg + col0 + j[c]) : load_raw8<T>(at + at_gate, j[c]);
         // sums of both norms: means first where there is a layer norm, then the
         // centred squares and a (z - mu)
         Stat sz{0.0f, 1.0f}, sy{0.0f, 1.0f};
@@ -1361,7 +1410,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                 }
             }
             if (!BULK) store8<T>(slots, at_dz / sizeof(T) + j[c], dr);
-            else if (q.dr) store8<T>(q.dr, row * q.lddr + j[c], dr);
+            else if (q.dr) store8<T>(q.dr, row * q.lddr + col0 + j[c], dr);
             if (!p.y) continue;
             const f2 rho = splat2(sy.rho);
             slot8<T>(at + at_y, j[c], hat[c]);
@@ -1391,7 +1440,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                 if (p.gate_mode == GATE_FULL) {
                     pairs8(own[c], gate);
                     if (!BULK) store8<T>(slots, at_gate / sizeof(T) + j[c], u);
-                    else if (q.dgate) store8<T>(q.dgate, row * q.lddg + j[c], u);
+                    else if (q.dgate) store8<T>(q.dgate, row * q.lddg + col0 + j[c], u);
                 } else {
                     const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
 #pragma unroll
@@ -1417,7 +1466,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
             g.sum(v);
             b0 = p.post.kind == RT_NORM_LAYER ? -v[0] * inv_n : 0.0f;
             b1 = v[1];
-            if (g.t == 0 && q.dgate && p.gate_mode == GATE_COLUMN) static_cast<float*>(q.dgate)[row * q.lddg] = v[2];
+            if (g.t == 0 && g.rank == 0 && q.dgate && p.gate_mode == GATE_COLUMN) static_cast<float*>(q.dgate)[row * q.lddg] = v[2];
         } else {
             g.sum(b1);
         }
@@ -1433,7 +1482,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                         if (FULL) b[c][i] = add2(b[c][i], add);
                         b[c][i] = mul2(fma2(hat[c][i], less_b1, b[c][i]), rho);
                     }
-                    if (BULK) store8<T>(q.dy, row * q.lddy + j[c], b[c]);
+                    if (BULK) store8<T>(q.dy, row * q.lddy + col0 + j[c], b[c]);
                     else store8<T>(slots, at_y / sizeof(T) + j[c], b[c]);
                 }
         }
@@ -1454,11 +1503,11 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     if (!q.partials) return;
     __syncthreads();  // the slots are all read
     float* acc = reinterpret_cast<float*>(sm.slots);
-    join_sums<G>(g, q, acc, n, 0, sum_a, j, has);
-    join_sums<G>(g, q, acc, n, 2, sum_c, j, has);
+    join_sums<G>(g, q, acc, p.n, part, col0, 0, sum_a, j, has);
+    join_sums<G>(g, q, acc, p.n, part, col0, 2, sum_c, j, has);
     if constexpr (FULL) {
-        join_sums<G>(g, q, acc, n, 1, sum_b, j, has);
-        join_sums<G>(g, q, acc, n, 3, sum_d, j, has);
+        join_sums<G>(g, q, acc, p.n, part, col0, 1, sum_b, j, has);
+        join_sums<G>(g, q, acc, p.n, part, col0, 3, sum_d, j, has);
     }
 }
 
@@ -1467,24 +1516,30 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
 // dr is computed and summed against y^ its successor's three sums are taken, and
 // all four are joined at once.  z, y and dh of a row are read into registers when
 // its sums are taken and their slots are then free; dz has slots of its own.
-template <int TPR>
+// 8192 x 8192: 132 us and 6.1 TB/s with 11 us of column_kernel behind them; the
+// kernel above, whose barriers come one after another, took 195 in all.
+template <int TPR, int CL>
 __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p, GradP q, RingP r) {
     using T = __nv_bfloat16;
     extern __shared__ __align__(128) uint8_t smem[];
-    using G = Group<kBackThreads, TPR>;
+    using G = Group<kBackThreads, TPR, CL>;
     constexpr int C = 2;
-    const int n = (int)p.n, depth = r.depth;
-    const RingSmem sm = ring_smem(smem, r, n, G::COUNT);
+    const int width = share_of<CL>(p.n), depth = r.depth;
+    const RingSmem sm = ring_smem(smem, r, width, G::COUNT, CL);
     G g;
     g.index = threadIdx.x / TPR;
     g.t = threadIdx.x % TPR;
     g.red = sm.red + g.index * 256;
+    g.join_cluster();
+    // the CTA's columns: n from col0 on
+    const int col0 = CL > 1 ? g.rank * width : 0, n = CL > 1 ? min(width, (int)p.n - col0) : (int)p.n;
+    const int part = blockIdx.x / CL;
     // slots: [depth] of z, y, dh, then [depth] of dz; barriers likewise
     uint8_t* slots = sm.slots + (size_t)g.index * depth * r.slot_bytes;
     const uint32_t row_bytes = (uint32_t)n * sizeof(T);
     uint8_t* slots_dz = slots + (size_t)depth * 3 * row_bytes;
     const uint32_t full = tc::smem_u32(sm.full + g.index * 2 * depth), full_dz = full + depth * 8;
-    const int64_t step = (int64_t)gridDim.x * G::COUNT, first = (int64_t)blockIdx.x * G::COUNT + g.index;
+    const int64_t step = (int64_t)(gridDim.x / CL) * G::COUNT, first = (int64_t)part * G::COUNT + g.index;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * 2 * depth);
 
     if (threadIdx.x == 0) {
@@ -1496,22 +1551,23 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
     pdl_launch_dependents();
     float *v2 = sm.vec, *vp = v2 + n;
     for (int j = threadIdx.x; j < n; j += kBackThreads) {
-        v2[j] = p.pre.gamma ? __ldg(p.pre.gamma + j) : 1.0f;
-        vp[j] = p.scale * shared_gate(p, j) * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
+        const int at = col0 + j;
+        v2[j] = p.pre.gamma ? __ldg(p.pre.gamma + at) : 1.0f;
+        vp[j] = p.scale * shared_gate(p, at) * (p.post.gamma ? __ldg(p.post.gamma + at) : 1.0f);
     }
     __syncthreads();
     bool ok = true;  // this thread's waits so far
     auto issue = [&](int64_t row, int slot) {
         const uint32_t bar = full + slot * 8, dst = tc::smem_u32(slots + (size_t)slot * 3 * row_bytes);
         tc::mbar_expect_tx(bar, 3 * row_bytes);
-        bulk_load(dst, static_cast<const T*>(p.z) + row * p.ldz, row_bytes, bar);
-        bulk_load(dst + row_bytes, static_cast<const T*>(p.y) + row * p.ldy, row_bytes, bar);
-        bulk_load(dst + 2 * row_bytes, static_cast<const T*>(q.dh) + row * q.lddh, row_bytes, bar);
+        bulk_load(dst, static_cast<const T*>(p.z) + row * p.ldz + col0, row_bytes, bar);
+        bulk_load(dst + row_bytes, static_cast<const T*>(p.y) + row * p.ldy + col0, row_bytes, bar);
+        bulk_load(dst + 2 * row_bytes, static_cast<const T*>(q.dh) + row * q.lddh + col0, row_bytes, bar);
     };
     auto issue_dz = [&](int64_t row, int slot) {
         const uint32_t bar = full_dz + slot * 8;
         tc::mbar_expect_tx(bar, row_bytes);
-        bulk_load(tc::smem_u32(slots_dz + (size_t)slot * row_bytes), static_cast<const T*>(q.dz) + row * q.lddz, row_bytes, bar);
+        bulk_load(tc::smem_u32(slots_dz + (size_t)slot * row_bytes), static_cast<const T*>(q.dz) + row * q.lddz + col0, row_bytes, bar);
     };
     if (g.t == 0)
         for (int d = 0; d < depth && first + d * step < p.m; ++d) {
@@ -1525,7 +1581,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
             ok = false;
         }
     };
-    const float inv_n = 1.0f / (float)n;
+    const float inv_n = 1.0f / (float)p.n;
     int j[C];
     bool has[C];
     f2 sum_a[C][4], sum_c[C][4];
@@ -1600,7 +1656,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
             vec8(v2, j[c], w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) dr[i] = fma2(fma2(h[i], less_a1, mul2(d[i], w[i])), rz2, dr[i]);
-            if (q.dr) store8<T>(q.dr, row * q.lddr + j[c], dr);
+            if (q.dr) store8<T>(q.dr, row * q.lddr + col0 + j[c], dr);
             pairs8(ry[c], hat[c]);
             vec8(vp, j[c], w);
 #pragma unroll
@@ -1632,7 +1688,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
                 if (has[c]) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) b[c][i] = mul2(fma2(hat[c][i], less_b1, b[c][i]), ry2);
-                    store8<T>(q.dy, row * q.lddy + j[c], b[c]);
+                    store8<T>(q.dy, row * q.lddy + col0 + j[c], b[c]);
                 }
         }
         stats(v[0], v[1], v[2]);
@@ -1646,8 +1702,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
     if (!q.partials) return;
     __syncthreads();  // the slots are all read
     float* acc = reinterpret_cast<float*>(sm.slots);
-    join_sums<G>(g, q, acc, n, 0, sum_a, j, has);
-    join_sums<G>(g, q, acc, n, 2, sum_c, j, has);
+    join_sums<G>(g, q, acc, p.n, part, col0, 0, sum_a, j, has);
+    join_sums<G>(g, q, acc, p.n, part, col0, 2, sum_c, j, has);
 }
 
 struct ReduceP {
@@ -1807,10 +1863,10 @@ cudaError_t launch_forward_rows(bool pdl, const BlockP& p, cudaStream_t st) {
 
 // Fills in the ring's shape, of at most `most` slots a group; false where not even
 // one fits.
-bool plan_ring(RingP* r, int64_t n, int groups, int tensors, size_t es, int vectors, int most = 4) {
+bool plan_ring(RingP* r, int64_t n, int groups, int tensors, size_t es, int vectors, int most = 4, int cluster = 1) {
     r->slot_bytes = (int)(tensors * n * (int64_t)es);
     r->vectors = vectors;
-    const int64_t room = kRingSmem - ring_scratch(groups) - (int64_t)vectors * n * 4;
+    const int64_t room = kRingSmem - ring_scratch(groups, cluster) - (int64_t)vectors * n * 4;
     r->depth = (int)std::min<int64_t>(most, room / ((int64_t)groups * r->slot_bytes));
     r->smem = (int)(kRingSmem - room) + groups * r->depth * r->slot_bytes;
     return r->depth >= 1;
@@ -1848,51 +1904,100 @@ int forward_ring(rt_ctx* ctx, const BlockP& p, cudaStream_t st, bool* done) {
     return launch_forward_ring<T, 512, 2>(ctx, p, r, mask, st);
 }
 
-template <typename T, int TPR, int C, bool FULL, bool BULK = true>
-int launch_backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, const RingP& r, int mask, int ctas, cudaStream_t st) {
-    auto* kernel = backward_ring_kernel<T, TPR, C, FULL, BULK>;
+template <typename T, int TPR, int C, bool FULL, bool BULK, int CL = 1>
+int launch_backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, const RingP& r, int mask, int parts, cudaStream_t st) {
+    auto* kernel = backward_ring_kernel<T, TPR, C, FULL, BULK, CL>;
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)ctas, kBackThreads, r.smem, st, p, q, r, mask));
+    RT_CUDA(launch_cluster(CL, ctx->pdl, kernel, (unsigned)(parts * CL), kBackThreads, r.smem, st, p, q, r, mask));
     return RT_OK;
 }
 
-template <int TPR>
-int launch_backward_pipe(bool pdl, const BlockP& p, const GradP& q, const RingP& r, int ctas, cudaStream_t st) {
-    RT_CUDA(cudaFuncSetAttribute(backward_pipe_kernel<TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-    RT_CUDA(launch_k(pdl, backward_pipe_kernel<TPR>, (unsigned)ctas, kBackThreads, r.smem, st, p, q, r));
+template <int TPR, int CL = 1>
+int launch_backward_pipe(bool pdl, const BlockP& p, const GradP& q, const RingP& r, int parts, cudaStream_t st) {
+    auto* kernel = backward_pipe_kernel<TPR, CL>;
+    RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+    RT_CUDA(launch_cluster(CL, pdl, kernel, (unsigned)(parts * CL), kBackThreads, r.smem, st, p, q, r));
     return RT_OK;
 }
 
-// The backward pass through the ring, where a row of every tensor fits in it for
-// each group: up to 8192 wide.  *parts is then the number of partials.
+template <typename T, bool BULK>
+int launch_backward_full(rt_ctx* ctx, const BlockP& p, const GradP& q, const RingP& r, int mask, int tpr, int cluster, int parts,
+                         cudaStream_t st) {
+    if (cluster == 4) return launch_backward_ring<T, 512, 1, true, BULK, 4>(ctx, p, q, r, mask, parts, st);
+    if (cluster == 2) return launch_backward_ring<T, 512, 1, true, BULK, 2>(ctx, p, q, r, mask, parts, st);
+    switch (tpr) {
+        case 32: return launch_backward_ring<T, 32, 1, true, BULK>(ctx, p, q, r, mask, parts, st);
+        case 64: return launch_backward_ring<T, 64, 1, true, BULK>(ctx, p, q, r, mask, parts, st);
+        case 128: return launch_backward_ring<T, 128, 1, true, BULK>(ctx, p, q, r, mask, parts, st);
+        case 256: return launch_backward_ring<T, 256, 1, true, BULK>(ctx, p, q, r, mask, parts, st);
+        default: return launch_backward_ring<T, 512, 1, true, BULK>(ctx, p, q, r, mask, parts, st);
+    }
+}
+
+// Rings that take a row by four CTAs: how many such clusters the device runs at once
+// (what it is divided into decides that, so it is asked, once).
+int ring_clusters(rt_ctx* ctx, int cluster, int* count) {
+    *count = ctx->sm_count / cluster;
+    if (cluster <= 2) return RT_OK;
+    if (ctx->ring_clusters4 == 0) {
+        auto* kernel = backward_ring_kernel<float, kBackThreads, 1, true, true, 4>;
+        RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = 4 * *count;
+        cfg.blockDim = kBackThreads;
+        cfg.dynamicSmemBytes = kRingSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {4, 1, 1};
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        RT_CUDA(cudaOccupancyMaxActiveClusters(&ctx->ring_clusters4, kernel, &cfg));
+        RT_CHECK(ctx->ring_clusters4 > 0, "no cluster of four thread blocks fits the device");
+    }
+    *count = std::min(*count, ctx->ring_clusters4);
+    return RT_OK;
+}
+
+// The backward pass through the ring, up to 16384 wide.  *parts is then the number of
+// partials.  A CTA takes 8192 columns, 4096 with all features (which want registers):
+// wider rows are shared by a cluster.  1000 x 16384 bf16 RMS 61 us so, layer norms with
+// a full gate 164, against 301 and 416 by the kernel for any width; 4096 x 4099 with
+// all features 423 against 540 by one CTA whose threads spill.  Unaligned rows up to
+// 4096 wide take the full kernel without its features: eight columns a thread, 4000 x
+// 1001 37 us.
 template <typename T>
 int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st, int* parts, bool* done) {
     *done = false;
     const size_t es = sizeof(T);
-    if (p.n > 8192 || p.m == 0 || !aligned16(q.partials, 0, 4)) return RT_OK;
+    if (p.n > 16384 || p.m == 0 || !aligned16(q.partials, 0, 4)) return RT_OK;
     const bool bulk = rows_aligned(p, es) && aligned16(q.dz, q.lddz, es) && aligned16(q.dh, q.lddh, es) &&
                       aligned16(q.dr, q.lddr, es) && aligned16(q.dy, q.lddy, es) &&
                       (p.gate_mode != GATE_FULL || aligned16(q.dgate, q.lddg, es));
     const bool shared = p.gate_mode == GATE_ONE || p.gate_mode == GATE_ROW;
     const int mask = (p.pre.gamma ? 1 : 0) | (p.post.gamma || (p.y && shared) ? 2 : 0) |
                      (p.post.beta && q.dgate && !shared ? 4 : 0);
-    const bool full = p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
+    const bool full = (!bulk && p.n <= 4096) || p.post.kind == RT_NORM_LAYER || p.pre.kind == RT_NORM_LAYER || (q.sums & 10) ||
                       p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL;
-    const int eights = (full || !bulk) && p.n <= 4096 ? 1 : 2;
-    int tpr = 32;
-    while (tpr * eights * 8 < p.n) tpr *= 2;
+    const int eights = full ? 1 : 2;
+    int tpr = 32, cluster = 1;
+    while (tpr < kBackThreads && tpr * eights * 8 < p.n) tpr *= 2;
+    while (cluster * tpr * eights * 8 < p.n) cluster *= 2;
     const int groups = kBackThreads / tpr;
+    const int64_t width = columns((p.n + cluster - 1) / cluster);
     RingP r{};
     r.err = ctx->dev_err;
     const int tensors = bulk ? 1 + (p.y ? 1 : 0) + (q.dz ? 1 : 0) + (q.dh ? 1 : 0) : p.gate_mode == GATE_FULL ? 5 : 4;
-    if (!plan_ring(&r, columns(p.n), groups, tensors, es, __builtin_popcount(mask), bulk ? 4 : 1)) return RT_OK;
+    if (!plan_ring(&r, width, groups, tensors, es, __builtin_popcount(mask), bulk ? 4 : 1, cluster)) return RT_OK;
     *done = true;
-    *parts = (int)std::min<int64_t>(ctx->sm_count, (p.m + groups - 1) / groups);
+    int clusters = 0;
+    RT_TRY(ring_clusters(ctx, cluster, &clusters));
+    *parts = (int)std::min<int64_t>(clusters, (p.m + groups - 1) / groups);
     if constexpr (sizeof(T) == 2) {
         RingP two{};
         two.err = ctx->dev_err;
         if (bulk && !full && p.post.kind == RT_NORM_RMS && p.pre.kind == RT_NORM_RMS && q.dz && q.dh &&
-            plan_ring(&two, p.n, groups, 4, es, 2) && two.depth >= 2) {
+            plan_ring(&two, width, groups, 4, es, 2, 4, cluster) && two.depth >= 2) {
+            if (cluster == 2) return launch_backward_pipe<512, 2>(ctx->pdl, p, q, two, *parts, st);
             switch (tpr) {
                 case 32: return launch_backward_pipe<32>(ctx->pdl, p, q, two, *parts, st);
                 case 64: return launch_backward_pipe<64>(ctx->pdl, p, q, two, *parts, st);
@@ -1902,33 +2007,21 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
             }
         }
     }
-    if (!bulk) {
-        if (eights == 2)
-            return full ? launch_backward_ring<T, 512, 2, true, false>(ctx, p, q, r, mask, *parts, st)
-                        : launch_backward_ring<T, 512, 2, false, false>(ctx, p, q, r, mask, *parts, st);
+    if (!full && !bulk)
+        return cluster == 2 ? launch_backward_ring<T, 512, 2, false, false, 2>(ctx, p, q, r, mask, *parts, st)
+                            : launch_backward_ring<T, 512, 2, false, false>(ctx, p, q, r, mask, *parts, st);
+    if (!full) {
+        if (cluster == 2) return launch_backward_ring<T, 512, 2, false, true, 2>(ctx, p, q, r, mask, *parts, st);
         switch (tpr) {
-            case 32: return launch_backward_ring<T, 32, 1, true, false>(ctx, p, q, r, mask, *parts, st);
-            case 64: return launch_backward_ring<T, 64, 1, true, false>(ctx, p, q, r, mask, *parts, st);
-            case 128: return launch_backward_ring<T, 128, 1, true, false>(ctx, p, q, r, mask, *parts, st);
-            case 256: return launch_backward_ring<T, 256, 1, true, false>(ctx, p, q, r, mask, *parts, st);
-            default: return launch_backward_ring<T, 512, 1, true, false>(ctx, p, q, r, mask, *parts, st);
+            case 32: return launch_backward_ring<T, 32, 2, false, true>(ctx, p, q, r, mask, *parts, st);
+            case 64: return launch_backward_ring<T, 64, 2, false, true>(ctx, p, q, r, mask, *parts, st);
+            case 128: return launch_backward_ring<T, 128, 2, false, true>(ctx, p, q, r, mask, *parts, st);
+            case 256: return launch_backward_ring<T, 256, 2, false, true>(ctx, p, q, r, mask, *parts, st);
+            default: return launch_backward_ring<T, 512, 2, false, true>(ctx, p, q, r, mask, *parts, st);
         }
     }
-    if (!full) switch (tpr) {
-            case 32: return launch_backward_ring<T, 32, 2, false>(ctx, p, q, r, mask, *parts, st);
-            case 64: return launch_backward_ring<T, 64, 2, false>(ctx, p, q, r, mask, *parts, st);
-            case 128: return launch_backward_ring<T, 128, 2, false>(ctx, p, q, r, mask, *parts, st);
-            case 256: return launch_backward_ring<T, 256, 2, false>(ctx, p, q, r, mask, *parts, st);
-            default: return launch_backward_ring<T, 512, 2, false>(ctx, p, q, r, mask, *parts, st);
-        }
-    if (eights == 2) return launch_backward_ring<T, 512, 2, true>(ctx, p, q, r, mask, *parts, st);
-    switch (tpr) {
-        case 32: return launch_backward_ring<T, 32, 1, true>(ctx, p, q, r, mask, *parts, st);
-        case 64: return launch_backward_ring<T, 64, 1, true>(ctx, p, q, r, mask, *parts, st);
-        case 128: return launch_backward_ring<T, 128, 1, true>(ctx, p, q, r, mask, *parts, st);
-        case 256: return launch_backward_ring<T, 256, 1, true>(ctx, p, q, r, mask, *parts, st);
-        default: return launch_backward_ring<T, 512, 1, true>(ctx, p, q, r, mask, *parts, st);
-    }
+    return bulk ? launch_backward_full<T, true>(ctx, p, q, r, mask, tpr, cluster, *parts, st)
+                : launch_backward_full<T, false>(ctx, p, q, r, mask, tpr, cluster, *parts, st);
 }
 
 // Up to 16384 wide: the fewest threads that hold a row eight elements each (the

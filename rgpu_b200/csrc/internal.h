@@ -72,6 +72,7 @@ struct rt_ctx {
     // device address of rt_matmul_split_k_noalloc's built-in scratch array
     // (looked up on that entry point's first call on this context)
     float* splitk_static = nullptr;
+    int ring_clusters4 = 0;  // clusters of four CTAs that fit the device at once (block_norm.cu; 0: not asked yet)
     uint64_t launches = 0;
     char name[256] = {0};
 };
@@ -184,21 +185,29 @@ __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepc
 // and set-up overlap that kernel's tail, and each waits for it before it
 // touches memory.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_k(bool pdl, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                     Args... args) {
+cudaError_t launch_cluster(int cluster, bool pdl, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                           cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
     if (pdl) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs++].val.clusterDim = {(unsigned)cluster, 1, 1};
     }
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_k(bool pdl, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                     Args... args) {
+    return launch_cluster(1, pdl, kernel, grid, block, smem, st, args...);
 }
 
 // Peer memory of a communicator's ranks (comm.cu).

@@ -171,6 +171,17 @@ def test_wide_and_odd_rows(gpu, m, n, pad, kind, vectors, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind,vectors", [("layer", True), ("rms", "gamma"), ("none", False)])
+@pytest.mark.parametrize("m,n", [(160, 4104), (76, 8192), (1, 8200), (90, 9000), (150, 16384), (41, 10003), (2, 16392), (3, 20001)])
+def test_rows_of_several_thread_blocks(gpu, m, n, kind, vectors, dtype):
+    # 4096 or 8192 columns to a thread block in the backward pass
+    for gate in ("column", "full") if vectors is True else ("row",):
+        c = Case(gpu, m, n, dtype, kind, kind, gate, seed=m + n, vectors=vectors)
+        which = None if vectors is True else ("dr", "dy", "dgamma_post", "dgamma_pre", "dgate") if vectors else ("dr", "dy", "dgate")
+        _backward_check(c, c.host["r"], _backward(gpu, c, c.dev["r"], which=which), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("gate", ["none", "one", "row", "column", "full"])
 def test_every_gate_and_in_place(gpu, gate, dtype):
     c = Case(gpu, 19, 320, dtype, "layer", "rms", gate, seed=4)
