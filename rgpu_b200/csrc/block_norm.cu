@@ -1141,13 +1141,13 @@ __device__ __host__ __forceinline__ int share_of(int64_t n) {
     return CL == 1 ? (int)n : (int)columns((n + CL - 1) / CL);
 }
 
-// The groups' sums of one kind, added in order through acc [n], to the partial
+// The sums of one kind of the groups that had a row, added in order through acc [n], to the partial
 // `part` of rows of n columns, from column col0 on.
 template <typename G, int C>
-__device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc, int64_t n, int part, int col0, int which,
+__device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc, int groups, int64_t n, int part, int col0, int which,
                                           const f2 (&sums)[C][4], const int (&j)[C], const bool (&has)[C]) {
     if (!((q.sums >> which) & 1)) return;
-    for (int k = 0; k < G::COUNT; ++k) {
+    for (int k = 0; k < groups; ++k) {
         if (g.index == k)
 #pragma unroll
             for (int c = 0; c < C; ++c)
@@ -1156,18 +1156,19 @@ __device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc
                     f2 x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = k > 0 ? add2(a[i], sums[c][i]) : sums[c][i];
-                    if (k == G::COUNT - 1)
+                    if (k == groups - 1)
                         a = reinterpret_cast<f2*>(q.partials + ((int64_t)part * 4 + which) * columns(n) + col0 + j[c]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) a[i] = x[i];
                 }
-        if (G::COUNT > 1) __syncthreads();
+        if (groups > 1) __syncthreads();
     }
 }
 
 // C: eights of a thread.  With the betas' sums a thread of sixteen columns spills
-// (and with all of shared memory taken, spills go to L2), so FULL takes eight: 2047 x 1000 f32 layer norms, full gate: 45 us with C = 2, 30 so,
-// bound by the latency of a row's barriers among 16 warps (3.5 rows a group).
+// (and with all of shared memory taken, spills go to L2), so FULL takes eight: 2047 x 1000 f32 layer norms, full gate: 26 us with the sums
+// over columns behind it, 15 more with C = 2; bound by the latency of a row's barriers
+// among 16 warps (3.5 rows a group).
 //
 // BULK: rows arrive by bulk copies, which want 16-byte aligned rows of whole eights.
 // Else the group copies a row's tensors into its one slot itself, neighbouring
@@ -1192,7 +1193,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     uint8_t* slots = sm.slots + (size_t)g.index * r.depth * r.slot_bytes;
     const uint32_t full = tc::smem_u32(sm.full + g.index * r.depth);
     const uint32_t row_bytes = (uint32_t)(CL > 1 && BULK ? n : cols) * sizeof(T);
-    const int64_t step = (int64_t)(gridDim.x / CL) * G::COUNT, first = (int64_t)part * G::COUNT + g.index;
+    // rows go to the thread blocks in turn, then to their groups: few rows spread over the device
+    const int64_t parts = gridDim.x / CL, step = parts * G::COUNT, first = g.index * parts + part;
     const bool own_gate = FULL && (p.gate_mode == GATE_COLUMN || p.gate_mode == GATE_FULL);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * r.depth);
 
@@ -1503,11 +1505,12 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     if (!q.partials) return;
     __syncthreads();  // the slots are all read
     float* acc = reinterpret_cast<float*>(sm.slots);
-    join_sums<G>(g, q, acc, p.n, part, col0, 0, sum_a, j, has);
-    join_sums<G>(g, q, acc, p.n, part, col0, 2, sum_c, j, has);
+    const int groups = (int)min((p.m - part + parts - 1) / parts, (int64_t)G::COUNT);  // that had a row
+    join_sums<G>(g, q, acc, groups, p.n, part, col0, 0, sum_a, j, has);
+    join_sums<G>(g, q, acc, groups, p.n, part, col0, 2, sum_c, j, has);
     if constexpr (FULL) {
-        join_sums<G>(g, q, acc, p.n, part, col0, 1, sum_b, j, has);
-        join_sums<G>(g, q, acc, p.n, part, col0, 3, sum_d, j, has);
+        join_sums<G>(g, q, acc, groups, p.n, part, col0, 1, sum_b, j, has);
+        join_sums<G>(g, q, acc, groups, p.n, part, col0, 3, sum_d, j, has);
     }
 }
 
@@ -1516,7 +1519,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
 // dr is computed and summed against y^ its successor's three sums are taken, and
 // all four are joined at once.  z, y and dh of a row are read into registers when
 // its sums are taken and their slots are then free; dz has slots of its own.
-// 8192 x 8192: 132 us and 6.1 TB/s with 11 us of column_kernel behind them; the
+// 8192 x 8192: 132 us and 6.1 TB/s with 10 us of column_kernel behind them; the
 // kernel above, whose barriers come one after another, took 195 in all.
 template <int TPR, int CL>
 __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p, GradP q, RingP r) {
@@ -1539,7 +1542,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
     const uint32_t row_bytes = (uint32_t)n * sizeof(T);
     uint8_t* slots_dz = slots + (size_t)depth * 3 * row_bytes;
     const uint32_t full = tc::smem_u32(sm.full + g.index * 2 * depth), full_dz = full + depth * 8;
-    const int64_t step = (int64_t)(gridDim.x / CL) * G::COUNT, first = (int64_t)part * G::COUNT + g.index;
+    // rows go to the thread blocks in turn, then to their groups: few rows spread over the device
+    const int64_t parts = gridDim.x / CL, step = parts * G::COUNT, first = g.index * parts + part;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm.full + G::COUNT * 2 * depth);
 
     if (threadIdx.x == 0) {
@@ -1702,8 +1706,9 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
     if (!q.partials) return;
     __syncthreads();  // the slots are all read
     float* acc = reinterpret_cast<float*>(sm.slots);
-    join_sums<G>(g, q, acc, p.n, part, col0, 0, sum_a, j, has);
-    join_sums<G>(g, q, acc, p.n, part, col0, 2, sum_c, j, has);
+    const int groups = (int)min((p.m - part + parts - 1) / parts, (int64_t)G::COUNT);  // that had a row
+    join_sums<G>(g, q, acc, groups, p.n, part, col0, 0, sum_a, j, has);
+    join_sums<G>(g, q, acc, groups, p.n, part, col0, 2, sum_c, j, has);
 }
 
 struct ReduceP {
@@ -1718,30 +1723,53 @@ struct ReduceP {
     float* gate_row;  // [n]: a [1,1] gate's gradient by column
 };
 
-// Column sums of the partials and the vectors they give.  A CTA takes 32 columns;
-// each of its 16 warps adds every 16th part in order, the warps' sums are added
-// in order: 148 parts one after another took 82 us at 8192 columns, all latency.
-__global__ void __launch_bounds__(512) column_kernel(ReduceP p) {
-    __shared__ float sums[16][4][32];
+// Column sums of the partials and the vectors they give.  All latency: a CTA takes
+// COLS columns, Q = 32 / COLS lanes of each of its warps every (Q WARPS)th part, all
+// reads under way together; the lanes' and then the warps' sums are added in order.
+// Eight columns (a sector) up to 4096 wide: 148 parts of 1000 columns 3 us behind the
+// kernel before it, where 32 columns and reads one after another took 10.  Wider, 32
+// columns keep the CTAs to one wave.
+template <int COLS>
+__global__ void __launch_bounds__(COLS * 16 + 512) column_kernel(ReduceP p) {
+    constexpr int WARPS = COLS / 2 + 16, Q = 32 / COLS, STEP = WARPS * Q, U = 160 / STEP;
+    __shared__ float sums[WARPS][4 * COLS];
+    __shared__ float totals[4 * COLS];
     pdl_wait();
     pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, column = lane % COLS;
+    const int64_t j = (int64_t)blockIdx.x * COLS + column, stride = columns(p.n);
     float s[4] = {};
-    if (j < p.n)
-#pragma unroll 5
-        for (int i = warp; i < p.parts; i += 16)
+    for (int i0 = warp * Q + lane / COLS; i0 < p.parts; i0 += U * STEP) {
+        float x[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int v = 0; v < 4; ++v)
-                if ((p.sums >> v) & 1) s[v] += p.partials[((int64_t)i * 4 + v) * columns(p.n) + j];
+                x[u][v] = j < p.n && i0 + u * STEP < p.parts && ((p.sums >> v) & 1)
+                              ? p.partials[((int64_t)(i0 + u * STEP) * 4 + v) * stride + j]
+                              : 0.0f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) sums[warp][v][lane] = s[v];
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) s[v] += x[u][v];
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+#pragma unroll
+        for (int o = COLS; o < 32; o *= 2) s[v] += __shfl_xor_sync(0xffffffffu, s[v], o);
+        if (lane < COLS) sums[warp][v * COLS + column] = s[v];
+    }
     __syncthreads();
-    if (warp > 0 || j >= p.n) return;
+    if (threadIdx.x < 4 * COLS) {
+        float total = 0.0f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+        for (int w = 0; w < WARPS; ++w) total += sums[w][threadIdx.x];
+        totals[threadIdx.x] = total;
+    }
+    __syncthreads();
+    if (threadIdx.x >= COLS || j >= p.n) return;
 #pragma unroll
-        for (int w = 1; w < 16; ++w) s[v] += sums[w][v][lane];
+    for (int v = 0; v < 4; ++v) s[v] = totals[v * COLS + column];
     s[0] *= p.scale;
     s[1] *= p.scale;
     const float g = p.gate_mode == GATE_ONE ? p.gate[0] : p.gate_mode == GATE_ROW ? p.gate[j] : 1.0f;
@@ -1991,7 +2019,7 @@ int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st,
     *done = true;
     int clusters = 0;
     RT_TRY(ring_clusters(ctx, cluster, &clusters));
-    *parts = (int)std::min<int64_t>(clusters, (p.m + groups - 1) / groups);
+    *parts = (int)std::min<int64_t>(clusters, p.m);
     if constexpr (sizeof(T) == 2) {
         RingP two{};
         two.err = ctx->dev_err;
@@ -2209,7 +2237,11 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     c.gamma = p.post.gamma;
     c.beta = p.post.beta;
     if (gate_sums && p.gate_mode == GATE_ONE) c.gate_row = q.partials + (int64_t)parts_for(ctx, p.m) * 4 * columns(p.n);
-    RT_CUDA(launch_k(ctx->pdl, column_kernel, (unsigned)((p.n + 31) / 32), 512, 0, ctx->stream, c));
+    if (p.n <= 4096) {
+        RT_CUDA(launch_k(ctx->pdl, column_kernel<8>, (unsigned)((p.n + 7) / 8), 640, 0, ctx->stream, c));
+    } else {
+        RT_CUDA(launch_k(ctx->pdl, column_kernel<32>, (unsigned)((p.n + 31) / 32), 1024, 0, ctx->stream, c));
+    }
     count_launch(ctx);
     if (c.gate_row) {
         RT_CUDA(launch_k(ctx->pdl, gate_one_kernel, 1, kWide, 0, ctx->stream, c.gate_row, p.n, c.dgate));
