@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) skinny_n_kernel(SkinnyParams p) {
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (32 * u >= kn) break;  // a[u] is zero past k; its B rows were not staged
+            if (lane + 32 * u >= kn) break;  // past k nothing was staged: zero times whatever lies there may be NaN
             const float4* br = reinterpret_cast<const float4*>(&sb[lane + 32 * u][0]);
 #pragma unroll
             for (int t4 = 0; t4 < 4; ++t4) {
