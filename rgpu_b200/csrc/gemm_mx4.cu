@@ -237,21 +237,22 @@ __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, ui
 // along k.  Their sums meet in shared memory and are added in rank order, tokens
 // dealt out over the CTAs.  One token by 8192 x 8192: 9.7 us in a stream of launches,
 // 5.4 of them the weights' 36 MB at the rate of a copy, the others the launch and the
-// join.  64 x 8192 x 4096: 7.8 us, a stage (0.25 us) bound by the way from L2 and the
-// issue of its copies and MMAs, not by the tensor cores (under 30 % busy).
+// join.  64 x 8192 x 4096: 7.0 us.  2047 x 1000 x 8192: 12.0 us, a stage 0.23 us for 35
+// KB, 19 TB/s from L2 to all SMs.
 template <int TN>
 struct Geo1 {
     static constexpr int T_BYTES = TN * kRowBytes;
     static constexpr int STAGE_BYTES = kWBytes + T_BYTES + 4 * kScaleTile;  // codes, two scale tiles of either side
-    static constexpr int STAGES = 4;
-    static constexpr int TMEM_COLS = 256;  // two accumulators of TN, and 16 of scales a stage
+    static constexpr int CTAS = TN > 64 ? 1 : 2;  // to an SM
+    static constexpr int STAGES = CTAS > 1 ? 4 : 6;
+    static constexpr int TMEM_COLS = 512 / CTAS;  // two accumulators of TN, and 16 of scales a stage
     static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
     static_assert(2 * TN + 16 * STAGES <= TMEM_COLS, "TMEM columns");
-    static_assert(2 * SMEM <= 226 * 1024, "two CTAs to an SM");
+    static_assert(CTAS * SMEM <= 226 * 1024, "shared memory of an SM");
     static_assert(TN * 512 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
 };
 
-constexpr int kThreads1 = 192;  // warps: 0 TMA, 1 MMA, 2-5 epilogue (one TMEM lane quadrant each)
+constexpr int kThreads1 = 224;  // warps: 0 TMA, 1 MMA, 2-5 epilogue (one TMEM lane quadrant each), 6 MMA
 
 template <int TN>
 __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
         }
-        mbar_init(smem_u32(done), 1);
+        mbar_init(smem_u32(done), 2);
         *abort_flag = 0;
         *issued_all = 0;
         fence_barrier_init();
@@ -336,19 +337,21 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
                 *abort_flag = 1;
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 6) {
+        // A stage's copies and MMAs take a warp 0.3 us to issue, more than they take to run:
+        // two warps take every second stage, with an accumulator each (100 x 1000 x 4096: 6.7
+        // us, with one 7.6).
+        const int odd = warp == 6;
         const uint32_t token_col = (uint32_t)((tm * TN % 128) / 32);  // the tile's place in its 128-row scale tile
         const uint64_t w0 = smem_desc(smem_u32(smem_w), 16, 1024), t0 = smem_desc(smem_u32(smem_t), 16, 1024);
         const uint64_t sc0 = scale_desc(smem_u32(smem_s));
-        const uint32_t cols0 = tmem + 2 * TN;
+        const uint32_t cols0 = tmem + 2 * TN, sum = tmem + odd * TN;
+        static_assert(G::STAGES % 2 == 0, "a warp's stages are every second slot");
         bool ok = true;
-        int slot = 0, phase = 0;
-        for (int s = s0; s < s1; ++s) {
-            ok = mbar_wait(smem_u32(&full[slot]), phase, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
+        int slot = odd, phase = 0;
+        for (int s = s0 + odd; s < s1; s += 2) {
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), phase, abort_flag));
+            if (!ok) break;
             tc_fence_after();
             const uint64_t w = w0 + slot * (kWBytes >> 4), t = t0 + slot * (G::T_BYTES >> 4);
             const uint64_t sc = sc0 + slot * (4 * kScaleTile >> 4);
@@ -360,14 +363,14 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
                     if (kk < steps)
-                        mma_mx4<1>(tmem + (kk & 1) * TN, w + kk * 2, t + kk * 2, mx4_idesc(128, TN, kk & 1),
-                                   cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 4 + token_col,
-                                   (s > s0 || kk > 1) ? 1u : 0u);
+                        mma_mx4<1>(sum, w + kk * 2, t + kk * 2, mx4_idesc(128, TN, kk & 1), cols + (kk >> 1) * 4,
+                                   cols + 8 + (kk >> 1) * 4 + token_col, (s > s0 + 1 || kk > 0) ? 1u : 0u);
                 tc_commit(smem_u32(&empty[slot]));
             }
             __syncwarp();
-            if (++slot == G::STAGES) {
-                slot = 0;
+            slot += 2;
+            if (slot >= G::STAGES) {
+                slot -= G::STAGES;
                 phase ^= 1;
             }
         }
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
             }
             tc_commit(smem_u32(done));
         }
-    } else if (warp >= 2) {
+    } else {
         const int quad = warp & 3;
         const int count = (int)min((int64_t)TN, p.m - (int64_t)tm * TN);
         const bool got = mbar_wait(smem_u32(done), 0, abort_flag);
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
         __syncwarp();
         tc_fence_after();
         float* sums = reinterpret_cast<float*>(smem) + quad * 32 + lane;  // [token][128 columns]; every stage has been read
-        const bool two = s1 - s0 > 1 || p.blocks - s0 * kStageBlocks > 2;  // the second accumulator was written
+        const bool two = s1 - s0 > 1;  // the second accumulator was written
         for (int c = 0; c < count && __all_sync(0xffffffffu, got); c += 32) {
             float v[32];
             tmem_ld_32x32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)c, v);
@@ -906,7 +909,8 @@ int gemm_mx4_init() {
     RT_TRY(allow_smem<32>());
     RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
     RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    return allow_smem<64>();
+    RT_TRY(allow_smem<64>());
+    return allow_smem<128>();
 }
 
 int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
@@ -930,16 +934,21 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
         count_launch(ctx);
         return RT_OK;
     }
-    // One-CTA tiles while they fit the device at once, two to an SM (2047 x 1000 x
-    // 8192: 14.4 us against 16.5 with pairs; 256 x 8192 x 2048: 7.5 / 9.2), else pairs,
-    // which load half as much per MMA (1024 x 4096 x 1024: 8.6 / 11.5; 2048^3: 9.8 /
-    // 13.9).
+    // One-CTA tiles while they fit the device at once, two of 64 tokens to an SM (256 x
+    // 8192 x 2048: 7.1 us against 9.2 with pairs), else pairs, which load half as much
+    // per MMA (1024 x 4096 x 1024: 8.6 / 11.5; 2048^3: 9.8 / 13.9).  Where most SMs would
+    // hold two, one of 128 tokens reads two thirds of the bytes, but has more to do after
+    // its last stage: 2047 x 1000 x 8192, 32 stages, 12.0 us / 13.7; 512 x 4096 x 4096, 16
+    // stages, 8.2 / 9.1; 256 x 8192 x 2048, 8 stages, 6.9 / 6.9; 2048 x 1024 x 1024, 4
+    // stages, 6.1 / 5.6.
     const int tn = p.m <= 32 ? 32 : 64;
     const int64_t tiles = ((p.m + tn - 1) / tn) * ((p.n + 127) / 128), slots = 2 * (int64_t)ctx->sm_count;
     if (tiles > slots) return launch_pair(ctx, a, b, p, stream);
+    if (tiles > ctx->sm_count && p.stages > 8 && ((p.m + 127) / 128) * ((p.n + 127) / 128) <= ctx->sm_count)
+        return launch_one<128>(ctx, a, b, p, 1, stream);
     // Split k until a CTA has at most 8 stages, within those slots: joining the
-    // splits costs about 2 us, a stage 0.25 (1024 x 1024 x 8192, 32 stages: 11.2 us in
-    // two, 13.1 in one; 1024^3, 4 stages: 7.1 / 5.6).
+    // splits costs about 2 us, a stage 0.2 to 0.3 (1024 x 1024 x 8192, 32 stages: 11.2 us
+    // in two, 13.1 in one; 1024^3, 4 stages: 7.1 / 5.6).
     int splits = 1;
     while (splits < 8 && p.stages > 8 * splits && tiles * splits * 2 <= slots) splits *= 2;
     if (tn == 32) return launch_one<32>(ctx, a, b, p, splits, stream);

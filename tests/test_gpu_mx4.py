@@ -174,6 +174,12 @@ def test_product(gpu, m, n, k, dtype):
         assert torch.equal(buf[mask].isnan(), before[mask].isnan())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(2047, 1000, 2500), (500, 4096, 2081), (1500, 1400, 3200), (255, 8200, 2304), (129, 9401, 4097)])
+def test_product_over_a_long_axis(gpu, m, n, k, dtype):
+    test_product(gpu, m, n, k, dtype)
+
+
 def test_product_with_scales_far_apart(gpu):
     a, av = _operand(gpu, 70, 512, 1, wide=True)
     b, bv = _operand(gpu, 200, 512, 2, wide=True)
