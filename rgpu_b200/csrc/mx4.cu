@@ -22,8 +22,8 @@ __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return
 
 // A lane's piece of a row: 32 bytes, 16 bf16 or 8 f32.  V: bytes of an access, 32
 // (one 256-bit access, Blackwell's widest) or 16 where the rows are so aligned.
-// Else (0) a warp's accesses take neighbouring elements, which change hands through
-// its kilobyte of shared memory; an aligned row's last piece goes element by element.
+// Else (0) a warp's accesses take neighbouring words, which change hands through its
+// kilobyte of shared memory; an aligned row's last piece goes element by element.
 template <typename T>
 struct Piece {
     static constexpr int E = 32 / sizeof(T);         // elements
@@ -75,28 +75,71 @@ struct Piece {
                 }
         }
     }
-    // The warp's piece of an unaligned row of which `left` elements lie from p on; box:
-    // the warp's 1 KB.  p and left are the warp's, not the lane's.
-    __device__ __forceinline__ void load_any(const T* p, int64_t left, T* box, int lane) {
-        T v[E];
+    // The warp's piece of an unaligned row of which `left` elements lie from p on, p and
+    // left the warp's, not the lane's: read as words, then shared out through box, the
+    // warp's 1 KB.  bf16 whose row starts between two words: pairs from element 1 on, and
+    // element 0 by itself (`head`); a lane's words are then half a word off.
+    struct Words {
+        uint32_t v[8], head;
+    };
+    static __device__ __forceinline__ bool between(const T* p) { return sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(p) & 2); }
+    static __device__ __forceinline__ uint32_t half(const T* p) { return *reinterpret_cast<const unsigned short*>(p); }
+    static __device__ __forceinline__ Words fetch_any(const T* p, int64_t left, int lane) {
+        Words r;
+        constexpr int N = 4 / sizeof(T);  // elements of a word
+        const int odd = between(p);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(p + odd);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = e * 32 + lane < left ? p[e * 32 + lane] : T(0.0f);
+        for (int i = 0; i < 8; ++i) {
+            const int at = i * 32 + lane;
+            const int64_t room = left - odd - at * N;
+            r.v[i] = room >= N ? __ldg(words + at) : N == 2 && room == 1 ? half(p + odd + at * N) : 0u;
+        }
+        r.head = odd && lane == 0 && left > 0 ? half(p) << 16 : 0u;
+        return r;
+    }
+    __device__ __forceinline__ void deal_any(const Words& r, bool odd, uint32_t* box, int lane) {
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < E; ++e) box[e * 32 + lane] = v[e];
+        for (int i = 0; i < 8; ++i) box[i * 32 + lane] = r.v[i];
         __syncwarp();
         const uint4 a = reinterpret_cast<const uint4*>(box)[lane * 2], b = reinterpret_cast<const uint4*>(box)[lane * 2 + 1];
         w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
         w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-    }
-    __device__ __forceinline__ void store_any(T* p, int64_t left, T* box, int lane) const {
-        __syncwarp();
-        reinterpret_cast<uint4*>(box)[lane * 2] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<uint4*>(box)[lane * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
-        __syncwarp();
+        if (sizeof(T) == 2 && odd) {  // the same of the whole warp
+            uint32_t before = __shfl_up_sync(0xffffffffu, w[7], 1);
+            if (lane == 0) before = r.head;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (e * 32 + lane < left) p[e * 32 + lane] = box[e * 32 + lane];
+            for (int i = 7; i >= 0; --i) w[i] = __funnelshift_l(i ? w[i - 1] : before, w[i], 16);
+        }
+    }
+    __device__ __forceinline__ void store_any(T* p, int64_t left, uint32_t* box, int lane) const {
+        constexpr int N = 4 / sizeof(T);
+        const int odd = between(p);
+        uint32_t s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = w[i];
+        if (sizeof(T) == 2 && odd) {
+            const uint32_t after = __shfl_down_sync(0xffffffffu, w[0], 1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = __funnelshift_r(w[i], i < 7 ? w[i + 1] : after, 16);
+            if (lane == 0 && left > 0) *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
+        }
+        __syncwarp();
+        reinterpret_cast<uint4*>(box)[lane * 2] = make_uint4(s[0], s[1], s[2], s[3]);
+        reinterpret_cast<uint4*>(box)[lane * 2 + 1] = make_uint4(s[4], s[5], s[6], s[7]);
+        __syncwarp();
+        uint32_t* words = reinterpret_cast<uint32_t*>(p + odd);
+        const int64_t end = min(left, (int64_t)WARP) - odd;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = i * 32 + lane;
+            const int64_t room = end - at * N;
+            if (room >= N)
+                words[at] = box[at];
+            else if (N == 2 && room == 1)
+                *reinterpret_cast<unsigned short*>(words + at) = (unsigned short)box[at];
+        }
     }
     // Bit pattern (as f32) of the largest magnitude in the lane.
     __device__ __forceinline__ uint32_t amax() const {
@@ -158,12 +201,12 @@ __device__ __forceinline__ int64_t set_row(const Rows& w, int64_t set) {
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
+__global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
                                                                int64_t k, Rows w, int64_t blocks, int64_t groups,
                                                                uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales) {
     using P = Piece<T>;
-    __shared__ __align__(16) T boxes[V ? 1 : 8][P::WARP];
+    __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -175,12 +218,15 @@ __global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const T* __restri
             const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);  // rows of the set that there are
             const T* p = src + row * ld + j0;
             P x[4];
+            if constexpr (V == 0) {
+                typename P::Words r[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if constexpr (V == 0)
-                    x[q].load_any(p + q * (32 * ld), q < live ? k - j0 : 0, boxes[threadIdx.x >> 5], lane);
-                else
-                    x[q].template load<V>(p + q * (32 * ld) + lane * P::E, q < live ? k - j : 0);
+                for (int q = 0; q < 4; ++q) r[q] = P::fetch_any(p + q * (32 * ld), q < live ? k - j0 : 0, lane);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[q].deal_any(r[q], P::between(p + q * (32 * ld)), boxes[threadIdx.x >> 5], lane);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[q].template load<V>(p + q * (32 * ld) + lane * P::E, q < live ? k - j : 0);
             }
             uint32_t word[4];
             uint8_t* out = codes + row * row_bytes + (j >> 1);
@@ -309,7 +355,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
                                                          Rows w, int64_t blocks, int64_t groups, T* __restrict__ dst,
                                                          int64_t ld) {
     using P = Piece<T>;
-    __shared__ __align__(16) T boxes[V ? 1 : 8][P::WARP];
+    __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
