@@ -235,10 +235,10 @@ __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, ui
 // the MMA's M rows and TN tokens its N columns, so a CTA computes 128 columns of C
 // for TN tokens over its share of k.  The CTAs of a cluster share one tile, split
 // along k.  Their sums meet in shared memory and are added in rank order, tokens
-// dealt out over the CTAs.  One token by 8192 x 8192: 8.2 us in a stream of launches,
-// 5.4 of them the weights' 36 MB at the rate of a copy, the others the launch and the
-// join.  64 x 8192 x 4096: 7.0 us.  2047 x 1000 x 8192: 12.0 us, a stage 0.23 us for 35
-// KB, 19 TB/s from L2 to all SMs.
+// dealt out over the CTAs.  One token by 8192 x 8192: 9.6 us, 5.4 of them the
+// weights' 36 MB at the rate of a copy, the others the launch and the join (8.2 with
+// the weights in L2).  64 x 8192 x 4096: 7.0 us.  2047 x 1000 x 8192: 12.0 us, a stage
+// 0.23 us for 35 KB, 19 TB/s from L2 to all SMs.
 template <int TN>
 struct Geo1 {
     static constexpr int T_BYTES = TN * kRowBytes;
