@@ -342,7 +342,15 @@ class Norm:
     def __init__(self, kind: str = "rms", eps: float = 1e-5, gamma: GpuTensor | None = None,
                  beta: GpuTensor | None = None):
         self.kind, self.eps, self.gamma, self.beta = kind, eps, gamma, beta
-        self.args = NormArgs(_NORMS[kind], eps, _handle(gamma), _handle(beta))
+        self._args = NormArgs(_NORMS[kind], eps, _handle(gamma), _handle(beta))
+
+    @property
+    def args(self) -> NormArgs:
+        """What a call passes on: the handles that gamma and beta have now, for a
+        tensor may have been freed since."""
+        a = self._args
+        a.gamma, a.beta = _handle(self.gamma), _handle(self.beta)
+        return a
 
 
 _NO_NORM = NormArgs(RT_NORM_NONE, 0.0, None, None)
