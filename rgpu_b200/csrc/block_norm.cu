@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <initializer_list>
 
+#include "landing.cuh"
 #include "mx4.cuh"
 #include "tc_common.cuh"
 
@@ -800,17 +801,9 @@ __device__ __forceinline__ void gave_up(const RingP& r, volatile int* abort_flag
     tc::record_error(r.err, DEV_TIMEOUT_ROWS, (int)blockIdx.x);
     if (group >= 0) abort_flag[1 + group] = slot * 2 + (int)phase;
 }
-__device__ __noinline__ void land_copies(uint32_t full, int depth, int at) {
-    int slot = at >> 1;
-    uint32_t phase = at & 1;
+__device__ __noinline__ void land_copies(uint32_t full, int depth, int count, int at) {
     volatile int never = 0;
-    for (int d = 0; d < depth; ++d) {
-        tc::mbar_wait(full + slot * 8, phase, &never);
-        if (++slot == depth) {
-            slot = 0;
-            phase ^= 1;
-        }
-    }
+    land_ring(depth, count, at >> 1, at & 1, [&](int slot, uint32_t phase) { tc::mbar_wait(full + slot * 8, phase, &never); });
 }
 
 // Shared memory of a ring kernel: vectors, slots, sums, barriers.
@@ -1124,7 +1117,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
             phase ^= 1;
         }
     }
-    if (!ok && g.t == 0) land_copies(full, r.depth, abort_flag[1 + g.index]);
+    if (!ok && g.t == 0) land_copies(full, r.depth, r.depth, abort_flag[1 + g.index]);
 }
 
 // Backward.  Slots hold z and those of y, dz and dh that there are; vectors
@@ -1501,7 +1494,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
             phase ^= 1;
         }
     }
-    if (BULK && !ok && g.t == 0) land_copies(full, r.depth, abort_flag[1 + g.index]);
+    if (BULK && !ok && g.t == 0) land_copies(full, r.depth, r.depth, abort_flag[1 + g.index]);
     if (!q.partials) return;
     __syncthreads();  // the slots are all read
     float* acc = reinterpret_cast<float*>(sm.slots);
@@ -1700,8 +1693,9 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
         phase = next_phase;
     }
     if (!ok && g.t == 0) {
-        land_copies(full, depth, abort_flag[1 + g.index]);
-        land_copies(full_dz, depth, abort_flag[1 + g.index]);
+        // a wait for dz that gave up: z's ring is one use further, its slot already filled again
+        land_copies(full, depth, depth + 1, abort_flag[1 + g.index]);
+        land_copies(full_dz, depth, depth, abort_flag[1 + g.index]);
     }
     if (!q.partials) return;
     __syncthreads();  // the slots are all read
