@@ -14,6 +14,7 @@
 // k's blocks are not NaN, so they meet zero codes harmlessly.
 #include <algorithm>
 
+#include "landing.cuh"
 #include "mx4.cuh"
 #include "tc_common.cuh"
 
@@ -489,6 +490,10 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Counts bytes off a barrier of this CTA as a copy does that has landed.
+__device__ __forceinline__ void complete_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
@@ -592,9 +597,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     uint64_t* tfull = empty + S;  // each CTA: accumulator complete
     uint64_t* tempty = tfull + 1; // leader: accumulator drawn by both CTAs' epilogues
     uint64_t* drain = tempty + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* told = drain + 1;   // leader: the peer's number of stages is there
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(told + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* issued_all = abort_flag + 1;
+    volatile int* issued_all = abort_flag + 1;   // stages that this CTA issued, and
+    volatile int* issued_peer = issued_all + 1;  // (leader) its peer
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t rank = cta_rank();
@@ -609,6 +616,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         mbar_init(smem_u32(tfull), 1);
         mbar_init(smem_u32(tempty), 16);  // epilogue warps of both CTAs
         mbar_init(smem_u32(drain), 1);
+        mbar_init(smem_u32(told), 1);
         *abort_flag = 0;
         *issued_all = 0;
         fence_barrier_init();
@@ -666,6 +674,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         }
         if (elect_one()) {
             *issued_all = issued;
+            if (rank != 0) {
+                store_cluster(in_cta(smem_u32((const void*)issued_peer), 0), (uint32_t)issued);
+                arrive_cluster(in_cta(smem_u32(told), 0));
+            }
             if (!ok) raise_abort(DEV_TIMEOUT_PRODUCER);
         }
     } else if (warp == 1 && rank == 0) {
@@ -718,7 +730,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         if (elect_one()) {
             if (!ok) raise_abort(DEV_TIMEOUT_MMA);
             commit_pair(smem_u32(drain));
-            mbar_wait(smem_u32(drain), 0, abort_flag);
+            volatile int never = 0;  // a run that gave up waits for its MMAs too: they read both CTAs' memory
+            mbar_wait(smem_u32(drain), 0, &never);
         }
     } else if (warp >= 2) {
         const int quad = warp & 3, half = (warp - 2) >> 2;  // lanes, columns
@@ -775,9 +788,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     __syncwarp();
     __syncthreads();
     if (*abort_flag && rank == 0 && threadIdx.x == 0) {
-        // the pair's copies complete on the leader's barriers: wait for the last ones issued
+        // the pair's copies complete on the leader's barriers
         volatile int never = 0;
-        for (int i = max(0, *issued_all - S); i < *issued_all; ++i) mbar_wait(smem_u32(&full[i % S]), (i / S) & 1, &never);
+        const bool both = mbar_wait(smem_u32(told), 0, &never);
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        land_pair(
+            S, *issued_all, both ? *issued_peer : *issued_all,
+            [&](int slot) { mbar_expect_tx(smem_u32(&full[slot]), kPairStageBytes); },
+            [&](int slot) { complete_tx(smem_u32(&full[slot]), kPairStageBytes); },
+            [&](int slot, uint32_t phase) { mbar_wait(smem_u32(&full[slot]), phase, &never); });
     }
     tc_fence_before();
     __syncthreads();

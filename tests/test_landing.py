@@ -1,6 +1,7 @@
 """A kernel whose wait ran out waits for the copies that it still has on their way.
 The rules of csrc/landing.cuh are held, on the host, to every order of issue and
-every place to give up that the ring kernels have; how the kernels call them is read from their source.  Nothing here runs on a GPU."""
+every place to give up that the ring kernels and the two-CTA product have; how
+the kernels call them is read from their source.  Nothing here runs on a GPU."""
 import os
 import re
 import subprocess
@@ -88,6 +89,31 @@ int two_rings(int depth, int rows, int stop, int count, int count_dz) {
     return full.left() + dz.left();
 }
 
+// mx4_pair_kernel: a leader that issued `own` stages and a peer that issued `peer`; every
+// copy lands.  Bytes count in halves of a stage.
+int pair(int slots, int own, int peer) {
+    const int last = own > peer ? own : peer;
+    std::vector<int> arrived(last), bytes(last), waited(last);
+    for (int i = 0; i < last; ++i) {
+        if (i < own) ++arrived[i], bytes[i] += 2 - 1;  // announces both halves, brings its own
+        if (i < peer) bytes[i] -= 1;
+    }
+    std::vector<int> phase(slots);  // of each barrier: the first stage not known to be complete
+    auto current = [&](int slot) { return slot + phase[slot] * slots; };
+    for (int s = 0; s < slots; ++s)
+        while (current(s) < last - slots) ++phase[s];  // read by the MMAs, so complete
+    rt::land_pair(slots, own, peer, [&](int s) { ++arrived[current(s)], bytes[current(s)] += 1; },
+                  [&](int s) { bytes[current(s)] -= 1; },
+                  [&](int s, unsigned p) {
+                      const int i = current(s);
+                      if ((unsigned)(phase[s] & 1) != p) return;
+                      if (arrived[i] == 1 && bytes[i] == 0) ++waited[i], ++phase[s];
+                  });
+    int left = 0;
+    for (int i = last > slots ? last - slots : 0; i < last; ++i) left += waited[i] != 1;
+    return left;
+}
+
 int main(int, char** v) {
     const int extra = atoi(v[1]), extra_dz = atoi(v[2]);
     int bad = 0;
@@ -97,6 +123,9 @@ int main(int, char** v) {
                 bad += one_ring(depth, rows, stop, depth) != 0;
                 if (depth >= 2 && rows) bad += two_rings(depth, rows, stop, depth + extra, depth + extra_dz) != 0;
             }
+    for (int slots : {4, 6})
+        for (int own = 0; own < 25; ++own)
+            for (int peer = own > slots ? own - slots : 0; peer <= own + slots; ++peer) bad += pair(slots, own, peer) != 0;
     printf("%d\n", bad);
 }
 """
@@ -132,3 +161,15 @@ def test_every_copy_of_a_run_that_gave_up_is_waited_for(check):
     for kernel in ("forward_ring_kernel", "backward_ring_kernel"):
         (count,) = re.findall(r"land_copies\(full, r\.depth, ([^,]+),", _body("block_norm.cu", kernel))
         assert _count(count) == 0
+
+
+@pytest.mark.parametrize("kernel,barriers", [("mx4_kernel", ["done"]), ("mx4_pair_kernel", ["drain", "told"])])
+def test_a_product_that_gave_up_waits_for_its_mmas_and_copies(kernel, barriers):
+    body = _body("gemm_mx4.cu", kernel)
+    for barrier in barriers:  # by a flag that nothing sets: the abort flag would end the wait at once
+        flags = re.findall(r"mbar_wait\(smem_u32\(" + barrier + r"\), 0, ([^)]+)\)", body)
+        assert flags and flags[-1] == "&never", (barrier, flags)
+    assert body.rindex("&never") < body.rindex("tcgen05.dealloc")
+    if kernel == "mx4_pair_kernel":
+        assert "abort_flag" not in re.findall(r"mbar_wait\(smem_u32\(drain\), 0, ([^)]+)\)", body)
+        assert re.search(r"land_pair\(\s*S, \*issued_all, both \? \*issued_peer : \*issued_all", body)
