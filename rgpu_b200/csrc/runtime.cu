@@ -21,6 +21,9 @@ int fail(int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     g_last_error = buf;
+    // The runtime also keeps the error of a call that failed, for the next cudaGetLastError of this
+    // thread: taken here, or the launch that asks next would be refused for it.
+    if (code == RT_ERR_CUDA || code == RT_ERR_OOM) cudaGetLastError();
     return code;
 }
 
