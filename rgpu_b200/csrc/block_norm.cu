@@ -2202,7 +2202,13 @@ int rt_block_backward(rt_ctx* ctx, const rt_block_args* a, const rt_block_grads*
     }
     q.sums = (g->dgamma_post || gate_sums ? 1 : 0) | (g->dbeta_post || (gate_sums && p.post.beta) ? 2 : 0) |
              (g->dgamma_pre ? 4 : 0) | (g->dbeta_pre ? 8 : 0);
-    if (p.n == 0) return RT_OK;
+    if (p.n == 0) {  // sums over no columns
+        if (g->dgate && p.m > 0 && (p.gate_mode == GATE_ONE || p.gate_mode == GATE_COLUMN)) {
+            RT_CUDA(cudaSetDevice(ctx->device));
+            RT_CUDA(cudaMemset2DAsync(g->dgate->ptr, (size_t)g->dgate->ld * 4, 0, 4, (size_t)g->dgate->rows, ctx->stream));
+        }
+        return RT_OK;
+    }
     int parts = parts_for(ctx, p.m);
     if (q.sums) {
         RT_CHECK(g->work && g->work->dtype == RT_F32 && g->work->rows == 1 &&
