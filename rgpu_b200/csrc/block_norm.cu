@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(kWide) backward_kernel(BlockP p, GradP g) {
             if (g.dz) row4<T>(g.dz, row * g.lddz, base, n, dr);
             if (!g.dh) return;
             row4<T>(g.dh, row * g.lddh, base, n, d);
-            z4(base, hat);
+            // without a norm z has no part in dr: an infinity in it would be a NaN times a1 = 0
+            if (p.pre.kind != RT_NORM_NONE) z4(base, hat);
             vector4(p.pre.gamma, 1.0f, base, n, gamma);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -276,6 +277,7 @@ __global__ void __launch_bounds__(kWide) backward_kernel(BlockP p, GradP g) {
             }
         };
         float b0 = 0.0f, b1 = 0.0f;
+        const bool normed = p.post.kind != RT_NORM_NONE;  // else y has no part in dy
         if (p.y) {
             float gsum = 0.0f;
             for (int64_t base = 0; base < n; base += 4 * kWide) {
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kWide) backward_kernel(BlockP p, GradP g) {
                 if (j >= n) continue;
                 if (p.y) {
                     const float dt = p.scale * dr[i], yh = (y[i] - sy.mu) * sy.rho, b = dt * gate[i] * gamma[i];
-                    if (g.dy) st<T>(g.dy, row * g.lddy + j, (b - b0 - yh * b1) * sy.rho);
+                    if (g.dy) st<T>(g.dy, row * g.lddy + j, (b - b0 - (normed ? yh : 0.0f) * b1) * sy.rho);
                     if (g.dgate && p.gate_mode == GATE_FULL)
                         st<T>(g.dgate, row * g.lddg + j, dt * (yh * gamma[i] + beta[i]));
                     const float w = own_gate ? dr[i] * gate[i] : dr[i];
@@ -1385,7 +1387,9 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                 f2 d[4], h[4];
                 const f2 rho = splat2(sz.rho), less_a0 = splat2(-a0), less_a1 = splat2(-a1);
                 slot8<T>(at + at_dh, j[c], d);
-                slot8<T>(at, j[c], h);
+                // without a norm z has no part in dr: an infinity in it would be a NaN times a1 = 0
+                if (back) slot8<T>(at, j[c], h);
+                else h[0] = h[1] = h[2] = h[3] = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     h[i] = mul2(FULL ? add2(h[i], less_z) : h[i], rho);
@@ -1453,6 +1457,13 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                 sums[1] = fma2(b[c][i], hat[c][i], sums[1]);
             }
         }
+        // likewise y, which has no part in dy without a norm
+        const bool normed = p.post.kind != RT_NORM_NONE;
+        if (!normed)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) hat[c][i] = 0;
         float b0 = 0.0f, b1 = both(sums[1]);
         if (!p.y) {
             g.sync();
@@ -1468,7 +1479,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
         // every thread of the group has read the slot: all of it before the last barrier
         if (BULK && g.t == 0 && ok && row + r.depth * step < p.m) issue(row + r.depth * step, slot);
         if (q.dy) {
-            const f2 rho = splat2(sy.rho), add = splat2(b0), less_b1 = splat2(p.post.kind != RT_NORM_NONE ? -b1 * inv_n : 0.0f);
+            const f2 rho = splat2(sy.rho), add = splat2(b0), less_b1 = splat2(normed ? -b1 * inv_n : 0.0f);
 #pragma unroll
             for (int c = 0; c < C; ++c)
                 if (has[c]) {
