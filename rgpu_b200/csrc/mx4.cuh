@@ -28,11 +28,6 @@ __device__ __forceinline__ float inv_scale(uint32_t byte) {
     return __uint_as_float((byte == kNanScale ? 0u : 254u - byte) << 23);
 }
 
-// 2^(byte - 127); byte 0 is the subnormal 2^-127, byte 255 NaN.
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-    return __uint_as_float(byte == 0 ? 0x00400000u : byte == kNanScale ? 0x7fc00000u : byte << 23);
-}
-
 // Two elements to E2M1 codes in one byte (lo in bits 0-3): round to nearest,
 // ties to even, magnitudes above 6 to 6.
 __device__ __forceinline__ uint32_t encode2(float lo, float hi) {
