@@ -302,10 +302,12 @@ int rt_block_forward(rt_ctx* ctx, const rt_block_args* args);
 /* The gradients of the above.  args is the forward call's, with z as it was
  * stored (y = NULL: z may be NULL, r is read); its r, h and hq are not read
  * otherwise.
- *   dz, dh  gradients of z and h, of y's type; NULL is zeros
+ *   dz, dh  gradients of z and h, of y's type; NULL is zeros (of one of them at
+ *           most, and dgamma_pre and dbeta_pre want dh)
  *   dr, dy  gradients of r and y, of y's type; dr may be dz itself
  *   dgamma_*, dbeta_*  [1,n] f32; dgate the gate's shape and type
- * A NULL output is not stored.  work: rt_block_backward_workspace(m, n) f32.
+ * A NULL output is not stored.  work: rt_block_backward_workspace(m, n) f32,
+ * needed for the dgamma, the dbeta and the dgate of a [1,1] or [1,n] gate.
  * Sums over rows are taken in a fixed order: results do not change from run
  * to run on one kind of device. */
 typedef struct {

@@ -491,7 +491,7 @@ __device__ __forceinline__ void store_h(const BlockP& p, int64_t row, int j, boo
 // in each of C turns, so y and r are read once, z and h written once and the
 // sums of a norm are taken twice over the same registers (mean, then the centred
 // squares).  HBM-bound: 4 elements moved for each of the row; few rows are bound by
-// the launch (one of 8192 bf16: 4.3 us in a stream of launches).  Needs 16-byte
+// the launch (one of 8192 bf16: 4 to 5 us in a stream of launches).  Needs 16-byte
 // aligned rows and whole eights (n % 8 = 0); a CTA holds ROWS = max(1, 128 / TPR)
 // rows.
 constexpr int cta_threads(int tpr) { return tpr < 128 ? 128 : tpr; }
@@ -912,7 +912,7 @@ __device__ __forceinline__ float shared_gate(const BlockP& p, int j) {
 
 // Forward.  Slots hold r and y; vectors P = s g gamma_post, Q = s g beta_post (g
 // where all rows share it), gamma_pre, beta_pre, those that there are (mask 1 2 4
-// 8).  8192 x 8192 bf16, RMS norms and a gate: 95 us and 5.7 TB/s, HBM-bound (a
+// 8).  8192 x 8192 bf16, RMS norms and a gate: 94 to 101 us, 5.3 to 5.7 TB/s, HBM-bound (a
 // device copy reaches 6.55); forward_rows_kernel, whose reads wait behind each row's
 // sums, took 241.
 // FULL: with layer norms, betas and gates that rows do not share; else RMS norms
@@ -1161,7 +1161,7 @@ __device__ __forceinline__ void join_sums(const G& g, const GradP& q, float* acc
 }
 
 // C: eights of a thread.  With the betas' sums a thread of sixteen columns spills
-// (and with all of shared memory taken, spills go to L2), so FULL takes eight: 2047 x 1000 f32 layer norms, full gate: 26 us with the sums
+// (and with all of shared memory taken, spills go to L2), so FULL takes eight: 2047 x 1000 f32 layer norms, full gate: 26 to 29 us with the sums
 // over columns behind it, 15 more with C = 2; bound by the latency of a row's barriers
 // among 16 warps (3.5 rows a group).
 //
@@ -1523,8 +1523,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
 // dr is computed and summed against y^ its successor's three sums are taken, and
 // all four are joined at once.  z, y and dh of a row are read into registers when
 // its sums are taken and their slots are then free; dz has slots of its own.
-// 8192 x 8192: 132 us and 6.1 TB/s with 10 us of column_kernel behind them; the
-// kernel above, whose barriers come one after another, took 195 in all.
+// 8192 x 8192: 143 to 156 us, 10 of them column_kernel; the kernel above, whose
+// barriers come one after another, took 195.
 template <int TPR, int CL>
 __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p, GradP q, RingP r) {
     using T = __nv_bfloat16;
@@ -1993,11 +1993,11 @@ int ring_clusters(rt_ctx* ctx, int cluster, int* count) {
 
 // The backward pass through the ring, up to 16384 wide.  *parts is then the number of
 // partials.  A CTA takes 8192 columns, 4096 with all features (which want registers):
-// wider rows are shared by a cluster.  1000 x 16384 bf16 RMS 61 us so, layer norms with
-// a full gate 164, against 301 and 416 by the kernel for any width; 4096 x 4099 with
-// all features 423 against 540 by one CTA whose threads spill.  Unaligned rows up to
+// wider rows are shared by a cluster.  1000 x 16384 bf16 RMS 61 to 69 us so, layer norms with
+// a full gate 164 to 173, against 301 and 416 by the kernel for any width; 4096 x 4099 with
+// all features 403 to 423 against 540 by one CTA whose threads spill.  Unaligned rows up to
 // 4096 wide take the full kernel without its features: eight columns a thread, 4000 x
-// 1001 37 us.
+// 1001 bf16 RMS 32 to 37 us.
 template <typename T>
 int backward_ring(rt_ctx* ctx, const BlockP& p, const GradP& q, cudaStream_t st, int* parts, bool* done) {
     *done = false;

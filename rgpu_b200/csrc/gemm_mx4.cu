@@ -238,8 +238,8 @@ __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, ui
 // along k.  Their sums meet in shared memory and are added in rank order, tokens
 // dealt out over the CTAs.  One token by 8192 x 8192: 9.6 us, 5.4 of them the
 // weights' 36 MB at the rate of a copy, the others the launch and the join (8.2 with
-// the weights in L2).  64 x 8192 x 4096: 7.0 us.  2047 x 1000 x 8192: 12.0 us, a stage
-// 0.23 us for 35 KB, 19 TB/s from L2 to all SMs.
+// the weights in L2).  64 x 8192 x 4096: 6.9 to 7.1 us.  2047 x 1000 x 8192: 12.3 to 12.7 us,
+// a stage 0.23 us for 35 KB, 19 TB/s from L2 to all SMs.
 template <int TN>
 struct Geo1 {
     static constexpr int T_BYTES = TN * kRowBytes;
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 // while this one's epilogue stores.
 //
 // 8192^3, bf16 out: 184 us for a single launch, the tensor pipe 84 % busy; launched
-// again and again 194 to 220 us, the clock held down by the 1 kW power limit (154 us
+// again and again 183 to 220 us, the clock held down by the 1 kW power limit (154 us
 // on matrices of zeros, which draw less).
 constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of T and W, two tiles of T's scales, four of W's
@@ -522,8 +522,9 @@ __device__ __forceinline__ void transpose32(float (&v)[32], int lane) {
 }
 
 // 32 rows of 128 columns of C whose rows are not 16-byte aligned: lanes and
-// columns change places, so that a warp's 2- or 4-byte stores are neighbours.  c: the
-// first row's; rows, left: how many rows and columns there are from it on.
+// columns change places, so that a warp's 2- or 4-byte stores are neighbours.  The 128
+// accumulators and the exchange do not fit 168 registers (some spill): 4096 x 4097 x
+// 1024 bf16 36 us, where 4096 columns, aligned, take 18.  c: the first row's; rows, left: how many rows and columns there are from it on.
 template <typename T>
 __device__ __forceinline__ void store_columns(T* c, int64_t ldc, int64_t rows, int64_t left, const float* bias,
                                               float floor, int lane, float (&v)[4][32]) {
@@ -954,20 +955,23 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
         return RT_OK;
     }
     // One-CTA tiles while they fit the device at once, two of 64 tokens to an SM (256 x
-    // 8192 x 2048: 7.1 us against 9.2 with pairs), else pairs, which load half as much
-    // per MMA (1024 x 4096 x 1024: 8.6 / 11.5; 2048^3: 9.8 / 13.9).  Where most SMs would
+    // 8192 x 2048: 7.3 us against 8.4 with pairs), else pairs, which load half as much
+    // per MMA (1024 x 4096 x 1024: 7.5 / 11.2; 2048^3: 8.7 / 13.6).  Where most SMs would
     // hold two, one of 128 tokens reads two thirds of the bytes, but has more to do after
-    // its last stage: 2047 x 1000 x 8192, 32 stages, 12.0 us / 13.7; 512 x 4096 x 4096, 16
-    // stages, 8.2 / 9.1; 256 x 8192 x 2048, 8 stages, 6.9 / 6.9; 2048 x 1024 x 1024, 4
-    // stages, 6.1 / 5.6.
+    // its last stage: 2047 x 1000 x 8192, 32 stages, 12.3 us / 14.3; 512 x 4096 x 4096, 16
+    // stages, 8.6 / 9.5; 256 x 8192 x 2048, 8 stages, 7.1 / 7.3; 2048 x 1024 x 1024, 4
+    // stages, 6.2 / 5.8.
     const int tn = p.m <= 32 ? 32 : 64;
     const int64_t tiles = ((p.m + tn - 1) / tn) * ((p.n + 127) / 128), slots = 2 * (int64_t)ctx->sm_count;
     if (tiles > slots) return launch_pair(ctx, a, b, p, stream);
     if (tiles > ctx->sm_count && p.stages > 8 && ((p.m + 127) / 128) * ((p.n + 127) / 128) <= ctx->sm_count)
         return launch_one<128>(ctx, a, b, p, 1, stream);
-    // Split k until a CTA has at most 8 stages, within those slots: joining the
-    // splits costs about 2 us, a stage 0.2 to 0.3 (1024 x 1024 x 8192, 32 stages: 11.2 us
-    // in two, 13.1 in one; 1024^3, 4 stages: 7.1 / 5.6).
+    // Split k until a CTA has at most 8 stages, within those slots: joining the splits costs
+    // about 2 us, and few tiles leave most SMs without work (16 x 1024 x 8192, 32 stages on 8
+    // tiles: 5.9 us in four, 8.4 in one; 64 x 1000 x 8192: 7.3 / 9.7; 1024^3, 4 stages: 6.6 in
+    // two, 4.9 in one).  With 64 tiles and more fewer splits would do (1 x 8192 x 8192: 8.2 in
+    // four, 7.3 in two; 1024 x 1024 x 8192: 11.1 in two, 10.3 in one; both with the operands in
+    // L2).
     int splits = 1;
     while (splits < 8 && p.stages > 8 * splits && tiles * splits * 2 <= slots) splits *= 2;
     if (tn == 32) return launch_one<32>(ctx, a, b, p, splits, stream);
