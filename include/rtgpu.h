@@ -270,6 +270,78 @@ int rt_mx4_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst);
  *   dW = X^T dY  A = X axis 0,  B = dY axis 0 */
 int rt_mx4_matmul(rt_ctx* ctx, const rt_mx4* a, const rt_mx4* b, rt_tensor* c, const rt_tensor* bias, int relu);
 
+/* ------------------------------------------- block-scaled 8-bit matrices */
+/* No counterpart in the reference.  A matrix [rows, k] in 8-bit floating point
+ * (E4M3: largest 448, no infinities) with one E8M0 scale (as above) for each
+ * block of 128 elements along k.  Device layout:
+ *   codes   rows of ceil(k/16) * 16 bytes, one element to a byte; what the
+ *           bytes past k hold does not matter
+ *   scales  tiles of 128 rows by 4 blocks, 512 bytes each, in the order of a
+ *           4-bit matrix's; those of blocks and rows past the last may hold
+ *           anything. */
+typedef struct rt_fp8 rt_fp8;
+/* rows x k zeros (rows, k >= 0). */
+int rt_fp8_zeros(rt_ctx* ctx, int64_t rows, int64_t k, rt_fp8** out);
+/* Non-owning view of caller memory in the layout above: codes of
+ * rt_fp8_code_bytes bytes, scales of rt_fp8_scale_bytes bytes, both 16-byte
+ * aligned. */
+int rt_fp8_wrap(rt_ctx* ctx, void* codes, void* scales, int64_t rows, int64_t k, rt_fp8** out);
+int rt_fp8_free(rt_fp8* q);
+int rt_fp8_dims(const rt_fp8* q, int64_t* rows, int64_t* k);
+void* rt_fp8_codes(const rt_fp8* q);
+void* rt_fp8_scales(const rt_fp8* q);
+/* Bytes of the codes and of the scales of a rows x k matrix (-1: bad extents). */
+int64_t rt_fp8_code_bytes(int64_t rows, int64_t k);
+int64_t rt_fp8_scale_bytes(int64_t rows, int64_t k);
+/* dst = src (f32 or bf16) in 8 bits; axes as in rt_mx4_quantize.  A block's scale
+ * is the least 2^e, e >= -127, with max|x| <= 448 * 2^e, so nothing saturates;
+ * elements are rounded to nearest, ties to even.  A block that holds a NaN or
+ * an infinity gets the NaN scale. */
+int rt_fp8_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_fp8* dst);
+/* dst [rows, k] (f32 or bf16) = the values q stands for. */
+int rt_fp8_dequantize(rt_ctx* ctx, const rt_fp8* q, rt_tensor* dst);
+/* C[m,n] = A[m,k] B[n,k]^T + 1 bias, ReLU if relu != 0, as rt_mx4_matmul: all
+ * three products of a Dense layer take this form. */
+int rt_fp8_matmul(rt_ctx* ctx, const rt_fp8* a, const rt_fp8* b, rt_tensor* c, const rt_tensor* bias, int relu);
+
+/* ------------------------------------------------------------- embedding */
+/* No counterpart in the reference.  y[i,:] = scale * table[tokens[i],:].
+ * tokens: u32, as many as y has rows; one that is no row of the table (>=
+ * its rows) is padding and gives a row of zeros.  table and y are f32 or bf16
+ * each. */
+int rt_embedding_forward(rt_ctx* ctx, const rt_tensor* table, const rt_tensor* tokens, float scale, rt_tensor* y);
+/* Its gradient: dtable[v,:] = scale * sum over i with tokens[i] = v of dy[i,:],
+ * every row of it (accumulate != 0: added to the rows that occur, the others
+ * as they were).  dtable [vocabulary, n] f32, dy [count, n] f32 or bf16.  work:
+ * rt_embedding_backward_workspace packed f32.  The positions are sorted by
+ * token and summed in a fixed order: results do not change from run to run.
+ * At most 2^21 - 1 rows of dtable, 2^31 - 1 tokens. */
+int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, float scale, int accumulate,
+                          rt_tensor* dtable, rt_tensor* work);
+/* f32 elements of work for `count` tokens (-1: bad extents). */
+int64_t rt_embedding_backward_workspace(int64_t count, int64_t vocabulary, int64_t n);
+
+/* --------------------------------------------------------------- dropout */
+/* No counterpart in the reference.  Which elements are dropped is a function of
+ * seed, site, step, row and column alone and is stored nowhere.  p is taken to
+ * the nearest 2^-16, q; element (i, j) is kept where
+ *   bits16[j % 8] >= q * 2^16,  the eight 16-bit words (low half first) of
+ *   Philox4x32-10(key (seed, seed >> 32), counter (j / 8, first_row + i, step, site)). */
+typedef struct {
+    double p;                 /* in [0, 1]; 1 drops everything */
+    uint64_t seed;
+    uint32_t site;            /* which dropout of a model */
+    uint32_t step;            /* which step of a training run */
+    const rt_tensor* step_at; /* one u32 on the device, read when the kernel runs and added to step
+                                 (a captured step can count by itself); may be NULL */
+    int64_t first_row;        /* row number of x's first row (of a global batch); rows end by 2^32 */
+} rt_dropout_mask;
+/* y = add + keep . x / (1 - q); add may be NULL (zeros), y may be x or add; all
+ * of one type, f32 or bf16.  The gradient of x is the same call with x = dy,
+ * add = NULL; that of add is dy.  A dropped element of x is not looked at: a
+ * NaN there does not come through. */
+int rt_dropout(rt_ctx* ctx, const rt_tensor* x, const rt_tensor* add, rt_tensor* y, const rt_dropout_mask* mask);
+
 /* ------------------------------------------------ residual-block norms */
 /* No counterpart in the reference.  The row-wise work between two blocks of a
  * residual stream r [m,n], in one pass:

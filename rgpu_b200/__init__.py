@@ -6,6 +6,8 @@ benchmark.  See ``rgpu_b200.gpu``.
 """
 from .gpu import (  # noqa: F401
     Comm,
+    Dropout,
+    Fp8Tensor,
     Gpu,
     GpuMlp,
     GpuTensor,
@@ -18,8 +20,8 @@ from .gpu import (  # noqa: F401
     upload_labels,
 )
 
-__all__ = ["Comm", "Gpu", "GpuMlp", "GpuTensor", "Mx4Tensor", "Norm", "RtError", "bf16_to_f32", "f32_to_bf16", "lib",
-           "upload_labels"]
+__all__ = ["Comm", "Dropout", "Fp8Tensor", "Gpu", "GpuMlp", "GpuTensor", "Mx4Tensor", "Norm", "RtError", "bf16_to_f32",
+           "f32_to_bf16", "lib", "upload_labels"]
 
 
 def build(verbose: bool = False) -> str:

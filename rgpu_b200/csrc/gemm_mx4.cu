@@ -1,17 +1,20 @@
-// Product of two microscaled 4-bit matrices on the tensor cores,
-// C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU): tcgen05.mma kind::mxf4 with one
-// E8M0 scale per 32 elements, f32 accumulators in TMEM.
+// Product of two block-scaled matrices on the tensor cores, C[m,n] = A[m,k] B[n,k]^T +
+// 1 bias (+ ReLU), f32 accumulators in TMEM: microscaled 4-bit matrices (E2M1, an E8M0
+// scale per 32 elements, tcgen05.mma kind::mxf4) and 8-bit ones (E4M3, an E8M0 scale per
+// 128, kind::mxf8f6f4).  The formats share the kernels: a row is as many bytes a
+// stage, only the scales' places differ.
 //
 // A's rows are called tokens here, T; B's rows are C's columns, W.
 //
-// A k stage is 256 elements: 128 bytes of codes per row (one 128-byte-swizzled
-// TMA box) and two 512-byte scale tiles per 128 rows, in memory already in the
+// A k stage is 128 bytes of codes per row (256 elements in 4 bits, 128 in 8; one
+// 128-byte-swizzled TMA box) and its 512-byte scale tiles per 128 rows (two; one), in
+// memory already in the
 // order that tcgen05.cp spreads over TMEM (32 lanes x 4 columns, repeated in the
 // four lane quadrants).  Each shared-memory stage has TMEM columns for its scales
 // of its own, so the barrier that frees a stage frees its scales too.  A stage is
-// four MMAs of 64 elements, two scales a row each.  Boxes past the matrices read
-// zeros; MMAs wholly past k are not issued, and the last scale tile's bytes past
-// k's blocks are not NaN, so they meet zero codes harmlessly.
+// four MMAs of 32 bytes a row.  Boxes past the matrices read
+// zeros; MMAs wholly past k are not issued.  In 4 bits an MMA's second scale may lie
+// past k's blocks: such bytes are not NaN, so they meet zero codes harmlessly.
 #include <algorithm>
 
 #include "landing.cuh"
@@ -23,16 +26,15 @@ namespace {
 
 using namespace tc;
 
-constexpr int kStageK = 256;          // elements of k in a stage
-constexpr int kStageBlocks = kStageK / 32;
 constexpr int kRowBytes = 128;        // codes of a row in a stage
+constexpr int kStageSteps = 4;        // MMAs of a stage, 32 bytes of codes each
 constexpr int kWBytes = 128 * kRowBytes;
 constexpr int kScaleTile = 512;       // scales of 128 rows x 4 blocks
 
 struct Mx4Params {
     int64_t m, n;                     // C's extents
     int tiles_m, tiles_n;             // token tiles, column tiles
-    int blocks;                       // blocks of 32 along k
+    int steps;                        // MMAs along k
     int stages, stages_per_split;     // k stages in all, and of one split
     void* c;
     int64_t ldc;
@@ -43,36 +45,65 @@ struct Mx4Params {
     int* err;
 };
 
-// kind::mxf4 instruction descriptor: E2M1 operands, both K-major, E8M0 scales;
-// `half` selects the scale bytes 0-1 or 2-3 of each TMEM word for A and B.
-__host__ __device__ constexpr uint32_t mx4_idesc(int m, int n, int half) {
-    return (1u << 7)                         // A: E2M1
-           | (1u << 10)                      // B: E2M1
-           | ((uint32_t)(n >> 3) << 17)      // N / 8
-           | (1u << 23)                      // scales: E8M0
-           | ((uint32_t)(m >> 7) << 27)      // M / 128
-           | ((uint32_t)(half * 2) << 29)    // A's scale bytes
-           | ((uint32_t)(half * 2) << 4);    // B's scale bytes
-}
+// The two formats.  GROUPS: scale tiles of 128 rows that a stage needs; scale_group: the
+// first of them along k; idesc: instruction descriptor of the stage's kk-th MMA (both
+// operands K-major, E8M0 scales; bits 29 and 4 the first scale byte of each TMEM word for
+// A and B), tile: the scale tile that it reads.
 
-template <int CG>
-__device__ __forceinline__ void mma_mx4(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
-                                        uint32_t sfb, uint32_t accumulate) {
-    if constexpr (CG == 1)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-            "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-            : "memory");
+// kind::mxf4: E2M1 operands, 64 elements an MMA, two scales a row.
+struct Mx4 {
+    using Matrix = rt_mx4;
+    static constexpr int GROUPS = 2;
+    static int steps(const rt_mx4& q) { return (int)((q.blocks() + 1) / 2); }
+    static __device__ __forceinline__ int scale_group(int stage) { return stage * 2; }
+    static __device__ __forceinline__ constexpr int tile(int kk) { return kk >> 1; }
+    static __device__ __forceinline__ constexpr uint32_t idesc(int m, int n, int kk, int /*stage*/) {
+        return (1u << 7) | (1u << 10)            // A, B: E2M1
+               | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27)
+               | ((uint32_t)((kk & 1) * 2) << 29) | ((uint32_t)((kk & 1) * 2) << 4);
+    }
+};
+
+// kind::mxf8f6f4: E4M3 operands, 32 elements an MMA, one scale a row.  The instruction
+// takes a scale for every 32 elements; a block of 128 is one stage, whose four MMAs read
+// the same byte, so a scale tile (four blocks) serves four stages and nothing is
+// repeated in memory.  Each stage loads its tile again all the same: 512 bytes beside 16
+// KB of codes.
+struct Fp8 {
+    using Matrix = rt_fp8;
+    static constexpr int GROUPS = 1;
+    static int steps(const rt_fp8& q) { return (int)((q.k + 31) / 32); }
+    static __device__ __forceinline__ int scale_group(int stage) { return stage >> 2; }
+    static __device__ __forceinline__ constexpr int tile(int) { return 0; }
+    static __device__ __forceinline__ constexpr uint32_t idesc(int m, int n, int /*kk*/, int stage) {
+        return ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27)
+               | ((uint32_t)(stage & 3) << 29) | ((uint32_t)(stage & 3) << 4);
+    }
+};
+
+#define RT_SCALED_MMA(CG, KIND)                                                                                        \
+    asm volatile("{\n\t.reg .pred p;\n\t"                                                                             \
+                 "setp.ne.b32 p, %6, 0;\n\t"                                                                           \
+                 "tcgen05.mma.cta_group::" CG ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),        \
+                 "l"(ad), "l"(bd), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                     \
+                 : "memory")
+
+template <typename F, int CG>
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
+                                           uint32_t sfb, uint32_t accumulate) {
+    if constexpr (F::GROUPS == 2) {
+        if constexpr (CG == 1)
+            RT_SCALED_MMA("1", "mxf4.block_scale.scale_vec::2X");
+        else
+            RT_SCALED_MMA("2", "mxf4.block_scale.scale_vec::2X");
+    } else {
+        if constexpr (CG == 1)
+            RT_SCALED_MMA("1", "mxf8f6f4.block_scale.scale_vec::1X");
+        else
+            RT_SCALED_MMA("2", "mxf8f6f4.block_scale.scale_vec::1X");
+    }
 }
+#undef RT_SCALED_MMA
 
 // Descriptor of a scale tile in shared memory: no swizzle, 8-row groups of
 // 16-byte rows 128 bytes apart.
@@ -240,10 +271,11 @@ __device__ __forceinline__ void add_splits(const Mx4Params& p, uint32_t sums, ui
 // weights' 36 MB at the rate of a copy, the others the launch and the join (8.2 with
 // the weights in L2).  64 x 8192 x 4096: 6.9 to 7.1 us.  2047 x 1000 x 8192: 12.3 to 12.7 us,
 // a stage 0.23 us for 35 KB, 19 TB/s from L2 to all SMs.
-template <int TN>
+template <typename F, int TN>
 struct Geo1 {
     static constexpr int T_BYTES = TN * kRowBytes;
-    static constexpr int STAGE_BYTES = kWBytes + T_BYTES + 4 * kScaleTile;  // codes, two scale tiles of either side
+    static constexpr int S_BYTES = 2 * F::GROUPS * kScaleTile;
+    static constexpr int STAGE_BYTES = kWBytes + T_BYTES + S_BYTES;  // codes, scale tiles of either side
     static constexpr int CTAS = TN > 64 ? 1 : 2;  // to an SM
     static constexpr int STAGES = CTAS > 1 ? 4 : 6;
     static constexpr int TMEM_COLS = 512 / CTAS;  // two accumulators of TN, and 16 of scales a stage
@@ -255,18 +287,19 @@ struct Geo1 {
 
 constexpr int kThreads1 = 224;  // warps: 0 TMA, 1 MMA, 2-5 epilogue (one TMEM lane quadrant each), 6 MMA
 
-template <int TN>
+template <typename F, int TN>
 __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ CUtensorMap map_w,
                                                         const __grid_constant__ CUtensorMap map_t,
                                                         const __grid_constant__ CUtensorMap map_sw,
                                                         const __grid_constant__ CUtensorMap map_st, Mx4Params p) {
-    using G = Geo1<TN>;
+    using G = Geo1<F, TN>;
+    constexpr int NG = F::GROUPS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* smem_w = smem;
     uint8_t* smem_t = smem + G::STAGES * kWBytes;
-    uint8_t* smem_s = smem_t + G::STAGES * G::T_BYTES;  // [stage][W 2 tiles, T 2 tiles]
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem_s + G::STAGES * 4 * kScaleTile);
+    uint8_t* smem_s = smem_t + G::STAGES * G::T_BYTES;  // [stage][W's NG tiles, T's]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem_s + G::STAGES * G::S_BYTES);
     uint64_t* empty = full + G::STAGES;
     uint64_t* done = empty + G::STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -318,12 +351,12 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
             ok = __all_sync(0xffffffffu, mbar_wait(empty0 + slot * 8, phase, abort_flag));
             if (!ok) break;
             if (elect_one()) {
-                const uint32_t bar = full0 + slot * 8, ss = sc0 + slot * 4 * kScaleTile;
+                const uint32_t bar = full0 + slot * 8, ss = sc0 + slot * G::S_BYTES;
                 mbar_expect_tx(bar, G::STAGE_BYTES);
                 tma_load_2d(w0 + slot * kWBytes, &map_w, s * kRowBytes, tn * 128, bar);
                 tma_load_2d(t0 + slot * G::T_BYTES, &map_t, s * kRowBytes, tm * TN, bar);
-                tma_load_3d(ss, &map_sw, 0, s * 2, tn, bar);
-                tma_load_3d(ss + 2 * kScaleTile, &map_st, 0, s * 2, tm * TN / 128, bar);
+                tma_load_3d(ss, &map_sw, 0, F::scale_group(s), tn, bar);
+                tma_load_3d(ss + NG * kScaleTile, &map_st, 0, F::scale_group(s), tm * TN / 128, bar);
             }
             __syncwarp();
             if (++slot == G::STAGES) {
@@ -355,17 +388,18 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
             if (!ok) break;
             tc_fence_after();
             const uint64_t w = w0 + slot * (kWBytes >> 4), t = t0 + slot * (G::T_BYTES >> 4);
-            const uint64_t sc = sc0 + slot * (4 * kScaleTile >> 4);
-            const uint32_t cols = cols0 + slot * 16;  // scales: W groups 0, 1, then T groups 0, 1
-            const int steps = min(4, (p.blocks - s * kStageBlocks + 1) / 2);
+            const uint64_t sc = sc0 + slot * (G::S_BYTES >> 4);
+            const uint32_t cols = cols0 + slot * 16;  // scales: W's groups, then (at 8) T's
+            const int steps = min(kStageSteps, p.steps - s * kStageSteps);
             if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) copy_scales<1>(cols + i * 4, sc + i * (kScaleTile >> 4));
+                for (int i = 0; i < 2 * NG; ++i)
+                    copy_scales<1>(cols + i / NG * 8 + i % NG * 4, sc + i * (kScaleTile >> 4));
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
+                for (int kk = 0; kk < kStageSteps; ++kk)
                     if (kk < steps)
-                        mma_mx4<1>(sum, w + kk * 2, t + kk * 2, mx4_idesc(128, TN, kk & 1), cols + (kk >> 1) * 4,
-                                   cols + 8 + (kk >> 1) * 4 + token_col, (s > s0 + 1 || kk > 0) ? 1u : 0u);
+                        mma_scaled<F, 1>(sum, w + kk * 2, t + kk * 2, F::idesc(128, TN, kk, s), cols + F::tile(kk) * 4,
+                                         cols + 8 + F::tile(kk) * 4 + token_col, (s > s0 + 1 || kk > 0) ? 1u : 0u);
                 tc_commit(smem_u32(&empty[slot]));
             }
             __syncwarp();
@@ -463,10 +497,12 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 // again and again 183 to 220 us, the clock held down by the 1 kW power limit (154 us
 // on matrices of zeros, which draw less).
 constexpr int kPairStages = 6;
-constexpr int kPairStageBytes = 2 * kWBytes + 6 * kScaleTile;  // codes of T and W, two tiles of T's scales, four of W's
-constexpr int kPairSmem = kPairStages * kPairStageBytes + 8 * 512 /* bias of each epilogue warp's columns */ + 256;
+template <typename F>
+constexpr int kPairStageBytes = 2 * kWBytes + 3 * F::GROUPS * kScaleTile;  // codes of T and W, a row tile of T's scales, two of W's
+template <typename F>
+constexpr int kPairSmem = kPairStages * kPairStageBytes<F> + 8 * 512 /* bias of each epilogue warp's columns */ + 256;
 constexpr int kPairThreads = 320;  // warps: 0 TMA, 1 MMA (leader), 2-9 epilogue (two to a TMEM lane quadrant)
-static_assert(kPairSmem <= 227 * 1024, "shared memory of a CTA");
+static_assert(kPairSmem<Mx4> <= 227 * 1024 && kPairSmem<Fp8> <= 227 * 1024, "shared memory of a CTA");
 static_assert(256 + 24 * kPairStages <= 512, "TMEM columns");
 
 __device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
@@ -581,18 +617,18 @@ __device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias,
 }
 
 // ALIGNED: C's rows are 16-byte aligned.
-template <bool ALIGNED>
+template <typename F, bool ALIGNED>
 __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ CUtensorMap map_t,
                                                                    const __grid_constant__ CUtensorMap map_sw,
                                                                    const __grid_constant__ CUtensorMap map_st,
                                                                    Mx4Params p) {
-    constexpr int S = kPairStages;
+    constexpr int S = kPairStages, NG = F::GROUPS, S_BYTES = 3 * NG * kScaleTile;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* smem_w = smem;
     uint8_t* smem_t = smem + S * kWBytes;
-    uint8_t* smem_s = smem + 2 * S * kWBytes;  // [stage][T groups 0, 1; columns 0-127 groups 0, 1; columns 128-255]
-    float* smem_bias = reinterpret_cast<float*>(smem_s + S * 6 * kScaleTile);  // [epilogue warp][128]
+    uint8_t* smem_s = smem + 2 * S * kWBytes;  // [stage][T's NG groups; those of columns 0-127; of columns 128-255]
+    float* smem_bias = reinterpret_cast<float*>(smem_s + S * S_BYTES);  // [epilogue warp][128]
     uint64_t* full = reinterpret_cast<uint64_t*>(smem_bias + 8 * 128);  // leader: both CTAs' bytes of a stage
     uint64_t* empty = full + S;   // each CTA: stage read by the MMAs
     uint64_t* tfull = empty + S;  // each CTA: accumulator complete
@@ -658,12 +694,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + slot * 8, phase, abort_flag));
                 if (!ok) break;
                 if (elect_one()) {
-                    if (rank == 0) mbar_expect_tx(full0 + slot * 8, 2 * kPairStageBytes);
-                    const uint32_t bar = leader_full0 + slot * 8, ss = sc0 + slot * 6 * kScaleTile;
+                    if (rank == 0) mbar_expect_tx(full0 + slot * 8, 2 * kPairStageBytes<F>);
+                    const uint32_t bar = leader_full0 + slot * 8, ss = sc0 + slot * S_BYTES;
                     tma_pair_2d(w0 + slot * kWBytes, &map_w, s * kRowBytes, w_row, bar);
                     tma_pair_2d(t0 + slot * kWBytes, &map_t, s * kRowBytes, t_row, bar);
-                    tma_pair_3d(ss, &map_st, 0, s * 2, tm * 2 + (int)rank, bar);
-                    tma_pair_3d(ss + 2 * kScaleTile, &map_sw, 0, s * 2, tn * 2, bar);
+                    tma_pair_3d(ss, &map_st, 0, F::scale_group(s), tm * 2 + (int)rank, bar);
+                    tma_pair_3d(ss + NG * kScaleTile, &map_sw, 0, F::scale_group(s), tn * 2, bar);
                 }
                 __syncwarp();
                 ++issued;
@@ -697,21 +733,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t wd = w0 + slot * (kWBytes >> 4), td = t0 + slot * (kWBytes >> 4);
-                const uint64_t sc = sc0 + slot * (6 * kScaleTile >> 4);
-                const uint32_t cols = tmem + 256 + slot * 24;  // T group 0, T group 1, W group 0 (8 wide), W group 1
-                const int steps = min(4, (p.blocks - s * kStageBlocks + 1) / 2);
+                const uint64_t sc = sc0 + slot * (S_BYTES >> 4);
+                const uint32_t cols = tmem + 256 + slot * 24;  // T's groups, then (at 8) W's, 8 wide each
+                const int steps = min(kStageSteps, p.steps - s * kStageSteps);
                 if (elect_one()) {
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
+                    for (int g = 0; g < NG; ++g) {
                         copy_scales<2>(cols + g * 4, sc + g * (kScaleTile >> 4));
-                        copy_scales<2>(cols + 8 + g * 8, sc + (2 + g) * (kScaleTile >> 4));
-                        copy_scales<2>(cols + 8 + g * 8 + 4, sc + (4 + g) * (kScaleTile >> 4));
+                        copy_scales<2>(cols + 8 + g * 8, sc + (NG + g) * (kScaleTile >> 4));
+                        copy_scales<2>(cols + 8 + g * 8 + 4, sc + (2 * NG + g) * (kScaleTile >> 4));
                     }
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
+                    for (int kk = 0; kk < kStageSteps; ++kk)
                         if (kk < steps)
-                            mma_mx4<2>(tmem, td + kk * 2, wd + kk * 2, mx4_idesc(256, 256, kk & 1),
-                                       cols + (kk >> 1) * 4, cols + 8 + (kk >> 1) * 8, (s > 0 || kk > 0) ? 1u : 0u);
+                            mma_scaled<F, 2>(tmem, td + kk * 2, wd + kk * 2, F::idesc(256, 256, kk, s),
+                                             cols + F::tile(kk) * 4, cols + 8 + F::tile(kk) * 8,
+                                             (s > 0 || kk > 0) ? 1u : 0u);
                     commit_pair(empty0 + slot * 8);
                     commit_pair(empty1 + slot * 8);
                 }
@@ -795,8 +832,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         asm volatile("fence.acq_rel.cluster;" ::: "memory");
         land_pair(
             S, *issued_all, both ? *issued_peer : *issued_all,
-            [&](int slot) { mbar_expect_tx(smem_u32(&full[slot]), kPairStageBytes); },
-            [&](int slot) { complete_tx(smem_u32(&full[slot]), kPairStageBytes); },
+            [&](int slot) { mbar_expect_tx(smem_u32(&full[slot]), kPairStageBytes<F>); },
+            [&](int slot) { complete_tx(smem_u32(&full[slot]), kPairStageBytes<F>); },
             [&](int slot, uint32_t phase) { mbar_wait(smem_u32(&full[slot]), phase, &never); });
     }
     tc_fence_before();
@@ -836,43 +873,47 @@ int encode(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* bas
     return RT_OK;
 }
 
-// Codes: rows of row_bytes bytes, box of `rows` x 128 bytes.
-int map_codes(CUtensorMap* map, const rt_mx4& q, int rows) {
-    const cuuint64_t dims[2] = {(cuuint64_t)q.row_bytes(), (cuuint64_t)q.rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)q.row_bytes()};
+// Codes: rows of `bytes` bytes, row_bytes apart; box of `rows` x 128 bytes.
+int map_codes(CUtensorMap* map, const rt_scaled& q, int64_t bytes, int64_t row_bytes, int rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)q.rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
     const cuuint32_t box[2] = {kRowBytes, (cuuint32_t)rows};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q.codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Scales: tiles of 128 words, [row tile][k group]; box of 2 k groups of `tiles` row tiles.
-int map_scales(CUtensorMap* map, const rt_mx4& q, int tiles) {
-    const cuuint64_t dims[3] = {128, (cuuint64_t)q.groups(), (cuuint64_t)((q.rows + 127) / 128)};
-    const cuuint64_t strides[2] = {kScaleTile, (cuuint64_t)(q.groups() * kScaleTile)};
-    const cuuint32_t box[3] = {128, 2, (cuuint32_t)tiles};
+// Scales: tiles of 128 words, [row tile][k group]; box of `along` k groups of `tiles` row tiles.
+int map_scales(CUtensorMap* map, const rt_scaled& q, int64_t groups, int along, int tiles) {
+    const cuuint64_t dims[3] = {128, (cuuint64_t)groups, (cuuint64_t)((q.rows + 127) / 128)};
+    const cuuint64_t strides[2] = {kScaleTile, (cuuint64_t)(groups * kScaleTile)};
+    const cuuint32_t box[3] = {128, (cuuint32_t)along, (cuuint32_t)tiles};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, q.scales, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+int encode_maps(rt_scaled* q, int64_t bytes, int64_t row_bytes, int64_t groups, int along) {
+    if (q->rows == 0 || q->k == 0) return RT_OK;
+    for (int i = 0; i < 3; ++i) RT_TRY(map_codes(&q->maps.codes[i], *q, bytes, row_bytes, 32 << i));
+    for (int i = 0; i < 2; ++i) RT_TRY(map_scales(&q->maps.scales[i], *q, groups, along, 1 + i));
+    return RT_OK;
 }
 
 }  // namespace
 
-int mx4_encode_maps(rt_mx4* q) {
-    if (q->rows == 0 || q->k == 0) return RT_OK;
-    for (int i = 0; i < 3; ++i) RT_TRY(map_codes(&q->maps.codes[i], *q, 32 << i));
-    for (int i = 0; i < 2; ++i) RT_TRY(map_scales(&q->maps.scales[i], *q, 1 + i));
-    return RT_OK;
-}
+int mx4_encode_maps(rt_mx4* q) { return encode_maps(q, q->row_bytes(), q->row_bytes(), q->groups(), Mx4::GROUPS); }
+// The bytes between k and row_bytes lie outside the box: they read as zeros whatever they hold.
+int fp8_encode_maps(rt_fp8* q) { return encode_maps(q, q->k, q->row_bytes(), q->groups(), Fp8::GROUPS); }
 
 namespace {
 
-template <int TN>
-int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int splits, cudaStream_t stream) {
-    using G = Geo1<TN>;
+template <typename F, int TN>
+int launch_one(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p, int splits, cudaStream_t stream) {
+    using G = Geo1<F, TN>;
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[TN / 64], &sw = b.maps.scales[0], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + TN - 1) / TN);
     p.tiles_n = (int)((p.n + 127) / 128);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     p.stages_per_split = (p.stages + splits - 1) / splits;
     splits = (p.stages + p.stages_per_split - 1) / p.stages_per_split;
-    RT_CHECK(tiles * splits <= INT32_MAX, "rt_mx4_matmul: C is too large");
+    RT_CHECK(tiles * splits <= INT32_MAX, "block-scaled product: C is too large");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * splits));
     cfg.blockDim = dim3(kThreads1);
@@ -887,21 +928,22 @@ int launch_one(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, int s
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 2 : 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<TN>, w, t, sw, st, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, mx4_kernel<F, TN>, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
 }
 
-int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cudaStream_t stream) {
+template <typename F>
+int launch_pair(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p, cudaStream_t stream) {
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[1], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    RT_CHECK(tiles <= INT32_MAX, "rt_mx4_matmul: C is too large");
+    RT_CHECK(tiles <= INT32_MAX, "block-scaled product: C is too large");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.dynamicSmemBytes = kPairSmem<F>;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -912,34 +954,44 @@ int launch_pair(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, Mx4Params p, cuda
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 2 : 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, p.access >= 16 ? mx4_pair_kernel<true> : mx4_pair_kernel<false>, w, t, sw, st, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, p.access >= 16 ? mx4_pair_kernel<F, true> : mx4_pair_kernel<F, false>, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
 }
 
-template <int TN>
+template <typename F, int TN>
 int allow_smem() {
-    RT_CUDA(cudaFuncSetAttribute(mx4_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<TN>::SMEM));
+    RT_CUDA(cudaFuncSetAttribute(mx4_kernel<F, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo1<F, TN>::SMEM));
+    return RT_OK;
+}
+
+template <typename F>
+int allow_all() {
+    RT_TRY((allow_smem<F, 32>()));
+    RT_TRY((allow_smem<F, 64>()));
+    RT_TRY((allow_smem<F, 128>()));
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<F, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<F>));
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<F, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<F>));
     return RT_OK;
 }
 
 }  // namespace
 
 int gemm_mx4_init() {
-    RT_TRY(allow_smem<32>());
-    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-    RT_TRY(allow_smem<64>());
-    return allow_smem<128>();
+    RT_TRY(allow_all<Mx4>());
+    return allow_all<Fp8>();
 }
 
-int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
-                    cudaStream_t stream) {
+namespace {
+
+template <typename F>
+int launch_product(rt_ctx* ctx, const typename F::Matrix& a, const typename F::Matrix& b, const rt_tensor& c,
+                   const float* bias, bool relu, cudaStream_t stream) {
     Mx4Params p{};
     p.m = c.rows;
     p.n = c.cols;
-    p.blocks = (int)a.blocks();
-    p.stages = (int)((a.blocks() + kStageBlocks - 1) / kStageBlocks);
+    p.steps = F::steps(a);
+    p.stages = (p.steps + kStageSteps - 1) / kStageSteps;
     p.c = c.ptr;
     p.ldc = c.ld;
     p.out_bf16 = c.dtype == RT_BF16;
@@ -949,7 +1001,7 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
     const uintptr_t rows = reinterpret_cast<uintptr_t>(p.c) | (uintptr_t)(p.ldc * (p.out_bf16 ? 2 : 4));
     p.access = (rows & 31) == 0 ? 32 : (rows & 15) == 0 ? 16 : (rows & 7) == 0 ? 8 : 0;
     RT_CUDA(cudaSetDevice(ctx->device));
-    if (p.blocks == 0) {
+    if (p.steps == 0) {
         RT_CUDA(launch_k(ctx->pdl, bias_kernel, ctx->sm_count * 4, 256, 0, stream, p));
         count_launch(ctx);
         return RT_OK;
@@ -963,9 +1015,9 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
     // stages, 6.2 / 5.8.
     const int tn = p.m <= 32 ? 32 : 64;
     const int64_t tiles = ((p.m + tn - 1) / tn) * ((p.n + 127) / 128), slots = 2 * (int64_t)ctx->sm_count;
-    if (tiles > slots) return launch_pair(ctx, a, b, p, stream);
+    if (tiles > slots) return launch_pair<F>(ctx, a, b, p, stream);
     if (tiles > ctx->sm_count && p.stages > 8 && ((p.m + 127) / 128) * ((p.n + 127) / 128) <= ctx->sm_count)
-        return launch_one<128>(ctx, a, b, p, 1, stream);
+        return launch_one<F, 128>(ctx, a, b, p, 1, stream);
     // Split k until a CTA has at most 8 stages, within those slots: joining the splits costs
     // about 2 us, and few tiles leave most SMs without work (16 x 1024 x 8192, 32 stages on 8
     // tiles: 5.9 us in four, 8.4 in one; 64 x 1000 x 8192: 7.3 / 9.7; 1024^3, 4 stages: 6.6 in
@@ -974,8 +1026,20 @@ int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tens
     // L2).
     int splits = 1;
     while (splits < 8 && p.stages > 8 * splits && tiles * splits * 2 <= slots) splits *= 2;
-    if (tn == 32) return launch_one<32>(ctx, a, b, p, splits, stream);
-    return launch_one<64>(ctx, a, b, p, splits, stream);
+    if (tn == 32) return launch_one<F, 32>(ctx, a, b, p, splits, stream);
+    return launch_one<F, 64>(ctx, a, b, p, splits, stream);
+}
+
+}  // namespace
+
+int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
+                    cudaStream_t stream) {
+    return launch_product<Mx4>(ctx, a, b, c, bias, relu, stream);
+}
+
+int launch_gemm_fp8(rt_ctx* ctx, const rt_fp8& a, const rt_fp8& b, const rt_tensor& c, const float* bias, bool relu,
+                    cudaStream_t stream) {
+    return launch_product<Fp8>(ctx, a, b, c, bias, relu, stream);
 }
 
 }  // namespace rt

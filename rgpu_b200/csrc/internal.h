@@ -86,8 +86,8 @@ struct rt_tensor {
     bool owned = false;
 };
 
-// A matrix [rows, k] in microscaled 4-bit floating point (rtgpu.h has the layout).
-struct rt_mx4 {
+// What the block-scaled matrices [rows, k] share (rtgpu.h has their layouts).
+struct rt_scaled {
     rt_ctx* ctx = nullptr;
     uint8_t* codes = nullptr;
     uint8_t* scales = nullptr;
@@ -98,9 +98,20 @@ struct rt_mx4 {
     struct {
         CUtensorMap codes[3], scales[2];
     } maps;
+};
+
+// Microscaled 4-bit floating point, a scale for 32 elements.
+struct rt_mx4 : rt_scaled {
     __host__ __device__ int64_t blocks() const { return (k + 31) / 32; }
     __host__ __device__ int64_t row_bytes() const { return blocks() * 16; }
     __host__ __device__ int64_t groups() const { return (blocks() + 3) / 4; }  // scale tiles along k
+};
+
+// 8-bit floating point (E4M3), a scale for 128 elements.
+struct rt_fp8 : rt_scaled {
+    __host__ __device__ int64_t blocks() const { return (k + 127) / 128; }
+    __host__ __device__ int64_t row_bytes() const { return (k + 15) / 16 * 16; }
+    __host__ __device__ int64_t groups() const { return (blocks() + 3) / 4; }
 };
 
 namespace rt {
@@ -280,10 +291,15 @@ int launch_sum_partials_own(rt_ctx* ctx, float* out, const float* own, const flo
 int launch_fill_column(rt_ctx* ctx, void* p, rt_dtype dt, int64_t rows, int64_t ld, int64_t col, float value,
                        cudaStream_t stream);
 
+int embedding_init();
 int gemm_mx4_init();
 int mx4_encode_maps(rt_mx4* q);
 // C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU) of microscaled 4-bit matrices.
 int launch_gemm_mx4(rt_ctx* ctx, const rt_mx4& a, const rt_mx4& b, const rt_tensor& c, const float* bias, bool relu,
+                    cudaStream_t stream);
+// The same of 8-bit matrices.
+int fp8_encode_maps(rt_fp8* q);
+int launch_gemm_fp8(rt_ctx* ctx, const rt_fp8& a, const rt_fp8& b, const rt_tensor& c, const float* bias, bool relu,
                     cudaStream_t stream);
 
 // Multi-tensor optimiser.  Each entry updates a packed f32 buffer of n

@@ -1,9 +1,7 @@
 // Microscaled 4-bit matrices: handles, quantisation and dequantisation.
-#include <algorithm>
-#include <climits>
-#include <new>
-
 #include "mx4.cuh"
+#include "row_piece.cuh"
+#include "scaled.cuh"
 
 namespace rt {
 namespace {
@@ -20,155 +18,14 @@ __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// A lane's piece of a row: 32 bytes, 16 bf16 or 8 f32.  V: bytes of an access, 32
-// (one 256-bit access, Blackwell's widest) or 16 where the rows are so aligned.
-// Else (0) a warp's accesses take neighbouring words, which change hands through its
-// kilobyte of shared memory; an aligned row's last piece goes element by element.
+// Codes of the piece's elements 8 i .. 8 i + 7.
 template <typename T>
-struct Piece {
-    static constexpr int E = 32 / sizeof(T);         // elements
-    static constexpr int PER_BLOCK = 32 / E;         // lanes that share a block
-    static constexpr int PER_GROUP = 128 / E;        // and a scale group
-    static constexpr int WARP = 32 * E;              // elements of a warp
-    uint32_t w[8];
-
-    template <int V>
-    __device__ __forceinline__ void load(const T* p, int64_t left) {
-        if (V == 32 && left >= E) {
-            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                         : "l"(p));
-        } else if (V == 16 && left >= E) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-        } else {
+__device__ __forceinline__ uint32_t encode(const Piece<T>& x, int i, float inv) {
+    float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e < left) {
-                    if constexpr (sizeof(T) == 2)
-                        w[e / 2] |= (uint32_t)__bfloat16_as_ushort(p[e]) << (16 * (e & 1));
-                    else
-                        w[e] = __float_as_uint(p[e]);
-                }
-        }
-    }
-    template <int V>
-    __device__ __forceinline__ void store(T* p, int64_t left) const {
-        if (V == 32 && left >= E) {
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                         "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                         : "memory");
-        } else if (V == 16 && left >= E) {
-            reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (e < left) {
-                    if constexpr (sizeof(T) == 2)
-                        p[e] = __ushort_as_bfloat16((unsigned short)(w[e / 2] >> (16 * (e & 1))));
-                    else
-                        p[e] = __uint_as_float(w[e]);
-                }
-        }
-    }
-    // The warp's piece of an unaligned row of which `left` elements lie from p on, p and
-    // left the warp's, not the lane's: read as words, then shared out through box, the
-    // warp's 1 KB.  bf16 whose row starts between two words: pairs from element 1 on, and
-    // element 0 by itself (`head`); a lane's words are then half a word off.
-    struct Words {
-        uint32_t v[8], head;
-    };
-    static __device__ __forceinline__ bool between(const T* p) { return sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(p) & 2); }
-    static __device__ __forceinline__ uint32_t half(const T* p) { return *reinterpret_cast<const unsigned short*>(p); }
-    static __device__ __forceinline__ Words fetch_any(const T* p, int64_t left, int lane) {
-        Words r;
-        constexpr int N = 4 / sizeof(T);  // elements of a word
-        const int odd = between(p);
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(p + odd);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int at = i * 32 + lane;
-            const int64_t room = left - odd - at * N;
-            r.v[i] = room >= N ? __ldg(words + at) : N == 2 && room == 1 ? half(p + odd + at * N) : 0u;
-        }
-        r.head = odd && lane == 0 && left > 0 ? half(p) << 16 : 0u;
-        return r;
-    }
-    __device__ __forceinline__ void deal_any(const Words& r, bool odd, uint32_t* box, int lane) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) box[i * 32 + lane] = r.v[i];
-        __syncwarp();
-        const uint4 a = reinterpret_cast<const uint4*>(box)[lane * 2], b = reinterpret_cast<const uint4*>(box)[lane * 2 + 1];
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-        if (sizeof(T) == 2 && odd) {  // the same of the whole warp
-            uint32_t before = __shfl_up_sync(0xffffffffu, w[7], 1);
-            if (lane == 0) before = r.head;
-#pragma unroll
-            for (int i = 7; i >= 0; --i) w[i] = __funnelshift_l(i ? w[i - 1] : before, w[i], 16);
-        }
-    }
-    __device__ __forceinline__ void store_any(T* p, int64_t left, uint32_t* box, int lane) const {
-        constexpr int N = 4 / sizeof(T);
-        const int odd = between(p);
-        uint32_t s[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = w[i];
-        if (sizeof(T) == 2 && odd) {
-            const uint32_t after = __shfl_down_sync(0xffffffffu, w[0], 1);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = __funnelshift_r(w[i], i < 7 ? w[i + 1] : after, 16);
-            if (lane == 0 && left > 0) *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
-        }
-        __syncwarp();
-        reinterpret_cast<uint4*>(box)[lane * 2] = make_uint4(s[0], s[1], s[2], s[3]);
-        reinterpret_cast<uint4*>(box)[lane * 2 + 1] = make_uint4(s[4], s[5], s[6], s[7]);
-        __syncwarp();
-        uint32_t* words = reinterpret_cast<uint32_t*>(p + odd);
-        const int64_t end = min(left, (int64_t)WARP) - odd;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int at = i * 32 + lane;
-            const int64_t room = end - at * N;
-            if (room >= N)
-                words[at] = box[at];
-            else if (N == 2 && room == 1)
-                *reinterpret_cast<unsigned short*>(words + at) = (unsigned short)box[at];
-        }
-    }
-    // Bit pattern (as f32) of the largest magnitude in the lane.
-    __device__ __forceinline__ uint32_t amax() const {
-        uint32_t m = 0;
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
-            return max(m << 16, m & 0xffff0000u);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
-            return m;
-        }
-    }
-    // Codes of the elements 8 i .. 8 i + 7.
-    __device__ __forceinline__ uint32_t encode(int i, float inv) const {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if constexpr (sizeof(T) == 2) {
-                const uint32_t x = w[i * 4 + e / 2];
-                v[e] = __uint_as_float(e & 1 ? x & 0xffff0000u : x << 16);
-            } else {
-                v[e] = __uint_as_float(w[e]);
-            }
-        }
-        return encode8(v, inv);
-    }
-};
+    for (int e = 0; e < 8; ++e) v[e] = x.value(i * 8 + e);
+    return encode8(v, inv);
+}
 
 // Blocks along a row.  A warp takes 512 (f32: 256) elements of the four rows r,
 // r + 32, r + 64, r + 96 of a 128-row tile: the scales of these rows lie side by
@@ -176,36 +33,13 @@ struct Piece {
 // lanes to a block keep the instructions per element low enough for HBM to be the
 // bound: 2 (f32: 4) bytes in and 17/32 out per element.  8192 x 8192 bf16: 30 us,
 // 5.7 TB/s.
-struct Rows {
-    int64_t sets;  // sets of four rows
-    int rcount;    // rows r of a tile: 32, or fewer where the matrix has fewer
-    int chunks;    // warps' worth of elements along k
-    int split;     // log2 of the warps of a CTA that lie along k; the others take other sets
-};
-
-// The warp's first chunk along k and first set, and the grid's strides.
-struct Place {
-    int chunk, chunk_step;
-    int64_t set, set_step;
-    __device__ __forceinline__ explicit Place(const Rows& w) {
-        const int warp = threadIdx.x >> 5;
-        chunk = ((int)blockIdx.x << w.split) + (warp & ((1 << w.split) - 1));
-        chunk_step = (int)gridDim.x << w.split;
-        set = ((int64_t)blockIdx.y << (3 - w.split)) + (warp >> w.split);
-        set_step = (int64_t)gridDim.y << (3 - w.split);
-    }
-};
-// First row of a set.
-__device__ __forceinline__ int64_t set_row(const Rows& w, int64_t set) {
-    return w.rcount == 32 ? (set >> 5) * 128 + (set & 31) : set;
-}
-
 template <typename T, int V>
 __global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
                                                                int64_t k, Rows w, int64_t blocks, int64_t groups,
                                                                uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales) {
     using P = Piece<T>;
+    constexpr int PER_BLOCK = 32 / P::E, PER_GROUP = 128 / P::E;  // lanes that share a block, a scale group
     __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
     pdl_wait();
     pdl_launch_dependents();
@@ -235,23 +69,23 @@ __global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* 
             for (int q = 0; q < 4; ++q) {
                 uint32_t amax = x[q].amax();
 #pragma unroll
-                for (int o = 1; o < P::PER_BLOCK; o *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                for (int o = 1; o < PER_BLOCK; o *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 const uint32_t byte = scale_byte(amax);
                 const float inv = inv_scale(byte);
                 const bool nan = byte == kNanScale;
                 if (q < live && inside) {
                     if constexpr (sizeof(T) == 2)
                         *reinterpret_cast<uint2*>(out + q * (32 * row_bytes)) =
-                            make_uint2(nan ? 0u : x[q].encode(0, inv), nan ? 0u : x[q].encode(1, inv));
+                            make_uint2(nan ? 0u : encode(x[q], 0, inv), nan ? 0u : encode(x[q], 1, inv));
                     else
-                        *reinterpret_cast<uint32_t*>(out + q * (32 * row_bytes)) = nan ? 0u : x[q].encode(0, inv);
+                        *reinterpret_cast<uint32_t*>(out + q * (32 * row_bytes)) = nan ? 0u : encode(x[q], 0, inv);
                 }
                 // the bytes of a group's four blocks into its first lane
-                word[q] = byte | __shfl_down_sync(0xffffffffu, byte, P::PER_BLOCK) << 8;
-                word[q] |= __shfl_down_sync(0xffffffffu, word[q], 2 * P::PER_BLOCK) << 16;
+                word[q] = byte | __shfl_down_sync(0xffffffffu, byte, PER_BLOCK) << 8;
+                word[q] |= __shfl_down_sync(0xffffffffu, word[q], 2 * PER_BLOCK) << 16;
             }
             const int64_t group = j >> 7;
-            if (lane % P::PER_GROUP == 0 && group < groups)
+            if (lane % PER_GROUP == 0 && group < groups)
                 *reinterpret_cast<uint4*>(scales + ((row >> 7) * groups + group) * 512 + (row & 31) * 16) =
                     make_uint4(word[0], word[1], word[2], word[3]);
         }
@@ -411,27 +245,6 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
         }
 }
 
-// Sets and chunks, and a grid that covers chunks before sets.
-Rows rows_for(const rt_ctx* ctx, int64_t rows, int64_t k, int chunk, dim3* grid) {
-    Rows w;
-    w.rcount = (int)std::min<int64_t>(rows, 32);
-    w.sets = w.rcount * ((rows + 127) / 128);
-    w.chunks = (int)((k + chunk - 1) / chunk);
-    w.split = w.chunks > 4 ? 3 : w.chunks > 2 ? 2 : w.chunks > 1 ? 1 : 0;
-    const int64_t along = (w.chunks + (1 << w.split) - 1) >> w.split;
-    const int64_t across = (w.sets + (8 >> w.split) - 1) >> (3 - w.split), limit = (int64_t)ctx->sm_count * 64;
-    grid->x = (unsigned)std::min(along, limit);
-    grid->y = (unsigned)std::min<int64_t>(std::min(across, std::max<int64_t>(1, limit / grid->x)), 65535);
-    grid->z = 1;
-    return w;
-}
-
-// Widest access that every row of t allows: 32, 16 or 0.
-int access_of(const rt_tensor* t) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(t->ptr) | (uintptr_t)(t->ld * (int64_t)dtype_size(t->dtype));
-    return (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 0;
-}
-
 template <typename T>
 int launch_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_mx4* q) {
     const T* p = static_cast<const T*>(src->ptr);
@@ -467,13 +280,7 @@ int launch_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst) {
     return RT_OK;
 }
 
-int check_extents(int64_t rows, int64_t k) {
-    RT_CHECK(rows >= 0 && k >= 0, "mx4: negative extent %lld x %lld", (long long)rows, (long long)k);
-    // box coordinates and the block count of a row are 32-bit
-    RT_CHECK(rows <= INT_MAX - 256 && k <= INT_MAX - 256, "mx4: extent above 2^31 - 257: %lld x %lld", (long long)rows,
-             (long long)k);
-    return RT_OK;
-}
+int check_extents(int64_t rows, int64_t k) { return check_scaled_extents("mx4", rows, k); }
 
 }  // namespace
 }  // namespace rt
@@ -496,72 +303,18 @@ int rt_mx4_zeros(rt_ctx* ctx, int64_t rows, int64_t k, rt_mx4** out) {
     RT_CHECK(ctx && out, "rt_mx4_zeros: bad arguments");
     *out = nullptr;
     RT_TRY(check_extents(rows, k));
-    const size_t cb = (size_t)rt_mx4_code_bytes(rows, k), sb = (size_t)rt_mx4_scale_bytes(rows, k);
-    const size_t scales_at = (cb + 511) / 512 * 512;
-    RT_CUDA(cudaSetDevice(ctx->device));
-    void* p = nullptr;
-    cudaError_t e = cudaMalloc(&p, std::max<size_t>(scales_at + sb, 16));
-    if (e != cudaSuccess)
-        return fail(RT_ERR_OOM, "cudaMalloc(%zu) failed: %s", scales_at + sb, cudaGetErrorString(e));
-    e = cudaMemsetAsync(p, 0, std::max<size_t>(scales_at + sb, 16), ctx->stream);
-    if (e != cudaSuccess) {
-        cudaFree(p);
-        return fail(RT_ERR_CUDA, "cudaMemsetAsync failed: %s", cudaGetErrorString(e));
-    }
-    rt_mx4* q = new (std::nothrow) rt_mx4;
-    if (!q) {
-        cudaFree(p);
-        return fail(RT_ERR_OOM, "rt_mx4_zeros: out of host memory");
-    }
-    q->ctx = ctx;
-    q->codes = static_cast<uint8_t*>(p);
-    q->scales = q->codes + scales_at;
-    q->rows = rows;
-    q->k = k;
-    q->owned = true;
-    const int s = mx4_encode_maps(q);
-    if (s != RT_OK) {
-        cudaFree(p);
-        delete q;
-        return s;
-    }
-    *out = q;
-    return RT_OK;
+    return scaled_zeros(ctx, rows, k, (size_t)rt_mx4_code_bytes(rows, k), (size_t)rt_mx4_scale_bytes(rows, k),
+                        mx4_encode_maps, out);
 }
 
 int rt_mx4_wrap(rt_ctx* ctx, void* codes, void* scales, int64_t rows, int64_t k, rt_mx4** out) {
     RT_CHECK(ctx && out, "rt_mx4_wrap: bad arguments");
     *out = nullptr;
     RT_TRY(check_extents(rows, k));
-    RT_CHECK((codes && scales) || rows == 0 || k == 0, "rt_mx4_wrap: codes or scales is NULL");
-    RT_CHECK(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15) == 0,
-             "rt_mx4_wrap: codes and scales must be 16-byte aligned");
-    rt_mx4* q = new (std::nothrow) rt_mx4;
-    if (!q) return fail(RT_ERR_OOM, "rt_mx4_wrap: out of host memory");
-    q->ctx = ctx;
-    q->codes = static_cast<uint8_t*>(codes);
-    q->scales = static_cast<uint8_t*>(scales);
-    q->rows = rows;
-    q->k = k;
-    const int s = mx4_encode_maps(q);
-    if (s != RT_OK) {
-        delete q;
-        return s;
-    }
-    *out = q;
-    return RT_OK;
+    return scaled_wrap("rt_mx4_wrap", ctx, codes, scales, rows, k, mx4_encode_maps, out);
 }
 
-int rt_mx4_free(rt_mx4* q) {
-    if (!q) return RT_OK;
-    if (q->owned) {
-        cudaSetDevice(q->ctx->device);
-        cudaStreamSynchronize(q->ctx->stream);
-        cudaFree(q->codes);
-    }
-    delete q;
-    return RT_OK;
-}
+int rt_mx4_free(rt_mx4* q) { return scaled_free(q); }
 
 int rt_mx4_dims(const rt_mx4* q, int64_t* rows, int64_t* k) {
     RT_CHECK(q, "mx4 matrix is NULL");
@@ -599,19 +352,7 @@ int rt_mx4_dequantize(rt_ctx* ctx, const rt_mx4* q, rt_tensor* dst) {
 }
 
 int rt_mx4_matmul(rt_ctx* ctx, const rt_mx4* a, const rt_mx4* b, rt_tensor* c, const rt_tensor* bias, int relu) {
-    RT_CHECK(ctx && a && b && c, "rt_mx4_matmul: bad arguments");
-    RT_CHECK(a->ctx == ctx && b->ctx == ctx && c->ctx == ctx && (!bias || bias->ctx == ctx),
-             "tensor belongs to another context");
-    RT_CHECK(c->dtype == RT_F32 || c->dtype == RT_BF16, "rt_mx4_matmul: C must be f32 or bf16");
-    RT_CHECK(a->k == b->k, "rt_mx4_matmul: A is %lldx%lld, B %lldx%lld: the second extents differ", (long long)a->rows,
-             (long long)a->k, (long long)b->rows, (long long)b->k);
-    RT_CHECK(c->rows == a->rows && c->cols == b->rows, "rt_mx4_matmul: C is %lldx%lld, not %lldx%lld",
-             (long long)c->rows, (long long)c->cols, (long long)a->rows, (long long)b->rows);
-    if (bias) {
-        RT_CHECK(bias->dtype == RT_F32, "rt_mx4_matmul: bias must be f32");
-        RT_CHECK(bias->rows == 1 && bias->cols == b->rows, "rt_mx4_matmul: bias is %lldx%lld, not 1x%lld",
-                 (long long)bias->rows, (long long)bias->cols, (long long)b->rows);
-    }
+    RT_TRY(check_scaled_matmul("rt_mx4_matmul", ctx, a, b, c, bias));
     if (c->rows == 0 || c->cols == 0) return RT_OK;
     return launch_gemm_mx4(ctx, *a, *b, *c, bias ? static_cast<const float*>(bias->ptr) : nullptr, relu != 0,
                            ctx->stream);

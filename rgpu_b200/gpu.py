@@ -78,6 +78,11 @@ class BlockGrads(C.Structure):
                                           "dbeta_pre", "dgate", "work")]
 
 
+class DropoutMask(C.Structure):
+    _fields_ = [("p", C.c_double), ("seed", C.c_uint64), ("site", C.c_uint32), ("step", C.c_uint32),
+                ("step_at", C.c_void_p), ("first_row", C.c_int64)]
+
+
 _lib = None
 
 # (name, restype, argtypes)
@@ -137,6 +142,21 @@ _SIGS = [
     ("rt_mx4_quantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     ("rt_mx4_dequantize", C.c_int, [C.c_void_p] * 3),
     ("rt_mx4_matmul", C.c_int, [C.c_void_p] * 5 + [C.c_int]),
+    ("rt_fp8_zeros", C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.POINTER(C.c_void_p)]),
+    ("rt_fp8_wrap", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.POINTER(C.c_void_p)]),
+    ("rt_fp8_free", C.c_int, [C.c_void_p]),
+    ("rt_fp8_dims", C.c_int, [C.c_void_p, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
+    ("rt_fp8_codes", C.c_void_p, [C.c_void_p]),
+    ("rt_fp8_scales", C.c_void_p, [C.c_void_p]),
+    ("rt_fp8_code_bytes", C.c_int64, [C.c_int64, C.c_int64]),
+    ("rt_fp8_scale_bytes", C.c_int64, [C.c_int64, C.c_int64]),
+    ("rt_fp8_quantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    ("rt_fp8_dequantize", C.c_int, [C.c_void_p] * 3),
+    ("rt_fp8_matmul", C.c_int, [C.c_void_p] * 5 + [C.c_int]),
+    ("rt_embedding_forward", C.c_int, [C.c_void_p] * 3 + [C.c_float, C.c_void_p]),
+    ("rt_embedding_backward", C.c_int, [C.c_void_p] * 3 + [C.c_float, C.c_int] + [C.c_void_p] * 2),
+    ("rt_embedding_backward_workspace", C.c_int64, [C.c_int64] * 3),
+    ("rt_dropout", C.c_int, [C.c_void_p] * 4 + [C.POINTER(DropoutMask)]),
     ("rt_block_forward", C.c_int, [C.c_void_p, C.POINTER(BlockArgs)]),
     ("rt_block_backward", C.c_int, [C.c_void_p, C.POINTER(BlockArgs), C.POINTER(BlockGrads)]),
     ("rt_block_backward_workspace", C.c_int64, [C.c_void_p, C.c_int64, C.c_int64]),
@@ -294,16 +314,19 @@ class GpuTensor:
             pass
 
 
-class Mx4Tensor:
-    """A device matrix [rows, k] in microscaled 4-bit floating point (rt_mx4):
-    E2M1 elements, one power-of-two scale per 32 along k."""
+class _ScaledTensor:
+    """A block-scaled device matrix [rows, k]; `_name` is its C prefix."""
 
     def __init__(self, gpu: "Gpu", handle: int):
         self.gpu = gpu
         self.handle = C.c_void_p(handle)
         r, k = C.c_int64(), C.c_int64()
-        _check(lib().rt_mx4_dims(self.handle, C.byref(r), C.byref(k)))
+        _check(self._call("dims")(self.handle, C.byref(r), C.byref(k)))
         self.rows, self.k = r.value, k.value
+
+    @classmethod
+    def _call(cls, what: str):
+        return getattr(lib(), f"{cls._name}_{what}")
 
     @property
     def shape(self):
@@ -311,21 +334,21 @@ class Mx4Tensor:
 
     @property
     def codes_ptr(self) -> int:
-        return lib().rt_mx4_codes(self.handle)
+        return self._call("codes")(self.handle)
 
     @property
     def scales_ptr(self) -> int:
-        return lib().rt_mx4_scales(self.handle)
+        return self._call("scales")(self.handle)
 
-    @staticmethod
-    def nbytes(rows: int, k: int):
+    @classmethod
+    def nbytes(cls, rows: int, k: int):
         """(bytes of the codes, bytes of the scales) of a rows x k matrix."""
-        return lib().rt_mx4_code_bytes(rows, k), lib().rt_mx4_scale_bytes(rows, k)
+        return cls._call("code_bytes")(rows, k), cls._call("scale_bytes")(rows, k)
 
     def free(self):
         if self.handle and self.handle.value:
             if self.gpu.alive():
-                lib().rt_mx4_free(self.handle)
+                self._call("free")(self.handle)
             self.handle = C.c_void_p(0)
 
     def __del__(self):
@@ -333,6 +356,20 @@ class Mx4Tensor:
             self.free()
         except Exception:
             pass
+
+
+class Mx4Tensor(_ScaledTensor):
+    """A device matrix [rows, k] in microscaled 4-bit floating point (rt_mx4):
+    E2M1 elements, one power-of-two scale per 32 along k."""
+
+    _name = "rt_mx4"
+
+
+class Fp8Tensor(_ScaledTensor):
+    """A device matrix [rows, k] in 8-bit floating point (rt_fp8): E4M3
+    elements, one power-of-two scale per 128 along k."""
+
+    _name = "rt_fp8"
 
 
 class Norm:
@@ -351,6 +388,33 @@ class Norm:
         a, gamma, beta = self._args, self.gamma, self.beta
         a.gamma = None if gamma is None else gamma.handle or _freed()
         a.beta = None if beta is None else beta.handle or _freed()
+        return a
+
+
+class Dropout:
+    """Which elements Gpu.dropout drops: a share p of them, by the generator's
+    seed, the dropout's site in the model, the step and the row's number from
+    first_row on.  step_at: one u32 on the device, added to step when the kernel
+    runs."""
+
+    def __init__(self, p: float, seed: int, *, site: int = 0, step: int = 0, step_at: GpuTensor | None = None,
+                 first_row: int = 0):
+        if not 0 <= seed < 1 << 64 or not 0 <= site < 1 << 32 or not 0 <= step < 1 << 32 or not 0 <= first_row <= 1 << 32:
+            raise RtError(RT_ERR_INVALID, "Dropout: seed has 64 bits, site, step and first_row 32")
+        self.step_at = step_at
+        self._args = DropoutMask(p, seed, site, step, None, first_row)
+
+    p = property(lambda self: self._args.p)
+    seed = property(lambda self: self._args.seed)
+    site = property(lambda self: self._args.site)
+    step = property(lambda self: self._args.step)
+    first_row = property(lambda self: self._args.first_row)
+
+    @property
+    def args(self) -> DropoutMask:
+        """What a call passes on: step_at's handle as it is now, for the tensor may have been freed since."""
+        a, t = self._args, self.step_at
+        a.step_at = None if t is None else t.handle or _freed()
         return a
 
 
@@ -548,6 +612,58 @@ class Gpu:
     def mx4_matmul(self, a: Mx4Tensor, b: Mx4Tensor, c: GpuTensor, bias: GpuTensor | None = None, relu: bool = False):
         """C[m,n] = A[m,k] B[n,k]^T + bias, ReLU if asked."""
         _check(lib().rt_mx4_matmul(self.handle, a.handle, b.handle, c.handle, _handle(bias), int(relu)))
+
+    # --- block-scaled 8-bit matrices (new; rtgpu.h has the format)
+    def fp8_zeros(self, rows: int, k: int) -> Fp8Tensor:
+        h = C.c_void_p()
+        _check(lib().rt_fp8_zeros(self.handle, rows, k, C.byref(h)))
+        return Fp8Tensor(self, h.value)
+
+    def fp8_wrap(self, codes_ptr: int, scales_ptr: int, rows: int, k: int) -> Fp8Tensor:
+        """View of caller memory; Fp8Tensor.nbytes gives the sizes."""
+        h = C.c_void_p()
+        _check(lib().rt_fp8_wrap(self.handle, codes_ptr, scales_ptr, rows, k, C.byref(h)))
+        return Fp8Tensor(self, h.value)
+
+    def fp8_quantize(self, src: GpuTensor, dst: Fp8Tensor | None = None, axis: int = 1) -> Fp8Tensor:
+        """src in 8 bits with blocks along a row (axis 1), or down a column and
+        laid out transposed (axis 0)."""
+        if dst is None:
+            dst = self.fp8_zeros(*(src.shape if axis == 1 else src.shape[::-1]))
+        _check(lib().rt_fp8_quantize(self.handle, src.handle, axis, dst.handle))
+        return dst
+
+    def fp8_dequantize(self, q: Fp8Tensor, dst: GpuTensor):
+        _check(lib().rt_fp8_dequantize(self.handle, q.handle, dst.handle))
+
+    def fp8_matmul(self, a: Fp8Tensor, b: Fp8Tensor, c: GpuTensor, bias: GpuTensor | None = None, relu: bool = False):
+        """C[m,n] = A[m,k] B[n,k]^T + bias, ReLU if asked."""
+        _check(lib().rt_fp8_matmul(self.handle, a.handle, b.handle, c.handle, _handle(bias), int(relu)))
+
+    # --- embedding (new)
+    def embedding_forward(self, table: GpuTensor, tokens: GpuTensor, y: GpuTensor, scale: float = 1.0):
+        """y[i] = scale * table[tokens[i]]; tokens u32 (upload_labels), those past the table give zeros."""
+        _check(lib().rt_embedding_forward(self.handle, table.handle, tokens.handle, scale, y.handle))
+
+    def embedding_backward(self, tokens: GpuTensor, dy: GpuTensor, dtable: GpuTensor, work: GpuTensor, scale: float = 1.0,
+                           accumulate: bool = False):
+        """dtable[v] = scale * the sum of dy[i] over tokens[i] = v, or added to
+        what dtable holds; work embedding_backward_workspace(tokens, vocabulary, width) f32."""
+        _check(lib().rt_embedding_backward(self.handle, tokens.handle, dy.handle, scale, int(accumulate), dtable.handle,
+                                           work.handle))
+
+    @staticmethod
+    def embedding_backward_workspace(tokens: int, vocabulary: int, width: int) -> int:
+        v = lib().rt_embedding_backward_workspace(tokens, vocabulary, width)
+        if v < 0:
+            raise RtError(RT_ERR_INVALID, lib().rt_last_error().decode(errors="replace"))
+        return v
+
+    # --- dropout (new)
+    def dropout(self, x: GpuTensor, y: GpuTensor, mask: Dropout, add: GpuTensor | None = None):
+        """y = add + x / (1 - p) where the mask keeps x, add elsewhere.  The
+        gradient of x is the same call on that of y."""
+        _check(lib().rt_dropout(self.handle, x.handle, _handle(add), y.handle, C.byref(mask.args)))
 
     # --- residual-block norms (new)
     def block_forward(self, r: GpuTensor, *, y: GpuTensor | None = None, post: Norm | None = None,
