@@ -21,103 +21,153 @@
 namespace rt {
 namespace {
 
-constexpr int kVec = 8;               // elements of a lane
-constexpr int kSpan = 32 * kVec;      // and of a warp
+constexpr int64_t kMaxWidth = 1 << 22;  // spans fit a grid's second extent
 constexpr int64_t kMaxVocabulary = (1 << 21) - 1;  // keys 0 .. V fit 21 bits
 
-// A lane's eight neighbouring elements.  ALIGNED: by 16-byte accesses where all eight exist
-// (rows on 16 bytes); else a warp's accesses are neighbours, element lane + 32 i the i-th.
-template <typename T, bool ALIGNED>
+// A lane's N columns (4 or 8) of a warp's span of 32 N.  ACCESS: bytes that the rows are
+// aligned to, 32 or 16: neighbouring columns, by accesses of that width where all of them
+// exist; 0: a warp's accesses are neighbours, column lane + 32 i the lane's i-th.
+template <int ACCESS, int N>
+struct Columns {
+    static constexpr int SPAN = 32 * N, STEP = ACCESS ? 1 : 32;
+    int64_t first, n;  // the lane's first column, the row's length
+    bool all;          // the lane's neighbouring columns exist
+    __device__ __forceinline__ Columns(int64_t span, int64_t n, int lane)
+        : first(span * SPAN + lane * (ACCESS ? N : 1)), n(n), all(ACCESS && first + N <= n) {}
+};
+
+// The lane's elements of a row as they lie in memory, to be converted when they are used:
+// bf16 takes half the registers on its way.
+template <typename T, int ACCESS, int N>
 struct Lane {
-    static __device__ __forceinline__ int64_t at(int64_t j0, int i, int lane) {
-        return ALIGNED ? j0 + lane * kVec + i : j0 + i * 32 + lane;
+    using C = Columns<ACCESS, N>;
+    static constexpr int WORDS = N * sizeof(T) / 4;
+    static constexpr int WIDE = WORDS == 8 && ACCESS == 32 ? 8 : WORDS >= 4 ? 4 : 2;  // words of an access
+    uint32_t w[WORDS];
+
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 2) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else return __uint_as_float(w[i]);
     }
-    static __device__ __forceinline__ float one(const T* p) {
-        if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
-        else return *p;
-    }
-    static __device__ __forceinline__ void put(T* p, float v) {
-        if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(v);
-        else *p = v;
-    }
-    // of row p, from column j0 on, of n; NC: the kernel writes no row of p's matrix
+    // NC: the kernel writes no row of this matrix
     template <bool NC = true>
-    static __device__ __forceinline__ void load(const T* p, int64_t j0, int64_t n, int lane, float (&v)[kVec]) {
-        const int64_t j = j0 + lane * kVec;
-        if (ALIGNED && j + kVec <= n) {
-            if constexpr (sizeof(T) == 2) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + j));
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    __device__ __forceinline__ void load(const T* row, const C& c) {
+        const T* p = row + c.first;
+        if (c.all) {
+            if constexpr (WIDE == 8 && NC)
+                asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                             : "l"(p));
+            else if constexpr (WIDE >= 4)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            } else {
-                const float4* f = reinterpret_cast<const float4*>(p + j);
-                const float4 a = NC ? __ldg(f) : f[0], b = NC ? __ldg(f + 1) : f[1];
-                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+                for (int i = 0; i < WORDS; i += 4) {
+                    const uint4* q = reinterpret_cast<const uint4*>(p) + i / 4;
+                    const uint4 u = NC ? __ldg(q) : *q;
+                    w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+                }
+            else {
+                const uint2* q = reinterpret_cast<const uint2*>(p);
+                const uint2 u = NC ? __ldg(q) : *q;
+                w[0] = u.x, w[1] = u.y;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = at(j0, i, lane) < n ? one(p + at(j0, i, lane)) : 0.0f;
+            for (int i = 0; i < WORDS; ++i) w[i] = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (c.first + i * C::STEP < c.n) {
+                    if constexpr (sizeof(T) == 2) w[i / 2] |= (uint32_t)__bfloat16_as_ushort(p[i * C::STEP]) << (16 * (i & 1));
+                    else w[i] = __float_as_uint(p[i * C::STEP]);
+                }
         }
     }
-    static __device__ __forceinline__ void store(T* p, int64_t j0, int64_t n, int lane, const float (&v)[kVec]) {
-        const int64_t j = j0 + lane * kVec;
-        if (ALIGNED && j + kVec <= n) {
-            if constexpr (sizeof(T) == 2) {
-                uint32_t w[4];
+    static __device__ __forceinline__ void store(T* row, const C& c, const float (&v)[N]) {
+        T* p = row + c.first;
+        if (c.all) {
+            uint32_t u[WORDS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < WORDS; ++i) {
+                if constexpr (sizeof(T) == 2) {
                     const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    u[i] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    u[i] = __float_as_uint(v[i]);
                 }
-                *reinterpret_cast<uint4*>(p + j) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-                reinterpret_cast<float4*>(p + j)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(p + j)[1] = make_float4(v[4], v[5], v[6], v[7]);
             }
+            if constexpr (WIDE == 8)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]),
+                             "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                             : "memory");
+            else if constexpr (WIDE == 4)
+#pragma unroll
+                for (int i = 0; i < WORDS; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
+            else
+                *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
         } else {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i)
-                if (at(j0, i, lane) < n) put(p + at(j0, i, lane), v[i]);
+            for (int i = 0; i < N; ++i)
+                if (c.first + i * C::STEP < c.n) {
+                    if constexpr (sizeof(T) == 2) p[i * C::STEP] = __float2bfloat16_rn(v[i]);
+                    else p[i * C::STEP] = v[i];
+                }
         }
     }
 };
 
-// --------------------------------------------------------------------- forward
-// A warp takes kSpan columns of kRows positions, all their reads under way at once.
-constexpr int kRows = 4;
+// A CTA's eight warps lie over groups of rows and spans of columns: 2^along of them beside one
+// another, so that they read neighbouring parts of the same rows, gridDim.y such groups of
+// spans.  Shifts only: a division for each warp's place cost as much as its work.
+struct Lay {
+    int along;
+    dim3 grid;
+    Lay(int64_t groups, int64_t spans) : along(0) {
+        while (along < 3 && spans % (2 << along) == 0) ++along;
+        grid = dim3((unsigned)((groups + (8 >> along) - 1) / (8 >> along)), (unsigned)(spans >> along));
+    }
+};
+__device__ __forceinline__ int64_t lay_group(int along) {
+    return ((int64_t)blockIdx.x << (3 - along)) + (threadIdx.x >> (5 + along));
+}
+__device__ __forceinline__ int64_t lay_span(int along) {
+    return ((int64_t)blockIdx.y << along) + ((threadIdx.x >> 5) & ((1 << along) - 1));
+}
 
-template <typename TE, typename TY, bool ALIGNED>
+// --------------------------------------------------------------------- forward
+// A warp takes 256 columns of kRows positions, all their reads under way at once.
+constexpr int kRows = 4, kLookup = 8;
+
+template <typename TE, typename TY, int ACCESS>
 __global__ void __launch_bounds__(256) lookup_kernel(const TE* __restrict__ table, int64_t lde, int64_t vocabulary,
                                                      const uint32_t* __restrict__ tokens, int64_t count, int64_t n,
-                                                     int64_t spans, float scale, TY* __restrict__ y, int64_t ldy) {
+                                                     int along, float scale, TY* __restrict__ y, int64_t ldy) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int64_t units = (count + kRows - 1) / kRows * spans;
-    for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
-        const int64_t i0 = u / spans * kRows, j0 = u % spans * kSpan;
-        float v[kRows][kVec];
-        bool there[kRows];
+    const int64_t i0 = lay_group(along) * kRows;
+    const Columns<ACCESS, kLookup> c(lay_span(along), n, lane);
+    const int live = (int)max((int64_t)0, min((int64_t)kRows, count - i0));
+    Lane<TE, ACCESS, kLookup> e[kRows];
+    bool there[kRows];
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            const uint32_t token = i0 + r < count ? __ldg(tokens + i0 + r) : 0u;
-            there[r] = i0 + r < count && token < vocabulary;
-            if (there[r]) Lane<TE, ALIGNED>::load(table + token * lde, j0, n, lane, v[r]);
-        }
+    for (int r = 0; r < kRows; ++r) {
+        const uint32_t token = r < live ? __ldg(tokens + i0 + r) : 0u;
+        there[r] = r < live && token < vocabulary;
+        if (there[r]) e[r].load(table + token * lde, c);
+    }
+    TY* to = y + i0 * ldy;
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            if (i0 + r >= count) break;
+    for (int r = 0; r < kRows; ++r, to += ldy) {
+        if (r >= live) break;
+        float v[kLookup];
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[r][i] = there[r] ? v[r][i] * scale : 0.0f;
-            Lane<TY, ALIGNED>::store(y + (i0 + r) * ldy, j0, n, lane, v[r]);
-        }
+        for (int i = 0; i < kLookup; ++i) v[i] = there[r] ? e[r].value(i) * scale : 0.0f;
+        Lane<TY, ACCESS, kLookup>::store(to, c, v);
     }
 }
 
 // -------------------------------------------------------------------- backward
 // The workspace, in 32-bit words.  B: CTAs of the first pass; bins: buckets; a run's
-// partial sums: two rows of `width` floats (n rounded up to kVec) a piece.
+// partial sums: two rows of `width` floats (n rounded up to 8) a piece.
 struct Sort {
     int64_t count, vocabulary;
     int low, high;       // bits of a key: bucket high, order in it low
@@ -132,23 +182,11 @@ struct Sort {
     uint32_t* start;     // [vocabulary + 1] first of each token in the sorted list
 };
 
-constexpr int kSortThreads = 256, kSortWarps = 8;
 constexpr int kMaxHigh = 11, kMaxLow = 10;
 
 __device__ __forceinline__ uint32_t key_of(const Sort& s, const uint32_t* tokens, int64_t i) {
     return min(__ldg(tokens + i), (uint32_t)s.vocabulary);
 }
-
-// Each warp of a CTA owns neighbouring elements of [first, first + n) and a row of
-// counters; both passes below go over them 32 at a time, in order.
-struct Share {
-    int64_t begin, end;
-    __device__ __forceinline__ Share(int64_t n, int warp) {
-        const int64_t each = (n + kSortWarps * 32 - 1) / (kSortWarps * 32) * 32;
-        begin = min(n, warp * each);
-        end = min(n, begin + each);
-    }
-};
 
 // cnt[digit] += how many lanes have it; returns the lane's rank: those of this warp before it.
 __device__ __forceinline__ uint32_t count_rank(uint32_t* cnt, uint32_t digit, bool there, int lane) {
@@ -164,23 +202,40 @@ __device__ __forceinline__ uint32_t count_rank(uint32_t* cnt, uint32_t digit, bo
     return before + __popc(same & ((1u << lane) - 1));
 }
 
+// Each warp of a CTA owns neighbouring elements of [0, n) and goes over them in order, 32
+// at a time: f(rank's digit counter row, index, there).  Four keys are under way at once.
+template <int WARPS, typename Key, typename Each>
+__device__ __forceinline__ void in_order(int64_t n, int warp, int lane, Key key, Each each) {
+    const int64_t share = (n + WARPS * 32 - 1) / (WARPS * 32) * 32;
+    const int64_t begin = min(n, warp * share), end = min(n, begin + share);
+    for (int64_t i = begin; i < end; i += 128) {
+        uint32_t k[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) k[x] = i + x * 32 + lane < end ? key(i + x * 32 + lane) : 0u;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (i + x * 32 < end) each(i + x * 32 + lane, k[x], i + x * 32 + lane < end);
+    }
+}
+
 // How many positions of each CTA's span fall in each bucket.
-__global__ void __launch_bounds__(kSortThreads) bucket_count_kernel(Sort s, const uint32_t* __restrict__ tokens) {
+__global__ void __launch_bounds__(256) bucket_count_kernel(Sort s, const uint32_t* __restrict__ tokens) {
     extern __shared__ uint32_t cnt[];
     pdl_wait();
     pdl_launch_dependents();
     const int bins = 1 << s.high;
-    for (int i = threadIdx.x; i < bins; i += kSortThreads) cnt[i] = 0;
+    for (int i = threadIdx.x; i < bins; i += 256) cnt[i] = 0;
     __syncthreads();
     const int64_t first = blockIdx.x * s.span, n = min(s.span, s.count - first);
-    for (int64_t i = threadIdx.x; i < n; i += kSortThreads) atomicAdd(&cnt[key_of(s, tokens, first + i) >> s.low], 1u);
+    for (int64_t i = threadIdx.x; i < n; i += 256) atomicAdd(&cnt[key_of(s, tokens, first + i) >> s.low], 1u);
     __syncthreads();
-    for (int i = threadIdx.x; i < bins; i += kSortThreads) s.counts[(int64_t)blockIdx.x * bins + i] = cnt[i];
+    for (int i = threadIdx.x; i < bins; i += 256) s.counts[(int64_t)blockIdx.x * bins + i] = cnt[i];
 }
 
-// Exclusive sums of v[0..bins) in place, by the whole CTA (bins a multiple of nothing in particular).
+// Exclusive sums of v[0..bins) in place, by the whole CTA; sums holds a word a warp.
+template <int WARPS>
 __device__ __forceinline__ void exclusive(uint32_t* v, int bins, uint32_t* sums) {
-    const int each = (bins + kSortThreads - 1) / kSortThreads, b = threadIdx.x * each, e = min(bins, b + each);
+    const int each = (bins + WARPS * 32 - 1) / (WARPS * 32), b = min(bins, (int)threadIdx.x * each), e = min(bins, b + each);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t own = 0;
     for (int i = b; i < e; ++i) own += v[i];
@@ -202,247 +257,493 @@ __device__ __forceinline__ void exclusive(uint32_t* v, int bins, uint32_t* sums)
     __syncthreads();
 }
 
-// Deals the positions out to their buckets, in order.  A CTA adds up the other CTAs'
-// counts itself.
-__global__ void __launch_bounds__(kSortThreads) bucket_deal_kernel(Sort s, const uint32_t* __restrict__ tokens) {
+// Deals the positions out to their buckets, in order.  A CTA adds up the CTAs' counts
+// itself: with at most 256 of them that is cheaper than a launch that does it once.
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) bucket_deal_kernel(Sort s, const uint32_t* __restrict__ tokens) {
     extern __shared__ uint32_t shared[];
+    constexpr int THREADS = WARPS * 32;
     const int bins = 1 << s.high;
-    uint32_t* base = shared;              // [bins]
-    uint32_t* cnt = shared + bins;        // [warps][bins]
-    __shared__ uint32_t sums[kSortWarps];
+    uint32_t* base = shared;         // [bins] of the whole list
+    uint32_t* own = base + bins;     // [bins] of the CTAs before this one
+    uint32_t* cnt = own + bins;      // [warps][bins]
+    __shared__ uint32_t sums[WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int b = threadIdx.x; b < bins * (WARPS + 2); b += THREADS) shared[b] = 0;
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int b = threadIdx.x; b < bins; b += kSortThreads) {
+    const int parts = max(1, THREADS / bins);
+    for (int i = threadIdx.x; i < bins * parts; i += THREADS) {
+        const int b = i & (bins - 1), part = i >> s.high;
         uint32_t all = 0, before = 0;
-        for (int c = 0; c < s.ctas; ++c) {
+#pragma unroll 8
+        for (int c = part; c < s.ctas; c += parts) {
             const uint32_t x = s.counts[(int64_t)c * bins + b];
-            if (c < (int)blockIdx.x) before += x;
             all += x;
+            if (c < (int)blockIdx.x) before += x;
         }
-        base[b] = all;
-        cnt[b] = before;
-#pragma unroll
-        for (int w = 1; w < kSortWarps; ++w) cnt[w * bins + b] = 0;
+        atomicAdd(&base[b], all);
+        atomicAdd(&own[b], before);
     }
-    __syncthreads();
-    exclusive(base, bins, sums);
-    for (int b = threadIdx.x; b < bins; b += kSortThreads) {
-        if (blockIdx.x == 0) s.bucket[b] = base[b];
-        base[b] += cnt[b];
-        cnt[b] = 0;
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) s.bucket[bins] = (uint32_t)s.count;
-    __syncthreads();
     const int64_t first = blockIdx.x * s.span, n = min(s.span, s.count - first);
-    const Share own(n, warp);
     uint32_t* mine = cnt + warp * bins;
-    for (int64_t i = own.begin; i < own.end; i += 32) {
-        const bool there = i + lane < own.end;
-        count_rank(mine, there ? key_of(s, tokens, first + i + lane) >> s.low : 0u, there, lane);
-    }
+    auto key = [&](int64_t i) { return key_of(s, tokens, first + i); };
+    in_order<WARPS>(n, warp, lane, key, [&](int64_t, uint32_t k, bool there) { count_rank(mine, k >> s.low, there, lane); });
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kSortThreads) {
+    exclusive<WARPS>(base, bins, sums);
+    for (int b = threadIdx.x; b < bins; b += THREADS) {
         uint32_t run = base[b];
+        if (blockIdx.x == 0) s.bucket[b] = run;
+        run += own[b];
 #pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const uint32_t x = cnt[w * bins + b];
             cnt[w * bins + b] = run;
             run += x;
         }
     }
+    if (blockIdx.x == 0 && threadIdx.x == 0) s.bucket[bins] = (uint32_t)s.count;
     __syncthreads();
-    for (int64_t i = own.begin; i < own.end; i += 32) {
-        const bool there = i + lane < own.end;
-        const uint32_t key = there ? key_of(s, tokens, first + i + lane) : 0u;
-        const uint32_t to = count_rank(mine, key >> s.low, there, lane);
+    in_order<WARPS>(n, warp, lane, key, [&](int64_t i, uint32_t k, bool there) {
+        const uint32_t to = count_rank(mine, k >> s.low, there, lane);
         if (there) {
-            s.key[to] = key;
-            s.place[to] = (uint32_t)(first + i + lane);
+            s.key[to] = k;
+            s.place[to] = (uint32_t)(first + i);
         }
-    }
+    });
 }
 
 // Sorts a bucket by the low bits and writes where each of its tokens starts.
-__global__ void __launch_bounds__(kSortThreads) bucket_sort_kernel(Sort s) {
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) bucket_sort_kernel(Sort s) {
     extern __shared__ uint32_t shared[];
+    constexpr int THREADS = WARPS * 32;
     const int bins = 1 << s.low;
     uint32_t* base = shared;        // [bins]
     uint32_t* cnt = shared + bins;  // [warps][bins]
-    __shared__ uint32_t sums[kSortWarps];
+    __shared__ uint32_t sums[WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int b = threadIdx.x; b < bins * WARPS; b += THREADS) cnt[b] = 0;
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t first = s.bucket[blockIdx.x], n = s.bucket[blockIdx.x + 1] - first;
-    for (int b = threadIdx.x; b < bins * kSortWarps; b += kSortThreads) cnt[b] = 0;
-    __syncthreads();
-    const Share own(n, warp);
     uint32_t* mine = cnt + warp * bins;
     const uint32_t mask = (uint32_t)bins - 1;
-    for (int64_t i = own.begin; i < own.end; i += 32) {
-        const bool there = i + lane < own.end;
-        count_rank(mine, there ? s.key[first + i + lane] & mask : 0u, there, lane);
-    }
+    auto key = [&](int64_t i) { return s.key[first + i]; };
+    in_order<WARPS>(n, warp, lane, key, [&](int64_t, uint32_t k, bool there) { count_rank(mine, k & mask, there, lane); });
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kSortThreads) {
+    for (int b = threadIdx.x; b < bins; b += THREADS) {
         uint32_t all = 0;
 #pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) all += cnt[w * bins + b];
+        for (int w = 0; w < WARPS; ++w) all += cnt[w * bins + b];
         base[b] = all;
     }
     __syncthreads();
-    exclusive(base, bins, sums);
-    for (int b = threadIdx.x; b < bins; b += kSortThreads) {
+    exclusive<WARPS>(base, bins, sums);
+    for (int b = threadIdx.x; b < bins; b += THREADS) {
         uint32_t run = (uint32_t)first + base[b];
         const int64_t token = ((int64_t)blockIdx.x << s.low) + b;
         if (token <= s.vocabulary) s.start[token] = run;
 #pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const uint32_t x = cnt[w * bins + b];
             cnt[w * bins + b] = run;
             run += x;
         }
     }
     __syncthreads();
-    for (int64_t i = own.begin; i < own.end; i += 32) {
-        const bool there = i + lane < own.end;
-        const uint32_t key = there ? s.key[first + i + lane] : 0u, place = there ? s.place[first + i + lane] : 0u;
-        const uint32_t to = count_rank(mine, key & mask, there, lane);
+    in_order<WARPS>(n, warp, lane, key, [&](int64_t i, uint32_t k, bool there) {
+        const uint32_t to = count_rank(mine, k & mask, there, lane);
         if (there) {
-            s.token[to] = key;
-            s.position[to] = place;
+            s.token[to] = k;
+            s.position[to] = s.place[first + i];
         }
-    }
+    });
 }
 
-// The sums.  A warp takes kSpan columns of a piece of kCut positions, or of 32 rows of dE
-// that are looked over for tokens that do not occur.
-constexpr int kCut = 64, kEmpty = 32;
+// The whole sort in one launch where the positions fit the shared memory of one cluster:
+// a CTA holds kChunk of them, and passes by 8 bits of the key, the low ones first, move
+// them through distributed shared memory.  65536 positions of 50257 tokens: about 10 us; the
+// launches above take 25.
+constexpr int kChunk = 4096, kMaxCluster = 16, kStride = 257;  // kStride: counters of a warp, off a bank each
+
+struct ClusterSmem {
+    uint2 item[kChunk];  // key, position
+    uint32_t cnt[32 * kStride];
+    uint32_t hist[256], base[256], sums[8];
+    uint32_t gaps;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sync_cluster() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32_t* __restrict__ tokens, int passes) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    ClusterSmem& m = *reinterpret_cast<ClusterSmem*>(raw);
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), ranks = cluster_size();
+    const int64_t first = (int64_t)rank * kChunk;
+    const int live = (int)max((int64_t)0, min((int64_t)kChunk, s.count - first));  // positions of this CTA
+    uint2 item[4];
+    const int slot = warp * 128 + lane;  // of the thread's first item; the others 32 apart
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+        if (slot + x * 32 < live) item[x] = make_uint2(key_of(s, tokens, first + slot + x * 32), (uint32_t)first + slot + x * 32);
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * 8;
+        for (int i = threadIdx.x; i < 32 * kStride; i += 1024) m.cnt[i] = 0;
+        if (pass)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (slot + x * 32 < live) item[x] = m.item[slot + x * 32];
+        __syncthreads();
+        uint32_t before[4];  // of the item's digit: items before it in its warp
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            before[x] = count_rank(m.cnt + warp * kStride, item[x].x >> shift & 255u, slot + x * 32 < live, lane);
+        __syncthreads();
+        // the warps' counters to exclusive sums over the warps: four threads a digit, eight warps each
+        const int digit = threadIdx.x >> 2, part = threadIdx.x & 3;
+        uint32_t c[8], own = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            c[w] = m.cnt[(part * 8 + w) * kStride + digit];
+            own += c[w];
+        }
+        uint32_t upto = own;
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (part >= o) upto += x;
+        }
+        if (part == 3) m.hist[digit] = upto;
+        uint32_t run = upto - own;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            m.cnt[(part * 8 + w) * kStride + digit] = run;
+            run += c[w];
+        }
+        sync_cluster();  // every CTA's items are in registers, its counts in hist
+        uint32_t all = 0, earlier = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxCluster / 4; ++i) {
+            const uint32_t r = part + i * 4;
+            const uint32_t x = r < ranks ? ld_cluster(in_cta(&m.hist[digit], r)) : 0u;
+            all += x;
+            if (r < rank) earlier += x;
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) {
+            all += __shfl_xor_sync(0xffffffffu, all, o);
+            earlier += __shfl_xor_sync(0xffffffffu, earlier, o);
+        }
+        // exclusive sums over the digits: a warp has eight of them
+        uint32_t in = part == 0 ? all : 0u;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, in, o);
+            if (lane >= o) in += x;
+        }
+        if (lane == 31) m.cnt[warp * kStride + 256] = in;  // the word between two warps' counters
+        __syncthreads();
+        uint32_t lower = 0;
+        if (lane < warp) lower = m.cnt[lane * kStride + 256];
+#pragma unroll
+        for (int o = 16; o; o /= 2) lower += __shfl_xor_sync(0xffffffffu, lower, o);
+        if (part == 0) m.base[digit] = lower + in - all + earlier;
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (slot + x * 32 < live) {
+                const uint32_t d = item[x].x >> shift & 255u, to = m.base[d] + m.cnt[warp * kStride + d] + before[x];
+                const uint32_t at = in_cta(&m.item[to % kChunk], to / kChunk);
+                asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(item[x].x), "r"(item[x].y) : "memory");
+            }
+        sync_cluster();
+    }
+    // sorted: token and position out; where tokens start from the places where the key changes
+    if (threadIdx.x == 0) m.gaps = 0;
+    const uint32_t previous = rank && live ? ld_cluster(in_cta(&m.item[kChunk - 1], rank - 1)) : 0u;
+    __syncthreads();
+    uint32_t* list = m.cnt;  // places of wide gaps
+    static_assert(32 * kStride >= kChunk + 1, "every place fits the list");
+    for (int i = threadIdx.x; i < live; i += 1024) {
+        const uint2 now = m.item[i];
+        s.token[first + i] = now.x;
+        s.position[first + i] = now.y;
+        const int64_t from = first + i == 0 ? 0 : (int64_t)(i ? m.item[i - 1].x : previous) + 1;
+        if ((int64_t)now.x - from >= 8)
+            list[atomicAdd(&m.gaps, 1u)] = i;
+        else
+            for (int64_t t = from; t <= now.x; ++t) s.start[t] = (uint32_t)(first + i);
+    }
+    const bool last = first + live == s.count && (live || s.count == 0) && (live || rank == 0);
+    if (last && threadIdx.x == 0) list[atomicAdd(&m.gaps, 1u)] = live;  // the tokens behind the last
+    __syncthreads();
+    const int gaps = (int)m.gaps;
+    for (int g = warp; g < gaps; g += 32) {
+        const int i = (int)list[g];
+        const int64_t from = first + i == 0 ? 0 : (int64_t)(i ? m.item[i - 1].x : previous) + 1;
+        const int64_t to = i < live ? (int64_t)m.item[i].x : s.vocabulary;
+        for (int64_t t = from + lane; t <= to; t += 32) s.start[t] = (uint32_t)(first + i);
+    }
+    sync_cluster();  // a CTA's last item is read by the next one
+}
+
+// The rows of dE whose tokens do not occur: zeros.  A CTA marks the tokens of its share of
+// the rows by going over all positions itself, so it needs no sort, and this kernel runs beside
+// the last kernel of the sort, on the SMs that one leaves idle: it waits for it at its
+// end only (65536 positions leave 132 SMs idle for 25 us, the time of 130 MB).
+constexpr int kMarks = 8192;  // rows at a time
+
+template <int ACCESS>
+__global__ void __launch_bounds__(1024) fill_kernel(const uint32_t* __restrict__ tokens, int64_t count, int64_t vocabulary,
+                                                    float* __restrict__ out, int64_t ldo, int64_t n) {
+    __shared__ uint8_t marks[kMarks];
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t begin = vocabulary * blockIdx.x / gridDim.x, end = vocabulary * (blockIdx.x + 1) / gridDim.x;
+    for (int64_t b = begin; b < end; b += kMarks) {
+        const uint32_t rows = (uint32_t)min(end - b, (int64_t)kMarks);
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < rows; i += 1024) marks[i] = 0;
+        __syncthreads();
+        auto mark = [&](uint32_t token) {
+            if (token - (uint32_t)b < rows) marks[token - (uint32_t)b] = 1;
+        };
+        const int64_t lead = min(count, (int64_t)((16 - (reinterpret_cast<uintptr_t>(tokens) & 15)) & 15) / 4);
+        const int64_t quads = (count - lead) / 4;
+        const uint4* four = reinterpret_cast<const uint4*>(tokens + lead);
+#pragma unroll 8
+        for (int64_t i = threadIdx.x; i < quads; i += 1024) {
+            const uint4 t = __ldg(four + i);
+            mark(t.x), mark(t.y), mark(t.z), mark(t.w);
+        }
+        if (threadIdx.x < lead) mark(tokens[threadIdx.x]);
+        if (threadIdx.x < count - lead - quads * 4) mark(tokens[lead + quads * 4 + threadIdx.x]);
+        __syncthreads();
+        const float zero[8] = {};
+        for (uint32_t r = warp; r < rows; r += 32) {
+            if (marks[r]) continue;
+            float* row = out + (b + r) * ldo;
+            for (int64_t j = 0; j * 256 < n; ++j) Lane<float, ACCESS, 8>::store(row, Columns<ACCESS, 8>(j, n, lane), zero);
+        }
+    }
+    pdl_wait();
+}
+
+// The sums.  A token that occurs at most kCut times is light: a warp takes 512 bytes' columns of
+// kTokens neighbouring rows of dE, whose positions lie one after another, and writes each
+// row once, the rows of tokens that do not occur as zeros.  The others are heavy: the sorted
+// list is cut into pieces of kCut positions whatever the tokens, so a heavy run crosses
+// pieces; each leaves a partial sum of it, and join_kernel adds these in order.
+constexpr int kCut = 64, kTokens = 8;
+static_assert(kTokens < 32, "a lane reads where the next row starts");
+
+// Columns of a lane: 16 bytes of dy.
+template <typename T>
+constexpr int kColumns = 16 / (int)sizeof(T);
 
 struct Sums {
     int64_t count, vocabulary, n, spans, width;
     int64_t pieces;
+    int along;         // Lay's
+    int piece_blocks;  // CTAs in front that take pieces
     const uint32_t* token;
     const uint32_t* position;
     const uint32_t* start;
-    float* partial;  // [pieces][2][width]: the run that began in an earlier piece, the one that goes on in the next
+    float* partial;  // [pieces][2][width]: the heavy run that began in an earlier piece, the one that began in this one
     float scale;
     int accumulate;
     float* out;
     int64_t ldo;
 };
 
-template <bool ALIGNED>
-__device__ __forceinline__ void emit(const Sums& s, uint32_t token, int64_t j0, int lane, float (&v)[kVec]) {
+template <int ACCESS, int N>
+__device__ __forceinline__ void emit(const Sums& s, uint32_t token, const Columns<ACCESS, N>& c, float (&v)[N]) {
+    using L = Lane<float, ACCESS, N>;
     float* row = s.out + token * s.ldo;
-    float old[kVec];
-    if (s.accumulate) Lane<float, ALIGNED>::template load<false>(row, j0, s.n, lane, old);
+    if (s.accumulate) {
+        L old;
+        old.template load<false>(row, c);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = s.accumulate ? old[i] + v[i] * s.scale : v[i] * s.scale;
-    Lane<float, ALIGNED>::store(row, j0, s.n, lane, v);
+        for (int i = 0; i < N; ++i) v[i] = old.value(i) + v[i] * s.scale;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= s.scale;
+    }
+    L::store(row, c, v);
 }
 
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) sum_kernel(Sums s, const T* __restrict__ dy, int64_t ldy, int64_t units,
-                                                  int64_t piece_units) {
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(256, 4) sum_kernel(Sums s, const T* __restrict__ dy, int64_t ldy) {
     pdl_wait();
     pdl_launch_dependents();
-    constexpr int U = sizeof(T) == 2 ? 8 : 4;  // rows of dy under way
+    constexpr int N = kColumns<T>, U = 4;  // U: rows of dy under way
+    using L = Lane<T, ACCESS, N>;
     const int lane = threadIdx.x & 31;
-    const int64_t real = s.start[s.vocabulary];  // positions that hold a token
-    for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
-        if (u >= piece_units) {
-            const int64_t r0 = (u - piece_units) / s.spans * kEmpty, j0 = (u - piece_units) % s.spans * kSpan;
-            const int64_t r = r0 + lane;
-            uint32_t empty = __ballot_sync(0xffffffffu, r < s.vocabulary && s.start[r] == s.start[r + 1]);
-            const float zero[kVec] = {};
-            for (; empty; empty &= empty - 1)
-                Lane<float, ALIGNED>::store(s.out + (r0 + __ffs(empty) - 1) * s.ldo, j0, s.n, lane, zero);
-            continue;
-        }
-        const int64_t piece = u / s.spans, j0 = u % s.spans * kSpan, p0 = piece * kCut, p1 = min(real, p0 + kCut);
-        if (p0 >= p1) continue;
-        const uint32_t before = p0 ? s.token[p0 - 1] : 0xffffffffu, after = p1 < real ? s.token[p1] : 0xffffffffu;
-        uint32_t token[2], position[2];
+    const Columns<ACCESS, N> c(lay_span(s.along), s.n, lane);
+    if ((int)blockIdx.x < s.piece_blocks) {
+        const int64_t real = s.start[s.vocabulary];  // positions that hold a token
+        const int64_t piece = lay_group(s.along), p0 = piece * kCut, p1 = min(real, p0 + kCut);
+        if (p0 >= p1) return;
+        // a heavy run holds the piece's first position or its last
+        const uint32_t ends[2] = {s.token[p0], s.token[p1 - 1]};
+        for (int h = 0; h < (ends[0] == ends[1] ? 1 : 2); ++h) {
+            const int64_t run0 = s.start[ends[h]], run1 = s.start[ends[h] + 1];
+            if (run1 - run0 <= kCut) continue;
+            const int64_t begin = max(run0, p0), end = min(run1, p1);
+            float sum[N] = {};
+            for (int64_t q = begin; q < end; q += 32) {
+                const uint32_t position = q + lane < end ? s.position[q + lane] : 0u;
+                const int live = (int)min((int64_t)32, end - q);
+                for (int g = 0; g < live; g += U) {
+                    L v[U];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t p = p0 + h * 32 + lane;
-            token[h] = p < p1 ? s.token[p] : 0xffffffffu;
-            position[h] = p < p1 ? s.position[p] : 0u;
+                    for (int x = 0; x < U; ++x) {
+                        const uint32_t row = __shfl_sync(0xffffffffu, position, (g + x) & 31);
+                        if (g + x < live) v[x].load(dy + row * ldy, c);
+                    }
+#pragma unroll
+                    for (int x = 0; x < U; ++x)
+                        if (g + x < live)
+#pragma unroll
+                            for (int i = 0; i < N; ++i) sum[i] += v[x].value(i);
+                }
+            }
+            Lane<float, ACCESS, N>::store(s.partial + (piece * 2 + (run0 < p0 ? 0 : 1)) * s.width, c, sum);
         }
-        const int live = (int)(p1 - p0);
-        float sum[kVec] = {};
-        uint32_t run = __shfl_sync(0xffffffffu, token[0], 0);
-        bool carried = run == before;  // the run began in an earlier piece
+        return;
+    }
+    const int64_t t0 = (lay_group(s.along) - ((int64_t)s.piece_blocks << (3 - s.along))) * kTokens;
+    if (t0 >= s.vocabulary) return;
+    const int64_t token = min(t0 + min(lane, kTokens), s.vocabulary);
+    const uint32_t first = s.start[token], next = __shfl_down_sync(0xffffffffu, first, 1);
+    const uint32_t count = lane < kTokens && token < s.vocabulary ? next - first : 0u;
+    const uint32_t light = count <= kCut ? count : 0u;
+    uint32_t upto = light;  // light positions of the rows up to the lane's
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, upto, 31);
+    float sum[N] = {};
+    int run = -1;
+    for (uint32_t e0 = 0; e0 < total; e0 += 32) {
+        // lane: the e-th light position, of row t0 + of: the first row with upto > e
+        const uint32_t e = e0 + lane;
+        int of = 0;
+#pragma unroll
+        for (int step = 16; step; step /= 2) {
+            const uint32_t x = __shfl_sync(0xffffffffu, upto, of + step - 1);
+            if (x <= e) of += step;
+        }
+        const uint32_t at = __shfl_sync(0xffffffffu, first, of) + e - (__shfl_sync(0xffffffffu, upto, of) - __shfl_sync(0xffffffffu, light, of));
+        const uint32_t position = e < total ? s.position[at] : 0u;
+        const int live = (int)min(32u, total - e0);
         for (int g = 0; g < live; g += U) {
-            float v[U][kVec];
-            uint32_t t[U];
+            L v[U];
+            int t[U];
 #pragma unroll
             for (int x = 0; x < U; ++x) {
-                const int at = g + x;
-                t[x] = __shfl_sync(0xffffffffu, at < 32 ? token[0] : token[1], at & 31);
-                const uint32_t row = __shfl_sync(0xffffffffu, at < 32 ? position[0] : position[1], at & 31);
-                if (at < live) Lane<T, ALIGNED>::load(dy + row * ldy, j0, s.n, lane, v[x]);
+                t[x] = __shfl_sync(0xffffffffu, of, (g + x) & 31);
+                const uint32_t row = __shfl_sync(0xffffffffu, position, (g + x) & 31);
+                if (g + x < live) v[x].load(dy + row * ldy, c);
             }
 #pragma unroll
             for (int x = 0; x < U; ++x) {
                 if (g + x >= live) break;
                 if (t[x] != run) {
-                    if (carried)
-                        Lane<float, ALIGNED>::store(s.partial + piece * 2 * s.width, j0, s.width, lane, sum);
-                    else
-                        emit<ALIGNED>(s, run, j0, lane, sum);
-                    carried = false;
+                    if (run >= 0) emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
                     run = t[x];
 #pragma unroll
-                    for (int i = 0; i < kVec; ++i) sum[i] = 0.0f;
+                    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
                 }
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) sum[i] += v[x][i];
+                for (int i = 0; i < N; ++i) sum[i] += v[x].value(i);
             }
         }
-        if (carried)
-            Lane<float, ALIGNED>::store(s.partial + piece * 2 * s.width, j0, s.width, lane, sum);
-        else if (run == after)
-            Lane<float, ALIGNED>::store(s.partial + (piece * 2 + 1) * s.width, j0, s.width, lane, sum);
-        else
-            emit<ALIGNED>(s, run, j0, lane, sum);
     }
+    if (run >= 0) emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
 }
 
-// Adds the partial sums of the runs that begin in piece blockIdx.x / spans and go on: its
-// second row and the first rows of the pieces that follow, dealt out over the CTA's warps
-// in order.
-template <bool ALIGNED>
+// Adds the partial sums of the heavy runs that begin in the CTA's kJoin pieces: a run's
+// second row there and the first rows of the pieces that follow, dealt out over the CTA's
+// warps in order.
+constexpr int kJoin = 16;
+
+template <int ACCESS, int N>
 __global__ void __launch_bounds__(256) join_kernel(Sums s) {
-    __shared__ float part[8][kSpan];
+    using L = Lane<float, ACCESS, N>;
+    __shared__ float part[8][32 * N];
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t real = s.start[s.vocabulary];
-    const int64_t piece = blockIdx.x / s.spans, j0 = blockIdx.x % s.spans * kSpan, end = (piece + 1) * kCut;
-    if (end >= real) return;
-    const uint32_t token = s.token[end - 1];
-    if (s.token[end] != token || s.start[token] < piece * kCut) return;
-    const int64_t last = (s.start[token + 1] - 1) / kCut, count = last - piece + 1, each = (count + 7) / 8;
-    const int64_t b = min(count, warp * each), e = min(count, b + each);
-    float sum[kVec] = {};
-    for (int64_t c = b; c < e; ++c) {
-        float v[kVec];
-        const float* row = s.partial + ((piece + c) * 2 + (c == 0 ? 1 : 0)) * s.width;
-        Lane<float, ALIGNED>::load(row, j0, s.width, lane, v);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) sum[i] += v[i];
+    const int64_t piece0 = (int64_t)blockIdx.x * kJoin;
+    const Columns<ACCESS, N> c(blockIdx.y, s.n, lane);
+    // every warp looks at the last position of each of the pieces
+    const int64_t end = (piece0 + lane + 1) * kCut;
+    uint32_t token = 0;
+    int64_t first = 0, next = 0;
+    bool begins = lane < kJoin && end < real;
+    if (begins) {
+        token = s.token[end - 1];
+        first = s.start[token], next = s.start[token + 1];
+        begins = next > end && first >= end - kCut && next - first > kCut;
     }
+    for (uint32_t found = __ballot_sync(0xffffffffu, begins); found; found &= found - 1) {
+        const int of = __ffs(found) - 1;
+        const int64_t piece = piece0 + of, last = (__shfl_sync(0xffffffffu, next, of) - 1) / kCut;
+        const int64_t count = last - piece + 1, each = (count + 7) / 8;
+        const int64_t b = min(count, warp * each), e = min(count, b + each);
+        float sum[N] = {};
+#pragma unroll 4
+        for (int64_t q = b; q < e; ++q) {
+            L v;
+            const float* row = s.partial + ((piece + q) * 2 + (q == 0 ? 1 : 0)) * s.width;
+            v.load(row, c);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) part[warp][i * 32 + lane] = sum[i];
-    __syncthreads();
-    if (warp) return;
-    const int64_t used = (count + each - 1) / each;
-    for (int w = 1; w < used; ++w)
+            for (int i = 0; i < N; ++i) sum[i] += v.value(i);
+        }
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) sum[i] += part[w][i * 32 + lane];
-    emit<ALIGNED>(s, token, j0, lane, sum);
+        for (int i = 0; i < N; ++i) part[warp][i * 32 + lane] = sum[i];
+        __syncthreads();
+        if (warp == 0) {
+            const int64_t used = (count + each - 1) / each;
+            for (int w = 1; w < used; ++w)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += part[w][i * 32 + lane];
+            emit<ACCESS, N>(s, __shfl_sync(0xffffffffu, token, of), c, sum);
+        }
+        __syncthreads();
+    }
 }
 
 int bits_of(int64_t v) {
@@ -463,7 +764,7 @@ int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) 
     s->ctas = (int)std::min<int64_t>(256, std::max<int64_t>(1, (count + 1023) / 1024));
     s->span = (count + s->ctas - 1) / s->ctas;
     m->pieces = (count + kCut - 1) / kCut;
-    m->width = (n + kVec - 1) / kVec * kVec;
+    m->width = (n + 7) / 8 * 8;
     auto words = [](int64_t v) { return (v + 31) / 32 * 32; };
     int64_t at = 0;
     uint32_t* base = s->counts;
@@ -487,37 +788,53 @@ int check_backward(int64_t count, int64_t vocabulary, int64_t n) {
     RT_CHECK(count >= 0 && vocabulary >= 0 && n >= 0, "embedding: negative extent");
     RT_CHECK(count <= INT_MAX, "embedding: %lld positions are over 2^31 - 1", (long long)count);
     RT_CHECK(vocabulary <= kMaxVocabulary, "embedding: the gradient of %lld tokens is over 2^21 - 1", (long long)vocabulary);
-    RT_CHECK(n <= (int64_t)1 << 31, "embedding: %lld columns are over 2^31", (long long)n);
+    RT_CHECK(n <= kMaxWidth, "embedding: %lld columns are over 2^22", (long long)n);
     return RT_OK;
 }
 
-bool aligned(const rt_tensor* t) {
-    return ((reinterpret_cast<uintptr_t>(t->ptr) | (uintptr_t)(t->ld * (int64_t)dtype_size(t->dtype))) & 15) == 0;
+// Bytes that every row of t is aligned to: 32, 16 or 0.
+int access_of(const rt_tensor* t) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t->ptr) | (uintptr_t)(t->ld * (int64_t)dtype_size(t->dtype));
+    return (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 0;
 }
 
 template <typename TE, typename TY>
 int launch_lookup(rt_ctx* ctx, const rt_tensor* table, const rt_tensor* tokens, float scale, rt_tensor* y) {
-    const int64_t spans = (y->cols + kSpan - 1) / kSpan, units = (y->rows + kRows - 1) / kRows * spans;
-    const int64_t grid = std::min<int64_t>((units + 7) / 8, (int64_t)ctx->sm_count * 64);
-    auto* kernel = aligned(table) && aligned(y) ? lookup_kernel<TE, TY, true> : lookup_kernel<TE, TY, false>;
-    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)grid, 256, 0, ctx->stream, static_cast<const TE*>(table->ptr), table->ld,
-                     table->rows, static_cast<const uint32_t*>(tokens->ptr), y->rows, y->cols, spans, scale,
+    const Lay lay((y->rows + kRows - 1) / kRows, (y->cols + 32 * kLookup - 1) / (32 * kLookup));
+    const int access = std::min(access_of(table), access_of(y));
+    auto* kernel = access == 32   ? lookup_kernel<TE, TY, 32>
+                   : access == 16 ? lookup_kernel<TE, TY, 16>
+                                  : lookup_kernel<TE, TY, 0>;
+    RT_CUDA(launch_k(ctx->pdl, kernel, lay.grid, 256, 0, ctx->stream, static_cast<const TE*>(table->ptr), table->ld,
+                     table->rows, static_cast<const uint32_t*>(tokens->ptr), y->rows, y->cols, lay.along, scale,
                      static_cast<TY*>(y->ptr), y->ld));
     count_launch(ctx);
     return RT_OK;
 }
 
-template <typename T>
-int launch_sums(rt_ctx* ctx, const rt_tensor* dy, Sums m, bool all_aligned) {
-    const int64_t piece_units = m.pieces * m.spans;
-    const int64_t units = piece_units + (m.accumulate ? 0 : (m.vocabulary + kEmpty - 1) / kEmpty * m.spans);
-    if (units == 0) return RT_OK;
-    const int64_t grid = std::min<int64_t>((units + 7) / 8, (int64_t)ctx->sm_count * 64);
-    auto* kernel = all_aligned ? sum_kernel<T, true> : sum_kernel<T, false>;
-    RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)grid, 256, 0, ctx->stream, m, static_cast<const T*>(dy->ptr), dy->ld,
-                     units, piece_units));
+template <typename T, int ACCESS>
+int launch_sums(rt_ctx* ctx, const rt_tensor* dy, Sums m) {
+    constexpr int SPAN = 32 * kColumns<T>;
+    m.spans = (m.n + SPAN - 1) / SPAN;
+    const Lay pieces(m.pieces, m.spans), rows((m.vocabulary + kTokens - 1) / kTokens, m.spans);
+    m.along = pieces.along;
+    m.piece_blocks = m.pieces > 1 ? (int)pieces.grid.x : 0;  // one piece holds no heavy run
+    const dim3 grid(m.piece_blocks + rows.grid.x, rows.grid.y);
+    RT_CUDA(launch_k(ctx->pdl, sum_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, static_cast<const T*>(dy->ptr), dy->ld));
     count_launch(ctx);
+    if (m.pieces > 1) {
+        const dim3 joins((unsigned)((m.pieces + kJoin - 1) / kJoin), (unsigned)m.spans);
+        RT_CUDA(launch_k(ctx->pdl, join_kernel<ACCESS, kColumns<T>>, joins, 256, 0, ctx->stream, m));
+        count_launch(ctx);
+    }
     return RT_OK;
+}
+
+template <typename T>
+int launch_sums(rt_ctx* ctx, const rt_tensor* dy, const rt_tensor* dtable, const Sums& m) {
+    int access = std::min(access_of(dy), access_of(dtable));
+    if (reinterpret_cast<uintptr_t>(m.partial) & 31) access = std::min(access, 16);
+    return access == 32 ? launch_sums<T, 32>(ctx, dy, m) : access == 16 ? launch_sums<T, 16>(ctx, dy, m) : launch_sums<T, 0>(ctx, dy, m);
 }
 
 int check_tokens(const char* what, const rt_tensor* tokens, const rt_tensor* rows) {
@@ -529,11 +846,16 @@ int check_tokens(const char* what, const rt_tensor* tokens, const rt_tensor* row
     return RT_OK;
 }
 
+int deal_bytes(int high, int warps) { return (4 << high) * (warps + 2); }
+int sort_bytes(int low, int warps) { return (4 << low) * (warps + 1); }
+
 }  // namespace
 
 int embedding_init() {
-    const int deal = (1 << kMaxHigh) * 4 * (kSortWarps + 1);
-    RT_CUDA(cudaFuncSetAttribute(bucket_deal_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, deal));
+    RT_CUDA(cudaFuncSetAttribute(bucket_deal_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, deal_bytes(kMaxHigh, 8)));
+    RT_CUDA(cudaFuncSetAttribute(bucket_sort_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_bytes(kMaxLow, 32)));
+    RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSmem)));
+    RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return RT_OK;
 }
 
@@ -550,6 +872,8 @@ int rt_embedding_forward(rt_ctx* ctx, const rt_tensor* table, const rt_tensor* t
     RT_CHECK(table->cols == y->cols, "rt_embedding_forward: table is %lldx%lld, y %lldx%lld", (long long)table->rows,
              (long long)table->cols, (long long)y->rows, (long long)y->cols);
     RT_TRY(check_tokens("rt_embedding_forward", tokens, y));
+    RT_CHECK(y->cols <= kMaxWidth && y->rows <= (int64_t)1 << 32, "rt_embedding_forward: y %lldx%lld is over 2^32 x 2^22",
+             (long long)y->rows, (long long)y->cols);
     if (y->rows == 0 || y->cols == 0) return RT_OK;
     RT_CUDA(cudaSetDevice(ctx->device));
     if (table->dtype == RT_BF16)
@@ -584,20 +908,40 @@ int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor*
     RT_CHECK(work->dtype == RT_F32 && (work->rows <= 1 || work->ld == work->cols) && work->rows * work->cols >= need &&
                  (reinterpret_cast<uintptr_t>(work->ptr) & 15) == 0,
              "rt_embedding_backward: work must be %lld packed f32, 16-byte aligned", (long long)need);
-    m.n = dy->cols;
-    m.spans = (m.n + kSpan - 1) / kSpan;
-    RT_CHECK(m.pieces * m.spans <= INT_MAX, "rt_embedding_backward: dy is too large");
     if (dtable->rows == 0 || dtable->cols == 0) return RT_OK;
     RT_CUDA(cudaSetDevice(ctx->device));
     const uint32_t* t = static_cast<const uint32_t*>(tokens->ptr);
     const bool pdl = ctx->pdl;
-    const int bins = 1 << s.high, low = 1 << s.low;
-    RT_CUDA(launch_k(pdl, bucket_count_kernel, s.ctas, kSortThreads, bins * 4, ctx->stream, s, t));
-    RT_CUDA(launch_k(pdl, bucket_deal_kernel, s.ctas, kSortThreads, bins * 4 * (kSortWarps + 1), ctx->stream, s, t));
-    RT_CUDA(launch_k(pdl, bucket_sort_kernel, bins, kSortThreads, low * 4 * (kSortWarps + 1), ctx->stream, s));
+    int64_t others = ctx->sm_count;  // SMs that the last kernel of the sort leaves idle
+    if (s.count <= kChunk * kMaxCluster) {
+        int ranks = 1;
+        while (ranks * kChunk < s.count) ranks *= 2;
+        RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t,
+                               (bits_of(s.vocabulary) + 7) / 8));
+        others -= ranks;
+        count_launch(ctx);
+    } else {
+    // With up to 256 buckets 32 warps a CTA, whose counters fit; with more (2^18 tokens and up) 8.
+    const int bins = 1 << s.high, warps = s.high <= 8 ? 32 : 8;
+    auto* deal = warps == 32 ? bucket_deal_kernel<32> : bucket_deal_kernel<8>;
+    auto* sort = warps == 32 ? bucket_sort_kernel<32> : bucket_sort_kernel<8>;
+    RT_CUDA(launch_k(pdl, bucket_count_kernel, s.ctas, 256, bins * 4, ctx->stream, s, t));
+    RT_CUDA(launch_k(pdl, deal, s.ctas, warps * 32, deal_bytes(s.high, warps), ctx->stream, s, t));
+    RT_CUDA(launch_k(pdl, sort, bins, warps * 32, sort_bytes(s.low, warps), ctx->stream, s));
     count_launch(ctx, 3);
+    }
+    if (!accumulate) {
+        // 16 rows or more to a CTA: each goes over all tokens
+        const int64_t grid = std::max<int64_t>(1, std::min(others, s.vocabulary / 16));
+        const int access = access_of(dtable);
+        auto* fill = access == 32 ? fill_kernel<32> : access == 16 ? fill_kernel<16> : fill_kernel<0>;
+        RT_CUDA(launch_k(pdl, fill, (unsigned)grid, 1024, 0, ctx->stream, t, s.count, s.vocabulary,
+                         static_cast<float*>(dtable->ptr), dtable->ld, dtable->cols));
+        count_launch(ctx);
+    }
     m.count = s.count;
     m.vocabulary = s.vocabulary;
+    m.n = dy->cols;
     m.token = s.token;
     m.position = s.position;
     m.start = s.start;
@@ -605,14 +949,7 @@ int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor*
     m.accumulate = accumulate != 0;
     m.out = static_cast<float*>(dtable->ptr);
     m.ldo = dtable->ld;
-    const bool all = aligned(dy) && aligned(dtable);
-    RT_TRY(dy->dtype == RT_BF16 ? launch_sums<__nv_bfloat16>(ctx, dy, m, all) : launch_sums<float>(ctx, dy, m, all));
-    if (m.pieces > 1) {
-        auto* kernel = all ? join_kernel<true> : join_kernel<false>;
-        RT_CUDA(launch_k(pdl, kernel, (unsigned)(m.pieces * m.spans), 256, 0, ctx->stream, m));
-        count_launch(ctx);
-    }
-    return RT_OK;
+    return dy->dtype == RT_BF16 ? launch_sums<__nv_bfloat16>(ctx, dy, dtable, m) : launch_sums<float>(ctx, dy, dtable, m);
 }
 
 }  // extern "C"
