@@ -15,6 +15,7 @@
 // pieces leaves a partial sum in each, which a second kernel adds in order.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "internal.h"
 
@@ -25,65 +26,73 @@ constexpr int64_t kMaxWidth = 1 << 22;  // spans fit a grid's second extent
 constexpr int64_t kMaxVocabulary = (1 << 21) - 1;  // keys 0 .. V fit 21 bits
 
 // A lane's N columns (4 or 8) of a warp's span of 32 N.  ACCESS: bytes that the rows are
-// aligned to, 32 or 16: neighbouring columns, by accesses of that width where all of them
-// exist; 0: a warp's accesses are neighbours, column lane + 32 i the lane's i-th.
+// aligned to, 32 or 16: neighbouring columns, by accesses of that width; the row's length is
+// then a multiple of N, so a lane has all of its columns or none.  0: anything else, a
+// warp's accesses are neighbours, column lane + 32 i the lane's i-th.
 template <int ACCESS, int N>
 struct Columns {
-    static constexpr int SPAN = 32 * N, STEP = ACCESS ? 1 : 32;
     int64_t first, n;  // the lane's first column, the row's length
-    bool all;          // the lane's neighbouring columns exist
+    bool on;           // it exists
     __device__ __forceinline__ Columns(int64_t span, int64_t n, int lane)
-        : first(span * SPAN + lane * (ACCESS ? N : 1)), n(n), all(ACCESS && first + N <= n) {}
+        : first(span * (32 * N) + lane * (ACCESS ? N : 1)), n(n), on(first < n) {
+        if (ACCESS && !on) first = 0;  // reads without a condition; what it reads is not stored
+    }
 };
 
-// The lane's elements of a row as they lie in memory, to be converted when they are used:
-// bf16 takes half the registers on its way.
+// The lane's elements of a row as they lie in memory, to be converted when they are used: a
+// load is then not waited for before the next one is issued.
 template <typename T, int ACCESS, int N>
 struct Lane {
     using C = Columns<ACCESS, N>;
-    static constexpr int WORDS = N * sizeof(T) / 4;
+    static constexpr int WORDS = ACCESS ? N * sizeof(T) / 4 : N;
     static constexpr int WIDE = WORDS == 8 && ACCESS == 32 ? 8 : WORDS >= 4 ? 4 : 2;  // words of an access
     uint32_t w[WORDS];
 
     __device__ __forceinline__ float value(int i) const {
-        if constexpr (sizeof(T) == 2) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-        else return __uint_as_float(w[i]);
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (ACCESS == 0) return __uint_as_float(w[i] << 16);
+        else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
     // NC: the kernel writes no row of this matrix
     template <bool NC = true>
     __device__ __forceinline__ void load(const T* row, const C& c) {
         const T* p = row + c.first;
-        if (c.all) {
-            if constexpr (WIDE == 8 && NC)
-                asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                             : "l"(p));
-            else if constexpr (WIDE >= 4)
+        if constexpr (ACCESS == 0) {
 #pragma unroll
-                for (int i = 0; i < WORDS; i += 4) {
-                    const uint4* q = reinterpret_cast<const uint4*>(p) + i / 4;
-                    const uint4 u = NC ? __ldg(q) : *q;
-                    w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+            for (int i = 0; i < N; ++i) {
+                w[i] = 0;
+                if (c.first + i * 32 < c.n) {
+                    if constexpr (sizeof(T) == 2) w[i] = reinterpret_cast<const unsigned short*>(p)[i * 32];
+                    else w[i] = reinterpret_cast<const uint32_t*>(p)[i * 32];
                 }
-            else {
-                const uint2* q = reinterpret_cast<const uint2*>(p);
-                const uint2 u = NC ? __ldg(q) : *q;
-                w[0] = u.x, w[1] = u.y;
+            }
+        } else if constexpr (WIDE == 8 && NC) {
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(p));
+        } else if constexpr (WIDE >= 4) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4* q = reinterpret_cast<const uint4*>(p) + i / 4;
+                const uint4 u = NC ? __ldg(q) : *q;
+                w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) w[i] = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (c.first + i * C::STEP < c.n) {
-                    if constexpr (sizeof(T) == 2) w[i / 2] |= (uint32_t)__bfloat16_as_ushort(p[i * C::STEP]) << (16 * (i & 1));
-                    else w[i] = __float_as_uint(p[i * C::STEP]);
-                }
+            const uint2* q = reinterpret_cast<const uint2*>(p);
+            const uint2 u = NC ? __ldg(q) : *q;
+            w[0] = u.x, w[1] = u.y;
         }
     }
     static __device__ __forceinline__ void store(T* row, const C& c, const float (&v)[N]) {
         T* p = row + c.first;
-        if (c.all) {
+        if constexpr (ACCESS == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (c.first + i * 32 < c.n) {
+                    if constexpr (sizeof(T) == 2) p[i * 32] = __float2bfloat16_rn(v[i]);
+                    else p[i * 32] = v[i];
+                }
+        } else if (c.on) {
             uint32_t u[WORDS];
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) {
@@ -103,13 +112,6 @@ struct Lane {
                 for (int i = 0; i < WORDS; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
             else
                 *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (c.first + i * C::STEP < c.n) {
-                    if constexpr (sizeof(T) == 2) p[i * C::STEP] = __float2bfloat16_rn(v[i]);
-                    else p[i * C::STEP] = v[i];
-                }
         }
     }
 };
@@ -557,13 +559,12 @@ __global__ void __launch_bounds__(1024) fill_kernel(const uint32_t* __restrict__
     pdl_wait();
 }
 
-// The sums.  A token that occurs at most kCut times is light: a warp takes 512 bytes' columns of
-// kTokens neighbouring rows of dE, whose positions lie one after another, and writes each
-// row once, the rows of tokens that do not occur as zeros.  The others are heavy: the sorted
-// list is cut into pieces of kCut positions whatever the tokens, so a heavy run crosses
-// pieces; each leaves a partial sum of it, and join_kernel adds these in order.
-constexpr int kCut = 64, kTokens = 8;
-static_assert(kTokens < 32, "a lane reads where the next row starts");
+// The sums.  A token that occurs at most kLight times is light: a warp takes 512 bytes' columns
+// of `tokens` neighbouring rows of dE, whose positions lie one after another, and writes
+// each row once.  The others are heavy: the sorted list is cut into pieces of kCut positions
+// whatever the tokens, a warp each; where a heavy run crosses pieces, each leaves a partial
+// sum of it, and join() adds these in order.
+constexpr int kCut = 64, kLight = 16;
 
 // Columns of a lane: 16 bytes of dy.
 template <typename T>
@@ -572,8 +573,6 @@ constexpr int kColumns = 16 / (int)sizeof(T);
 struct Sums {
     int64_t count, vocabulary, n, spans, width;
     int64_t pieces;
-    int along;         // Lay's
-    int piece_blocks;  // CTAs in front that take pieces
     const uint32_t* token;
     const uint32_t* position;
     const uint32_t* start;
@@ -600,52 +599,143 @@ __device__ __forceinline__ void emit(const Sums& s, uint32_t token, const Column
     L::store(row, c, v);
 }
 
+// Heavy runs, a warp a piece and span: their sums where they lie inside it, else partial ones.
 template <typename T, int ACCESS>
-__global__ void __launch_bounds__(256, 4) sum_kernel(Sums s, const T* __restrict__ dy, int64_t ldy) {
+__global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* __restrict__ dy, int64_t ldy, int along) {
     pdl_wait();
     pdl_launch_dependents();
-    constexpr int N = kColumns<T>, U = 4;  // U: rows of dy under way
+    constexpr int N = kColumns<T>, U = 8;  // U: rows of dy under way
     using L = Lane<T, ACCESS, N>;
     const int lane = threadIdx.x & 31;
-    const Columns<ACCESS, N> c(lay_span(s.along), s.n, lane);
-    if ((int)blockIdx.x < s.piece_blocks) {
-        const int64_t real = s.start[s.vocabulary];  // positions that hold a token
-        const int64_t piece = lay_group(s.along), p0 = piece * kCut, p1 = min(real, p0 + kCut);
-        if (p0 >= p1) return;
-        // a heavy run holds the piece's first position or its last
-        const uint32_t ends[2] = {s.token[p0], s.token[p1 - 1]};
-        for (int h = 0; h < (ends[0] == ends[1] ? 1 : 2); ++h) {
-            const int64_t run0 = s.start[ends[h]], run1 = s.start[ends[h] + 1];
-            if (run1 - run0 <= kCut) continue;
-            const int64_t begin = max(run0, p0), end = min(run1, p1);
-            float sum[N] = {};
-            for (int64_t q = begin; q < end; q += 32) {
-                const uint32_t position = q + lane < end ? s.position[q + lane] : 0u;
-                const int live = (int)min((int64_t)32, end - q);
-                for (int g = 0; g < live; g += U) {
-                    L v[U];
+    const Columns<ACCESS, N> c(lay_span(along), s.n, lane);
+    const int64_t real = s.start[s.vocabulary];  // positions that hold a token
+    const int64_t piece = lay_group(along), p0 = piece * kCut;
+    const int live = (int)max((int64_t)0, min((int64_t)kCut, real - p0));
+    uint32_t token[kCut / 32], row[kCut / 32], begin[kCut / 32], end[kCut / 32];
+    uint64_t heavy = 0;  // a bit a position
 #pragma unroll
-                    for (int x = 0; x < U; ++x) {
-                        const uint32_t row = __shfl_sync(0xffffffffu, position, (g + x) & 31);
-                        if (g + x < live) v[x].load(dy + row * ldy, c);
-                    }
-#pragma unroll
-                    for (int x = 0; x < U; ++x)
-                        if (g + x < live)
-#pragma unroll
-                            for (int i = 0; i < N; ++i) sum[i] += v[x].value(i);
-                }
-            }
+    for (int h = 0; h < kCut / 32; ++h) {
+        const bool there = h * 32 + lane < live;
+        token[h] = there ? s.token[p0 + h * 32 + lane] : 0u;
+        row[h] = there ? s.position[p0 + h * 32 + lane] : 0u;
+        begin[h] = s.start[token[h]], end[h] = s.start[token[h] + 1];
+        heavy |= (uint64_t)__ballot_sync(0xffffffffu, there && end[h] - begin[h] > kLight) << (32 * h);
+    }
+    if (!heavy) return;
+    auto of = [&](const uint32_t (&v)[kCut / 32], int at) { return __shfl_sync(0xffffffffu, at < 32 ? v[0] : v[1], at & 31); };
+    static_assert(kCut == 64, "two positions a lane");
+    float sum[N] = {};
+    int run = __ffsll((long long)heavy) - 1;  // a position of the run
+    uint32_t run_token = of(token, run);
+    auto flush = [&]() {
+        const int64_t run0 = of(begin, run), run1 = of(end, run);
+        if (run0 >= p0 && run1 <= p0 + kCut)
+            emit<ACCESS, N>(s, run_token, c, sum);
+        else
             Lane<float, ACCESS, N>::store(s.partial + (piece * 2 + (run0 < p0 ? 0 : 1)) * s.width, c, sum);
+    };
+    while (heavy) {
+        L v[U];
+        int at[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            at[x] = heavy ? __ffsll((long long)heavy) - 1 : -1;
+            heavy &= heavy - 1;
+            v[x].load(dy + of(row, max(at[x], 0)) * ldy, c);  // past the last one any row
         }
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            if (at[x] < 0) break;
+            const uint32_t t = of(token, at[x]);
+            if (t != run_token) {
+                flush();
+                run = at[x];
+                run_token = t;
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += v[x].value(i);
+        }
+    }
+    flush();
+}
+
+// Adds the partial sums of the heavy runs that begin in kJoin pieces: a run's second row
+// there and the first rows of the pieces that follow, dealt out over the CTA's warps in
+// order.
+constexpr int kJoin = 8;
+
+template <int ACCESS, int N>
+__device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span) {
+    using L = Lane<float, ACCESS, N>;
+    __shared__ float part[8][32 * N];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t real = s.start[s.vocabulary];
+    const Columns<ACCESS, N> c(span, s.n, lane);
+    // every warp looks at the last position of each of the pieces
+    const int64_t end = (piece0 + lane + 1) * kCut;
+    uint32_t token = 0;
+    int64_t first = 0, next = 0;
+    bool begins = lane < kJoin && end < real;
+    if (begins) {
+        token = s.token[end - 1];
+        first = s.start[token], next = s.start[token + 1];
+        begins = next > end && first >= end - kCut && next - first > kLight;
+    }
+    pdl_wait();  // for the partial sums
+    for (uint32_t found = __ballot_sync(0xffffffffu, begins); found; found &= found - 1) {
+        const int of = __ffs(found) - 1;
+        const int64_t piece = piece0 + of, last = (__shfl_sync(0xffffffffu, next, of) - 1) / kCut;
+        const int64_t count = last - piece + 1, each = (count + 7) / 8;
+        const int64_t b = min(count, warp * each), e = min(count, b + each);
+        float sum[N] = {};
+#pragma unroll 4
+        for (int64_t q = b; q < e; ++q) {
+            L v;
+            const float* row = s.partial + ((piece + q) * 2 + (q == 0 ? 1 : 0)) * s.width;
+            v.load(row, c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += v.value(i);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[warp][i * 32 + lane] = sum[i];
+        __syncthreads();
+        if (warp == 0) {
+            const int64_t used = (count + each - 1) / each;
+            for (int w = 1; w < used; ++w)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += part[w][i * 32 + lane];
+            emit<ACCESS, N>(s, __shfl_sync(0xffffffffu, token, of), c, sum);
+        }
+        __syncthreads();
+    }
+}
+
+// Light tokens, a warp `tokens` (at most 31) rows of dE and a span; in the CTAs behind those, of which the
+// last ones of the grid are, the joins.  Only the joins need piece_kernel's results, so only
+// they wait for it: what the others read was complete when it passed its own wait.
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict__ dy, int64_t ldy, int along, int tokens,
+                                                     int row_blocks, int alone) {
+    constexpr int N = kColumns<T>, U = 4;  // U: rows of dy under way
+    using L = Lane<T, ACCESS, N>;
+    // Nothing lets the next kernel launch before this one's CTAs end: the sort of the next call
+    // would take 16 SMs whole to wait there.
+    if (alone) pdl_wait();  // no piece_kernel before this one
+    if ((int)blockIdx.x >= row_blocks) {
+        const unsigned q = blockIdx.x - row_blocks;  // 2^along neighbours take the spans of the same pieces
+        join<ACCESS, N>(s, (int64_t)(q >> along) * kJoin, ((int64_t)blockIdx.y << along) + (q & ((1u << along) - 1)));
         return;
     }
-    const int64_t t0 = (lay_group(s.along) - ((int64_t)s.piece_blocks << (3 - s.along))) * kTokens;
+    const int lane = threadIdx.x & 31;
+    const Columns<ACCESS, N> c(lay_span(along), s.n, lane);
+    const int64_t t0 = lay_group(along) * tokens;
     if (t0 >= s.vocabulary) return;
-    const int64_t token = min(t0 + min(lane, kTokens), s.vocabulary);
+    const int64_t token = min(t0 + min(lane, tokens), s.vocabulary);
     const uint32_t first = s.start[token], next = __shfl_down_sync(0xffffffffu, first, 1);
-    const uint32_t count = lane < kTokens && token < s.vocabulary ? next - first : 0u;
-    const uint32_t light = count <= kCut ? count : 0u;
+    const uint32_t count = lane < tokens && token < s.vocabulary ? next - first : 0u;
+    const uint32_t light = count <= kLight ? count : 0u;
     uint32_t upto = light;  // light positions of the rows up to the lane's
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -673,8 +763,7 @@ __global__ void __launch_bounds__(256, 4) sum_kernel(Sums s, const T* __restrict
 #pragma unroll
             for (int x = 0; x < U; ++x) {
                 t[x] = __shfl_sync(0xffffffffu, of, (g + x) & 31);
-                const uint32_t row = __shfl_sync(0xffffffffu, position, (g + x) & 31);
-                if (g + x < live) v[x].load(dy + row * ldy, c);
+                v[x].load(dy + __shfl_sync(0xffffffffu, position, min(g + x, live - 1)) * ldy, c);
             }
 #pragma unroll
             for (int x = 0; x < U; ++x) {
@@ -693,57 +782,114 @@ __global__ void __launch_bounds__(256, 4) sum_kernel(Sums s, const T* __restrict
     if (run >= 0) emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
 }
 
-// Adds the partial sums of the heavy runs that begin in the CTA's kJoin pieces: a run's
-// second row there and the first rows of the pieces that follow, dealt out over the CTA's
-// warps in order.
-constexpr int kJoin = 16;
+// Few positions: one launch.  A CTA takes `group` neighbouring rows of dE and a span of columns;
+// it goes over all positions, sorts those of its rows in shared memory, and its warps take
+// equal shares of them.  A run that crosses shares is joined through shared memory, in order.
+constexpr int kFew = 4096, kGroup = 128;
 
-template <int ACCESS, int N>
-__global__ void __launch_bounds__(256) join_kernel(Sums s) {
-    using L = Lane<float, ACCESS, N>;
-    __shared__ float part[8][32 * N];
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(256, 4) few_kernel(Sums s, const uint32_t* __restrict__ tokens, const T* __restrict__ dy,
+                                                  int64_t ldy, int group) {
+    constexpr int N = kColumns<T>, WARPS = 8;
+    using L = Lane<T, ACCESS, N>;
+    __shared__ uint32_t base[kGroup + 1], sums[WARPS];
+    __shared__ uint32_t cnt[WARPS][kGroup];
+    __shared__ uint32_t list[kFew];  // row << 16 | position, sorted
+    __shared__ float part[WARPS][2][32 * N];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < WARPS * kGroup; i += 256) cnt[0][i] = 0;
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t real = s.start[s.vocabulary];
-    const int64_t piece0 = (int64_t)blockIdx.x * kJoin;
+    const int64_t t0 = (int64_t)blockIdx.x * group;
+    const int rows = (int)min((int64_t)group, s.vocabulary - t0);
     const Columns<ACCESS, N> c(blockIdx.y, s.n, lane);
-    // every warp looks at the last position of each of the pieces
-    const int64_t end = (piece0 + lane + 1) * kCut;
-    uint32_t token = 0;
-    int64_t first = 0, next = 0;
-    bool begins = lane < kJoin && end < real;
-    if (begins) {
-        token = s.token[end - 1];
-        first = s.start[token], next = s.start[token + 1];
-        begins = next > end && first >= end - kCut && next - first > kCut;
-    }
-    for (uint32_t found = __ballot_sync(0xffffffffu, begins); found; found &= found - 1) {
-        const int of = __ffs(found) - 1;
-        const int64_t piece = piece0 + of, last = (__shfl_sync(0xffffffffu, next, of) - 1) / kCut;
-        const int64_t count = last - piece + 1, each = (count + 7) / 8;
-        const int64_t b = min(count, warp * each), e = min(count, b + each);
-        float sum[N] = {};
-#pragma unroll 4
-        for (int64_t q = b; q < e; ++q) {
-            L v;
-            const float* row = s.partial + ((piece + q) * 2 + (q == 0 ? 1 : 0)) * s.width;
-            v.load(row, c);
+    auto key = [&](int64_t i) { return __ldg(tokens + i) - (uint32_t)t0; };
+    auto mine = [&](uint32_t k, bool there) { return there && k < (uint32_t)rows; };
+    in_order<WARPS>(s.count, warp, lane, key, [&](int64_t, uint32_t k, bool there) {
+        if (__ballot_sync(0xffffffffu, mine(k, there))) count_rank(cnt[warp], k, mine(k, there), lane);
+    });
+    __syncthreads();
+    if (threadIdx.x <= kGroup) {
+        uint32_t all = 0;
+        if (threadIdx.x < kGroup)
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] += v.value(i);
+            for (int w = 0; w < WARPS; ++w) all += cnt[w][threadIdx.x];
+        base[threadIdx.x] = all;
+    }
+    __syncthreads();
+    exclusive<WARPS>(base, kGroup + 1, sums);
+    if (threadIdx.x < kGroup) {
+        uint32_t run = base[threadIdx.x];
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const uint32_t x = cnt[w][threadIdx.x];
+            cnt[w][threadIdx.x] = run;
+            run += x;
+        }
+    }
+    __syncthreads();
+    in_order<WARPS>(s.count, warp, lane, key, [&](int64_t i, uint32_t k, bool there) {
+        if (!__ballot_sync(0xffffffffu, mine(k, there))) return;
+        const uint32_t to = count_rank(cnt[warp], k, mine(k, there), lane);
+        if (mine(k, there)) list[to] = k << 16 | (uint32_t)i;
+    });
+    if (!s.accumulate) {
+        const float zero[N] = {};
+        for (int r = warp; r < rows; r += WARPS)
+            if (base[r] == base[r + 1]) Lane<float, ACCESS, N>::store(s.out + (t0 + r) * s.ldo, c, zero);
+    }
+    __syncthreads();
+    const int total = (int)base[kGroup], each = (total + WARPS - 1) / WARPS;
+    const int begin = min(total, warp * each), end = min(total, begin + each);
+    float sum[N] = {};
+    int run = begin < end ? (int)(list[begin] >> 16) : -1;
+    auto flush = [&]() {
+        const int run0 = (int)base[run], run1 = (int)base[run + 1];
+        if (run0 >= begin && run1 <= end) {
+            emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[warp][run0 < begin ? 0 : 1][i * 32 + lane] = sum[i];
+        }
+    };
+    // U entries from e on, all of their rows of dy under way at once
+    auto add = [&](int e, auto width) {
+        constexpr int U = decltype(width)::value;
+        L v[U];
+        uint32_t entry[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
+            entry[x] = list[min(e + x, end - 1)];
+            v[x].load(dy + (entry[x] & 0xffffu) * ldy, c);
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) part[warp][i * 32 + lane] = sum[i];
-        __syncthreads();
-        if (warp == 0) {
-            const int64_t used = (count + each - 1) / each;
-            for (int w = 1; w < used; ++w)
+        for (int x = 0; x < U; ++x) {
+            if (e + x >= end) break;
+            if ((int)(entry[x] >> 16) != run) {
+                flush();
+                run = (int)(entry[x] >> 16);
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += part[w][i * 32 + lane];
-            emit<ACCESS, N>(s, __shfl_sync(0xffffffffu, token, of), c, sum);
+                for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += v[x].value(i);
         }
-        __syncthreads();
-    }
+    };
+    constexpr int MANY = ACCESS ? 8 : 4;  // with a register an element eight rows would spill
+    int e = begin;
+    for (; end - e >= MANY; e += MANY) add(e, std::integral_constant<int, MANY>());
+    for (; e < end; e += 3) add(e, std::integral_constant<int, 3>());
+    if (run >= 0) flush();
+    __syncthreads();
+    // the warp in whose share a run begins that goes on adds it up
+    if (run < 0 || (int)base[run + 1] <= end || (int)base[run] < begin) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = part[warp][1][i * 32 + lane];
+    for (int w = warp + 1; w < WARPS && w * each < (int)base[run + 1]; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] += part[w][0][i * 32 + lane];
+    emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
 }
 
 int bits_of(int64_t v) {
@@ -773,13 +919,15 @@ int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) 
         at += words(v);
         return p;
     };
+    if (count <= kFew) return words(1);  // few_kernel needs none
     m->partial = reinterpret_cast<float*>(take(m->pieces * 2 * m->width));
-    s->bucket = take((1 << s->high) + 1);
-    s->key = take(count);
-    s->place = take(count);
     s->token = take(count);
     s->position = take(count);
     s->start = take(vocabulary + 1);
+    if (count <= kChunk * kMaxCluster) return at;  // the rest of the sort happens in shared memory
+    s->bucket = take((1 << s->high) + 1);
+    s->key = take(count);
+    s->place = take(count);
     s->counts = take((int64_t)s->ctas << s->high);
     return at;
 }
@@ -792,16 +940,16 @@ int check_backward(int64_t count, int64_t vocabulary, int64_t n) {
     return RT_OK;
 }
 
-// Bytes that every row of t is aligned to: 32, 16 or 0.
-int access_of(const rt_tensor* t) {
+// Bytes that every row of t is aligned to, 32 or 16, if rows are whole columns of a lane (n); else 0.
+int access_of(const rt_tensor* t, int n) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(t->ptr) | (uintptr_t)(t->ld * (int64_t)dtype_size(t->dtype));
-    return (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 0;
+    return t->cols % n ? 0 : (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 0;
 }
 
 template <typename TE, typename TY>
 int launch_lookup(rt_ctx* ctx, const rt_tensor* table, const rt_tensor* tokens, float scale, rt_tensor* y) {
     const Lay lay((y->rows + kRows - 1) / kRows, (y->cols + 32 * kLookup - 1) / (32 * kLookup));
-    const int access = std::min(access_of(table), access_of(y));
+    const int access = std::min(access_of(table, kLookup), access_of(y, kLookup));
     auto* kernel = access == 32   ? lookup_kernel<TE, TY, 32>
                    : access == 16 ? lookup_kernel<TE, TY, 16>
                                   : lookup_kernel<TE, TY, 0>;
@@ -816,25 +964,87 @@ template <typename T, int ACCESS>
 int launch_sums(rt_ctx* ctx, const rt_tensor* dy, Sums m) {
     constexpr int SPAN = 32 * kColumns<T>;
     m.spans = (m.n + SPAN - 1) / SPAN;
-    const Lay pieces(m.pieces, m.spans), rows((m.vocabulary + kTokens - 1) / kTokens, m.spans);
-    m.along = pieces.along;
-    m.piece_blocks = m.pieces > 1 ? (int)pieces.grid.x : 0;  // one piece holds no heavy run
-    const dim3 grid(m.piece_blocks + rows.grid.x, rows.grid.y);
-    RT_CUDA(launch_k(ctx->pdl, sum_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, static_cast<const T*>(dy->ptr), dy->ld));
-    count_launch(ctx);
-    if (m.pieces > 1) {
-        const dim3 joins((unsigned)((m.pieces + kJoin - 1) / kJoin), (unsigned)m.spans);
-        RT_CUDA(launch_k(ctx->pdl, join_kernel<ACCESS, kColumns<T>>, joins, 256, 0, ctx->stream, m));
+    // 16 rows a warp where that makes warps enough for every place on the device (65536 x 1024 of 50257:
+    // 77 us, with 4 rows 87), else 4, whose chain of reads is shorter (2047 x 1000 of 1000: 13.9 us, with 16 18.1)
+    const int tokens = m.vocabulary / 16 * m.spans >= (int64_t)ctx->sm_count * 32 ? 16 : 4;
+    const Lay pieces(m.pieces, m.spans), rows((m.vocabulary + tokens - 1) / tokens, m.spans);
+    const bool heavy = m.count > kLight;
+    const T* p = static_cast<const T*>(dy->ptr);
+    if (heavy) {
+        RT_CUDA(launch_k(ctx->pdl, piece_kernel<T, ACCESS>, pieces.grid, 256, 0, ctx->stream, m, p, dy->ld, pieces.along));
         count_launch(ctx);
     }
+    dim3 grid = rows.grid;
+    if (heavy) grid.x += (unsigned)((m.pieces + kJoin - 1) / kJoin) << rows.along;
+    RT_CUDA(launch_k(ctx->pdl, row_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, p, dy->ld, rows.along, tokens, (int)rows.grid.x,
+                     heavy ? 0 : 1));
+    count_launch(ctx);
     return RT_OK;
 }
 
+template <typename T, int ACCESS>
+int launch_few(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, const Sums& m) {
+    constexpr int SPAN = 32 * kColumns<T>;
+    const int64_t spans = (m.n + SPAN - 1) / SPAN;
+    // so many rows, 4 to kGroup, that the CTAs fit the device at once, four to an SM: each goes over all positions
+    int group = 4;
+    while (group < kGroup && (m.vocabulary + group - 1) / group * spans > 4 * (int64_t)ctx->sm_count) group *= 2;
+    const dim3 grid((unsigned)((m.vocabulary + group - 1) / group), (unsigned)spans);
+    RT_CUDA(launch_k(ctx->pdl, few_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, static_cast<const uint32_t*>(tokens->ptr),
+                     static_cast<const T*>(dy->ptr), dy->ld, group));
+    count_launch(ctx);
+    return RT_OK;
+}
+
+// Rows of dy and dE aligned to 32 bytes, 16 or less; few: positions that one launch handles.
 template <typename T>
-int launch_sums(rt_ctx* ctx, const rt_tensor* dy, const rt_tensor* dtable, const Sums& m) {
-    int access = std::min(access_of(dy), access_of(dtable));
-    if (reinterpret_cast<uintptr_t>(m.partial) & 31) access = std::min(access, 16);
-    return access == 32 ? launch_sums<T, 32>(ctx, dy, m) : access == 16 ? launch_sums<T, 16>(ctx, dy, m) : launch_sums<T, 0>(ctx, dy, m);
+int launch_sums(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, const rt_tensor* dtable, const Sums& m, bool few) {
+    int access = std::min(access_of(dy, kColumns<T>), access_of(dtable, kColumns<T>));
+    if (!few && (reinterpret_cast<uintptr_t>(m.partial) & 31)) access = std::min(access, 16);
+    if (few)
+        return access == 32   ? launch_few<T, 32>(ctx, tokens, dy, m)
+               : access == 16 ? launch_few<T, 16>(ctx, tokens, dy, m)
+                              : launch_few<T, 0>(ctx, tokens, dy, m);
+    return access == 32   ? launch_sums<T, 32>(ctx, dy, m)
+           : access == 16 ? launch_sums<T, 16>(ctx, dy, m)
+                          : launch_sums<T, 0>(ctx, dy, m);
+}
+
+// Shared memory of the kernels of the sort over launches.
+int deal_bytes(int high, int warps) { return (4 << high) * (warps + 2); }
+int sort_bytes(int low, int warps) { return (4 << low) * (warps + 1); }
+
+// The sort and, beside its last kernel, the rows of dE that no token has.
+int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, const Sums& m, const rt_tensor* dtable) {
+    const bool pdl = ctx->pdl;
+    int64_t others = ctx->sm_count;  // SMs that the last kernel of the sort leaves idle
+    if (s.count <= kChunk * kMaxCluster) {
+        int ranks = 1;
+        while (ranks * kChunk < s.count) ranks *= 2;
+        RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t,
+                               (bits_of(s.vocabulary) + 7) / 8));
+        others -= ranks;
+        count_launch(ctx);
+    } else {
+    // With up to 256 buckets 32 warps a CTA, whose counters fit; with more (2^18 tokens and up) 8.
+    const int bins = 1 << s.high, warps = s.high <= 8 ? 32 : 8;
+    auto* deal = warps == 32 ? bucket_deal_kernel<32> : bucket_deal_kernel<8>;
+    auto* sort = warps == 32 ? bucket_sort_kernel<32> : bucket_sort_kernel<8>;
+    RT_CUDA(launch_k(pdl, bucket_count_kernel, s.ctas, 256, bins * 4, ctx->stream, s, t));
+    RT_CUDA(launch_k(pdl, deal, s.ctas, warps * 32, deal_bytes(s.high, warps), ctx->stream, s, t));
+    RT_CUDA(launch_k(pdl, sort, bins, warps * 32, sort_bytes(s.low, warps), ctx->stream, s));
+    count_launch(ctx, 3);
+    }
+    if (!m.accumulate) {
+        // 16 rows or more to a CTA: each goes over all tokens
+        const int64_t grid = std::max<int64_t>(1, std::min(others, s.vocabulary / 16));
+        const int access = access_of(dtable, 8);
+        auto* fill = access == 32 ? fill_kernel<32> : access == 16 ? fill_kernel<16> : fill_kernel<0>;
+        RT_CUDA(launch_k(pdl, fill, (unsigned)grid, 1024, 0, ctx->stream, t, s.count, s.vocabulary,
+                         static_cast<float*>(dtable->ptr), dtable->ld, dtable->cols));
+        count_launch(ctx);
+    }
+    return RT_OK;
 }
 
 int check_tokens(const char* what, const rt_tensor* tokens, const rt_tensor* rows) {
@@ -845,9 +1055,6 @@ int check_tokens(const char* what, const rt_tensor* tokens, const rt_tensor* row
              (long long)(tokens->rows * tokens->cols), (long long)rows->rows);
     return RT_OK;
 }
-
-int deal_bytes(int high, int warps) { return (4 << high) * (warps + 2); }
-int sort_bytes(int low, int warps) { return (4 << low) * (warps + 1); }
 
 }  // namespace
 
@@ -910,35 +1117,6 @@ int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor*
              "rt_embedding_backward: work must be %lld packed f32, 16-byte aligned", (long long)need);
     if (dtable->rows == 0 || dtable->cols == 0) return RT_OK;
     RT_CUDA(cudaSetDevice(ctx->device));
-    const uint32_t* t = static_cast<const uint32_t*>(tokens->ptr);
-    const bool pdl = ctx->pdl;
-    int64_t others = ctx->sm_count;  // SMs that the last kernel of the sort leaves idle
-    if (s.count <= kChunk * kMaxCluster) {
-        int ranks = 1;
-        while (ranks * kChunk < s.count) ranks *= 2;
-        RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t,
-                               (bits_of(s.vocabulary) + 7) / 8));
-        others -= ranks;
-        count_launch(ctx);
-    } else {
-    // With up to 256 buckets 32 warps a CTA, whose counters fit; with more (2^18 tokens and up) 8.
-    const int bins = 1 << s.high, warps = s.high <= 8 ? 32 : 8;
-    auto* deal = warps == 32 ? bucket_deal_kernel<32> : bucket_deal_kernel<8>;
-    auto* sort = warps == 32 ? bucket_sort_kernel<32> : bucket_sort_kernel<8>;
-    RT_CUDA(launch_k(pdl, bucket_count_kernel, s.ctas, 256, bins * 4, ctx->stream, s, t));
-    RT_CUDA(launch_k(pdl, deal, s.ctas, warps * 32, deal_bytes(s.high, warps), ctx->stream, s, t));
-    RT_CUDA(launch_k(pdl, sort, bins, warps * 32, sort_bytes(s.low, warps), ctx->stream, s));
-    count_launch(ctx, 3);
-    }
-    if (!accumulate) {
-        // 16 rows or more to a CTA: each goes over all tokens
-        const int64_t grid = std::max<int64_t>(1, std::min(others, s.vocabulary / 16));
-        const int access = access_of(dtable);
-        auto* fill = access == 32 ? fill_kernel<32> : access == 16 ? fill_kernel<16> : fill_kernel<0>;
-        RT_CUDA(launch_k(pdl, fill, (unsigned)grid, 1024, 0, ctx->stream, t, s.count, s.vocabulary,
-                         static_cast<float*>(dtable->ptr), dtable->ld, dtable->cols));
-        count_launch(ctx);
-    }
     m.count = s.count;
     m.vocabulary = s.vocabulary;
     m.n = dy->cols;
@@ -949,7 +1127,10 @@ int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor*
     m.accumulate = accumulate != 0;
     m.out = static_cast<float*>(dtable->ptr);
     m.ldo = dtable->ld;
-    return dy->dtype == RT_BF16 ? launch_sums<__nv_bfloat16>(ctx, dy, dtable, m) : launch_sums<float>(ctx, dy, dtable, m);
+    const bool few = s.count <= kFew;
+    if (!few) RT_TRY(launch_sort(ctx, static_cast<const uint32_t*>(tokens->ptr), s, m, dtable));
+    return dy->dtype == RT_BF16 ? launch_sums<__nv_bfloat16>(ctx, tokens, dy, dtable, m, few)
+                                : launch_sums<float>(ctx, tokens, dy, dtable, m, few);
 }
 
 }  // extern "C"
