@@ -11,6 +11,8 @@
 // each: p is taken to the nearest 2^-16, and 1 - p in the scale is that of the rounded p,
 // so the expectation is exact.  32 bits an element would double the rounds, whose
 // integer products then take longer than HBM.
+#include <climits>
+
 #include "row_piece.cuh"
 
 namespace rt {
@@ -22,7 +24,7 @@ struct DropoutParams {
     const uint32_t* step_at;  // added to step; may be null
     uint32_t drop;            // kept where the 16 bits are at least this
     float scale;
-    Rows w;
+    int chunks, along;        // warps' pieces of a row; log2 of the warps of a CTA that lie along a row
 };
 
 // The 128 bits of eight columns, two elements a word.
@@ -40,17 +42,19 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
     return make_uint4(c0, c1, c2, c3);
 }
 
-template <typename T>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A warp takes a piece of up to four rows (row_piece.cuh), a lane 16 (f32: 8) neighbouring
-// elements of each: whole groups of eight, so no two lanes compute the same numbers.
+// A warp takes a piece of a row, a lane 16 (f32: 8) neighbouring elements: whole groups of
+// eight, so no two lanes compute the same numbers.  8192 x 8192 bf16 with a sum: 66 us,
+// 6.1 TB/s; two rows a warp take 72, four 69, for fewer warps then fit an SM, and what hides a
+// warp's ten rounds is the reads of others.
 // Elements that are dropped are chosen away, not multiplied by zero: an infinity or a
 // NaN there does not come through.  x and add are read before y is written, by the
-// same warp, so y may be either.
+// same warp, so y may be either.  V: bytes that the rows, which are whole pieces, are
+// aligned to, 32 or 16; 0: any rows.
 template <typename T, int V, bool ADD>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, int64_t ldx, const T* add, int64_t lda, T* y,
                                                       int64_t ldy, DropoutParams p) {
@@ -58,68 +62,55 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* x, int64_t ldx, c
     __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    uint32_t* box = boxes[V ? 0 : threadIdx.x >> 5];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t* box = boxes[V ? 0 : warp];
     const uint32_t step = p.step + (p.step_at ? *p.step_at : 0u);
-    const Place at(p.w);
-    for (int64_t set = at.set; set < p.w.sets; set += at.set_step)
-        for (int chunk = at.chunk; chunk < p.w.chunks; chunk += at.chunk_step) {
-            const int64_t row = set_row(p.w, set), j0 = (int64_t)chunk * P::WARP, j = j0 + lane * P::E;
-            const int live = (int)min((int64_t)4, (p.rows - row + 31) >> 5);
-            const T* px = x + row * ldx + j0;
-            const T* pa = ADD ? add + row * lda + j0 : nullptr;
-            P v[4], a[4];
-            if constexpr (V == 0) {
-                typename P::Words r[4], s[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    r[q] = P::template fetch_any<false>(px + q * (32 * ldx), q < live ? p.cols - j0 : 0, lane);
-                    if (ADD) s[q] = P::template fetch_any<false>(pa + q * (32 * lda), q < live ? p.cols - j0 : 0, lane);
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    v[q].deal_any(r[q], P::between(px + q * (32 * ldx)), box, lane);
-                    if (ADD) a[q].deal_any(s[q], P::between(pa + q * (32 * lda)), box, lane);
-                }
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t left = q < live ? p.cols - j : 0;
-                    v[q].template load<V, false>(px + q * (32 * ldx) + lane * P::E, left);
-                    if (ADD) a[q].template load<V, false>(pa + q * (32 * lda) + lane * P::E, left);
-                }
+    const int64_t row = ((int64_t)blockIdx.x << (3 - p.along)) + (warp >> p.along);
+    if (row >= p.rows) return;
+    x += row * ldx;
+    if (ADD) add += row * lda;
+    y += row * ldy;
+    for (int chunk = (blockIdx.y << p.along) + (warp & ((1 << p.along) - 1)); chunk < p.chunks; chunk += gridDim.y << p.along) {
+        const int64_t j0 = (int64_t)chunk * P::WARP, j = j0 + lane * P::E;
+        P v, a;
+        if constexpr (V == 0) {
+            const auto r = P::template fetch_any<false>(x + j0, p.cols - j0, lane);
+            if (ADD) {
+                const auto s = P::template fetch_any<false>(add + j0, p.cols - j0, lane);
+                a.deal_any(s, P::between(add + j0), box, lane);
             }
+            v.deal_any(r, P::between(x + j0), box, lane);
+        } else {
+            if (j >= p.cols) break;
+            v.template load_whole<V, false>(x + j);
+            if (ADD) a.template load_whole<V, false>(add + j);
+        }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (q >= live) break;
+        for (int g = 0; g < P::E / 8; ++g) {
+            const uint4 r = philox((uint32_t)(j >> 3) + g, p.first_row + (uint32_t)row, step, p.site, p.key0, p.key1);
+            const uint32_t bits[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-                for (int g = 0; g < P::E / 8; ++g) {
-                    const uint4 r = philox((uint32_t)(j >> 3) + g, p.first_row + (uint32_t)(row + 32 * q), step, p.site,
-                                           p.key0, p.key1);
-                    const uint32_t bits[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int e = g * 8 + i * 2;
-                        float lo = (bits[i] & 0xffffu) >= p.drop ? __fmul_rn(v[q].value(e), p.scale) : 0.0f;
-                        float hi = (bits[i] >> 16) >= p.drop ? __fmul_rn(v[q].value(e + 1), p.scale) : 0.0f;
-                        if (ADD) {
-                            lo = __fadd_rn(a[q].value(e), lo);
-                            hi = __fadd_rn(a[q].value(e + 1), hi);
-                        }
-                        if constexpr (sizeof(T) == 2) {
-                            v[q].w[e / 2] = pack<T>(lo, hi);
-                        } else {
-                            v[q].w[e] = __float_as_uint(lo);
-                            v[q].w[e + 1] = __float_as_uint(hi);
-                        }
-                    }
+            for (int i = 0; i < 4; ++i) {
+                const int e = g * 8 + i * 2;
+                float lo = (bits[i] & 0xffffu) >= p.drop ? __fmul_rn(v.value(e), p.scale) : 0.0f;
+                float hi = (bits[i] >> 16) >= p.drop ? __fmul_rn(v.value(e + 1), p.scale) : 0.0f;
+                if (ADD) {
+                    lo = __fadd_rn(a.value(e), lo);
+                    hi = __fadd_rn(a.value(e + 1), hi);
                 }
-                if constexpr (V == 0)
-                    v[q].store_any(y + (row + 32 * q) * ldy + j0, p.cols - j0, box, lane);
-                else
-                    v[q].template store<V>(y + (row + 32 * q) * ldy + j, p.cols - j);
+                if constexpr (sizeof(T) == 2) {
+                    v.w[e / 2] = pack(lo, hi);
+                } else {
+                    v.w[e] = __float_as_uint(lo);
+                    v.w[e + 1] = __float_as_uint(hi);
+                }
             }
         }
+        if constexpr (V == 0)
+            v.store_any(y + j0, p.cols - j0, box, lane);
+        else
+            v.template store<V>(y + j, P::E);
+    }
 }
 
 template <typename T, int V>
@@ -134,10 +125,14 @@ int launch(rt_ctx* ctx, dim3 grid, const rt_tensor* x, const rt_tensor* add, rt_
 
 template <typename T>
 int launch_dropout(rt_ctx* ctx, const rt_tensor* x, const rt_tensor* add, rt_tensor* y, DropoutParams p) {
-    dim3 grid;
-    p.w = rows_for(ctx, p.rows, p.cols, Piece<T>::WARP, &grid);
+    p.chunks = (int)((p.cols + Piece<T>::WARP - 1) / Piece<T>::WARP);
+    for (p.along = 0; p.along < 3 && p.chunks % (2 << p.along) == 0;) ++p.along;
+    const int64_t groups = (p.rows + (8 >> p.along) - 1) >> (3 - p.along);
+    RT_CHECK(groups <= INT_MAX, "rt_dropout: %lld rows are too many", (long long)p.rows);
+    const dim3 grid((unsigned)groups, (unsigned)std::min(p.chunks >> p.along, 65535));
     int v = std::min(access_of(x), access_of(y));
     if (add) v = std::min(v, access_of(add));
+    if (p.cols % Piece<T>::E) v = 0;
     if (v == 32) return launch<T, 32>(ctx, grid, x, add, y, p);
     if (v == 16) return launch<T, 16>(ctx, grid, x, add, y, p);
     return launch<T, 0>(ctx, grid, x, add, y, p);

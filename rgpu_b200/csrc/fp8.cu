@@ -84,8 +84,15 @@ __global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* 
 #pragma unroll
                 for (int q = 0; q < 4; ++q) x[q].deal_any(r[q], P::between(p + q * (32 * ld)), boxes[threadIdx.x >> 5], lane);
             } else {
+                // V: rows are whole pieces; in place of a row or a piece that is not there another is read
+                const T* at = src + row * ld + (j < k ? j : 0);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) x[q].template load<V>(p + q * (32 * ld) + lane * P::E, q < live ? k - j : 0);
+                for (int q = 0; q < 4; ++q) x[q].template load_whole<V, true>(at + min(q, live - 1) * (32 * ld));
+                if (j >= k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[q].w[i] = 0;
             }
             uint32_t word[4];
             uint8_t* out = codes + row * row_bytes + j;
@@ -124,15 +131,15 @@ __global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* 
 }
 
 // Blocks down a column, laid out transposed.  A CTA takes 128 columns of src by one block
-// of 128 of its rows.  A thread holds 64 rows of one column (bf16: 32 of two neighbouring
+// of 128 of its rows.  A thread holds 32 rows of one column (bf16: of two neighbouring
 // ones), all its reads under way at once, a warp 128 bytes of a row each; the maxima of a
-// column's two (four) threads meet in shared memory.
-template <typename T, bool PAIR>
-__global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
-                                                               int64_t k, int64_t blocks, int64_t row_bytes,
-                                                               int64_t groups, uint8_t* __restrict__ codes,
-                                                               uint8_t* __restrict__ scales) {
-    constexpr int W = PAIR ? 2 : 1, N = 64 / W, SHARES = 128 / N;  // columns, rows of a thread; threads to a column
+// column's four threads meet in shared memory.  A thread's 32 codes of a column are one
+// sector of the output (WIDE: and one store, where the output's rows are so aligned).
+template <typename T, bool PAIR, bool WIDE>
+__global__ void __launch_bounds__(PAIR ? 256 : 512) quantize_columns_kernel(
+    const T* __restrict__ src, int64_t ld, int64_t rows, int64_t k, int64_t blocks, int64_t row_bytes, int64_t groups,
+    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    constexpr int W = PAIR ? 2 : 1, N = 32, SHARES = 128 / N;  // columns, rows of a thread; threads to a column
     __shared__ uint32_t maxima[SHARES][128];
     pdl_wait();
     pdl_launch_dependents();
@@ -157,7 +164,7 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restri
         } else if constexpr (sizeof(T) == 2) {
             v[0][i] = i < live && col < rows ? __bfloat162float(p[i * ld]) : 0.0f;
         } else {
-            v[0][i] = i < live && col < rows ? p[i * ld] : 0.0f;
+            v[0][i] = i < live && col < rows ? __ldg(p + i * ld) : 0.0f;
         }
     }
 #pragma unroll
@@ -176,16 +183,23 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restri
         for (int s = 0; s < SHARES; ++s) amax = max(amax, maxima[s][c + x]);
         const uint32_t byte = scale_byte(amax);
         const float inv = inv_scale(byte);
+        uint32_t e[N / 4];
+#pragma unroll
+        for (int y = 0; y < N / 4; ++y) {
+            const float* u = &v[x][4 * y];
+            e[y] = byte == kNanScale ? 0u : encode4(u[0], u[1], u[2], u[3], inv);
+        }
         uint8_t* out = codes + (col + x) * row_bytes + k0;
+        if constexpr (WIDE) {
+            if (k0 < row_bytes)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "r"(e[0]), "r"(e[1]),
+                             "r"(e[2]), "r"(e[3]), "r"(e[4]), "r"(e[5]), "r"(e[6]), "r"(e[7])
+                             : "memory");
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; i += 16) {
-            uint32_t e[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const float* u = &v[x][i + 4 * y];
-                e[y] = byte == kNanScale ? 0u : encode4(u[0], u[1], u[2], u[3], inv);
-            }
-            if (k0 + i < row_bytes) *reinterpret_cast<uint4*>(out + i) = make_uint4(e[0], e[1], e[2], e[3]);
+            for (int i = 0; i < N; i += 16)
+                if (k0 + i < row_bytes)
+                    *reinterpret_cast<uint4*>(out + i) = make_uint4(e[i / 4], e[i / 4 + 1], e[i / 4 + 2], e[i / 4 + 3]);
         }
         if (share == 0) {
             const int r = c + x;  // row of the scale tile
@@ -211,24 +225,21 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
         for (int chunk = at.chunk; chunk < w.chunks; chunk += at.chunk_step) {
             const int64_t row = set_row(w, set), j0 = (int64_t)chunk * P::WARP, j = j0 + lane * P::E;
             if (V ? j >= k : j0 >= k) continue;
-            const bool inside = j < k;
             const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);
             const uint4 s = __ldg(reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j0 >> 9)) * 512 + (row & 31) * 16));
             const uint32_t word[4] = {s.x, s.y, s.z, s.w};
-            const uint8_t* in = codes + row * row_bytes + j;
+            // without a branch (Piece::load_whole): another piece or row in place of one that is not there
+            const uint8_t* in = codes + row * row_bytes + (j < k ? j : j0);
             uint32_t c[4][P::E / 4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-#pragma unroll
-                for (int i = 0; i < P::E / 4; ++i) c[q][i] = 0;
-                if (q < live && inside) {
-                    if constexpr (P::E == 16) {
-                        const uint4 four = __ldg(reinterpret_cast<const uint4*>(in + q * (32 * row_bytes)));
-                        c[q][0] = four.x, c[q][1] = four.y, c[q][2] = four.z, c[q][3] = four.w;
-                    } else {
-                        const uint2 two = __ldg(reinterpret_cast<const uint2*>(in + q * (32 * row_bytes)));
-                        c[q][0] = two.x, c[q][1] = two.y;
-                    }
+                const uint8_t* at = in + min(q, live - 1) * (32 * row_bytes);
+                if constexpr (P::E == 16) {
+                    const uint4 four = __ldg(reinterpret_cast<const uint4*>(at));
+                    c[q][0] = four.x, c[q][1] = four.y, c[q][2] = four.z, c[q][3] = four.w;
+                } else {
+                    const uint2 two = __ldg(reinterpret_cast<const uint2*>(at));
+                    c[q][0] = two.x, c[q][1] = two.y;
                 }
             }
             const int shift = (int)(j >> 7 & 3) * 8;
@@ -262,17 +273,22 @@ int launch_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_fp8* q) {
     if (axis == 1) {
         dim3 grid;
         const Rows w = rows_for(ctx, q->rows, q->k, Piece<T>::WARP, &grid);
-        const int v = access_of(src);
+        const int v = q->k % Piece<T>::E ? 0 : access_of(src);
         auto* kernel = v == 32 ? quantize_rows_kernel<T, 32> : v == 16 ? quantize_rows_kernel<T, 16> : quantize_rows_kernel<T, 0>;
         RT_CUDA(launch_k(ctx->pdl, kernel, grid, 256, 0, ctx->stream, p, src->ld, q->rows, q->k, w, q->row_bytes(),
                          q->groups(), q->codes, q->scales));
     } else {
         const int64_t grid = q->blocks() * ((q->rows + 127) / 128);
         RT_CHECK(grid <= INT_MAX, "rt_fp8_quantize: src is too large");
-        auto* kernel = quantize_columns_kernel<T, false>;
+        const bool wide = ((reinterpret_cast<uintptr_t>(q->codes) | (uintptr_t)q->row_bytes()) & 31) == 0;
+        auto* kernel = wide ? quantize_columns_kernel<T, false, true> : quantize_columns_kernel<T, false, false>;
+        int threads = 512;
         if constexpr (sizeof(T) == 2)
-            if ((reinterpret_cast<uintptr_t>(p) & 3) == 0 && src->ld % 2 == 0) kernel = quantize_columns_kernel<T, true>;
-        RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)grid, 256, 0, ctx->stream, p, src->ld, q->rows, q->k, q->blocks(),
+            if ((reinterpret_cast<uintptr_t>(p) & 3) == 0 && src->ld % 2 == 0) {
+                kernel = wide ? quantize_columns_kernel<T, true, true> : quantize_columns_kernel<T, true, false>;
+                threads = 256;
+            }
+        RT_CUDA(launch_k(ctx->pdl, kernel, (unsigned)grid, threads, 0, ctx->stream, p, src->ld, q->rows, q->k, q->blocks(),
                          q->row_bytes(), q->groups(), q->codes, q->scales));
     }
     count_launch(ctx);

@@ -14,26 +14,41 @@ namespace rt {
 // (one 256-bit access, Blackwell's widest) or 16 where the rows are so aligned.
 // Else (0) a warp's accesses take neighbouring words, which change hands through its
 // kilobyte of shared memory; an aligned row's last piece goes element by element.
-// NC: the kernel writes none of what it reads.
 template <typename T>
 struct Piece {
     static constexpr int E = 32 / sizeof(T);         // elements
     static constexpr int WARP = 32 * E;              // elements of a warp
     uint32_t w[8];
 
-    template <int V, bool NC = true>
-    __device__ __forceinline__ void load(const T* p, int64_t left) {
-        if (V == 32 && left >= E && !NC) {
+    // All of the piece.  Without a branch, so that one load is not waited for before the next
+    // is issued (dropout of 8192 x 8192 bf16 78 us, with load below 92).  NC: the kernel
+    // writes none of what it reads.
+    template <int V, bool NC>
+    __device__ __forceinline__ void load_whole(const T* p) {
+        if constexpr (V == 32 && NC) {
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(p));
+        } else if constexpr (V == 32) {
             asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                          : "l"(p)
                          : "memory");
-        } else if (V == 32 && left >= E) {
+        } else {
+            const uint4* at = reinterpret_cast<const uint4*>(p);
+            const uint4 a = NC ? __ldg(at) : at[0], b = NC ? __ldg(at + 1) : at[1];
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+        }
+    }
+    template <int V>
+    __device__ __forceinline__ void load(const T* p, int64_t left) {
+        if (V == 32 && left >= E) {
             asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                          : "l"(p));
         } else if (V == 16 && left >= E) {
-            const uint4 *at = reinterpret_cast<const uint4*>(p), a = NC ? __ldg(at) : *at, b = NC ? __ldg(at + 1) : at[1];
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
             w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
             w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
         } else {
