@@ -149,23 +149,29 @@ __global__ void __launch_bounds__(PAIR ? 256 : 512) quantize_columns_kernel(
     float v[W][N];
     const T* p = src + k0 * ld + col;
     const int live = (int)max((int64_t)0, min((int64_t)N, k - k0));
+    if (live == N && col + W <= rows) {  // without conditions on each: all loads are issued, then waited for
+        uint32_t u[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if constexpr (PAIR) {
-            uint32_t u = 0;
-            if (i < live && col < rows) {
-                if (col + 1 < rows)
-                    u = __ldg(reinterpret_cast<const uint32_t*>(p + i * ld));
-                else
-                    u = *reinterpret_cast<const uint16_t*>(p + i * ld);
-            }
-            v[0][i] = __uint_as_float(u << 16);
-            v[1][i] = __uint_as_float(u & 0xffff0000u);
-        } else if constexpr (sizeof(T) == 2) {
-            v[0][i] = i < live && col < rows ? __bfloat162float(p[i * ld]) : 0.0f;
-        } else {
-            v[0][i] = i < live && col < rows ? __ldg(p + i * ld) : 0.0f;
+        for (int i = 0; i < N; ++i) {
+            if constexpr (PAIR || sizeof(T) == 4) u[i] = __ldg(reinterpret_cast<const uint32_t*>(p + i * ld));
+            else u[i] = *reinterpret_cast<const uint16_t*>(p + i * ld);
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[0][i] = __uint_as_float(sizeof(T) == 4 ? u[i] : u[i] << 16);
+            if constexpr (PAIR) v[1][i] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int x = 0; x < W; ++x) {
+                v[x][i] = 0.0f;
+                if (i < live && col + x < rows) {
+                    if constexpr (sizeof(T) == 2) v[x][i] = __bfloat162float(p[i * ld + x]);
+                    else v[x][i] = p[i * ld + x];
+                }
+            }
     }
 #pragma unroll
     for (int x = 0; x < W; ++x) {
