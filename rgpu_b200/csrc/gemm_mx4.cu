@@ -563,31 +563,28 @@ __device__ __forceinline__ void transpose32(float (&v)[32], int lane) {
 // 1024 bf16 36 us, where 4096 columns, aligned, take 18.  c: the first row's; rows, left: how many rows and columns there are from it on.
 template <typename T>
 __device__ __forceinline__ void store_columns(T* c, int64_t ldc, int64_t rows, int64_t left, const float* bias,
-                                              float floor, int lane, float (&v)[4][32]) {
+                                              float floor, int lane, float (&v)[32]) {
+    transpose32(v, lane);
+    const float b = bias[lane];
+    T* to = c + lane;
+    if (lane < left)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        transpose32(v[k], lane);
-        const float b = bias[k * 32 + lane];
-        T* to = c + k * 32 + lane;
-        if (k * 32 + lane < left)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i < rows) store_one(to + i * ldc, at_least(v[k][i] + b, floor));
-    }
+        for (int i = 0; i < 32; ++i)
+            if (i < rows) store_one(to + i * ldc, at_least(v[i] + b, floor));
 }
 
-// 128 neighbouring elements of a row of C.  ACCESS: bytes that every 32 of them are
+// 32 neighbouring elements of a row of C.  ACCESS: bytes that they are
 // aligned to (32 or 16; past the row's end element by element).
 template <typename T, int ACCESS>
-__device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias, float floor, float (&v)[4][32]) {
+__device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias, float floor, float (&v)[32]) {
     constexpr int E = ACCESS / (int)sizeof(T);  // elements of a store
 #pragma unroll
-    for (int k = 0; k < 128; k += E) {
+    for (int k = 0; k < 32; k += E) {
         float x[E];
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
             const float4 b = *reinterpret_cast<const float4*>(bias + k + i);
-            const float* y = &v[k / 32][k % 32 + i];
+            const float* y = &v[k + i];
             x[i] = at_least(y[0] + b.x, floor), x[i + 1] = at_least(y[1] + b.y, floor);
             x[i + 2] = at_least(y[2] + b.z, floor), x[i + 3] = at_least(y[3] + b.w, floor);
         }
@@ -616,8 +613,24 @@ __device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias,
     }
 }
 
-// ALIGNED: C's rows are 16-byte aligned.
-template <typename F, bool ALIGNED>
+// A warp's 32 rows (lanes) of 32 columns of C from column `col` on; rows: how many there
+// are from the lane's on.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void store_block(const Mx4Params& p, int64_t row, int64_t rows, int64_t col, const float* bias,
+                                            float floor, int lane, float (&v)[32]) {
+    T* to = static_cast<T*>(p.c) + row * p.ldc + col;
+    if constexpr (!ALIGNED) {
+        store_columns(to - lane * p.ldc, p.ldc, rows + lane, p.n - col, bias, floor, lane, v);
+    } else if (rows > 0) {
+        if (p.access == 32) store_row<T, 32>(to, p.n - col, bias, floor, v);
+        else store_row<T, 16>(to, p.n - col, bias, floor, v);
+    }
+}
+
+// ALIGNED: C's rows are 16-byte aligned.  SPLIT: a cluster is two to four pairs, which share
+// one tile and split k.  They leave their sums in shared memory, and each adds up a share of
+// the tile's columns, in order of the splits.
+template <typename F, bool ALIGNED, bool SPLIT>
 __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ CUtensorMap map_t,
                                                                    const __grid_constant__ CUtensorMap map_sw,
@@ -641,9 +654,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     volatile int* issued_peer = issued_all + 1;  // (leader) its peer
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const uint32_t rank = cta_rank();
-    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+    const uint32_t in_cluster = cta_rank(), rank = in_cluster & 1u, leader = in_cluster - rank;  // rank: in the pair
+    const int splits = SPLIT ? (int)cluster_size() / 2 : 1, split = SPLIT ? (int)(in_cluster >> 1) : 0;
+    const int cluster = SPLIT ? blockIdx.x / (2 * splits) : blockIdx.x >> 1, clusters = SPLIT ? gridDim.x / (2 * splits) : gridDim.x >> 1;
     const int tiles = p.tiles_m * p.tiles_n;
+    const int s0 = SPLIT ? split * p.stages_per_split : 0, s1 = SPLIT ? min(p.stages, s0 + p.stages_per_split) : p.stages;
+    float* sums = reinterpret_cast<float*>(smem);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -678,19 +694,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     auto raise_abort = [&](int code) {
         record_error(p.err, code, blockIdx.x);
         *abort_flag = 1;
-        store_cluster(in_cta(smem_u32((const void*)abort_flag), rank ^ 1u), 1u);
+        store_cluster(in_cta(smem_u32((const void*)abort_flag), in_cluster ^ 1u), 1u);
     };
 
     if (warp == 0) {
         const uint32_t w0 = smem_u32(smem_w), t0 = smem_u32(smem_t), sc0 = smem_u32(smem_s);
-        const uint32_t full0 = smem_u32(full), leader_full0 = in_cta(full0, 0), empty0 = smem_u32(empty);
+        const uint32_t full0 = smem_u32(full), leader_full0 = in_cta(full0, leader), empty0 = smem_u32(empty);
         int slot = 0, phase = 1, issued = 0;
         bool ok = true;
         for (int t = cluster; t < tiles && ok; t += clusters) {
             int tm, tn;
             pair_tile(p, t, tm, tn);
             const int w_row = tn * 256 + (int)rank * 128, t_row = tm * 256 + (int)rank * 128;
-            for (int s = 0; s < p.stages; ++s) {
+            for (int s = s0; s < s1; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + slot * 8, phase, abort_flag));
                 if (!ok) break;
                 if (elect_one()) {
@@ -712,23 +728,23 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         if (elect_one()) {
             *issued_all = issued;
             if (rank != 0) {
-                store_cluster(in_cta(smem_u32((const void*)issued_peer), 0), (uint32_t)issued);
-                arrive_cluster(in_cta(smem_u32(told), 0));
+                store_cluster(in_cta(smem_u32((const void*)issued_peer), leader), (uint32_t)issued);
+                arrive_cluster(in_cta(smem_u32(told), leader));
             }
             if (!ok) raise_abort(DEV_TIMEOUT_PRODUCER);
         }
     } else if (warp == 1 && rank == 0) {
         const uint64_t w0 = smem_desc(smem_u32(smem_w), 16, 1024), t0 = smem_desc(smem_u32(smem_t), 16, 1024);
         const uint64_t sc0 = scale_desc(smem_u32(smem_s));
-        const uint32_t empty0 = smem_u32(empty), empty1 = in_cta(empty0, 1);
-        const uint32_t tfull0 = smem_u32(tfull), tfull1 = in_cta(tfull0, 1);
+        const uint32_t empty0 = smem_u32(empty), empty1 = in_cta(empty0, leader + 1);
+        const uint32_t tfull0 = smem_u32(tfull), tfull1 = in_cta(tfull0, leader + 1);
         int slot = 0, phase = 0, done = 0;
         bool ok = true;
         for (int t = cluster; t < tiles && ok; t += clusters, ++done) {
             ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(tempty), (done & 1) ^ 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            for (int s = 0; s < p.stages; ++s) {
+            for (int s = s0; s < s1; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), phase, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
@@ -748,7 +764,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                         if (kk < steps)
                             mma_scaled<F, 2>(tmem, td + kk * 2, wd + kk * 2, F::idesc(256, 256, kk, s),
                                              cols + F::tile(kk) * 4, cols + 8 + F::tile(kk) * 8,
-                                             (s > 0 || kk > 0) ? 1u : 0u);
+                                             (s > s0 || kk > 0) ? 1u : 0u);
                     commit_pair(empty0 + slot * 8);
                     commit_pair(empty1 + slot * 8);
                 }
@@ -800,30 +816,54 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             tmem_ld_wait(v);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), 0));
-            const int64_t at = row * p.ldc + col0, left = p.n - col0, rows = p.m - row;
-            const float floor = p.relu ? 0.0f : -INFINITY;
-            if constexpr (!ALIGNED) {
-                const int64_t first = at - lane * p.ldc;
-                if (p.out_bf16)
-                    store_columns(static_cast<__nv_bfloat16*>(p.c) + first, p.ldc, rows + lane, left, bias, floor, lane, v);
-                else
-                    store_columns(static_cast<float*>(p.c) + first, p.ldc, rows + lane, left, bias, floor, lane, v);
-            } else if (rows > 0) {
-                if (p.out_bf16) {
-                    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.c) + at;
-                    if (p.access == 32) store_row<__nv_bfloat16, 32>(to, left, bias, floor, v);
-                    else store_row<__nv_bfloat16, 16>(to, left, bias, floor, v);
-                } else {
-                    float* to = static_cast<float*>(p.c) + at;
-                    if (p.access == 32) store_row<float, 32>(to, left, bias, floor, v);
-                    else store_row<float, 16>(to, left, bias, floor, v);
+            if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), leader));
+            if constexpr (SPLIT) {
+                // [column][row]; every stage has been read
+                float* to = sums + half * 128 * 128 + quad * 32 + lane;
+#pragma unroll
+                for (int j = 0; j < 128; ++j) to[j * 128] = v[j / 32][j % 32];
+            } else {
+                const float floor = p.relu ? 0.0f : -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (p.out_bf16) store_block<__nv_bfloat16, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, v[c]);
+                    else store_block<float, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, v[c]);
                 }
             }
         }
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
     }
     __syncwarp();
+    if constexpr (SPLIT) {
+        sync_cluster();
+        if (warp >= 2) {
+            // the split's blocks of 32 columns, dealt out over the two warps of a lane quadrant
+            const int quad = warp & 3, half = (warp - 2) >> 2;
+            int tm, tn;
+            pair_tile(p, cluster, tm, tn);
+            const int64_t row = (int64_t)tm * 256 + rank * 128 + quad * 32 + lane;
+            const float floor = p.relu ? 0.0f : -INFINITY;
+            for (int block = (split * 8 + splits - 1) / splits + half; block * splits / 8 == split && block < 8; block += 2) {
+                float x[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = 0.0f;
+                for (int r = 0; r < splits; ++r) {
+                    const uint32_t from = in_cta(smem_u32(sums + block * 32 * 128 + quad * 32 + lane), (uint32_t)(2 * r) + rank);
+                    float y[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y[j]) : "r"(from + j * 512) : "memory");
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] += y[j];
+                }
+                const int64_t col = (int64_t)tn * 256 + block * 32;
+                const float* bias = smem_bias + (block / 4 * 4) * 128 + block % 4 * 32;  // as a warp of that half left it
+                if (p.out_bf16) store_block<__nv_bfloat16, ALIGNED>(p, row, p.m - row, col, bias, floor, lane, x);
+                else store_block<float, ALIGNED>(p, row, p.m - row, col, bias, floor, lane, x);
+            }
+        }
+        __syncwarp();
+    }
     __syncthreads();
     if (*abort_flag && rank == 0 && threadIdx.x == 0) {
         // the pair's copies complete on the leader's barriers
@@ -907,6 +947,9 @@ namespace {
 template <typename F, int TN>
 int launch_one(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p, int splits, cudaStream_t stream) {
     using G = Geo1<F, TN>;
+    // A second tile's scales would begin at an odd TMEM column, which the MMA does not take (a
+    // tile of 64 tokens has them at column 0 or 2).
+    if (TN == 32) RT_CHECK(p.m <= 32, "block-scaled product: %lld tokens in a tile of 32", (long long)p.m);
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[TN / 64], &sw = b.maps.scales[0], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + TN - 1) / TN);
     p.tiles_n = (int)((p.n + 127) / 128);
@@ -933,15 +976,20 @@ int launch_one(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p,
     return RT_OK;
 }
 
-template <typename F>
-int launch_pair(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p, cudaStream_t stream) {
+template <typename F, bool SPLIT = false>
+int launch_pair(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p, cudaStream_t stream, int splits = 1) {
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[1], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     RT_CHECK(tiles <= INT32_MAX, "block-scaled product: C is too large");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
+    if (SPLIT) {
+        p.stages_per_split = (p.stages + splits - 1) / splits;
+        splits = (p.stages + p.stages_per_split - 1) / p.stages_per_split;
+    }
+    // persistent, or a cluster for each tile
+    cfg.gridDim = dim3((unsigned)(SPLIT ? 2 * splits * tiles : 2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
     cfg.blockDim = dim3(kPairThreads);
     cfg.dynamicSmemBytes = kPairSmem<F>;
     cfg.stream = stream;
@@ -949,12 +997,12 @@ int launch_pair(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = 2 * splits;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctx->pdl ? 2 : 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, p.access >= 16 ? mx4_pair_kernel<F, true> : mx4_pair_kernel<F, false>, w, t, sw, st, p));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, p.access >= 16 ? mx4_pair_kernel<F, true, SPLIT> : mx4_pair_kernel<F, false, SPLIT>, w, t, sw, st, p));
     count_launch(ctx);
     return RT_OK;
 }
@@ -970,8 +1018,8 @@ int allow_all() {
     RT_TRY((allow_smem<F, 32>()));
     RT_TRY((allow_smem<F, 64>()));
     RT_TRY((allow_smem<F, 128>()));
-    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<F, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<F>));
-    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<F, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<F>));
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<F, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<F>));
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<F, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<F>));
     return RT_OK;
 }
 
@@ -979,10 +1027,43 @@ int allow_all() {
 
 int gemm_mx4_init() {
     RT_TRY(allow_all<Mx4>());
-    return allow_all<Fp8>();
+    RT_TRY(allow_all<Fp8>());
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<Fp8, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<Fp8>));
+    RT_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<Fp8, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem<Fp8>));
+    return RT_OK;
 }
 
 namespace {
+
+// The tiles of an 8-bit product of more than 32 tokens and at most two 64-token tiles to an
+// SM (`tiles` of them).  A stage is half as deep as in 4 bits, so there are twice as many, and
+// the rule is its own; bf16 out, us, operands in L2:
+//  - two to an SM: 128-token tiles, one to an SM, from 9 stages on (512 x 4096 x 4096: 12.5, 64 tokens 14.4;
+//    2048 x 1000 x 1024, 8 stages: 7.6 / 7.2); from 49 on pairs that split k (2048 x 1000 x 8192:
+//    18.5 / 128 tokens 21.1; 512 x 4096 x 8192: 18.7 / 20.6; with 32 stages 13.3 / 11.7)
+//  - fewer, but 32 or more of 128 tokens, and more than 32 stages: those, k split until every
+//    SM has one (1024 x 1000 x 8192: 13.4 in two, 64 tokens in two 15.0; 256 x 1000 x 8192, 16 such tiles: 10.6 in four / 9.0)
+//  - else 64 tokens, k split while a CTA has more than 8 stages and every SM at most one
+//    CTA (256 x 4096 x 2048: 6.9 in one, 8.4 in two), two only above 24 stages (128 x 4096 x 8192: 14.2 in four, 16.4
+//    in two); in eight only where that leaves half of the SMs idle (128 x 1000 x 8192: 8.6 in four, 9.9 in eight)
+int launch_fp8(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, const Mx4Params& p, int64_t tiles, cudaStream_t stream) {
+    const int64_t sms = ctx->sm_count, tiles128 = ((p.m + 127) / 128) * ((p.n + 127) / 128);
+    const int64_t pairs = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    int splits = 1;
+    if (tiles > sms) {
+        if (p.stages > 48 && p.m >= 256 && pairs * 4 <= sms) return launch_pair<Fp8, true>(ctx, a, b, p, stream, 2);
+        if (p.stages > 8 && tiles128 <= sms) return launch_one<Fp8, 128>(ctx, a, b, p, 1, stream);
+        return launch_one<Fp8, 64>(ctx, a, b, p, 1, stream);
+    }
+    if (p.m > 64 && p.stages > 32 && tiles128 >= 32) {
+        while (splits < 4 && tiles128 * splits * 2 <= sms) splits *= 2;
+        return launch_one<Fp8, 128>(ctx, a, b, p, splits, stream);
+    }
+    while (splits < 8 && p.stages > 8 * splits &&
+           (tiles * splits * (splits == 4 ? 4 : 2) <= sms || (splits < 4 && p.stages > 24 * splits && tiles * splits <= sms)))
+        splits *= 2;
+    return launch_one<Fp8, 64>(ctx, a, b, p, splits, stream);
+}
 
 template <typename F>
 int launch_product(rt_ctx* ctx, const typename F::Matrix& a, const typename F::Matrix& b, const rt_tensor& c,
@@ -1016,6 +1097,8 @@ int launch_product(rt_ctx* ctx, const typename F::Matrix& a, const typename F::M
     const int tn = p.m <= 32 ? 32 : 64;
     const int64_t tiles = ((p.m + tn - 1) / tn) * ((p.n + 127) / 128), slots = 2 * (int64_t)ctx->sm_count;
     if (tiles > slots) return launch_pair<F>(ctx, a, b, p, stream);
+    if constexpr (F::GROUPS == 1)
+        if (tn == 64) return launch_fp8(ctx, a, b, p, tiles, stream);
     if (tiles > ctx->sm_count && p.stages > 8 && ((p.m + 127) / 128) * ((p.n + 127) / 128) <= ctx->sm_count)
         return launch_one<F, 128>(ctx, a, b, p, 1, stream);
     // Split k until a CTA has at most 8 stages, within those slots: joining the splits costs
