@@ -610,6 +610,11 @@ int rt_var_sum(rt_var* a, rt_var** out);
 int rt_var_mean(rt_var* a, rt_var** out);
 /* Var::softmax (ops.rs:288-309): row softmax with its O(c) adjoint. */
 int rt_var_softmax(rt_var* a, rt_var** out);
+/* No counterpart in the reference: rt_dropout on a variable (mask->step_at must
+ * be NULL), and rt_embedding_forward of a table (a watched parameter, say); the
+ * tokens are copied into the tape. */
+int rt_var_dropout(rt_var* a, const rt_dropout_mask* mask, rt_var** out);
+int rt_var_embedding(rt_var* table, const rt_tensor* tokens, float scale, rt_var** out);
 /* losses::mse (losses.rs:31-34), losses::mae (46-55) and
  * losses::binary_cross_entropy (143-160) against an f32 target of the
  * prediction's shape (copied into the tape). */

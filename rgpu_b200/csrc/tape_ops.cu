@@ -452,6 +452,82 @@ int rt_var_unary(rt_var* a, rt_unary_op op, float param, rt_var** out) {
     return RT_OK;
 }
 
+// The next two hand their buffers to the op-level calls of the same operators, as tensors on the stack.
+static rt_tensor as_tensor(rt_ctx* ctx, const Buf& b) {
+    rt_tensor t;
+    t.ctx = ctx;
+    t.ptr = b.p;
+    t.rows = b.rows;
+    t.cols = b.cols;
+    t.ld = b.ld;
+    return t;
+}
+
+int rt_var_dropout(rt_var* a, const rt_dropout_mask* mask, rt_var** out) {
+    RT_TRY(check_var(a));
+    RT_CHECK(mask && out, "rt_var_dropout: bad arguments");
+    RT_CHECK(!mask->step_at, "rt_var_dropout: step_at may change before the backward sweep: give the step");
+    rt_tape* t = a->tape;
+    const Buf X = t->nodes[a->idx].value;
+    Buf Y;
+    RT_TRY(t->alloc(Y, X.rows, X.cols));
+    const rt_dropout_mask m = *mask;
+    const rt_tensor x = as_tensor(t->ctx, X);
+    rt_tensor y = as_tensor(t->ctx, Y);
+    RT_TRY(rt_dropout(t->ctx, &x, nullptr, &y, &m));
+    const int ia = a->idx;
+    *out = t->push({ia},
+                   [t, ia, m](const Buf& g) -> int {
+                       Buf gx;
+                       RT_TRY(t->alloc(gx, g.rows, g.cols));
+                       const rt_tensor dy = as_tensor(t->ctx, g);
+                       rt_tensor dx = as_tensor(t->ctx, gx);
+                       RT_TRY(rt_dropout(t->ctx, &dy, nullptr, &dx, &m));
+                       return t->accumulate(ia, gx);
+                   },
+                   Y);
+    return RT_OK;
+}
+
+int rt_var_embedding(rt_var* table, const rt_tensor* tokens, float scale, rt_var** out) {
+    RT_TRY(check_var(table));
+    RT_CHECK(tokens && out, "rt_var_embedding: bad arguments");
+    rt_tape* t = table->tape;
+    RT_CHECK(tokens->ctx == t->ctx, "tensor belongs to another context");
+    RT_CHECK(tokens->dtype == RT_U32 && (tokens->rows <= 1 || tokens->ld == tokens->cols),
+             "rt_var_embedding: tokens must be packed u32");
+    const Buf E = t->nodes[table->idx].value;
+    const int64_t count = tokens->rows * tokens->cols;
+    const int64_t words = rt_embedding_backward_workspace(count, E.rows, E.cols);
+    if (words < 0) return RT_ERR_INVALID;
+    Buf Y, ids;  // the tokens, kept for the backward sweep (a word holds one)
+    RT_TRY(t->alloc(Y, count, E.cols));
+    RT_TRY(t->alloc(ids, 1, count));
+    if (count > 0)
+        RT_CUDA(cudaMemcpyAsync(ids.p, tokens->ptr, (size_t)count * 4, cudaMemcpyDeviceToDevice, t->ctx->stream));
+    auto token_tensor = [t, ids]() {
+        rt_tensor v = as_tensor(t->ctx, ids);
+        v.dtype = RT_U32;
+        return v;
+    };
+    const rt_tensor e = as_tensor(t->ctx, E), v = token_tensor();
+    rt_tensor y = as_tensor(t->ctx, Y);
+    RT_TRY(rt_embedding_forward(t->ctx, &e, &v, scale, &y));
+    const int ie = table->idx;
+    *out = t->push({ie},
+                   [t, ie, E, token_tensor, words, scale](const Buf& g) -> int {
+                       Buf work, &d = t->grads[ie];
+                       const bool more = d.p != nullptr;  // rows that occur are added to it, no other is touched
+                       if (!more) RT_TRY(t->alloc(d, E.rows, E.cols));
+                       RT_TRY(t->alloc(work, 1, words));
+                       const rt_tensor dy = as_tensor(t->ctx, g), v = token_tensor();
+                       rt_tensor de = as_tensor(t->ctx, d), w = as_tensor(t->ctx, work);
+                       return rt_embedding_backward(t->ctx, &v, &dy, scale, more, &de, &w);
+                   },
+                   Y);
+    return RT_OK;
+}
+
 int rt_var_binary(rt_var* a, rt_var* b, rt_binary_op op, rt_var** out) {
     RT_TRY(check_var(a));
     RT_TRY(check_var(b));

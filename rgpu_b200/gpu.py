@@ -206,6 +206,8 @@ _SIGS = [
     ("rt_var_unary", C.c_int, [C.c_void_p, C.c_int, C.c_float, C.POINTER(C.c_void_p)]),
     ("rt_var_sum", C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     ("rt_var_mean", C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
+    ("rt_var_dropout", C.c_int, [C.c_void_p, C.POINTER(DropoutMask), C.POINTER(C.c_void_p)]),
+    ("rt_var_embedding", C.c_int, [C.c_void_p, C.c_void_p, C.c_float, C.POINTER(C.c_void_p)]),
     ("rt_var_softmax", C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     ("rt_loss_mse", C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
     ("rt_loss_mae", C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),

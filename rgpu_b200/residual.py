@@ -10,14 +10,19 @@ their gradients one ``Gpu.block_backward``.  ``Mx4ResidualMlp`` holds the traine
 weights in microscaled 4-bit floating point and answers with 4-bit products.
 The reference has neither (its networks are plain Dense stacks, nn.rs:161-207).
 
+``TokenResidualMlp`` is the same over a window of tokens: embeddings, dropout,
+and the Dense layers' products in 8 bits.
+
     python -m rgpu_b200.residual        trains on points in four quadrants and
                                         compares the f32 and the 4-bit answers
+    python -m rgpu_b200.residual tokens trains to say the next token of a text
+                                        drawn from a random grammar
 """
 from __future__ import annotations
 
 import numpy as np
 
-from .gpu import Gpu, GpuTensor, Norm, upload_labels
+from .gpu import Dropout, Gpu, GpuTensor, Norm, upload_labels
 
 
 class ResidualMlp:
@@ -67,15 +72,27 @@ class ResidualMlp:
     def forward(self, x: GpuTensor) -> GpuTensor:
         """Logits [batch, classes] of x [batch, inputs]."""
         g, p = self.gpu, self.params
-        g.matmul_bias(x, p["w_in"], self._z[0], p["b_in"], False)
+        self._dense(x, "w_in", "b_in", self._z[0])
         g.block_forward(self._z[0], pre=self._pre(0), h=self._h[0])
         for i in range(self.blocks):
-            g.matmul_bias(self._h[i], p[f"w1_{i}"], self._a[i], p[f"b1_{i}"], True)
-            g.matmul_bias(self._a[i], p[f"w2_{i}"], self._y[i], p[f"b2_{i}"], False)
+            self._dense(self._h[i], f"w1_{i}", f"b1_{i}", self._a[i], relu=True)
+            self._drop(self._a[i], i)
+            self._dense(self._a[i], f"w2_{i}", f"b2_{i}", self._y[i])
             g.block_forward(self._z[i], y=self._y[i], post=self._post(i), gate=p[f"gate_{i}"], scale=self.scale,
                             z=self._z[i + 1], pre=self._pre(i + 1), h=self._h[i + 1])
-        g.matmul_bias(self._h[-1], p["w_out"], self._logits, p["b_out"], False)
+        self._dense(self._h[-1], "w_out", "b_out", self._logits)
         return self._logits
+
+    # What a kind of model does its own way: a Dense layer's products, and dropout of block i's hidden activations or
+    # of their gradient (in place; here there is none).
+    def _dense(self, x: GpuTensor, w: str, b: str, y: GpuTensor, relu: bool = False):
+        self.gpu.matmul_bias(x, self.params[w], y, self.params[b], relu)
+
+    def _dense_dx(self, dy: GpuTensor, w: str, dx: GpuTensor):
+        self.gpu.matmul_a_bt(dy, self.params[w], dx)
+
+    def _drop(self, a: GpuTensor, i: int):
+        pass
 
     def _dense_grads(self, x: GpuTensor, dy: GpuTensor, w: str, b: str):
         self.gpu.matmul_at_b(x, dy, self.grads[w])
@@ -86,7 +103,7 @@ class ResidualMlp:
         g, p, d = self.gpu, self.params, self.grads
         g.softmax_xent(self._logits, labels, self._delta, self._loss)
         self._dense_grads(self._h[-1], self._delta, "w_out", "b_out")
-        g.matmul_a_bt(self._delta, p["w_out"], self._dh)
+        self._dense_dx(self._delta, "w_out", self._dh)
         dz = None  # the last block's stream has no reader but the norm before the head
         for i in reversed(range(self.blocks)):
             g.block_backward(self._z[i + 1], y=self._y[i], post=self._post(i), gate=p[f"gate_{i}"], scale=self.scale,
@@ -95,10 +112,11 @@ class ResidualMlp:
                              work=self._work)
             dz = self._dz
             self._dense_grads(self._a[i], self._dy, f"w2_{i}", f"b2_{i}")
-            g.matmul_a_bt(self._dy, p[f"w2_{i}"], self._da)
+            self._dense_dx(self._dy, f"w2_{i}", self._da)
+            self._drop(self._da, i)
             g.relu_bwd(self._a[i], self._da)
             self._dense_grads(self._h[i], self._da, f"w1_{i}", f"b1_{i}")
-            g.matmul_a_bt(self._da, p[f"w1_{i}"], self._dh)
+            self._dense_dx(self._da, f"w1_{i}", self._dh)
         g.block_backward(self._z[0], pre=self._pre(0), dz=dz, dh=self._dh, dr=self._dz, dgamma_pre=d["pre_0"],
                          work=self._work)
         self._dense_grads(x, self._dz, "w_in", "b_in")
@@ -117,6 +135,91 @@ class ResidualMlp:
 
     def predict(self, x: np.ndarray) -> np.ndarray:
         return self.gpu.download(self.forward(self.gpu.upload(x))).argmax(1)
+
+
+class TokenResidualMlp(ResidualMlp):
+    """A ResidualMlp over a window of tokens: its input is their embeddings side
+    by side, scaled by sqrt(embed); a place of the window without a token holds
+    an index past the vocabulary and gives zeros.  While it trains, a share
+    `dropout` of the embeddings and of every block's hidden activations is
+    dropped.  products: "fp8" takes the Dense layers' three products in 8 bits
+    (parameters, stream and gradients stay f32), "f32" as they are."""
+
+    def __init__(self, gpu: Gpu, vocabulary: int, context: int, embed: int, width: int, hidden: int, classes: int,
+                 blocks: int, batch: int, *, dropout: float = 0.1, products: str = "fp8", seed: int = 0, **kw):
+        if embed % 4:
+            raise ValueError("embed must be a multiple of 4: a window's embeddings lie side by side")
+        if products not in ("fp8", "f32"):
+            raise ValueError(f"unknown products {products!r}")
+        super().__init__(gpu, context * embed, width, hidden, classes, blocks, batch, seed=seed, **kw)
+        self.vocabulary, self.context, self.embed = vocabulary, context, embed
+        self.dropout, self.seed, self.training, self.fp8 = dropout, seed, True, products == "fp8"
+        table = np.random.default_rng(seed + 1).standard_normal((vocabulary, embed)).astype(np.float32) / np.sqrt(embed)
+        self.params["embedding"] = gpu.upload(table)
+        for held in (self.grads, self._m, self._v):
+            held["embedding"] = gpu.zeros(table.shape)
+        rows = batch * context
+        self._x, self._dx = (gpu.zeros((rows, embed)) for _ in range(2))
+        # the same memory as rows of the batch
+        self._x_rows, self._dx_rows = (gpu.wrap(t.ptr, (batch, self.inputs)) for t in (self._x, self._dx))
+        self._embedding_work = gpu.zeros((gpu.embedding_backward_workspace(rows, vocabulary, embed),))
+        self._held = {}  # buffers of the 8-bit operands by layer, role and axis
+
+    def _mask(self, site: int) -> Dropout:
+        # the step that is under way: backward sees the same as forward
+        return Dropout(self.dropout, self.seed, site=site, step=self.steps)
+
+    def _drop(self, a: GpuTensor, i: int):
+        if self.training and self.dropout:
+            self.gpu.dropout(a, a, self._mask(1 + i))
+
+    def _quantized(self, layer: str, role: str, t: GpuTensor, axis: int):
+        """t in 8 bits, in the buffer of the layer's operand of that role."""
+        key = (layer, role, axis)
+        self._held[key] = self.gpu.fp8_quantize(t, self._held.get(key), axis=axis)
+        return self._held[key]
+
+    def _dense(self, x, w, b, y, relu=False):
+        if not self.fp8:
+            return super()._dense(x, w, b, y, relu)
+        self.gpu.fp8_matmul(self._quantized(w, "x", x, 1), self._quantized(w, "w", self.params[w], 0), y, bias=self.params[b],
+                            relu=relu)
+
+    def _dense_dx(self, dy, w, dx):
+        if not self.fp8:
+            return super()._dense_dx(dy, w, dx)
+        self.gpu.fp8_matmul(self._quantized(w, "dy", dy, 1), self._quantized(w, "w", self.params[w], 1), dx)
+
+    def _dense_grads(self, x, dy, w, b):
+        if not self.fp8:
+            return super()._dense_grads(x, dy, w, b)
+        self.gpu.fp8_matmul(self._quantized(w, "x", x, 0), self._quantized(w, "dy", dy, 0), self.grads[w])
+        self.gpu.colsum(dy, self.grads[b], self._colsum)
+
+    def forward(self, tokens: GpuTensor) -> GpuTensor:
+        """Logits [batch, classes] of tokens, u32 [batch * context]."""
+        g = self.gpu
+        g.embedding_forward(self.params["embedding"], tokens, self._x, scale=float(np.sqrt(self.embed)))
+        if self.training and self.dropout:
+            g.dropout(self._x_rows, self._x_rows, self._mask(0))
+        return super().forward(self._x_rows)
+
+    def backward(self, tokens: GpuTensor, labels: GpuTensor):
+        g = self.gpu
+        super().backward(self._x_rows, labels)
+        self._dense_dx(self._dz, "w_in", self._dx_rows)
+        if self.training and self.dropout:
+            g.dropout(self._dx_rows, self._dx_rows, self._mask(0))
+        g.embedding_backward(tokens, self._dx, self.grads["embedding"], self._embedding_work,
+                             scale=float(np.sqrt(self.embed)))
+
+    def predict(self, tokens: np.ndarray) -> np.ndarray:
+        """Classes of tokens [batch, context], without dropout."""
+        was, self.training = self.training, False
+        try:
+            return self.gpu.download(self.forward(upload_labels(self.gpu, tokens.ravel()))).argmax(1)
+        finally:
+            self.training = was
 
 
 class Mx4ResidualMlp:
@@ -173,5 +276,36 @@ def main(steps: int = 150):
           f"they agree on {np.mean(full == small):.3f}")
 
 
+def sentences(rows: int, context: int, vocabulary: int, seed: int):
+    """Windows of a text in which a token is followed by one of three that depend
+    on it and the one before, and the tokens that follow; places before the
+    beginning hold the index `vocabulary`."""
+    rng = np.random.default_rng(seed)
+    t = np.full((rows, context + 1), vocabulary, np.int64)
+    begin = rng.integers(0, context, rows)  # padding in front
+    for j in range(context + 1):
+        before, last = (t[:, j - k] % vocabulary if j >= k else np.zeros(rows, np.int64) for k in (2, 1))
+        following = (7 * last + 3 * before + rng.integers(0, 3, rows)) % vocabulary
+        t[:, j] = np.where(j < begin, vocabulary, np.where(j == begin, rng.integers(0, vocabulary, rows), following))
+    return t[:, :-1].astype(np.uint32), t[:, -1].astype(np.uint32)
+
+
+def main_tokens(steps: int = 300, vocabulary: int = 61):
+    gpu = Gpu(0)
+    models = {kind: TokenResidualMlp(gpu, vocabulary, context=8, embed=32, width=256, hidden=512, classes=vocabulary,
+                                     blocks=3, batch=1024, scale=0.5, products=kind) for kind in ("f32", "fp8")}
+    for step in range(steps):
+        x, labels = sentences(1024, 8, vocabulary, step)
+        for kind, model in models.items():
+            model.step(upload_labels(gpu, x.ravel()), upload_labels(gpu, labels), 1e-3)
+            if step % 60 == 0 or step == steps - 1:
+                print(f"step {step}: {kind} products, loss {model.loss():.4f}")
+    x, labels = sentences(1024, 8, vocabulary, 10**6)
+    print("next token right (a third is what can be known): " +
+          ", ".join(f"{kind} {np.mean(model.predict(x) == labels):.3f}" for kind, model in models.items()))
+
+
 if __name__ == "__main__":
-    main()
+    import sys
+
+    main_tokens() if sys.argv[1:] == ["tokens"] else main()

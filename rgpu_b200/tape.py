@@ -17,7 +17,7 @@ import ctypes as C
 
 import numpy as np
 
-from .gpu import Gpu, GpuTensor, _check, lib, upload_labels
+from .gpu import Dropout, Gpu, GpuTensor, _check, lib, upload_labels
 
 # rt_binary_op / rt_unary_op (include/rtgpu.h)
 ADD, SUB, MUL, DIV = range(4)
@@ -200,6 +200,18 @@ class Var:
     __mul__ = mul
     __truediv__ = div
     __neg__ = neg
+
+    def dropout(self, mask: Dropout) -> "Var":
+        """The values that the mask keeps over 1 - p, zeros elsewhere (new)."""
+        h = C.c_void_p()
+        _check(lib().rt_var_dropout(self.handle, C.byref(mask.args), C.byref(h)))
+        return Var(self.tape, h)
+
+    def embedding(self, tokens: GpuTensor, scale: float = 1.0) -> "Var":
+        """scale times this table's rows of the u32 tokens; zeros for those past it (new)."""
+        h = C.c_void_p()
+        _check(lib().rt_var_embedding(self.handle, tokens.handle, scale, C.byref(h)))
+        return Var(self.tape, h)
 
     def value(self) -> np.ndarray:
         h = C.c_void_p()

@@ -91,3 +91,49 @@ def embedding_backward(vocabulary, tokens, dy, scale):
             size[t] += abs(scale) * np.abs(dy[i])
             count[t] += 1
     return d, size, count
+
+
+def token_model(p, tokens, labels, blocks, scale, masks):
+    """Mean softmax cross-entropy and gradients of the residual MLP over windows of tokens
+    [batch, context] in 64 bits, RMS norms.  masks: for the embeddings and each block's hidden
+    activations what an element is multiplied by (1 / (1 - p) or 0)."""
+    from tests import ref_mx4 as N
+
+    eps = 1e-5
+    batch, context = tokens.shape
+    root = np.sqrt(p["embedding"].shape[1])
+    x = embedding(p["embedding"], tokens.ravel(), root).reshape(batch, -1) * masks[0]
+    z, h, a, y = [x @ p["w_in"] + p["b_in"]], [], [], []
+    h.append(N.norm(z[0], "rms", eps, p["pre_0"], 0.0))
+    for i in range(blocks):
+        a.append(np.maximum(h[i] @ p[f"w1_{i}"] + p[f"b1_{i}"], 0) * masks[1 + i])
+        y.append(a[i] @ p[f"w2_{i}"] + p[f"b2_{i}"])
+        zi, hi = N.block_forward(z[i], y[i], ("rms", eps, p[f"post_{i}"], 0.0), p[f"gate_{i}"], scale,
+                                 ("rms", eps, p[f"pre_{i + 1}"], 0.0))
+        z.append(zi)
+        h.append(hi)
+    logits = h[-1] @ p["w_out"] + p["b_out"]
+    e = np.exp(logits - logits.max(1, keepdims=True))
+    prob = e / e.sum(1, keepdims=True)
+    rows = np.arange(batch)
+    loss = -np.log(prob[rows, labels]).mean()
+    delta = prob.copy()
+    delta[rows, labels] -= 1
+    delta /= batch
+    g = {"w_out": h[-1].T @ delta, "b_out": delta.sum(0, keepdims=True)}
+    dh, dz = delta @ p["w_out"].T, 0.0
+    for i in reversed(range(blocks)):
+        b = N.block_backward(z[i + 1], y[i], ("rms", eps, p[f"post_{i}"], 0.0), p[f"gate_{i}"], scale,
+                             ("rms", eps, p[f"pre_{i + 1}"], 0.0), dz, dh)
+        g[f"pre_{i + 1}"], g[f"post_{i}"], g[f"gate_{i}"] = b["dgamma_pre"], b["dgamma_post"], b["dgate"].sum(0, keepdims=True)
+        dz, dy = b["dr"], b["dy"]
+        g[f"w2_{i}"], g[f"b2_{i}"] = a[i].T @ dy, dy.sum(0, keepdims=True)
+        da = (dy @ p[f"w2_{i}"].T) * masks[1 + i] * (a[i] > 0)
+        g[f"w1_{i}"], g[f"b1_{i}"] = h[i].T @ da, da.sum(0, keepdims=True)
+        dh = da @ p[f"w1_{i}"].T
+    b = N.block_backward(z[0], None, None, None, 1.0, ("rms", eps, p["pre_0"], 0.0), dz, dh)
+    g["pre_0"] = b["dgamma_pre"]
+    g["w_in"], g["b_in"] = x.T @ b["dr"], b["dr"].sum(0, keepdims=True)
+    dx = (b["dr"] @ p["w_in"].T) * masks[0]
+    g["embedding"] = embedding_backward(p["embedding"].shape[0], tokens.ravel(), dx.reshape(batch * context, -1), root)[0]
+    return loss, g

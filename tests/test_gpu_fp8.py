@@ -160,7 +160,9 @@ PRODUCTS = [(1, 1, 1), (1, 1, 16), (1, 17, 33), (2, 130, 64), (3, 128, 129), (16
             (2000, 2001, 1100), (1601, 2304, 800), (2305, 1537, 64), (4100, 3001, 33),
             # rings that turn over, unequal shares of k
             (2600, 2050, 1050), (1600, 2304, 1697), (7, 1000, 2176), (3, 520, 4100), (33, 300, 4608), (1, 128, 32801),
-            (2047, 1000, 1250), (500, 4096, 1041), (129, 9401, 2049)]
+            (2047, 1000, 1250), (500, 4096, 1041), (129, 9401, 2049),
+            # pairs that split k, evenly and not; 128 tokens with k split in two and four
+            (300, 4300, 6209), (2047, 1000, 6400), (513, 2300, 8193), (200, 2100, 4200), (1024, 1000, 4353)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

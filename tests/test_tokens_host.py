@@ -109,3 +109,22 @@ def test_reference_gradient_is_the_difference_quotient():
     d, size, count = R.embedding_backward(5, tokens, c, 1.5)
     assert abs(slope - (d * way).sum()) <= 1e-8 * (size * np.abs(way)).sum()
     assert count.tolist() == [1, 3, 0, 2, 0]
+
+
+def test_reference_model_gradient_is_the_difference_quotient():
+    rng = np.random.default_rng(5)
+    vocabulary, context, embed, width, hidden, batch = 6, 3, 4, 8, 10, 9
+    shapes = {"embedding": (vocabulary, embed), "w_in": (context * embed, width), "b_in": (1, width),
+              "w1_0": (width, hidden), "b1_0": (1, hidden), "w2_0": (hidden, width), "b2_0": (1, width),
+              "post_0": (1, width), "gate_0": (1, width), "pre_0": (1, width), "pre_1": (1, width),
+              "w_out": (width, 5), "b_out": (1, 5)}
+    p = {k: rng.standard_normal(s) for k, s in shapes.items()}
+    tokens, labels = rng.integers(0, vocabulary + 2, (batch, context)), rng.integers(0, 5, batch)
+    masks = [(rng.random(s) < 0.7) / 0.7 for s in ((batch, context * embed), (batch, hidden))]
+    _, g = R.token_model(p, tokens, labels, 1, 0.5, masks)
+    assert sorted(g) == sorted(p)
+    t = 1e-6
+    for k in p:
+        way = rng.standard_normal(p[k].shape)
+        up, down = (R.token_model(p | {k: p[k] + s * t * way}, tokens, labels, 1, 0.5, masks)[0] for s in (1, -1))
+        assert abs((up - down) / (2 * t) - (g[k] * way).sum()) <= 1e-6 * (1 + np.abs(g[k] * way).sum()), k
