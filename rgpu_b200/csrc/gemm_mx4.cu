@@ -627,9 +627,9 @@ __device__ __forceinline__ void store_block(const Mx4Params& p, int64_t row, int
     }
 }
 
-// ALIGNED: C's rows are 16-byte aligned.  SPLIT: a cluster is two to four pairs, which share
-// one tile and split k.  They leave their sums in shared memory, and each adds up a share of
-// the tile's columns, in order of the splits.
+// ALIGNED: C's rows are 16-byte aligned.  SPLIT: a cluster is two pairs, which share one
+// tile, each half of k.  Each leaves the sums of half of the columns (of every warp's 128, 64) in
+// shared memory for the other and adds up the other half: 2 us.
 template <typename F, bool ALIGNED, bool SPLIT>
 __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ CUtensorMap map_t,
@@ -655,8 +655,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t in_cluster = cta_rank(), rank = in_cluster & 1u, leader = in_cluster - rank;  // rank: in the pair
-    const int splits = SPLIT ? (int)cluster_size() / 2 : 1, split = SPLIT ? (int)(in_cluster >> 1) : 0;
-    const int cluster = SPLIT ? blockIdx.x / (2 * splits) : blockIdx.x >> 1, clusters = SPLIT ? gridDim.x / (2 * splits) : gridDim.x >> 1;
+    constexpr int CTAS = SPLIT ? 4 : 2;  // of a cluster
+    const int split = SPLIT ? (int)(in_cluster >> 1) : 0;
+    const int cluster = blockIdx.x / CTAS, clusters = gridDim.x / CTAS;
     const int tiles = p.tiles_m * p.tiles_n;
     const int s0 = SPLIT ? split * p.stages_per_split : 0, s1 = SPLIT ? min(p.stages, s0 + p.stages_per_split) : p.stages;
     float* sums = reinterpret_cast<float*>(smem);
@@ -697,6 +698,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
         store_cluster(in_cta(smem_u32((const void*)abort_flag), in_cluster ^ 1u), 1u);
     };
 
+    float own[2][SPLIT ? 32 : 1];  // SPLIT: an epilogue thread's 64 sums
     if (warp == 0) {
         const uint32_t w0 = smem_u32(smem_w), t0 = smem_u32(smem_t), sc0 = smem_u32(smem_s);
         const uint32_t full0 = smem_u32(full), leader_full0 = in_cta(full0, leader), empty0 = smem_u32(empty);
@@ -818,10 +820,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             __syncwarp();
             if (lane == 0) arrive_cluster(in_cta(smem_u32(tempty), leader));
             if constexpr (SPLIT) {
-                // [column][row]; every stage has been read
-                float* to = sums + half * 128 * 128 + quad * 32 + lane;
+                // the other's 64 columns, [column][row]; every stage has been read
+                float* to = sums + half * 64 * 128 + quad * 32 + lane;
 #pragma unroll
-                for (int j = 0; j < 128; ++j) to[j * 128] = v[j / 32][j % 32];
+                for (int j = 0; j < 64; ++j) {
+                    to[j * 128] = split ? v[j / 32][j % 32] : v[2 + j / 32][j % 32];
+                    if (!split) continue;
+                    v[j / 32][j % 32] = v[2 + j / 32][j % 32];  // its own in front
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) own[c][j] = v[c][j];
             } else {
                 const float floor = p.relu ? 0.0f : -INFINITY;
 #pragma unroll
@@ -837,29 +847,23 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
     if constexpr (SPLIT) {
         sync_cluster();
         if (warp >= 2) {
-            // the split's blocks of 32 columns, dealt out over the two warps of a lane quadrant
             const int quad = warp & 3, half = (warp - 2) >> 2;
             int tm, tn;
             pair_tile(p, cluster, tm, tn);
-            const int64_t row = (int64_t)tm * 256 + rank * 128 + quad * 32 + lane;
+            const int64_t row = (int64_t)tm * 256 + rank * 128 + quad * 32 + lane, col0 = (int64_t)tn * 256 + half * 128 + split * 64;
+            const float* bias = smem_bias + (warp - 2) * 128 + split * 64;
             const float floor = p.relu ? 0.0f : -INFINITY;
-            for (int block = (split * 8 + splits - 1) / splits + half; block * splits / 8 == split && block < 8; block += 2) {
-                float x[32];
+            const uint32_t from = in_cta(smem_u32(sums + half * 64 * 128 + quad * 32 + lane), in_cluster ^ 2u);
+            float y[2][32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] = 0.0f;
-                for (int r = 0; r < splits; ++r) {
-                    const uint32_t from = in_cta(smem_u32(sums + block * 32 * 128 + quad * 32 + lane), (uint32_t)(2 * r) + rank);
-                    float y[32];
+            for (int j = 0; j < 64; ++j)
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y[j / 32][j % 32]) : "r"(from + j * 512) : "memory");
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y[j]) : "r"(from + j * 512) : "memory");
+            for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] += y[j];
-                }
-                const int64_t col = (int64_t)tn * 256 + block * 32;
-                const float* bias = smem_bias + (block / 4 * 4) * 128 + block % 4 * 32;  // as a warp of that half left it
-                if (p.out_bf16) store_block<__nv_bfloat16, ALIGNED>(p, row, p.m - row, col, bias, floor, lane, x);
-                else store_block<float, ALIGNED>(p, row, p.m - row, col, bias, floor, lane, x);
+                for (int j = 0; j < 32; ++j) y[c][j] += own[c][j];
+                if (p.out_bf16) store_block<__nv_bfloat16, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, y[c]);
+                else store_block<float, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, y[c]);
             }
         }
         __syncwarp();
@@ -977,19 +981,16 @@ int launch_one(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p,
 }
 
 template <typename F, bool SPLIT = false>
-int launch_pair(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p, cudaStream_t stream, int splits = 1) {
+int launch_pair(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p, cudaStream_t stream) {
     const CUtensorMap &w = b.maps.codes[2], &t = a.maps.codes[2], &sw = b.maps.scales[1], &st = a.maps.scales[0];
     p.tiles_m = (int)((p.m + 255) / 256);
     p.tiles_n = (int)((p.n + 255) / 256);
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
     RT_CHECK(tiles <= INT32_MAX, "block-scaled product: C is too large");
     cudaLaunchConfig_t cfg = {};
-    if (SPLIT) {
-        p.stages_per_split = (p.stages + splits - 1) / splits;
-        splits = (p.stages + p.stages_per_split - 1) / p.stages_per_split;
-    }
+    p.stages_per_split = (p.stages + 1) / 2;  // SPLIT: two stages or more
     // persistent, or a cluster for each tile
-    cfg.gridDim = dim3((unsigned)(SPLIT ? 2 * splits * tiles : 2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
+    cfg.gridDim = dim3((unsigned)(SPLIT ? 4 * tiles : 2 * std::min<int64_t>(tiles, ctx->sm_count / 2)));
     cfg.blockDim = dim3(kPairThreads);
     cfg.dynamicSmemBytes = kPairSmem<F>;
     cfg.stream = stream;
@@ -997,7 +998,7 @@ int launch_pair(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, Mx4Params p
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2 * splits;
+    attr[0].val.clusterDim.x = SPLIT ? 4 : 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -1051,7 +1052,7 @@ int launch_fp8(rt_ctx* ctx, const rt_scaled& a, const rt_scaled& b, const Mx4Par
     const int64_t pairs = ((p.m + 255) / 256) * ((p.n + 255) / 256);
     int splits = 1;
     if (tiles > sms) {
-        if (p.stages > 48 && p.m >= 256 && pairs * 4 <= sms) return launch_pair<Fp8, true>(ctx, a, b, p, stream, 2);
+        if (p.stages > 48 && p.m >= 256 && pairs * 4 <= sms) return launch_pair<Fp8, true>(ctx, a, b, p, stream);
         if (p.stages > 8 && tiles128 <= sms) return launch_one<Fp8, 128>(ctx, a, b, p, 1, stream);
         return launch_one<Fp8, 64>(ctx, a, b, p, 1, stream);
     }
