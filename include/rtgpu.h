@@ -313,7 +313,9 @@ int rt_embedding_forward(rt_ctx* ctx, const rt_tensor* table, const rt_tensor* t
 /* Its gradient: dtable[v,:] = scale * sum over i with tokens[i] = v of dy[i,:],
  * every row of it (accumulate != 0: added to the rows that occur, the others
  * as they were).  dtable [vocabulary, n] f32, dy [count, n] f32 or bf16.  work:
- * rt_embedding_backward_workspace packed f32.  The positions are sorted by
+ * rt_embedding_backward_workspace packed f32, 16-byte aligned, used by this
+ * call only (calls that may run at the same time, or graphs replayed so, need
+ * one each).  The positions are sorted by
  * token and summed in a fixed order: results do not change from run to run.
  * At most 2^21 - 1 rows of dtable, 2^31 - 1 tokens. */
 int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, float scale, int accumulate,
@@ -336,7 +338,8 @@ typedef struct {
                                  (a captured step can count by itself); may be NULL */
     int64_t first_row;        /* row number of x's first row (of a global batch); rows end by 2^32 */
 } rt_dropout_mask;
-/* y = add + keep . x / (1 - q); add may be NULL (zeros), y may be x or add; all
+/* y = add + keep . x / (1 - q); add may be NULL (zeros), y may be x or add (and
+ * overlap them in no other way); all
  * of one type, f32 or bf16.  The gradient of x is the same call with x = dy,
  * add = NULL; that of add is dy.  A dropped element of x is not looked at: a
  * NaN there does not come through. */

@@ -76,7 +76,10 @@ BACK = [("uniform", 1, 1, 1), ("uniform", 5, 3, 2), ("uniform", 63, 256, 300), (
         ("one", 5000, 264, 3), ("padding", 100, 16, 9), ("padding", 3000, 8, 70000), ("zipf", 1023, 100, 255),
         ("zipf", 2047, 1000, 256), ("zipf", 1025, 30, 257), ("zipf", 10000, 512, 5000), ("zipf", 4096, 24, 70001),
         ("uniform", 2049, 17, 2 ** 21 - 1), ("uniform", 70000, 9, 300), ("runs", 2500, 300, 11), ("runs", 9000, 72, 1000),
-        ("zipf", 300000, 8, 50257)]
+        ("zipf", 300000, 8, 50257),
+        # the sorts' other forms: over launches with more buckets than warps' counters, keys of three digits, wide gaps
+        ("uniform", 70000, 5, 2 ** 21 - 1), ("zipf", 66000, 4, 300000), ("one", 65537, 12, 100), ("padding", 70000, 4, 1000),
+        ("uniform", 5000, 5, 2 ** 21 - 1), ("one", 4097, 8, 2000003), ("zipf", 65536, 4, 66000), ("uniform", 12289, 130, 9000)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -215,3 +218,38 @@ def test_refusals(gpu):
     other = rgpu_b200.Gpu(0)
     refused(lambda: gpu.embedding_forward(other.zeros((10, 8)), t, y), "another context")
     refused(lambda: gpu.embedding_backward(t, y, e, other.zeros((5000,))), "another context")
+
+
+def test_offsets_past_32_bits(gpu):
+    # a table and a gradient of more than 2^31 elements: rows at both ends
+    vocabulary, n, count = 1100000, 2048, 5000
+    table = torch.zeros(vocabulary, n, dtype=torch.bfloat16, device="cuda")
+    table[-1], table[0], table[vocabulary // 2] = 3.0, 1.0, 2.0
+    tokens = np.random.default_rng(0).choice([0, vocabulary // 2, vocabulary - 1, vocabulary], count).astype(np.uint32)
+    torch.cuda.synchronize()
+    t, y = rgpu_b200.upload_labels(gpu, tokens), torch.zeros(count, n, device="cuda")
+    ty = gpu.wrap(y.data_ptr(), (count, n))
+    gpu.embedding_forward(gpu.wrap(table.data_ptr(), (vocabulary, n), "bf16"), t, ty)
+    gpu.sync()
+    want = np.select([tokens == 0, tokens == vocabulary // 2, tokens == vocabulary - 1], [1.0, 2.0, 3.0], 0.0)
+    assert np.array_equal(y.cpu().numpy(), np.repeat(want[:, None], n, 1))
+    del table
+    d = torch.full((vocabulary, n), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    gpu.embedding_backward(t, ty, gpu.wrap(d.data_ptr(), (vocabulary, n)),
+                           gpu.zeros((gpu.embedding_backward_workspace(count, vocabulary, n),)))
+    gpu.sync()
+    for row, value in ((0, 1), (vocabulary // 2, 2), (vocabulary - 1, 3)):
+        assert (d[row] == value * np.sum(tokens == row)).all()  # whole numbers
+        d[row] = 0
+    assert not d.any(), "a row of a token that does not occur is not zero"
+
+
+def test_a_vector_of_tokens_may_be_a_column(gpu):
+    t = gpu.wrap(rgpu_b200.upload_labels(gpu, [3, 1, 2]).ptr, (3,), "u32")
+    column = gpu.wrap(t.ptr, (3, 1), "u32")
+    e, y, z = gpu.upload(np.arange(32).reshape(4, 8)), gpu.zeros((3, 8)), gpu.zeros((3, 8))
+    gpu.sync()
+    gpu.embedding_forward(e, t, y)
+    gpu.embedding_forward(e, column, z)
+    assert np.array_equal(gpu.download(y), gpu.download(z))

@@ -276,6 +276,36 @@ def test_same_bits_every_time_and_on_another_stream(gpu):
     assert np.array_equal(out[0], out[1]) and np.array_equal(out[0], out[2])
 
 
+@pytest.mark.parametrize("m,n,k", [(20, 300, 700), (300, 4300, 6209)])
+def test_captured(gpu, m, n, k):
+    x = torch.zeros(m, k, device="cuda")
+    w = torch.randn(k, n, device="cuda")
+    c = torch.zeros(m, n, device="cuda")
+    tx, tw, tc = (gpu.wrap(t.data_ptr(), t.shape) for t in (x, w, c))
+    qx, qw = gpu.fp8_zeros(m, k), gpu.fp8_zeros(n, k)
+    gpu.sync()
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    gpu.set_stream(stream.cuda_stream)
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            gpu.fp8_quantize(tx, qx)
+            gpu.fp8_quantize(tw, qw, axis=0)
+            gpu.fp8_matmul(qx, qw, tc)
+    finally:
+        gpu.set_stream(None)
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        x.copy_(torch.randn(m, k, device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = c.clone()
+        gpu.fp8_matmul(gpu.fp8_quantize(tx), gpu.fp8_quantize(tw, axis=0), tc)
+        gpu.sync()
+        assert torch.equal(got, c) and got.any()
+
+
 def test_refusals(gpu):
     q = gpu.fp8_zeros(4, 64)
     f = gpu.zeros((4, 64))
