@@ -317,7 +317,7 @@ int rt_embedding_forward(rt_ctx* ctx, const rt_tensor* table, const rt_tensor* t
  * call only (calls that may run at the same time, or graphs replayed so, need
  * one each).  The positions are sorted by
  * token and summed in a fixed order: results do not change from run to run.
- * At most 2^21 - 1 rows of dtable, 2^31 - 1 tokens. */
+ * At most 2^31 - 1 rows of dtable and tokens. */
 int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, float scale, int accumulate,
                           rt_tensor* dtable, rt_tensor* work);
 /* f32 elements of work for `count` tokens (-1: bad extents). */

@@ -10,8 +10,8 @@
 // same call gives the same bits.  Three ways by how many positions there are:
 //  - up to kFew one launch (few_kernel): every CTA sorts the positions of its own rows
 //  - up to kChunk * kMaxCluster the sort takes one cluster (cluster_sort_kernel)
-//  - above, three launches (bucket_*): keys have at most 21 bits, one pass over the high
-//    bits deals the positions out to buckets, a CTA a bucket finishes by the low bits
+//  - above, passes over launches (digit_*), each of which moves all positions: how often
+//    the most frequent token occurs does not decide how evenly a pass is spread
 // In the last two the rows of tokens that do not occur are written beside the sort
 // (fill_kernel), then piece_kernel and row_kernel sum.  65536 x 1024 bf16 rows of 50257
 // tokens as frequent as words: 75 us, 52 of bytes; 2047 x 1000 f32 of 1000: 7.6 us.
@@ -25,7 +25,6 @@ namespace rt {
 namespace {
 
 constexpr int64_t kMaxWidth = 1 << 22;  // spans fit a grid's second extent
-constexpr int64_t kMaxVocabulary = (1 << 21) - 1;  // keys 0 .. V fit 21 bits
 
 // A lane's N columns (4 or 8) of a warp's span of 32 N.  ACCESS: bytes that the rows are
 // aligned to, 32 or 16: neighbouring columns, by accesses of that width; the row's length is
@@ -164,23 +163,19 @@ __global__ void __launch_bounds__(256) lookup_kernel(const TE* __restrict__ tabl
 }
 
 // -------------------------------------------------------------------- backward
-// The workspace, in 32-bit words.  B: CTAs of the first pass; bins: buckets; a run's
-// partial sums: two rows of `width` floats (n rounded up to 8) a piece.
+// The sort's arrays in the workspace, in 32-bit words.  A key is a token, or V for padding.
 struct Sort {
     int64_t count, vocabulary;
-    int low, high;       // bits of a key: bucket high, order in it low
-    int ctas;            // of the first pass
-    int64_t span;        // positions of a CTA
-    uint32_t* counts;    // [ctas][bins]
-    uint32_t* bucket;    // [bins + 1] first position of each bucket
-    uint32_t* key;       // [count] keys in bucket order
+    int passes;          // by 8 bits of a key
+    int ctas;            // of a pass over launches,
+    int64_t span;        // and positions of a CTA
+    uint32_t* counts;    // [ctas][256]
+    uint32_t* key;       // [count] between passes,
     uint32_t* place;     // [count] and their positions
     uint32_t* token;     // [count] sorted
     uint32_t* position;  // [count]
     uint32_t* start;     // [vocabulary + 1] first of each token in the sorted list
 };
-
-constexpr int kMaxHigh = 11, kMaxLow = 10;
 
 __device__ __forceinline__ uint32_t key_of(const Sort& s, const uint32_t* tokens, int64_t i) {
     return min(__ldg(tokens + i), (uint32_t)s.vocabulary);
@@ -216,18 +211,28 @@ __device__ __forceinline__ void in_order(int64_t n, int warp, int lane, Key key,
     }
 }
 
-// How many positions of each CTA's span fall in each bucket.
-__global__ void __launch_bounds__(256) bucket_count_kernel(Sort s, const uint32_t* __restrict__ tokens) {
-    extern __shared__ uint32_t cnt[];
+// A pass over launches: from the tokens themselves (keys null) or what the pass before
+// left, to `to_key` and `to_place`.
+struct Pass {
+    const uint32_t *tokens, *keys, *places;
+    uint32_t *to_key, *to_place;
+    int shift;
+    __device__ __forceinline__ uint32_t key(const Sort& s, int64_t i) const { return keys ? keys[i] : key_of(s, tokens, i); }
+    __device__ __forceinline__ uint32_t place(int64_t i) const { return keys ? places[i] : (uint32_t)i; }
+};
+
+// How many positions of each CTA's span have each digit.
+__global__ void __launch_bounds__(256) digit_count_kernel(Sort s, Pass p) {
+    __shared__ uint32_t cnt[256];
+    cnt[threadIdx.x] = 0;
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int bins = 1 << s.high;
-    for (int i = threadIdx.x; i < bins; i += 256) cnt[i] = 0;
-    __syncthreads();
     const int64_t first = blockIdx.x * s.span, n = min(s.span, s.count - first);
-    for (int64_t i = threadIdx.x; i < n; i += 256) atomicAdd(&cnt[key_of(s, tokens, first + i) >> s.low], 1u);
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += 256) atomicAdd(&cnt[p.key(s, first + i) >> p.shift & 255u], 1u);
     __syncthreads();
-    for (int i = threadIdx.x; i < bins; i += 256) s.counts[(int64_t)blockIdx.x * bins + i] = cnt[i];
+    s.counts[(int64_t)blockIdx.x * 256 + threadIdx.x] = cnt[threadIdx.x];
 }
 
 // Exclusive sums of v[0..bins) in place, by the whole CTA; sums holds a word a warp.
@@ -255,116 +260,88 @@ __device__ __forceinline__ void exclusive(uint32_t* v, int bins, uint32_t* sums)
     __syncthreads();
 }
 
-// Deals the positions out to their buckets, in order.  A CTA adds up the CTAs' counts
+// Moves the positions to their digits' places, in order.  A CTA adds up the CTAs' counts
 // itself: with at most 256 of them that is cheaper than a launch that does it once.
-template <int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) bucket_deal_kernel(Sort s, const uint32_t* __restrict__ tokens) {
-    extern __shared__ uint32_t shared[];
-    constexpr int THREADS = WARPS * 32;
-    const int bins = 1 << s.high;
-    uint32_t* base = shared;         // [bins] of the whole list
-    uint32_t* own = base + bins;     // [bins] of the CTAs before this one
-    uint32_t* cnt = own + bins;      // [warps][bins]
-    __shared__ uint32_t sums[WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int b = threadIdx.x; b < bins * (WARPS + 2); b += THREADS) shared[b] = 0;
+__global__ void __launch_bounds__(1024) digit_deal_kernel(Sort s, Pass p) {
+    constexpr int WARPS = 32, BINS = 256, PARTS = 4;
+    __shared__ uint32_t cnt[WARPS][BINS];
+    __shared__ uint32_t base[BINS], own[BINS], sums[WARPS];  // of the whole list; of the CTAs before this one
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bin = threadIdx.x % BINS;
+    for (int i = threadIdx.x; i < WARPS * BINS; i += 1024) cnt[0][i] = 0;
+    if (threadIdx.x < BINS) base[bin] = own[bin] = 0;
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int parts = max(1, THREADS / bins);
-    for (int i = threadIdx.x; i < bins * parts; i += THREADS) {
-        const int b = i & (bins - 1), part = i >> s.high;
+    {
         uint32_t all = 0, before = 0;
 #pragma unroll 8
-        for (int c = part; c < s.ctas; c += parts) {
-            const uint32_t x = s.counts[(int64_t)c * bins + b];
+        for (int c = threadIdx.x / BINS; c < s.ctas; c += PARTS) {
+            const uint32_t x = s.counts[(int64_t)c * BINS + bin];
             all += x;
             if (c < (int)blockIdx.x) before += x;
         }
-        atomicAdd(&base[b], all);
-        atomicAdd(&own[b], before);
+        atomicAdd(&base[bin], all);
+        atomicAdd(&own[bin], before);
     }
     const int64_t first = blockIdx.x * s.span, n = min(s.span, s.count - first);
-    uint32_t* mine = cnt + warp * bins;
-    auto key = [&](int64_t i) { return key_of(s, tokens, first + i); };
-    in_order<WARPS>(n, warp, lane, key, [&](int64_t, uint32_t k, bool there) { count_rank(mine, k >> s.low, there, lane); });
+    auto key = [&](int64_t i) { return p.key(s, first + i); };
+    in_order<WARPS>(n, warp, lane, key, [&](int64_t, uint32_t k, bool there) { count_rank(cnt[warp], k >> p.shift & 255u, there, lane); });
     __syncthreads();
-    exclusive<WARPS>(base, bins, sums);
-    for (int b = threadIdx.x; b < bins; b += THREADS) {
-        uint32_t run = base[b];
-        if (blockIdx.x == 0) s.bucket[b] = run;
-        run += own[b];
+    exclusive<WARPS>(base, BINS, sums);
+    if (threadIdx.x < BINS) {
+        uint32_t run = base[bin] + own[bin];
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const uint32_t x = cnt[w * bins + b];
-            cnt[w * bins + b] = run;
+            const uint32_t x = cnt[w][bin];
+            cnt[w][bin] = run;
             run += x;
         }
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) s.bucket[bins] = (uint32_t)s.count;
     __syncthreads();
     in_order<WARPS>(n, warp, lane, key, [&](int64_t i, uint32_t k, bool there) {
-        const uint32_t to = count_rank(mine, k >> s.low, there, lane);
+        const uint32_t to = count_rank(cnt[warp], k >> p.shift & 255u, there, lane);
         if (there) {
-            s.key[to] = k;
-            s.place[to] = (uint32_t)(first + i);
+            p.to_key[to] = k;
+            p.to_place[to] = p.place(first + i);
         }
     });
 }
 
-// Sorts a bucket by the low bits and writes where each of its tokens starts.
-template <int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) bucket_sort_kernel(Sort s) {
-    extern __shared__ uint32_t shared[];
-    constexpr int THREADS = WARPS * 32;
-    const int bins = 1 << s.low;
-    uint32_t* base = shared;        // [bins]
-    uint32_t* cnt = shared + bins;  // [warps][bins]
-    __shared__ uint32_t sums[WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int b = threadIdx.x; b < bins * WARPS; b += THREADS) cnt[b] = 0;
+// Where each token starts in the sorted list: at the places where the key changes, for the
+// tokens from the one after the last key to the new one.  Few by the thread that finds
+// them, else by a warp, thousands by the CTA.
+__global__ void __launch_bounds__(256) starts_kernel(Sort s) {
+    __shared__ uint32_t list[257], found;
+    if (threadIdx.x == 0) found = 0;
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t first = s.bucket[blockIdx.x], n = s.bucket[blockIdx.x + 1] - first;
-    uint32_t* mine = cnt + warp * bins;
-    const uint32_t mask = (uint32_t)bins - 1;
-    auto key = [&](int64_t i) { return s.key[first + i]; };
-    in_order<WARPS>(n, warp, lane, key, [&](int64_t, uint32_t k, bool there) { count_rank(mine, k & mask, there, lane); });
-    __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += THREADS) {
-        uint32_t all = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) all += cnt[w * bins + b];
-        base[b] = all;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t first = (int64_t)blockIdx.x * 256, i = first + threadIdx.x;
+    auto from = [&](int64_t at) { return at ? (int64_t)s.token[at - 1] + 1 : (int64_t)0; };
+    auto upto = [&](int64_t at) { return at < s.count ? (int64_t)s.token[at] : s.vocabulary; };
+    if (i < s.count) {
+        const int64_t b = from(i), e = upto(i);
+        if (e - b >= 8)
+            list[atomicAdd(&found, 1u)] = threadIdx.x;
+        else
+            for (int64_t t = b; t <= e; ++t) s.start[t] = (uint32_t)i;
+        if (i == s.count - 1) list[atomicAdd(&found, 1u)] = threadIdx.x + 1;  // the tokens behind the last
     }
     __syncthreads();
-    exclusive<WARPS>(base, bins, sums);
-    for (int b = threadIdx.x; b < bins; b += THREADS) {
-        uint32_t run = (uint32_t)first + base[b];
-        const int64_t token = ((int64_t)blockIdx.x << s.low) + b;
-        if (token <= s.vocabulary) s.start[token] = run;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const uint32_t x = cnt[w * bins + b];
-            cnt[w * bins + b] = run;
-            run += x;
-        }
+    for (int g = 0; g < (int)found; ++g) {
+        const int64_t at = first + list[g], b = from(at), e = upto(at);
+        if (e - b >= 4096)
+            for (int64_t t = b + threadIdx.x; t <= e; t += 256) s.start[t] = (uint32_t)at;
+        else if (g % 8 == warp)
+            for (int64_t t = b + lane; t <= e; t += 32) s.start[t] = (uint32_t)at;
     }
-    __syncthreads();
-    in_order<WARPS>(n, warp, lane, key, [&](int64_t i, uint32_t k, bool there) {
-        const uint32_t to = count_rank(mine, k & mask, there, lane);
-        if (there) {
-            s.token[to] = k;
-            s.position[to] = s.place[first + i];
-        }
-    });
 }
 
 // The whole sort in one launch where the positions fit the shared memory of one cluster:
 // a CTA holds kChunk of them, and passes by 8 bits of the key, the low ones first, move
 // them through distributed shared memory.  65536 positions of 50257 tokens: about 10 us; the
-// launches above take 25.
+// launches above take as long, but leave no SM idle for fill_kernel.
 constexpr int kChunk = 4096, kMaxCluster = 16, kStride = 257;  // kStride: counters of a warp, off a bank each
 
 struct ClusterSmem {
@@ -398,7 +375,7 @@ __device__ __forceinline__ void sync_cluster() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32_t* __restrict__ tokens, int passes) {
+__global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32_t* __restrict__ tokens) {
     extern __shared__ __align__(16) uint8_t raw[];
     ClusterSmem& m = *reinterpret_cast<ClusterSmem*>(raw);
     pdl_wait();
@@ -412,7 +389,7 @@ __global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32
 #pragma unroll
     for (int x = 0; x < 4; ++x)
         if (slot + x * 32 < live) item[x] = make_uint2(key_of(s, tokens, first + slot + x * 32), (uint32_t)first + slot + x * 32);
-    for (int pass = 0; pass < passes; ++pass) {
+    for (int pass = 0; pass < s.passes; ++pass) {
         const int shift = pass * 8;
         for (int i = threadIdx.x; i < 32 * kStride; i += 1024) m.cnt[i] = 0;
         if (pass)
@@ -895,10 +872,7 @@ int bits_of(int64_t v) {
 
 // The workspace's layout from its sizes; the words it needs.
 int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) {
-    const int bits = std::max(1, bits_of(vocabulary));
-    s->low = std::max(0, bits - 8);
-    if (s->low > kMaxLow) s->low = kMaxLow;
-    s->high = bits - s->low;
+    s->passes = (std::max(1, bits_of(vocabulary)) + 7) / 8;
     s->count = count;
     s->vocabulary = vocabulary;
     // spans of at least 1024 positions: with more CTAs each would add up more counts
@@ -920,17 +894,16 @@ int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) 
     s->position = take(count);
     s->start = take(vocabulary + 1);
     if (count <= kChunk * kMaxCluster) return at;  // the rest of the sort happens in shared memory
-    s->bucket = take((1 << s->high) + 1);
     s->key = take(count);
     s->place = take(count);
-    s->counts = take((int64_t)s->ctas << s->high);
+    s->counts = take((int64_t)s->ctas * 256);
     return at;
 }
 
 int check_backward(int64_t count, int64_t vocabulary, int64_t n) {
     RT_CHECK(count >= 0 && vocabulary >= 0 && n >= 0, "embedding: negative extent");
     RT_CHECK(count <= INT_MAX, "embedding: %lld positions are over 2^31 - 1", (long long)count);
-    RT_CHECK(vocabulary <= kMaxVocabulary, "embedding: the gradient of %lld tokens is over 2^21 - 1", (long long)vocabulary);
+    RT_CHECK(vocabulary <= INT_MAX, "embedding: the gradient of %lld tokens is over 2^31 - 1", (long long)vocabulary);
     RT_CHECK(n <= kMaxWidth, "embedding: %lld columns are over 2^22", (long long)n);
     return RT_OK;
 }
@@ -1001,10 +974,6 @@ int launch_sums(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, const
                           : launch_sums<T, 0>(ctx, dy, m);
 }
 
-// Shared memory of the kernels of the sort over launches.
-int deal_bytes(int high, int warps) { return (4 << high) * (warps + 2); }
-int sort_bytes(int low, int warps) { return (4 << low) * (warps + 1); }
-
 // The sort and, beside its last kernel, the rows of dE that no token has.
 int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, const Sums& m, const rt_tensor* dtable) {
     const bool pdl = ctx->pdl;
@@ -1012,19 +981,22 @@ int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, const Sums& m, co
     if (s.count <= kChunk * kMaxCluster) {
         int ranks = 1;
         while (ranks * kChunk < s.count) ranks *= 2;
-        RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t,
-                               (bits_of(s.vocabulary) + 7) / 8));
+        RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t));
         others -= ranks;
         count_launch(ctx);
     } else {
-    // With up to 256 buckets 32 warps a CTA, whose counters fit; with more (2^18 tokens and up) 8.
-    const int bins = 1 << s.high, warps = s.high <= 8 ? 32 : 8;
-    auto* deal = warps == 32 ? bucket_deal_kernel<32> : bucket_deal_kernel<8>;
-    auto* sort = warps == 32 ? bucket_sort_kernel<32> : bucket_sort_kernel<8>;
-    RT_CUDA(launch_k(pdl, bucket_count_kernel, s.ctas, 256, bins * 4, ctx->stream, s, t));
-    RT_CUDA(launch_k(pdl, deal, s.ctas, warps * 32, deal_bytes(s.high, warps), ctx->stream, s, t));
-    RT_CUDA(launch_k(pdl, sort, bins, warps * 32, sort_bytes(s.low, warps), ctx->stream, s));
-    count_launch(ctx, 3);
+        Pass p{t, nullptr, nullptr, nullptr, nullptr, 0};
+        for (int i = 0; i < s.passes; ++i, p.shift += 8) {
+            const bool last = (s.passes - 1 - i) % 2 == 0;  // to the arrays that the last pass writes
+            p.to_key = last ? s.token : s.key;
+            p.to_place = last ? s.position : s.place;
+            RT_CUDA(launch_k(pdl, digit_count_kernel, s.ctas, 256, 0, ctx->stream, s, p));
+            RT_CUDA(launch_k(pdl, digit_deal_kernel, s.ctas, 1024, 0, ctx->stream, s, p));
+            p.keys = p.to_key;
+            p.places = p.to_place;
+        }
+        RT_CUDA(launch_k(pdl, starts_kernel, (unsigned)((s.count + 255) / 256), 256, 0, ctx->stream, s));
+        count_launch(ctx, 2 * s.passes + 1);
     }
     if (!m.accumulate) {
         // 16 rows or more to a CTA: each goes over all tokens
@@ -1050,8 +1022,6 @@ int check_tokens(const char* what, const rt_tensor* tokens, const rt_tensor* row
 }  // namespace
 
 int embedding_init() {
-    RT_CUDA(cudaFuncSetAttribute(bucket_deal_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, deal_bytes(kMaxHigh, 8)));
-    RT_CUDA(cudaFuncSetAttribute(bucket_sort_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_bytes(kMaxLow, 32)));
     RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSmem)));
     RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return RT_OK;

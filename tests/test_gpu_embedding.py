@@ -78,7 +78,7 @@ BACK = [("uniform", 1, 1, 1), ("uniform", 5, 3, 2), ("uniform", 63, 256, 300), (
         ("uniform", 2049, 17, 2 ** 21 - 1), ("uniform", 70000, 9, 300), ("runs", 2500, 300, 11), ("runs", 9000, 72, 1000),
         ("zipf", 300000, 8, 50257),
         # the sorts' other forms: over launches with more buckets than warps' counters, keys of three digits, wide gaps
-        ("uniform", 70000, 5, 2 ** 21 - 1), ("zipf", 66000, 4, 300000), ("one", 65537, 12, 100), ("padding", 70000, 4, 1000),
+        ("uniform", 70000, 5, 2 ** 21 - 1), ("zipf", 66000, 4, 300000), ("uniform", 70000, 1, 17000000), ("one", 65537, 12, 100), ("padding", 70000, 4, 1000),
         ("uniform", 5000, 5, 2 ** 21 - 1), ("one", 4097, 8, 2000003), ("zipf", 65536, 4, 66000), ("uniform", 12289, 130, 9000)]
 
 
@@ -214,7 +214,7 @@ def test_refusals(gpu):
     refused(lambda: gpu.embedding_backward(t, y, gpu.zeros((10, 9)), work), "dtable 10x9")
     refused(lambda: gpu.embedding_backward(t, gpu.zeros((4, 8)), e, work), "3 tokens for 4 rows")
     refused(lambda: gpu.embedding_backward(t, gpu.zeros((3, 8), "u32"), e, work), "f32 or bf16")
-    refused(lambda: gpu.embedding_backward(t, gpu.zeros((3, 1)), gpu.zeros((1 << 21, 1)), work), "2^21")
+    refused(lambda: gpu.embedding_backward(t, gpu.zeros((3, 1)), gpu.wrap(e.ptr, (1 << 31, 1)), work), "2^31")
     other = rgpu_b200.Gpu(0)
     refused(lambda: gpu.embedding_forward(other.zeros((10, 8)), t, y), "another context")
     refused(lambda: gpu.embedding_backward(t, y, e, other.zeros((5000,))), "another context")

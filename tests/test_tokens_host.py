@@ -34,10 +34,10 @@ def test_workspace():
     assert f(0, 1, 1) > 0
     # two rows of partial sums for each 64 positions, four words a position, one a token
     assert f(1 << 20, 50257, 1024) >= (1 << 20) // 64 * 2 * 1024 + 4 * (1 << 20) + 50257
-    for bad in ((-1, 1, 1), (1, -1, 1), (1, 1, -1), (1 << 31, 1, 1), (1, 1 << 21, 1)):
+    for bad in ((-1, 1, 1), (1, -1, 1), (1, 1, -1), (1 << 31, 1, 1), (1, 1 << 31, 1)):
         with pytest.raises(rgpu_b200.RtError):
             f(*bad)
-    assert f((1 << 31) - 1, (1 << 21) - 1, 8192) > 1 << 32
+    assert f((1 << 31) - 1, (1 << 31) - 1, 8192) > 1 << 32
 
 
 def test_struct_matches_the_header(tmp_path):
