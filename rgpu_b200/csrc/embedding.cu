@@ -12,8 +12,8 @@
 //  - up to kChunk * kMaxCluster the sort takes one cluster (cluster_sort_kernel)
 //  - above, passes over launches (digit_*), each of which moves all positions: how often
 //    the most frequent token occurs does not decide how evenly a pass is spread
-// In the last two the rows of tokens that do not occur are written beside the sort
-// (fill_kernel), then piece_kernel and row_kernel sum.  65536 x 1024 bf16 rows of 50257
+// In the last two piece_kernel and row_kernel sum; the rows of tokens that do not occur are
+// written beside the cluster's sort (fill_kernel), or by row_kernel.  65536 x 1024 bf16 rows of 50257
 // tokens as frequent as words: 75 us, 52 of bytes; 2047 x 1000 f32 of 1000: 7.6 us.
 #include <algorithm>
 #include <climits>
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32
 
 // The rows of dE whose tokens do not occur: zeros.  A CTA marks the tokens of its share of
 // the rows by going over all positions itself, so it needs no sort, and this kernel runs beside
-// the last kernel of the sort, on the SMs that one leaves idle: it waits for it at its
+// the sort in one cluster, on the SMs that it leaves idle: it waits for it at its
 // end only (65536 positions leave 132 SMs idle for 25 us, the time of 130 MB).
 constexpr int kMarks = 8192;  // rows at a time
 
@@ -552,6 +552,7 @@ struct Sums {
     float* partial;  // [pieces][2][width]: the heavy run that began in an earlier piece, the one that began in this one
     float scale;
     int accumulate;
+    int zeros;       // row_kernel also writes the rows of tokens that do not occur
     float* out;
     int64_t ldo;
 };
@@ -663,7 +664,7 @@ __device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span
         const int64_t count = last - piece + 1, each = (count + 7) / 8;
         const int64_t b = min(count, warp * each), e = min(count, b + each);
         float sum[N] = {};
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t q = b; q < e; ++q) {
             L v;
             const float* row = s.partial + ((piece + q) * 2 + (q == 0 ? 1 : 0)) * s.width;
@@ -707,6 +708,11 @@ __global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict
     const int64_t token = min(t0 + min(lane, tokens), s.vocabulary);
     const uint32_t first = s.start[token], next = __shfl_down_sync(0xffffffffu, first, 1);
     const uint32_t count = lane < tokens && token < s.vocabulary ? next - first : 0u;
+    if (s.zeros) {
+        const float zero[N] = {};
+        for (uint32_t empty = __ballot_sync(0xffffffffu, lane < tokens && token < s.vocabulary && count == 0); empty; empty &= empty - 1)
+            Lane<float, ACCESS, N>::store(s.out + (t0 + __ffs(empty) - 1) * s.ldo, c, zero);
+    }
     const uint32_t light = count <= kLight ? count : 0u;
     uint32_t upto = light;  // light positions of the rows up to the lane's
 #pragma unroll
@@ -974,39 +980,37 @@ int launch_sums(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, const
                           : launch_sums<T, 0>(ctx, dy, m);
 }
 
-// The sort and, beside its last kernel, the rows of dE that no token has.
-int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, const Sums& m, const rt_tensor* dtable) {
+// The sort; in one cluster, the rows of dE that no token has beside it.
+int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, Sums* m, const rt_tensor* dtable) {
     const bool pdl = ctx->pdl;
-    int64_t others = ctx->sm_count;  // SMs that the last kernel of the sort leaves idle
     if (s.count <= kChunk * kMaxCluster) {
         int ranks = 1;
         while (ranks * kChunk < s.count) ranks *= 2;
         RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t));
-        others -= ranks;
         count_launch(ctx);
-    } else {
-        Pass p{t, nullptr, nullptr, nullptr, nullptr, 0};
-        for (int i = 0; i < s.passes; ++i, p.shift += 8) {
-            const bool last = (s.passes - 1 - i) % 2 == 0;  // to the arrays that the last pass writes
-            p.to_key = last ? s.token : s.key;
-            p.to_place = last ? s.position : s.place;
-            RT_CUDA(launch_k(pdl, digit_count_kernel, s.ctas, 256, 0, ctx->stream, s, p));
-            RT_CUDA(launch_k(pdl, digit_deal_kernel, s.ctas, 1024, 0, ctx->stream, s, p));
-            p.keys = p.to_key;
-            p.places = p.to_place;
+        if (!m->accumulate) {
+            // a CTA to an SM that is left, each with 16 rows or more: it goes over all tokens
+            const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count - ranks, s.vocabulary / 16));
+            const int access = access_of(dtable, 8);
+            auto* fill = access == 32 ? fill_kernel<32> : access == 16 ? fill_kernel<16> : fill_kernel<0>;
+            RT_CUDA(launch_k(pdl, fill, (unsigned)grid, 1024, 0, ctx->stream, t, s.count, s.vocabulary, m->out, m->ldo, m->n));
+            count_launch(ctx);
         }
-        RT_CUDA(launch_k(pdl, starts_kernel, (unsigned)((s.count + 255) / 256), 256, 0, ctx->stream, s));
-        count_launch(ctx, 2 * s.passes + 1);
+        return RT_OK;
     }
-    if (!m.accumulate) {
-        // 16 rows or more to a CTA: each goes over all tokens
-        const int64_t grid = std::max<int64_t>(1, std::min(others, s.vocabulary / 16));
-        const int access = access_of(dtable, 8);
-        auto* fill = access == 32 ? fill_kernel<32> : access == 16 ? fill_kernel<16> : fill_kernel<0>;
-        RT_CUDA(launch_k(pdl, fill, (unsigned)grid, 1024, 0, ctx->stream, t, s.count, s.vocabulary,
-                         static_cast<float*>(dtable->ptr), dtable->ld, dtable->cols));
-        count_launch(ctx);
+    Pass p{t, nullptr, nullptr, nullptr, nullptr, 0};
+    for (int i = 0; i < s.passes; ++i, p.shift += 8) {
+        const bool last = (s.passes - 1 - i) % 2 == 0;  // to the arrays that the last pass writes
+        p.to_key = last ? s.token : s.key;
+        p.to_place = last ? s.position : s.place;
+        RT_CUDA(launch_k(pdl, digit_count_kernel, s.ctas, 256, 0, ctx->stream, s, p));
+        RT_CUDA(launch_k(pdl, digit_deal_kernel, s.ctas, 1024, 0, ctx->stream, s, p));
+        p.keys = p.to_key;
+        p.places = p.to_place;
     }
+    RT_CUDA(launch_k(pdl, starts_kernel, (unsigned)((s.count + 255) / 256), 256, 0, ctx->stream, s));
+    count_launch(ctx, 2 * s.passes + 1);
+    m->zeros = !m->accumulate;  // each filling CTA would go over more tokens than the sorted list costs
     return RT_OK;
 }
 
@@ -1089,7 +1093,7 @@ int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor*
     m.out = static_cast<float*>(dtable->ptr);
     m.ldo = dtable->ld;
     const bool few = s.count <= kFew;
-    if (!few) RT_TRY(launch_sort(ctx, static_cast<const uint32_t*>(tokens->ptr), s, m, dtable));
+    if (!few) RT_TRY(launch_sort(ctx, static_cast<const uint32_t*>(tokens->ptr), s, &m, dtable));
     return dy->dtype == RT_BF16 ? launch_sums<__nv_bfloat16>(ctx, tokens, dy, dtable, m, few)
                                 : launch_sums<float>(ctx, tokens, dy, dtable, m, few);
 }
