@@ -146,6 +146,39 @@ def test_infinities_stay_in_their_rows(gpu):
     assert np.isposinf(got[6]).all() and np.isnan(got[5]).all() and np.isfinite(got[:5]).all()
 
 
+@pytest.mark.parametrize("count", [300, 9000, 70000])
+def test_what_padding_rows_hold_does_not_matter(gpu, count):
+    rng = np.random.default_rng(count)
+    tokens = rng.integers(0, 60, count).astype(np.uint32)
+    tokens[rng.random(count) < 0.5] = 40 + 20 + rng.integers(0, 9)  # half of them: past the 40 rows of the table
+    dy = rng.integers(-3, 4, (count, 24)).astype(np.float32)
+    want = R.embedding_backward(40, tokens, dy.astype(np.float64), 1.0)[0]
+    dy[tokens >= 40] = np.nan
+    d = gpu.zeros((40, 24))
+    gpu.embedding_backward(rgpu_b200.upload_labels(gpu, tokens), gpu.upload(dy), d,
+                           gpu.zeros((gpu.embedding_backward_workspace(count, 40, 24),)))
+    assert np.array_equal(gpu.download(d), want)  # whole numbers
+
+
+def test_two_contexts_at_once(gpu):
+    # each with its own stream and workspace, their launches between one another's
+    other = rgpu_b200.Gpu(0)
+    rng = np.random.default_rng(8)
+    jobs = []
+    for g, count in ((gpu, 5000), (other, 66000)):
+        tokens = rng.integers(0, 700, count).astype(np.uint32)
+        dy = rng.integers(-3, 4, (count, 40)).astype(np.float32)
+        jobs.append((g, rgpu_b200.upload_labels(g, tokens), g.upload(dy), g.zeros((650, 40)),
+                     g.zeros((g.embedding_backward_workspace(count, 650, 40),)), R.embedding_backward(650, tokens, dy.astype(np.float64), 2.0)[0]))
+    for _ in range(20):
+        for g, t, dy, d, work, _w in jobs:
+            g.embedding_backward(t, dy, d, work, scale=2.0)
+    for g, _t, _dy, d, _work, want in jobs:
+        assert np.array_equal(g.download(d), want)
+    del jobs
+    other.close()
+
+
 def test_empty_extents(gpu):
     none = gpu.wrap(gpu.zeros((4,)).ptr, (0,), "u32")
     work = gpu.zeros((gpu.embedding_backward_workspace(0, 5, 8),))
