@@ -497,20 +497,20 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 // 8192^3, bf16 out: 184 us for a single launch, the tensor pipe 84 % busy; launched
 // again and again 183 to 220 us, the clock held down by the 1 kW power limit (154 us
 // on matrices of zeros, which draw less).  In 8 bits, twice the stages: 362 us for a single
-// launch, the tensor pipe 92 % busy, 441 to 448 again and again.
-constexpr int kPairStages = 6;
+// launch, the tensor pipe 92 % busy, 429 to 443 again and again.
+template <typename F>
+constexpr int kPairStages = F::GROUPS == 1 ? 5 : 6;  // 8 bits: the sixth's room is the epilogue's
 template <typename F>
 constexpr int kPairStageBytes = 2 * kWBytes + 3 * F::GROUPS * kScaleTile;  // codes of T and W, a row tile of T's scales, two of W's
-// Floats of a warp's stage for rows of C that are not 16-byte aligned: 32 rows of 16 columns
-// and one that turns the banks.  In 4 bits the ring leaves no room for it.
-constexpr int kStageFloats = 32 * 17;
+// Floats of an epilogue warp's stage, in 8 bits: 32 rows of 128 bytes, and 16 that turn the banks.
+constexpr int kStageFloats = 32 * 36;
 template <typename F>
 constexpr int kStagesBytes = F::GROUPS == 1 ? 8 * kStageFloats * 4 : 0;
 template <typename F>
-constexpr int kPairSmem = kPairStages * kPairStageBytes<F> + 8 * 512 /* bias of each epilogue warp's columns */ + kStagesBytes<F> + 256;
+constexpr int kPairSmem = kPairStages<F> * kPairStageBytes<F> + 8 * 512 /* bias of each epilogue warp's columns */ + kStagesBytes<F> + 256;
 constexpr int kPairThreads = 320;  // warps: 0 TMA, 1 MMA (leader), 2-9 epilogue (two to a TMEM lane quadrant)
 static_assert(kPairSmem<Mx4> <= 227 * 1024 && kPairSmem<Fp8> <= 227 * 1024, "shared memory of a CTA");
-static_assert(256 + 24 * kPairStages <= 512, "TMEM columns");
+static_assert(256 + 24 * kPairStages<Mx4> <= 512, "TMEM columns");
 
 __device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
     asm volatile(
@@ -570,18 +570,21 @@ __device__ __forceinline__ void transpose32(float (&v)[32], int lane) {
 // 1024 bf16 36 us, where 4096 columns, aligned, take 18.  c: the first row's; rows, left: how many rows and columns there are from it on.
 template <typename T>
 __device__ __forceinline__ void store_columns(T* c, int64_t ldc, int64_t rows, int64_t left, const float* bias,
-                                              float floor, int lane, float (&v)[32]) {
-    transpose32(v, lane);
-    const float b = bias[lane];
-    T* to = c + lane;
-    if (lane < left)
+                                              float floor, int lane, float (&v)[4][32]) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < rows) store_one(to + i * ldc, at_least(v[i] + b, floor));
+    for (int k = 0; k < 4; ++k) {
+        transpose32(v[k], lane);
+        const float b = bias[k * 32 + lane];
+        T* to = c + k * 32 + lane;
+        if (k * 32 + lane < left)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i < rows) store_one(to + i * ldc, at_least(v[k][i] + b, floor));
+    }
 }
 
 // The same through the warp's stage in shared memory, 16 columns at a time: no exchange
-// in registers.  4096 x 4097 x 1024 in 8 bits 34 us (f32 out 37), through the exchange above 55 (79).
+// in registers.  4096 x 4097 x 1024 in 8 bits 31 us (f32 out 36; codes of zero), through the exchange above 36 (42).
 template <typename T>
 __device__ __forceinline__ void store_staged(T* c, int64_t ldc, int64_t rows, int64_t left, const float* bias, float floor,
                                              int lane, const float (&v)[32], float* stage) {
@@ -600,18 +603,18 @@ __device__ __forceinline__ void store_staged(T* c, int64_t ldc, int64_t rows, in
     }
 }
 
-// 32 neighbouring elements of a row of C.  ACCESS: bytes that they are
+// N times 32 neighbouring elements of a row of C.  ACCESS: bytes that every 32 of them are
 // aligned to (32 or 16; past the row's end element by element).
-template <typename T, int ACCESS>
-__device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias, float floor, float (&v)[32]) {
+template <typename T, int ACCESS, int N>
+__device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias, float floor, float (&v)[N][32]) {
     constexpr int E = ACCESS / (int)sizeof(T);  // elements of a store
 #pragma unroll
-    for (int k = 0; k < 32; k += E) {
+    for (int k = 0; k < 32 * N; k += E) {
         float x[E];
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
             const float4 b = *reinterpret_cast<const float4*>(bias + k + i);
-            const float* y = &v[k + i];
+            const float* y = &v[k / 32][k % 32 + i];
             x[i] = at_least(y[0] + b.x, floor), x[i + 1] = at_least(y[1] + b.y, floor);
             x[i + 2] = at_least(y[2] + b.z, floor), x[i + 3] = at_least(y[3] + b.w, floor);
         }
@@ -640,19 +643,82 @@ __device__ __forceinline__ void store_row(T* c, int64_t left, const float* bias,
     }
 }
 
-// A warp's 32 rows (lanes) of 32 columns of C from column `col` on; rows: how many there
-// are from the lane's on.  stage: the warp's, in 8 bits.
-template <typename F, typename T, bool ALIGNED>
-__device__ __forceinline__ void store_block(const Mx4Params& p, int64_t row, int64_t rows, int64_t col, const float* bias,
-                                            float floor, int lane, float (&v)[32], float* stage) {
+// The same through the warp's stage: full lines of C, 128 bytes of a row, four rows an
+// instruction.  The stores above touch 32 rows each.
+// 4096 x 4096 x 1024, f32 out: 25 us, with them 29; 8192^3 432, 447 (pairs that split k, half
+// of the columns a warp: 21.3, with them 20.6, so those keep them).  c: the
+// warp's first row, rows and left: how many there are from there on.
+template <typename T>
+__device__ __forceinline__ void store_line(T* c, int64_t ldc, int64_t rows, int64_t left, const float* bias, float floor,
+                                           int lane, const float (*v)[32], float* stage) {
+    constexpr int E = 16 / (int)sizeof(T), V = 128 / (int)sizeof(T);  // elements of an access, of a line
+    uint4* mine = reinterpret_cast<uint4*>(stage + lane * 36);
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < V; k += E) {
+        float x[E];
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + k + i);
+            const float* y = &v[(k + i) / 32][(k + i) % 32];
+            x[i] = at_least(y[0] + b.x, floor), x[i + 1] = at_least(y[1] + b.y, floor);
+            x[i + 2] = at_least(y[2] + b.z, floor), x[i + 3] = at_least(y[3] + b.w, floor);
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                w[i] = __float_as_uint(x[i]);
+            }
+        }
+        mine[k / E] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+    const int first = lane >> 3, at = (lane & 7) * E;
+    const int end = (int)max((int64_t)0, min((int64_t)32, rows));
+    T* to = c + first * ldc + at;
+    if (left >= at + E) {
+#pragma unroll 4
+        for (int r = first; r < end; r += 4, to += 4 * ldc)
+            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(stage + r * 36 + (lane & 7) * 4);
+    } else {
+        for (int r = first; r < end; r += 4, to += 4 * ldc)
+            for (int i = 0; i < E && at + i < left; ++i) to[i] = reinterpret_cast<const T*>(stage + r * 36)[at + i];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_lines(T* c, int64_t ldc, int64_t rows, int64_t left, const float* bias, float floor,
+                                            int lane, const float (&v)[4][32], float* stage) {
+    constexpr int STEP = 4 / (int)sizeof(T);  // blocks of 32 columns in a line
+#pragma unroll
+    for (int k = 0; k < 4; k += STEP)
+        store_line(c + k * 32, ldc, rows, left - k * 32, bias + k * 32, floor, lane, v + k, stage);
+}
+
+// A warp's 32 rows (lanes; `row` is the lane's) of N times 32 columns of C from `col` on, the
+// way that fits C's alignment and the room for a stage.
+template <typename F, typename T, bool ALIGNED, int N>
+__device__ __forceinline__ void store_tile(const Mx4Params& p, int64_t row, int64_t col, const float* bias, float floor,
+                                           int lane, float (&v)[N][32], float* stage) {
     T* to = static_cast<T*>(p.c) + row * p.ldc + col;
-    if constexpr (!ALIGNED && F::GROUPS == 1) {
-        store_staged(to - lane * p.ldc, p.ldc, rows + lane, p.n - col, bias, floor, lane, v, stage);
-    } else if constexpr (!ALIGNED) {
-        store_columns(to - lane * p.ldc, p.ldc, rows + lane, p.n - col, bias, floor, lane, v);
-    } else if (rows > 0) {
-        if (p.access == 32) store_row<T, 32>(to, p.n - col, bias, floor, v);
-        else store_row<T, 16>(to, p.n - col, bias, floor, v);
+    const int64_t left = p.n - col, rows = p.m - row;
+    if constexpr (ALIGNED) {
+        if constexpr (F::GROUPS == 1 && N == 4) {
+            store_lines(to - lane * p.ldc, p.ldc, rows + lane, left, bias, floor, lane, v, stage);
+        } else if (rows > 0) {
+            if (p.access == 32) store_row<T, 32>(to, left, bias, floor, v);
+            else store_row<T, 16>(to, left, bias, floor, v);
+        }
+    } else if constexpr (F::GROUPS == 1) {
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+            store_staged(to - lane * p.ldc + c * 32, p.ldc, rows + lane, left - c * 32, bias + c * 32, floor, lane, v[c], stage);
+    } else {
+        store_columns(to - lane * p.ldc, p.ldc, rows + lane, left, bias, floor, lane, v);
     }
 }
 
@@ -667,7 +733,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                                                                    const __grid_constant__ CUtensorMap map_sw,
                                                                    const __grid_constant__ CUtensorMap map_st,
                                                                    Mx4Params p) {
-    constexpr int S = kPairStages, NG = F::GROUPS, S_BYTES = 3 * NG * kScaleTile;
+    constexpr int S = kPairStages<F>, NG = F::GROUPS, S_BYTES = 3 * NG * kScaleTile;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* smem_w = smem;
     uint8_t* smem_t = smem + S * kWBytes;
@@ -866,11 +932,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
                     for (int j = 0; j < 32; ++j) own[c][j] = v[c][j];
             } else {
                 const float floor = p.relu ? 0.0f : -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (p.out_bf16) store_block<F, __nv_bfloat16, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, v[c], stage);
-                    else store_block<F, float, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, v[c], stage);
-                }
+                if (p.out_bf16) store_tile<F, __nv_bfloat16, ALIGNED>(p, row, col0, bias, floor, lane, v, stage);
+                else store_tile<F, float, ALIGNED>(p, row, col0, bias, floor, lane, v, stage);
             }
         }
         if (!ok && lane == 0) raise_abort(DEV_TIMEOUT_EPILOGUE);
@@ -892,12 +955,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx4_pair_kernel(const __grid_
             for (int j = 0; j < 64; ++j)
                 asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y[j / 32][j % 32]) : "r"(from + j * 512) : "memory");
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) y[c][j] += own[c][j];
-                if (p.out_bf16) store_block<F, __nv_bfloat16, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, y[c], stage);
-                else store_block<F, float, ALIGNED>(p, row, p.m - row, col0 + c * 32, bias + c * 32, floor, lane, y[c], stage);
-            }
+            for (int j = 0; j < 64; ++j) y[j / 32][j % 32] += own[j / 32][j % 32];
+            if (p.out_bf16) store_tile<F, __nv_bfloat16, ALIGNED>(p, row, col0, bias, floor, lane, y, stage);
+            else store_tile<F, float, ALIGNED>(p, row, col0, bias, floor, lane, y, stage);
         }
         __syncwarp();
     }
