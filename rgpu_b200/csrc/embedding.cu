@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(1024) fill_kernel(const uint32_t* __restrict__
 // The sums.  A token that occurs at most kLight times is light: a warp takes 512 bytes' columns
 // of `tokens` neighbouring rows of dE, whose positions lie one after another, and writes
 // each row once.  The others are heavy: the sorted list is cut into pieces of kCut positions
-// whatever the tokens, a warp each; where a heavy run crosses pieces, each leaves a partial
+// (fewer where there are few) whatever the tokens, a warp each; where a heavy run crosses pieces, each leaves a partial
 // sum of it, and join() adds these in order.
 constexpr int kCut = 64, kLight = 16;
 
@@ -546,6 +546,7 @@ constexpr int kColumns = 16 / (int)sizeof(T);
 struct Sums {
     int64_t count, vocabulary, n, spans, width;
     int64_t pieces;
+    int cut;  // positions of a piece: kCut, a half or a quarter
     const uint32_t* token;
     const uint32_t* position;
     const uint32_t* start;
@@ -583,8 +584,8 @@ __global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* __restrict_
     const int lane = threadIdx.x & 31;
     const Columns<ACCESS, N> c(lay_span(along), s.n, lane);
     const int64_t real = s.start[s.vocabulary];  // positions that hold a token
-    const int64_t piece = lay_group(along), p0 = piece * kCut;
-    const int live = (int)max((int64_t)0, min((int64_t)kCut, real - p0));
+    const int64_t piece = lay_group(along), p0 = piece * s.cut;
+    const int live = (int)max((int64_t)0, min((int64_t)s.cut, real - p0));
     uint32_t token[kCut / 32], row[kCut / 32], begin[kCut / 32], end[kCut / 32];
     uint64_t heavy = 0;  // a bit a position
 #pragma unroll
@@ -603,7 +604,7 @@ __global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* __restrict_
     uint32_t run_token = of(token, run);
     auto flush = [&]() {
         const int64_t run0 = of(begin, run), run1 = of(end, run);
-        if (run0 >= p0 && run1 <= p0 + kCut)
+        if (run0 >= p0 && run1 <= p0 + s.cut)
             emit<ACCESS, N>(s, run_token, c, sum);
         else
             Lane<float, ACCESS, N>::store(s.partial + (piece * 2 + (run0 < p0 ? 0 : 1)) * s.width, c, sum);
@@ -636,9 +637,11 @@ __global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* __restrict_
 }
 
 // Adds the partial sums of the heavy runs that begin in kJoin pieces: a run's second row
-// there and the first rows of the pieces that follow, dealt out over the CTA's warps in
-// order.
-constexpr int kJoin = 8;
+// there and the first rows of the pieces that follow. A warp takes a run that lies in
+// kAlone pieces at most (17314 x 33 of 593: 34 us; by the whole CTA, one after another, 40); longer
+// ones are dealt out over the CTA's warps in order.
+constexpr int kJoin = 8, kAlone = 16;
+static_assert(kJoin == 8, "a warp each");
 
 template <int ACCESS, int N>
 __device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span) {
@@ -648,35 +651,43 @@ __device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span
     const int64_t real = s.start[s.vocabulary];
     const Columns<ACCESS, N> c(span, s.n, lane);
     // every warp looks at the last position of each of the pieces
-    const int64_t end = (piece0 + lane + 1) * kCut;
+    const int64_t end = (piece0 + lane + 1) * s.cut;
     uint32_t token = 0;
     int64_t first = 0, next = 0;
     bool begins = lane < kJoin && end < real;
     if (begins) {
         token = s.token[end - 1];
         first = s.start[token], next = s.start[token + 1];
-        begins = next > end && first >= end - kCut && next - first > kLight;
+        begins = next > end && first >= end - s.cut && next - first > kLight;
     }
-    pdl_wait();  // for the partial sums
-    for (uint32_t found = __ballot_sync(0xffffffffu, begins); found; found &= found - 1) {
-        const int of = __ffs(found) - 1;
-        const int64_t piece = piece0 + of, last = (__shfl_sync(0xffffffffu, next, of) - 1) / kCut;
-        const int64_t count = last - piece + 1, each = (count + 7) / 8;
-        const int64_t b = min(count, warp * each), e = min(count, b + each);
-        float sum[N] = {};
+    const int pieces = begins ? (int)((next - 1) / s.cut - (piece0 + lane)) + 1 : 0;  // that the run lies in
+    const uint32_t few = __ballot_sync(0xffffffffu, begins && pieces <= kAlone);
+    float sum[N];
+    auto add = [&](int64_t piece, int b, int e) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = 0.0f;
 #pragma unroll 8
-        for (int64_t q = b; q < e; ++q) {
+        for (int q = b; q < e; ++q) {
             L v;
-            const float* row = s.partial + ((piece + q) * 2 + (q == 0 ? 1 : 0)) * s.width;
-            v.load(row, c);
+            v.load(s.partial + ((piece + q) * 2 + (q == 0 ? 1 : 0)) * s.width, c);
 #pragma unroll
             for (int i = 0; i < N; ++i) sum[i] += v.value(i);
         }
+    };
+    pdl_wait();  // for the partial sums
+    if (few >> warp & 1) {
+        add(piece0 + warp, 0, __shfl_sync(0xffffffffu, pieces, warp));
+        emit<ACCESS, N>(s, __shfl_sync(0xffffffffu, token, warp), c, sum);
+    }
+    for (uint32_t found = __ballot_sync(0xffffffffu, pieces > kAlone); found; found &= found - 1) {
+        const int of = __ffs(found) - 1, count = __shfl_sync(0xffffffffu, pieces, of), each = (count + 7) / 8;
+        const int b = min(count, warp * each);
+        add(piece0 + of, b, min(count, b + each));
 #pragma unroll
         for (int i = 0; i < N; ++i) part[warp][i * 32 + lane] = sum[i];
         __syncthreads();
         if (warp == 0) {
-            const int64_t used = (count + each - 1) / each;
+            const int used = (count + each - 1) / each;
             for (int w = 1; w < used; ++w)
 #pragma unroll
                 for (int i = 0; i < N; ++i) sum[i] += part[w][i * 32 + lane];
@@ -884,7 +895,12 @@ int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) 
     // spans of at least 1024 positions: with more CTAs each would add up more counts
     s->ctas = (int)std::min<int64_t>(256, std::max<int64_t>(1, (count + 1023) / 1024));
     s->span = (count + s->ctas - 1) / s->ctas;
-    m->pieces = (count + kCut - 1) / kCut;
+    // Shorter pieces while there are fewer than eight warps for each of the 148 SMs: a warp's reads of a piece wait for one another,
+    // but a long run leaves more partial sums.  17314 x 33 of 593: 25.5 us with 16, 28 with 32, 34 with 64;
+    // 65536 x 1024 of 50257: 85, 78 and 75.
+    m->cut = kCut;
+    while (m->cut > kCut / 4 && (count / m->cut) * ((n + 255) / 256) < 8 * 148) m->cut /= 2;
+    m->pieces = (count + m->cut - 1) / m->cut;
     m->width = (n + 7) / 8 * 8;
     auto words = [](int64_t v) { return (v + 31) / 32 * 32; };
     int64_t at = 0;
@@ -939,8 +955,10 @@ int launch_sums(rt_ctx* ctx, const rt_tensor* dy, Sums m) {
     constexpr int SPAN = 32 * kColumns<T>;
     m.spans = (m.n + SPAN - 1) / SPAN;
     // 16 rows a warp where that makes warps enough for every place on the device (65536 x 1024 of 50257:
-    // 77 us, with 4 rows 87), else 4, whose chain of reads is shorter (2047 x 1000 of 1000: 13.9 us, with 16 18.1)
-    const int tokens = m.vocabulary / 16 * m.spans >= (int64_t)ctx->sm_count * 32 ? 16 : 4;
+    // 75 us, with 4 rows 87, with one 117); one, whose chain of reads is the shortest, where the device
+    // holds most of the warps at once (7813 x 3979 of 430 bf16: 48 us, with 4 rows 57); else 4
+    const int64_t sms = ctx->sm_count;
+    const int tokens = m.vocabulary / 16 * m.spans >= sms * 32 ? 16 : m.vocabulary * m.spans < sms * 48 ? 1 : 4;
     const Lay pieces(m.pieces, m.spans), rows((m.vocabulary + tokens - 1) / tokens, m.spans);
     const T* p = static_cast<const T*>(dy->ptr);
     RT_CUDA(launch_k(ctx->pdl, piece_kernel<T, ACCESS>, pieces.grid, 256, 0, ctx->stream, m, p, dy->ld, pieces.along));
