@@ -14,7 +14,7 @@
 //    the most frequent token occurs does not decide how evenly a pass is spread
 // In the last two piece_kernel and row_kernel sum; the rows of tokens that do not occur are
 // written beside the cluster's sort (fill_kernel), or by row_kernel.  65536 x 1024 bf16 rows of 50257
-// tokens as frequent as words: 75 us, 52 of bytes; 2047 x 1000 f32 of 1000: 7.6 us.
+// tokens as frequent as words: 75 us, 52 of bytes; 2047 x 1000 f32 of 1000: 6.5 us.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -776,17 +776,17 @@ __global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict
 // equal shares of them.  A run that crosses shares is joined through shared memory, in order.
 constexpr int kFew = 4096, kGroup = 128;
 
-template <typename T, int ACCESS>
-__global__ void __launch_bounds__(256, 4) few_kernel(Sums s, const uint32_t* __restrict__ tokens, const T* __restrict__ dy,
+template <typename T, int ACCESS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, const uint32_t* __restrict__ tokens, const T* __restrict__ dy,
                                                   int64_t ldy, int group) {
-    constexpr int N = kColumns<T>, WARPS = 8;
+    constexpr int N = kColumns<T>;
     using L = Lane<T, ACCESS, N>;
     __shared__ uint32_t base[kGroup + 1], sums[WARPS];
     __shared__ uint32_t cnt[WARPS][kGroup];
     __shared__ uint32_t list[kFew];  // row << 16 | position, sorted
-    __shared__ float part[WARPS][2][32 * N];
+    __shared__ float part[WARPS][32 * N];  // of the run that began in an earlier share
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < WARPS * kGroup; i += 256) cnt[0][i] = 0;
+    for (int i = threadIdx.x; i < WARPS * kGroup; i += 32 * WARPS) cnt[0][i] = 0;
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
@@ -837,9 +837,9 @@ __global__ void __launch_bounds__(256, 4) few_kernel(Sums s, const uint32_t* __r
         const int run0 = (int)base[run], run1 = (int)base[run + 1];
         if (run0 >= begin && run1 <= end) {
             emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
-        } else {
+        } else if (run0 < begin) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) part[warp][run0 < begin ? 0 : 1][i * 32 + lane] = sum[i];
+            for (int i = 0; i < N; ++i) part[warp][i * 32 + lane] = sum[i];
         }
     };
     // U entries from e on, all of their rows of dy under way at once
@@ -871,13 +871,11 @@ __global__ void __launch_bounds__(256, 4) few_kernel(Sums s, const uint32_t* __r
     for (; e < end; e += 3) add(e, std::integral_constant<int, 3>());
     if (run >= 0) flush();
     __syncthreads();
-    // the warp in whose share a run begins that goes on adds it up
+    // the warp in whose share a run begins that goes on, its last one, adds it up
     if (run < 0 || (int)base[run + 1] <= end || (int)base[run] < begin) return;
-#pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] = part[warp][1][i * 32 + lane];
     for (int w = warp + 1; w < WARPS && w * each < (int)base[run + 1]; ++w)
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += part[w][0][i * 32 + lane];
+        for (int i = 0; i < N; ++i) sum[i] += part[w][i * 32 + lane];
     emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
 }
 
@@ -974,12 +972,17 @@ template <typename T, int ACCESS>
 int launch_few(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, const Sums& m) {
     constexpr int SPAN = 32 * kColumns<T>;
     const int64_t spans = (m.n + SPAN - 1) / SPAN;
-    // so many rows, 4 to kGroup, that the CTAs fit the device at once, four to an SM: each goes over all positions
-    int group = 4;
-    while (group < kGroup && (m.vocabulary + group - 1) / group * spans > 4 * (int64_t)ctx->sm_count) group *= 2;
+    // So many rows a CTA that the CTAs fit the device at once, 32 warps to an SM: each goes over all positions.
+    // 16 warps a CTA if such a number (at most kGroup) exists: they share a frequent token's positions
+    // (2047 x 1000 of 1000: 6.6 us, with 8 warps 7.9; 4096 x 1024 of 1000, as frequent as words, bf16: 15.9 / 20.4);
+    // else 8, which keep waiting less for one another (4096 x 1024 of 50257: 53 us, with 16 56; 1024 x 1024 f32: 40 / 57)
+    auto ctas = [&](int group) { return (m.vocabulary + group - 1) / group * spans; };
+    const bool wide = ctas(kGroup) <= 2 * (int64_t)ctx->sm_count;
+    int group = 1;
+    while (group < kGroup && ctas(group) > (wide ? 2 : 4) * (int64_t)ctx->sm_count) group *= 2;
     const dim3 grid((unsigned)((m.vocabulary + group - 1) / group), (unsigned)spans);
-    RT_CUDA(launch_k(ctx->pdl, few_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, static_cast<const uint32_t*>(tokens->ptr),
-                     static_cast<const T*>(dy->ptr), dy->ld, group));
+    RT_CUDA(launch_k(ctx->pdl, wide ? few_kernel<T, ACCESS, 16> : few_kernel<T, ACCESS, 8>, grid, wide ? 512 : 256, 0, ctx->stream, m,
+                     static_cast<const uint32_t*>(tokens->ptr), static_cast<const T*>(dy->ptr), dy->ld, group));
     count_launch(ctx);
     return RT_OK;
 }
