@@ -774,7 +774,7 @@ __global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict
 // Few positions: one launch.  A CTA takes `group` neighbouring rows of dE and a span of columns;
 // it goes over all positions, sorts those of its rows in shared memory, and its warps take
 // equal shares of them.  A run that crosses shares is joined through shared memory, in order.
-constexpr int kFew = 4096, kGroup = 128;
+constexpr int kFew = 8192, kGroup = 128;
 
 template <typename T, int ACCESS, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, const uint32_t* __restrict__ tokens, const T* __restrict__ dy,
@@ -782,9 +782,13 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, con
     constexpr int N = kColumns<T>;
     using L = Lane<T, ACCESS, N>;
     __shared__ uint32_t base[kGroup + 1], sums[WARPS];
-    __shared__ uint32_t cnt[WARPS][kGroup];
     __shared__ uint32_t list[kFew];  // row << 16 | position, sorted
-    __shared__ float part[WARPS][32 * N];  // of the run that began in an earlier share
+    __shared__ union {
+        uint32_t cnt[WARPS][kGroup];
+        float part[WARPS - 1][32 * N];  // of the run that began before a warp's share; the first has none
+    } m;
+    auto& cnt = m.cnt;
+    auto& part = m.part;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int i = threadIdx.x; i < WARPS * kGroup; i += 32 * WARPS) cnt[0][i] = 0;
     __syncthreads();
@@ -839,7 +843,7 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, con
             emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
         } else if (run0 < begin) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) part[warp][i * 32 + lane] = sum[i];
+            for (int i = 0; i < N; ++i) part[warp - 1][i * 32 + lane] = sum[i];
         }
     };
     // U entries from e on, all of their rows of dy under way at once
@@ -875,7 +879,7 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, con
     if (run < 0 || (int)base[run + 1] <= end || (int)base[run] < begin) return;
     for (int w = warp + 1; w < WARPS && w * each < (int)base[run + 1]; ++w)
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += part[w][i * 32 + lane];
+        for (int i = 0; i < N; ++i) sum[i] += part[w - 1][i * 32 + lane];
     emit<ACCESS, N>(s, (uint32_t)t0 + run, c, sum);
 }
 
@@ -883,6 +887,16 @@ int bits_of(int64_t v) {
     int b = 0;
     while (v >> b) ++b;
     return b;
+}
+
+// Whether few_kernel takes them all: up to kFew / 2 positions always, up to kFew if its CTAs, of which each
+// goes over all positions, are no more than the device holds at once and the table is narrow, but not so short that a
+// few CTAs have most of the positions (7424 x 128 of 1792: 8.7 us, with the cluster's sort 19.4; 8192 x 1024 bf16 of 1000: 13.9 / 21.8,
+// as frequent as words 26.8 / 24.4; 8192 x 1024 of 50257: 74 / 50; 8192 x 64 of 16: 25 / 16; 8192 x 1001 bf16 of 300: 40 / 27).
+bool is_few(int64_t count, int64_t vocabulary, int64_t n) {
+    const int64_t spans = (n + 255) / 256;
+    return count <= kFew / 2 ||
+           (count <= kFew && vocabulary >= std::max<int64_t>(256, 128 * spans) && spans <= 4 && (vocabulary + kGroup - 1) / kGroup * spans <= 4 * 148);
 }
 
 // The workspace's layout from its sizes; the words it needs.
@@ -908,7 +922,7 @@ int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) 
         at += words(v);
         return p;
     };
-    if (count <= kFew) return words(1);  // few_kernel needs none
+    if (is_few(count, vocabulary, n)) return words(1);  // few_kernel needs none
     m->partial = reinterpret_cast<float*>(take(m->pieces * 2 * m->width));
     s->token = take(count);
     s->position = take(count);
@@ -1113,7 +1127,7 @@ int rt_embedding_backward(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor*
     m.accumulate = accumulate != 0;
     m.out = static_cast<float*>(dtable->ptr);
     m.ldo = dtable->ld;
-    const bool few = s.count <= kFew;
+    const bool few = is_few(s.count, s.vocabulary, m.n);
     if (!few) RT_TRY(launch_sort(ctx, static_cast<const uint32_t*>(tokens->ptr), s, &m, dtable));
     return dy->dtype == RT_BF16 ? launch_sums<__nv_bfloat16>(ctx, tokens, dy, dtable, m, few)
                                 : launch_sums<float>(ctx, tokens, dy, dtable, m, few);
