@@ -8,7 +8,7 @@
 // Backward.  The positions are sorted by token, stably, so that the rows of dy that a row
 // of dE sums lie one after another and their order is fixed: no atomic adds floats, the
 // same call gives the same bits.  Three ways by how many positions there are:
-//  - up to kFew one launch (few_kernel): every CTA sorts the positions of its own rows
+//  - up to kFew / 2, of narrow tables up to kFew, one launch (few_kernel): every CTA sorts the positions of its own rows
 //  - up to kChunk * kMaxCluster the sort takes one cluster (cluster_sort_kernel)
 //  - above, passes over launches (digit_*), each of which moves all positions: how often
 //    the most frequent token occurs does not decide how evenly a pass is spread
@@ -169,6 +169,7 @@ struct Sort {
     int passes;          // by 8 bits of a key
     int ctas;            // of a pass over launches,
     int64_t span;        // and positions of a CTA
+    int log_chunk;       // of the positions of a CTA of the cluster
     uint32_t* counts;    // [ctas][256]
     uint32_t* key;       // [count] between passes,
     uint32_t* place;     // [count] and their positions
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(256) starts_kernel(Sort s) {
 }
 
 // The whole sort in one launch where the positions fit the shared memory of one cluster:
-// a CTA holds kChunk of them, and passes by 8 bits of the key, the low ones first, move
+// a CTA holds up to kChunk of them, and passes by 8 bits of the key, the low ones first, move
 // them through distributed shared memory.  65536 positions of 50257 tokens: 26 us under a
 // profiler, as long as the launches above, but on 16 SMs: fill_kernel has the others meanwhile.
 constexpr int kChunk = 4096, kMaxCluster = 16, kStride = 257;  // kStride: counters of a warp, off a bank each
@@ -382,25 +383,27 @@ __global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
-    const int64_t first = (int64_t)rank * kChunk;
-    const int live = (int)max((int64_t)0, min((int64_t)kChunk, s.count - first));  // positions of this CTA
+    const int chunk = 1 << s.log_chunk, share = chunk / 32;  // positions of a CTA, of a warp
+    const int64_t first = (int64_t)rank * chunk;
+    const int live = (int)max((int64_t)0, min((int64_t)chunk, s.count - first));  // positions of this CTA
     uint2 item[4];
-    const int slot = warp * 128 + lane;  // of the thread's first item; the others 32 apart
+    const int slot = warp * share + lane;  // of the thread's first item; the others 32 apart
+    auto there = [&](int x) { return x * 32 < share && slot + x * 32 < live; };
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-        if (slot + x * 32 < live) item[x] = make_uint2(key_of(s, tokens, first + slot + x * 32), (uint32_t)first + slot + x * 32);
+        if (there(x)) item[x] = make_uint2(key_of(s, tokens, first + slot + x * 32), (uint32_t)first + slot + x * 32);
     for (int pass = 0; pass < s.passes; ++pass) {
         const int shift = pass * 8;
         for (int i = threadIdx.x; i < 32 * kStride; i += 1024) m.cnt[i] = 0;
         if (pass)
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-                if (slot + x * 32 < live) item[x] = m.item[slot + x * 32];
+                if (there(x)) item[x] = m.item[slot + x * 32];
         __syncthreads();
         uint32_t before[4];  // of the item's digit: items before it in its warp
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-            before[x] = count_rank(m.cnt + warp * kStride, item[x].x >> shift & 255u, slot + x * 32 < live, lane);
+            if (x * 32 < share) before[x] = count_rank(m.cnt + warp * kStride, item[x].x >> shift & 255u, there(x), lane);
         __syncthreads();
         // the warps' counters to exclusive sums over the warps: four threads a digit, eight warps each
         const int digit = threadIdx.x >> 2, part = threadIdx.x & 3;
@@ -454,16 +457,16 @@ __global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-            if (slot + x * 32 < live) {
+            if (there(x)) {
                 const uint32_t d = item[x].x >> shift & 255u, to = m.base[d] + m.cnt[warp * kStride + d] + before[x];
-                const uint32_t at = in_cta(&m.item[to % kChunk], to / kChunk);
+                const uint32_t at = in_cta(&m.item[to & (chunk - 1)], to >> s.log_chunk);
                 asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(item[x].x), "r"(item[x].y) : "memory");
             }
         sync_cluster();
     }
     // sorted: token and position out; where tokens start from the places where the key changes
     if (threadIdx.x == 0) m.gaps = 0;
-    const uint32_t previous = rank && live ? ld_cluster(in_cta(&m.item[kChunk - 1], rank - 1)) : 0u;
+    const uint32_t previous = rank && live ? ld_cluster(in_cta(&m.item[chunk - 1], rank - 1)) : 0u;
     __syncthreads();
     uint32_t* list = m.cnt;  // places of wide gaps
     static_assert(32 * kStride >= kChunk + 1, "every place fits the list");
@@ -638,7 +641,7 @@ __global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* __restrict_
 
 // Adds the partial sums of the heavy runs that begin in kJoin pieces: a run's second row
 // there and the first rows of the pieces that follow. A warp takes a run that lies in
-// kAlone pieces at most (17314 x 33 of 593: 34 us; by the whole CTA, one after another, 40); longer
+// kAlone pieces at most (17314 x 33 of 593, pieces of 64: 34 us; by the whole CTA, one after another, 40); longer
 // ones are dealt out over the CTA's warps in order.
 constexpr int kJoin = 8, kAlone = 16;
 static_assert(kJoin == 8, "a warp each");
@@ -889,14 +892,13 @@ int bits_of(int64_t v) {
     return b;
 }
 
-// Whether few_kernel takes them all: up to kFew / 2 positions always, up to kFew if its CTAs, of which each
-// goes over all positions, are no more than the device holds at once and the table is narrow, but not so short that a
-// few CTAs have most of the positions (7424 x 128 of 1792: 8.7 us, with the cluster's sort 19.4; 8192 x 1024 bf16 of 1000: 13.9 / 21.8,
-// as frequent as words 26.8 / 24.4; 8192 x 1024 of 50257: 74 / 50; 8192 x 64 of 16: 25 / 16; 8192 x 1001 bf16 of 300: 40 / 27).
+// Whether few_kernel takes them all: up to kFew / 2 positions always, up to kFew if the table is narrow and so
+// short that the CTAs, of which each goes over all positions, fit the device at once, but not so short that a few
+// of them have most of the positions (7424 x 128 of 1792: 8.7 us, with the cluster's sort 14.0; 8192 x 100 of 75000: 18 / 32;
+// but as frequent as words 8192 x 64 of 256: 18.6 / 17.3; 8192 x 512 of 5000: 24 / 19; 8192 x 1024 of 1000: 26.6 / 20.4).
 bool is_few(int64_t count, int64_t vocabulary, int64_t n) {
-    const int64_t spans = (n + 255) / 256;
     return count <= kFew / 2 ||
-           (count <= kFew && vocabulary >= std::max<int64_t>(256, 128 * spans) && spans <= 4 && (vocabulary + kGroup - 1) / kGroup * spans <= 4 * 148);
+           (count <= kFew && n <= 256 && vocabulary >= 1000 && (vocabulary + kGroup - 1) / kGroup <= 4 * 148);
 }
 
 // The workspace's layout from its sizes; the words it needs.
@@ -913,6 +915,10 @@ int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) 
     m->cut = kCut;
     while (m->cut > kCut / 4 && (count / m->cut) * ((n + 255) / 256) < 8 * 148) m->cut /= 2;
     m->pieces = (count + m->cut - 1) / m->cut;
+    // all 16 CTAs before a CTA takes more than 1024: 16384 x 256 of 4000: 21 us, 4096 each 26.5; 10000 x 100
+    // of 75000: 34.5 / 56; beside zeros that take as long 32768 x 1024 of 50257: 62.4 / 61.6
+    s->log_chunk = 10;
+    while (s->log_chunk < 12 && count > kMaxCluster << s->log_chunk) ++s->log_chunk;
     m->width = (n + 7) / 8 * 8;
     auto words = [](int64_t v) { return (v + 31) / 32 * 32; };
     int64_t at = 0;
@@ -1020,7 +1026,7 @@ int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, Sums* m, const rt
     const bool pdl = ctx->pdl;
     if (s.count <= kChunk * kMaxCluster) {
         int ranks = 1;
-        while (ranks * kChunk < s.count) ranks *= 2;
+        while ((int64_t)ranks << s.log_chunk < s.count) ranks *= 2;
         RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t));
         count_launch(ctx);
         if (!m->accumulate) {

@@ -79,8 +79,8 @@ BACK = [("uniform", 1, 1, 1), ("uniform", 5, 3, 2), ("uniform", 63, 256, 300), (
         ("zipf", 300000, 8, 50257),
         # the sorts' other forms: over launches with more buckets than warps' counters, keys of three digits, wide gaps
         ("uniform", 70000, 5, 2 ** 21 - 1), ("zipf", 66000, 4, 300000), ("uniform", 70000, 1, 17000000), ("one", 65537, 12, 100), ("padding", 70000, 4, 1000),
-        ("zipf", 8192, 100, 300), ("one", 8191, 40, 256), ("uniform", 5000, 1000, 600), ("padding", 8000, 24, 70000),
-        ("zipf", 8193, 64, 1000), ("uniform", 4097, 16, 255), ("zipf", 4097, 513, 384), ("uniform", 6001, 1021, 511),
+        ("zipf", 8192, 100, 1300), ("one", 8191, 40, 1000), ("uniform", 5000, 256, 1600), ("padding", 8000, 24, 70000), ("runs", 8100, 33, 1001),
+        ("zipf", 8193, 64, 1000), ("uniform", 4097, 16, 255), ("zipf", 4097, 513, 1384), ("uniform", 6001, 1021, 511), ("zipf", 17000, 40, 70000),
         ("uniform", 5000, 5, 2 ** 21 - 1), ("one", 4097, 8, 2000003), ("zipf", 65536, 4, 66000), ("uniform", 12289, 130, 9000)]
 
 
