@@ -496,8 +496,8 @@ __global__ void __launch_bounds__(kThreads1) mx4_kernel(const __grid_constant__ 
 //
 // 8192^3, bf16 out: 184 us for a single launch, the tensor pipe 84 % busy; launched
 // again and again 183 to 220 us, the clock held down by the 1 kW power limit (154 us
-// on matrices of zeros, which draw less).  In 8 bits, twice the stages: 362 us for a single
-// launch, the tensor pipe 92 % busy, 429 to 443 again and again.
+// on matrices of zeros, which draw less).  In 8 bits, twice the stages: 340 us for a single
+// launch, the tensor pipe 91 % busy, 429 to 443 again and again.
 template <typename F>
 constexpr int kPairStages = F::GROUPS == 1 ? 5 : 6;  // 8 bits: the sixth's room is the epilogue's
 template <typename F>
