@@ -13,8 +13,12 @@
 //  - above, passes over launches (digit_*), each of which moves all positions: how often
 //    the most frequent token occurs does not decide how evenly a pass is spread
 // In the last two piece_kernel and row_kernel sum; the rows of tokens that do not occur are
-// written beside the cluster's sort (fill_kernel), or by row_kernel.  65536 x 1024 bf16 rows of 50257
-// tokens as frequent as words: 75 us, 52 of bytes; 2047 x 1000 f32 of 1000: 6.5 us.
+// written beside the cluster's sort and beside the pieces.  65536 x 1024 bf16 rows of 50257
+// tokens as frequent as words: 81 us, 52 of bytes; 2047 x 1000 f32 of 1000: 6.5 us.
+//
+// Each kernel waits (pdl_wait) for the one before it on the stream before it reads or writes
+// anything: only that wait makes what earlier kernels wrote visible, those before the last one too.  Rows that did not
+// wait for the pieces, of which they need none, took 6 us of these less.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -122,8 +126,8 @@ struct Lay {
         grid = dim3((unsigned)((groups + (8 >> along) - 1) / (8 >> along)), (unsigned)(spans >> along));
     }
 };
-__device__ __forceinline__ int64_t lay_group(int along) {
-    return ((int64_t)blockIdx.x << (3 - along)) + (threadIdx.x >> (5 + along));
+__device__ __forceinline__ int64_t lay_group(int along, unsigned block) {
+    return ((int64_t)block << (3 - along)) + (threadIdx.x >> (5 + along));
 }
 __device__ __forceinline__ int64_t lay_span(int along) {
     return ((int64_t)blockIdx.y << along) + ((threadIdx.x >> 5) & ((1 << along) - 1));
@@ -140,7 +144,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const TE* __restrict__ tabl
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int64_t i0 = lay_group(along) * kRows;
+    const int64_t i0 = lay_group(along, blockIdx.x) * kRows;
     const Columns<ACCESS, kLookup> c(lay_span(along), n, lane);
     const int live = (int)max((int64_t)0, min((int64_t)kRows, count - i0));
     Lane<TE, ACCESS, kLookup> e[kRows];
@@ -166,6 +170,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const TE* __restrict__ tabl
 // The sort's arrays in the workspace, in 32-bit words.  A key is a token, or V for padding.
 struct Sort {
     int64_t count, vocabulary;
+    int64_t filled;      // rows of dE that the cluster's sort looks after: zeros to the absent ones
     int passes;          // by 8 bits of a key
     int ctas;            // of a pass over launches,
     int64_t span;        // and positions of a CTA
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(256) starts_kernel(Sort s) {
 // The whole sort in one launch where the positions fit the shared memory of one cluster:
 // a CTA holds up to kChunk of them, and passes by 8 bits of the key, the low ones first, move
 // them through distributed shared memory.  65536 positions of 50257 tokens: 26 us under a
-// profiler, as long as the launches above, but on 16 SMs: fill_kernel has the others meanwhile.
+// profiler, as long as the launches above, but on 16 SMs: the others have fill() meanwhile.
 constexpr int kChunk = 4096, kMaxCluster = 16, kStride = 257;  // kStride: counters of a warp, off a bank each
 
 struct ClusterSmem {
@@ -376,11 +381,54 @@ __device__ __forceinline__ void sync_cluster() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32_t* __restrict__ tokens) {
+// The first `all` rows of dE, where their tokens do not occur: zeros.  CTA `part` of `parts` marks the tokens of its
+// share of the rows by going over all positions itself, so it needs no sort.
+constexpr int kMarks = 8192;  // rows at a time
+
+template <int ACCESS>
+__device__ __forceinline__ void fill(uint8_t* marks, const uint32_t* tokens, int64_t count, int64_t all, float* out,
+                                     int64_t ldo, int64_t n, uint32_t part, uint32_t parts) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t begin = all * part / parts, end = all * (part + 1) / parts;
+    for (int64_t b = begin; b < end; b += kMarks) {
+        const uint32_t rows = (uint32_t)min(end - b, (int64_t)kMarks);
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < rows; i += 1024) marks[i] = 0;
+        __syncthreads();
+        auto mark = [&](uint32_t token) {
+            if (token - (uint32_t)b < rows) marks[token - (uint32_t)b] = 1;
+        };
+        const int64_t lead = min(count, (int64_t)((16 - (reinterpret_cast<uintptr_t>(tokens) & 15)) & 15) / 4);
+        const int64_t quads = (count - lead) / 4;
+        const uint4* four = reinterpret_cast<const uint4*>(tokens + lead);
+#pragma unroll 8
+        for (int64_t i = threadIdx.x; i < quads; i += 1024) {
+            const uint4 t = __ldg(four + i);
+            mark(t.x), mark(t.y), mark(t.z), mark(t.w);
+        }
+        if (threadIdx.x < lead) mark(tokens[threadIdx.x]);
+        if (threadIdx.x < count - lead - quads * 4) mark(tokens[lead + quads * 4 + threadIdx.x]);
+        __syncthreads();
+        const float zero[8] = {};
+        for (uint32_t r = warp; r < rows; r += 32) {
+            if (marks[r]) continue;
+            float* row = out + (b + r) * ldo;
+            for (int64_t j = 0; j * 256 < n; ++j) Lane<float, ACCESS, 8>::store(row, Columns<ACCESS, 8>(j, n, lane), zero);
+        }
+    }
+}
+
+// The grid's first cluster sorts; the others, on SMs that it leaves idle, write the absent ones of the first s.filled rows.
+template <int ACCESS>
+__global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32_t* tokens, float* out, int64_t ldo, int64_t n) {
     extern __shared__ __align__(16) uint8_t raw[];
     ClusterSmem& m = *reinterpret_cast<ClusterSmem*>(raw);
     pdl_wait();
     pdl_launch_dependents();
+    if (blockIdx.x >= cluster_size()) {
+        fill<ACCESS>(raw, tokens, s.count, s.filled, out, ldo, n, blockIdx.x - cluster_size(), gridDim.x - cluster_size());
+        return;
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
     const int chunk = 1 << s.log_chunk, share = chunk / 32;  // positions of a CTA, of a warp
@@ -493,48 +541,6 @@ __global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32
     sync_cluster();  // a CTA's last item is read by the next one
 }
 
-// The rows of dE whose tokens do not occur: zeros.  A CTA marks the tokens of its share of
-// the rows by going over all positions itself, so it needs no sort, and this kernel runs beside
-// the sort in one cluster, on the SMs that it leaves idle: it waits for it at its
-// end only (65536 positions leave 132 SMs idle for 25 us, the time of 130 MB).
-constexpr int kMarks = 8192;  // rows at a time
-
-template <int ACCESS>
-__global__ void __launch_bounds__(1024) fill_kernel(const uint32_t* __restrict__ tokens, int64_t count, int64_t vocabulary,
-                                                    float* __restrict__ out, int64_t ldo, int64_t n) {
-    __shared__ uint8_t marks[kMarks];
-    pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t begin = vocabulary * blockIdx.x / gridDim.x, end = vocabulary * (blockIdx.x + 1) / gridDim.x;
-    for (int64_t b = begin; b < end; b += kMarks) {
-        const uint32_t rows = (uint32_t)min(end - b, (int64_t)kMarks);
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < rows; i += 1024) marks[i] = 0;
-        __syncthreads();
-        auto mark = [&](uint32_t token) {
-            if (token - (uint32_t)b < rows) marks[token - (uint32_t)b] = 1;
-        };
-        const int64_t lead = min(count, (int64_t)((16 - (reinterpret_cast<uintptr_t>(tokens) & 15)) & 15) / 4);
-        const int64_t quads = (count - lead) / 4;
-        const uint4* four = reinterpret_cast<const uint4*>(tokens + lead);
-#pragma unroll 8
-        for (int64_t i = threadIdx.x; i < quads; i += 1024) {
-            const uint4 t = __ldg(four + i);
-            mark(t.x), mark(t.y), mark(t.z), mark(t.w);
-        }
-        if (threadIdx.x < lead) mark(tokens[threadIdx.x]);
-        if (threadIdx.x < count - lead - quads * 4) mark(tokens[lead + quads * 4 + threadIdx.x]);
-        __syncthreads();
-        const float zero[8] = {};
-        for (uint32_t r = warp; r < rows; r += 32) {
-            if (marks[r]) continue;
-            float* row = out + (b + r) * ldo;
-            for (int64_t j = 0; j * 256 < n; ++j) Lane<float, ACCESS, 8>::store(row, Columns<ACCESS, 8>(j, n, lane), zero);
-        }
-    }
-    pdl_wait();
-}
-
 // The sums.  A token that occurs at most kLight times is light: a warp takes 512 bytes' columns
 // of `tokens` neighbouring rows of dE, whose positions lie one after another, and writes
 // each row once.  The others are heavy: the sorted list is cut into pieces of kCut positions
@@ -549,6 +555,7 @@ constexpr int kColumns = 16 / (int)sizeof(T);
 struct Sums {
     int64_t count, vocabulary, n, spans, width;
     int64_t pieces;
+    int64_t filled;  // rows that have their zeros, where they are absent; piece_kernel writes the others'
     int cut;  // positions of a piece: kCut, a half or a quarter
     const uint32_t* token;
     const uint32_t* position;
@@ -556,7 +563,6 @@ struct Sums {
     float* partial;  // [pieces][2][width]: the heavy run that began in an earlier piece, the one that began in this one
     float scale;
     int accumulate;
-    int zeros;       // row_kernel also writes the rows of tokens that do not occur
     float* out;
     int64_t ldo;
 };
@@ -577,17 +583,35 @@ __device__ __forceinline__ void emit(const Sums& s, uint32_t token, const Column
     L::store(row, c, v);
 }
 
-// Heavy runs, a warp a piece and span: their sums where they lie inside it, else partial ones.
+// Zeros to the rows of tokens that do not occur, a warp kZeros rows and a span.
+constexpr int kZeros = 16;
+
+template <int ACCESS, int N>
+__device__ __forceinline__ void zeros(const Sums& s, int64_t t0, int64_t span) {
+    const int lane = threadIdx.x & 31;
+    const Columns<ACCESS, N> c(span, s.n, lane);
+    const bool there = lane < kZeros && t0 + lane < s.vocabulary;
+    const float zero[N] = {};
+    for (uint32_t empty = __ballot_sync(0xffffffffu, there && s.start[t0 + lane] == s.start[t0 + lane + 1]); empty; empty &= empty - 1)
+        Lane<float, ACCESS, N>::store(s.out + (t0 + __ffs(empty) - 1) * s.ldo, c, zero);
+}
+
+// Heavy runs, a warp a piece and span: their sums where they lie inside it, else partial ones.  The CTAs behind those
+// of the pieces write zeros.
 template <typename T, int ACCESS>
-__global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* __restrict__ dy, int64_t ldy, int along) {
+__global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* dy, int64_t ldy, int along, int piece_blocks) {
     pdl_wait();
     pdl_launch_dependents();
+    if ((int)blockIdx.x >= piece_blocks) {
+        zeros<ACCESS, kColumns<T>>(s, s.filled + lay_group(along, blockIdx.x - piece_blocks) * kZeros, lay_span(along));
+        return;
+    }
     constexpr int N = kColumns<T>, U = 8;  // U: rows of dy under way
     using L = Lane<T, ACCESS, N>;
     const int lane = threadIdx.x & 31;
     const Columns<ACCESS, N> c(lay_span(along), s.n, lane);
     const int64_t real = s.start[s.vocabulary];  // positions that hold a token
-    const int64_t piece = lay_group(along), p0 = piece * s.cut;
+    const int64_t piece = lay_group(along, blockIdx.x), p0 = piece * s.cut;
     const int live = (int)max((int64_t)0, min((int64_t)s.cut, real - p0));
     uint32_t token[kCut / 32], row[kCut / 32], begin[kCut / 32], end[kCut / 32];
     uint64_t heavy = 0;  // a bit a position
@@ -669,15 +693,22 @@ __device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span
     auto add = [&](int64_t piece, int b, int e) {
 #pragma unroll
         for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-#pragma unroll 8
-        for (int q = b; q < e; ++q) {
-            L v;
-            v.load(s.partial + ((piece + q) * 2 + (q == 0 ? 1 : 0)) * s.width, c);
+        constexpr int U = 32 / N;  // partial sums under way
+        for (int q = b; q < e; q += U) {
+            L v[U];
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] += v.value(i);
+            for (int x = 0; x < U; ++x) {
+                const int at = min(q + x, e - 1);
+                v[x].template load<false>(s.partial + ((piece + at) * 2 + (at == 0 ? 1 : 0)) * s.width, c);
+            }
+#pragma unroll
+            for (int x = 0; x < U; ++x)
+                if (q + x < e) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[i] += v[x].value(i);
+                }
         }
     };
-    pdl_wait();  // for the partial sums
     if (few >> warp & 1) {
         add(piece0 + warp, 0, __shfl_sync(0xffffffffu, pieces, warp));
         emit<ACCESS, N>(s, __shfl_sync(0xffffffffu, token, warp), c, sum);
@@ -700,14 +731,13 @@ __device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span
     }
 }
 
-// Light tokens, a warp `tokens` (at most 31) rows of dE and a span; in the CTAs behind those, of which the
-// last ones of the grid are, the joins.  Only the joins need piece_kernel's results, so only
-// they wait for it: what the others read was complete when it passed its own wait.
+// Light tokens, a warp `tokens` (at most 31) rows of dE and a span; in the CTAs behind those, the joins.
 template <typename T, int ACCESS>
 __global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict__ dy, int64_t ldy, int along, int tokens,
                                                      int row_blocks) {
     constexpr int N = kColumns<T>, U = 4;  // U: rows of dy under way
     using L = Lane<T, ACCESS, N>;
+    pdl_wait();
     // Nothing lets the next kernel launch before this one's CTAs end: the sort of the next call
     // would take 16 SMs whole to wait there.
     if ((int)blockIdx.x >= row_blocks) {
@@ -717,16 +747,11 @@ __global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict
     }
     const int lane = threadIdx.x & 31;
     const Columns<ACCESS, N> c(lay_span(along), s.n, lane);
-    const int64_t t0 = lay_group(along) * tokens;
+    const int64_t t0 = lay_group(along, blockIdx.x) * tokens;
     if (t0 >= s.vocabulary) return;
     const int64_t token = min(t0 + min(lane, tokens), s.vocabulary);
     const uint32_t first = s.start[token], next = __shfl_down_sync(0xffffffffu, first, 1);
     const uint32_t count = lane < tokens && token < s.vocabulary ? next - first : 0u;
-    if (s.zeros) {
-        const float zero[N] = {};
-        for (uint32_t empty = __ballot_sync(0xffffffffu, lane < tokens && token < s.vocabulary && count == 0); empty; empty &= empty - 1)
-            Lane<float, ACCESS, N>::store(s.out + (t0 + __ffs(empty) - 1) * s.ldo, c, zero);
-    }
     const uint32_t light = count <= kLight ? count : 0u;
     uint32_t upto = light;  // light positions of the rows up to the lane's
 #pragma unroll
@@ -979,8 +1004,10 @@ int launch_sums(rt_ctx* ctx, const rt_tensor* dy, Sums m) {
     const int tokens = m.vocabulary / 16 * m.spans >= sms * 32 ? 16 : m.vocabulary * m.spans < sms * 48 ? 1 : 4;
     const Lay pieces(m.pieces, m.spans), rows((m.vocabulary + tokens - 1) / tokens, m.spans);
     const T* p = static_cast<const T*>(dy->ptr);
-    RT_CUDA(launch_k(ctx->pdl, piece_kernel<T, ACCESS>, pieces.grid, 256, 0, ctx->stream, m, p, dy->ld, pieces.along));
-    dim3 grid = rows.grid;
+    dim3 grid = pieces.grid;
+    if (!m.accumulate) grid.x += Lay((m.vocabulary - m.filled + kZeros - 1) / kZeros, m.spans).grid.x;
+    RT_CUDA(launch_k(ctx->pdl, piece_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, p, dy->ld, pieces.along, (int)pieces.grid.x));
+    grid = rows.grid;
     grid.x += (unsigned)((m.pieces + kJoin - 1) / kJoin) << rows.along;
     RT_CUDA(launch_k(ctx->pdl, row_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, p, dy->ld, rows.along, tokens,
                      (int)rows.grid.x));
@@ -1022,21 +1049,27 @@ int launch_sums(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, const
 }
 
 // The sort; in one cluster, the rows of dE that no token has beside it.
-int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, Sums* m, const rt_tensor* dtable) {
+int launch_sort(rt_ctx* ctx, const uint32_t* t, Sort s, Sums* m, const rt_tensor* dtable) {
     const bool pdl = ctx->pdl;
     if (s.count <= kChunk * kMaxCluster) {
         int ranks = 1;
         while ((int64_t)ranks << s.log_chunk < s.count) ranks *= 2;
-        RT_CUDA(launch_cluster(ranks, pdl, cluster_sort_kernel, ranks, 1024, sizeof(ClusterSmem), ctx->stream, s, t));
+        const int access = access_of(dtable, 8);
+        auto* kernel = access == 32 ? cluster_sort_kernel<32> : access == 16 ? cluster_sort_kernel<16> : cluster_sort_kernel<0>;
+        // Beside the sort as many clusters as the device holds, a CTA with 16 rows or more: it goes over all tokens.
+        // Both wait for the memory, so beside the sort lie as many rows as it has time for, the others beside the pieces:
+        // half of them or more (8192 x 1024 of 50257: 49 us, all 52, none 59), and 32 MB with 1.5 KB a position (65536 x 1024
+        // of 50257: 81 us, all 83, none 90; 65536 x 256 of 128256: 61, half 66, none 74).  Tables below 16 MB
+        // have them all beside the pieces (17314 x 33 of 593: 23.4, beside the sort 24.2; 10000 x 100 of 75000,
+        // 30 MB: 37.5 / 34.3).
+        const int64_t row = m->n * 4;
+        if (!m->accumulate && s.vocabulary * row >= 16 << 20)
+            s.filled = std::min(s.vocabulary, std::max(s.vocabulary / 2, ((32 << 20) + s.count * 1536) / row));
+        const int64_t fills = std::min<int64_t>(ctx->sort_clusters[ranks == 16] - 1, s.filled / (16 * ranks));
+        m->filled = s.filled = fills ? s.filled : 0;
+        RT_CUDA(launch_cluster(ranks, pdl, kernel, (unsigned)((1 + fills) * ranks), 1024, sizeof(ClusterSmem), ctx->stream, s, t, m->out,
+                               m->ldo, m->n));
         count_launch(ctx);
-        if (!m->accumulate) {
-            // a CTA to an SM that is left, each with 16 rows or more: it goes over all tokens
-            const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count - ranks, s.vocabulary / 16));
-            const int access = access_of(dtable, 8);
-            auto* fill = access == 32 ? fill_kernel<32> : access == 16 ? fill_kernel<16> : fill_kernel<0>;
-            RT_CUDA(launch_k(pdl, fill, (unsigned)grid, 1024, 0, ctx->stream, t, s.count, s.vocabulary, m->out, m->ldo, m->n));
-            count_launch(ctx);
-        }
         return RT_OK;
     }
     Pass p{t, nullptr, nullptr, nullptr, nullptr, 0};
@@ -1051,7 +1084,6 @@ int launch_sort(rt_ctx* ctx, const uint32_t* t, const Sort& s, Sums* m, const rt
     }
     RT_CUDA(launch_k(pdl, starts_kernel, (unsigned)((s.count + 255) / 256), 256, 0, ctx->stream, s));
     count_launch(ctx, 2 * s.passes + 1);
-    m->zeros = !m->accumulate;  // each filling CTA would go over more tokens than the sorted list costs
     return RT_OK;
 }
 
@@ -1066,9 +1098,29 @@ int check_tokens(const char* what, const rt_tensor* tokens, const rt_tensor* row
 
 }  // namespace
 
-int embedding_init() {
-    RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSmem)));
-    RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+template <int ACCESS>
+int allow_sort() {
+    RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel<ACCESS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSmem)));
+    RT_CUDA(cudaFuncSetAttribute(cluster_sort_kernel<ACCESS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    return RT_OK;
+}
+
+int embedding_init(rt_ctx* ctx) {
+    RT_TRY(allow_sort<0>());
+    RT_TRY(allow_sort<16>());
+    RT_TRY(allow_sort<32>());
+    for (int i = 0; i < 2; ++i) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr;
+        cfg.gridDim = dim3(1024);
+        cfg.blockDim = dim3(1024);
+        cfg.dynamicSmemBytes = sizeof(ClusterSmem);
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {8u << i, 1, 1};
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        RT_CUDA(cudaOccupancyMaxActiveClusters(&ctx->sort_clusters[i], cluster_sort_kernel<32>, &cfg));
+    }
     return RT_OK;
 }
 

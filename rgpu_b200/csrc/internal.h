@@ -69,6 +69,7 @@ struct rt_ctx {
     size_t x3_scratch_bytes = 0;
     std::vector<void*> x3_retired;
     int l2_group = 8;
+    int sort_clusters[2] = {1, 1};  // clusters of 8 and of 16 CTAs of the embedding's sort that the device holds at once
     // device address of rt_matmul_split_k_noalloc's built-in scratch array
     // (looked up on that entry point's first call on this context)
     float* splitk_static = nullptr;
@@ -291,7 +292,7 @@ int launch_sum_partials_own(rt_ctx* ctx, float* out, const float* own, const flo
 int launch_fill_column(rt_ctx* ctx, void* p, rt_dtype dt, int64_t rows, int64_t ld, int64_t col, float value,
                        cudaStream_t stream);
 
-int embedding_init();
+int embedding_init(rt_ctx* ctx);
 int gemm_mx4_init();
 int mx4_encode_maps(rt_mx4* q);
 // C[m,n] = A[m,k] B[n,k]^T + 1 bias (+ ReLU) of microscaled 4-bit matrices.

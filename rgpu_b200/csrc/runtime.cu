@@ -119,7 +119,7 @@ int rt_ctx_create(int device, rt_ctx** out) {
     if (st == RT_OK) st = gemm_x3_init(c);
     if (st == RT_OK) st = gemm_skinny_init();
     if (st == RT_OK) st = gemm_mx4_init();
-    if (st == RT_OK) st = embedding_init();
+    if (st == RT_OK) st = embedding_init(c);
     if (st != RT_OK) {
         cudaFree(c->dev_err);
         cudaStreamDestroy(c->own_stream);
