@@ -74,16 +74,16 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* x, int64_t ldx, c
         const int64_t j0 = (int64_t)chunk * P::WARP, j = j0 + lane * P::E;
         P v, a;
         if constexpr (V == 0) {
-            const auto r = P::template fetch_any<false>(x + j0, p.cols - j0, lane);
+            const auto r = P::fetch_any(x + j0, p.cols - j0, lane);
             if (ADD) {
-                const auto s = P::template fetch_any<false>(add + j0, p.cols - j0, lane);
+                const auto s = P::fetch_any(add + j0, p.cols - j0, lane);
                 a.deal_any(s, P::between(add + j0), box, lane);
             }
             v.deal_any(r, P::between(x + j0), box, lane);
         } else {
             if (j >= p.cols) break;
-            v.template load_whole<V, false>(x + j);
-            if (ADD) a.template load_whole<V, false>(add + j);
+            v.template load_whole<V>(x + j);
+            if (ADD) a.template load_whole<V>(add + j);
         }
 #pragma unroll
         for (int g = 0; g < P::E / 8; ++g) {

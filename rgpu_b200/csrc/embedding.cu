@@ -58,8 +58,6 @@ struct Lane {
         else if constexpr (ACCESS == 0) return __uint_as_float(w[i] << 16);
         else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
-    // NC: the kernel writes no row of this matrix
-    template <bool NC = true>
     __device__ __forceinline__ void load(const T* row, const C& c) {
         const T* p = row + c.first;
         if constexpr (ACCESS == 0) {
@@ -71,15 +69,16 @@ struct Lane {
                     else w[i] = reinterpret_cast<const uint32_t*>(p)[i * 32];
                 }
             }
-        } else if constexpr (WIDE == 8 && NC) {
-            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        } else if constexpr (WIDE == 8) {
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                         : "l"(p));
+                         : "l"(p)
+                         : "memory");
         } else {
 #pragma unroll
             for (int i = 0; i < WORDS; i += 4) {
                 const uint4* q = reinterpret_cast<const uint4*>(p) + i / 4;
-                const uint4 u = NC ? __ldg(q) : *q;
+                const uint4 u = *q;
                 w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
             }
         }
@@ -138,9 +137,9 @@ __device__ __forceinline__ int64_t lay_span(int along) {
 constexpr int kRows = 4, kLookup = 8;
 
 template <typename TE, typename TY, int ACCESS>
-__global__ void __launch_bounds__(256) lookup_kernel(const TE* __restrict__ table, int64_t lde, int64_t vocabulary,
-                                                     const uint32_t* __restrict__ tokens, int64_t count, int64_t n,
-                                                     int along, float scale, TY* __restrict__ y, int64_t ldy) {
+__global__ void __launch_bounds__(256) lookup_kernel(const TE* table, int64_t lde, int64_t vocabulary,
+                                                     const uint32_t* tokens, int64_t count, int64_t n,
+                                                     int along, float scale, TY* y, int64_t ldy) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -151,7 +150,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const TE* __restrict__ tabl
     bool there[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-        const uint32_t token = r < live ? __ldg(tokens + i0 + r) : 0u;
+        const uint32_t token = r < live ? tokens[i0 + r] : 0u;
         there[r] = r < live && token < vocabulary;
         if (there[r]) e[r].load(table + token * lde, c);
     }
@@ -184,7 +183,7 @@ struct Sort {
 };
 
 __device__ __forceinline__ uint32_t key_of(const Sort& s, const uint32_t* tokens, int64_t i) {
-    return min(__ldg(tokens + i), (uint32_t)s.vocabulary);
+    return min(tokens[i], (uint32_t)s.vocabulary);
 }
 
 // cnt[digit] += how many lanes have it; returns the lane's rank: those of this warp before it.
@@ -403,7 +402,7 @@ __device__ __forceinline__ void fill(uint8_t* marks, const uint32_t* tokens, int
         const uint4* four = reinterpret_cast<const uint4*>(tokens + lead);
 #pragma unroll 8
         for (int64_t i = threadIdx.x; i < quads; i += 1024) {
-            const uint4 t = __ldg(four + i);
+            const uint4 t = four[i];
             mark(t.x), mark(t.y), mark(t.z), mark(t.w);
         }
         if (threadIdx.x < lead) mark(tokens[threadIdx.x]);
@@ -573,7 +572,7 @@ __device__ __forceinline__ void emit(const Sums& s, uint32_t token, const Column
     float* row = s.out + token * s.ldo;
     if (s.accumulate) {
         L old;
-        old.template load<false>(row, c);
+        old.load(row, c);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = old.value(i) + v[i] * s.scale;
     } else {
@@ -699,7 +698,7 @@ __device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span
 #pragma unroll
             for (int x = 0; x < U; ++x) {
                 const int at = min(q + x, e - 1);
-                v[x].template load<false>(s.partial + ((piece + at) * 2 + (at == 0 ? 1 : 0)) * s.width, c);
+                v[x].load(s.partial + ((piece + at) * 2 + (at == 0 ? 1 : 0)) * s.width, c);
             }
 #pragma unroll
             for (int x = 0; x < U; ++x)
@@ -733,7 +732,7 @@ __device__ __forceinline__ void join(const Sums& s, int64_t piece0, int64_t span
 
 // Light tokens, a warp `tokens` (at most 31) rows of dE and a span; in the CTAs behind those, the joins.
 template <typename T, int ACCESS>
-__global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict__ dy, int64_t ldy, int along, int tokens,
+__global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* dy, int64_t ldy, int along, int tokens,
                                                      int row_blocks) {
     constexpr int N = kColumns<T>, U = 4;  // U: rows of dy under way
     using L = Lane<T, ACCESS, N>;
@@ -805,7 +804,7 @@ __global__ void __launch_bounds__(256, 4) row_kernel(Sums s, const T* __restrict
 constexpr int kFew = 8192, kGroup = 128;
 
 template <typename T, int ACCESS, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, const uint32_t* __restrict__ tokens, const T* __restrict__ dy,
+__global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, const uint32_t* tokens, const T* dy,
                                                   int64_t ldy, int group) {
     constexpr int N = kColumns<T>;
     using L = Lane<T, ACCESS, N>;
@@ -825,7 +824,7 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, con
     const int64_t t0 = (int64_t)blockIdx.x * group;
     const int rows = (int)min((int64_t)group, s.vocabulary - t0);
     const Columns<ACCESS, N> c(blockIdx.y, s.n, lane);
-    auto key = [&](int64_t i) { return __ldg(tokens + i) - (uint32_t)t0; };
+    auto key = [&](int64_t i) { return tokens[i] - (uint32_t)t0; };
     auto mine = [&](uint32_t k, bool there) { return there && k < (uint32_t)rows; };
     in_order<WARPS>(s.count, warp, lane, key, [&](int64_t, uint32_t k, bool there) {
         if (__ballot_sync(0xffffffffu, mine(k, there))) count_rank(cnt[warp], k, mine(k, there), lane);

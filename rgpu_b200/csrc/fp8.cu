@@ -59,11 +59,11 @@ __device__ __forceinline__ float2 decode2(uint32_t codes) {
 // four blocks (f32: two), eight (sixteen) lanes to a block.  HBM-bound: 2 (f32: 4) bytes in,
 // 129/128 out per element; 8192 x 8192 bf16 30 us, 6.7 TB/s.
 template <typename T, int V>
-__global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* __restrict__ src, int64_t ld,
+__global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* src, int64_t ld,
                                                                        int64_t rows, int64_t k, Rows w,
                                                                        int64_t row_bytes, int64_t groups,
-                                                                       uint8_t* __restrict__ codes,
-                                                                       uint8_t* __restrict__ scales) {
+                                                                       uint8_t* codes,
+                                                                       uint8_t* scales) {
     using P = Piece<T>;
     constexpr int PER_BLOCK = 128 / P::E;
     __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* 
                 // V: rows are whole pieces; in place of a row or a piece that is not there another is read
                 const T* at = src + row * ld + (j < k ? j : 0);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) x[q].template load_whole<V, true>(at + min(q, live - 1) * (32 * ld));
+                for (int q = 0; q < 4; ++q) x[q].template load_whole<V>(at + min(q, live - 1) * (32 * ld));
                 if (j >= k)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* 
 // 4096 x 8192 f32: 31 us, 5.4 TB/s; with 64 rows a thread and a condition on each load 39.
 template <typename T, bool PAIR, bool WIDE>
 __global__ void __launch_bounds__(PAIR ? 256 : 512) quantize_columns_kernel(
-    const T* __restrict__ src, int64_t ld, int64_t rows, int64_t k, int64_t blocks, int64_t row_bytes, int64_t groups,
-    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    const T* src, int64_t ld, int64_t rows, int64_t k, int64_t blocks, int64_t row_bytes, int64_t groups,
+    uint8_t* codes, uint8_t* scales) {
     constexpr int W = PAIR ? 2 : 1, N = 32, SHARES = 128 / N;  // columns, rows of a thread; threads to a column
     __shared__ uint32_t maxima[SHARES][128];
     pdl_wait();
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(PAIR ? 256 : 512) quantize_columns_kernel(
         uint32_t u[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if constexpr (PAIR || sizeof(T) == 4) u[i] = __ldg(reinterpret_cast<const uint32_t*>(p + i * ld));
+            if constexpr (PAIR || sizeof(T) == 4) u[i] = *reinterpret_cast<const uint32_t*>(p + i * ld);
             else u[i] = *reinterpret_cast<const uint16_t*>(p + i * ld);
         }
 #pragma unroll
@@ -219,9 +219,9 @@ __global__ void __launch_bounds__(PAIR ? 256 : 512) quantize_columns_kernel(
 // The rows of quantize_rows_kernel, the other way.  f32 holds every value exactly; bf16 all
 // but the smallest (below 2^-133), rounded.  8192 x 8192 bf16: 29 us, 6.9 TB/s.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes,
-                                                         const uint8_t* __restrict__ scales, int64_t rows, int64_t k,
-                                                         Rows w, int64_t row_bytes, int64_t groups, T* __restrict__ dst,
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* codes,
+                                                         const uint8_t* scales, int64_t rows, int64_t k,
+                                                         Rows w, int64_t row_bytes, int64_t groups, T* dst,
                                                          int64_t ld) {
     using P = Piece<T>;
     __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
             if (V ? j >= k : j0 >= k) continue;
             const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);
             if (live <= 0) continue;
-            const uint4 s = __ldg(reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j0 >> 9)) * 512 + (row & 31) * 16));
+            const uint4 s = *reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j0 >> 9)) * 512 + (row & 31) * 16);
             const uint32_t word[4] = {s.x, s.y, s.z, s.w};
             // without a branch (Piece::load_whole): another piece or row in place of one that is not there
             const uint8_t* in = codes + row * row_bytes + (j < k ? j : j0);
@@ -244,10 +244,10 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
             for (int q = 0; q < 4; ++q) {
                 const uint8_t* at = in + min(q, live - 1) * (32 * row_bytes);
                 if constexpr (P::E == 16) {
-                    const uint4 four = __ldg(reinterpret_cast<const uint4*>(at));
+                    const uint4 four = *reinterpret_cast<const uint4*>(at);
                     c[q][0] = four.x, c[q][1] = four.y, c[q][2] = four.z, c[q][3] = four.w;
                 } else {
-                    const uint2 two = __ldg(reinterpret_cast<const uint2*>(at));
+                    const uint2 two = *reinterpret_cast<const uint2*>(at);
                     c[q][0] = two.x, c[q][1] = two.y;
                 }
             }

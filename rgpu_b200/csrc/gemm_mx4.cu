@@ -190,7 +190,7 @@ __device__ __forceinline__ float at_least(float v, float floor) {
 
 __device__ __forceinline__ void load_bias4(const Mx4Params& p, int64_t col, float (&bias)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? __ldg(p.bias + col + i) : 0.0f;
+    for (int i = 0; i < 4; ++i) bias[i] = p.bias && col + i < p.n ? p.bias[col + i] : 0.0f;
 }
 
 template <typename T>

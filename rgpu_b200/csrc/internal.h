@@ -186,7 +186,9 @@ enum { PDL_NONE = 0, PDL_WAIT_START = 1, PDL_WAIT_EPILOGUE = 2, PDL_NO_WAIT = 3 
 // Programmatic dependent launch in device code (PTX griddepcontrol): wait
 // until the grid this one depends on has completed and its writes are
 // visible; let the grids that depend on this one launch.  Both are no-ops in
-// a kernel launched the ordinary way.
+// a kernel launched the ordinary way.  What is read behind the wait may have been
+// written while this grid was already there, so it is not read by loads for memory that does
+// not change (ld.global.nc, __ldg, restricted pointers to const).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -34,10 +34,10 @@ __device__ __forceinline__ uint32_t encode(const Piece<T>& x, int i, float inv) 
 // bound: 2 (f32: 4) bytes in and 17/32 out per element.  8192 x 8192 bf16: 30 us,
 // 5.7 TB/s.
 template <typename T, int V>
-__global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
+__global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* src, int64_t ld, int64_t rows,
                                                                int64_t k, Rows w, int64_t blocks, int64_t groups,
-                                                               uint8_t* __restrict__ codes,
-                                                               uint8_t* __restrict__ scales) {
+                                                               uint8_t* codes,
+                                                               uint8_t* scales) {
     using P = Piece<T>;
     constexpr int PER_BLOCK = 32 / P::E, PER_GROUP = 128 / P::E;  // lanes that share a block, a scale group
     __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(256, V ? 4 : 3) quantize_rows_kernel(const T* 
 // where their bytes take 23 and 13 at the rate of a copy: bound by the 32 scattered
 // rows of a warp's reads, not by HBM.
 template <typename T, bool PAIR>
-__global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
+__global__ void __launch_bounds__(256) quantize_columns_kernel(const T* src, int64_t ld, int64_t rows,
                                                                int64_t k, int64_t blocks, int64_t groups,
-                                                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+                                                               uint8_t* codes, uint8_t* scales) {
     __shared__ uint32_t tile[128];
     pdl_wait();
     pdl_launch_dependents();
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) quantize_columns_kernel(const T* __restri
                 uint32_t u = 0;
                 if (k0 + i < k && col < rows) {
                     if (col + 1 < rows)
-                        u = __ldg(reinterpret_cast<const uint32_t*>(p + i * ld));
+                        u = *reinterpret_cast<const uint32_t*>(p + i * ld);
                     else
                         u = *reinterpret_cast<const uint16_t*>(p + i * ld);
                 }
@@ -185,9 +185,9 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // in f32).  HBM-bound: 17/32 bytes in, 2 (f32: 4) out per element.  8192 x 8192
 // bf16: 28 us, 6.0 TB/s.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ codes,
-                                                         const uint8_t* __restrict__ scales, int64_t rows, int64_t k,
-                                                         Rows w, int64_t blocks, int64_t groups, T* __restrict__ dst,
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* codes,
+                                                         const uint8_t* scales, int64_t rows, int64_t k,
+                                                         Rows w, int64_t blocks, int64_t groups, T* dst,
                                                          int64_t ld) {
     using P = Piece<T>;
     __shared__ __align__(16) uint32_t boxes[V ? 1 : 8][256];
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
             if (V ? j >= k : j0 >= k) continue;
             const bool inside = j < blocks * 32;
             const int live = (int)min((int64_t)4, (rows - row + 31) >> 5);
-            const uint4 s = !inside ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j >> 7)) * 512 + (row & 31) * 16));
+            const uint4 s = !inside ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(scales + ((row >> 7) * groups + (j >> 7)) * 512 + (row & 31) * 16);
             const uint32_t word[4] = {s.x, s.y, s.z, s.w};
             const uint8_t* in = codes + row * row_bytes + (j >> 1);
             uint32_t c[4][P::E / 8];
@@ -211,11 +211,11 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
                 c[q][0] = c[q][P::E / 8 - 1] = 0;
                 if (q < live && inside) {
                     if constexpr (sizeof(T) == 2) {
-                        const uint2 two = __ldg(reinterpret_cast<const uint2*>(in + q * (32 * row_bytes)));
+                        const uint2 two = *reinterpret_cast<const uint2*>(in + q * (32 * row_bytes));
                         c[q][0] = two.x;
                         c[q][P::E / 8 - 1] = two.y;
                     } else {
-                        c[q][0] = __ldg(reinterpret_cast<const uint32_t*>(in + q * (32 * row_bytes)));
+                        c[q][0] = *reinterpret_cast<const uint32_t*>(in + q * (32 * row_bytes));
                     }
                 }
             }

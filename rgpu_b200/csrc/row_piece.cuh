@@ -21,22 +21,17 @@ struct Piece {
     uint32_t w[8];
 
     // All of the piece.  Without a branch, so that one load is not waited for before the next
-    // is issued (dropout of 8192 x 8192 bf16 78 us, with load below 92).  NC: the kernel
-    // writes none of what it reads.
-    template <int V, bool NC>
+    // is issued (dropout of 8192 x 8192 bf16 78 us, with load below 92).
+    template <int V>
     __device__ __forceinline__ void load_whole(const T* p) {
-        if constexpr (V == 32 && NC) {
-            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                         : "l"(p));
-        } else if constexpr (V == 32) {
+        if constexpr (V == 32) {
             asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                          : "l"(p)
                          : "memory");
         } else {
             const uint4* at = reinterpret_cast<const uint4*>(p);
-            const uint4 a = NC ? __ldg(at) : at[0], b = NC ? __ldg(at + 1) : at[1];
+            const uint4 a = at[0], b = at[1];
             w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
             w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
         }
@@ -44,13 +39,9 @@ struct Piece {
     template <int V>
     __device__ __forceinline__ void load(const T* p, int64_t left) {
         if (V == 32 && left >= E) {
-            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                         : "l"(p));
+            load_whole<32>(p);
         } else if (V == 16 && left >= E) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+            load_whole<16>(p);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] = 0;
@@ -93,7 +84,6 @@ struct Piece {
     };
     static __device__ __forceinline__ bool between(const T* p) { return sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(p) & 2); }
     static __device__ __forceinline__ uint32_t half(const T* p) { return *reinterpret_cast<const unsigned short*>(p); }
-    template <bool NC = true>
     static __device__ __forceinline__ Words fetch_any(const T* p, int64_t left, int lane) {
         Words r;
         constexpr int N = 4 / sizeof(T);  // elements of a word
@@ -103,7 +93,7 @@ struct Piece {
         for (int i = 0; i < 8; ++i) {
             const int at = i * 32 + lane;
             const int64_t room = left - odd - at * N;
-            r.v[i] = room >= N ? (NC ? __ldg(words + at) : words[at]) : N == 2 && room == 1 ? half(p + odd + at * N) : 0u;
+            r.v[i] = room >= N ? words[at] : N == 2 && room == 1 ? half(p + odd + at * N) : 0u;
         }
         r.head = odd && lane == 0 && left > 0 ? half(p) << 16 : 0u;
         return r;

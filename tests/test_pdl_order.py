@@ -37,3 +37,11 @@ def test_every_kernel_waits_first(name, count):
         before = body[:at]
         assert before.count("{") == before.count("}"), f"{name}: {what} waits on one of its paths only"
         assert "return" not in before and "launch_dependents" not in before, f"{name}: {what} waits too late"
+
+
+@pytest.mark.parametrize("name", ["embedding.cu", "dropout.cu", "fp8.cu", "row_piece.cuh", "scaled.cuh", "mx4.cu", "mx4.cuh", "gemm_mx4.cu"])
+def test_no_load_needs_memory_that_never_changes(name):
+    # ld.global.nc, which __ldg is and which a compiler may make of a restricted pointer to const, is for memory that
+    # is not written for as long as the grid runs.  A dependent grid runs while the one before it writes what it reads.
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+    assert not re.findall(r"__ldg|\.nc\b|const [\w:]+\s*\*\s*__restrict__", text)
