@@ -125,7 +125,7 @@ __device__ __forceinline__ void vector4(const float* x, float other, int64_t bas
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t j = base + i * kWide + threadIdx.x;
-        v[i] = x && j < n ? __ldg(x + j * stride) : other;
+        v[i] = x && j < n ? x[j * stride] : other;
     }
 }
 template <typename T>
@@ -400,7 +400,7 @@ __device__ __forceinline__ void store8(void* base, int64_t at, const float (&v)[
 // v = p[at..], or `other` where there is no vector.
 __device__ __forceinline__ void vector8(const float* p, int64_t at, float other, float (&v)[8]) {
     if (p) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p + at)), b = __ldg(reinterpret_cast<const float4*>(p + at) + 1);
+        const float4 a = *reinterpret_cast<const float4*>(p + at), b = reinterpret_cast<const float4*>(p + at)[1];
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
         v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
@@ -525,8 +525,8 @@ __global__ void __launch_bounds__(cta_threads(TPR)) forward_rows_kernel(BlockP p
             unpack8<T>(raw, y[c]);
         }
         const Stat s = stat_of<TPR, C>(p.post, y, has, inv_n, red, turn);
-        const float one = p.gate_mode == GATE_ONE              ? __ldg(static_cast<const float*>(p.gate))
-                          : p.gate_mode == GATE_COLUMN && live ? __ldg(static_cast<const float*>(p.gate) + row * p.ldg)
+        const float one = p.gate_mode == GATE_ONE              ? *static_cast<const float*>(p.gate)
+                          : p.gate_mode == GATE_COLUMN && live ? static_cast<const float*>(p.gate)[row * p.ldg]
                                                                : 1.0f;
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_strided_kernel(Bloc
         for (int i = 0; i < E; ++i) x[i] = (x[i] - s.mu) * s.rho * gamma[i];
         if (beta) {
             float w[E];
-            load([&](int j) { return __ldg(beta + j); }, 0.0f, w);
+            load([&](int j) { return beta[j]; }, 0.0f, w);
 #pragma unroll
             for (int i = 0; i < E; ++i) x[i] += w[i];
         }
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) forward_strided_kernel(Bloc
     // thread's elements, so that their reads are under way together
     auto vector = [&](const float* x, int stride, float (&v)[E]) {
         if (x)
-            load([&](int j) { return __ldg(x + (int64_t)j * stride); }, 0.0f, v);
+            load([&](int j) { return x[(int64_t)j * stride]; }, 0.0f, v);
         else
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] = 1.0f;
@@ -905,8 +905,8 @@ __device__ __forceinline__ void store8(void* base, int64_t at, const f2 (&v)[4])
 
 // The gate where it is the same for every row (1 where it is not).
 __device__ __forceinline__ float shared_gate(const BlockP& p, int j) {
-    return p.gate_mode == GATE_ONE   ? __ldg(static_cast<const float*>(p.gate))
-           : p.gate_mode == GATE_ROW ? __ldg(static_cast<const float*>(p.gate) + j)
+    return p.gate_mode == GATE_ONE   ? *static_cast<const float*>(p.gate)
+           : p.gate_mode == GATE_ROW ? static_cast<const float*>(p.gate)[j]
                                      : 1.0f;
 }
 
@@ -943,10 +943,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
     float *vp = sm.vec, *vq = vp + (mask & 1 ? n : 0), *v2 = vq + (mask & 2 ? n : 0), *vb = v2 + (mask & 4 ? n : 0);
     for (int j = threadIdx.x; j < n; j += kRingThreads) {
         const float sg = p.scale * shared_gate(p, j);
-        if (mask & 1) vp[j] = sg * (p.post.gamma ? __ldg(p.post.gamma + j) : 1.0f);
-        if (mask & 2) vq[j] = sg * __ldg(p.post.beta + j);
-        if (mask & 4) v2[j] = __ldg(p.pre.gamma + j);
-        if (mask & 8) vb[j] = __ldg(p.pre.beta + j);
+        if (mask & 1) vp[j] = sg * (p.post.gamma ? p.post.gamma[j] : 1.0f);
+        if (mask & 2) vq[j] = sg * p.post.beta[j];
+        if (mask & 4) v2[j] = p.pre.gamma[j];
+        if (mask & 8) vb[j] = p.pre.beta[j];
     }
     __syncthreads();
     bool ok = true;  // this thread's waits so far
@@ -1039,7 +1039,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) forward_ring_kernel(BlockP p,
                             for (int i = 0; i < 4; ++i) y[i] = add2(y[i], w[i]);
                         }
                         if (p.gate_mode == GATE_COLUMN) {
-                            const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
+                            const f2 one = splat2(static_cast<const float*>(p.gate)[row * p.ldg]);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) y[i] = mul2(y[i], one);
                         } else if (p.gate_mode == GATE_FULL) {
@@ -1204,9 +1204,9 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
     for (int j = threadIdx.x; j < cols; j += kBackThreads) {
         const bool in = (BULK && CL == 1) || j < n;
         const int at = col0 + j;
-        if (mask & 1) v2[j] = in ? __ldg(p.pre.gamma + at) : 0.0f;
-        if (mask & 2) vp[j] = in ? p.scale * shared_gate(p, at) * (p.post.gamma ? __ldg(p.post.gamma + at) : 1.0f) : 0.0f;
-        if (mask & 4) vb[j] = in ? p.scale * __ldg(p.post.beta + at) : 0.0f;
+        if (mask & 1) v2[j] = in ? p.pre.gamma[at] : 0.0f;
+        if (mask & 2) vp[j] = in ? p.scale * shared_gate(p, at) * (p.post.gamma ? p.post.gamma[at] : 1.0f) : 0.0f;
+        if (mask & 4) vb[j] = in ? p.scale * p.post.beta[at] : 0.0f;
     }
     __syncthreads();
     // the slot's rows: z, then y, dz, dh; not BULK: all of them, and a gate's
@@ -1441,7 +1441,7 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_ring_kernel(BlockP p
                     if (!BULK) store8<T>(slots, at_gate / sizeof(T) + j[c], u);
                     else if (q.dgate) store8<T>(q.dgate, row * q.lddg + col0 + j[c], u);
                 } else {
-                    const f2 one = splat2(__ldg(static_cast<const float*>(p.gate) + row * p.ldg));
+                    const f2 one = splat2(static_cast<const float*>(p.gate)[row * p.ldg]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) gate[i] = one;
                 }
@@ -1560,8 +1560,8 @@ __global__ void __launch_bounds__(kBackThreads, 1) backward_pipe_kernel(BlockP p
     float *v2 = sm.vec, *vp = v2 + n;
     for (int j = threadIdx.x; j < n; j += kBackThreads) {
         const int at = col0 + j;
-        v2[j] = p.pre.gamma ? __ldg(p.pre.gamma + at) : 1.0f;
-        vp[j] = p.scale * shared_gate(p, at) * (p.post.gamma ? __ldg(p.post.gamma + at) : 1.0f);
+        v2[j] = p.pre.gamma ? p.pre.gamma[at] : 1.0f;
+        vp[j] = p.scale * shared_gate(p, at) * (p.post.gamma ? p.post.gamma[at] : 1.0f);
     }
     __syncthreads();
     bool ok = true;  // this thread's waits so far

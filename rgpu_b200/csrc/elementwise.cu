@@ -47,9 +47,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 // one exp per element, one write of delta (the generic form below reads a
 // row three times and takes each exp twice).  Both forms give the same bits.
 template <typename TD, int VPL>
-__global__ void xent_reg_kernel(const float* __restrict__ logits, int64_t ldz, const uint32_t* __restrict__ labels,
-                                int64_t n, int64_t C, float scale, TD* __restrict__ delta, int64_t ldd,
-                                float* __restrict__ loss) {
+__global__ void xent_reg_kernel(const float* logits, int64_t ldz, const uint32_t* labels,
+                                int64_t n, int64_t C, float scale, TD* delta, int64_t ldd,
+                                float* loss) {
     pdl_wait();  // programmatic dependent launch: the kernel before this one is done
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -61,7 +61,7 @@ __global__ void xent_reg_kernel(const float* __restrict__ logits, int64_t ldz, c
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
         const int64_t j = lane + 32 * k;
-        v[k] = j < C ? __ldg(z + j) : -INFINITY;
+        v[k] = j < C ? z[j] : -INFINITY;
         mx = fmaxf(mx, v[k]);
     }
     mx = warp_max(mx);
@@ -90,9 +90,9 @@ __global__ void xent_reg_kernel(const float* __restrict__ logits, int64_t ldz, c
 }
 
 template <typename TD>
-__global__ void xent_kernel(const float* __restrict__ logits, int64_t ldz, const uint32_t* __restrict__ labels,
-                            int64_t n, int64_t C, float scale, TD* __restrict__ delta, int64_t ldd,
-                            float* __restrict__ loss) {
+__global__ void xent_kernel(const float* logits, int64_t ldz, const uint32_t* labels,
+                            int64_t n, int64_t C, float scale, TD* delta, int64_t ldd,
+                            float* loss) {
     pdl_wait();  // programmatic dependent launch: the kernel before this one is done
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

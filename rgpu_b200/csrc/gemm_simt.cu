@@ -223,7 +223,7 @@ __global__ void splitk_reduce_kernel(SimtParams p, int slices) {
         for (int z0 = 0; z0 < slices; z0 += 8) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = z0 + u < slices ? __ldg(p.ws + (int64_t)(z0 + u) * total + idx) : 0.0f;
+            for (int u = 0; u < 8; ++u) v[u] = z0 + u < slices ? p.ws[(int64_t)(z0 + u) * total + idx] : 0.0f;
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 if (z0 + u < slices) s += v[u];
@@ -256,7 +256,7 @@ __global__ void splitk_reduce4_kernel(SimtParams p, int slices) {
                 float4 v[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    v[u] = z0 + u < slices ? __ldg(reinterpret_cast<const float4*>(src + (int64_t)(z0 + u) * total))
+                    v[u] = z0 + u < slices ? *reinterpret_cast<const float4*>(src + (int64_t)(z0 + u) * total)
                                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int u = 0; u < 4; ++u)

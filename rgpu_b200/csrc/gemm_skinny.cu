@@ -27,7 +27,7 @@ template <typename T>
 __device__ __forceinline__ float ld_f(const T* p, int64_t i);
 template <>
 __device__ __forceinline__ float ld_f<float>(const float* p, int64_t i) {
-    return __ldg(p + i);
+    return p[i];
 }
 template <>
 __device__ __forceinline__ float ld_f<__nv_bfloat16>(const __nv_bfloat16* p, int64_t i) {
@@ -35,9 +35,9 @@ __device__ __forceinline__ float ld_f<__nv_bfloat16>(const __nv_bfloat16* p, int
 }
 
 // Four consecutive elements from a 4-element-aligned address, as f32.
-__device__ __forceinline__ float4 ld4_f(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ float4 ld4_f(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 ld4_f(const __nv_bfloat16* p) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
     const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
     const float2 hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
     return make_float4(lo.x, lo.y, hi.x, hi.y);
@@ -219,8 +219,8 @@ __global__ void __launch_bounds__(kThreads) skinny_n_kernel(SkinnyParams p) {
             // whole 16-float B rows as four 16-byte loads
             for (int t = threadIdx.x; t < kn * 4; t += kThreads) {
                 const int r = t / 4, c4 = t % 4;
-                const float4 v = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(B) +
-                                                                       (kc + r) * p.ldb) + c4);
+                const float4 v = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(B) +
+                                                                       (kc + r) * p.ldb)[c4];
                 *reinterpret_cast<float4*>(&sb[r][4 * c4]) = v;
             }
         } else {
@@ -436,11 +436,11 @@ template <typename TIn>
 __device__ __forceinline__ float2 ld2_f(const TIn* p);
 template <>
 __device__ __forceinline__ float2 ld2_f<float>(const float* p) {
-    return __ldg(reinterpret_cast<const float2*>(p));
+    return *reinterpret_cast<const float2*>(p);
 }
 template <>
 __device__ __forceinline__ float2 ld2_f<__nv_bfloat16>(const __nv_bfloat16* p) {
-    const uint32_t u = __ldg(reinterpret_cast<const unsigned int*>(p));
+    const uint32_t u = *reinterpret_cast<const unsigned int*>(p);
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
 }
 

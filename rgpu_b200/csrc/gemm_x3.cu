@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_planes_kernel(Operand a, 
             const int64_t total = o.mn * q;
             for (int64_t i = (int64_t)blockIdx.x * kSplitThreads + tid; i < total; i += stride) {
                 const int64_t r = i / q, c = (i - r * q) * 4;
-                float4 x = __ldg(reinterpret_cast<const float4*>(o.src + r * o.ld_src + c));
+                float4 x = *reinterpret_cast<const float4*>(o.src + r * o.ld_src + c);
                 float4 h, l;
                 split_tf32(x.x, h.x, l.x);
                 split_tf32(x.y, h.y, l.y);
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_planes_kernel(Operand a, 
             for (int64_t i = (int64_t)blockIdx.x * kSplitThreads + tid; i < total; i += stride) {
                 const int64_t r = i / o.k, c = i - r * o.k;
                 float h, l;
-                split_tf32(__ldg(o.src + r * o.ld_src + c), h, l);
+                split_tf32(o.src[r * o.ld_src + c], h, l);
                 hi_plane[r * o.ldw + c] = h;
                 lo_plane[r * o.ldw + c] = l;
             }
@@ -150,11 +150,11 @@ __global__ void __launch_bounds__(kSplitThreads) split_planes_kernel(Operand a, 
             const int64_t kk = k0 + r, c = mn0 + 4 * quad;
             float v[4];
             if (kk < o.k && full_mn && src_vec) {
-                const float4 x = __ldg(reinterpret_cast<const float4*>(o.src + kk * o.ld_src + c));
+                const float4 x = *reinterpret_cast<const float4*>(o.src + kk * o.ld_src + c);
                 v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (kk < o.k && c + e < o.mn) ? __ldg(o.src + kk * o.ld_src + c + e) : 0.0f;
+                for (int e = 0; e < 4; ++e) v[e] = (kk < o.k && c + e < o.mn) ? o.src[kk * o.ld_src + c + e] : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) tile[r][4 * quad + e] = v[e];

@@ -278,7 +278,7 @@ __device__ __forceinline__ void epilogue_math(const TcParams& p, int64_t row, in
     const bool full = col0 + 32 <= n;
     if (p.epi == RT_EPI_BIAS || p.epi == RT_EPI_BIAS_RELU) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = v[j] + (col0 + j < n ? __ldg(p.bias + col0 + j) : 0.0f);
+        for (int j = 0; j < 32; ++j) v[j] = v[j] + (col0 + j < n ? p.bias[col0 + j] : 0.0f);
         if (p.epi == RT_EPI_BIAS_RELU) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = fmaxf(v[j], 0.0f);
