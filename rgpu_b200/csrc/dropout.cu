@@ -154,9 +154,8 @@ extern "C" int rt_dropout(rt_ctx* ctx, const rt_tensor* x, const rt_tensor* add,
     RT_CHECK(!add || (add->rows == x->rows && add->cols == x->cols), "rt_dropout: x is %lldx%lld, add %lldx%lld",
              (long long)x->rows, (long long)x->cols, (long long)(add ? add->rows : 0), (long long)(add ? add->cols : 0));
     RT_CHECK(mask->p >= 0.0 && mask->p <= 1.0, "rt_dropout: p must be in [0, 1] (got %g)", mask->p);
-    RT_CHECK(mask->first_row >= 0 && mask->first_row + x->rows <= (int64_t)1 << 32 && mask->first_row <= (int64_t)1 << 32,
-             "rt_dropout: rows %lld to %lld are not within 2^32", (long long)mask->first_row,
-             (long long)(mask->first_row + x->rows));
+    RT_CHECK(mask->first_row >= 0 && mask->first_row <= (int64_t)1 << 32 && x->rows <= ((int64_t)1 << 32) - mask->first_row,
+             "rt_dropout: %lld rows from row %lld on are not within 2^32", (long long)x->rows, (long long)mask->first_row);
     RT_CHECK(x->cols <= (int64_t)1 << 34, "rt_dropout: %lld columns are over 2^34", (long long)x->cols);
     const rt_tensor* s = mask->step_at;
     RT_CHECK(!s || (s->dtype == RT_U32 && s->rows * s->cols == 1), "rt_dropout: step_at must be one u32");
