@@ -298,7 +298,8 @@ int64_t rt_fp8_scale_bytes(int64_t rows, int64_t k);
  * elements are rounded to nearest, ties to even.  A block that holds a NaN or
  * an infinity gets the NaN scale. */
 int rt_fp8_quantize(rt_ctx* ctx, const rt_tensor* src, int axis, rt_fp8* dst);
-/* dst [rows, k] (f32 or bf16) = the values q stands for. */
+/* dst [rows, k] (f32 or bf16) = the values q stands for; bf16 rounds those
+ * below 2^-130, where it is subnormal. */
 int rt_fp8_dequantize(rt_ctx* ctx, const rt_fp8* q, rt_tensor* dst);
 /* C[m,n] = A[m,k] B[n,k]^T + 1 bias, ReLU if relu != 0, as rt_mx4_matmul: all
  * three products of a Dense layer take this form. */

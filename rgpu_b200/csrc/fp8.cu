@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(PAIR ? 256 : 512) quantize_columns_kernel(
 }
 
 // The rows of quantize_rows_kernel, the other way.  f32 holds every value exactly; bf16 all
-// but the smallest (below 2^-133), rounded.  8192 x 8192 bf16: 29 us, 6.9 TB/s.
+// from 2^-130 on, those below it are rounded to multiples of 2^-133.  8192 x 8192 bf16: 29 us, 6.9 TB/s.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* codes,
                                                          const uint8_t* scales, int64_t rows, int64_t k,
