@@ -1064,7 +1064,7 @@ int launch_sort(rt_ctx* ctx, const uint32_t* t, Sort s, Sums* m, const rt_tensor
         const int64_t row = m->n * 4;
         if (!m->accumulate && s.vocabulary * row >= 16 << 20)
             s.filled = std::min(s.vocabulary, std::max(s.vocabulary / 2, ((32 << 20) + s.count * 1536) / row));
-        const int64_t fills = std::min<int64_t>(ctx->sort_clusters[ranks == 16] - 1, s.filled / (16 * ranks));
+        const int64_t fills = std::max<int64_t>(0, std::min<int64_t>(ctx->sort_clusters[ranks == 16] - 1, s.filled / (16 * ranks)));
         m->filled = s.filled = fills ? s.filled : 0;
         RT_CUDA(launch_cluster(ranks, pdl, kernel, (unsigned)((1 + fills) * ranks), 1024, sizeof(ClusterSmem), ctx->stream, s, t, m->out,
                                m->ldo, m->n));

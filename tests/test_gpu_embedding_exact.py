@@ -80,3 +80,28 @@ def test_rounding(gpu, kind, count, n, vocabulary):
                            gpu.zeros((gpu.embedding_backward_workspace(count, vocabulary, n),)), scale=1.5)
     bound = 1.01 * U * _depth(count, times, n)[:, None] * 1.5 * size
     assert np.all(np.abs(gpu.download(d) - 1.5 * want) <= bound)
+
+
+@pytest.mark.parametrize("pad,offset", [(0, 0), (4, 4), (3, 1)])
+@pytest.mark.parametrize("count,n,vocabulary", [(4200, 16500, 255), (9000, 16500, 255), (9000, 1024, 20000), (5000, 1021, 9000), (40000, 48, 90000),
+                                                (4500, 8, 600000), (70000, 256, 20000)])
+def test_large_tables(gpu, count, n, vocabulary, pad, offset):
+    # absent rows get their zeros beside the sort or beside the pieces, by the table's size: every row is written, once
+    rng = np.random.default_rng(count + n)
+    tokens = torch.from_numpy(_tokens("zipf", rng, count, vocabulary).astype(np.int64)).cuda()
+    dy = torch.full((offset + count * (n + pad),), float("nan"), device="cuda")
+    rows = dy[offset:].view(count, n + pad)[:, :n]
+    rows.copy_(torch.from_numpy(_whole(count, n)))
+    want = torch.zeros(vocabulary, n, dtype=torch.float64, device="cuda")
+    real = tokens < vocabulary
+    want.index_add_(0, tokens[real], rows[real].double())
+    out = torch.full((offset + vocabulary * (n + pad),), float("nan"), device="cuda")
+    work = torch.full((gpu.embedding_backward_workspace(count, vocabulary, n),), float("nan"), device="cuda")
+    ids = tokens.int()
+    torch.cuda.synchronize()
+    gpu.embedding_backward(gpu.wrap(ids.data_ptr(), (count,), "u32"), gpu.wrap(dy.data_ptr() + offset * 4, (count, n), ld=n + pad),
+                           gpu.wrap(out.data_ptr() + offset * 4, (vocabulary, n), ld=n + pad), gpu.wrap(work.data_ptr(), (work.numel(),)))
+    gpu.sync()
+    got = out[offset:].view(vocabulary, n + pad)
+    assert torch.equal(got[:, :n].double(), want)
+    assert got[:, n:].isnan().all() and out[:offset].isnan().all(), "elements beside dtable were written"
