@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const TE* table, int64_t ld
 // The sort's arrays in the workspace, in 32-bit words.  A key is a token, or V for padding.
 struct Sort {
     int64_t count, vocabulary;
-    int64_t filled;      // rows of dE that the cluster's sort looks after: zeros to the absent ones
+    int beside;          // eighths of the rows of dE that get their zeros beside the cluster's sort
     int passes;          // by 8 bits of a key
     int ctas;            // of a pass over launches,
     int64_t span;        // and positions of a CTA
@@ -380,15 +380,20 @@ __device__ __forceinline__ void sync_cluster() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The first `all` rows of dE, where their tokens do not occur: zeros.  CTA `part` of `parts` marks the tokens of its
-// share of the rows by going over all positions itself, so it needs no sort.
+// Rows whose tokens do not occur get zeros, by groups of kZeros of them: of eight groups the first `beside` beside
+// the sort, the others beside the pieces.  Neighbouring tokens are about as frequent in many vocabularies, so
+// neither has one end of the table.
+constexpr int kZeros = 32;
+
+// Those beside the sort.  CTA `part` of `parts` marks the tokens of its share of the rows by going over all positions
+// itself, so it needs no sort.
 constexpr int kMarks = 8192;  // rows at a time
 
 template <int ACCESS>
-__device__ __forceinline__ void fill(uint8_t* marks, const uint32_t* tokens, int64_t count, int64_t all, float* out,
-                                     int64_t ldo, int64_t n, uint32_t part, uint32_t parts) {
+__device__ __forceinline__ void fill(uint8_t* marks, const uint32_t* tokens, const Sort& s, float* out, int64_t ldo, int64_t n,
+                                     uint32_t part, uint32_t parts) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t begin = all * part / parts, end = all * (part + 1) / parts;
+    const int64_t begin = s.vocabulary * part / parts, end = s.vocabulary * (part + 1) / parts;
     for (int64_t b = begin; b < end; b += kMarks) {
         const uint32_t rows = (uint32_t)min(end - b, (int64_t)kMarks);
         __syncthreads();
@@ -397,8 +402,8 @@ __device__ __forceinline__ void fill(uint8_t* marks, const uint32_t* tokens, int
         auto mark = [&](uint32_t token) {
             if (token - (uint32_t)b < rows) marks[token - (uint32_t)b] = 1;
         };
-        const int64_t lead = min(count, (int64_t)((16 - (reinterpret_cast<uintptr_t>(tokens) & 15)) & 15) / 4);
-        const int64_t quads = (count - lead) / 4;
+        const int64_t lead = min(s.count, (int64_t)((16 - (reinterpret_cast<uintptr_t>(tokens) & 15)) & 15) / 4);
+        const int64_t quads = (s.count - lead) / 4;
         const uint4* four = reinterpret_cast<const uint4*>(tokens + lead);
 #pragma unroll 8
         for (int64_t i = threadIdx.x; i < quads; i += 1024) {
@@ -406,18 +411,18 @@ __device__ __forceinline__ void fill(uint8_t* marks, const uint32_t* tokens, int
             mark(t.x), mark(t.y), mark(t.z), mark(t.w);
         }
         if (threadIdx.x < lead) mark(tokens[threadIdx.x]);
-        if (threadIdx.x < count - lead - quads * 4) mark(tokens[lead + quads * 4 + threadIdx.x]);
+        if (threadIdx.x < s.count - lead - quads * 4) mark(tokens[lead + quads * 4 + threadIdx.x]);
         __syncthreads();
         const float zero[8] = {};
         for (uint32_t r = warp; r < rows; r += 32) {
-            if (marks[r]) continue;
+            if (marks[r] || (int)((b + r) / kZeros % 8) >= s.beside) continue;
             float* row = out + (b + r) * ldo;
             for (int64_t j = 0; j * 256 < n; ++j) Lane<float, ACCESS, 8>::store(row, Columns<ACCESS, 8>(j, n, lane), zero);
         }
     }
 }
 
-// The grid's first cluster sorts; the others, on SMs that it leaves idle, write the absent ones of the first s.filled rows.
+// The grid's first cluster sorts; the others write zeros on SMs that it leaves idle.
 template <int ACCESS>
 __global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32_t* tokens, float* out, int64_t ldo, int64_t n) {
     extern __shared__ __align__(16) uint8_t raw[];
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(1024) cluster_sort_kernel(Sort s, const uint32
     pdl_wait();
     pdl_launch_dependents();
     if (blockIdx.x >= cluster_size()) {
-        fill<ACCESS>(raw, tokens, s.count, s.filled, out, ldo, n, blockIdx.x - cluster_size(), gridDim.x - cluster_size());
+        fill<ACCESS>(raw, tokens, s, out, ldo, n, blockIdx.x - cluster_size(), gridDim.x - cluster_size());
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -554,7 +559,7 @@ constexpr int kColumns = 16 / (int)sizeof(T);
 struct Sums {
     int64_t count, vocabulary, n, spans, width;
     int64_t pieces;
-    int64_t filled;  // rows that have their zeros, where they are absent; piece_kernel writes the others'
+    int beside;  // eighths of the rows that have their zeros, where they are absent; piece_kernel writes the others'
     int cut;  // positions of a piece: kCut, a half or a quarter
     const uint32_t* token;
     const uint32_t* position;
@@ -582,14 +587,17 @@ __device__ __forceinline__ void emit(const Sums& s, uint32_t token, const Column
     L::store(row, c, v);
 }
 
-// Zeros to the rows of tokens that do not occur, a warp kZeros rows and a span.
-constexpr int kZeros = 16;
+// The zeros beside the pieces, a warp a part of a group's rows and a span.
+constexpr int kZerosWarp = 8;
 
 template <int ACCESS, int N>
-__device__ __forceinline__ void zeros(const Sums& s, int64_t t0, int64_t span) {
+__device__ __forceinline__ void zeros(const Sums& s, int64_t group, int64_t span) {
     const int lane = threadIdx.x & 31;
+    constexpr int PARTS = kZeros / kZerosWarp;
+    const uint32_t of = 8 - s.beside, at = (uint32_t)(group / PARTS);
+    const int64_t t0 = ((int64_t)(at / of) * 8 + s.beside + at % of) * kZeros + group % PARTS * kZerosWarp;
     const Columns<ACCESS, N> c(span, s.n, lane);
-    const bool there = lane < kZeros && t0 + lane < s.vocabulary;
+    const bool there = lane < kZerosWarp && t0 + lane < s.vocabulary;
     const float zero[N] = {};
     for (uint32_t empty = __ballot_sync(0xffffffffu, there && s.start[t0 + lane] == s.start[t0 + lane + 1]); empty; empty &= empty - 1)
         Lane<float, ACCESS, N>::store(s.out + (t0 + __ffs(empty) - 1) * s.ldo, c, zero);
@@ -602,7 +610,7 @@ __global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* dy, int64_t
     pdl_wait();
     pdl_launch_dependents();
     if ((int)blockIdx.x >= piece_blocks) {
-        zeros<ACCESS, kColumns<T>>(s, s.filled + lay_group(along, blockIdx.x - piece_blocks) * kZeros, lay_span(along));
+        zeros<ACCESS, kColumns<T>>(s, lay_group(along, blockIdx.x - piece_blocks), lay_span(along));
         return;
     }
     constexpr int N = kColumns<T>, U = 8;  // U: rows of dy under way
@@ -1004,7 +1012,7 @@ int launch_sums(rt_ctx* ctx, const rt_tensor* dy, Sums m) {
     const Lay pieces(m.pieces, m.spans), rows((m.vocabulary + tokens - 1) / tokens, m.spans);
     const T* p = static_cast<const T*>(dy->ptr);
     dim3 grid = pieces.grid;
-    if (!m.accumulate) grid.x += Lay((m.vocabulary - m.filled + kZeros - 1) / kZeros, m.spans).grid.x;
+    if (!m.accumulate && m.beside < 8) grid.x += Lay((m.vocabulary + 8 * kZeros - 1) / (8 * kZeros) * (8 - m.beside) * (kZeros / kZerosWarp), m.spans).grid.x;
     RT_CUDA(launch_k(ctx->pdl, piece_kernel<T, ACCESS>, grid, 256, 0, ctx->stream, m, p, dy->ld, pieces.along, (int)pieces.grid.x));
     grid = rows.grid;
     grid.x += (unsigned)((m.pieces + kJoin - 1) / kJoin) << rows.along;
@@ -1058,14 +1066,15 @@ int launch_sort(rt_ctx* ctx, const uint32_t* t, Sort s, Sums* m, const rt_tensor
         // Beside the sort as many clusters as the device holds, a CTA with 16 rows or more: it goes over all tokens.
         // Both wait for the memory, so beside the sort lie as many rows as it has time for, the others beside the pieces:
         // half of them or more (8192 x 1024 of 50257: 49 us, all 52, none 59), and 32 MB with 1.5 KB a position (65536 x 1024
-        // of 50257: 81 us, all 83, none 90; 65536 x 256 of 128256: 61, half 66, none 74).  Tables below 16 MB
+        // of 50257: 80 us, all 83, none 90; 65536 x 256 of 128256: 61, half 66, none 74).  Tables below 16 MB
         // have them all beside the pieces (17314 x 33 of 593: 23.4, beside the sort 24.2; 10000 x 100 of 75000,
         // 30 MB: 37.5 / 34.3).
-        const int64_t row = m->n * 4;
-        if (!m->accumulate && s.vocabulary * row >= 16 << 20)
-            s.filled = std::min(s.vocabulary, std::max(s.vocabulary / 2, ((32 << 20) + s.count * 1536) / row));
-        const int64_t fills = std::max<int64_t>(0, std::min<int64_t>(ctx->sort_clusters[ranks == 16] - 1, s.filled / (16 * ranks)));
-        m->filled = s.filled = fills ? s.filled : 0;
+        const int64_t bytes = s.vocabulary * m->n * 4;
+        if (!m->accumulate && bytes >= 16 << 20)
+            s.beside = (int)std::min<int64_t>(8, std::max<int64_t>(4, ((32 << 20) + s.count * 1536) * 8 / bytes));
+        int64_t fills = s.beside ? std::min<int64_t>(ctx->sort_clusters[ranks == 16] - 1, s.vocabulary / (16 * ranks)) : 0;
+        if (fills <= 0) fills = s.beside = 0;
+        m->beside = s.beside;
         RT_CUDA(launch_cluster(ranks, pdl, kernel, (unsigned)((1 + fills) * ranks), 1024, sizeof(ClusterSmem), ctx->stream, s, t, m->out,
                                m->ldo, m->n));
         count_launch(ctx);
