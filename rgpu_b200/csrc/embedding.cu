@@ -904,7 +904,10 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) few_kernel(Sums s, con
             for (int i = 0; i < N; ++i) sum[i] += v[x].value(i);
         }
     };
-    constexpr int MANY = ACCESS ? 8 : 4;  // with a register an element eight rows would spill
+    // Rows of dy under way: eight of aligned f32 (20 bytes spilled at the 64 registers that the SM's 32 warps have each),
+    // else four.  Eight aligned bf16 rows spill 84 bytes (4096 x 1024 of 1000, as frequent as words: 15.9 us, four
+    // 13.6), eight unaligned ones, a register an element, 328 (4096 x 1001: 38, four, which spill 64, 21.4).
+    constexpr int MANY = ACCESS && sizeof(T) == 4 ? 8 : 4;
     int e = begin;
     for (; end - e >= MANY; e += MANY) add(e, std::integral_constant<int, MANY>());
     for (; e < end; e += 3) add(e, std::integral_constant<int, 3>());
