@@ -14,7 +14,7 @@
 //    the most frequent token occurs does not decide how evenly a pass is spread
 // In the last two piece_kernel and row_kernel sum; the rows of tokens that do not occur are
 // written beside the cluster's sort and beside the pieces.  65536 x 1024 bf16 rows of 50257
-// tokens as frequent as words: 81 us, 52 of bytes; 2047 x 1000 f32 of 1000: 6.5 us.
+// tokens as frequent as words: 80 us, 52 of bytes; 2047 x 1000 f32 of 1000: 6.5 us.
 //
 // Each kernel waits (pdl_wait) for the one before it on the stream before it reads or writes
 // anything: only that wait makes what earlier kernels wrote visible, those before the last one too.  Rows that did not
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(256) piece_kernel(Sums s, const T* dy, int64_t
 
 // Adds the partial sums of the heavy runs that begin in kJoin pieces: a run's second row
 // there and the first rows of the pieces that follow. A warp takes a run that lies in
-// kAlone pieces at most (17314 x 33 of 593, pieces of 64: 34 us; by the whole CTA, one after another, 40); longer
+// kAlone pieces at most (17314 x 33 of 593, pieces of 64: 33 us; by the whole CTA, one after another, 38); longer
 // ones are dealt out over the CTA's warps in order.
 constexpr int kJoin = 8, kAlone = 16;
 static_assert(kJoin == 8, "a warp each");
@@ -929,8 +929,9 @@ int bits_of(int64_t v) {
 
 // Whether few_kernel takes them all: up to kFew / 2 positions always, up to kFew if the table is narrow and so
 // short that the CTAs, of which each goes over all positions, fit the device at once, but not so short that a few
-// of them have most of the positions (7424 x 128 of 1792: 8.7 us, with the cluster's sort 14.0; 8192 x 100 of 75000: 18 / 32;
-// but as frequent as words 8192 x 64 of 256: 18.6 / 17.3; 8192 x 512 of 5000: 24 / 19; 8192 x 1024 of 1000: 26.6 / 20.4).
+// of them have most of the positions (7424 x 128 of 1792: 8.9 us, with the cluster's sort 14.6; 8192 x 100 of 75000: 19 / 32;
+// but as frequent as words 8192 x 64 of 1000: 18.2 / 16.5; of 256: 19.1 / 16.4; 8192 x 512 of 5000: 20.8 / 20.1; 8192 x 1024
+// of 1000: 23.2 / 20.0).
 bool is_few(int64_t count, int64_t vocabulary, int64_t n) {
     return count <= kFew / 2 ||
            (count <= kFew && n <= 256 && vocabulary >= 1000 && (vocabulary + kGroup - 1) / kGroup <= 4 * 148);
@@ -945,13 +946,13 @@ int64_t lay_out(int64_t count, int64_t vocabulary, int64_t n, Sort* s, Sums* m) 
     s->ctas = (int)std::min<int64_t>(256, std::max<int64_t>(1, (count + 1023) / 1024));
     s->span = (count + s->ctas - 1) / s->ctas;
     // Shorter pieces while there are fewer than eight warps for each of the 148 SMs: a warp's reads of a piece wait for one another,
-    // but a long run leaves more partial sums.  17314 x 33 of 593: 25.5 us with 16, 28 with 32, 34 with 64;
-    // 65536 x 1024 of 50257: 85, 78 and 75.
+    // but a long run leaves more partial sums.  17314 x 33 of 593: 24 us with 16, 27 with 32, 33 with 64;
+    // 65536 x 1024 of 50257: 88, 81 and 80.
     m->cut = kCut;
     while (m->cut > kCut / 4 && (count / m->cut) * ((n + 255) / 256) < 8 * 148) m->cut /= 2;
     m->pieces = (count + m->cut - 1) / m->cut;
-    // all 16 CTAs before a CTA takes more than 1024: 16384 x 256 of 4000: 21 us, 4096 each 26.5; 10000 x 100
-    // of 75000: 34.5 / 56; beside zeros that take as long 32768 x 1024 of 50257: 62.4 / 61.6
+    // all 16 CTAs before a CTA takes more than 1024: 16384 x 256 of 4000: 20 us, 4096 each 26; 10000 x 100
+    // of 75000: 34 / 55; 32768 x 1024 of 50257: 66 / 69
     s->log_chunk = 10;
     while (s->log_chunk < 12 && count > kMaxCluster << s->log_chunk) ++s->log_chunk;
     m->width = (n + 7) / 8 * 8;
@@ -1008,8 +1009,8 @@ int launch_sums(rt_ctx* ctx, const rt_tensor* dy, Sums m) {
     constexpr int SPAN = 32 * kColumns<T>;
     m.spans = (m.n + SPAN - 1) / SPAN;
     // 16 rows a warp where that makes warps enough for every place on the device (65536 x 1024 of 50257:
-    // 75 us, with 4 rows 87, with one 117); one, whose chain of reads is the shortest, where the device
-    // holds most of the warps at once (7813 x 3979 of 430 bf16: 48 us, with 4 rows 57); else 4
+    // 80 us, with 4 rows 88, with one 121); one, whose chain of reads is the shortest, where the device
+    // holds most of the warps at once (7813 x 3979 of 430 bf16: 48 us, with 4 rows 56); else 4
     const int64_t sms = ctx->sm_count;
     const int tokens = m.vocabulary / 16 * m.spans >= sms * 32 ? 16 : m.vocabulary * m.spans < sms * 48 ? 1 : 4;
     const Lay pieces(m.pieces, m.spans), rows((m.vocabulary + tokens - 1) / tokens, m.spans);
@@ -1031,8 +1032,8 @@ int launch_few(rt_ctx* ctx, const rt_tensor* tokens, const rt_tensor* dy, const 
     const int64_t spans = (m.n + SPAN - 1) / SPAN;
     // So many rows a CTA that the CTAs fit the device at once, 32 warps to an SM: each goes over all positions.
     // 16 warps a CTA if such a number (at most kGroup) exists: they share a frequent token's positions
-    // (2047 x 1000 of 1000: 6.6 us, with 8 warps 7.9; 4096 x 1024 of 1000, as frequent as words, bf16: 15.9 / 20.4);
-    // else 8, which keep waiting less for one another (4096 x 1024 of 50257: 53 us, with 16 56; 1024 x 1024 f32: 40 / 57)
+    // (2047 x 1000 of 1000: 6.7 us, with 8 warps 8.1; 4096 x 1024 of 1000, as frequent as words, bf16: 13.6 / 18.6);
+    // else 8, which keep waiting less for one another (1024 x 1024 f32 of 50257: 41 us, with 16 57; 4096 x 1024 bf16: 52 / 53)
     auto ctas = [&](int group) { return (m.vocabulary + group - 1) / group * spans; };
     const bool wide = ctas(kGroup) <= 2 * (int64_t)ctx->sm_count;
     int group = 1;

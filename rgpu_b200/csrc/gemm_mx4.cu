@@ -1200,7 +1200,9 @@ int launch_product(rt_ctx* ctx, const typename F::Matrix& a, const typename F::M
     // tiles: 5.9 us in four, 8.4 in one; 64 x 1000 x 8192: 7.3 / 9.7; 1024^3, 4 stages: 6.6 in
     // two, 4.9 in one).  With 64 tiles and more fewer splits would do (1 x 8192 x 8192: 8.2 in
     // four, 7.3 in two; 1024 x 1024 x 8192: 11.1 in two, 10.3 in one; both with the operands in
-    // L2).
+    // L2).  Products of up to 32 tokens in 8 bits, of twice as many stages, take the same rule; weights from HBM:
+    // 1 x 8192 x 8192 14.9 in four, 16.7 in two, 20.5 in eight; 1 x 1000 x 8192 7.7 in eight, 9.0 in four; 8 x 16384 x 2048
+    // 9.5 in two, 14.5 in four (4 bits: 10.1, 11.0, 16.4; 6.4, 6.6; 7.3, 12.4 and 6.5 in one).
     int splits = 1;
     while (splits < 8 && p.stages > 8 * splits && tiles * splits * 2 <= slots) splits *= 2;
     if (tn == 32) return launch_one<F, 32>(ctx, a, b, p, splits, stream);

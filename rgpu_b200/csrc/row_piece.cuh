@@ -21,7 +21,7 @@ struct Piece {
     uint32_t w[8];
 
     // All of the piece.  Without a branch, so that one load is not waited for before the next
-    // is issued (dropout of 8192 x 8192 bf16 78 us, with load below 92).
+    // is issued (dropout of 8192 x 8192 bf16 with a sum 59.9 us, with load below 60.9; without one 46.1 and 47.8).
     template <int V>
     __device__ __forceinline__ void load_whole(const T* p) {
         if constexpr (V == 32) {
